@@ -437,6 +437,39 @@ int mrl_ppo_update_epoch_ahead(mrl_ctx *ctx, const mrl_update *u, const int32_t 
 int mrl_minibatch_adv_stats(mrl_ctx *ctx, const int32_t *indices, const float *advantages, int minibatch,
                             int n_minibatches, float *stats);
 
+/* ------------------------------------------------------------------ recurrent layer
+ * A gated linear recurrence over the rollout's time-major rows, for policies and values with a memory (no counterpart in the
+ * reference, whose models are stateless):
+ *     a = sigmoid(gate),   h[t] = a[t] * h[t-1] + (1 - a[t]) * value[t],
+ * element by element in D channels of each of N environments, h[-1] = state_in.  Where dones[t-1] (for the first step
+ * prev_dones) is above 0.5, h[t-1] counts as 0: dones [T, N] are the rollout's flags (r_dones) as they are, prev_dones [N] those
+ * of the step ahead of the first one, and the last row of dones is not read -- a rollout cut into pieces gives the states of the
+ * whole where every piece gets the state_out and the last flags of the one before.  Either may be NULL (no flag is set).  What a
+ * cut hides, infinities and NaN included, reaches nothing behind it.
+ *
+ * gate, value, out and their gradients have rows t * N + n of D elements of `dtype`, `ld` elements apart (ld >= D; gate and value
+ * can be halves of one buffer's rows); states are fp32 [N, D].  state_in NULL is zeros; state_out = h[T-1], may be NULL, and
+ * may be state_in.  T = 1 is a step of a collection loop.  No element of another output may be one of an input's or of another
+ * output's.  A row's elements need no alignment beyond their type's.
+ *
+ * Backward: out as forward left it, grad_out and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out;
+ * overwrites grad_gate, grad_value and grad_state_in (may be NULL, may be grad_state_out).  All sums are in a fixed order.
+ *
+ * The workspace (device, 16-byte aligned, need not be kept between calls; NULL where the size is 0) holds at least
+ * mrl_recurrence_workspace's bytes, the same for both directions and types: 0 unless few channels and many steps have the time
+ * axis split over workgroups. */
+enum mrl_dtype { MRL_F32 = 0, MRL_BF16 = 1 };
+int mrl_recurrence_workspace(mrl_ctx *ctx, int T, int N, int D, uint64_t *bytes);
+int mrl_recurrence_forward(mrl_ctx *ctx, int dtype, int T, int N, int D, const void *gate, int64_t gate_ld,
+                           const void *value, int64_t value_ld, const float *dones, const float *prev_dones,
+                           const float *state_in, void *out, int64_t out_ld, float *state_out, void *workspace,
+                           uint64_t workspace_bytes);
+int mrl_recurrence_backward(mrl_ctx *ctx, int dtype, int T, int N, int D, const void *gate, int64_t gate_ld,
+                            const void *value, int64_t value_ld, const void *out, int64_t out_ld, const float *dones,
+                            const float *prev_dones, const float *state_in, const void *grad_out, int64_t grad_out_ld,
+                            const float *grad_state_out, void *grad_gate, int64_t grad_gate_ld, void *grad_value,
+                            int64_t grad_value_ld, float *grad_state_in, void *workspace, uint64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

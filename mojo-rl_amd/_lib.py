@@ -20,6 +20,7 @@ ENV_CARTPOLE, ENV_PENDULUM, ENV_LUNARLANDER, ENV_BIPEDAL, ENV_HALFCHEETAH = 0, 1
 ENV_LUNARLANDER_CONTINUOUS = 5
 ENV_CARRACING = 6
 ENV_HOPPER_PLANAR, ENV_WALKER2D_PLANAR = 7, 8
+F32, BF16 = 0, 1   # element types
 
 
 class Layer(C.Structure):
@@ -63,7 +64,7 @@ class MrlError(RuntimeError):
     pass
 
 
-P, I, U32, U64, F, D = C.c_void_p, C.c_int, C.c_uint32, C.c_uint64, C.c_float, C.c_double
+P, I, I64, U32, U64, F, D = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_uint64, C.c_float, C.c_double
 DP, RP, UP = C.POINTER(MlpDesc), C.POINTER(Rollout), C.POINTER(Update)
 
 # name -> argtypes; every function returns int (0 = ok) unless listed in _SPECIAL
@@ -124,6 +125,9 @@ SIGNATURES = {
     "mrl_ppo_update_epoch": [P, UP, P, I, I, I],
     "mrl_ppo_update_epoch_ahead": [P, UP, P, I, I, I, I],
     "mrl_minibatch_adv_stats": [P, P, P, I, I, P],
+    "mrl_recurrence_workspace": [P, I, I, I, C.POINTER(U64)],
+    "mrl_recurrence_forward": [P, I, I, I, I, P, I64, P, I64, P, P, P, P, I64, P, P, U64],
+    "mrl_recurrence_backward": [P, I, I, I, I, P, I64, P, I64, P, I64, P, P, P, P, I64, P, P, I64, P, I64, P, P, U64],
 }
 _SPECIAL = {"mrl_version": (C.c_int, []), "mrl_last_error": (C.c_char_p, [])}
 # size queries return a count, not a status

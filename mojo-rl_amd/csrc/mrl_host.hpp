@@ -115,6 +115,20 @@ int cartpole_side(mrl_ctx *ctx, const float *states, int batch, int32_t **out);
 // (the current device); idempotent
 int clip_static_setup(int device);
 
+// Makes the context's device the current one for as long as it lives, for a caller whose current device is another.
+struct OnDevice {
+    int before;
+    bool moved;
+    explicit OnDevice(const mrl_ctx *ctx) : before(0), moved(false) {
+        if (hipGetDevice(&before) == hipSuccess && before != ctx->device) moved = hipSetDevice(ctx->device) == hipSuccess;
+    }
+    ~OnDevice() {
+        if (moved) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
 inline int grid_for(long n, int block) { return (int)((n + block - 1) / block); }
 
 // Records a phase boundary: the time since the previous mark is charged to `tag`; tag < 0 opens
