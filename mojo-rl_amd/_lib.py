@@ -31,6 +31,10 @@ class MlpDesc(C.Structure):
     _fields_ = [("n_layers", C.c_int32), ("layers", Layer * MAX_LAYERS)]
 
 
+class Matrix(C.Structure):
+    _fields_ = [("offset", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
 class Rollout(C.Structure):
     _fields_ = [
         ("env_id", C.c_int32), ("n_envs", C.c_int32), ("obs_dim", C.c_int32), ("num_actions", C.c_int32),
@@ -65,7 +69,7 @@ class MrlError(RuntimeError):
 
 
 P, I, I64, U32, U64, F, D = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_uint64, C.c_float, C.c_double
-DP, RP, UP = C.POINTER(MlpDesc), C.POINTER(Rollout), C.POINTER(Update)
+DP, RP, UP, MP = C.POINTER(MlpDesc), C.POINTER(Rollout), C.POINTER(Update), C.POINTER(Matrix)
 
 # name -> argtypes; every function returns int (0 = ok) unless listed in _SPECIAL
 SIGNATURES = {
@@ -128,6 +132,10 @@ SIGNATURES = {
     "mrl_recurrence_workspace": [P, I, I, I, C.POINTER(U64)],
     "mrl_recurrence_forward": [P, I, I, I, I, P, I64, P, I64, P, P, P, P, I64, P, P, U64],
     "mrl_recurrence_backward": [P, I, I, I, I, P, I64, P, I64, P, I64, P, P, P, P, I64, P, P, I64, P, I64, P, P, U64],
+    "mrl_orthogonalize_workspace": [I, I, I, C.POINTER(U64)],
+    "mrl_orthogonalize": [P, I, I, I, I, P, P, I, D, P, U64],
+    "mrl_muon_workspace": [I, MP, C.POINTER(U64)],
+    "mrl_muon_step": [P, P, P, P, I64, I, MP, I, D, D, I, D, I, D, D, D, D, D, P, U64],
 }
 _SPECIAL = {"mrl_version": (C.c_int, []), "mrl_last_error": (C.c_char_p, [])}
 # size queries return a count, not a status

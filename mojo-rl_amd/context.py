@@ -20,6 +20,11 @@ def _ptr(t):
     return t.data_ptr()
 
 
+def _on_device(ctx, name, t):
+    if t.device.type != ctx.device.type or t.device.index != ctx.device.index and ctx.device.index is not None:
+        raise _lib.MrlError("%s: a tensor on %s expected, got one on %s" % (name, ctx.device, t.device))
+
+
 class DeviceContext:
     def __init__(self, device="cuda:0", stream=None):
         if not torch.cuda.is_available():

@@ -245,4 +245,13 @@ MRL_DEV Uniform4 philox_uniform4(uint64_t seed, uint64_t offset, uint64_t call_i
     return u;
 }
 
+// One parameter's Adam step, deep_rl/optimizer/adam.mojo:52-105.
+MRL_DEV void adam_one(float &p, float g, float2 &state, float lr, float beta1, float beta2, float omb1, float omb2, float eps, float bc1, float bc2) {
+    const float m = beta1 * state.x + omb1 * g;
+    const float v = beta2 * state.y + omb2 * g * g;
+    state = make_float2(m, v);
+    const float m_hat = m / bc1, v_hat = v / bc2;
+    p = p - lr * m_hat / (sqrtf(v_hat) + eps);
+}
+
 }  // namespace mrl

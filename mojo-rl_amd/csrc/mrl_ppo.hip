@@ -610,13 +610,7 @@ __global__ __launch_bounds__(TPB) void adam_kernel(float *__restrict__ p, const 
                                                    float eps, float bc1, float bc2) {
     int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    float gi = g[i];
-    float2 mv = state[i];
-    float m_new = beta1 * mv.x + omb1 * gi;
-    float v_new = beta2 * mv.y + omb2 * gi * gi;
-    state[i] = make_float2(m_new, v_new);
-    float m_hat = m_new / bc1, v_hat = v_new / bc2;
-    p[i] = p[i] - lr * m_hat / (sqrtf(v_hat) + eps);
+    adam_one(p[i], g[i], state[i], lr, beta1, beta2, omb1, omb2, eps, bc1, bc2);
 }
 
 __global__ void clamp_log_std_kernel(float *params, int offset, int A) {

@@ -16,13 +16,9 @@ import ctypes as C
 import torch
 
 from . import _lib
+from .context import _on_device
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-
-
-def _on_device(ctx, name, t):
-    if t.device.type != ctx.device.type or t.device.index != ctx.device.index and ctx.device.index is not None:
-        raise _lib.MrlError("%s: a tensor on %s expected, got one on %s" % (name, ctx.device, t.device))
 
 
 class GatedRecurrence:

@@ -1,0 +1,260 @@
+"""orthogonalize and Muon against the formulas in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+NS = (3.4445, -4.7750, 2.0315)
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def ctx(mrl):
+    return mrl.DeviceContext("cuda:0")
+
+
+def polynomial(x, steps=5, eps=1e-7, gen=None):
+    """In 64 bits; with `gen` every stored value off by what the kernels' arithmetic may cost it, at random: operands keep 22 bits (and
+    2^-25 of a typical entry), a product's sum loses 2^-21 of the root of its terms' squares."""
+    x = x.double()
+    if x.shape[0] > x.shape[1]:
+        return polynomial(x.T, steps, eps, gen).T
+
+    def off(y, terms):
+        typical = y.square().mean().sqrt()
+        return y if gen is None else y + (2.0 ** -21 * terms + 2.0 ** -22 * y.abs() + 2.0 ** -25 * typical) * torch.randn(y.shape, generator=gen, dtype=torch.float64)
+
+    def root(p, q):
+        return ((p * p) @ (q * q)).sqrt() if gen is not None else None
+    x = x / (x.norm() + eps)
+    x = off(x, x.abs())
+    for _ in range(steps):
+        gram = off(x @ x.T, root(x, x.T))
+        b = off(NS[1] * gram + NS[2] * (gram @ gram), 5 * gram.abs() + (2 * root(gram, gram) if gen is not None else 0))
+        x = off(NS[0] * x + b @ x, 3.5 * x.abs() + (root(b, x) if gen is not None else 0))
+    return x
+
+
+def matrix(gen, rows, cols, rank=None):
+    rank = rank or max(1, min(rows, cols) // 8)
+    return torch.randn(rows, rank, generator=gen) @ torch.randn(rank, cols, generator=gen) / math.sqrt(rank) + 0.3 * torch.randn(rows, cols, generator=gen)
+
+
+def near(got, x, half, what, steps=5, eps=1e-7):
+    """Within eight times what the formula itself moves by when its intermediates are off as in polynomial(gen)."""
+    want = polynomial(x, steps, eps)
+    moved = (polynomial(x, steps, eps, torch.Generator().manual_seed(1)) - want).norm().item()
+    off = (got.double().cpu() - want).norm().item()
+    assert off <= 8 * moved + half * want.norm().item(), "%s: off by %g of %g, bound %g" % (what, off, want.norm(), 8 * moved + half * want.norm())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 50), (70, 1), (2, 2), (3, 4), (8, 256), (256, 4), (64, 64), (63, 65), (65, 63), (128, 128), (129, 127),
+                                       (40, 600), (600, 40), (256, 256), (300, 777), (777, 333), (130, 1030), (513, 512)])
+def test_orthogonalize(mrl, ctx, rows, cols, dtype):
+    print("orthogonalize", rows, cols, dtype, flush=True)
+    x = matrix(torch.Generator().manual_seed(rows * 1000 + cols), rows, cols).to(TYPES[dtype])
+    out = torch.full((rows, cols), 9.0, dtype=TYPES[dtype], device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda())
+    ctx.synchronize()
+    near(out, x, HALF[dtype], "out")
+
+
+@pytest.mark.parametrize("count,rows,cols,dtype", [(3, 30, 20, "f32"), (17, 9, 12, "bf16"), (40, 66, 70, "f32"), (2, 260, 100, "bf16"), (1, 5, 5, "f32")])
+def test_many_matrices_in_place_at_odd_addresses(mrl, ctx, count, rows, cols, dtype):
+    gen = torch.Generator().manual_seed(count)
+    x = torch.stack([matrix(gen, rows, cols) * 10.0 ** (k % 5 - 2) for k in range(count)]).to(TYPES[dtype])
+    flat = torch.full((x.numel() + 2,), -5.0, dtype=TYPES[dtype], device="cuda")
+    inside = flat[1:-1].view(count, rows, cols)
+    inside.copy_(x)
+    mrl.orthogonalize(ctx, inside, inside)
+    ctx.synchronize()
+    assert flat[0] == -5 and flat[-1] == -5
+    for k in range(count):
+        near(inside[k], x[k], HALF[dtype], "matrix %d" % k)
+
+
+@pytest.mark.parametrize("steps,eps", [(1, 1e-7), (2, 1e-3), (3, 0.0), (8, 1e-7)])
+def test_steps_and_eps(mrl, ctx, steps, eps):
+    x = matrix(torch.Generator().manual_seed(steps), 48, 90) * 1e-3
+    out = torch.empty(48, 90, device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda(), steps=steps, eps=eps)
+    ctx.synchronize()
+    near(out, x, HALF["f32"], "out", steps, eps)
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e30, 1e36])
+def test_scales_near_the_ends_of_the_range(mrl, ctx, scale):
+    """The norm is taken in 64 bits: neither its squares nor the quotient leave the range."""
+    x = matrix(torch.Generator().manual_seed(3), 70, 50) * scale
+    out = torch.empty(70, 50, device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda(), eps=0.0)
+    ctx.synchronize()
+    near(out, x, HALF["f32"], "out", eps=0.0)
+
+
+def test_zeros_ones_and_what_is_not_finite(mrl, ctx):
+    x = torch.zeros(4, 70, 90)
+    x[1] = 1.0                      # one direction only
+    x[2] = matrix(torch.Generator().manual_seed(1), 70, 90)
+    x[2, 3, 4] = float("inf")
+    x[3] = x[2]
+    x[3, 3, 4] = float("nan")
+    out = torch.empty_like(x, device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda())
+    ctx.synchronize()
+    assert not out[0].any() and torch.isnan(out[2]).all() and torch.isnan(out[3]).all()
+    near(out[1], x[1], HALF["f32"], "ones")
+
+
+def test_a_few_large_entries(mrl, ctx):
+    """Entries at the top of the pieces' range, next to ones far below."""
+    x = torch.randn(500, 700, generator=torch.Generator().manual_seed(2)) * 1e-4
+    x[3, 5], x[100, 200] = 1.0, -0.7
+    out = torch.empty(500, 700, device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda())
+    ctx.synchronize()
+    near(out, x, HALF["f32"], "out")
+
+
+def nets(mrl):
+    return {
+        "plain": mrl.seq(mrl.LinearReLU(8, 64), mrl.LinearReLU(64, 100), mrl.Linear(100, 4)),
+        "gauss": mrl.seq(mrl.LinearTanh(17, 33), mrl.LinearTanh(33, 70), mrl.StochasticActor(70, 6)),
+        "deep": mrl.seq(*[mrl.Linear(12, 12)] * 7, mrl.Linear(12, 300)),
+        "one": mrl.Linear(5, 3),
+    }
+
+
+@pytest.mark.parametrize("net,layers,nesterov,decay", [("plain", None, True, 0.0), ("plain", (0, 1, 2), False, 0.1), ("plain", (), True, 0.0), ("plain", (1,), True, 0.5),
+                                                       ("gauss", None, True, 0.01), ("gauss", (2,), True, 0.0), ("deep", None, False, 0.0),
+                                                       ("deep", range(8), True, 0.0), ("one", None, True, 0.0), ("one", (0,), True, 0.0)])
+def test_muon_steps(mrl, ctx, net, layers, nesterov, decay):
+    print("muon", net, layers, nesterov, decay, flush=True)
+    model = nets(mrl)[net]
+    opt = mrl.Muon(model, lr=0.03, momentum=0.9, nesterov=nesterov, weight_decay=decay, layers=layers, adam_lr=1e-3, beta1=0.8, beta2=0.99, adam_eps=1e-6)
+    n = model.PARAM_SIZE
+    gen = torch.Generator().manual_seed(n)
+    params, state = torch.randn(n, generator=gen), torch.zeros(2 * n)
+    grads = [torch.randn(n, generator=gen) * 0.1 for _ in range(3)]
+    p, s = params.cuda(), state.cuda()
+    chosen = set(range(len(model.layers) - 1) if layers is None else layers)
+    w, m2 = params.double(), state.double()
+    loose = torch.zeros(n, dtype=torch.float64)       # what the products may move each parameter by
+    for t, g in enumerate(grads, 1):
+        opt.step_gpu(ctx, p, g.cuda(), s)
+        g, at, adam = g.double(), 0, torch.ones(n, dtype=torch.bool)
+        for k, (kind, rows, cols) in enumerate(model.layers):
+            size = rows * cols
+            if k in chosen:
+                v = m2[2 * at:2 * at + size]
+                v.mul_(0.9).add_(g[at:at + size])
+                u = g[at:at + size] + 0.9 * v if nesterov else v
+                o = polynomial(u.view(rows, cols))
+                moved = (polynomial(u.view(rows, cols), gen=torch.Generator().manual_seed(t)) - o).norm().item()
+                factor = 0.03 * max(1.0, cols / rows) ** 0.5
+                w[at:at + size] = w[at:at + size] * (1 - 0.03 * decay) - factor * o.reshape(-1)
+                loose[at:at + size] += factor * 8 * moved
+                adam[at:at + size] = False
+            at += size + (2 if kind == mrl.STOCHASTIC_ACTOR else 1) * cols
+        assert at == n
+        m, v = m2[0::2][adam], m2[1::2][adam]
+        m, v = 0.8 * m + 0.2 * g[adam], 0.99 * v + 0.01 * g[adam] ** 2
+        m2[0::2][adam], m2[1::2][adam] = m, v
+        w[adam] -= 1e-3 * (m / (1 - 0.8 ** t)) / ((v / (1 - 0.99 ** t)).sqrt() + 1e-6)
+    ctx.synchronize()
+    assert opt.t == 3
+    # a step rounds a parameter twice and its update (at most 0.003 by Adam, as many roundings as Adam has operations); the constants
+    # 1 - beta, beta and the bias corrections are rounded to fp32
+    bound = loose + 3 * (3 * 2.0 ** -24 * (w.abs() + 0.1) + 0.003 * 40 * 2.0 ** -24)
+    assert ((p.cpu().double() - w).abs() <= bound).all()
+    assert ((s.cpu().double() - m2).abs() <= 3 * 6 * 2.0 ** -24 * (m2.abs() + 0.5)).all()
+
+
+def test_network_with_muon_trains_and_round_trips(mrl, ctx, tmp_path):
+    """Behind Network as any optimiser: the parameters after update_gpu are those of the step on its own buffers, a checkpoint holds the momentum."""
+    model = mrl.seq(mrl.LinearTanh(6, 48), mrl.LinearTanh(48, 48), mrl.Linear(48, 2))
+    net = mrl.Network(ctx, model, mrl.Muon(model, lr=0.05), mrl.Xavier(seed=4))
+    x, out, cache = torch.randn(32, 6, device="cuda"), torch.empty(64, device="cuda"), torch.empty(32 * model.CACHE_SIZE, device="cuda")
+    net.forward_gpu(out, x.view(-1), cache)
+    net.backward_gpu(torch.empty(192, device="cuda"), out.clone(), cache)
+    params, state = net.params.clone(), net.optimizer_state.clone()
+    other = mrl.Muon(model, lr=0.05)
+    other.step_gpu(ctx, params, net.grads, state)
+    net.update_gpu()
+    ctx.synchronize()
+    assert torch.equal(params, net.params) and torch.equal(state, net.optimizer_state) and state[:6 * 48].any()
+    net.save_checkpoint(str(tmp_path / "net.txt"))
+    again = mrl.Network(ctx, model, mrl.Muon(model), mrl.Xavier(seed=5))
+    again.load_checkpoint(str(tmp_path / "net.txt"))
+    assert torch.equal(again.params, net.params) and torch.equal(again.optimizer_state, net.optimizer_state)
+
+
+def test_captured_graphs_keep_their_workspaces(mrl, ctx):
+    gen = torch.Generator().manual_seed(8)
+    xs = [matrix(gen, 200, 330).cuda(), matrix(gen, 330, 200).cuda()]
+    wants = [torch.empty_like(x) for x in xs]
+    for x, w in zip(xs, wants):
+        mrl.orthogonalize(ctx, w, x)
+    model = nets(mrl)["plain"]
+    opt, n = mrl.Muon(model), model.PARAM_SIZE
+    p0, g = torch.randn(n, generator=gen).cuda(), torch.randn(n, generator=gen).cuda()
+    wp, ws = p0.clone(), torch.zeros(2 * n, device="cuda")
+    mrl.Muon(model).step_gpu(ctx, wp, g, ws)
+    ctx.synchronize()
+    side = torch.cuda.Stream()
+    cctx = mrl.DeviceContext("cuda:0", stream=side)
+    graphs, outs = [], [torch.empty_like(x) for x in xs]
+    p, s = p0.clone(), torch.zeros(2 * n, device="cuda")
+    for x, o in zip(xs, outs):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            mrl.orthogonalize(cctx, o, x)
+            if o is outs[0]:
+                opt.step_gpu(cctx, p, g, s)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        p.copy_(p0)
+        s.zero_()
+        for o in outs:
+            o.fill_(3)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        mrl.orthogonalize(ctx, torch.empty_like(xs[0]), xs[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants)) and torch.equal(p, wp) and torch.equal(s, ws)
+    del graphs
+    cctx.close()
+
+
+def test_library_refusals(mrl, ctx):
+    lib, x = mrl._lib.lib(), torch.zeros(1 << 16, device="cuda")
+    p, size = ctypes.c_void_p(x.data_ptr()), ctypes.c_uint64(0)
+    assert lib.mrl_orthogonalize_workspace(1, 8, 8, ctypes.byref(size)) == 0 and size.value <= 1 << 18
+
+    def orth(dtype=0, count=1, rows=8, cols=8, src=p, steps=5, eps=1e-7, ws=p, n=size.value):
+        return lib.mrl_orthogonalize(ctx.handle, dtype, count, rows, cols, src, p, steps, eps, ws, n)
+    for bad, text in ((dict(dtype=5), b"element type"), (dict(count=-1), b"count"), (dict(rows=0), b"sides"), (dict(cols=40000), b"sides"),
+                      (dict(src=None), b"NULL"), (dict(steps=0), b"steps"), (dict(steps=65), b"steps"), (dict(eps=-1.0), b"eps"),
+                      (dict(eps=float("nan")), b"eps"), (dict(n=size.value - 1), b"workspace holds"), (dict(ws=None), b"workspace holds"),
+                      (dict(ws=ctypes.c_void_p(x.data_ptr() + 8)), b"aligned"), (dict(count=2), b"workspace holds")):
+        assert orth(**bad) == -1 and text in lib.mrl_last_error(), bad
+    Matrix = mrl._lib.Matrix
+
+    def muon(mats=((0, 4, 4),), n=100, t=1, steps=5, params=p, ws=p, size=1 << 18):
+        array = (Matrix * max(1, len(mats)))(*[Matrix(*m) for m in mats])
+        return lib.mrl_muon_step(ctx.handle, params, p, p, n, len(mats), array, t, 0.1, 0.9, 1, 0.0, steps, 1e-7, 1e-3, 0.9, 0.99, 1e-8, ws, size)
+    for bad, text in ((dict(mats=((0, 4, 4), (15, 4, 4))), b"overlaps"), (dict(mats=((90, 4, 4),)), b"overlaps"), (dict(mats=((-1, 4, 4),)), b"overlaps"),
+                      (dict(mats=((0, 0, 4),)), b"sides"), (dict(n=-1), b"n <"), (dict(t=0), b"step count"), (dict(steps=0), b"steps"), (dict(params=None), b"NULL"),
+                      (dict(size=100), b"workspace holds")):
+        assert muon(**bad) == -1 and text in lib.mrl_last_error(), bad
+    ctx.synchronize()
+    assert not x.any()

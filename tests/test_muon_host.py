@@ -1,0 +1,68 @@
+"""What orthogonalize and Muon refuse before anything reaches the device, and the shares of the flat parameters that Muon takes."""
+import ctypes
+
+import pytest
+import torch
+
+
+class HostContext:
+    device, handle, stream = torch.device("cpu"), ctypes.c_void_p(), None
+
+
+@pytest.mark.parametrize("x,out,text", [
+    (torch.zeros(4), torch.zeros(4), "rows, cols"), (torch.zeros(2, 2, 2, 2), torch.zeros(2, 2, 2, 2), "rows, cols"),
+    (torch.zeros(3, 4, dtype=torch.float64), torch.zeros(3, 4, dtype=torch.float64), "float32 or bfloat16"),
+    (torch.zeros(3, 4), torch.zeros(4, 3), "does not fit"), (torch.zeros(3, 4), torch.zeros(3, 4, dtype=torch.bfloat16), "does not fit"),
+    (torch.zeros(4, 3).T, torch.zeros(3, 4), "contiguous"), (torch.zeros(3, 4), torch.zeros(4, 3).T, "contiguous"),
+    (torch.zeros(3, 4, device="meta"), torch.zeros(3, 4), "on cpu expected"),
+])
+def test_orthogonalize_refuses(mrl, x, out, text):
+    with pytest.raises(mrl.MrlError, match=text):
+        mrl.orthogonalize(HostContext, out, x)
+
+
+def test_nothing_to_do_needs_no_device(mrl):
+    for shape in ((0, 4), (4, 0), (0, 3, 4)):
+        mrl.orthogonalize(HostContext, torch.zeros(shape), torch.zeros(shape))
+
+
+def test_muon_shares(mrl):
+    model = mrl.seq(mrl.LinearReLU(8, 256), mrl.LinearTanh(256, 64), mrl.StochasticActor(64, 4))
+
+    def shares(**kw):
+        opt = mrl.Muon(model, **kw)
+        return [(m.offset, m.rows, m.cols) for m in opt._matrices[:opt._count]]
+    second = 8 * 256 + 256
+    third = second + 256 * 64 + 64
+    assert shares() == [(0, 8, 256), (second, 256, 64)]
+    assert shares(layers=(2, 0)) == [(0, 8, 256), (third, 64, 4)] and shares(layers=()) == []
+    assert mrl.Muon(model).STATE_PER_PARAM == 2 and mrl.Muon(model).t == 0
+    for bad in ((3,), (-1,)):
+        with pytest.raises(mrl.MrlError, match="layers"):
+            mrl.Muon(model, layers=bad)
+
+
+def test_muon_step_refuses(mrl):
+    model = mrl.seq(mrl.Linear(4, 6), mrl.Linear(6, 2))
+    n, opt = model.PARAM_SIZE, mrl.Muon(model)
+    for p, g, s, text in ((n - 1, n, 2 * n, "params"), (n, n + 1, 2 * n, "grads"), (n, n, n, "state")):
+        with pytest.raises(mrl.MrlError, match=text):
+            opt.step_gpu(HostContext, torch.zeros(p), torch.zeros(g), torch.zeros(s))
+    with pytest.raises(mrl.MrlError, match="params"):
+        opt.step_gpu(HostContext, torch.zeros(n, dtype=torch.bfloat16), torch.zeros(n), torch.zeros(2 * n))
+    assert opt.t == 0
+
+
+def test_null_contexts_and_workspace_queries(mrl):
+    size = ctypes.c_uint64(0)
+    mrl._lib.call("mrl_orthogonalize_workspace", 3, 100, 40, ctypes.byref(size))
+    assert size.value >= 3 * (6 * 2 * 40 * 100 + 4 * 2 * 40 * 40)
+    mrl._lib.call("mrl_muon_workspace", 0, None, ctypes.byref(size))
+    assert size.value == 0
+    for name, args in (("mrl_orthogonalize", (None, 0, 1, 4, 4, None, None, 5, 1e-7, None, 0)),
+                       ("mrl_muon_step", (None, None, None, None, 4, 0, None, 1, 0.1, 0.9, 1, 0.0, 5, 1e-7, 1e-3, 0.9, 0.99, 1e-8, None, 0))):
+        with pytest.raises(mrl.MrlError, match="ctx"):
+            mrl._lib.call(name, *args)
+    for args in ((1, 0, 4), (-1, 4, 4), (1, 4, 1 << 16)):
+        with pytest.raises(mrl.MrlError):
+            mrl._lib.call("mrl_orthogonalize_workspace", *args, ctypes.byref(size))
