@@ -25,6 +25,14 @@ def _on_device(ctx, name, t):
         raise _lib.MrlError("%s: a tensor on %s expected, got one on %s" % (name, ctx.device, t.device))
 
 
+def _scratch(ctx, n):
+    """n bytes from torch's allocator on the context's stream: a captured graph keeps its own."""
+    if torch.cuda.current_stream(ctx.device) == ctx.stream:
+        return torch.empty(n, dtype=torch.uint8, device=ctx.device)
+    with torch.cuda.stream(ctx.stream):
+        return torch.empty(n, dtype=torch.uint8, device=ctx.device)
+
+
 class DeviceContext:
     def __init__(self, device="cuda:0", stream=None):
         if not torch.cuda.is_available():

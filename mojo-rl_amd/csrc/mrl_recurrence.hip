@@ -23,73 +23,88 @@ namespace mrl {
 namespace {
 
 constexpr float TINY = 0x1p-149f;
-constexpr int MAX_WAVES = 16;
-
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+constexpr int MAX_WAVES = 8;   // of a workgroup with more than one channel per lane, for the registers; twice that with one
 
 struct bf16_t { unsigned short bits; };
 
-MRL_DEV void load_n(const float *p, float (&x)[4]) {
-    const f32x4u v = *reinterpret_cast<const f32x4u *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = v[i];
-}
-MRL_DEV void load_n(const bf16_t *p, float (&x)[4]) {
-    const u16x4u v = *reinterpret_cast<const u16x4u *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float((unsigned)v[i] << 16);
-}
-MRL_DEV void load_n(const float *p, float (&x)[1]) { x[0] = *p; }
-MRL_DEV void load_n(const bf16_t *p, float (&x)[1]) { x[0] = __uint_as_float((unsigned)p->bits << 16); }
+// V neighbouring values as they are in memory
+template <class E, int V> struct Raw;
+template <int V> struct Raw<float, V> {
+    typedef float vec __attribute__((ext_vector_type(V), aligned(4)));
+    vec v;
+    MRL_DEV void load(const float *p) { v = *reinterpret_cast<const vec *>(p); }
+    MRL_DEV float operator[](int i) const { return v[i]; }
+};
+template <int V> struct Raw<bf16_t, V> {
+    typedef unsigned short vec __attribute__((ext_vector_type(V), aligned(2)));
+    vec v;
+    MRL_DEV void load(const bf16_t *p) { v = *reinterpret_cast<const vec *>(p); }
+    MRL_DEV float operator[](int i) const { return __uint_as_float((unsigned)v[i] << 16); }
+};
 
-// the elements from `skip` on (the ones before belong to the neighbouring lane)
 template <int V>
-MRL_DEV void store_n(float *p, const float (&x)[V], int skip) {
-    if (V == 4 && skip == 0) {
-        *reinterpret_cast<f32x4u *>(p) = f32x4u{x[0], x[1], x[V - 2], x[V - 1]};
+MRL_DEV void load_state(const float *p, float (&x)[V]) {
+    Raw<float, V> r;
+    r.load(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = r[i];
+}
+
+// The elements from `skip` on (the ones before belong to the neighbouring lane); `whole`: no lane has any to skip.
+template <int V>
+MRL_DEV void store_n(float *p, const float (&x)[V], int skip, bool whole) {
+    typename Raw<float, V>::vec v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = x[i];
+    if (whole || skip == 0) {
+        *reinterpret_cast<typename Raw<float, V>::vec *>(p) = v;
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+        for (int i = 1; i < V; ++i)
             if (i >= skip) p[i] = x[i];
     }
 }
 template <int V>
-MRL_DEV void store_n(bf16_t *p, const float (&x)[V], int skip) {
-    if (V == 4) {
-        const v4bf h = __builtin_convertvector((v4f{x[0], x[V > 1 ? 1 : 0], x[V > 2 ? 2 : 0], x[V - 1]}), v4bf);
-        const u16x4u v = __builtin_bit_cast(u16x4u, h);
-        if (skip == 0) {
-            *reinterpret_cast<u16x4u *>(p) = v;
-        } else {
+MRL_DEV void store_n(bf16_t *p, const float (&x)[V], int skip, bool whole) {
+    typedef float floats __attribute__((ext_vector_type(V)));
+    typedef __bf16 halves __attribute__((ext_vector_type(V)));
+    floats f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i >= skip) p[i].bits = v[i];
-        }
+    for (int i = 0; i < V; ++i) f[i] = x[i];
+    const typename Raw<bf16_t, V>::vec v = __builtin_bit_cast(typename Raw<bf16_t, V>::vec, __builtin_convertvector(f, halves));
+    if (whole || skip == 0) {
+        *reinterpret_cast<typename Raw<bf16_t, V>::vec *>(p) = v;
     } else {
-        p->bits = __builtin_bit_cast(unsigned short, (__bf16)x[0]);
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+            if (i >= skip) p[i].bits = v[i];
     }
 }
 
-// a = sigmoid(g) and rest = 1 - a, both to a few roundings of their own value.  exp(-|g|) = 2^y (1 + r ln 2) with r what rounding
-// y = -|g| / ln 2 left; beyond 128 both ends are 0 and 1 in fp32 (and the difference of infinities would be NaN).
-MRL_DEV void gates(float g, float &a, float &rest) {
-    float m = fabsf(g);
-    m = m > 128.0f ? 128.0f : m;   // (NaN stays)
-    const float y = -m * 1.44269502f;
-    const float r = fmaf(-m, 1.44269502f, -y) - m * 1.92596299e-8f;
+// a = sigmoid(g) and rest = 1 - a, both relative to their own value: with e = exp(-g) = 2^y, a = 1 / (1 + e) and rest = e a.  The
+// argument is held where e stays finite (a below 2^-126 counts as 2^-126).  Rounding y = -g / ln 2 makes e |g| 2^-24 off; in fp32,
+// where memory leaves the time for it, that is taken back: 2^y (1 + r ln 2) with r what the rounding left.  In bf16 gate and
+// value are given to 2^-9, and the scan is bound by these instructions.
+// (minimum and maximum, unlike fmin and fmax, keep NaN.)
+MRL_DEV void gates(const float *, float g, float &a, float &rest) {
+    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 200.0f);
+    const float y = g * -1.44269502f;
+    const float r = fmaf(g, -1.44269502f, -y);
     float e = __builtin_amdgcn_exp2f(y);
     e = fmaf(e, r * 0.693147182f, e);
-    const float inv = __builtin_amdgcn_rcpf(1.0f + e), low = e * inv;
-    a = g >= 0.0f ? inv : low;
-    rest = g >= 0.0f ? low : inv;
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * a;
+}
+MRL_DEV void gates(const bf16_t *, float g, float &a, float &rest) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269502f, 125.0f));
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * a;
 }
 
 struct Scan {
-    int T, N, D, lanes_per_row, W, segments, segment_steps;
+    int T, N, D, lanes_per_row, W, segments, segment_steps, share;   // share: of a segment's steps, a wavefront's
     int groups;              // of 64 lanes
+    int whole;               // no lane has elements to skip
     long lanes;              // N * lanes_per_row
     const void *gate, *value, *out, *grad_out;
     long gate_ld, value_ld, out_ld, grad_out_ld, grad_gate_ld, grad_value_ld;
@@ -98,7 +113,7 @@ struct Scan {
     const float *state_in;   // backward
     float *last;             // forward: state_out; backward: grad_state_in
     void *dst, *dst2;        // forward: out; backward: grad_gate, grad_value
-    float *ws;               // [segments][2][lanes * V] (A, B), then [lanes * V]: the first state
+    float *ws;               // rows of lanes * V: (A, B) of every segment, (A, B) of every wavefront's share, the first state
 };
 
 // What a lane works on: V channels from column d of environment n.  The last lane of a row whose width is no multiple of V starts
@@ -124,250 +139,377 @@ MRL_DEV Place place(const Scan &s, int group) {
     return p;
 }
 
-// The flag of the step before t for environment n, 0 where the caller gave none: the load itself is from memory that is there
-// whatever t is, so that a tile's loads stand together without a branch or a wait among them.
-MRL_DEV float flag_ahead(const Scan &s, long t, int n) {
-    const float *row = t > 0 ? (s.dones ? s.dones + (t - 1) * s.N : s.prev_dones) : (s.prev_dones ? s.prev_dones : s.dones);
-    return row[n];
-}
-MRL_DEV bool is_cut(const Scan &s, long t, float flag) { return (t > 0 ? s.dones : s.prev_dones) != nullptr && flag > 0.5f; }
-
-template <int V>
-MRL_DEV void compose(float (&state)[V], const float *A, const float *B) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) state[i] = A[i] == 0.0f ? B[i] : fmaf(A[i], state[i], B[i]);
-}
-
-template <int V>
-MRL_DEV void put(float *p, const float (&x)[V]) {
-    if (V == 4) *reinterpret_cast<v4f *>(p) = v4f{x[0], x[V > 1 ? 1 : 0], x[V > 2 ? 2 : 0], x[V - 1]};
-    else p[0] = x[0];
-}
-template <int V>
-MRL_DEV void get(const float *p, float (&x)[V]) {
-    if (V == 4) {
-        const v4f v = *reinterpret_cast<const v4f *>(p);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = v[i];
-    } else {
-        x[0] = p[0];
-    }
-}
-
-// The state ahead of wavefront w's share, from the state ahead of the workgroup's and the shares' (A, B) in LDS; `carry` becomes
-// the state behind all of them.
-template <int V>
-MRL_DEV void through_waves(const float *lds, int W, int w, float (&carry)[V], float (&mine)[V]) {
-    for (int i = 0; i < W; ++i) {
-        if (i == w) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) mine[k] = carry[k];
-        }
-        float A[V], B[V];
-        get(lds + ((size_t)i * 2 * 64 + threadIdx.x) * V, A);
-        get(lds + (((size_t)i * 2 + 1) * 64 + threadIdx.x) * V, B);
-        compose(carry, A, B);
-    }
-}
-template <int V>
-MRL_DEV void leave(float *lds, int w, const float (&A)[V], const float (&B)[V]) {
-    put(lds + ((size_t)w * 2 * 64 + threadIdx.x) * V, A);
-    put(lds + (((size_t)w * 2 + 1) * 64 + threadIdx.x) * V, B);
-}
-
 // step number p of the scan: time p forwards, T - 1 - p backwards
 template <bool BACK>
 MRL_DEV long time_of(const Scan &s, long p) { return BACK ? s.T - 1 - p : p; }
 
-// One step's (A, B) on top of those before it.  The backward scan's state is G[t+1], what goes into step t from behind it.
-template <bool BACK, int V>
-MRL_DEV void add_step(float (&A)[V], float (&B)[V], float &low, bool cut, const float (&g)[V], const float (&x)[V]) {
-    low = cut ? 0.0f : low;
+// L steps' inputs of a lane
+template <class E, int V, int L, bool BACK>
+struct Steps {
+    Raw<E, V> g[L], x[L];
+    Raw<E, V> dh[BACK ? L : 1], before[BACK ? L : 1];
+    float flag[L];   // of the step before: above 0.5 where it ended an episode
+    bool full;       // all L steps are there, none is the rollout's first going backwards
+};
+// and their gates
+template <int V, int L>
+struct Gates {
+    float a[L][V], rest[L][V];
+    template <class E, bool BACK>
+    MRL_DEV explicit Gates(const Steps<E, V, L, BACK> &k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float a, rest;
-        gates(g[i], a, rest);
-        const float after = BACK ? a * (B[i] + x[i]) : fmaf(a, B[i], rest * x[i]);
-        B[i] = cut ? (BACK ? 0.0f : rest * x[i]) : after;
-        A[i] = cut ? 0.0f : fmaxf(A[i] * a, low);
+        for (int j = 0; j < L; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) gates((const E *)nullptr, k.g[j][i], a[j][i], rest[j][i]);
+    }
+};
+template <class E, int V, bool BACK>
+struct Rows {   // where a lane's columns of step 0 are, and from a step to the next
+    const E *gate, *value, *out, *grad;
+    long gate_step, value_step, out_step, grad_step;
+    bool flagged, whole;
+    MRL_DEV Rows(const Scan &s, const Place &at) {
+        gate = (const E *)s.gate + (long)at.n * s.gate_ld + at.d;
+        value = (const E *)s.value + (long)at.n * s.value_ld + at.d;
+        out = (const E *)s.out + (long)at.n * s.out_ld + at.d;
+        grad = (const E *)s.grad_out + (long)at.n * s.grad_out_ld + at.d;
+        gate_step = (long)s.N * s.gate_ld;
+        value_step = (long)s.N * s.value_ld;
+        out_step = (long)s.N * s.out_ld;
+        grad_step = (long)s.N * s.grad_out_ld;
+        flagged = s.dones != nullptr || s.prev_dones != nullptr;
+        whole = s.whole != 0;
+    }
+};
+
+// Steps p0 .. p0 + L - 1; those from `to` on are step to - 1 again, so that all loads stand together without a branch or a wait
+// among them.  COEFFICIENTS: only what (A, B) take.
+template <class E, int V, int L, bool BACK, bool COEFFICIENTS = false>
+MRL_DEV void load_steps(const Scan &s, const Place &at, const Rows<E, V, BACK> &r, long p0, long to, Steps<E, V, L, BACK> &k) {
+    const bool full = p0 + L <= to && (!BACK || p0 + L < s.T);
+    if (full) {
+        long t = time_of<BACK>(s, p0);
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            k.g[j].load(r.gate + t * r.gate_step);
+            if (!(BACK && COEFFICIENTS)) k.x[j].load(r.value + t * r.value_step);
+            if constexpr (BACK) {
+                k.dh[j].load(r.grad + t * r.grad_step);
+                if (!COEFFICIENTS) k.before[j].load(r.out + (t - 1) * r.out_step);
+            }
+            t += BACK ? -1 : 1;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const long t = time_of<BACK>(s, min(p0 + j, to - 1));
+            k.g[j].load(r.gate + t * r.gate_step);
+            if (!(BACK && COEFFICIENTS)) k.x[j].load(r.value + t * r.value_step);
+            if constexpr (BACK) {
+                k.dh[j].load(r.grad + t * r.grad_step);
+                if (!COEFFICIENTS) k.before[j].load(r.out + max(t - 1, 0L) * r.out_step);
+            }
+        }
+    }
+    k.full = full;
+    if (r.flagged) {
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const long t = time_of<BACK>(s, min(p0 + j, to - 1));
+            const float *row = t > 0 ? s.dones + (t - 1) * s.N : s.prev_dones;
+            k.flag[j] = (t > 0 ? s.dones : s.prev_dones) != nullptr ? row[at.n] : 0.0f;
+        }
+    }
+}
+// full, and no lane has a cut among the steps
+template <class E, int V, int L, bool BACK>
+MRL_DEV bool is_plain(const Rows<E, V, BACK> &r, const Steps<E, V, L, BACK> &k) {
+    if (!r.flagged) return k.full;
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < L; ++j) most = fmaxf(most, k.flag[j]);
+    return k.full && __ballot(most > 0.5f) == 0;
+}
+
+template <int V>
+MRL_DEV void compose(float (&state)[V], const float (&A)[V], const float (&B)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) state[i] = A[i] == 0.0f ? B[i] : fmaf(A[i], state[i], B[i]);
+}
+// (A, B) <- (A1, B1) after (A, B)
+template <int V>
+MRL_DEV void compose(float (&A)[V], float (&B)[V], const float (&A1)[V], const float (&B1)[V]) {
+    compose(B, A1, B1);
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = A1[i] == 0.0f || A[i] == 0.0f ? 0.0f : fmaxf(A[i] * A1[i], TINY);
+}
+
+template <int V>
+MRL_DEV void put(float *p, const float (&x)[V]) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    vec v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = x[i];
+    *reinterpret_cast<vec *>(p) = v;
+}
+template <int V>
+MRL_DEV void get(const float *p, float (&x)[V]) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const vec v = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = v[i];
+}
+template <int V>
+MRL_DEV void identity(float (&A)[V], float (&B)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { A[i] = 1.0f; B[i] = 0.0f; }
+}
+
+// The state ahead of wavefront w's share, from the state ahead of the workgroup's and the shares' (A, B), `apart` floats from
+// one coefficient's row to the next; `carry` becomes the state behind all of them.
+template <int V>
+MRL_DEV void through_waves(const float *shares, long apart, int W, int w, float (&carry)[V], float (&mine)[V]) {
+#pragma unroll 4
+    for (int i = 0; i < W; ++i) {
+        float A[V], B[V];
+        get(shares + (long)i * 2 * apart, A);
+        get(shares + ((long)i * 2 + 1) * apart, B);
+#pragma unroll
+        for (int k = 0; k < V; ++k) mine[k] = i == w ? carry[k] : mine[k];
+        compose(carry, A, B);
     }
 }
 
-// A segment's (A, B): every wavefront composes the steps of its own share, the first one the shares.
+// (A, B) of these steps on top of those before them; `cuts`: whether a lane has seen a cut.  The backward scan's state is G[t+1],
+// what goes into step t from behind it.
+template <bool PLAIN, class E, int V, int L, bool BACK>
+MRL_DEV void add_steps(const Rows<E, V, BACK> &r, const Steps<E, V, L, BACK> &k, const Gates<V, L> &gate, long p0, long to, float (&A)[V], float (&B)[V], bool &cuts) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        if (!PLAIN && p0 + j >= to) break;
+        const bool cut = !PLAIN && r.flagged && k.flag[j] > 0.5f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (BACK) {
+                B[i] = gate.a[j][i] * (B[i] + k.dh[j][i]);
+                if (!PLAIN) B[i] = cut ? 0.0f : B[i];
+            } else {
+                if (!PLAIN) B[i] = cut ? 0.0f : B[i];
+                B[i] = fmaf(gate.a[j][i], B[i], gate.rest[j][i] * k.x[j][i]);
+            }
+            A[i] *= gate.a[j][i];
+        }
+        if (!PLAIN) cuts |= cut;
+    }
+}
+// A of a chain that has a cut is 0, that of one without never
+template <int V>
+MRL_DEV void settle(float (&A)[V], bool cuts) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = cuts ? 0.0f : fmaxf(A[i], TINY);
+}
+
+// These steps from the state ahead of them: results out, `mine` the state behind them.
+template <bool PLAIN, class E, int V, int L, bool BACK>
+MRL_DEV void do_steps(const Scan &s, const Place &at, const Rows<E, V, BACK> &r, const Steps<E, V, L, BACK> &k, const Gates<V, L> &gate, long p0,
+                      long to, float (&mine)[V]) {
+    E *dst = (E *)s.dst + (long)at.n * (BACK ? s.grad_gate_ld : s.out_ld) + at.d;
+    E *dst2 = (E *)s.dst2 + (long)at.n * s.grad_value_ld + at.d;
+    const long dst_step = (long)s.N * (BACK ? s.grad_gate_ld : s.out_ld), dst2_step = (long)s.N * s.grad_value_ld;
+    long t = time_of<BACK>(s, p0);
+#pragma unroll
+    for (int j = 0; j < L; ++j, t += BACK ? -1 : 1) {
+        if (!PLAIN && p0 + j >= to) break;
+        const bool cut = !PLAIN && r.flagged && k.flag[j] > 0.5f;
+        float y[V];
+        if constexpr (BACK) {
+            float y2[V], before[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) before[i] = k.before[j][i];
+            if (!PLAIN) {
+                if (t == 0) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) before[i] = 0.0f;
+                    if (s.state_in != nullptr) load_state(s.state_in + (long)at.n * s.D + at.d, before);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) before[i] = cut ? 0.0f : before[i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = k.dh[j][i] + mine[i];
+                y2[i] = gate.rest[j][i] * d;
+                mine[i] = gate.a[j][i] * d;
+                y[i] = gate.rest[j][i] * mine[i] * (before[i] - k.x[j][i]);
+                if (!PLAIN) mine[i] = cut ? 0.0f : mine[i];
+            }
+            if (at.live) store_n(dst2 + t * dst2_step, y2, at.skip, r.whole);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (!PLAIN) mine[i] = cut ? 0.0f : mine[i];
+                y[i] = mine[i] = fmaf(gate.a[j][i], mine[i], gate.rest[j][i] * k.x[j][i]);
+            }
+        }
+        if (at.live) store_n(dst + t * dst_step, y, at.skip, r.whole);
+        if (j == L - 1 || !PLAIN) {
+            if (p0 + j == s.T - 1 && at.live && s.last != nullptr) store_n(s.last + (long)at.n * s.D + at.d, mine, at.skip, r.whole);
+        }
+    }
+}
+
+// All steps from `from` to `to` in a row, the first L of them loaded.
+template <class E, int V, int L, bool BACK>
+MRL_DEV void stream_steps(const Scan &s, const Place &at, const Rows<E, V, BACK> &rows, long from, long to, Steps<E, V, L, BACK> &k, float (&mine)[V]) {
+    for (long p0 = from; p0 < to; p0 += L) {
+        if (p0 != from) load_steps(s, at, rows, p0, to, k);
+        const Gates<V, L> gate(k);
+        if (is_plain(rows, k)) do_steps<true>(s, at, rows, k, gate, p0, to, mine);
+        else do_steps<false>(s, at, rows, k, gate, p0, to, mine);
+    }
+}
+
+// A wavefront per group of lanes, all steps.
+template <class E, int V, int L, bool BACK>
+__global__ __launch_bounds__(256) void scan_alone_kernel(Scan s) {
+    const int group = blockIdx.x * blockDim.y + threadIdx.y;
+    if (group >= s.groups) return;
+    const Place at = place<V>(s, group);
+    const Rows<E, V, BACK> rows(s, at);
+    Steps<E, V, L, BACK> k;
+    load_steps(s, at, rows, 0, s.T, k);
+    float mine[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) mine[i] = 0.0f;
+    if (s.first != nullptr) load_state(s.first + (long)at.n * s.D + at.d, mine);
+    stream_steps(s, at, rows, 0, s.T, k, mine);
+}
+
+// A workgroup per group of lanes, its wavefronts L steps each of a tile of W L.
+template <class E, int V, int L, bool BACK>
+__global__ __launch_bounds__(64 * MAX_WAVES * (V == 1 ? 2 : 1)) void scan_tiles_kernel(Scan s) {
+    extern __shared__ float lds[];
+    const Place at = place<V>(s, blockIdx.x);
+    const Rows<E, V, BACK> rows(s, at);
+    const int w = threadIdx.y, W = s.W;
+    const int half = W * 2 * 64 * V;
+    float carry[V], mine[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) carry[i] = mine[i] = 0.0f;
+    if (s.first != nullptr) load_state(s.first + (long)at.n * s.D + at.d, carry);
+    int buffer = 0;
+    for (long t0 = 0; t0 < s.T; t0 += (long)W * L) {
+        const long p0 = t0 + w * L;
+        Steps<E, V, L, BACK> k;
+        load_steps(s, at, rows, p0, s.T, k);
+        const Gates<V, L> gate(k);
+        const bool plain = is_plain(rows, k);
+        float A[V], B[V];
+        bool cuts = false;
+        identity(A, B);
+        if (plain) add_steps<true>(rows, k, gate, p0, s.T, A, B, cuts);
+        else add_steps<false>(rows, k, gate, p0, s.T, A, B, cuts);
+        settle(A, cuts);
+        float *shares = lds + buffer * half + threadIdx.x * V;
+        put(shares + (w * 2) * 64 * V, A);
+        put(shares + (w * 2 + 1) * 64 * V, B);
+        __syncthreads();   // (the buffers alternate: the next tile's values go where nobody reads any more)
+        through_waves(shares, 64 * V, W, w, carry, mine);
+        buffer ^= 1;
+        if (plain) do_steps<true>(s, at, rows, k, gate, p0, s.T, mine);
+        else do_steps<false>(s, at, rows, k, gate, p0, s.T, mine);
+    }
+}
+
+MRL_DEV void share_of(const Scan &s, int seg, int w, long &from, long &to) {
+    const long end = min((long)s.T, (long)(seg + 1) * s.segment_steps);
+    from = min(end, (long)seg * s.segment_steps + (long)w * s.share);
+    to = min(end, from + s.share);
+}
+
+// First launch of a scan in segments: every wavefront's (A, B), and the segment's.
+template <class E, int V, int L, bool BACK>
+__global__ __launch_bounds__(64 * MAX_WAVES) void scan_coefficients_kernel(Scan s) {
+    extern __shared__ float lds[];
+    const Place at = place<V>(s, blockIdx.x);
+    const Rows<E, V, BACK> rows(s, at);
+    const int w = threadIdx.y, seg = blockIdx.y;
+    long from, to;
+    share_of(s, seg, w, from, to);
+    float A[V], B[V];
+    bool cuts = false;
+    identity(A, B);
+    for (long p0 = from; p0 < to; p0 += L) {
+        Steps<E, V, L, BACK> k;
+        load_steps<E, V, L, BACK, true>(s, at, rows, p0, to, k);
+        const Gates<V, L> gate(k);
+        if (is_plain(rows, k)) add_steps<true>(rows, k, gate, p0, to, A, B, cuts);
+        else add_steps<false>(rows, k, gate, p0, to, A, B, cuts);
+    }
+    settle(A, cuts);
+    const long row = s.lanes * V;
+    float *segments = s.ws + at.q * V, *shares = segments + (long)s.segments * 2 * row;
+    if (at.live) {
+        put(shares + ((long)seg * s.W + w) * 2 * row, A);
+        put(shares + (((long)seg * s.W + w) * 2 + 1) * row, B);
+    }
+    float *mine = lds + threadIdx.x * V;
+    put(mine + (w * 2) * 64 * V, A);
+    put(mine + (w * 2 + 1) * 64 * V, B);
+    __syncthreads();
+    if (w != 0 || !at.live) return;
+    for (int i = 1; i < s.W; ++i) {
+        float A1[V], B1[V];
+        get(mine + (i * 2) * 64 * V, A1);
+        get(mine + (i * 2 + 1) * 64 * V, B1);
+        compose(A, B, A1, B1);
+    }
+    put(segments + (long)seg * 2 * row, A);
+    put(segments + ((long)seg * 2 + 1) * row, B);
+    if (seg == 0) {   // the first state, which `last` may overwrite while segments still start
+        float first[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) first[i] = 0.0f;
+        if (s.first != nullptr) load_state(s.first + (long)at.n * s.D + at.d, first);
+        put(shares + (long)s.segments * s.W * 2 * row, first);
+    }
+}
+
+// Second launch: a wavefront starts from the segments ahead (its share of them, exchanged through LDS) and the wavefronts ahead.
 template <class E, int V, int L, bool BACK>
 __global__ __launch_bounds__(64 * MAX_WAVES) void scan_segments_kernel(Scan s) {
     extern __shared__ float lds[];
     const Place at = place<V>(s, blockIdx.x);
+    const Rows<E, V, BACK> rows(s, at);
     const int w = threadIdx.y, seg = blockIdx.y;
-    const long begin = (long)seg * s.segment_steps, end = min((long)s.T, begin + s.segment_steps);
-    const long share = (end - begin + s.W - 1) / s.W, from = min(end, begin + w * share), to = min(end, from + share);
-    const E *gate = (const E *)s.gate + (long)at.n * s.gate_ld + at.d;
-    const E *value = BACK ? (const E *)s.grad_out + (long)at.n * s.grad_out_ld + at.d : (const E *)s.value + (long)at.n * s.value_ld + at.d;
-    const long gate_step = (long)s.N * s.gate_ld, value_step = (long)s.N * (BACK ? s.grad_out_ld : s.value_ld);
-    const bool flagged = s.dones != nullptr || s.prev_dones != nullptr;
-    float A[V], B[V], low = TINY;
-#pragma unroll
-    for (int i = 0; i < V; ++i) { A[i] = 1.0f; B[i] = 0.0f; }
-    for (long p0 = from; p0 < to; p0 += L) {
-        float g[L][V], x[L][V], flag[L] = {};
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const long t = time_of<BACK>(s, min(p0 + j, to - 1));
-            load_n(gate + t * gate_step, g[j]);
-            load_n(value + t * value_step, x[j]);
-        }
-        if (flagged) {
-#pragma unroll
-            for (int j = 0; j < L; ++j) flag[j] = flag_ahead(s, time_of<BACK>(s, min(p0 + j, to - 1)), at.n);
-        }
-#pragma unroll
-        for (int j = 0; j < L; ++j)
-            if (p0 + j < to) add_step<BACK>(A, B, low, is_cut(s, time_of<BACK>(s, p0 + j), flag[j]), g[j], x[j]);
-    }
-    if (s.W > 1) leave(lds, w, A, B);
-    __syncthreads();
-    if (w != 0 || !at.live) return;
-    float total[V];
-    for (int i = 1; i < s.W; ++i) {
-        float A1[V], B1[V];
-        get(lds + ((size_t)i * 2 * 64 + threadIdx.x) * V, A1);
-        get(lds + (((size_t)i * 2 + 1) * 64 + threadIdx.x) * V, B1);
-        compose(B, A1, B1);
-#pragma unroll
-        for (int k = 0; k < V; ++k) A[k] = A1[k] == 0.0f || A[k] == 0.0f ? 0.0f : fmaxf(A[k] * A1[k], TINY);
-    }
+    long from, to;
+    share_of(s, seg, w, from, to);
+    Steps<E, V, L, BACK> k;
+    load_steps(s, at, rows, from, max(to, from + 1 - (from == s.T)), k);
     const long row = s.lanes * V;
-    put(s.ws + ((long)seg * 2) * row + at.q * V, A);
-    put(s.ws + ((long)seg * 2 + 1) * row + at.q * V, B);
-    if (seg == 0) {   // the first state, which `last` may overwrite while segments still start
-#pragma unroll
-        for (int k = 0; k < V; ++k) total[k] = 0.0f;
-        if (s.first != nullptr) load_n(s.first + (long)at.n * s.D + at.d, total);
-        put(s.ws + (long)s.segments * 2 * row + at.q * V, total);
+    const float *segments = s.ws + at.q * V, *shares = segments + (long)s.segments * 2 * row;
+    const int per = (seg + s.W - 1) / s.W, first = min(seg, w * per), last = min(seg, first + per);
+    float A[V], B[V];
+    identity(A, B);
+    for (int i = first; i < last; ++i) {
+        float A1[V], B1[V];
+        get(segments + (long)i * 2 * row, A1);
+        get(segments + ((long)i * 2 + 1) * row, B1);
+        compose(A, B, A1, B1);
     }
-}
-
-// The scan itself.  PART: a workgroup's W wavefronts share the steps of one group of lanes; otherwise every wavefront has a
-// group of its own.
-template <class E, int V, int L, bool BACK, bool PART>
-__global__ __launch_bounds__(PART ? 64 * MAX_WAVES : 256) void scan_kernel(Scan s) {
-    extern __shared__ float lds[];
-    const int w = PART ? threadIdx.y : 0, W = PART ? s.W : 1, seg = PART ? blockIdx.y : 0;
-    const int group = PART ? blockIdx.x : blockIdx.x * blockDim.y + threadIdx.y;
-    if (!PART && group >= s.groups) return;
-    const Place at = place<V>(s, group);
-    const long begin = PART ? (long)seg * s.segment_steps : 0, end = PART ? min((long)s.T, begin + s.segment_steps) : s.T;
-    const int half = W * 2 * 64 * V;
-    const bool flagged = s.dones != nullptr || s.prev_dones != nullptr;
-    int buffer = 0;
+    float *exchange = lds + threadIdx.x * V;
+    put(exchange + (w * 2) * 64 * V, A);
+    put(exchange + (w * 2 + 1) * 64 * V, B);
     float carry[V], mine[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = mine[i] = 0.0f;
-    if (PART && s.segments > 1) {
-        // each wavefront composes its share of the segments ahead of this one
-        const long row = s.lanes * V;
-        get(s.ws + (long)s.segments * 2 * row + at.q * V, carry);
-        const int share = (seg + W - 1) / W, from = min(seg, w * share), to = min(seg, from + share);
-        float A[V], B[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) { A[i] = 1.0f; B[i] = 0.0f; }
-        for (int k = from; k < to; ++k) {
-            float A1[V], B1[V];
-            get(s.ws + (long)k * 2 * row + at.q * V, A1);
-            get(s.ws + ((long)k * 2 + 1) * row + at.q * V, B1);
-            compose(B, A1, B1);
-#pragma unroll
-            for (int i = 0; i < V; ++i) A[i] = A1[i] == 0.0f || A[i] == 0.0f ? 0.0f : fmaxf(A[i] * A1[i], TINY);
-        }
-        leave(lds, w, A, B);
-        __syncthreads();
-        through_waves(lds, W, w, carry, mine);
-        buffer = 1;
-    } else if (s.first != nullptr) {
-        load_n(s.first + (long)at.n * s.D + at.d, carry);
+    get(shares + (long)s.segments * s.W * 2 * row, carry);
+    __syncthreads();
+    through_waves(exchange, 64 * V, s.W, -1, carry, mine);
+    for (int i = 0; i < w; ++i) {
+        get(shares + ((long)seg * s.W + i) * 2 * row, A);
+        get(shares + (((long)seg * s.W + i) * 2 + 1) * row, B);
+        compose(carry, A, B);
     }
-    const E *gate = (const E *)s.gate + (long)at.n * s.gate_ld + at.d;
-    const E *value = (const E *)s.value + (long)at.n * s.value_ld + at.d;
-    const long gate_step = (long)s.N * s.gate_ld, value_step = (long)s.N * s.value_ld, out_step = (long)s.N * s.out_ld;
-    const E *out = (const E *)s.out + (long)at.n * s.out_ld + at.d;
-    const E *grad = (const E *)s.grad_out + (long)at.n * s.grad_out_ld + at.d;
-    const long grad_step = (long)s.N * s.grad_out_ld, dgate_step = (long)s.N * s.grad_gate_ld, dvalue_step = (long)s.N * s.grad_value_ld;
-    E *dst = (E *)s.dst + (long)at.n * (BACK ? s.grad_gate_ld : s.out_ld) + at.d;
-    E *dst2 = (E *)s.dst2 + (long)at.n * s.grad_value_ld + at.d;
-    for (long tile = begin; tile < end; tile += (long)W * L) {
-        const long p0 = tile + w * L;
-        float g[L][V], x[L][V], dh[BACK ? L : 1][V], h1[BACK ? L : 1][V];
-        float flag[L] = {};
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const long t = time_of<BACK>(s, min(p0 + j, end - 1));
-            load_n(gate + t * gate_step, g[j]);
-            load_n(value + t * value_step, x[j]);
-            if (BACK) {
-                load_n(grad + t * grad_step, dh[j]);
-                load_n(out + max(t - 1, 0L) * out_step, h1[j]);
-            }
-        }
-        if (flagged) {
-#pragma unroll
-            for (int j = 0; j < L; ++j) flag[j] = flag_ahead(s, time_of<BACK>(s, min(p0 + j, end - 1)), at.n);
-        }
-        if (BACK && time_of<BACK>(s, min(p0 + L, end) - 1) == 0) {   // the tile's last step is the first of the rollout
-#pragma unroll
-            for (int j = 0; j < L; ++j) {
-                if (p0 + j != end - 1) continue;
-#pragma unroll
-                for (int i = 0; i < V; ++i) h1[BACK ? j : 0][i] = 0.0f;
-                if (s.state_in != nullptr) load_n(s.state_in + (long)at.n * s.D + at.d, h1[BACK ? j : 0]);
-            }
-        }
-        if (PART) {
-            float A[V], B[V], low = TINY;
-#pragma unroll
-            for (int i = 0; i < V; ++i) { A[i] = 1.0f; B[i] = 0.0f; }
-#pragma unroll
-            for (int j = 0; j < L; ++j)
-                if (p0 + j < end)
-                    add_step<BACK>(A, B, low, is_cut(s, time_of<BACK>(s, p0 + j), flag[j]), g[j], BACK ? dh[BACK ? j : 0] : x[j]);
-            leave(lds + buffer * half, w, A, B);
-            __syncthreads();   // (the buffers alternate: the next tile's values go where nobody reads any more)
-            through_waves(lds + buffer * half, W, w, carry, mine);
-            buffer ^= 1;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) mine[i] = carry[i];
-        }
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            if (p0 + j >= end) break;
-            const long t = time_of<BACK>(s, p0 + j);
-            const bool cut = is_cut(s, t, flag[j]);
-            float y[V], y2[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float a, rest;
-                gates(g[j][i], a, rest);
-                if (BACK) {
-                    const float d = dh[BACK ? j : 0][i] + mine[i];
-                    y2[i] = rest * d;
-                    y[i] = a * rest * ((cut ? 0.0f : h1[BACK ? j : 0][i]) - x[j][i]) * d;
-                    mine[i] = cut ? 0.0f : a * d;
-                } else {
-                    const float b = rest * x[j][i];
-                    mine[i] = y[i] = cut ? b : fmaf(a, mine[i], b);
-                }
-            }
-            if (at.live) {
-                store_n(dst + t * (BACK ? dgate_step : out_step), y, at.skip);
-                if (BACK) store_n(dst2 + t * dvalue_step, y2, at.skip);
-                if (p0 + j == s.T - 1 && s.last != nullptr) store_n(s.last + (long)at.n * s.D + at.d, mine, at.skip);
-            }
-        }
-        if (!PART) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = mine[i];
-        }
-    }
+    stream_steps(s, at, rows, from, to, k, carry);
 }
 
 // no step at all: the state goes through as it is
@@ -375,48 +517,73 @@ __global__ __launch_bounds__(256) void pass_state_kernel(const float *from, floa
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) to[i] = from ? from[i] : 0.0f;
 }
 
+constexpr int tile_steps(int V) { return V == 4 ? 4 : 8; }   // of a wavefront, for the registers
+
 // How a scan is laid out over the card.
 struct Plan {
-    int V, lanes_per_row, W, segments, segment_steps, groups;
+    int V, lanes_per_row, W, segments, segment_steps, share, groups;
     long lanes;
     size_t bytes;
 };
-constexpr int STEPS = 4;   // L of the kernels with more than one step
-Plan plan_of(const mrl_ctx *ctx, int T, int N, int D) {
-    Plan p;
-    p.V = D >= 4 ? 4 : 1;
-    p.lanes_per_row = (D + p.V - 1) / p.V;
+void channels(Plan &p, int V, int N, int D) {
+    p.V = V = D >= V ? V : D >= 2 ? std::min(V, 2) : 1;
+    p.lanes_per_row = (D + V - 1) / V;
     p.lanes = (long)N * p.lanes_per_row;
     p.groups = (int)((p.lanes + 63) / 64);
+}
+// Eight wavefronts per CU keep the memory busy.  Where one per group of 64 lanes with V = 4 channels gives fewer, workgroups of up to
+// 8 share a group's steps; with fewer groups than CUs lanes have 2 channels, then 1 (and up to 16 wavefronts): the exchange
+// between a tile's wavefronts costs as much whatever a lane holds.  us on 256 CUs, fp32, 1000 steps of width 256, V = 4 / 2 / 1:
+//   N = 16: 90 / 56 / 36   64: 115 / 71 / 55   128: 127 / 83 / 94   256: 153 / 165 / 178
+// Segments read gate and value twice but go through the time side by side.  Tiles / segments, 1000 steps, fp32 and bf16:
+//   N = 1: 34 / 18, 34 / 18   16: 36 / 23   32: 39 / 39, 37 / 25   64: 55 / 72, 46 / 42   128: 83 / 134, 61 / 78
+// (256 steps: N = 1 12 / 18, 32: 13 / 19; backward: 1000 steps, N = 32 66 / 58, 57 / 36, 64 90 / 108, 74 / 64).
+Plan plan_of(const mrl_ctx *ctx, int T, int N, int D, int size) {
+    Plan p = {};
+    const long want = 8L * ctx->n_cus;   // wavefronts
+    constexpr int SHARE = 16;            // steps that a wavefront of a segment has at least
+    channels(p, 4, N, D);
     p.W = 1;
     p.segments = 1;
-    const long want = 8L * ctx->n_cus;   // wavefronts
-    while (p.W < MAX_WAVES && (long)p.groups * p.W < want && (long)p.W * STEPS < T) p.W *= 2;
-    const long tile = (long)p.W * STEPS, tiles = (T + tile - 1) / tile;
-    if (p.W == MAX_WAVES && (long)p.groups * p.W < want && tiles >= 4) {
-        const long most = std::min<long>(tiles / 2, want / ((long)p.groups * p.W));
-        const long per = (tiles + most - 1) / most;
-        p.segments = (int)((tiles + per - 1) / per);
-        p.segment_steps = (int)(per * tile);
+    if (T >= 512 && (long)p.groups * size * 2 < ctx->n_cus) {
+        if ((long)p.groups * T < SHARE * want) channels(p, 2, N, D);
+        const long shares = std::min<long>((T + SHARE - 1) / SHARE, std::max<long>(2 * MAX_WAVES, want / p.groups));
+        p.W = MAX_WAVES;
+        p.share = (int)((T + shares - 1) / shares);
+        p.segment_steps = p.share * p.W;
+        p.segments = (T + p.segment_steps - 1) / p.segment_steps;
+        p.bytes = sizeof(float) * (size_t)p.lanes * p.V * (2 * (size_t)p.segments * (p.W + 1) + 1);
+        return p;
     }
-    if (p.segments == 1) p.segment_steps = T;
-    p.bytes = p.segments > 1 ? sizeof(float) * (size_t)p.lanes * p.V * (2 * (size_t)p.segments + 1) : 0;
+    if (T == 1) return p;
+    for (int V = 2; V >= 1 && p.groups <= ctx->n_cus / 2; --V) channels(p, V, N, D);
+    const int most = MAX_WAVES * (p.V == 1 ? 2 : 1);
+    while (p.W < most && (long)p.groups * p.W < want && (long)p.W * tile_steps(p.V) < T) p.W *= 2;
     return p;
 }
 
 template <class E, int V, bool BACK>
 void launch(const mrl_ctx *ctx, const Scan &s) {
-    if (s.W == 1) {
+    constexpr int L = 4;   // steps whose loads are under way together
+    if (s.segments > 1) {
+        const dim3 grid(s.groups, s.segments), block(64, s.W);
+        const size_t lds = sizeof(float) * s.W * 2 * 64 * V;
+        hipLaunchKernelGGL((scan_coefficients_kernel<E, V, L, BACK>), grid, block, lds, ctx->stream, s);
+        hipLaunchKernelGGL((scan_segments_kernel<E, V, L, BACK>), grid, block, lds, ctx->stream, s);
+    } else if (s.W > 1) {
+        hipLaunchKernelGGL((scan_tiles_kernel<E, V, tile_steps(V), BACK>), dim3(s.groups), dim3(64, s.W), sizeof(float) * 2 * s.W * 2 * 64 * V, ctx->stream, s);
+    } else {
         const int per = s.groups >= 4 * ctx->n_cus ? 4 : 1;
         const dim3 grid((s.groups + per - 1) / per), block(64, per);
-        if (s.T == 1) hipLaunchKernelGGL((scan_kernel<E, V, 1, BACK, false>), grid, block, 0, ctx->stream, s);
-        else hipLaunchKernelGGL((scan_kernel<E, V, STEPS, BACK, false>), grid, block, 0, ctx->stream, s);
-        return;
+        if (s.T == 1) hipLaunchKernelGGL((scan_alone_kernel<E, V, 1, BACK>), grid, block, 0, ctx->stream, s);
+        else hipLaunchKernelGGL((scan_alone_kernel<E, V, L, BACK>), grid, block, 0, ctx->stream, s);
     }
-    const dim3 grid(s.groups, s.segments), block(64, s.W);
-    const size_t half = sizeof(float) * s.W * 2 * 64 * V;
-    if (s.segments > 1) hipLaunchKernelGGL((scan_segments_kernel<E, V, STEPS, BACK>), grid, block, half, ctx->stream, s);
-    hipLaunchKernelGGL((scan_kernel<E, V, STEPS, BACK, true>), grid, block, 2 * half, ctx->stream, s);
+}
+template <class E, bool BACK>
+void launch(const mrl_ctx *ctx, const Scan &s, int V) {
+    if (V == 4) launch<E, 4, BACK>(ctx, s);
+    else if (V == 2) launch<E, 2, BACK>(ctx, s);
+    else launch<E, 1, BACK>(ctx, s);
 }
 
 template <bool BACK>
@@ -429,21 +596,17 @@ int scan(mrl_ctx *ctx, const char *who, int dtype, Scan &s, void *workspace, uin
         MRL_CHECK_LAUNCH();
         return MRL_OK;
     }
-    const Plan p = plan_of(ctx, s.T, s.N, s.D);
+    const Plan p = plan_of(ctx, s.T, s.N, s.D, dtype == MRL_F32 ? 4 : 2);
     MRL_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || workspace != nullptr),
                   "%s: the workspace holds %llu bytes, need %llu", who, (unsigned long long)(workspace ? workspace_bytes : 0),
                   (unsigned long long)p.bytes);
     MRL_CHECK_ARG(p.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", who);
     s.lanes_per_row = p.lanes_per_row; s.lanes = p.lanes; s.groups = p.groups;
-    s.W = p.W; s.segments = p.segments; s.segment_steps = p.segment_steps;
+    s.W = p.W; s.segments = p.segments; s.segment_steps = p.segment_steps; s.share = p.share;
+    s.whole = s.D % p.V == 0;
     s.ws = (float *)workspace;
-    if (dtype == MRL_F32) {
-        if (p.V == 4) launch<float, 4, BACK>(ctx, s);
-        else launch<float, 1, BACK>(ctx, s);
-    } else {
-        if (p.V == 4) launch<bf16_t, 4, BACK>(ctx, s);
-        else launch<bf16_t, 1, BACK>(ctx, s);
-    }
+    if (dtype == MRL_F32) launch<float, BACK>(ctx, s, p.V);
+    else launch<bf16_t, BACK>(ctx, s, p.V);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -466,7 +629,7 @@ int mrl_recurrence_workspace(mrl_ctx *ctx, int T, int N, int D, uint64_t *bytes)
     const int rc = mrl::check_sizes("mrl_recurrence_workspace", ctx, MRL_F32, T, N, D);
     if (rc != MRL_OK) return rc;
     MRL_CHECK_ARG(bytes, "mrl_recurrence_workspace: NULL result");
-    *bytes = T == 0 || N == 0 || D == 0 ? 0 : mrl::plan_of(ctx, T, N, D).bytes;
+    *bytes = T == 0 || N == 0 || D == 0 ? 0 : std::max(mrl::plan_of(ctx, T, N, D, 4).bytes, mrl::plan_of(ctx, T, N, D, 2).bytes);
     return MRL_OK;
 }
 

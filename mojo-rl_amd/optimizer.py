@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .context import _on_device, _ptr
+from .context import _on_device, _ptr, _scratch
 
 
 class Adam:
@@ -23,12 +23,6 @@ class Adam:
         self.t += 1
         _lib.call("mrl_adam_step", ctx.handle, _ptr(params_buf), _ptr(grads_buf), _ptr(state_buf), n,
                   self.t, self.lr, self.beta1, self.beta2, self.eps)
-
-
-def _workspace(ctx, n):
-    """From torch's allocator on the context's stream, so that a captured graph has its own."""
-    with torch.cuda.stream(ctx.stream):
-        return torch.empty(n, dtype=torch.uint8, device=ctx.device)
 
 
 def orthogonalize(ctx, out, x, steps=5, eps=1e-7):
@@ -50,7 +44,7 @@ def orthogonalize(ctx, out, x, steps=5, eps=1e-7):
         return
     size = C.c_uint64(0)
     _lib.call("mrl_orthogonalize_workspace", count, rows, cols, C.byref(size))
-    ws = _workspace(ctx, size.value)
+    ws = _scratch(ctx, size.value)
     _lib.call("mrl_orthogonalize", ctx.handle, _lib.F32 if x.dtype == torch.float32 else _lib.BF16, count, rows, cols, x.data_ptr(),
               out.data_ptr(), steps, eps, ws.data_ptr(), size.value)
 
@@ -92,7 +86,7 @@ class Muon:
             if t.numel() != want or t.dtype != torch.float32:
                 raise _lib.MrlError("Muon.step_gpu: %s must be %d floats, got %d of %s" % (name, want, t.numel(), t.dtype))
             _on_device(ctx, name, t)
-        ws = _workspace(ctx, self._bytes)
+        ws = _scratch(ctx, self._bytes)
         _lib.call("mrl_muon_step", ctx.handle, _ptr(params_buf), _ptr(grads_buf), _ptr(state_buf), n, self._count, self._matrices,
                   self.t + 1, self.lr, self.momentum, int(self.nesterov), self.weight_decay, self.steps, self.eps, self.adam_lr, self.beta1,
                   self.beta2, self.adam_eps, ws.data_ptr() if self._bytes else None, self._bytes)

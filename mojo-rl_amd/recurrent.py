@@ -16,7 +16,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .context import _on_device
+from .context import _on_device, _scratch
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -60,7 +60,7 @@ class GatedRecurrence:
         return gate.shape[0] // steps, _TYPES[gate.dtype]
 
     def _workspace(self, ctx, steps, envs):
-        """(tensor or None, pointer, bytes): from torch's allocator on the context's stream, so that a captured graph has its own."""
+        """(tensor or None, pointer, bytes)"""
         key = (ctx.handle.value, steps, envs)
         n = self._sizes.get(key)
         if n is None:
@@ -69,8 +69,7 @@ class GatedRecurrence:
             n = self._sizes[key] = size.value
         if n == 0:
             return None, None, 0
-        with torch.cuda.stream(ctx.stream):
-            ws = torch.empty(n, dtype=torch.uint8, device=ctx.device)
+        ws = _scratch(ctx, n)
         return ws, ws.data_ptr(), n
 
     def forward_gpu(self, ctx, output, gate, value, steps, state_in=None, state_out=None, dones=None, prev_dones=None):
