@@ -28,39 +28,47 @@ class GatedRecurrence:
         self.width = width
         self._sizes = {}   # (context, steps, envs) -> workspace bytes
 
-    def _rows(self, ctx, name, t, rows, dtype):
-        """(pointer, elements from a row to the next) of a [rows, width] tensor."""
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != self.width:
-            raise _lib.MrlError("%s: a [%d, %d] tensor expected, got %s" % (name, rows, self.width, list(t.shape)))
+    def _rows(self, ctx, name, t, size, dtype):
+        """(pointer, elements from a row to the next) of a tensor of size (rows, width)."""
+        if t.shape == size and t.dtype is dtype and t.device == ctx.device:
+            row, element = t.stride()
+            if element == 1 and row >= size[1]:
+                return t.data_ptr(), row
+        if t.shape != size:
+            raise _lib.MrlError("%s: a [%d, %d] tensor expected, got %s" % (name, *size, list(t.shape)))
         if t.dtype != dtype:
             raise _lib.MrlError("%s: %s expected, got %s" % (name, dtype, t.dtype))
         _on_device(ctx, name, t)
         row, element = t.stride()
-        if self.width > 1 and element != 1:
+        if size[1] > 1 and element != 1 and size[0] > 0:
             raise _lib.MrlError("%s: the elements of a row must be next to each other, got strides %s" % (name, t.stride()))
-        if rows < 2:
-            row = self.width
-        elif row < self.width:
+        if size[0] < 2:
+            row = size[1]
+        elif row < size[1]:
             raise _lib.MrlError("%s: rows overlap, got strides %s" % (name, t.stride()))
         return t.data_ptr(), row
 
     def _flat(self, ctx, name, t, n):
         if t is None:
             return None
-        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
             raise _lib.MrlError("%s: %d contiguous floats expected, got %s of %s" % (name, n, list(t.shape), t.dtype))
-        _on_device(ctx, name, t)
+        if t.device != ctx.device:
+            _on_device(ctx, name, t)
         return t.data_ptr()
 
     def _shape(self, gate, steps):
-        if steps < 1 or gate.dim() != 2 or gate.shape[0] % steps:
+        if steps < 1 or gate.dim() != 2 or gate.size(0) % steps:
             raise _lib.MrlError("gate: [steps * envs, %d] rows of %d steps expected, got %s" % (self.width, steps, list(gate.shape)))
-        if gate.dtype not in _TYPES:
+        kind = _TYPES.get(gate.dtype)
+        if kind is None:
             raise _lib.MrlError("gate: float32 or bfloat16 expected, got %s" % gate.dtype)
-        return gate.shape[0] // steps, _TYPES[gate.dtype]
+        return gate.size(0) // steps, kind
 
     def _workspace(self, ctx, steps, envs):
         """(tensor or None, pointer, bytes)"""
+        if steps == 1:
+            return None, None, 0
         key = (ctx.handle.value, steps, envs)
         n = self._sizes.get(key)
         if n is None:
@@ -76,9 +84,10 @@ class GatedRecurrence:
         """output and state_out (None: not wanted; may be state_in) from gate, value and state_in (None: zeros)."""
         envs, dtype = self._shape(gate, steps)
         rows, states = steps * envs, envs * self.width
-        g, g_ld = self._rows(ctx, "gate", gate, rows, gate.dtype)
-        v, v_ld = self._rows(ctx, "value", value, rows, gate.dtype)
-        o, o_ld = self._rows(ctx, "output", output, rows, gate.dtype)
+        size, kind = (rows, self.width), gate.dtype
+        g, g_ld = self._rows(ctx, "gate", gate, size, kind)
+        v, v_ld = self._rows(ctx, "value", value, size, kind)
+        o, o_ld = self._rows(ctx, "output", output, size, kind)
         flags, before = self._flat(ctx, "dones", dones, rows), self._flat(ctx, "prev_dones", prev_dones, envs)
         s_in, s_out = self._flat(ctx, "state_in", state_in, states), self._flat(ctx, "state_out", state_out, states)
         ws, ws_ptr, ws_bytes = self._workspace(ctx, steps, envs)
@@ -95,12 +104,13 @@ class GatedRecurrence:
         forward_gpu computed, from those of its output and (None: zeros) of state_out."""
         envs, dtype = self._shape(gate, steps)
         rows, states = steps * envs, envs * self.width
-        g, g_ld = self._rows(ctx, "gate", gate, rows, gate.dtype)
-        v, v_ld = self._rows(ctx, "value", value, rows, gate.dtype)
-        o, o_ld = self._rows(ctx, "output", output, rows, gate.dtype)
-        go, go_ld = self._rows(ctx, "grad_output", grad_output, rows, gate.dtype)
-        gg, gg_ld = self._rows(ctx, "grad_gate", grad_gate, rows, gate.dtype)
-        gv, gv_ld = self._rows(ctx, "grad_value", grad_value, rows, gate.dtype)
+        size, kind = (rows, self.width), gate.dtype
+        g, g_ld = self._rows(ctx, "gate", gate, size, kind)
+        v, v_ld = self._rows(ctx, "value", value, size, kind)
+        o, o_ld = self._rows(ctx, "output", output, size, kind)
+        go, go_ld = self._rows(ctx, "grad_output", grad_output, size, kind)
+        gg, gg_ld = self._rows(ctx, "grad_gate", grad_gate, size, kind)
+        gv, gv_ld = self._rows(ctx, "grad_value", grad_value, size, kind)
         flags, before = self._flat(ctx, "dones", dones, rows), self._flat(ctx, "prev_dones", prev_dones, envs)
         s_in = self._flat(ctx, "state_in", state_in, states)
         gs_out, gs_in = self._flat(ctx, "grad_state_out", grad_state_out, states), self._flat(ctx, "grad_state_in", grad_state_in, states)
