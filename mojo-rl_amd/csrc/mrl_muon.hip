@@ -28,8 +28,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float QA = 3.4445f, QB = -4.7750f, QC = 2.0315f;
-constexpr int TILE = 64;
 constexpr int MOST = 16;        // matrices of a launch
+constexpr int LOAD = 32;        // sides of what a workgroup of the second launch takes
 constexpr int CHUNK = 4096;     // elements that a workgroup of the first launch takes at a time
 constexpr int MOST_SUMS = 256;  // partial sums of squares per matrix
 
@@ -50,6 +50,7 @@ struct Mat {
 struct Rest { float *p; const float *g; float2 *state; long n; int begin; };   // parameters that Adam updates
 struct Group {
     int count, rests;
+    int tile;               // sides of the products' tiles; every matrix's sides are padded to it
     int total_sums;
     Mat mat[MOST];
     Rest rest[MOST + 1];
@@ -125,11 +126,11 @@ MRL_DEV f32x4 get_piece(const _Float16 *planes, int blocks, int row, int k) {
 template <int KIND>
 __global__ __launch_bounds__(256) void load_kernel(Group g) {
     __shared__ double part[256];
-    __shared__ float tile[TILE][TILE + 1];
+    __shared__ float tile[LOAD][LOAD + 1];
     int k = 0;
     while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_load) ++k;
     const Mat &m = g.mat[k];
-    const int block = blockIdx.x - m.begin_load, across = m.np / TILE, i0 = block / across * TILE, j0 = block % across * TILE;
+    const int block = blockIdx.x - m.begin_load, across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
     part[threadIdx.x] = (int)threadIdx.x < m.sums ? m.partial[threadIdx.x] : 0.0;
     __syncthreads();
     for (int w = 128; w > 0; w >>= 1) {
@@ -137,8 +138,8 @@ __global__ __launch_bounds__(256) void load_kernel(Group g) {
         __syncthreads();
     }
     const double scale = (double)m.sx / (sqrt(part[0]) + g.eps);
-    for (int e = threadIdx.x; e < TILE * TILE; e += 256) {
-        const int slow = e / TILE, fast = e % TILE;                            // fast runs along the caller's rows
+    for (int e = threadIdx.x; e < LOAD * LOAD; e += 256) {
+        const int slow = e / LOAD, fast = e % LOAD;                            // fast runs along the caller's rows
         const int i = m.tall ? fast : slow, j = m.tall ? slow : fast;
         float x = 0.0f;
         if (i0 + i < m.m && j0 + j < m.n) {
@@ -148,8 +149,8 @@ __global__ __launch_bounds__(256) void load_kernel(Group g) {
         tile[i][j] = x;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < TILE * TILE / 4; e += 256) {
-        const int r = e % TILE, c = e / TILE * 4;
+    for (int e = threadIdx.x; e < LOAD * LOAD / 4; e += 256) {
+        const int r = e % LOAD, c = e / LOAD * 4;
         put_piece(m.x, m.np / 32, i0 + r, j0 + c, f32x4{tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]});
         put_piece(m.xt[0], m.mp / 32, j0 + r, i0 + c, f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]});
     }
@@ -177,37 +178,176 @@ MRL_DEV f32x4 quad_transpose(f32x4 v) {
 
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
 
-// One product, a tile of 64 x 64 per workgroup, 32 x 32 per wavefront.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric,
-// so only tiles on and above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
-template <int STAGE, int KIND>
-__global__ __launch_bounds__(256) void product_kernel(Group g, int from, int last) {
+// Which tile of which matrix a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that
+// share operands, so that its L2 is read more often than what is behind it.
+template <int STAGE>
+MRL_DEV const Mat &find_tile(const Group &g, int total, int &bi, int &bj) {
+    const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
+    const int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
     int k = 0;
     if (STAGE == UPDATE) {
-        while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_update) ++k;
-    } else {
-        while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_sym) ++k;
+        while (k + 1 < g.count && id >= g.mat[k + 1].begin_update) ++k;
+        const Mat &m = g.mat[k];
+        const int block = id - m.begin_update, rows = m.mp / g.tile, panel = block / (4 * rows), in = block - panel * 4 * rows;
+        const int width = min(4, m.np / g.tile - 4 * panel);   // panels of four columns, row by row
+        bi = in / width;
+        bj = 4 * panel + in - bi * width;
+        return m;
     }
+    while (k + 1 < g.count && id >= g.mat[k + 1].begin_sym) ++k;
     const Mat &m = g.mat[k];
-    int bi, bj;
+    int block = id - m.begin_sym;
+    bj = (int)((sqrtf(8.0f * block + 1.0f) - 1.0f) * 0.5f);   // column bj has tiles 0 .. bj
+    while (bj * (bj + 1) / 2 > block) --bj;
+    while ((bj + 1) * (bj + 2) / 2 <= block) ++bj;
+    bi = block - bj * (bj + 1) / 2;
+    return m;
+}
+
+// What becomes of four sums: rows i .. i + 3 of column j, of a lane with column j % 16.
+template <int STAGE, int KIND>
+MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diagonal, int i, int j, f32x4 v) {
+    const int it = i + (j & 3), jt = j & ~3;   // transposed: row it, columns jt .. jt + 3
     if (STAGE == UPDATE) {
-        const int block = blockIdx.x - m.begin_update;
-        bi = block % (m.mp / TILE);
-        bj = block / (m.mp / TILE);
+        const f32x4 x = get_piece(m.xt[from], m.mp / 32, j, i);
+        v = QA * x + v * (1.0f / m.sa);
+        if (!last) {
+            put_piece(m.xt[from ^ 1], m.mp / 32, j, i, v);
+            put_piece(m.x, m.np / 32, it, jt, quad_transpose(v));
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i + e >= m.m || j >= m.n) continue;
+            const size_t at = m.tall ? (size_t)j * m.m + (i + e) : (size_t)(i + e) * m.n + j;
+            const float o = v[e] * (1.0f / m.sx);
+            if (KIND == BF16) {
+                ((unsigned short *)m.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)o);
+            } else if (KIND == F32) {
+                ((float *)m.out)[at] = o;
+            } else {
+                float *w = (float *)m.out + at;
+                *w = fmaf(-m.factor, o, *w * g.keep);
+            }
+        }
     } else {
-        int block = blockIdx.x - m.begin_sym;
-        bj = 0;
-        while (block > bj) block -= ++bj;   // column bj has tiles 0 .. bj
-        bi = block;
+        _Float16 *to = STAGE == GRAM ? m.a : m.b;
+        if (STAGE == GRAM) v = v * (m.sa / (m.sx * m.sx));
+        else v = QB * get_piece(m.a, m.mp / 32, j, i) + v * (QC / m.sa);
+        put_piece(to, m.mp / 32, j, i, v);
+        if (!diagonal) put_piece(to, m.mp / 32, it, jt, quad_transpose(v));
     }
-    const _Float16 *P = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b;
-    const _Float16 *Q = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[from];
-    const int blocks = (STAGE == GRAM ? m.np : m.mp) / 32;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = bi * TILE + (wave >> 1) * 32, j0 = bj * TILE + (wave & 1) * 32;
+}
+
+template <int F>
+MRL_DEV void multiply(const f16x8 (&ph)[F], const f16x8 (&pl)[F], const f16x8 (&qh)[F], const f16x8 (&ql)[F], f32x4 (&acc)[F][F]) {
+#pragma unroll
+    for (int fi = 0; fi < F; ++fi)
+#pragma unroll
+        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[fi], qh[fj], acc[fi][fj], 0, 0, 0);
+#pragma unroll
+    for (int fi = 0; fi < F; ++fi)
+#pragma unroll
+        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], ql[fj], acc[fi][fj], 0, 0, 0);
+#pragma unroll
+    for (int fi = 0; fi < F; ++fi)
+#pragma unroll
+        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], qh[fj], acc[fi][fj], 0, 0, 0);
+}
+
+template <int STAGE>
+MRL_DEV void operands(const Mat &m, int from, const _Float16 *&P, const _Float16 *&Q, int &blocks) {
+    P = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b;
+    Q = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[from];
+    blocks = (STAGE == GRAM ? m.np : m.mp) / 32;
+}
+
+// One product, a tile of 32 F x 32 F per workgroup.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric, so only tiles on and
+// above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
+// Four wavefronts share the tile, 16 F x 16 F each, and KG such sets share the contracted index, 32 of it each at a time, so that
+// a SIMD has KG wavefronts to take turns.  Operands go from memory to LDS past the registers, the next 32 KG while these are
+// multiplied.  In the end the sets exchange sums through LDS and each finishes a part of the tile.
+template <int STAGE, int KIND, int F, int KG>
+__global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(F == 4 ? 2 : 4))) void product_kernel(Group g, int total, int from, int last) {
+    constexpr int SIDE = 2 * F;                        // fragments of 16 along a side
+    constexpr int OPERAND = SIDE * KG * 1024;          // halves of one operand of a stage: [fragment][set][hi, lo][512]
+    extern __shared__ _Float16 lds[];
+    int bi, bj;
+    const Mat &m = find_tile<STAGE>(g, total, bi, bj);
+    const _Float16 *P, *Q;
+    int blocks;
+    operands<STAGE>(m, from, P, Q, blocks);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave >> 2, part = wave & 3;
+    const int stages = blocks / KG;   // (whole: the sides are padded to the tile)
+    // A stage of a fragment, KG times hi and lo, is one run of memory and of LDS; a wavefront brings in EACH fragments of an operand.
+    constexpr int EACH = SIDE / (2 * KG);
+    const int operand = wave / (2 * KG), first = wave % (2 * KG) * EACH;
+    const _Float16 *src = (operand ? Q + (size_t)(bj * SIDE + first) * blocks * 1024 : P + (size_t)(bi * SIDE + first) * blocks * 1024) + lane * 8;
+    _Float16 *to = lds + operand * OPERAND + first * KG * 1024;
+    auto stage_in = [&](int stage) {
+#pragma unroll
+        for (int e = 0; e < EACH * 2 * KG; ++e)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)(src + ((size_t)(e / (2 * KG)) * blocks + (size_t)stage * KG) * 1024 + e % (2 * KG) * 512),
+                (__attribute__((address_space(3))) void *)(to + (stage & 1) * 2 * OPERAND + e * 512), 16, 0, 0);
+    };
+    f32x4 acc[F][F] = {};
+    stage_in(0);
+    for (int s = 0; s < stages; ++s) {
+        __syncthreads();   // this stage is in LDS, and nobody reads the buffer of the next one any more
+        if (s + 1 < stages) stage_in(s + 1);
+        const _Float16 *p = lds + (s & 1) * 2 * OPERAND + ((part >> 1) * F * KG + set) * 1024 + lane * 8;
+        const _Float16 *q = lds + (s & 1) * 2 * OPERAND + OPERAND + ((part & 1) * F * KG + set) * 1024 + lane * 8;
+        f16x8 ph[F], pl[F], qh[F], ql[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            pl[f] = *reinterpret_cast<const f16x8 *>(p + f * KG * 1024 + 512);
+            qh[f] = *reinterpret_cast<const f16x8 *>(q + f * KG * 1024);
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            ph[f] = *reinterpret_cast<const f16x8 *>(p + f * KG * 1024);
+            ql[f] = *reinterpret_cast<const f16x8 *>(q + f * KG * 1024 + 512);
+        }
+        multiply<F>(ph, pl, qh, ql, acc);
+    }
+    const int i0 = (bi * SIDE + (part >> 1) * F) * 16 + 4 * (lane >> 4), j0 = (bj * SIDE + (part & 1) * F) * 16 + (lane & 15);
+    // set s finishes the fragments whose number is s modulo KG
+    {
+        f32x4 *sums = reinterpret_cast<f32x4 *>(lds);   // [set that finishes][set that has them][part][fragment / KG][lane]
+        constexpr int SHARE = F * F / KG;
+        __syncthreads();
+#pragma unroll
+        for (int f = 0; f < F * F; ++f)
+            if (f % KG != set) sums[(((f % KG) * KG + set) * 4 + part) * SHARE * 64 + (f / KG) * 64 + lane] = acc[f / F][f % F];
+        __syncthreads();
+#pragma unroll
+        for (int f = 0; f < F * F; ++f) {
+            if (f % KG != set) continue;
+            f32x4 v = acc[f / F][f % F];
+#pragma unroll
+            for (int other = 1; other < KG; ++other)
+                v += sums[((set * KG + (set + other) % KG) * 4 + part) * SHARE * 64 + (f / KG) * 64 + lane];
+            finish<STAGE, KIND>(g, m, from, last, bi == bj, i0 + 16 * (f / F), j0 + 16 * (f % F), v);
+        }
+    }
+}
+
+// The same for small matrices, where a launch is shorter than the way of a stage through memory and LDS and back: a tile of 32 x 32
+// per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.
+template <int STAGE, int KIND>
+__global__ __launch_bounds__(256) void small_product_kernel(Group g, int total, int from, int last) {
+    __shared__ f32x4 sums[4][4][64];   // [fragment][wavefront][lane]
+    int bi, bj;
+    const Mat &m = find_tile<STAGE>(g, total, bi, bj);
+    const _Float16 *P, *Q;
+    int blocks;
+    operands<STAGE>(m, from, P, Q, blocks);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const _Float16 *p = P + (size_t)bi * 2 * blocks * 1024 + lane * 8, *q = Q + (size_t)bj * 2 * blocks * 1024 + lane * 8;
     f32x4 acc[2][2] = {};
-    const _Float16 *p = P + (size_t)(i0 >> 4) * blocks * 1024 + lane * 8, *q = Q + (size_t)(j0 >> 4) * blocks * 1024 + lane * 8;
 #pragma unroll 2
-    for (int kb = 0; kb < blocks; ++kb) {
+    for (int kb = wave; kb < blocks; kb += 4) {
         f16x8 ph[2], pl[2], qh[2], ql[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
@@ -217,73 +357,59 @@ __global__ __launch_bounds__(256) void product_kernel(Group g, int from, int las
             qh[f] = *reinterpret_cast<const f16x8 *>(qf);
             ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
         }
-#pragma unroll
-        for (int fi = 0; fi < 2; ++fi)
-#pragma unroll
-            for (int fj = 0; fj < 2; ++fj) {
-                acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[fi], qh[fj], acc[fi][fj], 0, 0, 0);
-                acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], ql[fj], acc[fi][fj], 0, 0, 0);
-                acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], qh[fj], acc[fi][fj], 0, 0, 0);
-            }
+        multiply<2>(ph, pl, qh, ql, acc);
     }
-    const int quarter = lane >> 4, column = lane & 15;
 #pragma unroll
-    for (int fi = 0; fi < 2; ++fi)
-#pragma unroll
-        for (int fj = 0; fj < 2; ++fj) {
-            // this lane: rows i .. i + 3 of column j; transposed: row i + column % 4, columns from j - column % 4 on
-            const int i = i0 + 16 * fi + 4 * quarter, j = j0 + 16 * fj + column;
-            const int it = i + (column & 3), jt = j - (column & 3);
-            f32x4 v = acc[fi][fj];
-            if (STAGE == UPDATE) {
-                const f32x4 x = get_piece(m.xt[from], m.mp / 32, j, i);
-                v = QA * x + v * (1.0f / m.sa);
-                if (!last) {
-                    put_piece(m.xt[from ^ 1], m.mp / 32, j, i, v);
-                    put_piece(m.x, m.np / 32, it, jt, quad_transpose(v));
-                    continue;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (i + e >= m.m || j >= m.n) continue;
-                    const size_t at = m.tall ? (size_t)j * m.m + (i + e) : (size_t)(i + e) * m.n + j;
-                    const float o = v[e] * (1.0f / m.sx);
-                    if (KIND == BF16) {
-                        ((unsigned short *)m.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)o);
-                    } else if (KIND == F32) {
-                        ((float *)m.out)[at] = o;
-                    } else {
-                        float *w = (float *)m.out + at;
-                        *w = fmaf(-m.factor, o, *w * g.keep);
-                    }
-                }
-            } else {
-                _Float16 *to = STAGE == GRAM ? m.a : m.b;
-                if (STAGE == GRAM) v = v * (m.sa / (m.sx * m.sx));
-                else v = QB * get_piece(m.a, m.mp / 32, j, i) + v * (QC / m.sa);
-                put_piece(to, m.mp / 32, j, i, v);
-                if (bi != bj) put_piece(to, m.mp / 32, it, jt, quad_transpose(v));
-            }
-        }
+    for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
+    __syncthreads();
+    const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
+    finish<STAGE, KIND>(g, m, from, last, bi == bj, (bi * 2 + (wave >> 1)) * 16 + 4 * (lane >> 4), (bj * 2 + (wave & 1)) * 16 + (lane & 15), v);
 }
 
-inline int pad(int x) { return (x + TILE - 1) / TILE * TILE; }
+inline int pad(int x, int tile) { return (x + tile - 1) / tile * tile; }
 
 // bytes of one matrix's planes and sums
-size_t matrix_bytes(int rows, int cols) {
-    const size_t mp = pad(std::min(rows, cols)), np = pad(std::max(rows, cols));
+size_t matrix_bytes(int rows, int cols, int tile) {
+    const size_t mp = pad(std::min(rows, cols), tile), np = pad(std::max(rows, cols), tile);
     return sizeof(_Float16) * (6 * mp * np + 4 * mp * mp) + sizeof(double) * MOST_SUMS;
 }
 
+// The tiles of a launch: the largest of which the products have enough to go round.
+struct Sides { int rows, cols; };
+template <class S>
+int tile_of(const S *matrices, int count) {
+    for (int tile : {128, 64}) {
+        long tiles = 0;
+        for (int k = 0; k < count; ++k) tiles += (long)(pad(matrices[k].rows, tile) / tile) * (pad(matrices[k].cols, tile) / tile);
+        if (tiles >= (tile == 128 ? 128 : 64)) return tile;
+    }
+    return 32;
+}
+template <class S>
+size_t group_bytes(const S *matrices, int count) {
+    const int tile = tile_of(matrices, count);
+    size_t bytes = 0;
+    for (int k = 0; k < count; ++k) bytes += matrix_bytes(matrices[k].rows, matrices[k].cols, tile);
+    return bytes;
+}
+
+// of `count` alike, in launches of MOST; the last launch's tiles may be smaller, and so their padding
+size_t batch_bytes(int count, int rows, int cols) {
+    Sides sides[MOST];
+    std::fill(sides, sides + MOST, Sides{rows, cols});
+    const size_t whole = count >= MOST ? group_bytes(sides, MOST) : 0;
+    return std::max(whole, count % MOST ? group_bytes(sides, count % MOST) : (size_t)0);
+}
+
 // sides, scales and a share of the workspace
-void set_up(Mat &m, int rows, int cols, char *&ws) {
+void set_up(Mat &m, int rows, int cols, int tile, char *&ws) {
     m.rows = rows;
     m.cols = cols;
     m.tall = rows > cols;
     m.m = std::min(rows, cols);
     m.n = std::max(rows, cols);
-    m.mp = pad(m.m);
-    m.np = pad(m.n);
+    m.mp = pad(m.m, tile);
+    m.np = pad(m.n, tile);
     m.sums = (int)std::min<long>(MOST_SUMS, ((long)rows * cols + CHUNK - 1) / CHUNK);
     m.sx = (float)std::ldexp(1.0, std::min(14, (int)std::lround(0.5 * std::log2((double)m.m * m.n))));
     m.sa = (float)std::ldexp(1.0, std::min(13, (int)std::lround(std::log2((double)m.m))));
@@ -301,14 +427,24 @@ void set_up(Mat &m, int rows, int cols, char *&ws) {
     m.b = planes((size_t)m.mp * m.mp);
 }
 
+template <int STAGE, int KIND>
+void product(const mrl_ctx *ctx, const Group &g, int total, int from, int last) {
+    auto launch = [&](auto kernel, int threads, size_t lds) {
+        hipLaunchKernelGGL(kernel, dim3(total), dim3(threads), lds, ctx->stream, g, total, from, last);
+    };
+    if (g.tile == 128) launch(product_kernel<STAGE, KIND, 4, 2>, 512, 2 * 2 * 8 * 2 * 2048);
+    else if (g.tile == 64) launch(product_kernel<STAGE, KIND, 2, 2>, 512, 2 * 2 * 4 * 2 * 2048);
+    else launch(small_product_kernel<STAGE, KIND>, 256, 0);
+}
+
 template <int KIND>
 void run(const mrl_ctx *ctx, Group &g, int steps) {
     int sums = 0, load = 0, sym = 0, update = 0;
     for (int k = 0; k < g.count; ++k) {
         Mat &m = g.mat[k];
-        const int a = m.mp / TILE, b = m.np / TILE;
+        const int a = m.mp / g.tile, b = m.np / g.tile;
         m.begin_sums = sums; sums += m.sums;
-        m.begin_load = load; load += a * b;
+        m.begin_load = load; load += (m.mp / LOAD) * (m.np / LOAD);
         m.begin_sym = sym; sym += a * (a + 1) / 2;
         m.begin_update = update; update += a * b;
     }
@@ -322,9 +458,9 @@ void run(const mrl_ctx *ctx, Group &g, int steps) {
     if (g.count == 0) return;
     hipLaunchKernelGGL(load_kernel<KIND>, dim3(load), dim3(256), 0, ctx->stream, g);
     for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL((product_kernel<GRAM, KIND>), dim3(sym), dim3(256), 0, ctx->stream, g, s & 1, 0);
-        hipLaunchKernelGGL((product_kernel<SQUARE, KIND>), dim3(sym), dim3(256), 0, ctx->stream, g, s & 1, 0);
-        hipLaunchKernelGGL((product_kernel<UPDATE, KIND>), dim3(update), dim3(256), 0, ctx->stream, g, s & 1, s == steps - 1);
+        product<GRAM, KIND>(ctx, g, sym, s & 1, 0);
+        product<SQUARE, KIND>(ctx, g, sym, s & 1, 0);
+        product<UPDATE, KIND>(ctx, g, update, s & 1, s == steps - 1);
     }
 }
 
@@ -369,7 +505,7 @@ int mrl_orthogonalize_workspace(int count, int rows, int cols, uint64_t *bytes) 
     MRL_CHECK_ARG(bytes && count >= 0, "%s: bad arguments", who);
     const int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK) return rc;
-    *bytes = mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST);
+    *bytes = mrl::batch_bytes(count, rows, cols);
     return MRL_OK;
 }
 
@@ -383,7 +519,7 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK || count == 0) return rc;
     MRL_CHECK_ARG(in && out, "%s: NULL buffer", who);
-    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST));
+    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::batch_bytes(count, rows, cols));
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
     const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
@@ -392,8 +528,11 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
         g.eps = eps;
         g.count = std::min(mrl::MOST, count - done);
         char *ws = (char *)workspace;
+        mrl::Sides sides[mrl::MOST];
+        std::fill(sides, sides + mrl::MOST, mrl::Sides{rows, cols});
+        g.tile = mrl::tile_of(sides, g.count);
         for (int k = 0; k < g.count; ++k) {
-            mrl::set_up(g.mat[k], rows, cols, ws);
+            mrl::set_up(g.mat[k], rows, cols, g.tile, ws);
             g.mat[k].in = (const char *)in + (done + k) * one;
             g.mat[k].out = (char *)out + (done + k) * one;
         }
@@ -411,9 +550,7 @@ int mrl_muon_workspace(int n_matrices, const mrl_matrix *matrices, uint64_t *byt
     if (rc != MRL_OK) return rc;
     *bytes = 0;
     for (int done = 0; done < n_matrices; done += mrl::MOST) {
-        uint64_t group = 0;
-        for (int k = done; k < std::min(n_matrices, done + mrl::MOST); ++k) group += mrl::matrix_bytes(matrices[k].rows, matrices[k].cols);
-        *bytes = std::max(*bytes, group);
+        *bytes = std::max<uint64_t>(*bytes, mrl::group_bytes(matrices + done, std::min(mrl::MOST, n_matrices - done)));
     }
     return MRL_OK;
 }
@@ -447,6 +584,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         g.adam_eps = (float)adam_eps;
         g.bc1 = (float)(1.0 - pow(beta1, (double)t)); g.bc2 = (float)(1.0 - pow(beta2, (double)t));
         g.count = std::min(mrl::MOST, n_matrices - done);
+        g.tile = mrl::tile_of(matrices + done, g.count);
         char *ws = (char *)workspace;
         auto rest = [&](int64_t to) {
             if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at), 0};
@@ -455,7 +593,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
             const mrl_matrix &x = matrices[done + k];
             mrl::Mat &m = g.mat[k];
             rest(x.offset);
-            mrl::set_up(m, x.rows, x.cols, ws);
+            mrl::set_up(m, x.rows, x.cols, g.tile, ws);
             m.in = grads + x.offset;
             m.out = params + x.offset;
             m.momentum = state + 2 * x.offset;
