@@ -15,7 +15,7 @@
 // symmetric, X is kept both ways), so every operand is read the same way.  A plane pair holds, for 16 rows and 32 of the
 // contracted index, the 64 lanes' operands of v_mfma_f32_16x16x32_f16 in lane order, 1 KiB of hi and 1 KiB of lo next to
 // each other: loads are whole and in order.  Element (row r, index k): lane 16 ((k % 32) / 8) + r % 16, k % 8.
-// The sides are padded with zeros to whole tiles, which the products keep zero.
+// The sides are padded to multiples of 64 with zeros, which the products keep zero.
 #include <cmath>
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
@@ -31,7 +31,7 @@ constexpr float QA = 3.4445f, QB = -4.7750f, QC = 2.0315f;
 constexpr int MOST = 16;        // matrices of a launch
 constexpr int LOAD = 32;        // sides of what a workgroup of the second launch takes
 constexpr int CHUNK = 4096;     // elements that a workgroup of the first launch takes at a time
-constexpr int MOST_SUMS = 256;  // partial sums of squares per matrix
+constexpr int MOST_SUMS = 1024;  // partial sums of squares per matrix
 
 struct bf16_t { unsigned short bits; };
 
@@ -42,7 +42,8 @@ struct Mat {
     int rows, cols, m, n, mp, np;   // the caller's sides; the shorter and the longer one, and both padded
     int tall;                       // rows > cols: X is the transpose
     int sums, begin_sums, begin_load, begin_sym, begin_update;   // workgroups of each launch
-    float sx, sa;                   // what X and what A, B are stored times
+    float sx;                       // what X is stored times; A and B: sa
+    float gram, square, update, result;   // sums to A, A A to B, B X to X, X to the caller: sa / sx^2, c / sa, 1 / sa, 1 / sx
     float factor;                   // of the update
     _Float16 *x, *xt[2], *a, *b;
     double *partial;
@@ -50,7 +51,7 @@ struct Mat {
 struct Rest { float *p; const float *g; float2 *state; long n; int begin; };   // parameters that Adam updates
 struct Group {
     int count, rests;
-    int tile;               // sides of the products' tiles; every matrix's sides are padded to it
+    int sym_tile, update_tile;   // sides of the products' tiles
     int total_sums;
     Mat mat[MOST];
     Rest rest[MOST + 1];
@@ -105,22 +106,27 @@ __global__ __launch_bounds__(256) void sums_kernel(Group g) {
     if (threadIdx.x == 0) m.partial[block] = part[0];
 }
 
-// hi and lo pieces of four neighbours along the contracted index k (a multiple of 4) of row `row`
-MRL_DEV size_t piece_at(int blocks, int row, int k) {
-    return ((size_t)(row >> 4) * blocks + (k >> 5)) * 1024 + (16 * ((k & 31) >> 3) + (row & 15)) * 8 + (k & 7);
-}
-MRL_DEV void put_piece(_Float16 *planes, int blocks, int row, int k, const f32x4 x) {
-    const f16x4 hi = __builtin_convertvector(x, f16x4);
-    const f16x4 lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x4), f16x4);
-    _Float16 *p = planes + piece_at(blocks, row, k);
-    *reinterpret_cast<f16x4 *>(p) = hi;
-    *reinterpret_cast<f16x4 *>(p + 512) = lo;
-}
-MRL_DEV f32x4 get_piece(const _Float16 *planes, int blocks, int row, int k) {
-    const _Float16 *p = planes + piece_at(blocks, row, k);
-    return __builtin_convertvector(*reinterpret_cast<const f16x4 *>(p), f32x4) +
-           __builtin_convertvector(*reinterpret_cast<const f16x4 *>(p + 512), f32x4);
-}
+// Four neighbours along the contracted index (k a multiple of 4) of a row, in pieces
+struct Piece {
+    f16x4 hi, lo;
+    Piece() = default;
+    MRL_DEV explicit Piece(const f32x4 x) {
+        hi = __builtin_convertvector(x, f16x4);
+        lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x4), f16x4);
+    }
+    MRL_DEV f32x4 value() const { return __builtin_convertvector(hi, f32x4) + __builtin_convertvector(lo, f32x4); }
+    MRL_DEV void load(const _Float16 *p) {
+        hi = *reinterpret_cast<const f16x4 *>(p);
+        lo = *reinterpret_cast<const f16x4 *>(p + 512);
+    }
+    MRL_DEV void store(_Float16 *p) const {
+        *reinterpret_cast<f16x4 *>(p) = hi;
+        *reinterpret_cast<f16x4 *>(p + 512) = lo;
+    }
+};
+// where it is: of the 16 x 16 that start at (row, k), multiples of 16, and in them that of row r (below 16) and k = 4 quarter
+MRL_DEV size_t square_at(int rows, int row, int k) { return ((size_t)(k >> 5) * (rows >> 4) + (row >> 4)) * 1024 + (k & 16) * 16; }
+MRL_DEV int piece_in(int r, int quarter) { return (quarter >> 1) * 128 + r * 8 + (quarter & 1) * 4; }
 
 // X and its transpose in pieces, a tile per workgroup, through LDS: read along the caller's rows, written along both sides.
 template <int KIND>
@@ -131,7 +137,9 @@ __global__ __launch_bounds__(256) void load_kernel(Group g) {
     while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_load) ++k;
     const Mat &m = g.mat[k];
     const int block = blockIdx.x - m.begin_load, across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
-    part[threadIdx.x] = (int)threadIdx.x < m.sums ? m.partial[threadIdx.x] : 0.0;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < m.sums; i += 256) sum += m.partial[i];
+    part[threadIdx.x] = sum;
     __syncthreads();
     for (int w = 128; w > 0; w >>= 1) {
         if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
@@ -151,36 +159,32 @@ __global__ __launch_bounds__(256) void load_kernel(Group g) {
     __syncthreads();
     for (int e = threadIdx.x; e < LOAD * LOAD / 4; e += 256) {
         const int r = e % LOAD, c = e / LOAD * 4;
-        put_piece(m.x, m.np / 32, i0 + r, j0 + c, f32x4{tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]});
-        put_piece(m.xt[0], m.mp / 32, j0 + r, i0 + c, f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]});
+        const int in = (c & 16) * 16 + piece_in(r & 15, (c & 15) >> 2);
+        Piece(f32x4{tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]}).store(m.x + square_at(m.mp, i0 + r, j0) + in);
+        Piece(f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]}).store(m.xt[0] + square_at(m.np, j0 + r, i0) + in);
     }
 }
 
-// 4 x 4 values of four neighbouring lanes, transposed: v[c] of lane s becomes v[s] of lane c.
-MRL_DEV f32x4 quad_transpose(f32x4 v) {
+// 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
+// lanes away, then halves one lane away.
+MRL_DEV f16x4 quad_transpose(f16x4 v) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 d = __builtin_bit_cast(u32x2, v);
     const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-    auto swap1 = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xB1, 0xF, 0xF, true)); };
-    auto swap2 = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4E, 0xF, 0xF, true)); };
+    const unsigned away = __builtin_amdgcn_mov_dpp(high ? d[0] : d[1], 0x4E, 0xF, 0xF, true);
+    if (high) d[0] = away;
+    else d[1] = away;
+    const unsigned pick = odd ? 0x03020706u : 0x05040100u;   // bytes: 0 .. 3 of the own word, 4 .. 7 of the neighbour's
 #pragma unroll
-    for (int p = 0; p < 4; p += 2) {
-        const float other = swap1(odd ? v[p] : v[p + 1]);
-        v[p] = odd ? other : v[p];
-        v[p + 1] = odd ? v[p + 1] : other;
-    }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        const float other = swap2(high ? v[p] : v[p + 2]);
-        v[p] = high ? other : v[p];
-        v[p + 2] = high ? v[p + 2] : other;
-    }
-    return v;
+    for (int i = 0; i < 2; ++i) d[i] = __builtin_amdgcn_perm(__builtin_amdgcn_mov_dpp(d[i], 0xB1, 0xF, 0xF, true), d[i], pick);
+    return __builtin_bit_cast(f16x4, d);
 }
 
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
 
 // Which tile of which matrix a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that
 // share operands, so that its L2 is read more often than what is behind it.
-template <int STAGE>
+template <int STAGE, int TILE>
 MRL_DEV const Mat &find_tile(const Group &g, int total, int &bi, int &bj) {
     const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
     const int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
@@ -188,8 +192,8 @@ MRL_DEV const Mat &find_tile(const Group &g, int total, int &bi, int &bj) {
     if (STAGE == UPDATE) {
         while (k + 1 < g.count && id >= g.mat[k + 1].begin_update) ++k;
         const Mat &m = g.mat[k];
-        const int block = id - m.begin_update, rows = m.mp / g.tile, panel = block / (4 * rows), in = block - panel * 4 * rows;
-        const int width = min(4, m.np / g.tile - 4 * panel);   // panels of four columns, row by row
+        const int block = id - m.begin_update, rows = (m.mp + TILE - 1) / TILE, panel = block / (4 * rows), in = block - panel * 4 * rows;
+        const int width = min(4, (m.np + TILE - 1) / TILE - 4 * panel);   // panels of four columns, row by row
         bi = in / width;
         bj = 4 * panel + in - bi * width;
         return m;
@@ -204,23 +208,41 @@ MRL_DEV const Mat &find_tile(const Group &g, int total, int &bi, int &bj) {
     return m;
 }
 
-// What becomes of four sums: rows i .. i + 3 of column j, of a lane with column j % 16.
+// Fragments of 16 x 16 sums: a lane has rows i .. i + 3, i = 4 (lane / 16), of column j = lane % 16.  `fi`, `fj`: of the fragment.
+template <int STAGE>
+MRL_DEV bool inside(const Mat &m, int fi, int fj) { return fi < m.mp && fj < (STAGE == UPDATE ? m.np : m.mp); }
+// What the sums are added to, X or A there: asked for early, all at once.
+template <int STAGE>
+MRL_DEV void ask(const Mat &m, int from, int fi, int fj, Piece &piece) {
+    const int lane = threadIdx.x & 63;
+    if (STAGE != GRAM && inside<STAGE>(m, fi, fj)) piece.load((STAGE == UPDATE ? m.xt[from] : m.a) + square_at(STAGE == UPDATE ? m.np : m.mp, fj, fi) + piece_in(lane & 15, lane >> 4));
+}
+// A square's sums in pieces, as columns (row j, k = i) and as rows (row i, k = j)
+MRL_DEV void store_both(_Float16 *columns, int column_rows, _Float16 *rows, int row_rows, int fi, int fj, const f32x4 v) {
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, column = lane & 15;
+    Piece piece(v);
+    piece.store(columns + square_at(column_rows, fj, fi) + piece_in(column, quarter));
+    if (rows == nullptr) return;
+    piece.hi = quad_transpose(piece.hi);
+    piece.lo = quad_transpose(piece.lo);
+    piece.store(rows + square_at(row_rows, fi, fj) + piece_in(4 * quarter + (column & 3), column >> 2));
+}
+// What becomes of the sums.
 template <int STAGE, int KIND>
-MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diagonal, int i, int j, f32x4 v) {
-    const int it = i + (j & 3), jt = j & ~3;   // transposed: row it, columns jt .. jt + 3
+MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diagonal, int fi, int fj, f32x4 v, const Piece &piece) {
+    if (!inside<STAGE>(m, fi, fj)) return;
     if (STAGE == UPDATE) {
-        const f32x4 x = get_piece(m.xt[from], m.mp / 32, j, i);
-        v = QA * x + v * (1.0f / m.sa);
+        v = QA * piece.value() + v * m.update;
         if (!last) {
-            put_piece(m.xt[from ^ 1], m.mp / 32, j, i, v);
-            put_piece(m.x, m.np / 32, it, jt, quad_transpose(v));
+            store_both(m.xt[from ^ 1], m.np, m.x, m.mp, fi, fj, v);
             return;
         }
+        const int lane = threadIdx.x & 63, i = fi + 4 * (lane >> 4), j = fj + (lane & 15);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (i + e >= m.m || j >= m.n) continue;
             const size_t at = m.tall ? (size_t)j * m.m + (i + e) : (size_t)(i + e) * m.n + j;
-            const float o = v[e] * (1.0f / m.sx);
+            const float o = v[e] * m.result;
             if (KIND == BF16) {
                 ((unsigned short *)m.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)o);
             } else if (KIND == F32) {
@@ -232,27 +254,18 @@ MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diago
         }
     } else {
         _Float16 *to = STAGE == GRAM ? m.a : m.b;
-        if (STAGE == GRAM) v = v * (m.sa / (m.sx * m.sx));
-        else v = QB * get_piece(m.a, m.mp / 32, j, i) + v * (QC / m.sa);
-        put_piece(to, m.mp / 32, j, i, v);
-        if (!diagonal) put_piece(to, m.mp / 32, it, jt, quad_transpose(v));
+        if (STAGE == GRAM) v = v * m.gram;
+        else v = QB * piece.value() + v * m.square;
+        store_both(to, m.mp, diagonal ? nullptr : to, m.mp, fi, fj, v);
     }
 }
 
 template <int F>
-MRL_DEV void multiply(const f16x8 (&ph)[F], const f16x8 (&pl)[F], const f16x8 (&qh)[F], const f16x8 (&ql)[F], f32x4 (&acc)[F][F]) {
+MRL_DEV void multiply(const f16x8 (&p)[F], const f16x8 (&q)[F], f32x4 (&acc)[F][F]) {
 #pragma unroll
     for (int fi = 0; fi < F; ++fi)
 #pragma unroll
-        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[fi], qh[fj], acc[fi][fj], 0, 0, 0);
-#pragma unroll
-    for (int fi = 0; fi < F; ++fi)
-#pragma unroll
-        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], ql[fj], acc[fi][fj], 0, 0, 0);
-#pragma unroll
-    for (int fi = 0; fi < F; ++fi)
-#pragma unroll
-        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[fi], qh[fj], acc[fi][fj], 0, 0, 0);
+        for (int fj = 0; fj < F; ++fj) acc[fi][fj] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[fi], q[fj], acc[fi][fj], 0, 0, 0);
 }
 
 template <int STAGE>
@@ -262,75 +275,140 @@ MRL_DEV void operands(const Mat &m, int from, const _Float16 *&P, const _Float16
     blocks = (STAGE == GRAM ? m.np : m.mp) / 32;
 }
 
+// a wavefront's KiB of hi (0) or lo (1) from memory to LDS (the offset counts on both sides)
+template <int PIECE>
+MRL_DEV void bring(const _Float16 *from, _Float16 *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, PIECE * 1024, 0);
+}
+
+// Waits until at most LOADS of the wavefront's loads are under way and none of its LDS reads, then for the workgroup.
+template <int LOADS>
+MRL_DEV void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 7 << 4);   // (vmcnt; lgkmcnt 0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
 // One product, a tile of 32 F x 32 F per workgroup.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric, so only tiles on and
 // above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
-// Four wavefronts share the tile, 16 F x 16 F each, and KG such sets share the contracted index, 32 of it each at a time, so that
-// a SIMD has KG wavefronts to take turns.  Operands go from memory to LDS past the registers, the next 32 KG while these are
-// multiplied.  In the end the sets exchange sums through LDS and each finishes a part of the tile.
-template <int STAGE, int KIND, int F, int KG>
-__global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(F == 4 ? 2 : 4))) void product_kernel(Group g, int total, int from, int last) {
-    constexpr int SIDE = 2 * F;                        // fragments of 16 along a side
-    constexpr int OPERAND = SIDE * KG * 1024;          // halves of one operand of a stage: [fragment][set][hi, lo][512]
+// Four wavefronts share the tile, 16 F x 16 F each.  Operands go from memory to LDS past the registers, a stage of 32 of the
+// contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less time than memory takes to answer.
+// A tile at the edge reads the last rows' operands again where it has none of its own, and leaves what comes of them.
+template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
+template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
+template <int STAGE, int KIND, int F>
+__global__ __launch_bounds__(256) void product_kernel(Group g, int total, int from, int last) {
+    constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, LOADS = 2 * F;
     extern __shared__ _Float16 lds[];
     int bi, bj;
-    const Mat &m = find_tile<STAGE>(g, total, bi, bj);
+    const Mat &m = find_tile<STAGE, 32 * F>(g, total, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(m, from, P, Q, blocks);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave >> 2, part = wave & 3;
-    const int stages = blocks / KG;   // (whole: the sides are padded to the tile)
-    // A stage of a fragment, KG times hi and lo, is one run of memory and of LDS; a wavefront brings in EACH fragments of an operand.
-    constexpr int EACH = SIDE / (2 * KG);
-    const int operand = wave / (2 * KG), first = wave % (2 * KG) * EACH;
-    const _Float16 *src = (operand ? Q + (size_t)(bj * SIDE + first) * blocks * 1024 : P + (size_t)(bi * SIDE + first) * blocks * 1024) + lane * 8;
-    _Float16 *to = lds + operand * OPERAND + first * KG * 1024;
-    auto stage_in = [&](int stage) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // wavefronts 0 and 1 bring in P, the others Q, F fragments each
+    const int operand = wave >> 1, fragments = ((operand && STAGE == UPDATE) ? m.np : m.mp) / 16;
+    const _Float16 *src[F];
 #pragma unroll
-        for (int e = 0; e < EACH * 2 * KG; ++e)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(src + ((size_t)(e / (2 * KG)) * blocks + (size_t)stage * KG) * 1024 + e % (2 * KG) * 512),
-                (__attribute__((address_space(3))) void *)(to + (stage & 1) * 2 * OPERAND + e * 512), 16, 0, 0);
+    for (int f = 0; f < F; ++f)
+        src[f] = (operand ? Q : P) + min((operand ? bj : bi) * SIDE + (wave & 1) * F + f, fragments - 1) * 1024 + lane * 8;
+    int in_at = wave * F * 1024;   // where in LDS the next stage goes
+    auto brought = [&]() {
+#pragma unroll
+        for (int f = 0; f < F; ++f) src[f] += fragments * 1024;
+        in_at = in_at >= (AHEAD - 1) * STAGE_HALVES<F> ? in_at - (AHEAD - 1) * STAGE_HALVES<F> : in_at + STAGE_HALVES<F>;
     };
+    const int p = (wave >> 1) * F * 1024 + lane * 8, q = (SIDE + (wave & 1) * F) * 1024 + lane * 8;
+    int at = 0;   // of the stage that is worked on
+    auto read = [&](int where) { return *reinterpret_cast<const f16x8 *>(lds + at + where); };
     f32x4 acc[F][F] = {};
-    stage_in(0);
-    for (int s = 0; s < stages; ++s) {
-        __syncthreads();   // this stage is in LDS, and nobody reads the buffer of the next one any more
-        if (s + 1 < stages) stage_in(s + 1);
-        const _Float16 *p = lds + (s & 1) * 2 * OPERAND + ((part >> 1) * F * KG + set) * 1024 + lane * 8;
-        const _Float16 *q = lds + (s & 1) * 2 * OPERAND + OPERAND + ((part & 1) * F * KG + set) * 1024 + lane * 8;
-        f16x8 ph[F], pl[F], qh[F], ql[F];
+    // A stage's 3 F F products in three groups.  The meeting behind which the next stage is there, and this one's buffer free, stands
+    // ahead of the last group.  Requests to LDS and memory go out among the products, at most one ahead of each: a wavefront takes 16
+    // cycles or more to hand over either, in which the matrix cores would wait if they stood together.  A buffer that the meeting
+    // freed is asked for from there to the next meeting: EARLY loads in the last group, the others in the next stage's first two.
+    constexpr int N = F * F, EARLY = F == 4 ? 2 : F == 3 ? 1 : 0;
+    auto request = [&](int load) {
+        if (load % 2 == 0) bring<0>(src[load / 2], lds + in_at + load / 2 * 1024);
+        else bring<1>(src[load / 2], lds + in_at + load / 2 * 1024);
+    };
+    auto product = [&](int k, const f16x8 (&x)[F], const f16x8 (&y)[F]) {
+        acc[k / F][k % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[k / F], y[k % F], acc[k / F][k % F], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto first_groups = [&](f16x8 (&ph)[F], f16x8 (&pl)[F], f16x8 (&qh)[F], bool more) {
+        constexpr int FROM = 2 * F, STEP = (2 * N - FROM) / (LOADS - EARLY);
+        f16x8 ql[F];
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            pl[f] = *reinterpret_cast<const f16x8 *>(p + f * KG * 1024 + 512);
-            qh[f] = *reinterpret_cast<const f16x8 *>(q + f * KG * 1024);
+        for (int k = 0; k < 2 * N; ++k) {
+            if (k < F) ql[k] = read(q + 512 + k * 1024);
+            else if (k < 2 * F) ph[k - F] = read(p + (k - F) * 1024);
+            else if ((k - FROM) % STEP == 0 && (k - FROM) / STEP < LOADS - EARLY && more) request(EARLY + (k - FROM) / STEP);
+            if (k < N) product(k, pl, qh);
+            else product(k - N, ph, ql);
         }
+        if (more) brought();
+    };
+    auto last_group = [&](f16x8 (&ph)[F], f16x8 (&pl)[F], f16x8 (&qh)[F], f16x8 (&next)[F], bool more) {
+        at = at == (AHEAD - 1) * STAGE_HALVES<F> ? 0 : at + STAGE_HALVES<F>;
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            ph[f] = *reinterpret_cast<const f16x8 *>(p + f * KG * 1024);
-            ql[f] = *reinterpret_cast<const f16x8 *>(q + f * KG * 1024 + 512);
+        for (int k = 0; k < N; ++k) {
+            if (k < F) next[k] = read(q + k * 1024);
+            else if (k < 2 * F) pl[k - F] = read(p + 512 + (k - F) * 1024);
+            else if ((k - 2 * F) % 3 == 1 && (k - 2 * F) / 3 < EARLY && more) request((k - 2 * F) / 3);
+            product(k, ph, qh);
         }
-        multiply<F>(ph, pl, qh, ql, acc);
+    };
+    f16x8 ph[F], pl[F], qa[F], qb[F];
+    for (int s = 0; s < AHEAD - 1 && s < blocks; ++s) {
+#pragma unroll
+        for (int load = 0; load < LOADS; ++load) request(load);
+        brought();
     }
-    const int i0 = (bi * SIDE + (part >> 1) * F) * 16 + 4 * (lane >> 4), j0 = (bj * SIDE + (part & 1) * F) * 16 + (lane & 15);
-    // set s finishes the fragments whose number is s modulo KG
-    {
-        f32x4 *sums = reinterpret_cast<f32x4 *>(lds);   // [set that finishes][set that has them][part][fragment / KG][lane]
-        constexpr int SHARE = F * F / KG;
-        __syncthreads();
+    if (AHEAD - 1 < blocks) {
 #pragma unroll
-        for (int f = 0; f < F * F; ++f)
-            if (f % KG != set) sums[(((f % KG) * KG + set) * 4 + part) * SHARE * 64 + (f / KG) * 64 + lane] = acc[f / F][f % F];
-        __syncthreads();
+        for (int load = 0; load < EARLY; ++load) request(load);
+        meet<(AHEAD - 2) * LOADS + EARLY>();
+    } else {
+        meet<0>();
+    }
 #pragma unroll
-        for (int f = 0; f < F * F; ++f) {
-            if (f % KG != set) continue;
-            f32x4 v = acc[f / F][f % F];
+    for (int f = 0; f < F; ++f) {
+        qa[f] = read(q + f * 1024);
+        pl[f] = read(p + 512 + f * 1024);
+    }
+    // (the blocks are an even number: the sides are padded to 64)
+    int s = 0;
+    for (; s + 1 + AHEAD < blocks; s += 2) {
+        first_groups(ph, pl, qa, true);
+        meet<(AHEAD - 2) * LOADS>();   // stages s + 2 .. s + AHEAD - 1 may be on their way
+        last_group(ph, pl, qa, qb, true);
+        first_groups(ph, pl, qb, true);
+        meet<(AHEAD - 2) * LOADS>();
+        last_group(ph, pl, qb, qa, true);
+    }
+    for (; s < blocks; s += 2) {
+        first_groups(ph, pl, qa, s - 1 + AHEAD < blocks);
+        meet<0>();
+        last_group(ph, pl, qa, qb, s + AHEAD < blocks);
+        first_groups(ph, pl, qb, s + AHEAD < blocks);
+        if (s + 2 < blocks) {
+            meet<0>();
+            last_group(ph, pl, qb, qa, false);
+        } else {
 #pragma unroll
-            for (int other = 1; other < KG; ++other)
-                v += sums[((set * KG + (set + other) % KG) * 4 + part) * SHARE * 64 + (f / KG) * 64 + lane];
-            finish<STAGE, KIND>(g, m, from, last, bi == bj, i0 + 16 * (f / F), j0 + 16 * (f % F), v);
+            for (int k = 0; k < N; ++k) product(k, ph, qb);
         }
     }
+    const int fi = (bi * SIDE + (wave >> 1) * F) * 16, fj = (bj * SIDE + (wave & 1) * F) * 16;
+    Piece pieces[F * F];
+#pragma unroll
+    for (int f = 0; f < F * F; ++f) ask<STAGE>(m, from, fi + 16 * (f / F), fj + 16 * (f % F), pieces[f]);
+#pragma unroll
+    for (int f = 0; f < F * F; ++f)
+        finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / F), fj + 16 * (f % F), acc[f / F][f % F], pieces[f]);
 }
 
 // The same for small matrices, where a launch is shorter than the way of a stage through memory and LDS and back: a tile of 32 x 32
@@ -339,80 +417,86 @@ template <int STAGE, int KIND>
 __global__ __launch_bounds__(256) void small_product_kernel(Group g, int total, int from, int last) {
     __shared__ f32x4 sums[4][4][64];   // [fragment][wavefront][lane]
     int bi, bj;
-    const Mat &m = find_tile<STAGE>(g, total, bi, bj);
+    const Mat &m = find_tile<STAGE, 32>(g, total, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(m, from, P, Q, blocks);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const _Float16 *p = P + (size_t)bi * 2 * blocks * 1024 + lane * 8, *q = Q + (size_t)bj * 2 * blocks * 1024 + lane * 8;
+    const int p_fragments = m.mp / 16, q_fragments = (STAGE == UPDATE ? m.np : m.mp) / 16;
+    const _Float16 *p = P + bi * 2 * 1024 + lane * 8, *q = Q + bj * 2 * 1024 + lane * 8;
     f32x4 acc[2][2] = {};
+    const int fi = (bi * 2 + (wave >> 1)) * 16, fj = (bj * 2 + (wave & 1)) * 16;
+    Piece piece;
+    ask<STAGE>(m, from, fi, fj, piece);
 #pragma unroll 2
     for (int kb = wave; kb < blocks; kb += 4) {
         f16x8 ph[2], pl[2], qh[2], ql[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-            const _Float16 *pf = p + ((size_t)f * blocks + kb) * 1024, *qf = q + ((size_t)f * blocks + kb) * 1024;
+            const _Float16 *pf = p + ((size_t)kb * p_fragments + f) * 1024, *qf = q + ((size_t)kb * q_fragments + f) * 1024;
             ph[f] = *reinterpret_cast<const f16x8 *>(pf);
             pl[f] = *reinterpret_cast<const f16x8 *>(pf + 512);
             qh[f] = *reinterpret_cast<const f16x8 *>(qf);
             ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
         }
-        multiply<2>(ph, pl, qh, ql, acc);
+        multiply<2>(pl, qh, acc);
+        multiply<2>(ph, ql, acc);
+        multiply<2>(ph, qh, acc);
     }
 #pragma unroll
     for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
     __syncthreads();
     const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
-    finish<STAGE, KIND>(g, m, from, last, bi == bj, (bi * 2 + (wave >> 1)) * 16 + 4 * (lane >> 4), (bj * 2 + (wave & 1)) * 16 + (lane & 15), v);
+    finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
 }
 
-inline int pad(int x, int tile) { return (x + tile - 1) / tile * tile; }
+inline int pad(int x) { return (x + 63) / 64 * 64; }
 
 // bytes of one matrix's planes and sums
-size_t matrix_bytes(int rows, int cols, int tile) {
-    const size_t mp = pad(std::min(rows, cols), tile), np = pad(std::max(rows, cols), tile);
+size_t matrix_bytes(int rows, int cols) {
+    const size_t mp = pad(std::min(rows, cols)), np = pad(std::max(rows, cols));
     return sizeof(_Float16) * (6 * mp * np + 4 * mp * mp) + sizeof(double) * MOST_SUMS;
 }
 
-// The tiles of a launch: the largest of which the products have enough to go round.
-struct Sides { int rows, cols; };
-template <class S>
-int tile_of(const S *matrices, int count) {
-    for (int tile : {128, 64}) {
-        long tiles = 0;
-        for (int k = 0; k < count; ++k) tiles += (long)(pad(matrices[k].rows, tile) / tile) * (pad(matrices[k].cols, tile) / tile);
-        if (tiles >= (tile == 128 ? 128 : 64)) return tile;
+// Sides of the tiles of one of a group's products, and their number.
+int tiles_of(const Group &g, bool symmetric, int tile) {
+    int tiles = 0;
+    for (int k = 0; k < g.count; ++k) {
+        const int a = (g.mat[k].mp + tile - 1) / tile, b = (g.mat[k].np + tile - 1) / tile;
+        tiles += symmetric ? a * (a + 1) / 2 : a * b;
     }
-    return 32;
+    return tiles;
 }
-template <class S>
-size_t group_bytes(const S *matrices, int count) {
-    const int tile = tile_of(matrices, count);
-    size_t bytes = 0;
-    for (int k = 0; k < count; ++k) bytes += matrix_bytes(matrices[k].rows, matrices[k].cols, tile);
-    return bytes;
-}
-
-// of `count` alike, in launches of MOST; the last launch's tiles may be smaller, and so their padding
-size_t batch_bytes(int count, int rows, int cols) {
-    Sides sides[MOST];
-    std::fill(sides, sides + MOST, Sides{rows, cols});
-    const size_t whole = count >= MOST ? group_bytes(sides, MOST) : 0;
-    return std::max(whole, count % MOST ? group_bytes(sides, count % MOST) : (size_t)0);
+int tile_of(const mrl_ctx *ctx, const Group &g, bool symmetric) {
+    int best = 32;
+    double least = 0.25 * (2 + tiles_of(g, symmetric, 32) / (double)ctx->n_cus);
+    for (int F : {2, 3, 4}) {
+        const int tiles = tiles_of(g, symmetric, 32 * F), rounds = (tiles + ctx->n_cus - 1) / ctx->n_cus;
+        const double cost = F == 2 ? 0.5 * std::max(1.0, tiles / (double)ctx->n_cus) : rounds * (F == 3 ? 0.85 : 1.4);
+        if (cost < least) {
+            least = cost;
+            best = 32 * F;
+        }
+    }
+    return best;
 }
 
 // sides, scales and a share of the workspace
-void set_up(Mat &m, int rows, int cols, int tile, char *&ws) {
+void set_up(Mat &m, int rows, int cols, char *&ws) {
     m.rows = rows;
     m.cols = cols;
     m.tall = rows > cols;
     m.m = std::min(rows, cols);
     m.n = std::max(rows, cols);
-    m.mp = pad(m.m, tile);
-    m.np = pad(m.n, tile);
+    m.mp = pad(m.m);
+    m.np = pad(m.n);
     m.sums = (int)std::min<long>(MOST_SUMS, ((long)rows * cols + CHUNK - 1) / CHUNK);
     m.sx = (float)std::ldexp(1.0, std::min(14, (int)std::lround(0.5 * std::log2((double)m.m * m.n))));
-    m.sa = (float)std::ldexp(1.0, std::min(13, (int)std::lround(std::log2((double)m.m))));
+    const float sa = (float)std::ldexp(1.0, std::min(13, (int)std::lround(std::log2((double)m.m))));
+    m.gram = sa / (m.sx * m.sx);
+    m.square = QC / sa;
+    m.update = 1.0f / sa;
+    m.result = 1.0f / m.sx;
     auto planes = [&](size_t elements) {
         _Float16 *p = reinterpret_cast<_Float16 *>(ws);
         ws += sizeof(_Float16) * 2 * elements;
@@ -429,24 +513,28 @@ void set_up(Mat &m, int rows, int cols, int tile, char *&ws) {
 
 template <int STAGE, int KIND>
 void product(const mrl_ctx *ctx, const Group &g, int total, int from, int last) {
-    auto launch = [&](auto kernel, int threads, size_t lds) {
-        hipLaunchKernelGGL(kernel, dim3(total), dim3(threads), lds, ctx->stream, g, total, from, last);
+    const int tile = STAGE == UPDATE ? g.update_tile : g.sym_tile;
+    auto launch = [&](auto kernel, size_t lds) {
+        hipLaunchKernelGGL(kernel, dim3(total), dim3(256), lds, ctx->stream, g, total, from, last);
     };
-    if (g.tile == 128) launch(product_kernel<STAGE, KIND, 4, 2>, 512, 2 * 2 * 8 * 2 * 2048);
-    else if (g.tile == 64) launch(product_kernel<STAGE, KIND, 2, 2>, 512, 2 * 2 * 4 * 2 * 2048);
-    else launch(small_product_kernel<STAGE, KIND>, 256, 0);
+    if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>);
+    else if (tile == 96) launch(product_kernel<STAGE, KIND, 3>, sizeof(_Float16) * BUFFERS<3> * STAGE_HALVES<3>);
+    else if (tile == 64) launch(product_kernel<STAGE, KIND, 2>, sizeof(_Float16) * BUFFERS<2> * STAGE_HALVES<2>);
+    else launch(small_product_kernel<STAGE, KIND>, 0);
 }
 
 template <int KIND>
 void run(const mrl_ctx *ctx, Group &g, int steps) {
+    g.sym_tile = tile_of(ctx, g, true);
+    g.update_tile = tile_of(ctx, g, false);
     int sums = 0, load = 0, sym = 0, update = 0;
     for (int k = 0; k < g.count; ++k) {
         Mat &m = g.mat[k];
-        const int a = m.mp / g.tile, b = m.np / g.tile;
+        const int a = (m.mp + g.sym_tile - 1) / g.sym_tile;
         m.begin_sums = sums; sums += m.sums;
         m.begin_load = load; load += (m.mp / LOAD) * (m.np / LOAD);
         m.begin_sym = sym; sym += a * (a + 1) / 2;
-        m.begin_update = update; update += a * b;
+        m.begin_update = update; update += ((m.mp + g.update_tile - 1) / g.update_tile) * ((m.np + g.update_tile - 1) / g.update_tile);
     }
     g.total_sums = sums;
     int rest = 0;
@@ -505,7 +593,7 @@ int mrl_orthogonalize_workspace(int count, int rows, int cols, uint64_t *bytes) 
     MRL_CHECK_ARG(bytes && count >= 0, "%s: bad arguments", who);
     const int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK) return rc;
-    *bytes = mrl::batch_bytes(count, rows, cols);
+    *bytes = mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST);
     return MRL_OK;
 }
 
@@ -519,7 +607,7 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK || count == 0) return rc;
     MRL_CHECK_ARG(in && out, "%s: NULL buffer", who);
-    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::batch_bytes(count, rows, cols));
+    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST));
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
     const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
@@ -528,11 +616,8 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
         g.eps = eps;
         g.count = std::min(mrl::MOST, count - done);
         char *ws = (char *)workspace;
-        mrl::Sides sides[mrl::MOST];
-        std::fill(sides, sides + mrl::MOST, mrl::Sides{rows, cols});
-        g.tile = mrl::tile_of(sides, g.count);
         for (int k = 0; k < g.count; ++k) {
-            mrl::set_up(g.mat[k], rows, cols, g.tile, ws);
+            mrl::set_up(g.mat[k], rows, cols, ws);
             g.mat[k].in = (const char *)in + (done + k) * one;
             g.mat[k].out = (char *)out + (done + k) * one;
         }
@@ -550,7 +635,9 @@ int mrl_muon_workspace(int n_matrices, const mrl_matrix *matrices, uint64_t *byt
     if (rc != MRL_OK) return rc;
     *bytes = 0;
     for (int done = 0; done < n_matrices; done += mrl::MOST) {
-        *bytes = std::max<uint64_t>(*bytes, mrl::group_bytes(matrices + done, std::min(mrl::MOST, n_matrices - done)));
+        uint64_t group = 0;
+        for (int k = done; k < std::min(n_matrices, done + mrl::MOST); ++k) group += mrl::matrix_bytes(matrices[k].rows, matrices[k].cols);
+        *bytes = std::max(*bytes, group);
     }
     return MRL_OK;
 }
@@ -584,7 +671,6 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         g.adam_eps = (float)adam_eps;
         g.bc1 = (float)(1.0 - pow(beta1, (double)t)); g.bc2 = (float)(1.0 - pow(beta2, (double)t));
         g.count = std::min(mrl::MOST, n_matrices - done);
-        g.tile = mrl::tile_of(matrices + done, g.count);
         char *ws = (char *)workspace;
         auto rest = [&](int64_t to) {
             if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at), 0};
@@ -593,7 +679,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
             const mrl_matrix &x = matrices[done + k];
             mrl::Mat &m = g.mat[k];
             rest(x.offset);
-            mrl::set_up(m, x.rows, x.cols, g.tile, ws);
+            mrl::set_up(m, x.rows, x.cols, ws);
             m.in = grads + x.offset;
             m.out = params + x.offset;
             m.momentum = state + 2 * x.offset;
