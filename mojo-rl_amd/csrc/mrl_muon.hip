@@ -45,8 +45,7 @@ struct Mat {
     float sx;                       // what X is stored times; A and B: sa
     float gram, square, update, result;   // sums to A, A A to B, B X to X, X to the caller: sa / sx^2, c / sa, 1 / sa, 1 / sx
     float factor;                   // of the update
-    _Float16 *x, *xt[2], *a, *b;
-    double *partial;
+    size_t x, xt, xt1, a, b, partial; // planes and partial sums: bytes from the workspace's start
 };
 struct Rest { float *p; const float *g; float2 *state; long n; int begin; };   // parameters that Adam updates
 struct Group {
@@ -60,29 +59,60 @@ struct Group {
     int nesterov;
     float lr, beta1, beta2, omb1, omb2, adam_eps, bc1, bc2;
 };
-static_assert(sizeof(Group) <= 3584, "kernel arguments");
+static_assert(sizeof(Group) <= 3584 && sizeof(Group) % 4 == 0, "kernel arguments");
+constexpr size_t GROUP_BYTES = (sizeof(Group) + 63) / 64 * 64;
+
+// what is there, for pointers that come out of memory
+template <class T>
+MRL_DEV auto in_memory(T *p) { return (__attribute__((address_space(1))) T *)p; }
+template <class T>
+MRL_DEV T *in_workspace(const Group *kept, size_t bytes) { return (T *)((char *)kept + bytes); }
+MRL_DEV _Float16 *planes(const Group *kept, size_t bytes) { return in_workspace<_Float16>(kept, bytes); }
+
+// a description out of memory, all at once
+MRL_DEV Mat described(const Mat &m) {
+    Mat own;
+    __builtin_memcpy(&own, (const __attribute__((address_space(4))) Mat *)&m, sizeof(Mat));
+    return own;
+}
 
 enum { F32 = 0, BF16 = 1, MUON = 2 };   // what a matrix is read from and written to
 
-template <int KIND>
+// What is orthogonalised, element i; FIRST: with MUON its momentum is brought up to date.
+template <int KIND, bool FIRST = false>
 MRL_DEV float source(const Group &g, const Mat &m, size_t i) {
-    if (KIND == BF16) return __uint_as_float((unsigned)((const unsigned short *)m.in)[i] << 16);
-    const float x = ((const float *)m.in)[i];
+    if (KIND == BF16) return __uint_as_float((unsigned)in_memory((const unsigned short *)m.in)[i] << 16);
+    const float x = in_memory((const float *)m.in)[i];
     if (KIND == F32) return x;
-    const float v = m.momentum[i];   // (already this step's)
+    const auto at = in_memory(m.momentum) + i;
+    float v = *at;
+    if (FIRST) {
+        v = fmaf(g.mu, v, x);
+        *at = v;
+    }
     return g.nesterov ? fmaf(g.mu, v, x) : v;
 }
-
-// Sums of squares of every matrix, in 64 bits and a fixed order; with MUON also the new momentum, and Adam on the other parameters.
 template <int KIND>
-__global__ __launch_bounds__(256) void sums_kernel(Group g) {
+MRL_DEV double square_of(const Group &g, const Mat &m, size_t i) {
+    const double x = source<KIND, true>(g, m, i);
+    return x * x;
+}
+// Adam on the parameters between the matrices
+MRL_DEV void adam_rest(const Group &g, int block, int threads) {
+    int k = 0;
+    while (k + 1 < g.rests && block >= g.rest[k + 1].begin) ++k;
+    const Rest &r = g.rest[k];
+    const long i = (long)(block - r.begin) * threads + threadIdx.x;
+    if (i < r.n) adam_one(r.p[i], r.g[i], r.state[i], g.lr, g.beta1, g.beta2, g.omb1, g.omb2, g.adam_eps, g.bc1, g.bc2);
+}
+// Sums of squares of every matrix, in 64 bits and a fixed order, and Adam.  The group's description, 3 KiB of arguments that cost the
+// host 1.5 us a launch, goes to the workspace, where the launches behind this one find it.
+template <int KIND>
+__global__ __launch_bounds__(256) void sums_kernel(Group g, Group *kept) {
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < (int)(sizeof(Group) / 4); i += 256) reinterpret_cast<int *>(kept)[i] = reinterpret_cast<const int *>(&g)[i];
     if (KIND == MUON && (int)blockIdx.x >= g.total_sums) {
-        const int block = blockIdx.x - g.total_sums;
-        int k = 0;
-        while (k + 1 < g.rests && block >= g.rest[k + 1].begin) ++k;
-        const Rest &r = g.rest[k];
-        const long i = (long)(block - r.begin) * 256 + threadIdx.x;
-        if (i < r.n) adam_one(r.p[i], r.g[i], r.state[i], g.lr, g.beta1, g.beta2, g.omb1, g.omb2, g.adam_eps, g.bc1, g.bc2);
+        adam_rest(g, blockIdx.x - g.total_sums, 256);
         return;
     }
     int k = 0;
@@ -91,11 +121,8 @@ __global__ __launch_bounds__(256) void sums_kernel(Group g) {
     const int block = blockIdx.x - m.begin_sums;
     const size_t size = (size_t)m.rows * m.cols;
     double sum = 0.0;
-    for (size_t i = (size_t)block * 256 + threadIdx.x; i < size; i += (size_t)m.sums * 256) {
-        if (KIND == MUON) m.momentum[i] = fmaf(g.mu, m.momentum[i], ((const float *)m.in)[i]);
-        const float x = source<KIND>(g, m, i);
-        sum += (double)x * (double)x;
-    }
+#pragma unroll 4
+    for (size_t i = (size_t)block * 256 + threadIdx.x; i < size; i += (size_t)m.sums * 256) sum += square_of<KIND>(g, m, i);
     __shared__ double part[256];
     part[threadIdx.x] = sum;
     __syncthreads();
@@ -103,7 +130,7 @@ __global__ __launch_bounds__(256) void sums_kernel(Group g) {
         if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
         __syncthreads();
     }
-    if (threadIdx.x == 0) m.partial[block] = part[0];
+    if (threadIdx.x == 0) in_workspace<double>(kept, m.partial)[block] = part[0];
 }
 
 // Four neighbours along the contracted index (k a multiple of 4) of a row, in pieces
@@ -128,24 +155,22 @@ struct Piece {
 MRL_DEV size_t square_at(int rows, int row, int k) { return ((size_t)(k >> 5) * (rows >> 4) + (row >> 4)) * 1024 + (k & 16) * 16; }
 MRL_DEV int piece_in(int r, int quarter) { return (quarter >> 1) * 128 + r * 8 + (quarter & 1) * 4; }
 
-// X and its transpose in pieces, a tile per workgroup, through LDS: read along the caller's rows, written along both sides.
-template <int KIND>
-__global__ __launch_bounds__(256) void load_kernel(Group g) {
-    __shared__ double part[256];
-    __shared__ float tile[LOAD][LOAD + 1];
-    int k = 0;
-    while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_load) ++k;
-    const Mat &m = g.mat[k];
-    const int block = blockIdx.x - m.begin_load, across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
+// What X is multiplied by as it is read: the norm from the partial sums, in a fixed order.
+MRL_DEV double scale_of(const Group &g, const Mat &m, double *part) {
     double sum = 0.0;
-    for (int i = threadIdx.x; i < m.sums; i += 256) sum += m.partial[i];
+    for (int i = threadIdx.x; i < m.sums; i += 256) sum += in_workspace<double>(&g, m.partial)[i];
     part[threadIdx.x] = sum;
     __syncthreads();
     for (int w = 128; w > 0; w >>= 1) {
         if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
         __syncthreads();
     }
-    const double scale = (double)m.sx / (sqrt(part[0]) + g.eps);
+    return (double)m.sx / (sqrt(part[0]) + g.eps);
+}
+// A square of X and of its transpose in pieces, through LDS: read along the caller's rows, written along both sides.
+template <int KIND>
+MRL_DEV void load_square(const Group &g, const Mat &m, int block, double scale, float (&tile)[LOAD][LOAD + 1]) {
+    const int across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
     for (int e = threadIdx.x; e < LOAD * LOAD; e += 256) {
         const int slow = e / LOAD, fast = e % LOAD;                            // fast runs along the caller's rows
         const int i = m.tall ? fast : slow, j = m.tall ? slow : fast;
@@ -160,9 +185,19 @@ __global__ __launch_bounds__(256) void load_kernel(Group g) {
     for (int e = threadIdx.x; e < LOAD * LOAD / 4; e += 256) {
         const int r = e % LOAD, c = e / LOAD * 4;
         const int in = (c & 16) * 16 + piece_in(r & 15, (c & 15) >> 2);
-        Piece(f32x4{tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]}).store(m.x + square_at(m.mp, i0 + r, j0) + in);
-        Piece(f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]}).store(m.xt[0] + square_at(m.np, j0 + r, i0) + in);
+        Piece(f32x4{tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]}).store(planes(&g, m.x) + square_at(m.mp, i0 + r, j0) + in);
+        Piece(f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]}).store(planes(&g, m.xt) + square_at(m.np, j0 + r, i0) + in);
     }
+}
+template <int KIND>
+__global__ __launch_bounds__(256) void load_kernel(const Group *__restrict__ group) {
+    const Group &g = *group;
+    __shared__ double part[256];
+    __shared__ float tile[LOAD][LOAD + 1];
+    int k = 0;
+    while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_load) ++k;
+    const Mat m = described(g.mat[k]);
+    load_square<KIND>(g, m, blockIdx.x - m.begin_load, scale_of(g, m, part), tile);
 }
 
 // 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
@@ -182,29 +217,33 @@ MRL_DEV f16x4 quad_transpose(f16x4 v) {
 
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
 
+// tile number `tile` on and above the diagonal: column bj has tiles 0 .. bj
+MRL_DEV void above_diagonal(int tile, int &bi, int &bj) {
+    bj = __builtin_amdgcn_readfirstlane((int)((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f));
+    while (bj * (bj + 1) / 2 > tile) --bj;
+    while ((bj + 1) * (bj + 2) / 2 <= tile) ++bj;
+    bi = tile - bj * (bj + 1) / 2;
+}
+
 // Which tile of which matrix a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that
 // share operands, so that its L2 is read more often than what is behind it.
 template <int STAGE, int TILE>
-MRL_DEV const Mat &find_tile(const Group &g, int total, int &bi, int &bj) {
+MRL_DEV Mat find_tile(const Group &g, int total, int &bi, int &bj) {
     const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
     const int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
     int k = 0;
     if (STAGE == UPDATE) {
         while (k + 1 < g.count && id >= g.mat[k + 1].begin_update) ++k;
-        const Mat &m = g.mat[k];
-        const int block = id - m.begin_update, rows = (m.mp + TILE - 1) / TILE, panel = block / (4 * rows), in = block - panel * 4 * rows;
+        const Mat m = described(g.mat[k]);
+        const int block = id - m.begin_update, rows = (m.mp + TILE - 1) / TILE, panel = __builtin_amdgcn_readfirstlane(block / (4 * rows)), in = block - panel * 4 * rows;
         const int width = min(4, (m.np + TILE - 1) / TILE - 4 * panel);   // panels of four columns, row by row
-        bi = in / width;
+        bi = __builtin_amdgcn_readfirstlane(in / width);
         bj = 4 * panel + in - bi * width;
         return m;
     }
     while (k + 1 < g.count && id >= g.mat[k + 1].begin_sym) ++k;
-    const Mat &m = g.mat[k];
-    int block = id - m.begin_sym;
-    bj = (int)((sqrtf(8.0f * block + 1.0f) - 1.0f) * 0.5f);   // column bj has tiles 0 .. bj
-    while (bj * (bj + 1) / 2 > block) --bj;
-    while ((bj + 1) * (bj + 2) / 2 <= block) ++bj;
-    bi = block - bj * (bj + 1) / 2;
+    const Mat m = described(g.mat[k]);
+    above_diagonal(id - m.begin_sym, bi, bj);
     return m;
 }
 
@@ -213,9 +252,9 @@ template <int STAGE>
 MRL_DEV bool inside(const Mat &m, int fi, int fj) { return fi < m.mp && fj < (STAGE == UPDATE ? m.np : m.mp); }
 // What the sums are added to, X or A there: asked for early, all at once.
 template <int STAGE>
-MRL_DEV void ask(const Mat &m, int from, int fi, int fj, Piece &piece) {
+MRL_DEV void ask(const Group &g, const Mat &m, int from, int fi, int fj, Piece &piece) {
     const int lane = threadIdx.x & 63;
-    if (STAGE != GRAM && inside<STAGE>(m, fi, fj)) piece.load((STAGE == UPDATE ? m.xt[from] : m.a) + square_at(STAGE == UPDATE ? m.np : m.mp, fj, fi) + piece_in(lane & 15, lane >> 4));
+    if (STAGE != GRAM && inside<STAGE>(m, fi, fj)) piece.load(planes(&g, STAGE == UPDATE ? (from ? m.xt1 : m.xt) : m.a) + square_at(STAGE == UPDATE ? m.np : m.mp, fj, fi) + piece_in(lane & 15, lane >> 4));
 }
 // A square's sums in pieces, as columns (row j, k = i) and as rows (row i, k = j)
 MRL_DEV void store_both(_Float16 *columns, int column_rows, _Float16 *rows, int row_rows, int fi, int fj, const f32x4 v) {
@@ -227,33 +266,35 @@ MRL_DEV void store_both(_Float16 *columns, int column_rows, _Float16 *rows, int 
     piece.lo = quad_transpose(piece.lo);
     piece.store(rows + square_at(row_rows, fi, fj) + piece_in(4 * quarter + (column & 3), column >> 2));
 }
+// A square of the last X to the caller.
+template <int KIND>
+MRL_DEV void give(const Group &g, const Mat &m, int fi, int fj, const f32x4 v) {
+    const int lane = threadIdx.x & 63, i = fi + 4 * (lane >> 4), j = fj + (lane & 15);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i + e >= m.m || j >= m.n) continue;
+        const size_t at = m.tall ? (size_t)j * m.m + (i + e) : (size_t)(i + e) * m.n + j;
+        const float o = v[e] * m.result;
+        if (KIND == BF16) {
+            in_memory((unsigned short *)m.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)o);
+        } else if (KIND == F32) {
+            in_memory((float *)m.out)[at] = o;
+        } else {
+            const auto w = in_memory((float *)m.out) + at;
+            *w = fmaf(-m.factor, o, *w * g.keep);
+        }
+    }
+}
 // What becomes of the sums.
 template <int STAGE, int KIND>
 MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diagonal, int fi, int fj, f32x4 v, const Piece &piece) {
     if (!inside<STAGE>(m, fi, fj)) return;
     if (STAGE == UPDATE) {
         v = QA * piece.value() + v * m.update;
-        if (!last) {
-            store_both(m.xt[from ^ 1], m.np, m.x, m.mp, fi, fj, v);
-            return;
-        }
-        const int lane = threadIdx.x & 63, i = fi + 4 * (lane >> 4), j = fj + (lane & 15);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e >= m.m || j >= m.n) continue;
-            const size_t at = m.tall ? (size_t)j * m.m + (i + e) : (size_t)(i + e) * m.n + j;
-            const float o = v[e] * m.result;
-            if (KIND == BF16) {
-                ((unsigned short *)m.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)o);
-            } else if (KIND == F32) {
-                ((float *)m.out)[at] = o;
-            } else {
-                float *w = (float *)m.out + at;
-                *w = fmaf(-m.factor, o, *w * g.keep);
-            }
-        }
+        if (last) give<KIND>(g, m, fi, fj, v);
+        else store_both(planes(&g, (from ? m.xt : m.xt1)), m.np, planes(&g, m.x), m.mp, fi, fj, v);
     } else {
-        _Float16 *to = STAGE == GRAM ? m.a : m.b;
+        _Float16 *to = planes(&g, STAGE == GRAM ? m.a : m.b);
         if (STAGE == GRAM) v = v * m.gram;
         else v = QB * piece.value() + v * m.square;
         store_both(to, m.mp, diagonal ? nullptr : to, m.mp, fi, fj, v);
@@ -269,9 +310,9 @@ MRL_DEV void multiply(const f16x8 (&p)[F], const f16x8 (&q)[F], f32x4 (&acc)[F][
 }
 
 template <int STAGE>
-MRL_DEV void operands(const Mat &m, int from, const _Float16 *&P, const _Float16 *&Q, int &blocks) {
-    P = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b;
-    Q = STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[from];
+MRL_DEV void operands(const Group &g, const Mat &m, int from, const _Float16 *&P, const _Float16 *&Q, int &blocks) {
+    P = planes(&g, STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b);
+    Q = planes(&g, STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : (from ? m.xt1 : m.xt));
     blocks = (STAGE == GRAM ? m.np : m.mp) / 32;
 }
 
@@ -300,14 +341,15 @@ MRL_DEV void meet() {
 template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
 template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
 template <int STAGE, int KIND, int F>
-__global__ __launch_bounds__(256) void product_kernel(Group g, int total, int from, int last) {
+__global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ group, int total, int from, int last) {
+    const Group &g = *group;
     constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, LOADS = 2 * F;
     extern __shared__ _Float16 lds[];
     int bi, bj;
-    const Mat &m = find_tile<STAGE, 32 * F>(g, total, bi, bj);
+    const Mat m = find_tile<STAGE, 32 * F>(g, total, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
-    operands<STAGE>(m, from, P, Q, blocks);
+    operands<STAGE>(g, m, from, P, Q, blocks);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // wavefronts 0 and 1 bring in P, the others Q, F fragments each
     const int operand = wave >> 1, fragments = ((operand && STAGE == UPDATE) ? m.np : m.mp) / 16;
@@ -405,43 +447,56 @@ __global__ __launch_bounds__(256) void product_kernel(Group g, int total, int fr
     const int fi = (bi * SIDE + (wave >> 1) * F) * 16, fj = (bj * SIDE + (wave & 1) * F) * 16;
     Piece pieces[F * F];
 #pragma unroll
-    for (int f = 0; f < F * F; ++f) ask<STAGE>(m, from, fi + 16 * (f / F), fj + 16 * (f % F), pieces[f]);
+    for (int f = 0; f < F * F; ++f) ask<STAGE>(g, m, from, fi + 16 * (f / F), fj + 16 * (f % F), pieces[f]);
 #pragma unroll
     for (int f = 0; f < F * F; ++f)
         finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / F), fj + 16 * (f % F), acc[f / F][f % F], pieces[f]);
 }
 
-// The same for small matrices, where a launch is shorter than the way of a stage through memory and LDS and back: a tile of 32 x 32
-// per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.
+// The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
+// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.
+typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
 template <int STAGE, int KIND>
-__global__ __launch_bounds__(256) void small_product_kernel(Group g, int total, int from, int last) {
-    __shared__ f32x4 sums[4][4][64];   // [fragment][wavefront][lane]
-    int bi, bj;
-    const Mat &m = find_tile<STAGE, 32>(g, total, bi, bj);
+MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums) {
     const _Float16 *P, *Q;
     int blocks;
-    operands<STAGE>(m, from, P, Q, blocks);
+    operands<STAGE>(g, m, from, P, Q, blocks);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int p_fragments = m.mp / 16, q_fragments = (STAGE == UPDATE ? m.np : m.mp) / 16;
     const _Float16 *p = P + bi * 2 * 1024 + lane * 8, *q = Q + bj * 2 * 1024 + lane * 8;
     f32x4 acc[2][2] = {};
     const int fi = (bi * 2 + (wave >> 1)) * 16, fj = (bj * 2 + (wave & 1)) * 16;
     Piece piece;
-    ask<STAGE>(m, from, fi, fj, piece);
-#pragma unroll 2
-    for (int kb = wave; kb < blocks; kb += 4) {
-        f16x8 ph[2], pl[2], qh[2], ql[2];
+    ask<STAGE>(g, m, from, fi, fj, piece);
+    struct Operands { f16x8 ph[2], pl[2], qh[2], ql[2]; };
+    auto load = [&](int kb, Operands &o) {
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
             const _Float16 *pf = p + ((size_t)kb * p_fragments + f) * 1024, *qf = q + ((size_t)kb * q_fragments + f) * 1024;
-            ph[f] = *reinterpret_cast<const f16x8 *>(pf);
-            pl[f] = *reinterpret_cast<const f16x8 *>(pf + 512);
-            qh[f] = *reinterpret_cast<const f16x8 *>(qf);
-            ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
+            o.ph[f] = *reinterpret_cast<const f16x8 *>(pf);
+            o.pl[f] = *reinterpret_cast<const f16x8 *>(pf + 512);
+            o.qh[f] = *reinterpret_cast<const f16x8 *>(qf);
+            o.ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
         }
-        multiply<2>(pl, qh, acc);
-        multiply<2>(ph, ql, acc);
-        multiply<2>(ph, qh, acc);
+    };
+    auto work = [&](const Operands &o) {
+        multiply<2>(o.pl, o.qh, acc);
+        multiply<2>(o.ph, o.ql, acc);
+        multiply<2>(o.ph, o.qh, acc);
+    };
+    // two steps' operands under way together
+    int kb = wave;
+    for (; kb + 4 < blocks; kb += 8) {
+        Operands one, two;
+        load(kb, one);
+        load(kb + 4, two);
+        work(one);
+        work(two);
+    }
+    if (kb < blocks) {
+        Operands one;
+        load(kb, one);
+        work(one);
     }
 #pragma unroll
     for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
@@ -449,8 +504,126 @@ __global__ __launch_bounds__(256) void small_product_kernel(Group g, int total, 
     const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
     finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
 }
+template <int STAGE, int KIND>
+__global__ __launch_bounds__(256) void small_product_kernel(const Group *__restrict__ group, int total, int from, int last) {
+    const Group &g = *group;
+    __shared__ SmallSums sums;
+    int bi, bj;
+    const Mat m = find_tile<STAGE, 32>(g, total, bi, bj);
+    small_product<STAGE, KIND>(g, m, bi, bj, from, last, sums);
+}
 
-inline int pad(int x) { return (x + 63) / 64 * 64; }
+// A small matrix by one workgroup in one launch, the optimiser's part included: all operands stay in LDS, sixteen wavefronts take
+// 16 x 16 sums each and meet behind every product.  64 x 64: TIME1 us instead of 75 in launches of their own, 64 x 128 TIME2
+// instead of 78, eleven of 216 x 10 TIME3 instead of 116.  (Operands out of the caches instead: 28, 43 and 30, bound by what a CU's L1
+// gives, and from 96 x 128 on longer than the launches.)
+constexpr int WHOLE_LDS = 160 * 1024, WHOLE_MOST = 5;   // squares of 16 x 16 of X per wavefront
+constexpr size_t whole_lds(int mp, int np) { return sizeof(_Float16) * 4 * mp * (size_t)(np + mp); }   // X, its transpose, A, B
+// sums of square (bi, bj) over `blocks` times 32
+MRL_DEV f32x4 square_sum(const _Float16 *P, int p_rows, int bi, const _Float16 *Q, int q_rows, int bj, int blocks) {
+    const int lane = threadIdx.x & 63;
+    const _Float16 *p = P + bi * 1024 + lane * 8, *q = Q + bj * 1024 + lane * 8;
+    f32x4 acc = {};
+#pragma unroll 2
+    for (int kb = 0; kb < blocks; ++kb, p += p_rows * 64, q += q_rows * 64) {
+        const f16x8 ph = *reinterpret_cast<const f16x8 *>(p), pl = *reinterpret_cast<const f16x8 *>(p + 512);
+        const f16x8 qh = *reinterpret_cast<const f16x8 *>(q), ql = *reinterpret_cast<const f16x8 *>(q + 512);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    }
+    return acc;
+}
+template <int KIND>
+__global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
+    extern __shared__ _Float16 lds[];
+    if (KIND == MUON && (int)blockIdx.x >= g.count) {
+        adam_rest(g, blockIdx.x - g.count, 1024);
+        return;
+    }
+    const Mat &m = g.mat[blockIdx.x];
+    const int size = m.rows * m.cols, mp = m.mp, np = m.np;
+    double *part = reinterpret_cast<double *>(lds);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < size; i += 1024) sum += square_of<KIND>(g, m, i);
+    for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += part[w];
+    __syncthreads();
+    const double scale = (double)m.sx / (sqrt(sum) + g.eps);
+    _Float16 *X = lds, *XT = X + 2 * mp * np, *A = XT + 2 * mp * np, *B = A + 2 * mp * mp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = mp / 16, columns = np / 16;
+    // an element at a time, along the caller's rows
+    const int slow = m.tall ? np : mp, fast = m.tall ? mp : np;
+    for (int f = lane; f < fast; f += 64) {
+#pragma unroll 4
+        for (int r = wave; r < slow; r += 16) {
+            const int i = m.tall ? f : r, j = m.tall ? r : f;
+            const float x = i < m.m && j < m.n ? (float)((double)source<KIND>(g, m, r * m.cols + f) * scale) : 0.0f;
+            const _Float16 hi = (_Float16)x, lo = (_Float16)(x - (float)hi);
+            _Float16 *p = X + square_at(mp, i, j) + piece_in(i & 15, (j & 15) >> 2) + (j & 3);
+            p[0] = hi;
+            p[512] = lo;
+            p = XT + square_at(np, j, i) + piece_in(j & 15, (i & 15) >> 2) + (i & 3);
+            p[0] = hi;
+            p[512] = lo;
+        }
+    }
+    __syncthreads();
+    const int at = piece_in(lane & 15, lane >> 4);
+    for (int s = 0; s < steps; ++s) {
+        for (int t = wave; t < rows * (rows + 1) / 2; t += 16) {
+            int bi, bj;
+            above_diagonal(t, bi, bj);
+            store_both(A, mp, bi == bj ? nullptr : A, mp, bi * 16, bj * 16, square_sum(X, mp, bi, X, mp, bj, np / 32) * m.gram);
+        }
+        __syncthreads();
+        for (int t = wave; t < rows * (rows + 1) / 2; t += 16) {
+            int bi, bj;
+            above_diagonal(t, bi, bj);
+            Piece a;
+            a.load(A + square_at(mp, bj * 16, bi * 16) + at);
+            store_both(B, mp, bi == bj ? nullptr : B, mp, bi * 16, bj * 16, QB * a.value() + square_sum(A, mp, bi, A, mp, bj, mp / 32) * m.square);
+        }
+        __syncthreads();
+        f32x4 v[WHOLE_MOST];
+#pragma unroll
+        for (int i = 0; i < WHOLE_MOST; ++i) {
+            const int t = wave + 16 * i, bi = t % rows, bj = t / rows;
+            if (t >= rows * columns) continue;
+            Piece x;
+            x.load(XT + square_at(np, bj * 16, bi * 16) + at);
+            v[i] = QA * x.value() + square_sum(B, mp, bi, XT, np, bj, mp / 32) * m.update;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WHOLE_MOST; ++i) {
+            const int t = wave + 16 * i, bi = t % rows, bj = t / rows;
+            if (t >= rows * columns) continue;
+            if (s == steps - 1) give<KIND>(g, m, bi * 16, bj * 16, v[i]);
+            else store_both(XT, np, X, mp, bi * 16, bj * 16, v[i]);
+        }
+        __syncthreads();
+    }
+}
+
+inline int pad(int x, int to = 64) { return (x + to - 1) / to * to; }
+
+// Whether one workgroup takes every matrix of a group, and the LDS for it.
+template <class S>
+bool is_whole(const S *matrices, int count, size_t &lds) {
+    lds = 128;   // (the partial sums of squares)
+    for (int k = 0; k < count; ++k) {
+        const int mp = pad(std::min(matrices[k].rows, matrices[k].cols), 32), np = pad(std::max(matrices[k].rows, matrices[k].cols), 32);
+        lds = std::max(lds, whole_lds(mp, np));
+        if (whole_lds(mp, np) > WHOLE_LDS || mp / 16 * (np / 16) > 16 * WHOLE_MOST) return false;
+    }
+    return true;
+}
 
 // bytes of one matrix's planes and sums
 size_t matrix_bytes(int rows, int cols) {
@@ -458,64 +631,85 @@ size_t matrix_bytes(int rows, int cols) {
     return sizeof(_Float16) * (6 * mp * np + 4 * mp * mp) + sizeof(double) * MOST_SUMS;
 }
 
-// Sides of the tiles of one of a group's products, and their number.
-int tiles_of(const Group &g, bool symmetric, int tile) {
-    int tiles = 0;
-    for (int k = 0; k < g.count; ++k) {
-        const int a = (g.mat[k].mp + tile - 1) / tile, b = (g.mat[k].np + tile - 1) / tile;
-        tiles += symmetric ? a * (a + 1) / 2 : a * b;
-    }
-    return tiles;
+template <class S>
+size_t group_bytes(const S *matrices, int count) {
+    size_t lds, bytes = GROUP_BYTES;
+    if (is_whole(matrices, count, lds)) return 0;
+    for (int k = 0; k < count; ++k) bytes += matrix_bytes(matrices[k].rows, matrices[k].cols);
+    return bytes;
 }
+// of `count` alike
+size_t batch_bytes(int count, int rows, int cols) {
+    Mat alike[MOST] = {};
+    for (Mat &m : alike) m.rows = rows, m.cols = cols;
+    return group_bytes(alike, std::min(count, MOST));
+}
+
+// Sides of the tiles of a group's symmetric products, or of its updates: those of the least time by what products of one to sixteen
+// matrices of 256 to 2048 took, in us, K of the contracted index long (256 CUs; one workgroup per CU at 96 and 128):
+//   32: 5.0 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.015 + 0.009 share)
+// where share of the CUs have one; more of them get in each other's way at the caches.  Symmetric / update at 32, 64, 96, 128:
+//   256: 5 / 5, 6 / 7, 8 / 10, 10 / 13    1024: 11 / 15, 12 / 13, 17 / 20, 24 / 28    2048: 66 / 96, 49 / 67, 39 / 79, 47 / 58
 int tile_of(const mrl_ctx *ctx, const Group &g, bool symmetric) {
-    int best = 32;
-    double least = 0.25 * (2 + tiles_of(g, symmetric, 32) / (double)ctx->n_cus);
-    for (int F : {2, 3, 4}) {
-        const int tiles = tiles_of(g, symmetric, 32 * F), rounds = (tiles + ctx->n_cus - 1) / ctx->n_cus;
-        const double cost = F == 2 ? 0.5 * std::max(1.0, tiles / (double)ctx->n_cus) : rounds * (F == 3 ? 0.85 : 1.4);
-        if (cost < least) {
-            least = cost;
-            best = 32 * F;
+    int best = 0;
+    double least = 0.0;
+    for (int tile : {32, 64, 96, 128}) {
+        double tiles = 0.0, work = 0.0;
+        for (int k = 0; k < g.count; ++k) {
+            const double a = (g.mat[k].mp + tile - 1) / tile, b = (g.mat[k].np + tile - 1) / tile, own = symmetric ? a * (a + 1) / 2 : a * b;
+            tiles += own;
+            work += own * (symmetric ? 0.5 * (g.mat[k].mp + g.mat[k].np) : g.mat[k].mp);
+        }
+        const double K = work / tiles, per_cu = tiles / ctx->n_cus, rounds = std::ceil(per_cu), share = std::min(1.0, per_cu);
+        const double time = tile == 32   ? 5.0 + 11e-6 * 256 * per_cu * K
+                            : tile == 64 ? 5.5 + 0.0072 * K * rounds
+                            : tile == 96 ? 6.0 + K * rounds * (0.0105 + 0.006 * share)
+                                         : 7.0 + K * rounds * (0.015 + 0.009 * share);
+        if (best == 0 || time < least) {
+            least = time;
+            best = tile;
         }
     }
     return best;
 }
 
 // sides, scales and a share of the workspace
-void set_up(Mat &m, int rows, int cols, char *&ws) {
-    m.rows = rows;
-    m.cols = cols;
-    m.tall = rows > cols;
-    m.m = std::min(rows, cols);
-    m.n = std::max(rows, cols);
-    m.mp = pad(m.m);
-    m.np = pad(m.n);
-    m.sums = (int)std::min<long>(MOST_SUMS, ((long)rows * cols + CHUNK - 1) / CHUNK);
+void set_up(Mat &m, int to, size_t &used) {
+    m.mp = pad(m.m, to);
+    m.np = pad(m.n, to);
+    m.sums = (int)std::min<long>(MOST_SUMS, ((long)m.m * m.n + CHUNK - 1) / CHUNK);
     m.sx = (float)std::ldexp(1.0, std::min(14, (int)std::lround(0.5 * std::log2((double)m.m * m.n))));
     const float sa = (float)std::ldexp(1.0, std::min(13, (int)std::lround(std::log2((double)m.m))));
     m.gram = sa / (m.sx * m.sx);
     m.square = QC / sa;
     m.update = 1.0f / sa;
     m.result = 1.0f / m.sx;
-    auto planes = [&](size_t elements) {
-        _Float16 *p = reinterpret_cast<_Float16 *>(ws);
-        ws += sizeof(_Float16) * 2 * elements;
-        return p;
+    auto take = [&](size_t bytes) {
+        const size_t at = used;
+        used += bytes;
+        return at;
     };
-    m.partial = reinterpret_cast<double *>(ws);
-    ws += sizeof(double) * MOST_SUMS;
-    m.x = planes((size_t)m.mp * m.np);
-    m.xt[0] = planes((size_t)m.mp * m.np);
-    m.xt[1] = planes((size_t)m.mp * m.np);
-    m.a = planes((size_t)m.mp * m.mp);
-    m.b = planes((size_t)m.mp * m.mp);
+    const size_t X = sizeof(_Float16) * 2 * m.mp * (size_t)m.np, A = sizeof(_Float16) * 2 * m.mp * (size_t)m.mp;
+    m.partial = take(sizeof(double) * MOST_SUMS);
+    m.x = take(X);
+    m.xt = take(X);
+    m.xt1 = take(X);
+    m.a = take(A);
+    m.b = take(A);
+}
+void sides(Mat &m, int rows, int cols) {
+    m.rows = rows;
+    m.cols = cols;
+    m.tall = rows > cols;
+    m.m = std::min(rows, cols);
+    m.n = std::max(rows, cols);
 }
 
 template <int STAGE, int KIND>
-void product(const mrl_ctx *ctx, const Group &g, int total, int from, int last) {
+void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int total, int from, int last) {
     const int tile = STAGE == UPDATE ? g.update_tile : g.sym_tile;
     auto launch = [&](auto kernel, size_t lds) {
-        hipLaunchKernelGGL(kernel, dim3(total), dim3(256), lds, ctx->stream, g, total, from, last);
+        hipLaunchKernelGGL(kernel, dim3(total), dim3(256), lds, ctx->stream, kept, total, from, last);
     };
     if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>);
     else if (tile == 96) launch(product_kernel<STAGE, KIND, 3>, sizeof(_Float16) * BUFFERS<3> * STAGE_HALVES<3>);
@@ -524,31 +718,43 @@ void product(const mrl_ctx *ctx, const Group &g, int total, int from, int last) 
 }
 
 template <int KIND>
-void run(const mrl_ctx *ctx, Group &g, int steps) {
+void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
+    size_t used = GROUP_BYTES;
+    Group *kept = (Group *)workspace;
+    size_t lds;
+    const bool whole = is_whole(g.mat, g.count, lds);
+    const int threads = whole ? 1024 : 256;
+    int sums = 0, rest = 0;
+    for (int k = 0; k < g.count; ++k) {
+        set_up(g.mat[k], whole ? 32 : 64, used);   // (a whole group's planes are in LDS: there is no workspace)
+        g.mat[k].begin_sums = sums;
+        sums += g.mat[k].sums;
+    }
+    g.total_sums = sums;
+    for (int k = 0; k < g.rests; ++k) {
+        g.rest[k].begin = rest;
+        rest += grid_for(g.rest[k].n, threads);
+    }
+    if (whole) {
+        hipLaunchKernelGGL(whole_kernel<KIND>, dim3(g.count + rest), dim3(threads), lds, ctx->stream, g, steps);
+        return;
+    }
     g.sym_tile = tile_of(ctx, g, true);
     g.update_tile = tile_of(ctx, g, false);
-    int sums = 0, load = 0, sym = 0, update = 0;
+    int load = 0, sym = 0, update = 0;
     for (int k = 0; k < g.count; ++k) {
         Mat &m = g.mat[k];
         const int a = (m.mp + g.sym_tile - 1) / g.sym_tile;
-        m.begin_sums = sums; sums += m.sums;
         m.begin_load = load; load += (m.mp / LOAD) * (m.np / LOAD);
         m.begin_sym = sym; sym += a * (a + 1) / 2;
         m.begin_update = update; update += ((m.mp + g.update_tile - 1) / g.update_tile) * ((m.np + g.update_tile - 1) / g.update_tile);
     }
-    g.total_sums = sums;
-    int rest = 0;
-    for (int k = 0; k < g.rests; ++k) {
-        g.rest[k].begin = rest;
-        rest += grid_for(g.rest[k].n, 256);
-    }
-    if (sums + rest > 0) hipLaunchKernelGGL(sums_kernel<KIND>, dim3(sums + rest), dim3(256), 0, ctx->stream, g);
-    if (g.count == 0) return;
-    hipLaunchKernelGGL(load_kernel<KIND>, dim3(load), dim3(256), 0, ctx->stream, g);
+    hipLaunchKernelGGL(sums_kernel<KIND>, dim3(sums + rest), dim3(threads), 0, ctx->stream, g, kept);
+    hipLaunchKernelGGL(load_kernel<KIND>, dim3(load), dim3(256), 0, ctx->stream, kept);
     for (int s = 0; s < steps; ++s) {
-        product<GRAM, KIND>(ctx, g, sym, s & 1, 0);
-        product<SQUARE, KIND>(ctx, g, sym, s & 1, 0);
-        product<UPDATE, KIND>(ctx, g, update, s & 1, s == steps - 1);
+        product<GRAM, KIND>(ctx, g, kept, sym, s & 1, 0);
+        product<SQUARE, KIND>(ctx, g, kept, sym, s & 1, 0);
+        product<UPDATE, KIND>(ctx, g, kept, update, s & 1, s == steps - 1);
     }
 }
 
@@ -593,7 +799,7 @@ int mrl_orthogonalize_workspace(int count, int rows, int cols, uint64_t *bytes) 
     MRL_CHECK_ARG(bytes && count >= 0, "%s: bad arguments", who);
     const int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK) return rc;
-    *bytes = mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST);
+    *bytes = mrl::batch_bytes(count, rows, cols);
     return MRL_OK;
 }
 
@@ -607,7 +813,7 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK || count == 0) return rc;
     MRL_CHECK_ARG(in && out, "%s: NULL buffer", who);
-    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::matrix_bytes(rows, cols) * std::min(count, mrl::MOST));
+    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::batch_bytes(count, rows, cols));
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
     const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
@@ -615,14 +821,13 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
         mrl::Group g = {};
         g.eps = eps;
         g.count = std::min(mrl::MOST, count - done);
-        char *ws = (char *)workspace;
         for (int k = 0; k < g.count; ++k) {
-            mrl::set_up(g.mat[k], rows, cols, ws);
+            mrl::sides(g.mat[k], rows, cols);
             g.mat[k].in = (const char *)in + (done + k) * one;
             g.mat[k].out = (char *)out + (done + k) * one;
         }
-        if (dtype == MRL_F32) mrl::run<mrl::F32>(ctx, g, steps);
-        else mrl::run<mrl::BF16>(ctx, g, steps);
+        if (dtype == MRL_F32) mrl::run<mrl::F32>(ctx, g, steps, workspace);
+        else mrl::run<mrl::BF16>(ctx, g, steps, workspace);
         MRL_CHECK_LAUNCH();
     }
     return MRL_OK;
@@ -635,9 +840,7 @@ int mrl_muon_workspace(int n_matrices, const mrl_matrix *matrices, uint64_t *byt
     if (rc != MRL_OK) return rc;
     *bytes = 0;
     for (int done = 0; done < n_matrices; done += mrl::MOST) {
-        uint64_t group = 0;
-        for (int k = done; k < std::min(n_matrices, done + mrl::MOST); ++k) group += mrl::matrix_bytes(matrices[k].rows, matrices[k].cols);
-        *bytes = std::max(*bytes, group);
+        *bytes = std::max<uint64_t>(*bytes, mrl::group_bytes(matrices + done, std::min(mrl::MOST, n_matrices - done)));
     }
     return MRL_OK;
 }
@@ -671,7 +874,6 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         g.adam_eps = (float)adam_eps;
         g.bc1 = (float)(1.0 - pow(beta1, (double)t)); g.bc2 = (float)(1.0 - pow(beta2, (double)t));
         g.count = std::min(mrl::MOST, n_matrices - done);
-        char *ws = (char *)workspace;
         auto rest = [&](int64_t to) {
             if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at), 0};
         };
@@ -679,7 +881,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
             const mrl_matrix &x = matrices[done + k];
             mrl::Mat &m = g.mat[k];
             rest(x.offset);
-            mrl::set_up(m, x.rows, x.cols, ws);
+            mrl::sides(m, x.rows, x.cols);
             m.in = grads + x.offset;
             m.out = params + x.offset;
             m.momentum = state + 2 * x.offset;
@@ -688,7 +890,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         }
         done += g.count;
         if (done >= n_matrices) rest(n);
-        mrl::run<mrl::MUON>(ctx, g, steps);
+        mrl::run<mrl::MUON>(ctx, g, steps, workspace);
         MRL_CHECK_LAUNCH();
     } while (done < n_matrices);
     return MRL_OK;

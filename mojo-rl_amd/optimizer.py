@@ -3,6 +3,7 @@
 else by Adam.  `t` and `lr` live on the host object, as in the reference (the PPO agent anneals `lr` between rollouts); state is
 [PARAM_SIZE, 2] interleaved (m, v)."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -25,28 +26,38 @@ class Adam:
                   self.t, self.lr, self.beta1, self.beta2, self.eps)
 
 
+_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+@functools.lru_cache(maxsize=None)
+def _orthogonalize_bytes(count, rows, cols):
+    size = C.c_uint64(0)
+    _lib.call("mrl_orthogonalize_workspace", count, rows, cols, C.byref(size))
+    return size.value
+
+
 def orthogonalize(ctx, out, x, steps=5, eps=1e-7):
     """out = the Newton-Schulz polynomial of x [rows, cols] or of every matrix of x [count, rows, cols]: x / (|x| + eps), then `steps`
     times X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X, which takes the singular values into about [0.7, 1.2].  float32 or
     bfloat16, contiguous; out may be x."""
-    if x.dim() not in (2, 3) or x.dtype not in (torch.float32, torch.bfloat16):
+    shape, kind = x.shape, _TYPES.get(x.dtype)
+    if len(shape) not in (2, 3) or kind is None:
         raise _lib.MrlError("orthogonalize: a float32 or bfloat16 [rows, cols] or [count, rows, cols] tensor expected, got %s of %s"
-                            % (list(x.shape), x.dtype))
-    if out.shape != x.shape or out.dtype != x.dtype:
-        raise _lib.MrlError("orthogonalize: out %s of %s does not fit x %s of %s" % (list(out.shape), out.dtype, list(x.shape), x.dtype))
-    _on_device(ctx, "x", x)
-    _on_device(ctx, "out", out)
+                            % (list(shape), x.dtype))
+    if out.shape != shape or out.dtype is not x.dtype:
+        raise _lib.MrlError("orthogonalize: out %s of %s does not fit x %s of %s" % (list(out.shape), out.dtype, list(shape), x.dtype))
+    if x.device != ctx.device or out.device != ctx.device:
+        _on_device(ctx, "x", x)
+        _on_device(ctx, "out", out)
     if not (x.is_contiguous() and out.is_contiguous()):
         raise _lib.MrlError("orthogonalize: x and out must be contiguous")
-    count = x.shape[0] if x.dim() == 3 else 1
-    rows, cols = x.shape[-2:]
+    count, rows, cols = shape if len(shape) == 3 else (1, *shape)
     if count * rows * cols == 0:
         return
-    size = C.c_uint64(0)
-    _lib.call("mrl_orthogonalize_workspace", count, rows, cols, C.byref(size))
-    ws = _scratch(ctx, size.value)
-    _lib.call("mrl_orthogonalize", ctx.handle, _lib.F32 if x.dtype == torch.float32 else _lib.BF16, count, rows, cols, x.data_ptr(),
-              out.data_ptr(), steps, eps, ws.data_ptr(), size.value)
+    n = _orthogonalize_bytes(count, rows, cols)
+    ws = _scratch(ctx, n) if n else None
+    _lib.call("mrl_orthogonalize", ctx.handle, kind, count, rows, cols, x.data_ptr(), out.data_ptr(), steps, eps,
+              ws.data_ptr() if n else None, n)
 
 
 class Muon:
@@ -83,10 +94,11 @@ class Muon:
     def step_gpu(self, ctx, params_buf, grads_buf, state_buf):
         n = self._n
         for name, t, want in (("params", params_buf, n), ("grads", grads_buf, n), ("state", state_buf, 2 * n)):
-            if t.numel() != want or t.dtype != torch.float32:
+            if t.numel() != want or t.dtype is not torch.float32:
                 raise _lib.MrlError("Muon.step_gpu: %s must be %d floats, got %d of %s" % (name, want, t.numel(), t.dtype))
-            _on_device(ctx, name, t)
-        ws = _scratch(ctx, self._bytes)
+            if t.device != ctx.device:
+                _on_device(ctx, name, t)
+        ws = _scratch(ctx, self._bytes) if self._bytes else None
         _lib.call("mrl_muon_step", ctx.handle, _ptr(params_buf), _ptr(grads_buf), _ptr(state_buf), n, self._count, self._matrices,
                   self.t + 1, self.lr, self.momentum, int(self.nesterov), self.weight_decay, self.steps, self.eps, self.adam_lr, self.beta1,
                   self.beta2, self.adam_eps, ws.data_ptr() if self._bytes else None, self._bytes)

@@ -54,7 +54,7 @@ def near(got, x, half, what, steps=5, eps=1e-7):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 50), (70, 1), (2, 2), (3, 4), (8, 256), (256, 4), (64, 64), (63, 65), (65, 63), (128, 128), (129, 127),
-                                       (40, 600), (600, 40), (256, 256), (300, 777), (777, 333), (130, 1030), (513, 512)])
+                                       (40, 600), (600, 40), (256, 256), (300, 777), (777, 333), (130, 1030), (513, 512), (1, 640), (33, 600), (96, 96), (97, 96), (64, 256), (257, 64)])
 def test_orthogonalize(mrl, ctx, rows, cols, dtype):
     print("orthogonalize", rows, cols, dtype, flush=True)
     x = matrix(torch.Generator().manual_seed(rows * 1000 + cols), rows, cols).to(TYPES[dtype])
@@ -236,12 +236,14 @@ def test_captured_graphs_keep_their_workspaces(mrl, ctx):
 
 
 def test_library_refusals(mrl, ctx):
-    lib, x = mrl._lib.lib(), torch.zeros(1 << 16, device="cuda")
-    p, size = ctypes.c_void_p(x.data_ptr()), ctypes.c_uint64(0)
-    assert lib.mrl_orthogonalize_workspace(1, 8, 8, ctypes.byref(size)) == 0 and size.value <= 1 << 18
+    lib, size = mrl._lib.lib(), ctypes.c_uint64(0)
+    assert lib.mrl_orthogonalize_workspace(1, 130, 8, ctypes.byref(size)) == 0 and size.value == 0
+    x, y = torch.zeros(1 << 20, device="cuda"), torch.zeros(130 * 150, device="cuda")
+    p, q = ctypes.c_void_p(x.data_ptr()), ctypes.c_void_p(y.data_ptr())
+    assert lib.mrl_orthogonalize_workspace(1, 130, 150, ctypes.byref(size)) == 0 and 0 < size.value <= 1 << 22
 
-    def orth(dtype=0, count=1, rows=8, cols=8, src=p, steps=5, eps=1e-7, ws=p, n=size.value):
-        return lib.mrl_orthogonalize(ctx.handle, dtype, count, rows, cols, src, p, steps, eps, ws, n)
+    def orth(dtype=0, count=1, rows=130, cols=150, src=q, steps=5, eps=1e-7, ws=p, n=size.value):
+        return lib.mrl_orthogonalize(ctx.handle, dtype, count, rows, cols, src, q, steps, eps, ws, n)
     for bad, text in ((dict(dtype=5), b"element type"), (dict(count=-1), b"count"), (dict(rows=0), b"sides"), (dict(cols=40000), b"sides"),
                       (dict(src=None), b"NULL"), (dict(steps=0), b"steps"), (dict(steps=65), b"steps"), (dict(eps=-1.0), b"eps"),
                       (dict(eps=float("nan")), b"eps"), (dict(n=size.value - 1), b"workspace holds"), (dict(ws=None), b"workspace holds"),
@@ -249,12 +251,12 @@ def test_library_refusals(mrl, ctx):
         assert orth(**bad) == -1 and text in lib.mrl_last_error(), bad
     Matrix = mrl._lib.Matrix
 
-    def muon(mats=((0, 4, 4),), n=100, t=1, steps=5, params=p, ws=p, size=1 << 18):
+    def muon(mats=((0, 4, 4),), n=40000, t=1, steps=5, params=p, ws=p, size=1 << 18):
         array = (Matrix * max(1, len(mats)))(*[Matrix(*m) for m in mats])
         return lib.mrl_muon_step(ctx.handle, params, p, p, n, len(mats), array, t, 0.1, 0.9, 1, 0.0, steps, 1e-7, 1e-3, 0.9, 0.99, 1e-8, ws, size)
-    for bad, text in ((dict(mats=((0, 4, 4), (15, 4, 4))), b"overlaps"), (dict(mats=((90, 4, 4),)), b"overlaps"), (dict(mats=((-1, 4, 4),)), b"overlaps"),
+    for bad, text in ((dict(mats=((0, 4, 4), (15, 4, 4))), b"overlaps"), (dict(mats=((39990, 4, 4),)), b"overlaps"), (dict(mats=((-1, 4, 4),)), b"overlaps"),
                       (dict(mats=((0, 0, 4),)), b"sides"), (dict(n=-1), b"n <"), (dict(t=0), b"step count"), (dict(steps=0), b"steps"), (dict(params=None), b"NULL"),
-                      (dict(size=100), b"workspace holds")):
+                      (dict(mats=((0, 130, 150),), size=100), b"workspace holds")):
         assert muon(**bad) == -1 and text in lib.mrl_last_error(), bad
     ctx.synchronize()
     assert not x.any()

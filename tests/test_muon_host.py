@@ -55,8 +55,10 @@ def test_muon_step_refuses(mrl):
 
 def test_null_contexts_and_workspace_queries(mrl):
     size = ctypes.c_uint64(0)
-    mrl._lib.call("mrl_orthogonalize_workspace", 3, 100, 40, ctypes.byref(size))
-    assert size.value >= 3 * (6 * 2 * 40 * 100 + 4 * 2 * 40 * 40)
+    mrl._lib.call("mrl_orthogonalize_workspace", 3, 400, 340, ctypes.byref(size))
+    assert size.value >= 3 * (6 * 2 * 340 * 400 + 4 * 2 * 340 * 340)
+    mrl._lib.call("mrl_orthogonalize_workspace", 3, 40, 30, ctypes.byref(size))
+    assert size.value == 0   # (held in LDS)
     mrl._lib.call("mrl_muon_workspace", 0, None, ctypes.byref(size))
     assert size.value == 0
     for name, args in (("mrl_orthogonalize", (None, 0, 1, 4, 4, None, None, 5, 1e-7, None, 0)),
