@@ -16,6 +16,7 @@
 // contracted index, the 64 lanes' operands of v_mfma_f32_16x16x32_f16 in lane order, 1 KiB of hi and 1 KiB of lo next to
 // each other: loads are whole and in order.  Element (row r, index k): lane 16 ((k % 32) / 8) + r % 16, k % 8.
 // The sides are padded to multiples of 64 with zeros, which the products keep zero.
+#include <limits.h>
 #include <cmath>
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
@@ -30,7 +31,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr float QA = 3.4445f, QB = -4.7750f, QC = 2.0315f;
 constexpr int MOST = 16;        // matrices of a launch
 constexpr int LOAD = 32;        // sides of what a workgroup of the second launch takes
-constexpr int CHUNK = 4096;     // elements that a workgroup of the first launch takes at a time
+constexpr int CHUNK = 1024;     // elements that a workgroup of the first launch takes at a time
 constexpr int MOST_SUMS = 1024;  // partial sums of squares per matrix
 
 struct bf16_t { unsigned short bits; };
@@ -41,17 +42,17 @@ struct Mat {
     float *momentum;
     int rows, cols, m, n, mp, np;   // the caller's sides; the shorter and the longer one, and both padded
     int tall;                       // rows > cols: X is the transpose
-    int sums, begin_sums, begin_load, begin_sym, begin_update;   // workgroups of each launch
+    int sums;                       // partial sums of squares
     float sx;                       // what X is stored times; A and B: sa
     float gram, square, update, result;   // sums to A, A A to B, B X to X, X to the caller: sa / sx^2, c / sa, 1 / sa, 1 / sx
     float factor;                   // of the update
     size_t x, xt, xt1, a, b, partial; // planes and partial sums: bytes from the workspace's start
 };
-struct Rest { float *p; const float *g; float2 *state; long n; int begin; };   // parameters that Adam updates
+struct Rest { float *p; const float *g; float2 *state; long n; };   // parameters that Adam updates
 struct Group {
     int count, rests;
     int sym_tile, update_tile;   // sides of the products' tiles
-    int total_sums;
+    int begin_sym[MOST], begin_update[MOST];   // a matrix's first tile among all; none: INT_MAX
     Mat mat[MOST];
     Rest rest[MOST + 1];
     double eps;
@@ -97,28 +98,27 @@ MRL_DEV double square_of(const Group &g, const Mat &m, size_t i) {
     const double x = source<KIND, true>(g, m, i);
     return x * x;
 }
-// Adam on the parameters between the matrices
-MRL_DEV void adam_rest(const Group &g, int block, int threads) {
-    int k = 0;
-    while (k + 1 < g.rests && block >= g.rest[k + 1].begin) ++k;
-    const Rest &r = g.rest[k];
-    const long i = (long)(block - r.begin) * threads + threadIdx.x;
-    if (i < r.n) adam_one(r.p[i], r.g[i], r.state[i], g.lr, g.beta1, g.beta2, g.omb1, g.omb2, g.adam_eps, g.bc1, g.bc2);
+// Adam on the parameters between the matrices, by workgroup `block` of `blocks`
+MRL_DEV void adam_rest(const Group &g, int block, int blocks) {
+    for (int k = 0; k < g.rests; ++k) {
+        const Rest &r = g.rest[k];
+        for (long i = (long)block * blockDim.x + threadIdx.x; i < r.n; i += (long)blocks * blockDim.x)
+            adam_one(r.p[i], r.g[i], r.state[i], g.lr, g.beta1, g.beta2, g.omb1, g.omb2, g.adam_eps, g.bc1, g.bc2);
+    }
 }
 // Sums of squares of every matrix, in 64 bits and a fixed order, and Adam.  The group's description, 3 KiB of arguments that cost the
 // host 1.5 us a launch, goes to the workspace, where the launches behind this one find it.
 template <int KIND>
 __global__ __launch_bounds__(256) void sums_kernel(Group g, Group *kept) {
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int i = threadIdx.x; i < (int)(sizeof(Group) / 4); i += 256) reinterpret_cast<int *>(kept)[i] = reinterpret_cast<const int *>(&g)[i];
-    if (KIND == MUON && (int)blockIdx.x >= g.total_sums) {
-        adam_rest(g, blockIdx.x - g.total_sums, 256);
+    if (KIND == MUON && (int)blockIdx.y == g.count) {
+        adam_rest(g, blockIdx.x, gridDim.x);
         return;
     }
-    int k = 0;
-    while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_sums) ++k;
-    const Mat &m = g.mat[k];
-    const int block = blockIdx.x - m.begin_sums;
+    const Mat &m = g.mat[blockIdx.y];
+    const int block = blockIdx.x;
+    if (block >= m.sums) return;
     const size_t size = (size_t)m.rows * m.cols;
     double sum = 0.0;
 #pragma unroll 4
@@ -194,10 +194,8 @@ __global__ __launch_bounds__(256) void load_kernel(const Group *__restrict__ gro
     const Group &g = *group;
     __shared__ double part[256];
     __shared__ float tile[LOAD][LOAD + 1];
-    int k = 0;
-    while (k + 1 < g.count && (int)blockIdx.x >= g.mat[k + 1].begin_load) ++k;
-    const Mat m = described(g.mat[k]);
-    load_square<KIND>(g, m, blockIdx.x - m.begin_load, scale_of(g, m, part), tile);
+    const Mat m = described(g.mat[blockIdx.y]);
+    if ((int)blockIdx.x < m.mp / LOAD * (m.np / LOAD)) load_square<KIND>(g, m, blockIdx.x, scale_of(g, m, part), tile);
 }
 
 // 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
@@ -225,25 +223,28 @@ MRL_DEV void above_diagonal(int tile, int &bi, int &bj) {
     bi = tile - bj * (bj + 1) / 2;
 }
 
-// Which tile of which matrix a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles that
-// share operands, so that its L2 is read more often than what is behind it.
+// Which of `tiles` tiles, of which matrix, a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of
+// tiles that share operands, so that its L2 is read more often than what is behind it (every matrix on every XCD instead: eight of 777 x 333
+// 212 us for 177).  All first tiles are looked at, from one scalar load, not one after the other.
 template <int STAGE, int TILE>
-MRL_DEV Mat find_tile(const Group &g, int total, int &bi, int &bj) {
-    const int xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-    const int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
-    int k = 0;
+MRL_DEV Mat find_tile(const Group &g, int count, int tiles, int &bi, int &bj) {
+    const int xcd = blockIdx.x & 7, each = tiles >> 3, more = tiles & 7;
+    int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3), k = 0;
+    if (count > 1) {
+        const int(&begin)[MOST] = STAGE == UPDATE ? g.begin_update : g.begin_sym;
+#pragma unroll
+        for (int i = 1; i < MOST; ++i) k += id >= begin[i];
+        id -= begin[k];
+    }
+    const Mat m = described(g.mat[k]);
     if (STAGE == UPDATE) {
-        while (k + 1 < g.count && id >= g.mat[k + 1].begin_update) ++k;
-        const Mat m = described(g.mat[k]);
-        const int block = id - m.begin_update, rows = (m.mp + TILE - 1) / TILE, panel = __builtin_amdgcn_readfirstlane(block / (4 * rows)), in = block - panel * 4 * rows;
+        const int rows = (m.mp + TILE - 1) / TILE, panel = __builtin_amdgcn_readfirstlane(id / (4 * rows)), in = id - panel * 4 * rows;
         const int width = min(4, (m.np + TILE - 1) / TILE - 4 * panel);   // panels of four columns, row by row
         bi = __builtin_amdgcn_readfirstlane(in / width);
         bj = 4 * panel + in - bi * width;
-        return m;
+    } else {
+        above_diagonal(id, bi, bj);
     }
-    while (k + 1 < g.count && id >= g.mat[k + 1].begin_sym) ++k;
-    const Mat m = described(g.mat[k]);
-    above_diagonal(id - m.begin_sym, bi, bj);
     return m;
 }
 
@@ -341,12 +342,12 @@ MRL_DEV void meet() {
 template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
 template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
 template <int STAGE, int KIND, int F>
-__global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ group, int total, int from, int last) {
+__global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
     constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, LOADS = 2 * F;
     extern __shared__ _Float16 lds[];
     int bi, bj;
-    const Mat m = find_tile<STAGE, 32 * F>(g, total, bi, bj);
+    const Mat m = find_tile<STAGE, 32 * F>(g, count, tiles, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(g, m, from, P, Q, blocks);
@@ -505,11 +506,11 @@ MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int fro
     finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
 }
 template <int STAGE, int KIND>
-__global__ __launch_bounds__(256) void small_product_kernel(const Group *__restrict__ group, int total, int from, int last) {
+__global__ __launch_bounds__(256) void small_product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
     __shared__ SmallSums sums;
     int bi, bj;
-    const Mat m = find_tile<STAGE, 32>(g, total, bi, bj);
+    const Mat m = find_tile<STAGE, 32>(g, count, tiles, bi, bj);
     small_product<STAGE, KIND>(g, m, bi, bj, from, last, sums);
 }
 
@@ -538,7 +539,7 @@ template <int KIND>
 __global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
     extern __shared__ _Float16 lds[];
     if (KIND == MUON && (int)blockIdx.x >= g.count) {
-        adam_rest(g, blockIdx.x - g.count, 1024);
+        adam_rest(g, blockIdx.x - g.count, gridDim.x - g.count);
         return;
     }
     const Mat &m = g.mat[blockIdx.x];
@@ -706,10 +707,10 @@ void sides(Mat &m, int rows, int cols) {
 }
 
 template <int STAGE, int KIND>
-void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int total, int from, int last) {
+void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int tiles, int from, int last) {
     const int tile = STAGE == UPDATE ? g.update_tile : g.sym_tile;
     auto launch = [&](auto kernel, size_t lds) {
-        hipLaunchKernelGGL(kernel, dim3(total), dim3(256), lds, ctx->stream, kept, total, from, last);
+        hipLaunchKernelGGL(kernel, dim3(tiles), dim3(256), lds, ctx->stream, kept, g.count, tiles, from, last);
     };
     if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>);
     else if (tile == 96) launch(product_kernel<STAGE, KIND, 3>, sizeof(_Float16) * BUFFERS<3> * STAGE_HALVES<3>);
@@ -724,33 +725,34 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
     size_t lds;
     const bool whole = is_whole(g.mat, g.count, lds);
     const int threads = whole ? 1024 : 256;
-    int sums = 0, rest = 0;
+    int sums = 1;
     for (int k = 0; k < g.count; ++k) {
         set_up(g.mat[k], whole ? 32 : 64, used);   // (a whole group's planes are in LDS: there is no workspace)
-        g.mat[k].begin_sums = sums;
-        sums += g.mat[k].sums;
+        sums = std::max(sums, g.mat[k].sums);
     }
-    g.total_sums = sums;
-    for (int k = 0; k < g.rests; ++k) {
-        g.rest[k].begin = rest;
-        rest += grid_for(g.rest[k].n, threads);
-    }
+    long rest = 0;
+    for (int k = 0; k < g.rests; ++k) rest += g.rest[k].n;
+    rest = std::min<long>(2048, (rest + threads - 1) / threads);
     if (whole) {
         hipLaunchKernelGGL(whole_kernel<KIND>, dim3(g.count + rest), dim3(threads), lds, ctx->stream, g, steps);
         return;
     }
     g.sym_tile = tile_of(ctx, g, true);
     g.update_tile = tile_of(ctx, g, false);
-    int load = 0, sym = 0, update = 0;
+    std::fill(g.begin_sym, g.begin_sym + MOST, INT_MAX);
+    std::fill(g.begin_update, g.begin_update + MOST, INT_MAX);
+    int load = 0, sym = 0, update = 0;   // squares of the largest matrix, tiles of all
     for (int k = 0; k < g.count; ++k) {
-        Mat &m = g.mat[k];
+        const Mat &m = g.mat[k];
         const int a = (m.mp + g.sym_tile - 1) / g.sym_tile;
-        m.begin_load = load; load += (m.mp / LOAD) * (m.np / LOAD);
-        m.begin_sym = sym; sym += a * (a + 1) / 2;
-        m.begin_update = update; update += ((m.mp + g.update_tile - 1) / g.update_tile) * ((m.np + g.update_tile - 1) / g.update_tile);
+        load = std::max(load, m.mp / LOAD * (m.np / LOAD));
+        g.begin_sym[k] = sym;
+        sym += a * (a + 1) / 2;
+        g.begin_update[k] = update;
+        update += ((m.mp + g.update_tile - 1) / g.update_tile) * ((m.np + g.update_tile - 1) / g.update_tile);
     }
-    hipLaunchKernelGGL(sums_kernel<KIND>, dim3(sums + rest), dim3(threads), 0, ctx->stream, g, kept);
-    hipLaunchKernelGGL(load_kernel<KIND>, dim3(load), dim3(256), 0, ctx->stream, kept);
+    hipLaunchKernelGGL(sums_kernel<KIND>, dim3(std::max<long>(sums, rest), g.count + (rest > 0)), dim3(threads), 0, ctx->stream, g, kept);
+    hipLaunchKernelGGL(load_kernel<KIND>, dim3(load, g.count), dim3(256), 0, ctx->stream, kept);
     for (int s = 0; s < steps; ++s) {
         product<GRAM, KIND>(ctx, g, kept, sym, s & 1, 0);
         product<SQUARE, KIND>(ctx, g, kept, sym, s & 1, 0);
@@ -875,7 +877,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         g.bc1 = (float)(1.0 - pow(beta1, (double)t)); g.bc2 = (float)(1.0 - pow(beta2, (double)t));
         g.count = std::min(mrl::MOST, n_matrices - done);
         auto rest = [&](int64_t to) {
-            if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at), 0};
+            if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at)};
         };
         for (int k = 0; k < g.count; ++k) {
             const mrl_matrix &x = matrices[done + k];
