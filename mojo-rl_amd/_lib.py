@@ -182,15 +182,21 @@ def check(rc, what):
         raise MrlError("%s failed (%d): %s" % (what, rc, lib().mrl_last_error().decode()))
 
 
-def call(name, *args):
+_functions = {}   # looked up once: name -> (function, whether it returns a count)
+
+
+def _function(name):
     if name in lib()._mrl_missing:
         raise MrlError("%s is not exported by %s" % (name, LIB_PATH))
-    rc = getattr(lib(), name)(*args)
-    if name in _RAW_INT:
-        if rc < 0:
-            check(rc, name)
-        return rc
-    check(rc, name)
+    found = _functions[name] = getattr(lib(), name), name in _RAW_INT
+    return found
+
+
+def call(name, *args):
+    function, raw = _functions.get(name) or _function(name)
+    rc = function(*args)
+    if rc != 0 and not (raw and rc > 0):
+        check(rc, name)
     return rc
 
 

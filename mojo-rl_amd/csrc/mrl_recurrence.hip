@@ -541,17 +541,17 @@ void channels(Plan &p, int V, int N, int D) {
 Plan plan_of(const mrl_ctx *ctx, int T, int N, int D, int size) {
     Plan p = {};
     const long want = 8L * ctx->n_cus;   // wavefronts
-    constexpr int SHARE = 16;            // steps that a wavefront of a segment has at least
+    constexpr long SHARE = 16;            // steps that a wavefront of a segment has at least
     channels(p, 4, N, D);
     p.W = 1;
     p.segments = 1;
     if (T >= 512 && (long)p.groups * size * 2 < ctx->n_cus) {
         if ((long)p.groups * T < SHARE * want) channels(p, 2, N, D);
-        const long shares = std::min<long>((T + SHARE - 1) / SHARE, std::max<long>(2 * MAX_WAVES, want / p.groups));
+        const long shares = std::min<long>(((long)T + SHARE - 1) / SHARE, std::max<long>(2 * MAX_WAVES, want / p.groups));
         p.W = MAX_WAVES;
         p.share = (int)((T + shares - 1) / shares);
         p.segment_steps = p.share * p.W;
-        p.segments = (T + p.segment_steps - 1) / p.segment_steps;
+        p.segments = (int)(((long)T + p.segment_steps - 1) / p.segment_steps);
         p.bytes = sizeof(float) * (size_t)p.lanes * p.V * (2 * (size_t)p.segments * (p.W + 1) + 1);
         return p;
     }

@@ -89,7 +89,8 @@ class GatedRecurrence:
         v, v_ld = self._rows(ctx, "value", value, size, kind)
         o, o_ld = self._rows(ctx, "output", output, size, kind)
         flags, before = self._flat(ctx, "dones", dones, rows), self._flat(ctx, "prev_dones", prev_dones, envs)
-        s_in, s_out = self._flat(ctx, "state_in", state_in, states), self._flat(ctx, "state_out", state_out, states)
+        s_in = self._flat(ctx, "state_in", state_in, states)
+        s_out = s_in if state_out is state_in else self._flat(ctx, "state_out", state_out, states)
         ws, ws_ptr, ws_bytes = self._workspace(ctx, steps, envs)
         _lib.call("mrl_recurrence_forward", ctx.handle, dtype, steps, envs, self.width, g, g_ld, v, v_ld, flags, before, s_in, o, o_ld,
                   s_out, ws_ptr, ws_bytes)
