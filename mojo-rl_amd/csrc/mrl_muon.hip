@@ -336,15 +336,17 @@ MRL_DEV void meet() {
 
 // One product, a tile of 32 F x 32 F per workgroup.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric, so only tiles on and
 // above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
-// Four wavefronts share the tile, 16 F x 16 F each.  Operands go from memory to LDS past the registers, a stage of 32 of the
+// Four wavefronts share the tile, 16 F x 16 F each; that of 128 eight, 64 x 32 each: two on a SIMD hand over their requests while the
+// other multiplies (five steps of 2048 x 2048 570 us for 607, of four of 1024 x 1024 379 for 439).  Operands go from memory to LDS past the registers, a stage of 32 of the
 // contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less time than memory takes to answer.
 // A tile at the edge reads the last rows' operands again where it has none of its own, and leaves what comes of them.
 template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
 template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
+template <int F> constexpr int WAVES = F == 4 ? 8 : 4;
 template <int STAGE, int KIND, int F>
-__global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
+__global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
-    constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, LOADS = 2 * F;
+    constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, ACROSS = WAVES<F> / 2, FP = F, FQ = SIDE / ACROSS, OWN = SIDE / ACROSS, LOADS = 2 * OWN;
     extern __shared__ _Float16 lds[];
     int bi, bj;
     const Mat m = find_tile<STAGE, 32 * F>(g, count, tiles, bi, bj);
@@ -352,59 +354,59 @@ __global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ 
     int blocks;
     operands<STAGE>(g, m, from, P, Q, blocks);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // wavefronts 0 and 1 bring in P, the others Q, F fragments each
-    const int operand = wave >> 1, fragments = ((operand && STAGE == UPDATE) ? m.np : m.mp) / 16;
-    const _Float16 *src[F];
+    // the first half of the wavefronts brings in P, the other Q, OWN fragments each
+    const int row = wave / ACROSS, column = wave % ACROSS, operand = row, fragments = ((operand && STAGE == UPDATE) ? m.np : m.mp) / 16;
+    const _Float16 *src[OWN];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
-        src[f] = (operand ? Q : P) + min((operand ? bj : bi) * SIDE + (wave & 1) * F + f, fragments - 1) * 1024 + lane * 8;
-    int in_at = wave * F * 1024;   // where in LDS the next stage goes
+    for (int f = 0; f < OWN; ++f)
+        src[f] = (operand ? Q : P) + min((operand ? bj : bi) * SIDE + column * OWN + f, fragments - 1) * 1024 + lane * 8;
+    int in_at = wave * OWN * 1024;   // where in LDS the next stage goes
     auto brought = [&]() {
 #pragma unroll
-        for (int f = 0; f < F; ++f) src[f] += fragments * 1024;
+        for (int f = 0; f < OWN; ++f) src[f] += fragments * 1024;
         in_at = in_at >= (AHEAD - 1) * STAGE_HALVES<F> ? in_at - (AHEAD - 1) * STAGE_HALVES<F> : in_at + STAGE_HALVES<F>;
     };
-    const int p = (wave >> 1) * F * 1024 + lane * 8, q = (SIDE + (wave & 1) * F) * 1024 + lane * 8;
+    const int p = row * FP * 1024 + lane * 8, q = (SIDE + column * FQ) * 1024 + lane * 8;
     int at = 0;   // of the stage that is worked on
     auto read = [&](int where) { return *reinterpret_cast<const f16x8 *>(lds + at + where); };
-    f32x4 acc[F][F] = {};
-    // A stage's 3 F F products in three groups.  The meeting behind which the next stage is there, and this one's buffer free, stands
+    f32x4 acc[FP][FQ] = {};
+    // A stage's 3 FP FQ products in three groups.  The meeting behind which the next stage is there, and this one's buffer free, stands
     // ahead of the last group.  Requests to LDS and memory go out among the products, at most one ahead of each: a wavefront takes 16
     // cycles or more to hand over either, in which the matrix cores would wait if they stood together.  A buffer that the meeting
     // freed is asked for from there to the next meeting: EARLY loads in the last group, the others in the next stage's first two.
-    constexpr int N = F * F, EARLY = F == 4 ? 2 : F == 3 ? 1 : 0;
+    constexpr int N = FP * FQ, READS = FP + FQ, EARLY = F == 4 ? 1 : F == 3 ? 1 : 0;
     auto request = [&](int load) {
         if (load % 2 == 0) bring<0>(src[load / 2], lds + in_at + load / 2 * 1024);
         else bring<1>(src[load / 2], lds + in_at + load / 2 * 1024);
     };
-    auto product = [&](int k, const f16x8 (&x)[F], const f16x8 (&y)[F]) {
-        acc[k / F][k % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[k / F], y[k % F], acc[k / F][k % F], 0, 0, 0);
+    auto product = [&](int k, const f16x8 (&x)[FP], const f16x8 (&y)[FQ]) {
+        acc[k / FQ][k % FQ] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[k / FQ], y[k % FQ], acc[k / FQ][k % FQ], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto first_groups = [&](f16x8 (&ph)[F], f16x8 (&pl)[F], f16x8 (&qh)[F], bool more) {
-        constexpr int FROM = 2 * F, STEP = (2 * N - FROM) / (LOADS - EARLY);
-        f16x8 ql[F];
+    auto first_groups = [&](f16x8 (&ph)[FP], f16x8 (&pl)[FP], f16x8 (&qh)[FQ], bool more) {
+        constexpr int STEP = (2 * N - READS) / (LOADS - EARLY);
+        f16x8 ql[FQ];
 #pragma unroll
         for (int k = 0; k < 2 * N; ++k) {
-            if (k < F) ql[k] = read(q + 512 + k * 1024);
-            else if (k < 2 * F) ph[k - F] = read(p + (k - F) * 1024);
-            else if ((k - FROM) % STEP == 0 && (k - FROM) / STEP < LOADS - EARLY && more) request(EARLY + (k - FROM) / STEP);
+            if (k < FQ) ql[k] = read(q + 512 + k * 1024);
+            else if (k < READS) ph[k - FQ] = read(p + (k - FQ) * 1024);
+            else if ((k - READS) % STEP == 0 && (k - READS) / STEP < LOADS - EARLY && more) request(EARLY + (k - READS) / STEP);
             if (k < N) product(k, pl, qh);
             else product(k - N, ph, ql);
         }
         if (more) brought();
     };
-    auto last_group = [&](f16x8 (&ph)[F], f16x8 (&pl)[F], f16x8 (&qh)[F], f16x8 (&next)[F], bool more) {
+    auto last_group = [&](f16x8 (&ph)[FP], f16x8 (&pl)[FP], f16x8 (&qh)[FQ], f16x8 (&next)[FQ], bool more) {
         at = at == (AHEAD - 1) * STAGE_HALVES<F> ? 0 : at + STAGE_HALVES<F>;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (k < F) next[k] = read(q + k * 1024);
-            else if (k < 2 * F) pl[k - F] = read(p + 512 + (k - F) * 1024);
-            else if ((k - 2 * F) % 3 == 1 && (k - 2 * F) / 3 < EARLY && more) request((k - 2 * F) / 3);
+            if (k < FQ) next[k] = read(q + k * 1024);
+            else if (k < READS) pl[k - FQ] = read(p + 512 + (k - FQ) * 1024);
+            else if ((k - READS) % 3 == 1 && (k - READS) / 3 < EARLY && more) request((k - READS) / 3);
             product(k, ph, qh);
         }
     };
-    f16x8 ph[F], pl[F], qa[F], qb[F];
+    f16x8 ph[FP], pl[FP], qa[FQ], qb[FQ];
     for (int s = 0; s < AHEAD - 1 && s < blocks; ++s) {
 #pragma unroll
         for (int load = 0; load < LOADS; ++load) request(load);
@@ -418,10 +420,9 @@ __global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ 
         meet<0>();
     }
 #pragma unroll
-    for (int f = 0; f < F; ++f) {
-        qa[f] = read(q + f * 1024);
-        pl[f] = read(p + 512 + f * 1024);
-    }
+    for (int f = 0; f < FQ; ++f) qa[f] = read(q + f * 1024);
+#pragma unroll
+    for (int f = 0; f < FP; ++f) pl[f] = read(p + 512 + f * 1024);
     // (the blocks are an even number: the sides are padded to 64)
     int s = 0;
     for (; s + 1 + AHEAD < blocks; s += 2) {
@@ -445,13 +446,13 @@ __global__ __launch_bounds__(256) void product_kernel(const Group *__restrict__ 
             for (int k = 0; k < N; ++k) product(k, ph, qb);
         }
     }
-    const int fi = (bi * SIDE + (wave >> 1) * F) * 16, fj = (bj * SIDE + (wave & 1) * F) * 16;
-    Piece pieces[F * F];
+    const int fi = (bi * SIDE + row * FP) * 16, fj = (bj * SIDE + column * FQ) * 16;
+    Piece pieces[N];
 #pragma unroll
-    for (int f = 0; f < F * F; ++f) ask<STAGE>(g, m, from, fi + 16 * (f / F), fj + 16 * (f % F), pieces[f]);
+    for (int f = 0; f < N; ++f) ask<STAGE>(g, m, from, fi + 16 * (f / FQ), fj + 16 * (f % FQ), pieces[f]);
 #pragma unroll
-    for (int f = 0; f < F * F; ++f)
-        finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / F), fj + 16 * (f % F), acc[f / F][f % F], pieces[f]);
+    for (int f = 0; f < N; ++f)
+        finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / FQ), fj + 16 * (f % FQ), acc[f / FQ][f % FQ], pieces[f]);
 }
 
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
@@ -648,9 +649,9 @@ size_t batch_bytes(int count, int rows, int cols) {
 
 // Sides of the tiles of a group's symmetric products, or of its updates: those of the least time by what products of one to sixteen
 // matrices of 256 to 2048 took, in us, K of the contracted index long (256 CUs; one workgroup per CU at 96 and 128):
-//   32: 5.0 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.015 + 0.009 share)
+//   32: 5.0 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.012 + 0.0095 share)
 // where share of the CUs have one; more of them get in each other's way at the caches.  Symmetric / update at 32, 64, 96, 128:
-//   256: 5 / 5, 6 / 7, 8 / 10, 10 / 13    1024: 11 / 15, 12 / 13, 17 / 20, 24 / 28    2048: 66 / 96, 49 / 67, 39 / 79, 47 / 58
+//   256: 5 / 5, 6 / 7, 8 / 10, 9 / 11    1024: 11 / 15, 12 / 13, 17 / 20, 19 / 21    2048: 66 / 96, 49 / 67, 38 / 78, 42 / 50
 int tile_of(const mrl_ctx *ctx, const Group &g, bool symmetric) {
     int best = 0;
     double least = 0.0;
@@ -665,7 +666,7 @@ int tile_of(const mrl_ctx *ctx, const Group &g, bool symmetric) {
         const double time = tile == 32   ? 5.0 + 11e-6 * 256 * per_cu * K
                             : tile == 64 ? 5.5 + 0.0072 * K * rounds
                             : tile == 96 ? 6.0 + K * rounds * (0.0105 + 0.006 * share)
-                                         : 7.0 + K * rounds * (0.015 + 0.009 * share);
+                                         : 7.0 + K * rounds * (0.012 + 0.0095 * share);
         if (best == 0 || time < least) {
             least = time;
             best = tile;
@@ -709,10 +710,10 @@ void sides(Mat &m, int rows, int cols) {
 template <int STAGE, int KIND>
 void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int tiles, int from, int last) {
     const int tile = STAGE == UPDATE ? g.update_tile : g.sym_tile;
-    auto launch = [&](auto kernel, size_t lds) {
-        hipLaunchKernelGGL(kernel, dim3(tiles), dim3(256), lds, ctx->stream, kept, g.count, tiles, from, last);
+    auto launch = [&](auto kernel, size_t lds, int threads = 256) {
+        hipLaunchKernelGGL(kernel, dim3(tiles), dim3(threads), lds, ctx->stream, kept, g.count, tiles, from, last);
     };
-    if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>);
+    if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>, 64 * WAVES<4>);
     else if (tile == 96) launch(product_kernel<STAGE, KIND, 3>, sizeof(_Float16) * BUFFERS<3> * STAGE_HALVES<3>);
     else if (tile == 64) launch(product_kernel<STAGE, KIND, 2>, sizeof(_Float16) * BUFFERS<2> * STAGE_HALVES<2>);
     else launch(small_product_kernel<STAGE, KIND>, 0);
