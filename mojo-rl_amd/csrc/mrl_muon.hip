@@ -106,7 +106,7 @@ MRL_DEV void adam_rest(const Group &g, int block, int blocks) {
             adam_one(r.p[i], r.g[i], r.state[i], g.lr, g.beta1, g.beta2, g.omb1, g.omb2, g.adam_eps, g.bc1, g.bc2);
     }
 }
-// Sums of squares of every matrix, in 64 bits and a fixed order, and Adam.  The group's description, 3 KiB of arguments that cost the
+// Sums of squares of every matrix, in 64 bits and a fixed order, and Adam (3.6 us for 256 x 256, 8 for 2048 x 2048, 2 TB/s).  The group's description, 3 KiB of arguments that cost the
 // host 1.5 us a launch, goes to the workspace, where the launches behind this one find it.
 template <int KIND>
 __global__ __launch_bounds__(256) void sums_kernel(Group g, Group *kept) {
@@ -167,7 +167,8 @@ MRL_DEV double scale_of(const Group &g, const Mat &m, double *part) {
     }
     return (double)m.sx / (sqrt(part[0]) + g.eps);
 }
-// A square of X and of its transpose in pieces, through LDS: read along the caller's rows, written along both sides.
+// A square of X and of its transpose in pieces, through LDS: read along the caller's rows, written along both sides (5.3 us for 256 x
+// 256, 17 for 2048 x 2048: 3 TB/s, a fortieth of the whole).
 template <int KIND>
 MRL_DEV void load_square(const Group &g, const Mat &m, int block, double scale, float (&tile)[LOAD][LOAD + 1]) {
     const int across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
@@ -224,8 +225,8 @@ MRL_DEV void above_diagonal(int tile, int &bi, int &bj) {
 }
 
 // Which of `tiles` tiles, of which matrix, a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of
-// tiles that share operands, so that its L2 is read more often than what is behind it (every matrix on every XCD instead: eight of 777 x 333
-// 212 us for 177).  All first tiles are looked at, from one scalar load, not one after the other.
+// tiles that share operands, so that its L2 is read more often than what is behind it (every matrix on every XCD instead: eight of
+// 777 x 333 212 us for 177).  All first tiles are looked at, from one scalar load, not one after the other.
 template <int STAGE, int TILE>
 MRL_DEV Mat find_tile(const Group &g, int count, int tiles, int &bi, int &bj) {
     const int xcd = blockIdx.x & 7, each = tiles >> 3, more = tiles & 7;
@@ -336,9 +337,13 @@ MRL_DEV void meet() {
 
 // One product, a tile of 32 F x 32 F per workgroup.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric, so only tiles on and
 // above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
-// Four wavefronts share the tile, 16 F x 16 F each; that of 128 eight, 64 x 32 each: two on a SIMD hand over their requests while the
-// other multiplies (five steps of 2048 x 2048 570 us for 607, of four of 1024 x 1024 379 for 439).  Operands go from memory to LDS past the registers, a stage of 32 of the
-// contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less time than memory takes to answer.
+// Four wavefronts share the tile, 16 F x 16 F each; that of 128 eight, 64 x 32 each: of two on a SIMD one hands over its requests while
+// the other multiplies (five steps of 2048 x 2048 570 us for 607, of four of 1024 x 1024 379 for 439).  Operands go from memory to LDS
+// past the registers, a stage of 32 of the contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less
+// time than memory takes to answer.
+// Bound by the matrix cores where there are tiles for all CUs: 2048 x 2048 in tiles of 128, an update takes 50 us, 1.0 PFLOP/s in fp16
+// (a large fp16 product of this card's library: 1.1); a symmetric product in tiles of 96 37, 0.8 PFLOP/s,
+// with one wavefront on a SIMD.  Fewer tiles are bound by the stages' way through LDS, 0.35 us each at 64.
 // A tile at the edge reads the last rows' operands again where it has none of its own, and leaves what comes of them.
 template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
 template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
@@ -456,7 +461,8 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
 }
 
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
-// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.
+// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.  256 x 256: 4.6, 4.8 and
+// 5.2 us for the three, most of it the launch and the trips to memory one behind the other (description, operands, sums).
 typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
 template <int STAGE, int KIND>
 MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums) {
@@ -516,9 +522,9 @@ __global__ __launch_bounds__(256) void small_product_kernel(const Group *__restr
 }
 
 // A small matrix by one workgroup in one launch, the optimiser's part included: all operands stay in LDS, sixteen wavefronts take
-// 16 x 16 sums each and meet behind every product.  64 x 64: TIME1 us instead of 75 in launches of their own, 64 x 128 TIME2
-// instead of 78, eleven of 216 x 10 TIME3 instead of 116.  (Operands out of the caches instead: 28, 43 and 30, bound by what a CU's L1
-// gives, and from 96 x 128 on longer than the launches.)
+// 16 x 16 sums each and meet behind every product.  Five steps of 64 x 64: 20 us instead of 75 in launches of their own, 64 x 128 25
+// instead of 78, 64 x 256 37 instead of 82, eleven of 216 x 10 25 instead of 116.  (Operands out of the caches instead: 28, 43 and 30
+// us for the first, second and last, bound by what a CU's L1 gives, and from 96 x 128 on longer than the launches.)
 constexpr int WHOLE_LDS = 160 * 1024, WHOLE_MOST = 5;   // squares of 16 x 16 of X per wavefront
 constexpr size_t whole_lds(int mp, int np) { return sizeof(_Float16) * 4 * mp * (size_t)(np + mp); }   // X, its transpose, A, B
 // sums of square (bi, bj) over `blocks` times 32

@@ -5,13 +5,16 @@
 //
 // Both are first-order linear recurrences per channel, s <- A s + B, one forwards and one backwards in time, and both are bound by
 // memory: forward 3 values per element (12 bytes in fp32), backward 6.  What the kernels do about it is have enough loads in
-// flight at every shape.  A lane holds V = 4 neighbouring channels of one environment, a wavefront 256 of them.  Where that alone
-// fills the card (a rollout of many environments), a wavefront goes through the steps by itself, L steps' loads at a time.  With
-// fewer channels a workgroup's W wavefronts take L consecutive steps each of a tile of W L: a wavefront's steps compose to one
-// (A, B), these are exchanged through LDS, and each wavefront then repeats its steps from its own first state, so every state is
-// the result of the formula above on the state before it and the inputs are read once.  With a few channels only, the time axis
-// is also split into S segments over workgroups: a first launch leaves every segment's (A, B) in a workspace, the second starts each
-// segment from those before it.  That reads gate and value twice, the second time out of the caches where they fit.
+// flight at every shape.  A lane holds V = 4, 2 or 1 neighbouring channels of one environment, a wavefront 64 V of them.  Three forms:
+// - alone: where the channels fill the card, a wavefront goes through the steps by itself, L steps' loads at a time.  128 steps of
+//   2048 environments of width 256 in fp32: 150 us, 5.4 TB/s, more than a large copy gets (4.9); backward, 1024 of them: 151 us, 5.3.
+// - tiles: with fewer channels a workgroup's W wavefronts take L consecutive steps each of a tile of W L.  A wavefront's steps compose
+//   to one (A, B), these are exchanged through LDS, and each wavefront then repeats its steps from its own first state, so every state
+//   is the result of the formula above on the state before it and the inputs are read once.  1000 steps of 64 in fp32: 55 us.
+// - segments: with a few channels and many steps the time axis is also split over workgroups.  A first launch leaves every segment's
+//   (A, B) in a workspace, the second starts each segment from those before it.  Gate and value are read twice, the second time
+//   out of the caches where they fit: 16384 steps of 2 of width 512 in bf16 42 us, 18 and 24, 3.8 and 4.1 TB/s.  (One launch in which
+//   a segment waits for those ahead would save the second reading, but a wait among XCDs takes 5 us and more here.)
 //
 // A cut is a selection, never a product with 0: an infinity or NaN behind it goes nowhere.  In the composed coefficients A = 0
 // says so; a product of gates that underflows stays at the smallest subnormal instead.
@@ -538,6 +541,8 @@ void channels(Plan &p, int V, int N, int D) {
 // Segments read gate and value twice but go through the time side by side.  Tiles / segments, 1000 steps, fp32 and bf16:
 //   N = 1: 34 / 18, 34 / 18   16: 36 / 23   32: 39 / 39, 37 / 25   64: 55 / 72, 46 / 42   128: 83 / 134, 61 / 78
 // (256 steps: N = 1 12 / 18, 32: 13 / 19; backward: 1000 steps, N = 32 66 / 58, 57 / 36, 64 90 / 108, 74 / 64).
+// Where a few channels leave lanes without any, lanes have fewer.  65536 steps of width 64, V = 4 / 2 / 1: fp32 47 / 41 / 35, bf16
+// 43 / 36 / 31, backward 59 / 53 / 49, 53 / 42 / 38.
 Plan plan_of(const mrl_ctx *ctx, int T, int N, int D, int size) {
     Plan p = {};
     const long want = 8L * ctx->n_cus;   // wavefronts
@@ -546,7 +551,8 @@ Plan plan_of(const mrl_ctx *ctx, int T, int N, int D, int size) {
     p.W = 1;
     p.segments = 1;
     if (T >= 512 && (long)p.groups * size * 2 < ctx->n_cus) {
-        if ((long)p.groups * T < SHARE * want) channels(p, 2, N, D);
+        if ((long)p.groups * T < SHARE * want || p.lanes <= 32) channels(p, 2, N, D);
+        if (p.lanes <= 32) channels(p, 1, N, D);
         const long shares = std::min<long>(((long)T + SHARE - 1) / SHARE, std::max<long>(2 * MAX_WAVES, want / p.groups));
         p.W = MAX_WAVES;
         p.share = (int)((T + shares - 1) / shares);
