@@ -29,7 +29,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float QA = 3.4445f, QB = -4.7750f, QC = 2.0315f;
-constexpr int MOST = 16;        // matrices of a launch
+constexpr int MOST = 16;        // matrices of a launch, where they differ
+constexpr size_t BATCH_BYTES = 256 << 20;   // of workspace from which on a launch takes no more matrices that are alike
 constexpr int LOAD = 32;        // sides of what a workgroup of the second launch takes
 constexpr int CHUNK = 1024;     // elements that a workgroup of the first launch takes at a time
 constexpr int MOST_SUMS = 1024;  // partial sums of squares per matrix
@@ -53,6 +54,8 @@ struct Group {
     int count, rests;
     int sym_tile, update_tile;   // sides of the products' tiles
     int begin_sym[MOST], begin_update[MOST];   // a matrix's first tile among all; none: INT_MAX
+    size_t alike_in, alike_kept;               // mrl_orthogonalize: bytes from a matrix to the next, all described by the first
+    int alike_sym, alike_update;               // and its tiles
     Mat mat[MOST];
     Rest rest[MOST + 1];
     double eps;
@@ -78,6 +81,24 @@ MRL_DEV Mat described(const Mat &m) {
 }
 
 enum { F32 = 0, BF16 = 1, MUON = 2 };   // what a matrix is read from and written to
+// Matrix k of the group, from the one that describes it; those of mrl_orthogonalize are alike, any number of them in a launch.
+template <int KIND>
+MRL_DEV int describes(int k) { return KIND == MUON ? k : 0; }
+template <int KIND>
+MRL_DEV Mat matrix(const Group &g, Mat m, int k) {
+    if (KIND != MUON) {
+        m.in = (const char *)m.in + k * g.alike_in;
+        m.out = (char *)m.out + k * g.alike_in;
+        const size_t kept = k * g.alike_kept;
+        m.x += kept;
+        m.xt += kept;
+        m.xt1 += kept;
+        m.a += kept;
+        m.b += kept;
+        m.partial += kept;
+    }
+    return m;
+}
 
 // What is orthogonalised, element i; FIRST: with MUON its momentum is brought up to date.
 template <int KIND, bool FIRST = false>
@@ -116,7 +137,7 @@ __global__ __launch_bounds__(256) void sums_kernel(Group g, Group *kept) {
         adam_rest(g, blockIdx.x, gridDim.x);
         return;
     }
-    const Mat &m = g.mat[blockIdx.y];
+    const Mat m = matrix<KIND>(g, g.mat[describes<KIND>(blockIdx.y)], blockIdx.y);
     const int block = blockIdx.x;
     if (block >= m.sums) return;
     const size_t size = (size_t)m.rows * m.cols;
@@ -195,7 +216,7 @@ __global__ __launch_bounds__(256) void load_kernel(const Group *__restrict__ gro
     const Group &g = *group;
     __shared__ double part[256];
     __shared__ float tile[LOAD][LOAD + 1];
-    const Mat m = described(g.mat[blockIdx.y]);
+    const Mat m = matrix<KIND>(g, described(g.mat[describes<KIND>(blockIdx.y)]), blockIdx.y);
     if ((int)blockIdx.x < m.mp / LOAD * (m.np / LOAD)) load_square<KIND>(g, m, blockIdx.x, scale_of(g, m, part), tile);
 }
 
@@ -227,17 +248,21 @@ MRL_DEV void above_diagonal(int tile, int &bi, int &bj) {
 // Which of `tiles` tiles, of which matrix, a workgroup works on.  Workgroups go to the eight XCDs in turn; each XCD gets a run of
 // tiles that share operands, so that its L2 is read more often than what is behind it (every matrix on every XCD instead: eight of
 // 777 x 333 212 us for 177).  All first tiles are looked at, from one scalar load, not one after the other.
-template <int STAGE, int TILE>
+template <int STAGE, int KIND, int TILE>
 MRL_DEV Mat find_tile(const Group &g, int count, int tiles, int &bi, int &bj) {
     const int xcd = blockIdx.x & 7, each = tiles >> 3, more = tiles & 7;
     int id = xcd * each + min(xcd, more) + (blockIdx.x >> 3), k = 0;
-    if (count > 1) {
+    if (KIND != MUON && count > 1) {
+        const int each_has = STAGE == UPDATE ? g.alike_update : g.alike_sym;
+        k = __builtin_amdgcn_readfirstlane(id / each_has);
+        id -= k * each_has;
+    } else if (count > 1) {
         const int(&begin)[MOST] = STAGE == UPDATE ? g.begin_update : g.begin_sym;
 #pragma unroll
         for (int i = 1; i < MOST; ++i) k += id >= begin[i];
         id -= begin[k];
     }
-    const Mat m = described(g.mat[k]);
+    const Mat m = matrix<KIND>(g, described(g.mat[describes<KIND>(k)]), k);
     if (STAGE == UPDATE) {
         const int rows = (m.mp + TILE - 1) / TILE, panel = __builtin_amdgcn_readfirstlane(id / (4 * rows)), in = id - panel * 4 * rows;
         const int width = min(4, (m.np + TILE - 1) / TILE - 4 * panel);   // panels of four columns, row by row
@@ -354,7 +379,7 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
     constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, ACROSS = WAVES<F> / 2, FP = F, FQ = SIDE / ACROSS, OWN = SIDE / ACROSS, LOADS = 2 * OWN;
     extern __shared__ _Float16 lds[];
     int bi, bj;
-    const Mat m = find_tile<STAGE, 32 * F>(g, count, tiles, bi, bj);
+    const Mat m = find_tile<STAGE, KIND, 32 * F>(g, count, tiles, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(g, m, from, P, Q, blocks);
@@ -517,7 +542,7 @@ __global__ __launch_bounds__(256) void small_product_kernel(const Group *__restr
     const Group &g = *group;
     __shared__ SmallSums sums;
     int bi, bj;
-    const Mat m = find_tile<STAGE, 32>(g, count, tiles, bi, bj);
+    const Mat m = find_tile<STAGE, KIND, 32>(g, count, tiles, bi, bj);
     small_product<STAGE, KIND>(g, m, bi, bj, from, last, sums);
 }
 
@@ -549,7 +574,7 @@ __global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
         adam_rest(g, blockIdx.x - g.count, gridDim.x - g.count);
         return;
     }
-    const Mat &m = g.mat[blockIdx.x];
+    const Mat m = matrix<KIND>(g, g.mat[describes<KIND>(blockIdx.x)], blockIdx.x);
     const int size = m.rows * m.cols, mp = m.mp, np = m.np;
     double *part = reinterpret_cast<double *>(lds);
     double sum = 0.0;
@@ -646,11 +671,22 @@ size_t group_bytes(const S *matrices, int count) {
     for (int k = 0; k < count; ++k) bytes += matrix_bytes(matrices[k].rows, matrices[k].cols);
     return bytes;
 }
-// of `count` alike
+// Of `count` alike: how many a launch takes, and their workspace.  256 of 64 x 64 in one launch 21 us, sixteen at a time 319; 64 of
+// 256 x 256 255 and 397.
+int batch_of(int count, int rows, int cols) {
+    Mat m = {};
+    size_t lds;
+    m.rows = rows;
+    m.cols = cols;
+    const size_t room = is_whole(&m, 1, lds) ? 1 << 20 : std::max<size_t>(MOST, BATCH_BYTES / matrix_bytes(rows, cols));
+    return (int)std::min<size_t>(count, room);
+}
 size_t batch_bytes(int count, int rows, int cols) {
-    Mat alike[MOST] = {};
-    for (Mat &m : alike) m.rows = rows, m.cols = cols;
-    return group_bytes(alike, std::min(count, MOST));
+    Mat m = {};
+    size_t lds;
+    m.rows = rows;
+    m.cols = cols;
+    return is_whole(&m, 1, lds) ? 0 : GROUP_BYTES + batch_of(count, rows, cols) * matrix_bytes(rows, cols);
 }
 
 // Sides of the tiles of a group's symmetric products, or of its updates: those of the least time by what products of one to sixteen
@@ -658,13 +694,14 @@ size_t batch_bytes(int count, int rows, int cols) {
 //   32: 5.0 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.012 + 0.0095 share)
 // where share of the CUs have one; more of them get in each other's way at the caches.  Symmetric / update at 32, 64, 96, 128:
 //   256: 5 / 5, 6 / 7, 8 / 10, 9 / 11    1024: 11 / 15, 12 / 13, 17 / 20, 19 / 21    2048: 66 / 96, 49 / 67, 38 / 78, 42 / 50
-int tile_of(const mrl_ctx *ctx, const Group &g, bool symmetric) {
+int tile_of(const mrl_ctx *ctx, const Group &g, int described, int copies, bool symmetric) {
     int best = 0;
     double least = 0.0;
     for (int tile : {32, 64, 96, 128}) {
         double tiles = 0.0, work = 0.0;
-        for (int k = 0; k < g.count; ++k) {
-            const double a = (g.mat[k].mp + tile - 1) / tile, b = (g.mat[k].np + tile - 1) / tile, own = symmetric ? a * (a + 1) / 2 : a * b;
+        for (int k = 0; k < described; ++k) {
+            const double a = (g.mat[k].mp + tile - 1) / tile, b = (g.mat[k].np + tile - 1) / tile;
+            const double own = copies * (symmetric ? a * (a + 1) / 2 : a * b);
             tiles += own;
             work += own * (symmetric ? 0.5 * (g.mat[k].mp + g.mat[k].np) : g.mat[k].mp);
         }
@@ -730,10 +767,11 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
     size_t used = GROUP_BYTES;
     Group *kept = (Group *)workspace;
     size_t lds;
-    const bool whole = is_whole(g.mat, g.count, lds);
+    const int described = KIND == MUON ? g.count : 1, copies = KIND == MUON ? 1 : g.count;
+    const bool whole = is_whole(g.mat, described, lds);
     const int threads = whole ? 1024 : 256;
     int sums = 1;
-    for (int k = 0; k < g.count; ++k) {
+    for (int k = 0; k < described; ++k) {
         set_up(g.mat[k], whole ? 32 : 64, used);   // (a whole group's planes are in LDS: there is no workspace)
         sums = std::max(sums, g.mat[k].sums);
     }
@@ -744,12 +782,12 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
         hipLaunchKernelGGL(whole_kernel<KIND>, dim3(g.count + rest), dim3(threads), lds, ctx->stream, g, steps);
         return;
     }
-    g.sym_tile = tile_of(ctx, g, true);
-    g.update_tile = tile_of(ctx, g, false);
+    g.sym_tile = tile_of(ctx, g, described, copies, true);
+    g.update_tile = tile_of(ctx, g, described, copies, false);
     std::fill(g.begin_sym, g.begin_sym + MOST, INT_MAX);
     std::fill(g.begin_update, g.begin_update + MOST, INT_MAX);
     int load = 0, sym = 0, update = 0;   // squares of the largest matrix, tiles of all
-    for (int k = 0; k < g.count; ++k) {
+    for (int k = 0; k < described; ++k) {
         const Mat &m = g.mat[k];
         const int a = (m.mp + g.sym_tile - 1) / g.sym_tile;
         load = std::max(load, m.mp / LOAD * (m.np / LOAD));
@@ -758,6 +796,11 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
         g.begin_update[k] = update;
         update += ((m.mp + g.update_tile - 1) / g.update_tile) * ((m.np + g.update_tile - 1) / g.update_tile);
     }
+    g.alike_kept = used - GROUP_BYTES;
+    g.alike_sym = sym;
+    g.alike_update = update;
+    sym *= copies;
+    update *= copies;
     hipLaunchKernelGGL(sums_kernel<KIND>, dim3(std::max<long>(sums, rest), g.count + (rest > 0)), dim3(threads), 0, ctx->stream, g, kept);
     hipLaunchKernelGGL(load_kernel<KIND>, dim3(load, g.count), dim3(256), 0, ctx->stream, kept);
     for (int s = 0; s < steps; ++s) {
@@ -826,15 +869,15 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
     const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
-    for (int done = 0; done < count; done += mrl::MOST) {
+    const int most = mrl::batch_of(count, rows, cols);
+    for (long done = 0; done < count; done += most) {
         mrl::Group g = {};
         g.eps = eps;
-        g.count = std::min(mrl::MOST, count - done);
-        for (int k = 0; k < g.count; ++k) {
-            mrl::sides(g.mat[k], rows, cols);
-            g.mat[k].in = (const char *)in + (done + k) * one;
-            g.mat[k].out = (char *)out + (done + k) * one;
-        }
+        g.count = (int)std::min<long>(most, count - done);
+        g.alike_in = one;
+        mrl::sides(g.mat[0], rows, cols);
+        g.mat[0].in = (const char *)in + done * one;
+        g.mat[0].out = (char *)out + done * one;
         if (dtype == MRL_F32) mrl::run<mrl::F32>(ctx, g, steps, workspace);
         else mrl::run<mrl::BF16>(ctx, g, steps, workspace);
         MRL_CHECK_LAUNCH();

@@ -54,6 +54,8 @@ def orthogonalize(ctx, out, x, steps=5, eps=1e-7):
     count, rows, cols = shape if len(shape) == 3 else (1, *shape)
     if count * rows * cols == 0:
         return
+    if max(count, rows, cols) >= 1 << 31:
+        raise _lib.MrlError("orthogonalize: %s is more than the library counts" % list(shape))
     n = _orthogonalize_bytes(count, rows, cols)
     ws = _scratch(ctx, n) if n else None
     _lib.call("mrl_orthogonalize", ctx.handle, kind, count, rows, cols, x.data_ptr(), out.data_ptr(), steps, eps,

@@ -26,7 +26,7 @@ class GatedRecurrence:
         if width < 1:
             raise _lib.MrlError("GatedRecurrence: the width must be positive, got %d" % width)
         self.width = width
-        self._sizes = {}   # (context, steps, envs) -> workspace bytes
+        self._sizes = {}   # (device, steps, envs) -> workspace bytes
 
     def _rows(self, ctx, name, t, size, dtype):
         """(pointer, elements from a row to the next) of a tensor of size (rows, width)."""
@@ -63,13 +63,15 @@ class GatedRecurrence:
         kind = _TYPES.get(gate.dtype)
         if kind is None:
             raise _lib.MrlError("gate: float32 or bfloat16 expected, got %s" % gate.dtype)
+        if steps >= 1 << 31 or gate.size(0) // steps * self.width >= 1 << 31:
+            raise _lib.MrlError("gate: %s of %d steps: fewer than 2^31 steps and states expected" % (list(gate.shape), steps))
         return gate.size(0) // steps, kind
 
     def _workspace(self, ctx, steps, envs):
         """(tensor or None, pointer, bytes)"""
         if steps == 1:
             return None, None, 0
-        key = (ctx.handle.value, steps, envs)
+        key = (ctx.device, steps, envs)
         n = self._sizes.get(key)
         if n is None:
             size = C.c_uint64(0)

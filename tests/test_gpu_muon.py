@@ -78,6 +78,27 @@ def test_many_matrices_in_place_at_odd_addresses(mrl, ctx, count, rows, cols, dt
         near(inside[k], x[k], HALF[dtype], "matrix %d" % k)
 
 
+# shapes whose products are worked out in larger tiles, alone and in batches, with rows and columns behind the last whole tile; batches
+# in one launch, in one per product, and in more than one
+@pytest.mark.parametrize("count,rows,cols,dtype", [(12, 519, 513, "f32"), (15, 449, 511, "bf16"), (8, 643, 701, "f32"), (60, 129, 191, "f32"), (6, 831, 385, "f32"),
+                                                   (22, 193, 521, "bf16"), (1, 1411, 1500, "f32"), (700, 20, 33, "f32"), (300, 65, 64, "bf16"), (650, 100, 130, "f32")])
+def test_batches(mrl, ctx, count, rows, cols, dtype):
+    print("batch", count, rows, cols, dtype, flush=True)
+    gen = torch.Generator().manual_seed(count + rows)
+    x = torch.randn(count, rows, cols, generator=gen)
+    x[..., 0] += torch.arange(1.0, count + 1)[:, None] / count
+    x = x.to(TYPES[dtype])
+    out = torch.full((count, rows, cols), 9.0, dtype=TYPES[dtype], device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda())
+    ctx.synchronize()
+    for k in sorted({0, 1, 17, count // 2, 617, 618, count - 1}) if rows < 200 else {0, count - 1}:
+        if k < count:
+            near(out[k], x[k], HALF[dtype], "matrix %d" % k)
+    norms = out.float().square().sum((1, 2)).cpu()
+    # singular values of about [0.7, 1.2] have squares of 0.49 to 1.44; of random matrices' few start below the 1 / 485 that five steps lift
+    assert (norms > 0.25 * min(rows, cols)).all() and (norms < 1.6 * min(rows, cols)).all()
+
+
 @pytest.mark.parametrize("steps,eps", [(1, 1e-7), (2, 1e-3), (3, 0.0), (8, 1e-7)])
 def test_steps_and_eps(mrl, ctx, steps, eps):
     x = matrix(torch.Generator().manual_seed(steps), 48, 90) * 1e-3
@@ -173,6 +194,37 @@ def test_muon_steps(mrl, ctx, net, layers, nesterov, decay):
     bound = loose + 3 * (3 * 2.0 ** -24 * (w.abs() + 0.1) + 0.003 * 40 * 2.0 ** -24)
     assert ((p.cpu().double() - w).abs() <= bound).all()
     assert ((s.cpu().double() - m2).abs() <= 3 * 6 * 2.0 ** -24 * (m2.abs() + 0.5)).all()
+
+
+@pytest.mark.parametrize("large", [(), (3,), (30,)])
+def test_more_matrices_than_a_launch_takes(mrl, ctx, large):
+    """35 matrices with gaps between them in one call, against each in a call of its own."""
+    lib, Matrix, gen = mrl._lib.lib(), mrl._lib.Matrix, torch.Generator().manual_seed(6)
+    at, mats = 3, []
+    for k in range(35):
+        rows, cols = (150, 130) if k in large else (8 + k % 5, 12 - k % 3)
+        mats.append(Matrix(at, rows, cols))
+        at += rows * cols + k % 4
+    n = at + 5
+    p, g, s = torch.randn(n, generator=gen).cuda(), torch.randn(n, generator=gen).cuda(), torch.rand(2 * n, generator=gen).cuda()
+    one = [p.clone(), g, s.clone()]
+    ws = torch.empty(1 << 25, dtype=torch.uint8, device="cuda")
+
+    def step(params, grads, state, matrices):
+        array = (Matrix * max(1, len(matrices)))(*matrices)
+        assert lib.mrl_muon_step(ctx.handle, *(ctypes.c_void_p(t.data_ptr()) for t in (params, grads, state)), params.numel(), len(matrices), array, 2, 0.1, 0.9, 1, 0.01, 5,
+                                 1e-7, 1e-3, 0.9, 0.99, 1e-8, ctypes.c_void_p(ws.data_ptr()), ws.numel()) == 0, lib.mrl_last_error()
+    step(p, g, s, mats)
+    ctx.synchronize()
+    start = 0
+    for m in mats + [Matrix(n, 0, 0)]:
+        end = m.offset + m.rows * m.cols
+        step(one[0][start:end], g[start:end], one[2][2 * start:2 * end], [Matrix(m.offset - start, m.rows, m.cols)] if m.rows else [])
+        ctx.synchronize()
+        start = end
+    assert torch.equal(s, one[2])
+    # (a matrix in a launch of its own is worked out in other tiles: sums in another order, entries of at most 1.2 * 0.1 * sqrt(1.5))
+    assert (p - one[0]).abs().max() <= 0.15 * 2.0 ** -14
 
 
 def test_network_with_muon_trains_and_round_trips(mrl, ctx, tmp_path):

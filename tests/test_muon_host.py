@@ -21,6 +21,14 @@ def test_orthogonalize_refuses(mrl, x, out, text):
         mrl.orthogonalize(HostContext, out, x)
 
 
+@pytest.mark.parametrize("shape", [(1 << 31, 1, 1), (2, (1 << 32) + 5), (1, (1 << 32) + 5, 2)])
+def test_more_than_the_library_counts(mrl, shape):
+    class Context:
+        device, handle, stream = torch.device("meta"), ctypes.c_void_p(), None
+    with pytest.raises(mrl.MrlError, match="counts"):
+        mrl.orthogonalize(Context, torch.empty(shape, device="meta"), torch.empty(shape, device="meta"))
+
+
 def test_nothing_to_do_needs_no_device(mrl):
     for shape in ((0, 4), (4, 0), (0, 3, 4)):
         mrl.orthogonalize(HostContext, torch.zeros(shape), torch.zeros(shape))

@@ -48,3 +48,15 @@ def test_width_and_context(mrl):
                        ("mrl_recurrence_forward", (None, 0, 1, 1, 1, None, 1, None, 1, None, None, None, None, 1, None, None, 0))):
         with pytest.raises(mrl.MrlError, match="ctx"):
             mrl._lib.call(name, *args)
+
+
+@pytest.mark.parametrize("rows,width,steps", [(1 << 32, 1, 1 << 32), (1 << 31, 1, 1), (1 << 20, 1 << 12, 1), (1 << 32, 2, 2)])
+def test_more_than_the_library_counts(mrl, rows, width, steps):
+    class Context:
+        device, handle, stream = torch.device("meta"), ctypes.c_void_p(), None
+    x = torch.empty(rows, width, device="meta")
+    layer = mrl.GatedRecurrence(width)
+    with pytest.raises(mrl.MrlError, match="2\\^31"):
+        layer.forward_gpu(Context, x, x, x, steps)
+    with pytest.raises(mrl.MrlError, match="2\\^31"):
+        layer.backward_gpu(Context, x, x, x, x, x, x, steps)
