@@ -328,6 +328,18 @@ MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diago
     }
 }
 
+// Products of up to FEW rows on the fp32 matrix cores, which round to nearest: the fp16 ones round their sums down, and where a sum has few
+// terms these errors go one way in every entry.  Against 64 bits, fp16 / fp32 / all in fp32: 8 x 64 1.7e-6, 0.8e-6, 0.8e-6; 1 x 500
+// 1.1e-6, 0.4e-6, 0.4e-6; 8 x 721 1.6e-6, 1.1e-6, 0.9e-6; with 17 rows and more fp16 is as good, with 64 better.  (16 x 16: 18 us for 14.)
+constexpr int FEW = 16;
+// 16 x 16 sums over 32 of the contracted index, four at a time
+MRL_DEV void multiply_few(const f16x8 &ph, const f16x8 &pl, const f16x8 &qh, const f16x8 &ql, f32x4 &acc) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float p = (float)ph[i] + (float)pl[i], q = (float)qh[i] + (float)ql[i];
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(p, q, acc, 0, 0, 0);
+    }
+}
 template <int F>
 MRL_DEV void multiply(const f16x8 (&p)[F], const f16x8 (&q)[F], f32x4 (&acc)[F][F]) {
 #pragma unroll
@@ -486,8 +498,8 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
 }
 
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
-// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.  256 x 256: 4.6, 4.8 and
-// 5.2 us for the three, most of it the launch and the trips to memory one behind the other (description, operands, sums).
+// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.  256 x 256: 4.2, 4.3 and
+// 4.6 us for the three, most of it the launch and the trips to memory one behind the other (description, operands, sums).
 typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
 template <int STAGE, int KIND>
 MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums) {
@@ -512,12 +524,18 @@ MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int fro
             o.ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
         }
     };
+    const bool few = m.m <= FEW;   // then the other squares are of zeros
     auto work = [&](const Operands &o) {
+        if (few) {
+            multiply_few(o.ph[0], o.pl[0], o.qh[0], o.ql[0], acc[0][0]);
+            if (STAGE == UPDATE) multiply_few(o.ph[0], o.pl[0], o.qh[1], o.ql[1], acc[0][1]);
+            return;
+        }
         multiply<2>(o.pl, o.qh, acc);
         multiply<2>(o.ph, o.ql, acc);
         multiply<2>(o.ph, o.qh, acc);
     };
-    // two steps' operands under way together
+    // two steps' operands under way together (more bring nothing)
     int kb = wave;
     for (; kb + 4 < blocks; kb += 8) {
         Operands one, two;
@@ -552,11 +570,17 @@ __global__ __launch_bounds__(256) void small_product_kernel(const Group *__restr
 // us for the first, second and last, bound by what a CU's L1 gives, and from 96 x 128 on longer than the launches.)
 constexpr int WHOLE_LDS = 160 * 1024, WHOLE_MOST = 5;   // squares of 16 x 16 of X per wavefront
 constexpr size_t whole_lds(int mp, int np) { return sizeof(_Float16) * 4 * mp * (size_t)(np + mp); }   // X, its transpose, A, B
-// sums of square (bi, bj) over `blocks` times 32
-MRL_DEV f32x4 square_sum(const _Float16 *P, int p_rows, int bi, const _Float16 *Q, int q_rows, int bj, int blocks) {
+// sums of square (bi, bj) over `blocks` times 32, of those every `step`th from number `first`
+MRL_DEV f32x4 square_sum(bool few, const _Float16 *P, int p_rows, int bi, const _Float16 *Q, int q_rows, int bj, int blocks, int first = 0, int step = 1) {
     const int lane = threadIdx.x & 63;
-    const _Float16 *p = P + bi * 1024 + lane * 8, *q = Q + bj * 1024 + lane * 8;
+    const _Float16 *p = P + bi * 1024 + lane * 8 + first * p_rows * 64, *q = Q + bj * 1024 + lane * 8 + first * q_rows * 64;
     f32x4 acc = {};
+    if (few) {
+        for (int kb = first; kb < blocks; kb += step, p += step * p_rows * 64, q += step * q_rows * 64)
+            multiply_few(*reinterpret_cast<const f16x8 *>(p), *reinterpret_cast<const f16x8 *>(p + 512), *reinterpret_cast<const f16x8 *>(q),
+                         *reinterpret_cast<const f16x8 *>(q + 512), acc);
+        return acc;
+    }
 #pragma unroll 2
     for (int kb = 0; kb < blocks; ++kb, p += p_rows * 64, q += q_rows * 64) {
         const f16x8 ph = *reinterpret_cast<const f16x8 *>(p), pl = *reinterpret_cast<const f16x8 *>(p + 512);
@@ -567,7 +591,7 @@ MRL_DEV f32x4 square_sum(const _Float16 *P, int p_rows, int bi, const _Float16 *
     }
     return acc;
 }
-template <int KIND>
+template <int KIND, bool SOME_FEW>
 __global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
     extern __shared__ _Float16 lds[];
     if (KIND == MUON && (int)blockIdx.x >= g.count) {
@@ -608,11 +632,23 @@ __global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
     }
     __syncthreads();
     const int at = piece_in(lane & 15, lane >> 4);
+    const bool few = SOME_FEW && m.m <= FEW;
+    const int high = few ? 1 : rows;   // squares of X that are not of zeros
     for (int s = 0; s < steps; ++s) {
-        for (int t = wave; t < rows * (rows + 1) / 2; t += 16) {
-            int bi, bj;
-            above_diagonal(t, bi, bj);
-            store_both(A, mp, bi == bj ? nullptr : A, mp, bi * 16, bj * 16, square_sum(X, mp, bi, X, mp, bj, np / 32) * m.gram);
+        if (few) {   // one square, shared by four wavefronts over B's 4 KiB; the others are zeros
+            f32x4 *sums = reinterpret_cast<f32x4 *>(B);
+            if (wave < 4) sums[wave * 64 + lane] = square_sum(true, X, mp, 0, X, mp, 0, np / 32, wave, 4);
+            __syncthreads();
+            if (wave < 3) {
+                const f32x4 sum = (sums[lane] + sums[64 + lane]) + (sums[128 + lane] + sums[192 + lane]);
+                store_both(A, mp, wave == 1 ? A : nullptr, mp, wave > 1 ? 16 : 0, wave > 0 ? 16 : 0, wave == 0 ? sum * m.gram : f32x4{});
+            }
+        } else {
+            for (int t = wave; t < rows * (rows + 1) / 2; t += 16) {
+                int bi, bj;
+                above_diagonal(t, bi, bj);
+                store_both(A, mp, bi == bj ? nullptr : A, mp, bi * 16, bj * 16, square_sum(false, X, mp, bi, X, mp, bj, np / 32) * m.gram);
+            }
         }
         __syncthreads();
         for (int t = wave; t < rows * (rows + 1) / 2; t += 16) {
@@ -620,23 +656,23 @@ __global__ __launch_bounds__(1024) void whole_kernel(Group g, int steps) {
             above_diagonal(t, bi, bj);
             Piece a;
             a.load(A + square_at(mp, bj * 16, bi * 16) + at);
-            store_both(B, mp, bi == bj ? nullptr : B, mp, bi * 16, bj * 16, QB * a.value() + square_sum(A, mp, bi, A, mp, bj, mp / 32) * m.square);
+            store_both(B, mp, bi == bj ? nullptr : B, mp, bi * 16, bj * 16, QB * a.value() + square_sum(few, A, mp, bi, A, mp, bj, mp / 32) * m.square);
         }
         __syncthreads();
         f32x4 v[WHOLE_MOST];
 #pragma unroll
         for (int i = 0; i < WHOLE_MOST; ++i) {
-            const int t = wave + 16 * i, bi = t % rows, bj = t / rows;
-            if (t >= rows * columns) continue;
+            const int t = wave + 16 * i, bi = t % high, bj = t / high;
+            if (t >= high * columns) continue;
             Piece x;
             x.load(XT + square_at(np, bj * 16, bi * 16) + at);
-            v[i] = QA * x.value() + square_sum(B, mp, bi, XT, np, bj, mp / 32) * m.update;
+            v[i] = QA * x.value() + square_sum(few, B, mp, bi, XT, np, bj, mp / 32) * m.update;
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < WHOLE_MOST; ++i) {
-            const int t = wave + 16 * i, bi = t % rows, bj = t / rows;
-            if (t >= rows * columns) continue;
+            const int t = wave + 16 * i, bi = t % high, bj = t / high;
+            if (t >= high * columns) continue;
             if (s == steps - 1) give<KIND>(g, m, bi * 16, bj * 16, v[i]);
             else store_both(XT, np, X, mp, bi * 16, bj * 16, v[i]);
         }
@@ -691,9 +727,9 @@ size_t batch_bytes(int count, int rows, int cols) {
 
 // Sides of the tiles of a group's symmetric products, or of its updates: those of the least time by what products of one to sixteen
 // matrices of 256 to 2048 took, in us, K of the contracted index long (256 CUs; one workgroup per CU at 96 and 128):
-//   32: 5.0 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.012 + 0.0095 share)
+//   32: 4.5 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.012 + 0.0095 share)
 // where share of the CUs have one; more of them get in each other's way at the caches.  Symmetric / update at 32, 64, 96, 128:
-//   256: 5 / 5, 6 / 7, 8 / 10, 9 / 11    1024: 11 / 15, 12 / 13, 17 / 20, 19 / 21    2048: 66 / 96, 49 / 67, 38 / 78, 42 / 50
+//   256: 4 / 5, 6 / 7, 8 / 10, 9 / 11    1024: 10 / 16, 11 / 13, 17 / 20, 19 / 21    2048: 66 / 96, 49 / 67, 38 / 78, 42 / 50
 int tile_of(const mrl_ctx *ctx, const Group &g, int described, int copies, bool symmetric) {
     int best = 0;
     double least = 0.0;
@@ -706,7 +742,7 @@ int tile_of(const mrl_ctx *ctx, const Group &g, int described, int copies, bool 
             work += own * (symmetric ? 0.5 * (g.mat[k].mp + g.mat[k].np) : g.mat[k].mp);
         }
         const double K = work / tiles, per_cu = tiles / ctx->n_cus, rounds = std::ceil(per_cu), share = std::min(1.0, per_cu);
-        const double time = tile == 32   ? 5.0 + 11e-6 * 256 * per_cu * K
+        const double time = tile == 32   ? 4.5 + 11e-6 * 256 * per_cu * K
                             : tile == 64 ? 5.5 + 0.0072 * K * rounds
                             : tile == 96 ? 6.0 + K * rounds * (0.0105 + 0.006 * share)
                                          : 7.0 + K * rounds * (0.012 + 0.0095 * share);
@@ -779,11 +815,16 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
     for (int k = 0; k < g.rests; ++k) rest += g.rest[k].n;
     rest = std::min<long>(2048, (rest + threads - 1) / threads);
     if (whole) {
-        hipLaunchKernelGGL(whole_kernel<KIND>, dim3(g.count + rest), dim3(threads), lds, ctx->stream, g, steps);
+        bool some_few = false;
+        for (int k = 0; k < described; ++k) some_few |= g.mat[k].m <= FEW;
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(g.count + rest), dim3(threads), lds, ctx->stream, g, steps); };
+        if (some_few) launch(whole_kernel<KIND, true>);
+        else launch(whole_kernel<KIND, false>);   // (a twentieth faster)
         return;
     }
-    g.sym_tile = tile_of(ctx, g, described, copies, true);
-    g.update_tile = tile_of(ctx, g, described, copies, false);
+    const bool few = KIND != MUON && g.mat[0].m <= FEW;   // (worked out in tiles of 32 only)
+    g.sym_tile = few ? 32 : tile_of(ctx, g, described, copies, true);
+    g.update_tile = few ? 32 : tile_of(ctx, g, described, copies, false);
     std::fill(g.begin_sym, g.begin_sym + MOST, INT_MAX);
     std::fill(g.begin_update, g.begin_update + MOST, INT_MAX);
     int load = 0, sym = 0, update = 0;   // squares of the largest matrix, tiles of all

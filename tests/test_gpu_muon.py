@@ -99,6 +99,26 @@ def test_batches(mrl, ctx, count, rows, cols, dtype):
     assert (norms > 0.25 * min(rows, cols)).all() and (norms < 1.6 * min(rows, cols)).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 500), (2, 300), (3, 50), (8, 64), (8, 721), (4, 1000), (14, 300), (16, 16), (2000, 12)])
+def test_few_rows_as_close_as_fp32_products(mrl, ctx, rows, cols):
+    """With few rows errors go one way in every entry: on average over matrices within twice what fp32 products are off (operands
+    of 22 bits are rounded up to twice as far as those of 24)."""
+    off, plain = 0.0, 0.0
+    for seed in range(6):
+        x = matrix(torch.Generator().manual_seed(100 + seed), rows, cols)
+        out = torch.empty(rows, cols, device="cuda")
+        mrl.orthogonalize(ctx, out, x.cuda())
+        ctx.synchronize()
+        want, y = polynomial(x), (x if rows <= cols else x.T) / (x.norm() + 1e-7)
+        for _ in range(5):
+            gram = y @ y.T
+            y = NS[0] * y + (NS[1] * gram + NS[2] * gram @ gram) @ y
+        off += ((out.cpu().double() - want).norm() / want.norm()).item()
+        plain += (((y if rows <= cols else y.T).double() - want).norm() / want.norm()).item()
+    print(rows, cols, off / 6, plain / 6, flush=True)
+    assert off <= 2 * plain
+
+
 @pytest.mark.parametrize("steps,eps", [(1, 1e-7), (2, 1e-3), (3, 0.0), (8, 1e-7)])
 def test_steps_and_eps(mrl, ctx, steps, eps):
     x = matrix(torch.Generator().manual_seed(steps), 48, 90) * 1e-3
