@@ -378,7 +378,7 @@ MRL_DEV void meet() {
 // the other multiplies (five steps of 2048 x 2048 570 us for 607, of four of 1024 x 1024 379 for 439).  Operands go from memory to LDS
 // past the registers, a stage of 32 of the contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less
 // time than memory takes to answer.
-// Bound by the matrix cores where there are tiles for all CUs: 2048 x 2048 in tiles of 128, an update takes 50 us, 1.0 PFLOP/s in fp16
+// Bound by the matrix cores where there are tiles for all CUs: 2048 x 2048 in tiles of 128, an update takes 53 us, 0.97 PFLOP/s in fp16
 // (a large fp16 product of this card's library: 1.1); a symmetric product in tiles of 96 37, 0.8 PFLOP/s,
 // with one wavefront on a SIMD.  Fewer tiles are bound by the stages' way through LDS, 0.35 us each at 64.
 // A tile at the edge reads the last rows' operands again where it has none of its own, and leaves what comes of them.
