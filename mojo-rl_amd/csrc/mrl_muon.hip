@@ -281,7 +281,9 @@ MRL_DEV bool inside(const Mat &m, int fi, int fj) { return fi < m.mp && fj < (ST
 template <int STAGE>
 MRL_DEV void ask(const Group &g, const Mat &m, int from, int fi, int fj, Piece &piece) {
     const int lane = threadIdx.x & 63;
-    if (STAGE != GRAM && inside<STAGE>(m, fi, fj)) piece.load(planes(&g, STAGE == UPDATE ? (from ? m.xt1 : m.xt) : m.a) + square_at(STAGE == UPDATE ? m.np : m.mp, fj, fi) + piece_in(lane & 15, lane >> 4));
+    if (STAGE == GRAM || !inside<STAGE>(m, fi, fj)) return;
+    const _Float16 *of = planes(&g, STAGE == UPDATE ? (from ? m.xt1 : m.xt) : m.a);
+    piece.load(of + square_at(STAGE == UPDATE ? m.np : m.mp, fj, fi) + piece_in(lane & 15, lane >> 4));
 }
 // A square's sums in pieces, as columns (row j, k = i) and as rows (row i, k = j)
 MRL_DEV void store_both(_Float16 *columns, int column_rows, _Float16 *rows, int row_rows, int fi, int fj, const f32x4 v) {
@@ -374,43 +376,51 @@ MRL_DEV void meet() {
 
 // One product, a tile of 32 F x 32 F per workgroup.  GRAM: A = X X^T; SQUARE: B = b A + c A A; both symmetric, so only tiles on and
 // above the diagonal are worked out and written to both sides.  UPDATE: X <- a X + B X, `last` to the caller.
-// Four wavefronts share the tile, 16 F x 16 F each; that of 128 eight, 64 x 32 each: of two on a SIMD one hands over its requests while
-// the other multiplies (five steps of 2048 x 2048 570 us for 607, of four of 1024 x 1024 379 for 439).  Operands go from memory to LDS
-// past the registers, a stage of 32 of the contracted index at a time and BUFFERS stages ahead, because a stage is multiplied in less
-// time than memory takes to answer.
+// A set of four wavefronts shares the tile, 16 F x 16 F each, that of 128 of eight, 64 x 32 each.  At 96 two sets take turns at the
+// contracted index and add up at the end.  Either way there are two wavefronts on a SIMD, one of which hands over its requests while the
+// other multiplies (five steps of 2048 x 2048 564 us; 598 with one set at 96, 627 with four wavefronts at 128 too; 1536 x 1536 352
+// for 386).  At 64, where two workgroups fit a CU, two sets do so only if there are no more tiles than CUs and more than 1024 to contract:
+// 1400 x 1400 271 us for 289, 1000 x 4000 350 for 366, but 1024 x 1024 174 for 172 (a launch that takes all of a CU's LDS starts later).
+// Operands go from memory to LDS past the registers, a stage of 32 of the contracted index at a time and BUFFERS stages ahead, because
+// a stage is multiplied in less time than memory takes to answer.
 // Bound by the matrix cores where there are tiles for all CUs: 2048 x 2048 in tiles of 128, an update takes 53 us, 0.97 PFLOP/s in fp16
-// (a large fp16 product of this card's library: 1.1); a symmetric product in tiles of 96 37, 0.8 PFLOP/s,
-// with one wavefront on a SIMD.  Fewer tiles are bound by the stages' way through LDS, 0.35 us each at 64.
+// (a large fp16 product of this card's library: 1.1); a symmetric product in tiles of 96 34, 0.8 PFLOP/s.  Fewer tiles are bound by the
+// stages' way through LDS, 0.2 to 0.35 us each at 64.
 // A tile at the edge reads the last rows' operands again where it has none of its own, and leaves what comes of them.
-template <int F> constexpr int BUFFERS = F == 3 ? 6 : 4;
+template <int F> constexpr int BUFFERS = F == 3 ? 3 : 4;
+constexpr int TWO_SETS = 1024;   // what is contracted by two sets at 64 is longer
 template <int F> constexpr int STAGE_HALVES = 2 * 2 * F * 1024;   // [operand][fragment of 16 rows][hi, lo][512]
 template <int F> constexpr int WAVES = F == 4 ? 8 : 4;
-template <int STAGE, int KIND, int F>
-__global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
+template <int F, int SETS> constexpr size_t RING_BYTES = sizeof(_Float16) * SETS * BUFFERS<F> * STAGE_HALVES<F>;
+template <int STAGE, int KIND, int F, int SETS>
+__global__ __launch_bounds__(64 * WAVES<F> * SETS) void product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
-    constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, ACROSS = WAVES<F> / 2, FP = F, FQ = SIDE / ACROSS, OWN = SIDE / ACROSS, LOADS = 2 * OWN;
+    constexpr int SIDE = 2 * F, AHEAD = BUFFERS<F>, ACROSS = WAVES<F> / 2, FP = F, FQ = SIDE / ACROSS, OWN = FQ, LOADS = 2 * OWN;
     extern __shared__ _Float16 lds[];
     int bi, bj;
     const Mat m = find_tile<STAGE, KIND, 32 * F>(g, count, tiles, bi, bj);
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(g, m, from, P, Q, blocks);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES<F>;
+    const int set = SETS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES<F>;
+    _Float16 *const ring = lds + set * AHEAD * STAGE_HALVES<F>;
+    blocks /= SETS;
     // the first half of the wavefronts brings in P, the other Q, OWN fragments each
     const int row = wave / ACROSS, column = wave % ACROSS, operand = row, fragments = ((operand && STAGE == UPDATE) ? m.np : m.mp) / 16;
     const _Float16 *src[OWN];
 #pragma unroll
     for (int f = 0; f < OWN; ++f)
-        src[f] = (operand ? Q : P) + min((operand ? bj : bi) * SIDE + column * OWN + f, fragments - 1) * 1024 + lane * 8;
+        src[f] = (operand ? Q : P) + min((operand ? bj : bi) * SIDE + column * OWN + f, fragments - 1) * 1024 + lane * 8 + set * fragments * 1024;
     int in_at = wave * OWN * 1024;   // where in LDS the next stage goes
     auto brought = [&]() {
 #pragma unroll
-        for (int f = 0; f < OWN; ++f) src[f] += fragments * 1024;
+        for (int f = 0; f < OWN; ++f) src[f] += SETS * fragments * 1024;
         in_at = in_at >= (AHEAD - 1) * STAGE_HALVES<F> ? in_at - (AHEAD - 1) * STAGE_HALVES<F> : in_at + STAGE_HALVES<F>;
     };
     const int p = row * FP * 1024 + lane * 8, q = (SIDE + column * FQ) * 1024 + lane * 8;
     int at = 0;   // of the stage that is worked on
-    auto read = [&](int where) { return *reinterpret_cast<const f16x8 *>(lds + at + where); };
+    auto read = [&](int where) { return *reinterpret_cast<const f16x8 *>(ring + at + where); };
     f32x4 acc[FP][FQ] = {};
     // A stage's 3 FP FQ products in three groups.  The meeting behind which the next stage is there, and this one's buffer free, stands
     // ahead of the last group.  Requests to LDS and memory go out among the products, at most one ahead of each: a wavefront takes 16
@@ -418,8 +428,8 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
     // freed is asked for from there to the next meeting: EARLY loads in the last group, the others in the next stage's first two.
     constexpr int N = FP * FQ, READS = FP + FQ, EARLY = F == 4 ? 1 : F == 3 ? 1 : 0;
     auto request = [&](int load) {
-        if (load % 2 == 0) bring<0>(src[load / 2], lds + in_at + load / 2 * 1024);
-        else bring<1>(src[load / 2], lds + in_at + load / 2 * 1024);
+        if (load % 2 == 0) bring<0>(src[load / 2], ring + in_at + load / 2 * 1024);
+        else bring<1>(src[load / 2], ring + in_at + load / 2 * 1024);
     };
     auto product = [&](int k, const f16x8 (&x)[FP], const f16x8 (&y)[FQ]) {
         acc[k / FQ][k % FQ] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[k / FQ], y[k % FQ], acc[k / FQ][k % FQ], 0, 0, 0);
@@ -465,7 +475,6 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
     for (int f = 0; f < FQ; ++f) qa[f] = read(q + f * 1024);
 #pragma unroll
     for (int f = 0; f < FP; ++f) pl[f] = read(p + 512 + f * 1024);
-    // (the blocks are an even number: the sides are padded to 64)
     int s = 0;
     for (; s + 1 + AHEAD < blocks; s += 2) {
         first_groups(ph, pl, qa, true);
@@ -475,26 +484,47 @@ __global__ __launch_bounds__(64 * WAVES<F>) void product_kernel(const Group *__r
         meet<(AHEAD - 2) * LOADS>();
         last_group(ph, pl, qb, qa, true);
     }
+    auto end_group = [&](f16x8 (&qh)[FQ]) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) product(k, ph, qh);
+    };
     for (; s < blocks; s += 2) {
         first_groups(ph, pl, qa, s - 1 + AHEAD < blocks);
+        if (SETS > 1 && s + 1 == blocks) {
+            end_group(qa);
+            break;
+        }
         meet<0>();
         last_group(ph, pl, qa, qb, s + AHEAD < blocks);
         first_groups(ph, pl, qb, s + AHEAD < blocks);
-        if (s + 2 < blocks) {
-            meet<0>();
-            last_group(ph, pl, qb, qa, false);
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) product(k, ph, qb);
+        if (s + 2 == blocks) {
+            end_group(qb);
+            break;
         }
+        meet<0>();
+        last_group(ph, pl, qb, qa, false);
+    }
+    // sums of the other set: a set finishes every second fragment
+    auto mine = [&](int f) { return SETS == 1 || f % SETS == set; };
+    if (SETS > 1) {
+        f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + wave * N * 64 + lane;
+        meet<0>();
+#pragma unroll
+        for (int f = 0; f < N; ++f)
+            if (!mine(f)) sums[f * 64] = acc[f / FQ][f % FQ];
+        meet<0>();
+#pragma unroll
+        for (int f = 0; f < N; ++f)
+            if (mine(f)) acc[f / FQ][f % FQ] = acc[f / FQ][f % FQ] + sums[f * 64];
     }
     const int fi = (bi * SIDE + row * FP) * 16, fj = (bj * SIDE + column * FQ) * 16;
     Piece pieces[N];
 #pragma unroll
-    for (int f = 0; f < N; ++f) ask<STAGE>(g, m, from, fi + 16 * (f / FQ), fj + 16 * (f % FQ), pieces[f]);
+    for (int f = 0; f < N; ++f)
+        if (mine(f)) ask<STAGE>(g, m, from, fi + 16 * (f / FQ), fj + 16 * (f % FQ), pieces[f]);
 #pragma unroll
     for (int f = 0; f < N; ++f)
-        finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / FQ), fj + 16 * (f % FQ), acc[f / FQ][f % FQ], pieces[f]);
+        if (mine(f)) finish<STAGE, KIND>(g, m, from, last, bi == bj, fi + 16 * (f / FQ), fj + 16 * (f % FQ), acc[f / FQ][f % FQ], pieces[f]);
 }
 
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
@@ -727,9 +757,10 @@ size_t batch_bytes(int count, int rows, int cols) {
 
 // Sides of the tiles of a group's symmetric products, or of its updates: those of the least time by what products of one to sixteen
 // matrices of 256 to 2048 took, in us, K of the contracted index long (256 CUs; one workgroup per CU at 96 and 128):
-//   32: 4.5 + 11e-6 tiles K    64: 5.5 + 0.0072 K ceil(tiles / 256)    96, 128: 6, 7 + K rounds (0.0105 + 0.006 share, 0.012 + 0.0095 share)
+//   32: 4.5 + 11.5e-6 tiles K    64: 5.5 + 0.0072 K rounds, with two sets 5.5 + K (0.0036 + 0.0036 share)
+//   96: 7 + K (0.007 + 0.0062 share), 7 + 0.0155 K rounds in more than one    128: 7 + K rounds (0.012 + 0.0095 share)
 // where share of the CUs have one; more of them get in each other's way at the caches.  Symmetric / update at 32, 64, 96, 128:
-//   256: 4 / 5, 6 / 7, 8 / 10, 9 / 11    1024: 10 / 16, 11 / 13, 17 / 20, 19 / 21    2048: 66 / 96, 49 / 67, 38 / 78, 42 / 50
+//   256: 4 / 5, 6 / 7, 7 / 10, 9 / 11    1024: 10 / 16, 10 / 13, 14 / 17, 19 / 21    2048: 66 / 96, 48 / 66, 34 / 70, 42 / 50
 int tile_of(const mrl_ctx *ctx, const Group &g, int described, int copies, bool symmetric) {
     int best = 0;
     double least = 0.0;
@@ -742,9 +773,9 @@ int tile_of(const mrl_ctx *ctx, const Group &g, int described, int copies, bool 
             work += own * (symmetric ? 0.5 * (g.mat[k].mp + g.mat[k].np) : g.mat[k].mp);
         }
         const double K = work / tiles, per_cu = tiles / ctx->n_cus, rounds = std::ceil(per_cu), share = std::min(1.0, per_cu);
-        const double time = tile == 32   ? 4.5 + 11e-6 * 256 * per_cu * K
-                            : tile == 64 ? 5.5 + 0.0072 * K * rounds
-                            : tile == 96 ? 6.0 + K * rounds * (0.0105 + 0.006 * share)
+        const double time = tile == 32   ? 4.5 + 11.5e-6 * 256 * per_cu * K
+                            : tile == 64 ? 5.5 + K * (rounds > 1.0 || K <= TWO_SETS ? 0.0072 * rounds : 0.0036 + 0.0036 * share)
+                            : tile == 96 ? 7.0 + K * (rounds > 1.0 ? 0.0155 * rounds : 0.007 + 0.0062 * share)
                                          : 7.0 + K * rounds * (0.012 + 0.0095 * share);
         if (best == 0 || time < least) {
             least = time;
@@ -789,12 +820,15 @@ void sides(Mat &m, int rows, int cols) {
 template <int STAGE, int KIND>
 void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int tiles, int from, int last) {
     const int tile = STAGE == UPDATE ? g.update_tile : g.sym_tile;
+    int K = 0;   // the longest contracted index
+    for (int k = 0; k < (KIND == MUON ? g.count : 1); ++k) K = std::max(K, STAGE == GRAM ? g.mat[k].np : g.mat[k].mp);
     auto launch = [&](auto kernel, size_t lds, int threads = 256) {
         hipLaunchKernelGGL(kernel, dim3(tiles), dim3(threads), lds, ctx->stream, kept, g.count, tiles, from, last);
     };
-    if (tile == 128) launch(product_kernel<STAGE, KIND, 4>, sizeof(_Float16) * BUFFERS<4> * STAGE_HALVES<4>, 64 * WAVES<4>);
-    else if (tile == 96) launch(product_kernel<STAGE, KIND, 3>, sizeof(_Float16) * BUFFERS<3> * STAGE_HALVES<3>);
-    else if (tile == 64) launch(product_kernel<STAGE, KIND, 2>, sizeof(_Float16) * BUFFERS<2> * STAGE_HALVES<2>);
+    if (tile == 128) launch(product_kernel<STAGE, KIND, 4, 1>, RING_BYTES<4, 1>, 64 * WAVES<4>);
+    else if (tile == 96) launch(product_kernel<STAGE, KIND, 3, 2>, RING_BYTES<3, 2>, 512);
+    else if (tile == 64 && tiles <= ctx->n_cus && K > TWO_SETS) launch(product_kernel<STAGE, KIND, 2, 2>, RING_BYTES<2, 2>, 512);
+    else if (tile == 64) launch(product_kernel<STAGE, KIND, 2, 1>, RING_BYTES<2, 1>);
     else launch(small_product_kernel<STAGE, KIND>, 0);
 }
 

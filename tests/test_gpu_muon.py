@@ -81,7 +81,7 @@ def test_many_matrices_in_place_at_odd_addresses(mrl, ctx, count, rows, cols, dt
 # shapes whose products are worked out in larger tiles, alone and in batches, with rows and columns behind the last whole tile; batches
 # in one launch, in one per product, and in more than one
 @pytest.mark.parametrize("count,rows,cols,dtype", [(12, 519, 513, "f32"), (15, 449, 511, "bf16"), (8, 643, 701, "f32"), (60, 129, 191, "f32"), (6, 831, 385, "f32"),
-                                                   (22, 193, 521, "bf16"), (1, 1411, 1500, "f32"), (700, 20, 33, "f32"), (300, 65, 64, "bf16"), (650, 100, 130, "f32")])
+                                                   (22, 193, 521, "bf16"), (1, 1411, 1500, "f32"), (5, 485, 2467, "f32"), (700, 20, 33, "f32"), (300, 65, 64, "bf16"), (650, 100, 130, "f32")])
 def test_batches(mrl, ctx, count, rows, cols, dtype):
     print("batch", count, rows, cols, dtype, flush=True)
     gen = torch.Generator().manual_seed(count + rows)
