@@ -13,7 +13,7 @@
 //   is the result of the formula above on the state before it and the inputs are read once.  1000 steps of 64 in fp32: 55 us.
 // - segments: with a few channels and many steps the time axis is also split over workgroups.  A first launch leaves every segment's
 //   (A, B) in a workspace, the second starts each segment from those before it.  Gate and value are read twice, the second time
-//   out of the caches where they fit: 16384 steps of 2 of width 512 in bf16 42 us, 18 and 24, 3.8 and 4.1 TB/s.  (One launch in which
+//   out of the caches where they fit: 16384 steps of 2 of width 512 in bf16 44 us, 18 and 25, 3.7 and 4.0 TB/s.  (One launch in which
 //   a segment waits for those ahead would save the second reading, but a wait among XCDs takes 5 us and more here.)
 //
 // A cut is a selection, never a product with 0: an infinity or NaN behind it goes nowhere.  In the composed coefficients A = 0
@@ -84,28 +84,25 @@ MRL_DEV void store_n(bf16_t *p, const float (&x)[V], int skip, bool whole) {
     }
 }
 
-// a = sigmoid(g) and rest = 1 - a, both relative to their own value: with e = exp(-g) = 2^y, a = 1 / (1 + e) and rest = e a.  The
-// argument is held where e stays finite (a below 2^-126 counts as 2^-126).  Rounding y = -g / ln 2 makes e |g| 2^-24 off; in fp32,
-// where memory leaves the time for it, that is taken back, 2^y (1 + r ln 2) with r what the rounding left, and the reciprocal, which is
-// off by a step, takes one of Newton's: a scan is then as close to 64 bits as a sequence of plain fp32 steps (1.2 to 1.6 times as far
-// without) and takes a hundredth longer at most.  In bf16 gate and
-// value are given to 2^-9, and the scan is bound by these instructions.
+// a = sigmoid(g) and rest = 1 - a, both relative to their own value: with e = exp(-g), a = 1 / (1 + e) and rest = e a.  The argument is
+// held where e stays finite (a below 2^-126 counts as 2^-126).  The reciprocal is off by a step, always to one side, and takes one of
+// Newton's: without it states are 1.7 and their gradients 2.6 times as far from 64 bits as a sequence of plain fp32 steps, with it
+// as far (bf16: 44 us for 43 at 16384 steps of 2 of width 512, which these instructions bound).  e is 2^y with y = -g / ln 2; in fp32,
+// where memory leaves the time for it, what rounding y left of the argument, -g - y ln 2, is taken back.
 // (minimum and maximum, unlike fmin and fmax, keep NaN.)
-MRL_DEV void gates(const float *, float g, float &a, float &rest) {
-    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 200.0f);
-    const float y = g * -1.44269502f;
-    const float r = fmaf(g, -1.44269502f, -y);
-    float e = __builtin_amdgcn_exp2f(y);
-    e = fmaf(e, r * 0.693147182f, e);
+MRL_DEV void sigmoid(float e, float &a, float &rest) {
     const float u = 1.0f + e;
     a = __builtin_amdgcn_rcpf(u);
     a = fmaf(a, fmaf(-u, a, 1.0f), a);
     rest = e * a;
 }
+MRL_DEV void gates(const float *, float g, float &a, float &rest) {
+    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 200.0f);
+    const float y = g * -1.44269502f, e = __builtin_amdgcn_exp2f(y);
+    sigmoid(fmaf(e, fmaf(y, -0.693147182f, -g), e), a, rest);
+}
 MRL_DEV void gates(const bf16_t *, float g, float &a, float &rest) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269502f, 125.0f));
-    a = __builtin_amdgcn_rcpf(1.0f + e);
-    rest = e * a;
+    sigmoid(__builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269502f, 125.0f)), a, rest);
 }
 
 struct Scan {

@@ -178,6 +178,26 @@ def test_what_a_cut_hides_goes_nowhere(mrl, ctx, T, N, D):
         near(ds, wants[2], offs[2], 0.0, "grad_state_in")
 
 
+@pytest.mark.parametrize("T,N,D", [(128, 256, 256), (2000, 10, 200), (1, 300, 256)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_states_as_close_as_plain_fp32_steps(mrl, ctx, T, N, D, dtype):
+    """States and their gradients, fp32 in either type, against a sequence of plain fp32 steps: on average within 1.5 times its distance from
+    64 bits (the kernels' steps have as many roundings; a composed step adds its own once more)."""
+    c = Case(T, N, D, dtype)
+    out, last = c.forward(mrl, ctx)
+    _, _, ds = c.backward(mrl, ctx, out)
+    ctx.synchronize()
+    T, N, D = c.shape()
+    gate, value, h, g = (c.host(x, *s).float() for x, s in ((c.gate, (T, N, D)), (c.value, (T, N, D)), (c.state, (N, D)), (c.grad_last, (N, D))))
+    a, grad = 1 / (1 + torch.exp(-gate)), c.host(c.grad_out, T, N, D).float()
+    for t in range(T):
+        h = a[t] * torch.where(c.cut[t][:, None], torch.zeros_like(h), h) + (1 - a[t]) * value[t]
+    for t in range(T - 1, -1, -1):
+        g = torch.where(c.cut[t][:, None], torch.zeros_like(g), a[t] * (grad[t] + g))
+    for got, plain, want, what in ((last, h, c.forward64()[0][-1], "state"), (ds, g, c.backward64(out)[0][2], "gradient")):
+        assert (got.cpu().double() - want).norm() <= 1.5 * (plain.double() - want).norm(), what
+
+
 def test_extreme_gates(mrl, ctx):
     """Closed and open gates, far beyond where the exponential ends, and NaN."""
     inf, nan = float("inf"), float("nan")
