@@ -30,7 +30,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float QA = 3.4445f, QB = -4.7750f, QC = 2.0315f;
 constexpr int MOST = 16;        // matrices of a launch, where they differ
-constexpr size_t BATCH_BYTES = 256 << 20;   // of workspace from which on a launch takes no more matrices that are alike
+constexpr size_t BATCH_BYTES = 256 << 20, GROUP_ROOM = 1 << 30;   // of workspace from which on a launch takes no more matrices, alike or not
 constexpr int LOAD = 32;        // sides of what a workgroup of the second launch takes
 constexpr int CHUNK = 1024;     // elements that a workgroup of the first launch takes at a time
 constexpr int MOST_SUMS = 1024;  // partial sums of squares per matrix
@@ -738,6 +738,17 @@ size_t group_bytes(const S *matrices, int count) {
     for (int k = 0; k < count; ++k) bytes += matrix_bytes(matrices[k].rows, matrices[k].cols);
     return bytes;
 }
+// How many of these a launch takes.
+template <class S>
+int group_of(const S *matrices, int left) {
+    size_t bytes = 0;
+    int k = 0;
+    for (; k < std::min(MOST, left); ++k) {
+        bytes += matrix_bytes(matrices[k].rows, matrices[k].cols);
+        if (k > 0 && bytes > GROUP_ROOM) break;
+    }
+    return k;
+}
 // Of `count` alike: how many a launch takes, and their workspace.  256 of 64 x 64 in one launch 21 us, sixteen at a time 319; 64 of
 // 256 x 256 255 and 397.
 int batch_of(int count, int rows, int cols) {
@@ -745,7 +756,7 @@ int batch_of(int count, int rows, int cols) {
     size_t lds;
     m.rows = rows;
     m.cols = cols;
-    const size_t room = is_whole(&m, 1, lds) ? 1 << 20 : std::max<size_t>(MOST, BATCH_BYTES / matrix_bytes(rows, cols));
+    const size_t room = is_whole(&m, 1, lds) ? 1 << 20 : std::max<size_t>(1, BATCH_BYTES / matrix_bytes(rows, cols));
     return (int)std::min<size_t>(count, room);
 }
 size_t batch_bytes(int count, int rows, int cols) {
@@ -967,8 +978,9 @@ int mrl_muon_workspace(int n_matrices, const mrl_matrix *matrices, uint64_t *byt
     const int rc = mrl::check_matrices(who, n_matrices, matrices, INT64_MAX);
     if (rc != MRL_OK) return rc;
     *bytes = 0;
-    for (int done = 0; done < n_matrices; done += mrl::MOST) {
-        *bytes = std::max<uint64_t>(*bytes, mrl::group_bytes(matrices + done, std::min(mrl::MOST, n_matrices - done)));
+    for (int done = 0, group; done < n_matrices; done += group) {
+        group = mrl::group_of(matrices + done, n_matrices - done);
+        *bytes = std::max<uint64_t>(*bytes, mrl::group_bytes(matrices + done, group));
     }
     return MRL_OK;
 }
@@ -1001,7 +1013,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
         g.beta1 = (float)beta1; g.beta2 = (float)beta2; g.omb1 = (float)(1.0 - beta1); g.omb2 = (float)(1.0 - beta2);
         g.adam_eps = (float)adam_eps;
         g.bc1 = (float)(1.0 - pow(beta1, (double)t)); g.bc2 = (float)(1.0 - pow(beta2, (double)t));
-        g.count = std::min(mrl::MOST, n_matrices - done);
+        g.count = mrl::group_of(matrices + done, n_matrices - done);
         auto rest = [&](int64_t to) {
             if (to > at) g.rest[g.rests++] = {params + at, grads + at, reinterpret_cast<float2 *>(state) + at, (long)(to - at)};
         };

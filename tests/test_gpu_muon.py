@@ -81,7 +81,7 @@ def test_many_matrices_in_place_at_odd_addresses(mrl, ctx, count, rows, cols, dt
 # shapes whose products are worked out in larger tiles, alone and in batches, with rows and columns behind the last whole tile; batches
 # in one launch, in one per product, and in more than one
 @pytest.mark.parametrize("count,rows,cols,dtype", [(12, 519, 513, "f32"), (15, 449, 511, "bf16"), (8, 643, 701, "f32"), (60, 129, 191, "f32"), (6, 831, 385, "f32"),
-                                                   (22, 193, 521, "bf16"), (1, 1411, 1500, "f32"), (5, 485, 2467, "f32"), (700, 20, 33, "f32"), (300, 65, 64, "bf16"), (650, 100, 130, "f32")])
+                                                   (22, 193, 521, "bf16"), (1, 1411, 1500, "f32"), (5, 485, 2467, "f32"), (700, 20, 33, "f32"), (300, 65, 64, "bf16"), (650, 100, 130, "f32"), (14, 999, 1000, "bf16")])
 def test_batches(mrl, ctx, count, rows, cols, dtype):
     print("batch", count, rows, cols, dtype, flush=True)
     gen = torch.Generator().manual_seed(count + rows)
@@ -245,6 +245,29 @@ def test_more_matrices_than_a_launch_takes(mrl, ctx, large):
     assert torch.equal(s, one[2])
     # (a matrix in a launch of its own is worked out in other tiles: sums in another order, entries of at most 1.2 * 0.1 * sqrt(1.5))
     assert (p - one[0]).abs().max() <= 0.15 * 2.0 ** -14
+
+
+def test_large_matrices_go_one_by_one(mrl, ctx):
+    """Two matrices whose planes take more than a launch's share of a workspace: as each in a call of its own."""
+    lib, Matrix, rows, cols = mrl._lib.lib(), mrl._lib.Matrix, 6000, 6100
+    size, need = rows * cols, ctypes.c_uint64(0)
+    mats = [Matrix(7, rows, cols), Matrix(size + 20, rows, cols)]
+    assert lib.mrl_muon_workspace(2, (Matrix * 2)(*mats), ctypes.byref(need)) == 0
+    n = 2 * size + 30
+    torch.cuda.manual_seed(1)
+    p, g, s = torch.randn(n, device="cuda"), torch.randn(n, device="cuda"), torch.zeros(2 * n, device="cuda")
+    one, ws = [p.clone(), s.clone()], torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+
+    def step(params, grads, state, matrices):
+        array = (Matrix * len(matrices))(*matrices)
+        assert lib.mrl_muon_step(ctx.handle, *(ctypes.c_void_p(t.data_ptr()) for t in (params, grads, state)), params.numel(), len(matrices), array, 1, 0.1, 0.9, 1, 0.0, 5,
+                                 1e-7, 1e-3, 0.9, 0.99, 1e-8, ctypes.c_void_p(ws.data_ptr()), ws.numel()) == 0, lib.mrl_last_error()
+    step(p, g, s, mats)
+    step(one[0][:size + 20], g[:size + 20], one[1][:2 * size + 40], mats[:1])
+    step(one[0][size + 20:], g[size + 20:], one[1][2 * size + 40:], [Matrix(0, rows, cols)])
+    ctx.synchronize()
+    assert torch.equal(p, one[0]) and torch.equal(s, one[1]) and p.isfinite().all()
 
 
 def test_network_with_muon_trains_and_round_trips(mrl, ctx, tmp_path):

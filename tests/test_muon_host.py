@@ -67,6 +67,14 @@ def test_null_contexts_and_workspace_queries(mrl):
     assert size.value >= 3 * (6 * 2 * 340 * 400 + 4 * 2 * 340 * 340)
     mrl._lib.call("mrl_orthogonalize_workspace", 3, 40, 30, ctypes.byref(size))
     assert size.value == 0   # (held in LDS)
+    mrl._lib.call("mrl_orthogonalize_workspace", 1, 1 << 15, 1 << 15, ctypes.byref(size))
+    one = size.value
+    mrl._lib.call("mrl_orthogonalize_workspace", 1000, 1 << 15, 1 << 15, ctypes.byref(size))
+    assert size.value == one   # (a large matrix fills the device by itself)
+    Matrix = mrl._lib.Matrix
+    large = (Matrix * 20)(*[Matrix(k << 30, 1 << 15, 1 << 15) for k in range(20)])
+    mrl._lib.call("mrl_muon_workspace", 20, large, ctypes.byref(size))
+    assert size.value == one
     mrl._lib.call("mrl_muon_workspace", 0, None, ctypes.byref(size))
     assert size.value == 0
     for name, args in (("mrl_orthogonalize", (None, 0, 1, 4, 4, None, None, 5, 1e-7, None, 0)),
