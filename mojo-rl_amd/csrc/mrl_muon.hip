@@ -188,8 +188,7 @@ MRL_DEV double scale_of(const Group &g, const Mat &m, double *part) {
     }
     return (double)m.sx / (sqrt(part[0]) + g.eps);
 }
-// A square of X and of its transpose in pieces, through LDS: read along the caller's rows, written along both sides (5.3 us for 256 x
-// 256, 17 for 2048 x 2048: 3 TB/s, a fortieth of the whole).
+// A square of X and of its transpose in pieces, through LDS: read along the caller's rows, written along both sides.
 template <int KIND>
 MRL_DEV void load_square(const Group &g, const Mat &m, int block, double scale, float (&tile)[LOAD][LOAD + 1]) {
     const int across = m.np / LOAD, i0 = block / across * LOAD, j0 = block % across * LOAD;
@@ -211,13 +210,21 @@ MRL_DEV void load_square(const Group &g, const Mat &m, int block, double scale, 
         Piece(f32x4{tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]}).store(planes(&g, m.xt) + square_at(m.np, j0 + r, i0) + in);
     }
 }
+// 5 us for 256 x 256, 16 for 2048 x 2048, a thirtieth of the whole: 3 TB/s.  Up to eight workgroups a CU, so that the norm is taken less
+// often (a workgroup per square: 18 us, four of 1024 x 1024 19 for 15).
 template <int KIND>
 __global__ __launch_bounds__(256) void load_kernel(const Group *__restrict__ group) {
     const Group &g = *group;
     __shared__ double part[256];
     __shared__ float tile[LOAD][LOAD + 1];
     const Mat m = matrix<KIND>(g, described(g.mat[describes<KIND>(blockIdx.y)]), blockIdx.y);
-    if ((int)blockIdx.x < m.mp / LOAD * (m.np / LOAD)) load_square<KIND>(g, m, blockIdx.x, scale_of(g, m, part), tile);
+    const int squares = m.mp / LOAD * (m.np / LOAD);
+    if ((int)blockIdx.x >= squares) return;
+    const double scale = scale_of(g, m, part);
+    for (int block = blockIdx.x; block < squares; block += gridDim.x) {
+        load_square<KIND>(g, m, block, scale, tile);
+        __syncthreads();
+    }
 }
 
 // 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
@@ -889,6 +896,7 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
     sym *= copies;
     update *= copies;
     hipLaunchKernelGGL(sums_kernel<KIND>, dim3(std::max<long>(sums, rest), g.count + (rest > 0)), dim3(threads), 0, ctx->stream, g, kept);
+    load = std::min(load, std::max(1, 8 * ctx->n_cus / g.count));
     hipLaunchKernelGGL(load_kernel<KIND>, dim3(load, g.count), dim3(256), 0, ctx->stream, kept);
     for (int s = 0; s < steps; ++s) {
         product<GRAM, KIND>(ctx, g, kept, sym, s & 1, 0);
