@@ -69,7 +69,8 @@ class Muon:
         v <- momentum v + g;   u = g + momentum v (nesterov; else v);   W <- (1 - lr weight_decay) W - lr sqrt(max(1, out / in)) O(u),
 
     O as in orthogonalize(steps, eps).  Biases and the other layers are updated as by Adam(adam_lr, beta1, beta2, adam_eps).  State is
-    Adam's; a matrix's share of it starts with v."""
+    Adam's; a matrix's share of it starts with v.  For networks updated by Network.update_gpu: PPOUpdate, and with it the agents,
+    apply Adam in kernels of their own and refuse a Muon."""
     STATE_PER_PARAM = 2
 
     def __init__(self, model, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7, layers=None, adam_lr=3e-4,

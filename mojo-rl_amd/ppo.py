@@ -6,6 +6,7 @@ import torch
 
 from . import _lib
 from .context import _ptr
+from .optimizer import Adam
 
 
 def sample_actions(ctx, logits, actions, log_probs, seed):
@@ -250,6 +251,13 @@ def rollout_fused(desc):
     return bool(_lib.call("mrl_rollout_fused", C.byref(desc)))
 
 
+def _fused_adam(opt):
+    """`opt` where its step is Adam's, which the update's kernels apply themselves; another optimiser's would not be asked."""
+    if getattr(type(opt), "step_gpu", Adam.step_gpu) is not Adam.step_gpu:
+        raise _lib.MrlError("the PPO update applies Adam itself and cannot run %s: update such a network by Network.update_gpu" % type(opt).__name__)
+    return opt
+
+
 class PPOUpdate:
     """Phases 2 and 3 of train_gpu (deep_agents/ppo/ppo.mojo:2296-2727 for the discrete agent,
     ppo_continuous.mojo:2852-3260 for the continuous one) on device buffers: bootstrap value,
@@ -258,14 +266,14 @@ class PPOUpdate:
     critic forward / loss gradient / backward / clip / Adam (/ log_std clamp).  Nothing is copied
     to the host inside an epoch: the KL early-stop test runs on the device after every actor
     loss gradient, an update is not applied once it has fired (the reference's `break`), and
-    the flag is read once per epoch."""
+    the flag is read once per epoch.  Both optimisers are Adam; MrlError for any other."""
 
     def __init__(self, ctx, rb, minibatch, actor_opt, critic_opt, gamma=0.99, gae_lambda=0.95,
                  clip_epsilon=0.2, entropy_coef=0.01, value_loss_coef=0.5, max_grad_norm=0.5,
                  clip_value=True, normalize_advantages=True, norm_adv_per_minibatch=True,
                  target_kl=0.015, normalize_rewards=False):
         self.ctx, self.rb, self.mb = ctx, rb, minibatch
-        self.actor_opt, self.critic_opt = actor_opt, critic_opt
+        self.actor_opt, self.critic_opt = _fused_adam(actor_opt), _fused_adam(critic_opt)
         self.gamma, self.gae_lambda = gamma, gae_lambda
         self.clip_epsilon, self.entropy_coef, self.value_loss_coef = clip_epsilon, entropy_coef, value_loss_coef
         self.max_grad_norm, self.clip_value = max_grad_norm, clip_value
@@ -296,6 +304,7 @@ class PPOUpdate:
 
     def descriptor(self):
         """The mrl_update view of this object (buffers, hyper-parameters, current learning rates)."""
+        a, c = _fused_adam(self.actor_opt), _fused_adam(self.critic_opt)
         rb, u = self.rb, _lib.Update()
         u.minibatch, u.obs_dim, u.act_width = self.mb, rb.env.OBS_DIM, rb.act_width
         u.continuous = 1 if self.continuous else 0
@@ -315,7 +324,6 @@ class PPOUpdate:
         u.clip_epsilon, u.entropy_coef, u.value_loss_coef = self.clip_epsilon, self.entropy_coef, self.value_loss_coef
         u.max_grad_norm, u.target_kl = self.max_grad_norm, self.target_kl
         u.clip_value, u.norm_adv_per_minibatch = int(self.clip_value), int(self.norm_adv_per_minibatch)
-        a, c = self.actor_opt, self.critic_opt
         if (a.beta1, a.beta2, a.eps) != (c.beta1, c.beta2, c.eps):
             raise _lib.MrlError("actor and critic optimisers must share beta1, beta2 and eps")
         u.actor_lr, u.critic_lr, u.beta1, u.beta2, u.eps = a.lr, c.lr, a.beta1, a.beta2, a.eps

@@ -84,3 +84,31 @@ def test_null_contexts_and_workspace_queries(mrl):
     for args in ((1, 0, 4), (-1, 4, 4), (1, 4, 1 << 16)):
         with pytest.raises(mrl.MrlError):
             mrl._lib.call("mrl_orthogonalize_workspace", *args, ctypes.byref(size))
+
+
+def test_ppo_update_refuses_what_is_not_adam(mrl):
+    """The update's kernels apply Adam with the optimiser's lr, beta1, beta2 and eps, which mean something else in Muon."""
+    actor = mrl.seq(mrl.LinearReLU(4, 64), mrl.LinearReLU(64, 64), mrl.Linear(64, 2))
+    critic = mrl.seq(mrl.LinearReLU(4, 64), mrl.LinearReLU(64, 64), mrl.Linear(64, 1))
+    rb = mrl.ppo.RolloutBuffers(HostContext, mrl.CartPoleEnv, actor, critic, 5, 3)
+    for cls in (mrl.ppo.PPOUpdate, mrl.ppo.DiscreteUpdate, mrl.ppo.ContinuousUpdate):
+        for opts in ((mrl.Muon(actor), mrl.Muon(critic)), (mrl.Muon(actor), mrl.Adam()), (mrl.Adam(), mrl.Muon(critic))):
+            with pytest.raises(mrl.MrlError, match="cannot run Muon"):
+                cls(HostContext, rb, 4, *opts)
+
+    class Mine(mrl.Adam):
+        pass
+    upd = mrl.ppo.PPOUpdate(HostContext, rb, 4, Mine(lr=0.1), mrl.Adam(lr=0.2))
+    upd.actor_opt = mrl.Muon(actor)          # (put in place of the first one later)
+    with pytest.raises(mrl.MrlError, match="cannot run Muon"):
+        upd.minibatch_step(torch.zeros(4, dtype=torch.int32))
+    assert upd.actor_opt.t == 0 and upd.critic_opt.t == 0
+
+
+def test_agent_with_muon_networks_refuses_to_train(mrl):
+    agent = mrl.DeepPPOAgent(obs_dim=4, num_actions=2, hidden_dim=64, n_envs=4, rollout_len=8, gpu_minibatch_size=16)
+    am, cm = agent._nets()
+    net = lambda model: type("Net", (), dict(model=model, params=torch.zeros(model.PARAM_SIZE), optimizer=mrl.Muon(model)))  # noqa: E731
+    agent.actor, agent.critic = net(am), net(cm)
+    with pytest.raises(mrl.MrlError, match="cannot run Muon"):
+        agent._build(HostContext, mrl.CartPoleEnv)
