@@ -365,6 +365,78 @@ MRL_DEV void operands(const Group &g, const Mat &m, int from, const _Float16 *&P
     blocks = (STAGE == GRAM ? m.np : m.mp) / 32;
 }
 
+// A tile of 32 x 32 by four wavefronts that share the contracted index, operands straight to registers.  `there`: whether these four have
+// a tile, or only come to the barrier.
+typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
+template <int STAGE, int KIND>
+MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums, bool there = true) {
+    const _Float16 *P, *Q;
+    int blocks;
+    operands<STAGE>(g, m, from, P, Q, blocks);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int p_fragments = m.mp / 16, q_fragments = (STAGE == UPDATE ? m.np : m.mp) / 16;
+    const _Float16 *p = P + bi * 2 * 1024 + lane * 8, *q = Q + bj * 2 * 1024 + lane * 8;
+    f32x4 acc[2][2] = {};
+    const int fi = (bi * 2 + (wave >> 1)) * 16, fj = (bj * 2 + (wave & 1)) * 16;
+    Piece piece;
+    if (there) ask<STAGE>(g, m, from, fi, fj, piece);
+    struct Operands { f16x8 ph[2], pl[2], qh[2], ql[2]; };
+    auto load = [&](int kb, Operands &o) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const _Float16 *pf = p + ((size_t)kb * p_fragments + f) * 1024, *qf = q + ((size_t)kb * q_fragments + f) * 1024;
+            o.ph[f] = *reinterpret_cast<const f16x8 *>(pf);
+            o.pl[f] = *reinterpret_cast<const f16x8 *>(pf + 512);
+            o.qh[f] = *reinterpret_cast<const f16x8 *>(qf);
+            o.ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
+        }
+    };
+    const bool few = m.m <= FEW;   // then the other squares are of zeros
+    if (!there || (few && (bi > 0 || (STAGE != UPDATE && bj > 0)))) blocks = 0;
+    auto work = [&](const Operands &o) {
+        if (few) {
+            multiply_few(o.ph[0], o.pl[0], o.qh[0], o.ql[0], acc[0][0]);
+            if (STAGE == UPDATE) multiply_few(o.ph[0], o.pl[0], o.qh[1], o.ql[1], acc[0][1]);
+            return;
+        }
+        multiply<2>(o.pl, o.qh, acc);
+        multiply<2>(o.ph, o.ql, acc);
+        multiply<2>(o.ph, o.qh, acc);
+    };
+    // two steps' operands under way together (more bring nothing)
+    int kb = wave;
+    for (; kb + 4 < blocks; kb += 8) {
+        Operands one, two;
+        load(kb, one);
+        load(kb + 4, two);
+        work(one);
+        work(two);
+    }
+    if (kb < blocks) {
+        Operands one;
+        load(kb, one);
+        work(one);
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
+    __syncthreads();
+    const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
+    if (there) finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
+}
+// Tile (bi, bj) of a side of 32 F of a matrix with few rows, whose neighbours in the launch have more: in squares of 32 x 32, one behind the
+// other for each 256 lanes, so that such a matrix comes out the same bit by bit whatever it is updated with.  (8-1024-1024-1024-4 takes
+// 301 us with the fp16 cores for its first layer too: the squares are done before the other layers' tiles are.)
+template <int STAGE, int KIND, int F>
+MRL_DEV void few_squares(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums *sums) {
+    const int teams = blockDim.x / 256, team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int rows = min(F, m.mp / 32 - bi * F), columns = min(F, (STAGE == UPDATE ? m.np : m.mp) / 32 - bj * F);
+    for (int k0 = 0; k0 < rows * columns; k0 += teams) {
+        const int k = k0 + team, i = bi * F + k % rows, j = bj * F + k / rows;
+        small_product<STAGE, KIND>(g, m, i, j, from, last, sums[team], k < rows * columns && (STAGE == UPDATE || i <= j));
+        __syncthreads();
+    }
+}
+
 // a wavefront's KiB of hi (0) or lo (1) from memory to LDS (the offset counts on both sides)
 template <int PIECE>
 MRL_DEV void bring(const _Float16 *from, _Float16 *to) {
@@ -407,6 +479,11 @@ __global__ __launch_bounds__(64 * WAVES<F> * SETS) void product_kernel(const Gro
     extern __shared__ _Float16 lds[];
     int bi, bj;
     const Mat m = find_tile<STAGE, KIND, 32 * F>(g, count, tiles, bi, bj);
+    static_assert(RING_BYTES<F, SETS> >= sizeof(SmallSums) * WAVES<F> * SETS / 4, "sums of every four wavefronts");
+    if (KIND == MUON && m.m <= FEW) {   // (matrices that are alike go to tiles of 32 in this case)
+        few_squares<STAGE, KIND, F>(g, m, bi, bj, from, last, reinterpret_cast<SmallSums *>(lds));
+        return;
+    }
     const _Float16 *P, *Q;
     int blocks;
     operands<STAGE>(g, m, from, P, Q, blocks);
@@ -536,63 +613,8 @@ __global__ __launch_bounds__(64 * WAVES<F> * SETS) void product_kernel(const Gro
 }
 
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
-// 32 x 32 per workgroup, the contracted index shared by its four wavefronts, operands straight to registers.  256 x 256: 4.2, 4.3 and
-// 4.6 us for the three, most of it the launch and the trips to memory one behind the other (description, operands, sums).
-typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
-template <int STAGE, int KIND>
-MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums) {
-    const _Float16 *P, *Q;
-    int blocks;
-    operands<STAGE>(g, m, from, P, Q, blocks);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int p_fragments = m.mp / 16, q_fragments = (STAGE == UPDATE ? m.np : m.mp) / 16;
-    const _Float16 *p = P + bi * 2 * 1024 + lane * 8, *q = Q + bj * 2 * 1024 + lane * 8;
-    f32x4 acc[2][2] = {};
-    const int fi = (bi * 2 + (wave >> 1)) * 16, fj = (bj * 2 + (wave & 1)) * 16;
-    Piece piece;
-    ask<STAGE>(g, m, from, fi, fj, piece);
-    struct Operands { f16x8 ph[2], pl[2], qh[2], ql[2]; };
-    auto load = [&](int kb, Operands &o) {
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const _Float16 *pf = p + ((size_t)kb * p_fragments + f) * 1024, *qf = q + ((size_t)kb * q_fragments + f) * 1024;
-            o.ph[f] = *reinterpret_cast<const f16x8 *>(pf);
-            o.pl[f] = *reinterpret_cast<const f16x8 *>(pf + 512);
-            o.qh[f] = *reinterpret_cast<const f16x8 *>(qf);
-            o.ql[f] = *reinterpret_cast<const f16x8 *>(qf + 512);
-        }
-    };
-    const bool few = m.m <= FEW;   // then the other squares are of zeros
-    auto work = [&](const Operands &o) {
-        if (few) {
-            multiply_few(o.ph[0], o.pl[0], o.qh[0], o.ql[0], acc[0][0]);
-            if (STAGE == UPDATE) multiply_few(o.ph[0], o.pl[0], o.qh[1], o.ql[1], acc[0][1]);
-            return;
-        }
-        multiply<2>(o.pl, o.qh, acc);
-        multiply<2>(o.ph, o.ql, acc);
-        multiply<2>(o.ph, o.qh, acc);
-    };
-    // two steps' operands under way together (more bring nothing)
-    int kb = wave;
-    for (; kb + 4 < blocks; kb += 8) {
-        Operands one, two;
-        load(kb, one);
-        load(kb + 4, two);
-        work(one);
-        work(two);
-    }
-    if (kb < blocks) {
-        Operands one;
-        load(kb, one);
-        work(one);
-    }
-#pragma unroll
-    for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
-    __syncthreads();
-    const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
-    finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
-}
+// 32 x 32 per workgroup, straight to registers.  256 x 256: 4.2, 4.3 and 4.6 us for the three, most of it the launch and the trips to
+// memory one behind the other (description, operands, sums).
 template <int STAGE, int KIND>
 __global__ __launch_bounds__(256) void small_product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
@@ -875,7 +897,7 @@ void run(const mrl_ctx *ctx, Group &g, int steps, void *workspace) {
         else launch(whole_kernel<KIND, false>);   // (a twentieth faster)
         return;
     }
-    const bool few = KIND != MUON && g.mat[0].m <= FEW;   // (worked out in tiles of 32 only)
+    const bool few = KIND != MUON && g.mat[0].m <= FEW;   // (worked out in squares of 32 whatever the tile)
     g.sym_tile = few ? 32 : tile_of(ctx, g, described, copies, true);
     g.update_tile = few ? 32 : tile_of(ctx, g, described, copies, false);
     std::fill(g.begin_sym, g.begin_sym + MOST, INT_MAX);

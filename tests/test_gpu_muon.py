@@ -270,6 +270,45 @@ def test_large_matrices_go_one_by_one(mrl, ctx):
     assert torch.equal(p, one[0]) and torch.equal(s, one[1]) and p.isfinite().all()
 
 
+@pytest.mark.parametrize("thin,others", [((9, 700), [(700, 700)] * 2), ((700, 9), [(700, 700)] * 2), ((8, 1024), [(1024, 1024)] * 2), ((16, 1000), [(1000, 1000)] * 3),
+                                         ((1400, 16), [(900, 1400)]), ((5, 1500), [(1500, 1500)]), ((1, 900), [(600, 600)] * 6), ((2, 3000), [(2048, 2048)] * 2)])
+def test_thin_matrix_does_not_go_by_its_neighbours(mrl, ctx, thin, others):
+    """A matrix of up to 16 rows beside ones whose products are worked out in tiles of 64, 96 and 128: bit by bit what it is by itself, and as
+    close to 64 bits as products in fp32."""
+    print("thin", thin, others, flush=True)
+    lib, Matrix, rows, cols = mrl._lib.lib(), mrl._lib.Matrix, *thin
+    gen = torch.Generator().manual_seed(rows * cols)
+    off = plain = 0.0
+    large = torch.randn(sum(r * c for r, c in others), generator=gen).cuda()
+    for seed in range(4):
+        x = matrix(gen, rows, cols)
+        grads = torch.cat((x.reshape(-1).cuda(), large))
+        got = []
+        for shapes in ([thin], [thin] + others):
+            mats, at = [], 0
+            for r, c in shapes:
+                mats.append(Matrix(at, r, c))
+                at += r * c
+            array, need = (Matrix * len(mats))(*mats), ctypes.c_uint64(0)
+            assert lib.mrl_muon_workspace(len(mats), array, ctypes.byref(need)) == 0
+            ws, p, s = torch.empty(max(16, need.value), dtype=torch.uint8, device="cuda"), torch.zeros(at, device="cuda"), torch.zeros(2 * at, device="cuda")
+            torch.cuda.synchronize()
+            # momentum 0 and a rate of 1: the parameters become minus the polynomial, times the shape's factor
+            assert lib.mrl_muon_step(ctx.handle, *(ctypes.c_void_p(t.data_ptr()) for t in (p, grads, s)), at, len(mats), array, 1, 1.0, 0.0, 0, 0.0, 5, 1e-7, 1e-3, 0.9, 0.99,
+                                     1e-8, ctypes.c_void_p(ws.data_ptr()), ws.numel()) == 0, lib.mrl_last_error()
+            ctx.synchronize()
+            got.append(p[:rows * cols].cpu().view(rows, cols))
+        assert torch.equal(*got)
+        want, y = polynomial(x), (x if rows <= cols else x.T) / (x.norm() + 1e-7)
+        for _ in range(5):
+            gram = y @ y.T
+            y = NS[0] * y + (NS[1] * gram + NS[2] * gram @ gram) @ y
+        off += ((-got[1].double() / max(1.0, cols / rows) ** 0.5 - want).norm() / want.norm()).item()
+        plain += (((y if rows <= cols else y.T).double() - want).norm() / want.norm()).item()
+    # (operands of 22 bits are rounded up to twice as far as those of 24)
+    assert off <= 2 * plain
+
+
 def test_network_with_muon_trains_and_round_trips(mrl, ctx, tmp_path):
     """Behind Network as any optimiser: the parameters after update_gpu are those of the step on its own buffers, a checkpoint holds the momentum."""
     model = mrl.seq(mrl.LinearTanh(6, 48), mrl.LinearTanh(48, 48), mrl.Linear(48, 2))
