@@ -367,8 +367,12 @@ MRL_DEV void operands(const Group &g, const Mat &m, int from, const _Float16 *&P
 
 // A tile of 32 x 32 by four wavefronts that share the contracted index, operands straight to registers.  `there`: whether these four have
 // a tile, or only come to the barrier.
+// LONG: every STRETCH blocks of 32 of the contracted index begin sums of their own, so that rounding costs as much at 32768 as at 4096
+// (64 rows: 1.6e-6 off 64 bits at 4096, at 32768 2.9e-6 in one sum, 1.5e-6 in stretches).  The registers that it takes cost shorter
+// sums 0.2 us a launch, 256 x 256 69 us for 66.
+constexpr int STRETCH = 128;
 typedef f32x4 SmallSums[4][4][64];   // [fragment][wavefront][lane]
-template <int STAGE, int KIND>
+template <int STAGE, int KIND, bool LONG>
 MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums &sums, bool there = true) {
     const _Float16 *P, *Q;
     int blocks;
@@ -403,19 +407,36 @@ MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int fro
         multiply<2>(o.ph, o.ql, acc);
         multiply<2>(o.ph, o.qh, acc);
     };
-    // two steps' operands under way together (more bring nothing)
-    int kb = wave;
-    for (; kb + 4 < blocks; kb += 8) {
-        Operands one, two;
-        load(kb, one);
-        load(kb + 4, two);
-        work(one);
-        work(two);
-    }
-    if (kb < blocks) {
-        Operands one;
-        load(kb, one);
-        work(one);
+    auto stretch = [&](int start, int end) {
+        // two steps' operands under way together (more bring nothing)
+        int kb = start + wave;
+        for (; kb + 4 < end; kb += 8) {
+            Operands one, two;
+            load(kb, one);
+            load(kb + 4, two);
+            work(one);
+            work(two);
+        }
+        if (kb < end) {
+            Operands one;
+            load(kb, one);
+            work(one);
+        }
+    };
+    if (LONG) {
+        f32x4 total[2][2] = {};
+        for (int start = 0; start < blocks; start += STRETCH) {
+            stretch(start, min(blocks, start + STRETCH));
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                total[f >> 1][f & 1] = total[f >> 1][f & 1] + acc[f >> 1][f & 1];
+                acc[f >> 1][f & 1] = f32x4{};
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[f >> 1][f & 1] = total[f >> 1][f & 1];
+    } else {
+        stretch(0, blocks);
     }
 #pragma unroll
     for (int f = 0; f < 4; ++f) sums[f][wave][lane] = acc[f >> 1][f & 1];
@@ -432,7 +453,7 @@ MRL_DEV void few_squares(const Group &g, const Mat &m, int bi, int bj, int from,
     const int rows = min(F, m.mp / 32 - bi * F), columns = min(F, (STAGE == UPDATE ? m.np : m.mp) / 32 - bj * F);
     for (int k0 = 0; k0 < rows * columns; k0 += teams) {
         const int k = k0 + team, i = bi * F + k % rows, j = bj * F + k / rows;
-        small_product<STAGE, KIND>(g, m, i, j, from, last, sums[team], k < rows * columns && (STAGE == UPDATE || i <= j));
+        small_product<STAGE, KIND, STAGE == GRAM>(g, m, i, j, from, last, sums[team], k < rows * columns && (STAGE == UPDATE || i <= j));
         __syncthreads();
     }
 }
@@ -615,13 +636,13 @@ __global__ __launch_bounds__(64 * WAVES<F> * SETS) void product_kernel(const Gro
 // The same for small matrices, where a product is shorter than the way of a stage through memory and LDS and back: a tile of
 // 32 x 32 per workgroup, straight to registers.  256 x 256: 4.2, 4.3 and 4.6 us for the three, most of it the launch and the trips to
 // memory one behind the other (description, operands, sums).
-template <int STAGE, int KIND>
+template <int STAGE, int KIND, bool LONG>
 __global__ __launch_bounds__(256) void small_product_kernel(const Group *__restrict__ group, int count, int tiles, int from, int last) {
     const Group &g = *group;
     __shared__ SmallSums sums;
     int bi, bj;
     const Mat m = find_tile<STAGE, KIND, 32>(g, count, tiles, bi, bj);
-    small_product<STAGE, KIND>(g, m, bi, bj, from, last, sums);
+    small_product<STAGE, KIND, LONG>(g, m, bi, bj, from, last, sums);
 }
 
 // A small matrix by one workgroup in one launch, the optimiser's part included: all operands stay in LDS, sixteen wavefronts take
@@ -870,7 +891,8 @@ void product(const mrl_ctx *ctx, const Group &g, const Group *kept, int tiles, i
     else if (tile == 96) launch(product_kernel<STAGE, KIND, 3, 2>, RING_BYTES<3, 2>, 512);
     else if (tile == 64 && tiles <= ctx->n_cus && K > TWO_SETS) launch(product_kernel<STAGE, KIND, 2, 2>, RING_BYTES<2, 2>, 512);
     else if (tile == 64) launch(product_kernel<STAGE, KIND, 2, 1>, RING_BYTES<2, 1>);
-    else launch(small_product_kernel<STAGE, KIND>, 0);
+    else if (STAGE == GRAM && K > 32 * STRETCH) launch(small_product_kernel<STAGE, KIND, STAGE == GRAM>, 0);   // (what the others contract is short in tiles of 32)
+    else launch(small_product_kernel<STAGE, KIND, false>, 0);
 }
 
 template <int KIND>

@@ -309,6 +309,27 @@ def test_thin_matrix_does_not_go_by_its_neighbours(mrl, ctx, thin, others):
     assert off <= 2 * plain
 
 
+@pytest.mark.parametrize("rows", [24, 64, 96])
+def test_long_rows_cost_no_precision(mrl, ctx, rows):
+    """The distance from 64 bits does not grow with the length of the rows: a sum is rounded in pieces of a fixed length, and joining eight
+    of them adds about an eighth (in the root of the squares 1.06); the rest of the 1.5 is for the spread between matrices."""
+    off = []
+    for cols in (4096, 32768):
+        total = 0.0
+        for seed in range(6):
+            gen = torch.Generator(device="cuda").manual_seed(300 + seed)
+            rank = rows // 8
+            x = torch.randn(rows, rank, device="cuda", generator=gen) @ torch.randn(rank, cols, device="cuda", generator=gen) / math.sqrt(rank)
+            x += 0.5 * torch.randn(rows, cols, device="cuda", generator=gen)
+            out = torch.empty_like(x)
+            mrl.orthogonalize(ctx, out, x)
+            want = polynomial(x)
+            total += ((out.double() - want).norm() / want.norm()).item()
+        off.append(total / 6)
+    print(rows, off, flush=True)
+    assert off[1] <= 1.5 * off[0]
+
+
 def test_network_with_muon_trains_and_round_trips(mrl, ctx, tmp_path):
     """Behind Network as any optimiser: the parameters after update_gpu are those of the step on its own buffers, a checkpoint holds the momentum."""
     model = mrl.seq(mrl.LinearTanh(6, 48), mrl.LinearTanh(48, 48), mrl.Linear(48, 2))
