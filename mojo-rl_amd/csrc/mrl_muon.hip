@@ -339,8 +339,9 @@ MRL_DEV void finish(const Group &g, const Mat &m, int from, int last, bool diago
 
 // Products of up to FEW rows on the fp32 matrix cores, which round every sum to nearest.  The fp16 ones add eight products at a time and
 // cut off what is below 2^-23 of the largest, so their errors go towards 0, and with few rows the same way in every entry.  Off from 64
-// bits, fp16 / fp32 / plain fp32: 8 x 64 1.7e-6, 0.8e-6, 0.8e-6; 1 x 500 1.1e-6, 0.4e-6, 0.4e-6; 8 x 721 1.6e-6, 1.1e-6, 0.9e-6; with 17
-// rows and more fp16 is as good, with 64 better.  (16 x 16: 18 us for 14.)
+// bits, fp16 / fp32 / plain fp32: 8 x 64 1.7e-6, 0.8e-6, 0.8e-6; 1 x 500 1.1e-6, 0.4e-6, 0.4e-6; 8 x 721 1.6e-6, 1.1e-6, 0.9e-6.  On the fp16
+// ones matrices of 17 to 48 rows are 0.4 to 1.4 times as far off as plain fp32 products, of 64 and more 0.3 to 1.1 times.  (16 x 16: 18 us
+// for 14.)
 constexpr int FEW = 16;
 // 16 x 16 sums over 32 of the contracted index, four at a time
 MRL_DEV void multiply_few(const f16x8 &ph, const f16x8 &pl, const f16x8 &qh, const f16x8 &ql, f32x4 &acc) {

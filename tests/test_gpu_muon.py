@@ -119,6 +119,13 @@ def test_few_rows_as_close_as_fp32_products(mrl, ctx, rows, cols):
     assert off <= 2 * plain
 
 
+@pytest.mark.parametrize("rows", [17, 20, 24, 33, 48, 64])
+@pytest.mark.parametrize("cols", [64, 300, 1000])
+def test_more_rows_as_close_as_fp32_products(mrl, ctx, rows, cols):
+    """From 17 rows on products are taken on the fp16 cores: on average within twice what fp32 products are off, as those of fewer rows."""
+    test_few_rows_as_close_as_fp32_products(mrl, ctx, rows, cols)
+
+
 @pytest.mark.parametrize("steps,eps", [(1, 1e-7), (2, 1e-3), (3, 0.0), (8, 1e-7)])
 def test_steps_and_eps(mrl, ctx, steps, eps):
     x = matrix(torch.Generator().manual_seed(steps), 48, 90) * 1e-3
