@@ -223,6 +223,56 @@ def test_muon_steps(mrl, ctx, net, layers, nesterov, decay):
     assert ((s.cpu().double() - m2).abs() <= 3 * 6 * 2.0 ** -24 * (m2.abs() + 0.5)).all()
 
 
+# nets whose matrices take launches of their own for norms, products and update: tiles of 32 to 128, tall matrices, thin ones among
+# large ones, unequal ones in one group
+@pytest.mark.parametrize("widths,every,nesterov,decay", [((8, 256, 256, 4), False, True, 0.01), ((40, 700, 333, 900, 5), False, False, 0.1),
+                                                         ((376, 1024, 1024, 1024, 17), True, True, 0.0), ((1500, 600, 11, 900), True, True, 0.05), ((2, 900, 900, 900), True, False, 0.3)])
+def test_muon_steps_of_larger_nets(mrl, ctx, widths, every, nesterov, decay):
+    print("muon", widths, every, nesterov, decay, flush=True)
+    model = mrl.seq(*[mrl.LinearReLU(a, b) for a, b in zip(widths, widths[1:])])
+    lr, mu, n, last = 0.03, 0.9, model.PARAM_SIZE, len(widths) - 2
+    opt = mrl.Muon(model, lr=lr, momentum=mu, nesterov=nesterov, weight_decay=decay, layers=range(last + 1) if every else None, adam_lr=1e-3, beta1=0.8, beta2=0.99,
+                   adam_eps=1e-6)
+    gen = torch.Generator().manual_seed(sum(widths))
+    params, state = 0.05 * torch.randn(n, generator=gen), torch.zeros(2 * n)
+    shapes = list(zip(widths, widths[1:]))
+    grads = [torch.cat([torch.cat((matrix(gen, a, b).reshape(-1), torch.randn(b, generator=gen))) for a, b in shapes]) for _ in range(2)]
+    p, s = params.cuda(), state.cuda()
+    w, m2 = params.double(), state.double()
+    loose = [0.0] * len(shapes)       # what the products may move each matrix by, in the 2-norm
+    for t, g in enumerate(grads, 1):
+        opt.step_gpu(ctx, p, g.cuda(), s)
+        g, at, adam = g.double(), 0, torch.ones(n, dtype=torch.bool)
+        for k, (a, b) in enumerate(shapes):
+            size = a * b
+            if every or k < last:
+                v = m2[2 * at:2 * at + size]
+                v.mul_(mu).add_(g[at:at + size])
+                u = (g[at:at + size] + mu * v if nesterov else v).view(a, b)
+                o, factor = polynomial(u), lr * max(1.0, b / a) ** 0.5
+                w[at:at + size] = w[at:at + size] * (1 - lr * decay) - factor * o.reshape(-1)
+                loose[k] += factor * 8 * (polynomial(u, gen=torch.Generator().manual_seed(t)) - o).norm().item()
+                adam[at:at + size] = False
+            at += size + b
+        m, v = m2[0::2][adam], m2[1::2][adam]
+        m, v = 0.8 * m + 0.2 * g[adam], 0.99 * v + 0.01 * g[adam] ** 2
+        m2[0::2][adam], m2[1::2][adam] = m, v
+        w[adam] -= 1e-3 * (m / (1 - 0.8 ** t)) / ((v / (1 - 0.99 ** t)).sqrt() + 1e-6)
+    ctx.synchronize()
+    off, at = (p.cpu().double() - w), 0
+    for k, (a, b) in enumerate(shapes):
+        if every or k < last:
+            # a step rounds a parameter at its product with the decay and at its update, and the constants 1 - lr decay and the factor
+            here = slice(at, at + a * b)
+            rounding = 2 * 2.0 ** -24 * (3 * w[here].norm().item() + 2 * lr * max(1.0, b / a) ** 0.5 * 1.3 * min(a, b) ** 0.5)
+            assert off[here].norm().item() <= loose[k] + rounding, "matrix %d: %g, bound %g + %g" % (k, off[here].norm(), loose[k], rounding)
+        at += a * b + b
+    # Adam's share, element by element: an update of at most 0.003 of 40 roundings, a parameter rounded once, each of two steps
+    assert (off[adam].abs() <= 2 * (2.0 ** -24 * (w[adam].abs() + 0.1) + 0.003 * 40 * 2.0 ** -24)).all()
+    # gradients of up to 3 or so, a product and a sum rounded each step, constants rounded
+    assert ((s.cpu().double() - m2).abs() <= 2 * 6 * 2.0 ** -24 * (m2.abs() + grads[0].abs().max() + 0.5)).all()
+
+
 @pytest.mark.parametrize("large", [(), (3,), (30,)])
 def test_more_matrices_than_a_launch_takes(mrl, ctx, large):
     """35 matrices with gaps between them in one call, against each in a call of its own."""
