@@ -450,7 +450,7 @@ int mrl_minibatch_adv_stats(mrl_ctx *ctx, const int32_t *indices, const float *a
  * gate, value, out and their gradients have rows t * N + n of D elements of `dtype`, `ld` elements apart (ld >= D; gate and value
  * can be halves of one buffer's rows); states are fp32 [N, D].  state_in NULL is zeros; state_out = h[T-1], may be NULL, and
  * may be state_in.  T = 1 is a step of a collection loop.  No element of another output may be one of an input's or of another
- * output's.  A row's elements need no alignment beyond their type's.
+ * output's (MRL_E_ARG).  A row's elements need no alignment beyond their type's.
  *
  * Backward: out as forward left it, grad_out and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out;
  * overwrites grad_gate, grad_value and grad_state_in (may be NULL, may be grad_state_out).  All sums are in a fixed order.

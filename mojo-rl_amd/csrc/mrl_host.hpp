@@ -6,6 +6,7 @@
 #include <stdio.h>
 #include <stdarg.h>
 #include <algorithm>
+#include <initializer_list>
 #include <unordered_map>
 #include <vector>
 #include "../../include/mrl.h"
@@ -128,6 +129,49 @@ struct OnDevice {
     OnDevice(const OnDevice &) = delete;
     OnDevice &operator=(const OnDevice &) = delete;
 };
+
+// Rows of `width` bytes, `apart` from one to the next (at least `width`); NULL or no bytes: nothing.
+struct Region {
+    const char *name;
+    const void *at;
+    int64_t rows, width, apart;
+    Region(const char *name, const void *at, int64_t width) : Region(name, at, 1, width, width) {}
+    Region(const char *name, const void *at, int64_t rows, int64_t width, int64_t apart) : name(name), at(at), rows(rows), width(width), apart(apart) {}
+};
+// Whether two have a byte in common.  Rows of one distance that lie between each other (halves of a buffer's rows) are told apart by where
+// they start, those of different distances row by row.
+inline bool overlap(const Region &x, const Region &y) {
+    if (!x.at || !y.at || x.rows < 1 || y.rows < 1 || x.width < 1 || y.width < 1) return false;
+    const Region &a = x.rows <= y.rows ? x : y, &b = x.rows <= y.rows ? y : x;
+    const int64_t behind = (int64_t)((intptr_t)a.at - (intptr_t)b.at);   // of a's first row from b's
+    if (behind + (a.rows - 1) * a.apart + a.width <= 0 || behind >= (b.rows - 1) * b.apart + b.width) return false;
+    auto meets = [&](int64_t from) {   // a row of a that starts there, with the last row of b that starts ahead of its end
+        if (from + a.width <= 0) return false;
+        const int64_t row = std::min(b.rows - 1, (from + a.width - 1) / b.apart);
+        return row * b.apart + b.width > from;
+    };
+    if (a.rows > 1 && a.apart == b.apart) {
+        // every row of a stands to the rows of b as its neighbours do, but at b's ends
+        const int64_t first = behind >= 0 ? 0 : std::min(a.rows - 1, -behind / a.apart);
+        for (int64_t row = first; row < std::min(a.rows, first + 2); ++row)
+            if (meets(behind + row * a.apart)) return true;
+        return false;
+    }
+    for (int64_t row = 0; row < a.rows; ++row)
+        if (meets(behind + row * a.apart)) return true;
+    return false;
+}
+
+// MRL_E_ARG where an output has a byte of an input or of another output.
+inline int check_apart(const char *who, std::initializer_list<Region> outputs, std::initializer_list<Region> inputs) {
+    for (const Region *o = outputs.begin(); o != outputs.end(); ++o) {
+        for (const Region *other = o + 1; other != outputs.end(); ++other)
+            if (overlap(*o, *other)) return set_error(MRL_E_ARG, "%s: %s and %s overlap", who, o->name, other->name);
+        for (const Region &in : inputs)
+            if (overlap(*o, in)) return set_error(MRL_E_ARG, "%s: %s and %s overlap", who, o->name, in.name);
+    }
+    return MRL_OK;
+}
 
 inline int grid_for(long n, int block) { return (int)((n + block - 1) / block); }
 

@@ -593,11 +593,27 @@ void launch(const mrl_ctx *ctx, const Scan &s, int V) {
     else launch<E, 1, BACK>(ctx, s);
 }
 
+// No output has an element of an input or of another output; the last state may be the first.
+template <bool BACK>
+int check_buffers(const char *who, int dtype, const Scan &s, void *workspace, size_t workspace_bytes) {
+    const int64_t size = dtype == MRL_F32 ? 4 : 2, rows = (int64_t)s.T * s.N, states = 4LL * s.N * s.D;
+    auto of = [&](const char *name, const void *at, long ld) { return Region(name, at, rows, size * s.D, size * ld); };
+    const Region ahead(BACK ? "grad_state_out" : "state_in", s.first == s.last ? nullptr : s.first, states), behind(BACK ? "grad_state_in" : "state_out", s.last, states);
+    const Region gate = of("gate", s.gate, s.gate_ld), value = of("value", s.value, s.value_ld), scratch("the workspace", workspace, (int64_t)workspace_bytes);
+    const Region dones("dones", s.dones, 4 * rows), prev_dones("prev_dones", s.prev_dones, 4LL * s.N);
+    if (BACK)
+        return check_apart(who, {of("grad_gate", s.dst, s.grad_gate_ld), of("grad_value", s.dst2, s.grad_value_ld), behind, scratch},
+                           {gate, value, of("out", s.out, s.out_ld), of("grad_out", s.grad_out, s.grad_out_ld), dones, prev_dones, Region("state_in", s.state_in, states), ahead});
+    return check_apart(who, {of("out", s.dst, s.out_ld), behind, scratch}, {gate, value, dones, prev_dones, ahead});
+}
+
 template <bool BACK>
 int scan(mrl_ctx *ctx, const char *who, int dtype, Scan &s, void *workspace, uint64_t workspace_bytes) {
     OnDevice on(ctx);
     if (s.T == 0) {
         const long n = (long)s.N * s.D;
+        const int rc = check_buffers<BACK>(who, dtype, s, nullptr, 0);
+        if (rc != MRL_OK) return rc;
         if (s.last != nullptr && s.last != s.first)
             hipLaunchKernelGGL(pass_state_kernel, dim3((int)std::min<long>((n + 255) / 256, 4096)), dim3(256), 0, ctx->stream, s.first, s.last, n);
         MRL_CHECK_LAUNCH();
@@ -608,6 +624,8 @@ int scan(mrl_ctx *ctx, const char *who, int dtype, Scan &s, void *workspace, uin
                   "%s: the workspace holds %llu bytes, need %llu", who, (unsigned long long)(workspace ? workspace_bytes : 0),
                   (unsigned long long)p.bytes);
     MRL_CHECK_ARG(p.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", who);
+    const int rc = check_buffers<BACK>(who, dtype, s, workspace, p.bytes);
+    if (rc != MRL_OK) return rc;
     s.lanes_per_row = p.lanes_per_row; s.lanes = p.lanes; s.groups = p.groups;
     s.W = p.W; s.segments = p.segments; s.segment_steps = p.segment_steps; s.share = p.share;
     s.whole = s.D % p.V == 0;

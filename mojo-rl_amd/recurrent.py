@@ -10,6 +10,9 @@ Rows are the rollout's (row = t * envs + env): gate, value, output and their gra
 bfloat16, elements of a row next to each other and rows at any equal distance, so that `pre[:, :width]` and `pre[:, width:]` serve
 as they are.  States are float32 [envs, width].  `dones` are the rollout's own flags (RolloutBuffers.r_dones), `prev_dones` those
 of the step ahead of the first one: where a flag is above 0.5 the next step starts from a zero state.
+
+What a call writes lies apart from what it reads, but for the states that are named below: MrlError where an element of an output
+is one of an input or of another output.
 """
 import ctypes as C
 

@@ -365,3 +365,38 @@ def test_library_refusals(mrl, ctx):
     assert lib.mrl_recurrence_backward(ctx.handle, 0, 2, 3, 4, p, 4, p, 4, p, 4, None, None, None, p, 4, None, p, 4, None, 4, None, None, 0) == -1
     ctx.synchronize()
     assert not x.any()
+
+
+def test_outputs_on_inputs_are_refused(mrl, ctx):
+    """Before anything is launched: the buffers stay as they are.  Rows between each other are apart."""
+    T, N, D = 40, 3, 8
+    layer, wide, flat = mrl.GatedRecurrence(D), torch.randn(T * N + N, 5 * D, device="cuda"), torch.randn(4, N, D, device="cuda")
+    flags = torch.zeros(T, N, device="cuda")
+    gate, value, out, gg, gv = (wide[N:, k * D:(k + 1) * D] for k in range(5))
+    before = wide.clone()
+
+    def forward(**other):
+        layer.forward_gpu(ctx, **{**dict(output=out, gate=gate, value=value, steps=T, state_in=flat[0], state_out=flat[1], dones=flags), **other})
+
+    def backward(**other):
+        layer.backward_gpu(ctx, **{**dict(grad_gate=gg, grad_value=gv, grad_output=grad, gate=gate, value=value, output=out, steps=T, state_in=flat[0], dones=flags,
+                                          grad_state_out=flat[2], grad_state_in=flat[3]), **other})
+    grad = torch.randn(T * N, D, device="cuda")
+    for bad in (dict(output=gate), dict(output=value), dict(output=wide[:-N, D:2 * D]), dict(output=wide[N:, D - 1:2 * D - 1]), dict(output=wide[N:, 2 * D - 1:3 * D - 1]),
+                dict(state_out=flat.view(-1)[4:4 + N * D].view(N, D)), dict(dones=wide.view(-1)[-T * N:]), dict(prev_dones=flat[1].view(-1)[:N]),
+                dict(state_out=wide.view(-1)[9 * 5 * D:9 * 5 * D + N * D]), dict(state_in=wide.view(-1)[-N * D:])):
+        with pytest.raises(mrl.MrlError, match="overlap"):
+            forward(**bad)
+    for bad in (dict(grad_gate=gate), dict(grad_gate=gv), dict(grad_value=out), dict(grad_value=wide[:-N, 2 * D:3 * D]), dict(grad_output=gv), dict(grad_state_in=flat[0]),
+                dict(grad_state_in=grad[-N:]), dict(grad_state_out=flat.view(-1)[3 * N * D - 1:4 * N * D - 1]), dict(grad_gate=grad)):
+        with pytest.raises(mrl.MrlError, match="overlap"):
+            backward(**bad)
+    ctx.synchronize()
+    assert torch.equal(wide, before)
+    # the same buffers as they may lie, and the states that may be the same
+    forward()
+    forward(state_out=flat[0])
+    backward()
+    backward(grad_state_in=flat[2])
+    ctx.synchronize()
+    assert torch.equal(wide[:, :2 * D], before[:, :2 * D]) and torch.equal(wide[:N], before[:N]) and not torch.equal(wide[N:, 2 * D:], before[N:, 2 * D:])
