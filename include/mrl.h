@@ -475,7 +475,8 @@ int mrl_recurrence_backward(mrl_ctx *ctx, int dtype, int T, int N, int D, const 
  *     X = G / (|G| + eps)  (Frobenius norm);   `steps` times  X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X
  * takes its singular values into about [0.7, 1.2] in five steps and leaves its singular vectors.
  *
- * mrl_orthogonalize: `count` matrices [rows, cols] of `dtype`, one behind the other, row-major; out may be in.  Sums in fp32,
+ * mrl_orthogonalize: `count` matrices [rows, cols] of `dtype`, one behind the other, row-major; out may be in, but not overlap it
+ * otherwise, and params, grads and state of mrl_muon_step lie apart (MRL_E_ARG).  Sums in fp32,
  * operands of 22 significant bits; bf16 is rounded when stored.  A matrix of zeros gives zeros (eps > 0), one with an infinity or
  * NaN gives NaN.  Sides are 1 to 32768.
  *

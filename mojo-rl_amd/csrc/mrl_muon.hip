@@ -1005,10 +1005,13 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     int rc = mrl::check_matrix(who, rows, cols);
     if (rc != MRL_OK || count == 0) return rc;
     MRL_CHECK_ARG(in && out, "%s: NULL buffer", who);
-    rc = mrl::check_workspace(who, workspace, workspace_bytes, mrl::batch_bytes(count, rows, cols));
+    const uint64_t need = mrl::batch_bytes(count, rows, cols);
+    rc = mrl::check_workspace(who, workspace, workspace_bytes, need);
+    if (rc != MRL_OK) return rc;
+    const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
+    rc = mrl::check_apart(who, {{"out", out, (int64_t)(count * one)}, {"the workspace", workspace, (int64_t)need}}, {{"in", in == out ? nullptr : in, (int64_t)(count * one)}});
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
-    const size_t one = (size_t)rows * cols * (dtype == MRL_F32 ? 4 : 2);
     const int most = mrl::batch_of(count, rows, cols);
     for (long done = 0; done < count; done += most) {
         mrl::Group g = {};
@@ -1052,6 +1055,8 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
     uint64_t need = 0;
     rc = mrl_muon_workspace(n_matrices, matrices, &need);
     if (rc == MRL_OK) rc = mrl::check_workspace(who, workspace, workspace_bytes, need);
+    if (rc == MRL_OK)
+        rc = mrl::check_apart(who, {{"params", params, 4 * n}, {"state", state, 8 * n}, {"the workspace", workspace, (int64_t)need}}, {{"grads", grads, 4 * n}});
     if (rc != MRL_OK) return rc;
     mrl::OnDevice on(ctx);
     int64_t at = 0;

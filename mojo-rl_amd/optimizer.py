@@ -39,7 +39,7 @@ def _orthogonalize_bytes(count, rows, cols):
 def orthogonalize(ctx, out, x, steps=5, eps=1e-7):
     """out = the Newton-Schulz polynomial of x [rows, cols] or of every matrix of x [count, rows, cols]: x / (|x| + eps), then `steps`
     times X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X, which takes the singular values into about [0.7, 1.2].  float32 or
-    bfloat16, contiguous; out may be x."""
+    bfloat16, contiguous; out may be x, but not overlap it otherwise."""
     shape, kind = x.shape, _TYPES.get(x.dtype)
     if len(shape) not in (2, 3) or kind is None:
         raise _lib.MrlError("orthogonalize: a float32 or bfloat16 [rows, cols] or [count, rows, cols] tensor expected, got %s of %s"

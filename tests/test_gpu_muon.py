@@ -472,3 +472,25 @@ def test_library_refusals(mrl, ctx):
         assert muon(**bad) == -1 and text in lib.mrl_last_error(), bad
     ctx.synchronize()
     assert not x.any()
+
+
+def test_buffers_that_overlap_are_refused(mrl, ctx):
+    """Before anything is launched: they stay as they are."""
+    x, model = torch.randn(8, 40, 30, device="cuda"), mrl.seq(mrl.Linear(6, 9), mrl.Linear(9, 3))
+    n, before = model.PARAM_SIZE, x.clone()
+    for out, src in ((x[1:], x[:-1]), (x[:-1], x[1:]), (x.view(-1)[1:2401].view(2, 40, 30), x[:2]), (x[3], x.view(-1)[3 * 1200 - 7:4 * 1200 - 7].view(40, 30))):
+        with pytest.raises(mrl.MrlError, match="out and in overlap"):
+            mrl.orthogonalize(ctx, out, src)
+    flat, opt = x.view(-1), mrl.Muon(model)
+    for p, g, s in ((flat[:n], flat[n - 1:2 * n - 1], flat[4000:4000 + 2 * n]), (flat[:n], flat[:n], flat[4000:4000 + 2 * n]), (flat[2 * n:3 * n], flat[4000:4000 + n], flat[n + 2 - n % 2:3 * n + 2 - n % 2]),
+                    (flat[:n], flat[4000 + n:4000 + 2 * n], flat[4000:4000 + 2 * n])):
+        with pytest.raises(mrl.MrlError, match="overlap"):
+            opt.step_gpu(ctx, p, g, s)
+    ctx.synchronize()
+    assert opt.t == 0 and torch.equal(x, before)
+    mrl.orthogonalize(ctx, x[1:], x[1:])         # in place, and next to each other
+    mrl.orthogonalize(ctx, x[0], x[1])
+    opt.step_gpu(ctx, flat[:n], flat[n:2 * n], flat[2 * n:4 * n])
+    ctx.synchronize()
+    # (the state was random numbers: below zero, its second moments have no square root)
+    assert opt.t == 1 and flat[4 * n:].isfinite().all()
