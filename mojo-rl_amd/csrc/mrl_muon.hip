@@ -974,6 +974,9 @@ int check_matrices(const char *who, int count, const mrl_matrix *matrices, int64
     return MRL_OK;
 }
 
+// eps where zeros have a quotient in 64 bits.  A norm that is not 0 is 2^-149 or more: what is added here is far below its last bit.
+double norm_eps(double eps) { return eps > 0.0 ? std::max(eps, 0x1p-900) : eps; }
+
 int check_workspace(const char *who, const void *ws, uint64_t have, uint64_t need) {
     MRL_CHECK_ARG(need == 0 || (ws && have >= need), "%s: the workspace holds %llu bytes, need %llu", who, (unsigned long long)(ws ? have : 0),
                   (unsigned long long)need);
@@ -1015,7 +1018,7 @@ int mrl_orthogonalize(mrl_ctx *ctx, int dtype, int count, int rows, int cols, co
     const int most = mrl::batch_of(count, rows, cols);
     for (long done = 0; done < count; done += most) {
         mrl::Group g = {};
-        g.eps = eps;
+        g.eps = mrl::norm_eps(eps);
         g.count = (int)std::min<long>(most, count - done);
         g.alike_in = one;
         mrl::sides(g.mat[0], rows, cols);
@@ -1063,7 +1066,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
     int done = 0;
     do {
         mrl::Group g = {};
-        g.eps = eps;
+        g.eps = mrl::norm_eps(eps);
         g.mu = (float)momentum;
         g.nesterov = nesterov != 0;
         g.keep = (float)(1.0 - lr * weight_decay);

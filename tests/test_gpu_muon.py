@@ -159,6 +159,19 @@ def test_zeros_ones_and_what_is_not_finite(mrl, ctx):
     near(out[1], x[1], HALF["f32"], "ones")
 
 
+@pytest.mark.parametrize("eps", [5e-324, 1e-310, 1e-300])
+@pytest.mark.parametrize("rows,cols", [(4, 5), (130, 150)])
+def test_zeros_with_the_least_eps(mrl, ctx, rows, cols, eps):
+    """However small eps is above 0, zeros give zeros, and what is not zero is divided by its norm."""
+    x = torch.zeros(2, rows, cols)
+    x[1, 0, 0] = 2.0 ** -149
+    out = torch.full_like(x, 9.0, device="cuda")
+    mrl.orthogonalize(ctx, out, x.cuda(), eps=eps)
+    ctx.synchronize()
+    assert not out[0].any()
+    near(out[1], x[1], HALF["f32"], "the smallest", eps=eps)
+
+
 def test_a_few_large_entries(mrl, ctx):
     """Entries at the top of the pieces' range, next to ones far below."""
     x = torch.randn(500, 700, generator=torch.Generator().manual_seed(2)) * 1e-4
