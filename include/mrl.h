@@ -452,7 +452,7 @@ int mrl_minibatch_adv_stats(mrl_ctx *ctx, const int32_t *indices, const float *a
  * may be state_in.  T = 1 is a step of a collection loop.  No element of another output may be one of an input's or of another
  * output's (MRL_E_ARG).  A row's elements need no alignment beyond their type's.
  *
- * Backward: out as forward left it, grad_out and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out;
+ * Backward: out as forward left it (its states are rounded in bf16: grad_gate is off by up to 2^-8 of their share of it), grad_out and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out;
  * overwrites grad_gate, grad_value and grad_state_in (may be NULL, may be grad_state_out).  All sums are in a fixed order.
  *
  * The workspace (device, 16-byte aligned, need not be kept between calls; NULL where the size is 0) holds at least

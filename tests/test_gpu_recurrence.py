@@ -272,6 +272,32 @@ def test_rows_at_a_distance_and_odd_addresses(mrl, ctx, T, N, D, dtype):
     assert (wg[:, :1] == -3).all() and (wg[:, 1 + D:] == -3).all() and (wv[:, :4] == -3).all() and (wv[:, 4 + D:] == -3).all()
 
 
+@pytest.mark.parametrize("T,N,D", [(5, 3, 45), (64, 200, 64), (300, 9, 40), (2000, 2, 52)])
+def test_bf16_gradient_is_that_of_the_states_before_rounding(mrl, ctx, T, N, D):
+    """The backward pass takes h' from `out`, rounded to bf16: against autograd through the unrounded states in 64 bits, the gate's gradient is off by that
+    rounding, half a step of each h', and no more; the others do not depend on it."""
+    c = Case(T, N, D, "bf16", rate=0.1)
+    out, _ = c.forward(mrl, ctx)
+    got = c.backward(mrl, ctx, out)
+    ctx.synchronize()
+    gate, value, state = (x.requires_grad_() for x in (c.host(c.gate, T, N, D), c.host(c.value, T, N, D), c.host(c.state, N, D)))
+    a, h, states = torch.sigmoid(gate), state, []
+    for t in range(T):
+        h = a[t] * torch.where(c.cut[t][:, None], torch.zeros_like(h), h) + (1 - a[t]) * value[t]
+        states.append(h)
+    grad, last = c.host(c.grad_out, T, N, D), c.host(c.grad_last, N, D)
+    ((torch.stack(states) * grad).sum() + (h * last).sum()).backward()
+    wants = gate.grad, value.grad, state.grad
+    gate, value, state, a = gate.detach(), value.detach(), state.detach(), a.detach()
+    exact, off = c.forward64()
+    offs = backward64(gate, value, exact, c.cut, state, grad, last, STEP["bf16"])[1]
+    before, behind = torch.cat((torch.zeros(1, N, D), exact[:-1].abs())), torch.cat((torch.zeros(1, N, D), off[:-1]))
+    # the gradient's a (1 - a) d h', where (1 - a) d is that of the value
+    rounding = (~c.cut)[..., None] * (HALF["bf16"] * (before + behind) + behind) * a * wants[1].abs()
+    for x, want, o, what in zip(got, wants, (offs[0] + rounding, offs[1], offs[2]), ("grad_gate", "grad_value", "grad_state_in")):
+        near(x, want, o, 0.0 if what == "grad_state_in" else HALF["bf16"], what)
+
+
 def test_gradient_against_differences(mrl, ctx):
     """Directional derivatives of the recurrence in 64 bits, taken as differences."""
     c = Case(23, 3, 10, "f32", rate=0.1)
