@@ -452,8 +452,8 @@ int mrl_minibatch_adv_stats(mrl_ctx *ctx, const int32_t *indices, const float *a
  * may be state_in.  T = 1 is a step of a collection loop.  No element of another output may be one of an input's or of another
  * output's (MRL_E_ARG).  A row's elements need no alignment beyond their type's.
  *
- * Backward: out as forward left it (its states are rounded in bf16: grad_gate is off by up to 2^-8 of their share of it), grad_out and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out;
- * overwrites grad_gate, grad_value and grad_state_in (may be NULL, may be grad_state_out).  All sums are in a fixed order.
+ * Backward: out as forward left it (its states are rounded in bf16: grad_gate is off by up to 2^-8 of their share of it), grad_out
+ * and grad_state_out (NULL: zeros; fp32) the gradients of out and state_out; overwrites grad_gate, grad_value and grad_state_in (may be NULL, may be grad_state_out).  All sums are in a fixed order.
  *
  * The workspace (device, 16-byte aligned, need not be kept between calls; NULL where the size is 0) holds at least
  * mrl_recurrence_workspace's bytes, the same for both directions and types: 0 unless few channels and many steps have the time
@@ -476,15 +476,16 @@ int mrl_recurrence_backward(mrl_ctx *ctx, int dtype, int T, int N, int D, const 
  * takes its singular values into about [0.7, 1.2] in five steps and leaves its singular vectors.
  *
  * mrl_orthogonalize: `count` matrices [rows, cols] of `dtype`, one behind the other, row-major; out may be in, but not overlap it
- * otherwise, and params, grads and state of mrl_muon_step lie apart (MRL_E_ARG).  Sums in fp32,
- * operands of 22 significant bits; bf16 is rounded when stored.  A matrix of zeros gives zeros (eps > 0), one with an infinity or
- * NaN gives NaN.  Sides are 1 to 32768.
+ * otherwise (MRL_E_ARG).  Sums in fp32, operands of 22 significant bits, a matrix of up to 16 rows or columns on the fp32 matrix
+ * cores; bf16 is rounded when stored.  A matrix of zeros gives zeros (eps > 0), one with an infinity or NaN gives NaN.  Sides
+ * are 1 to 32768.
  *
  * mrl_muon_step: the optimiser's whole step on a flat parameter vector of n floats.  The `n_matrices` ranges
  * [offset, offset + rows * cols) (in order, apart) are weight matrices W [in, out] as the layers keep them; with their gradient g
  *     v <- momentum v + g;   u = nesterov ? g + momentum v : v;   W <- (1 - lr weight_decay) W - lr sqrt(max(1, out / in)) O(u),
  * O the polynomial above.  Everything between them is updated as by mrl_adam_step with adam_lr, beta1, beta2, adam_eps and step
  * count t.  state is Adam's [n, 2]; a matrix's share of it starts with v (rows * cols floats), the rest of that share is unused.
+ * params, grads and state lie apart (MRL_E_ARG).
  *
  * Workspaces (device, 16-byte aligned, need not be kept between calls) hold at least the bytes that the queries give. */
 typedef struct {

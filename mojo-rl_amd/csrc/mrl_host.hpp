@@ -130,13 +130,14 @@ struct OnDevice {
     OnDevice &operator=(const OnDevice &) = delete;
 };
 
-// Rows of `width` bytes, `apart` from one to the next (at least `width`); NULL or no bytes: nothing.
+// Rows of `width` bytes, `apart` from one to the next (at least `width`; of a single row it says nothing); NULL or no bytes: nothing.
 struct Region {
     const char *name;
     const void *at;
     int64_t rows, width, apart;
     Region(const char *name, const void *at, int64_t width) : Region(name, at, 1, width, width) {}
-    Region(const char *name, const void *at, int64_t rows, int64_t width, int64_t apart) : name(name), at(at), rows(rows), width(width), apart(apart) {}
+    Region(const char *name, const void *at, int64_t rows, int64_t width, int64_t apart)
+        : name(name), at(at), rows(rows), width(width), apart(rows > 1 ? std::max(apart, width) : width) {}
 };
 // Whether two have a byte in common.  Rows of one distance that lie between each other (halves of a buffer's rows) are told apart by where
 // they start, those of different distances row by row.

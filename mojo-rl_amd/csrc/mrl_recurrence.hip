@@ -13,8 +13,10 @@
 //   is the result of the formula above on the state before it and the inputs are read once.  1000 steps of 64 in fp32: 55 us.
 // - segments: with a few channels and many steps the time axis is also split over workgroups.  A first launch leaves every segment's
 //   (A, B) in a workspace, the second starts each segment from those before it.  Gate and value are read twice, the second time
-//   out of the caches where they fit: 16384 steps of 2 of width 512 in bf16 44 us, 18 and 25, 3.7 and 4.0 TB/s.  (One launch in which
-//   a segment waits for those ahead would save the second reading, but a wait among XCDs takes 5 us and more here.)
+//   out of the caches where they fit: 16384 steps of 2 of width 512 in bf16 44 us, 18 and 25, 3.7 and 4.0 TB/s.  Part of the 25 are trips
+//   to memory one behind the other: a wavefront waits for each of up to eight segments' coefficients, then for each of those
+//   of up to seven wavefronts ahead.  (One launch in which a segment waits for those ahead would save the second reading, but a wait
+//   among XCDs takes 5 us and more here.)
 //
 // A cut is a selection, never a product with 0: an infinity or NaN behind it goes nowhere.  In the composed coefficients A = 0
 // says so; a product of gates that underflows stays at the smallest subnormal instead.

@@ -426,3 +426,17 @@ def test_outputs_on_inputs_are_refused(mrl, ctx):
     backward(grad_state_in=flat[2])
     ctx.synchronize()
     assert torch.equal(wide[:, :2 * D], before[:, :2 * D]) and torch.equal(wide[:N], before[:N]) and not torch.equal(wide[N:, 2 * D:], before[N:, 2 * D:])
+
+
+def test_a_single_row_has_no_distance_to_a_next(mrl, ctx):
+    """Whatever is given for it, as one row of a larger buffer may have."""
+    lib, x = mrl._lib.lib(), torch.randn(3, 4, device="cuda")
+    p = [ctypes.c_void_p(row.data_ptr()) for row in x]
+    for ld in (4, 1 << 40, 1 << 62, (1 << 63) - 1):
+        assert lib.mrl_recurrence_forward(ctx.handle, 0, 1, 1, 4, p[0], ld, p[1], ld, None, None, None, p[2], ld, None, None, 0) == 0, lib.mrl_last_error()
+        ctx.synchronize()
+        want = (1 - torch.sigmoid(x[0].double())) * x[1].double()
+        assert ((x[2].double() - want).abs() <= STEP["f32"] * want.abs()).all()
+        x[2].zero_()
+        torch.cuda.synchronize()
+        assert lib.mrl_recurrence_forward(ctx.handle, 0, 1, 1, 4, p[0], ld, p[1], ld, None, None, None, p[1], ld, None, None, 0) == -1 and b"overlap" in lib.mrl_last_error()
