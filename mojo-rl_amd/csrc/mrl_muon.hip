@@ -446,8 +446,8 @@ MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int fro
     if (there) finish<STAGE, KIND>(g, m, from, last, bi == bj, fi, fj, v, piece);
 }
 // Tile (bi, bj) of a side of 32 F of a matrix with few rows, whose neighbours in the launch have more: in squares of 32 x 32, one behind the
-// other for each 256 lanes, so that such a matrix comes out the same bit by bit whatever it is updated with.  (8-1024-1024-1024-4 takes
-// 301 us with the fp16 cores for its first layer too: the squares are done before the other layers' tiles are.)
+// other for each 256 lanes, so that such a matrix comes out as in launches of its own, bit by bit.  (8-1024-1024-1024-4 takes 301 us
+// with the fp16 cores for its first layer too: the squares are done before the other layers' tiles are.)
 template <int STAGE, int KIND, int F>
 MRL_DEV void few_squares(const Group &g, const Mat &m, int bi, int bj, int from, int last, SmallSums *sums) {
     const int teams = blockDim.x / 256, team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);

@@ -341,7 +341,8 @@ def test_large_matrices_go_one_by_one(mrl, ctx):
 
 
 @pytest.mark.parametrize("thin,others", [((9, 700), [(700, 700)] * 2), ((700, 9), [(700, 700)] * 2), ((8, 1024), [(1024, 1024)] * 2), ((16, 1000), [(1000, 1000)] * 3),
-                                         ((1400, 16), [(900, 1400)]), ((5, 1500), [(1500, 1500)]), ((1, 900), [(600, 600)] * 6), ((2, 3000), [(2048, 2048)] * 2)])
+                                         ((1400, 16), [(900, 1400)]), ((5, 1500), [(1500, 1500)]), ((1, 900), [(600, 600)] * 6), ((2, 3000), [(2048, 2048)] * 2),
+                                         ((4, 9000), [(2048, 2048)] * 2)])
 def test_thin_matrix_does_not_go_by_its_neighbours(mrl, ctx, thin, others):
     """A matrix of up to 16 rows beside ones whose products are worked out in tiles of 64, 96 and 128: bit by bit what it is by itself, and as
     close to 64 bits as products in fp32."""
