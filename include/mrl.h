@@ -470,6 +470,41 @@ int mrl_recurrence_backward(mrl_ctx *ctx, int dtype, int T, int N, int D, const 
                             const float *grad_state_out, void *grad_gate, int64_t grad_gate_ld, void *grad_value,
                             int64_t grad_value_ld, float *grad_state_in, void *workspace, uint64_t workspace_bytes);
 
+/* ------------------------------------------------------------------ gated delta rule
+ * A recurrent layer whose memory is a matrix S [key_dim, value_dim] per head (no counterpart in the reference).  Per environment and head,
+ *     a = sigmoid(gate),  b = sigmoid(rate),  k = key / |key|,  q = query / (|query| sqrt(key_dim)),  |x| = sqrt(sum x^2 + 1e-6),
+ *     S' = a[t] S[t-1],  u[t] = b[t] (value[t] - S'^T k[t]),  S[t] = S' + k[t] u[t]^T,  out[t] = S[t]^T q[t],
+ * S[-1] = state_in: the memory fades by a, and what it answers to the key moves towards the value by the rate.  Head h of `heads`
+ * uses the query and key of key head h / (heads / key_heads).  Rows, `ld`, dones, prev_dones and cuts are those of the recurrent layer
+ * above: a row of query and key has key_heads * key_dim elements, of value and out heads * value_dim, of gate and rate `heads`;
+ * where a step before ended an episode S[t-1] counts as 0, and what a cut hides, infinities and NaN included, reaches nothing behind it.
+ * States are fp32 [N, heads, key_dim, value_dim]; state_in NULL is zeros; state_out = S[T-1], may be NULL, and may be state_in.
+ * T = 1 is a step of a collection loop.  Dims are 1 to 128, N * heads is below 2^22, T below 2^30.  Sums and states are fp32, bf16 is rounded
+ * when stored.
+ *
+ * Backward: grad_out and grad_state_out (NULL: zeros; fp32) are the gradients of out and state_out; overwrites the gradients of
+ * query, key, value, gate, rate and (may be NULL, may be grad_state_out) the first state.  It goes through the steps forwards once more
+ * by itself.  All sums are in a fixed order.
+ *
+ * No element of another output may be one of an input's or of another output's (MRL_E_ARG).  The workspace (device, 16-byte aligned,
+ * need not be kept between calls; NULL where the size is 0) holds at least mrl_delta_workspace's bytes for the description's sizes. */
+typedef struct {
+    int32_t dtype, T, N, heads, key_heads, key_dim, value_dim;
+    const void *query, *key, *value, *gate, *rate;
+    int64_t query_ld, key_ld, value_ld, gate_ld, rate_ld;
+    const float *dones, *prev_dones, *state_in;
+} mrl_delta;
+typedef struct {
+    void *query, *key, *value, *gate, *rate;
+    int64_t query_ld, key_ld, value_ld, gate_ld, rate_ld;
+    float *state;
+} mrl_delta_grads;
+int mrl_delta_workspace(mrl_ctx *ctx, const mrl_delta *r, int backward, uint64_t *bytes);
+int mrl_delta_forward(mrl_ctx *ctx, const mrl_delta *r, void *out, int64_t out_ld, float *state_out, void *workspace,
+                      uint64_t workspace_bytes);
+int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, int64_t grad_out_ld, const float *grad_state_out,
+                       const mrl_delta_grads *grads, void *workspace, uint64_t workspace_bytes);
+
 /* ------------------------------------------------------------------ orthogonalised updates
  * No counterpart in the reference, whose optimisers work element by element.  A matrix's polynomial
  *     X = G / (|G| + eps)  (Frobenius norm);   `steps` times  X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X

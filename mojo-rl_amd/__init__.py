@@ -13,7 +13,7 @@ from .context import DeviceContext  # noqa: E402
 from .envs import (CartPoleEnv, PendulumV2, LunarLanderV2, LunarLanderV2Continuous, BipedalWalkerV2,  # noqa: E402
                    HalfCheetahPlanarV2, CarRacingV2, HopperPlanar, Walker2dPlanar, VecStepResult)
 from .model import Model, Linear, LinearReLU, LinearTanh, StochasticActor, seq  # noqa: E402
-from .recurrent import GatedRecurrence  # noqa: E402
+from .recurrent import GatedRecurrence, GatedDeltaRule  # noqa: E402
 from .optimizer import Adam, Muon, orthogonalize  # noqa: E402
 from .training import Network, Xavier, Kaiming, init_params_small  # noqa: E402
 from . import ppo, checkpoint  # noqa: E402
@@ -21,7 +21,7 @@ from .agents import DeepPPOAgent, DeepPPOContinuousAgent, TrainingMetrics  # noq
 
 __all__ = ["DeviceContext", "CartPoleEnv", "PendulumV2", "LunarLanderV2", "LunarLanderV2Continuous", "BipedalWalkerV2",
            "HalfCheetahPlanarV2", "CarRacingV2", "HopperPlanar", "Walker2dPlanar", "VecStepResult", "MrlError", "Model",
-           "Linear", "LinearReLU", "LinearTanh", "StochasticActor", "seq", "GatedRecurrence", "Adam", "Muon", "orthogonalize", "ppo",
+           "Linear", "LinearReLU", "LinearTanh", "StochasticActor", "seq", "GatedRecurrence", "GatedDeltaRule", "Adam", "Muon", "orthogonalize", "ppo",
            "Network", "Xavier", "Kaiming", "init_params_small", "checkpoint",
            "DeepPPOAgent", "DeepPPOContinuousAgent", "TrainingMetrics",
            "LINEAR", "LINEAR_RELU", "LINEAR_TANH", "STOCHASTIC_ACTOR"]

@@ -35,6 +35,23 @@ class Matrix(C.Structure):
     _fields_ = [("offset", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32)]
 
 
+class Delta(C.Structure):
+    _fields_ = (
+        [(n, C.c_int32) for n in ("dtype", "T", "N", "heads", "key_heads", "key_dim", "value_dim")]
+        + [(n, C.c_void_p) for n in ("query", "key", "value", "gate", "rate")]
+        + [(n, C.c_int64) for n in ("query_ld", "key_ld", "value_ld", "gate_ld", "rate_ld")]
+        + [(n, C.c_void_p) for n in ("dones", "prev_dones", "state_in")]
+    )
+
+
+class DeltaGrads(C.Structure):
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("query", "key", "value", "gate", "rate")]
+        + [(n, C.c_int64) for n in ("query_ld", "key_ld", "value_ld", "gate_ld", "rate_ld")]
+        + [("state", C.c_void_p)]
+    )
+
+
 class Rollout(C.Structure):
     _fields_ = [
         ("env_id", C.c_int32), ("n_envs", C.c_int32), ("obs_dim", C.c_int32), ("num_actions", C.c_int32),
@@ -70,6 +87,7 @@ class MrlError(RuntimeError):
 
 P, I, I64, U32, U64, F, D = C.c_void_p, C.c_int, C.c_int64, C.c_uint32, C.c_uint64, C.c_float, C.c_double
 DP, RP, UP, MP = C.POINTER(MlpDesc), C.POINTER(Rollout), C.POINTER(Update), C.POINTER(Matrix)
+DELTA, DELTA_GRADS = C.POINTER(Delta), C.POINTER(DeltaGrads)
 
 # name -> argtypes; every function returns int (0 = ok) unless listed in _SPECIAL
 SIGNATURES = {
@@ -132,6 +150,9 @@ SIGNATURES = {
     "mrl_recurrence_workspace": [P, I, I, I, C.POINTER(U64)],
     "mrl_recurrence_forward": [P, I, I, I, I, P, I64, P, I64, P, P, P, P, I64, P, P, U64],
     "mrl_recurrence_backward": [P, I, I, I, I, P, I64, P, I64, P, I64, P, P, P, P, I64, P, P, I64, P, I64, P, P, U64],
+    "mrl_delta_workspace": [P, DELTA, I, C.POINTER(U64)],
+    "mrl_delta_forward": [P, DELTA, P, I64, P, P, U64],
+    "mrl_delta_backward": [P, DELTA, P, I64, P, DELTA_GRADS, P, U64],
     "mrl_orthogonalize_workspace": [I, I, I, C.POINTER(U64)],
     "mrl_orthogonalize": [P, I, I, I, I, P, P, I, D, P, U64],
     "mrl_muon_workspace": [I, MP, C.POINTER(U64)],

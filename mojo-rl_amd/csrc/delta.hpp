@@ -1,0 +1,354 @@
+// What the kernels of the gated delta rule share (mrl_delta.hip, mrl_delta_back.hip).
+//
+// Per environment and head, with a = sigmoid(gate), b = sigmoid(rate), k = key / |key|, q = query / (|query| sqrt(dk)):
+//   S' = a[t] S[t-1] (0 where the step before ended an episode),  u[t] = b[t] (v[t] - S'^T k[t]),  S[t] = S' + k[t] u[t]^T,
+//   out[t] = S[t]^T q[t].
+// TILE steps together, from the state S0 ahead of them: with G[i][j] = a[j+1] .. a[i] (1 for i = j, 0 for j > i, and 0 across a cut, whose
+// a counts as 0), F[i] = a[0] .. a[i] and L[j] = G[TILE - 1][j],
+//   A[i][j] = b[i] (k[i] k[j]) G[i][j] for j < i,   (1 + A) U = X,   X[i] = b[i] (v[i] - F[i] S0^T k[i]),
+//   out[i] = F[i] S0^T q[i] + sum_j P[i][j] U[j],   P[i][j] = (q[i] k[j]) G[i][j],
+//   S1 = F[TILE - 1] S0 + sum_j L[j] k[j] U[j]^T.
+// The decays are products of the a themselves, not exponentials of differences of sums: they keep their relative accuracy
+// whatever the a ahead of them were.
+//
+// Operands of v_mfma_f32_16x16x4_f32, lane = 16 g + n: A[row n][k = g], B[k = g][column n] -> D[row 4 g + r][column n], r = 0 .. 3.
+// Four of them contract 16 values of an index; the r-th takes 4 g + r from lane group g.  So a result [16 x 16] as it stands in
+// its registers is the B operand of a product that contracts its rows, and the A operand of such a product is four neighbouring
+// values of a row.
+#pragma once
+#include "mrl_host.hpp"
+#include "mrl_device.hpp"
+
+namespace mrl {
+namespace delta {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+struct bf16_t { unsigned short bits; };
+
+constexpr int TILE = 16;
+constexpr int MOST_DIM = 128;
+constexpr float EPS = 1e-6f;
+constexpr float LARGE = 1e30f;   // beyond this, or NaN: a value that products with 0 must not meet
+
+struct Delta {
+    int T, N, H, HK, dk, dv;
+    const void *query, *key, *value, *gate, *rate;
+    long query_ld, key_ld, value_ld, gate_ld, rate_ld;
+    const float *dones, *prev_dones, *state_in;
+    void *out;
+    long out_ld;
+    float *state_out;
+};
+
+MRL_DEV float value_of(float x) { return x; }
+MRL_DEV float value_of(bf16_t x) { return __uint_as_float((unsigned)x.bits << 16); }
+MRL_DEV void give(float *p, float x) { *p = x; }
+MRL_DEV void give(bf16_t *p, float x) { p->bits = __builtin_bit_cast(unsigned short, (__bf16)x); }
+
+// up to four neighbouring values, zeros from `n` on
+MRL_DEV f32x4 load4(const float *p, int n) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n >= 4) x = *reinterpret_cast<const f32x4u *>(p);
+    else {
+        if (n > 0) x[0] = p[0];
+        if (n > 1) x[1] = p[1];
+        if (n > 2) x[2] = p[2];
+    }
+    return x;
+}
+MRL_DEV f32x4 load4(const bf16_t *p, int n) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n >= 4) {
+        const u16x4u v = *reinterpret_cast<const u16x4u *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float((unsigned)v[i] << 16);
+    } else {
+        if (n > 0) x[0] = value_of(p[0]);
+        if (n > 1) x[1] = value_of(p[1]);
+        if (n > 2) x[2] = value_of(p[2]);
+    }
+    return x;
+}
+MRL_DEV void store4(float *p, f32x4 x, int n) {
+    if (n >= 4) *reinterpret_cast<f32x4u *>(p) = x;
+    else {
+        if (n > 0) p[0] = x[0];
+        if (n > 1) p[1] = x[1];
+        if (n > 2) p[2] = x[2];
+    }
+}
+MRL_DEV void store4(bf16_t *p, f32x4 x, int n) {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    const u16x4u v = __builtin_bit_cast(u16x4u, __builtin_convertvector(x, bf16x4));
+    if (n >= 4) *reinterpret_cast<u16x4u *>(p) = v;
+    else {
+        if (n > 0) p[0].bits = v[0];
+        if (n > 1) p[1].bits = v[1];
+        if (n > 2) p[2].bits = v[2];
+    }
+}
+
+// sigmoid(g) and 1 - sigmoid(g), each relative to its own value: e = exp(-g) is 2^y with what rounding y left taken back, the reciprocal
+// takes a Newton step.  The argument is held where e stays finite.  (minimum and maximum keep NaN.)
+MRL_DEV void sigmoid(float g, float &a, float &rest) {
+    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 200.0f);
+    const float y = g * -1.44269502f;
+    float e = __builtin_amdgcn_exp2f(y);
+    e = fmaf(e, fmaf(y, -0.693147182f, -g), e);
+    const float u = 1.0f + e;
+    a = __builtin_amdgcn_rcpf(u);
+    a = fmaf(a, fmaf(-u, a, 1.0f), a);
+    rest = e * a;
+}
+
+MRL_DEV bool is_cut(const Delta &d, int t, int n) {
+    const float *row = t > 0 ? d.dones : d.prev_dones;
+    return row != nullptr && (t > 0 ? row[(long)(t - 1) * d.N + n] : row[n]) > 0.5f;
+}
+
+MRL_DEV f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// c + A B over 16 values of the contracted index
+MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = mfma(a[r], b[r], c);
+    return c;
+}
+
+constexpr int tiles_of(int DK) { return DK == 128 ? 2 : 4; }   // tiles that a workgroup prepares together: a block
+constexpr int SIDE = TILE + 4;        // floats from a row of a 16 x 16 matrix in LDS to the next
+constexpr size_t rows_floats(int DK) { return 2 * TILE * tiles_of(DK) * (DK + 4) + 2 * tiles_of(DK) * TILE * SIDE + 6 * TILE * tiles_of(DK); }
+
+// The decays of a tile, from its 16 a in LDS.  Lane 16 g + n holds rows i = 4 g + r of column n.
+struct Decays {
+    float from[4];   // F[i]
+    float to[4];     // L[i]
+    float whole;     // F[15]
+    MRL_DEV void load(const float *a, int g) {
+        float block[4];
+        f32x4 own = {1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(a + 4 * p);
+            block[p] = x[0] * x[1] * (x[2] * x[3]);
+            if (p == g) own = x;
+        }
+        float before = 1.0f, behind = 1.0f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            before = p < g ? before * block[p] : before;
+            behind = p > g ? behind * block[p] : behind;
+        }
+        from[0] = before * own[0];
+#pragma unroll
+        for (int r = 1; r < 4; ++r) from[r] = from[r - 1] * own[r];
+        to[3] = behind;
+#pragma unroll
+        for (int r = 2; r >= 0; --r) to[r] = to[r + 1] * own[r + 1];
+        whole = block[0] * block[1] * (block[2] * block[3]);
+    }
+};
+// G[4 g + r][n], 0 above the diagonal
+MRL_DEV f32x4 between(const float *a, int g, int n) {
+    float run = 1.0f;
+    f32x4 own = {1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(a + 4 * p);
+        if (p == g) own = x;
+        if (p < g) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) run = 4 * p + r > n ? run * x[r] : run;
+        }
+    }
+    f32x4 out;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        run = 4 * g + r > n ? run * own[r] : run;
+        out[r] = 4 * g + r >= n ? run : 0.0f;
+    }
+    return out;
+}
+
+// column n of (1 + A)^-1, A [16][SIDE] strictly lower triangular: forward substitution, which is as exact as its terms allow
+// where powers of A would grow (keys that are alike)
+MRL_DEV void invert(const float *A, int n, float (&x)[TILE]) {
+#pragma unroll
+    for (int i = 0; i < TILE; ++i) {
+        float sum = i == n ? 1.0f : 0.0f;
+#pragma unroll
+        for (int p = 0; p < (i + 3) / 4; ++p) {
+            const f32x4 row = *reinterpret_cast<const f32x4 *>(A + i * SIDE + 4 * p);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (4 * p + r < i) sum = fmaf(-row[r], x[4 * p + r], sum);
+        }
+        x[i] = sum;
+    }
+}
+
+
+// What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.
+template <int DK>
+struct Block {
+    static constexpr int TILES = tiles_of(DK), STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
+    float *K, *Q, *Ts, *Ps, *as, *rests, *bs, *rate_rests, *kscale, *qscale;   // rests: 1 - a, 0 at a cut; rate_rests: 1 - b
+    int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
+    MRL_DEV explicit Block(float *lds) {
+        K = lds;
+        Q = K + STEPS * ROW;
+        Ts = Q + STEPS * ROW;
+        Ps = Ts + TILES * TILE * SIDE;
+        as = Ps + TILES * TILE * SIDE;
+        rests = as + STEPS;
+        bs = rests + STEPS;
+        rate_rests = bs + STEPS;
+        kscale = rate_rests + STEPS;
+        qscale = kscale + STEPS;
+    }
+    MRL_DEV int time_of(int slot) const { return t0 + (slot >> 4) * span + (slot & 15); }
+    MRL_DEV bool there(const Delta &d, int slot) const { return (slot & 15) < span && time_of(slot) < d.T; }
+    MRL_DEV f32x4 four(const float *scalars, int tile, int g) const { return *reinterpret_cast<const f32x4 *>(scalars + tile * TILE + 4 * g); }
+
+    // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
+    // Whether a value is too large for products with 0, or none.
+    template <class E, bool QUERIES>
+    MRL_DEV bool load(const Delta &d, int n, int h, int hk) {
+        bool odd = false;
+        const int part = (threadIdx.x & 63) % LANES;
+        for (int slot = (int)threadIdx.x / LANES; slot < STEPS; slot += (int)blockDim.x / LANES) {
+            const bool here = there(d, slot);
+            const long row = (long)time_of(slot) * d.N + n;
+            const int count = here ? d.dk - 4 * part : 0;
+            const f32x4 k = load4((const E *)d.key + (here ? row * d.key_ld + hk * d.dk + 4 * part : 0), count);
+            *reinterpret_cast<f32x4 *>(K + slot * ROW + 4 * part) = k;
+            float kk = fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))), qq = 0.0f;
+            if (QUERIES) {
+                const f32x4 q = load4((const E *)d.query + (here ? row * d.query_ld + hk * d.dk + 4 * part : 0), count);
+                *reinterpret_cast<f32x4 *>(Q + slot * ROW + 4 * part) = q;
+                qq = fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3])));
+            }
+#pragma unroll
+            for (int s = 1; s < LANES; s *= 2) {
+                kk += __shfl_xor(kk, s);
+                if (QUERIES) qq += __shfl_xor(qq, s);
+            }
+            odd |= !(kk < LARGE) || !(qq < LARGE);
+            if (part == 0) {
+                kscale[slot] = 1.0f / sqrtf(kk + EPS);
+                qscale[slot] = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
+            }
+        }
+        for (int slot = threadIdx.x; slot < STEPS; slot += blockDim.x) {
+            float a = 1.0f, rest = 0.0f, b = 0.0f, other = 0.0f;
+            if (there(d, slot)) {
+                const int t = time_of(slot);
+                const long row = (long)t * d.N + n;
+                sigmoid(value_of(((const E *)d.gate)[row * d.gate_ld + h]), a, rest);
+                sigmoid(value_of(((const E *)d.rate)[row * d.rate_ld + h]), b, other);
+                odd |= !(a + b < LARGE);
+                if (is_cut(d, t, n)) a = rest = 0.0f;
+            }
+            as[slot] = a;
+            rests[slot] = rest;
+            bs[slot] = b;
+            rate_rests[slot] = other;
+        }
+        return odd;
+    }
+
+    // (1 + A)^-1 and (QUERIES) P of a tile, by one wavefront
+    template <bool QUERIES>
+    MRL_DEV void prepare(int tile, int g, int c) {
+        const float *k_tile = K + tile * TILE * ROW + c * ROW + 4 * g, *q_tile = Q + tile * TILE * ROW + c * ROW + 4 * g;
+        f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i) {
+            const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + i * TILE);
+            kk = mfma16(k, k, kk);
+            if (QUERIES) qk = mfma16(*reinterpret_cast<const f32x4 *>(q_tile + i * TILE), k, qk);
+        }
+        const f32x4 decay = between(as + tile * TILE, g, c), b = four(bs, tile, g), ks = four(kscale, tile, g), qs = four(qscale, tile, g);
+        const float kc = kscale[tile * TILE + c];
+        float *T = Ts + tile * TILE * SIDE, *P = Ps + tile * TILE * SIDE;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = 4 * g + r;
+            T[i * SIDE + c] = i > c ? b[r] * ks[r] * (kc * kk[r]) * decay[r] : 0.0f;
+            if (QUERIES) P[i * SIDE + c] = i >= c ? qs[r] * (kc * qk[r]) * decay[r] : 0.0f;
+        }
+        __builtin_amdgcn_wave_barrier();
+        float x[TILE];
+        invert(T, c, x);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < TILE; ++r)
+            if (g == (r >> 2)) T[r * SIDE + c] = x[r];
+    }
+    MRL_DEV bool cut_ahead(int tile) const { return span == 1 && as[tile * TILE] == 0.0f; }   // hides whatever the state holds
+};
+
+// A value tile as a result's registers: row 4 g + r, column c
+template <class E, int DK>
+MRL_DEV bool load_values(const Delta &d, const Block<DK> &block, const void *rows, long ld, int n, int at, bool live, int g, f32x4 (&V)[Block<DK>::TILES]) {
+    bool odd = false;
+#pragma unroll
+    for (int tile = 0; tile < Block<DK>::TILES; ++tile)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int slot = tile * TILE + 4 * g + r;
+            V[tile][r] = live && block.there(d, slot) ? value_of(((const E *)rows)[((long)block.time_of(slot) * d.N + n) * ld + at]) : 0.0f;
+            odd |= !(fabsf(V[tile][r]) < LARGE);
+        }
+    return odd;
+}
+template <int B>
+MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd |= !(fabsf(S[i][r]) < LARGE);
+    return odd;
+}
+
+// U[4 g + r][c] of a tile from S0^T k (sk), and S0 <- S1
+template <int DK>
+MRL_DEV f32x4 solve(const Block<DK> &block, const Decays &decay, int tile, int g, int c, const f32x4 v, const f32x4 sk) {
+    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g);
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = b[r] * fmaf(-decay.from[r] * ks[r], sk[r], v[r]);
+    const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
+    return mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+}
+template <int DK>
+MRL_DEV void go_on(const Block<DK> &block, const Decays &decay, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
+    const f32x4 ks = block.four(block.kscale, tile, g);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) u[r] *= decay.to[r] * ks[r];
+#pragma unroll
+    for (int i = 0; i < DK / TILE; ++i) {
+        f32x4 k;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) k[r] = block.K[(tile * TILE + 4 * g + r) * Block<DK>::ROW + i * TILE + c];
+        S[i] = mfma16(k, u, S[i] * decay.whole);
+    }
+}
+
+// The backward pass's first launch: S ahead of every block but the first, as the lanes hold it, to
+// states [N * H][blocks][column tiles][DK / 16][64][4]
+int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, float *states, int blocks);
+inline int padded(int dk) { return dk <= 16 ? 16 : dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
+inline int column_tiles(int dv) { return (dv + TILE - 1) / TILE; }
+inline int blocks_of(int T, int dk) { return (T + TILE * tiles_of(padded(dk)) - 1) / (TILE * tiles_of(padded(dk))); }
+
+int check_sizes(const char *who, const mrl_delta *r);
+int check(const char *who, const mrl_ctx *ctx, const mrl_delta *r);
+Delta describe(const mrl_delta *r);
+__global__ void pass_state_kernel(const float *from, float *to, long n);
+
+}  // namespace delta
+}  // namespace mrl

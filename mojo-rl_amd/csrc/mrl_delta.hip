@@ -1,0 +1,297 @@
+// The gated delta rule over a time-major rollout, forwards: whole rollouts in tiles of 16 steps, and single steps.  The formulas are in
+// delta.hpp.
+#include "delta.hpp"
+
+namespace mrl {
+namespace delta {
+namespace {
+
+// ---------------------------------------------------------------- single steps
+// A wavefront holds 4 L columns of a head's state in registers: lane l columns 4 (l % L) on, rows l / L, l / L + 64 / L, ..., at most
+// R of them.  S^T k and S^T q are summed in one pass, out = a S^T q + (q k) u follows from them, and the state is read and written once.
+template <class E, int L, int R>
+__global__ __launch_bounds__(256) void step_kernel(Delta d, int units, int column_blocks) {
+    constexpr int G = 64 / L;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (unit >= units) return;
+    const int block = unit % column_blocks, nh = unit / column_blocks, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    const int c = block * 4 * L + 4 * (lane % L), mine = d.dv - c, rg = lane / L;
+    const long at = (long)nh * d.dk * d.dv + c;
+    f32x4 S[R];
+    const bool cut = is_cut(d, 0, n);
+#pragma unroll
+    for (int i = 0; i < R; ++i) S[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (d.state_in != nullptr && !cut) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) S[i] = load4(d.state_in + at + (long)(rg + i * G) * d.dv, rg + i * G < d.dk ? mine : 0);
+    }
+    const E *q_row = (const E *)d.query + n * d.query_ld + hk * d.dk, *k_row = (const E *)d.key + n * d.key_ld + hk * d.dk;
+    const f32x4 v = load4((const E *)d.value + n * d.value_ld + (long)h * d.dv + c, mine);
+    float a, b, rest;
+    sigmoid(value_of(((const E *)d.gate)[n * d.gate_ld + h]), a, rest);
+    sigmoid(value_of(((const E *)d.rate)[n * d.rate_ld + h]), b, rest);
+    float k[R], q[R], kk = 0.0f, qq = 0.0f, qk = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const bool there = rg + i * G < d.dk;
+        k[i] = there ? value_of(k_row[rg + i * G]) : 0.0f;
+        q[i] = there ? value_of(q_row[rg + i * G]) : 0.0f;
+    }
+    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        kk = fmaf(k[i], k[i], kk);
+        qq = fmaf(q[i], q[i], qq);
+        qk = fmaf(q[i], k[i], qk);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sk[j] = fmaf(k[i], S[i][j], sk[j]);
+            sq[j] = fmaf(q[i], S[i][j], sq[j]);
+        }
+    }
+#pragma unroll
+    for (int s = L; s < 64; s *= 2) {
+        kk += __shfl_xor(kk, s);
+        qq += __shfl_xor(qq, s);
+        qk += __shfl_xor(qk, s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sk[j] += __shfl_xor(sk[j], s);
+            sq[j] += __shfl_xor(sq[j], s);
+        }
+    }
+    const float ks = 1.0f / sqrtf(kk + EPS), qs = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
+    f32x4 u, o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        u[j] = b * fmaf(-a * ks, sk[j], v[j]);
+        o[j] = qs * fmaf(ks * qk, u[j], a * sq[j]);
+    }
+    if (rg == 0) store4((E *)d.out + n * d.out_ld + (long)h * d.dv + c, o, mine);
+    if (d.state_out == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const float ki = ks * k[i];
+        f32x4 s;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = fmaf(ki, u[j], a * S[i][j]);
+        if (rg + i * G < d.dk) store4(d.state_out + at + (long)(rg + i * G) * d.dv, s, mine);
+    }
+}
+
+// ---------------------------------------------------------------- rollouts
+constexpr int MOST_WAVES = 4;
+
+// A workgroup goes through the steps of one head of one environment; each of its wavefronts keeps 16 columns of the state in registers,
+// all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.  STATES: no outputs, the
+// state ahead of every block instead.
+template <class E, int DK, bool STATES>
+__global__ __launch_bounds__(64 * MOST_WAVES) void tiles_kernel(Delta d, int column_groups, float *states, int blocks) {
+    extern __shared__ float lds[];
+    constexpr int B = DK / TILE, TILES = Block<DK>::TILES, STEPS = Block<DK>::STEPS, ROW = Block<DK>::ROW;
+    Block<DK> block(lds);
+    const int W = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int group = blockIdx.x % column_groups, nh = blockIdx.x / column_groups, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    const int column_tile = group * W + w, column = column_tile * TILE + c;
+    const bool live = column < d.dv;
+    const long state_at = (long)nh * d.dk * d.dv + column;
+
+    f32x4 S[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = i * TILE + 4 * g + r;
+            S[i][r] = d.state_in != nullptr && live && row < d.dk ? d.state_in[state_at + (long)row * d.dv] : 0.0f;
+        }
+
+    block.span = TILE;
+    int begin = 0;   // of the block
+    for (block.t0 = 0; block.t0 < d.T;) {
+        if (STATES && block.t0 == begin) {
+            const int number = begin / STEPS;
+            if (number > 0 && column_tile * TILE < d.dv) {
+                float *to = states + ((((long)nh * blocks + number) * ((d.dv + TILE - 1) / TILE) + column_tile) * B * 64 + lane) * 4;
+#pragma unroll
+                for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = S[i];
+            }
+            if (number == blocks - 1) return;
+        }
+        f32x4 V[TILES];
+        bool odd = is_odd(S);
+        odd |= load_values<E, DK>(d, block, d.value, d.value_ld, n, h * d.dv + column, live, g, V);
+        odd |= block.template load<E, !STATES>(d, n, h, hk);
+        if (__syncthreads_or(odd) && block.span == TILE) {
+            block.span = 1;
+            continue;   // the same block again, one step to a tile
+        }
+        for (int tile = w; tile < TILES; tile += W) block.template prepare<!STATES>(tile, g, c);
+        __syncthreads();
+#pragma unroll 1
+        for (int tile = 0; tile < TILES; ++tile) {
+            if (block.t0 + tile * block.span >= d.T) break;
+            Decays decay;
+            decay.load(block.as + tile * TILE, g);
+            if (block.cut_ahead(tile)) {
+#pragma unroll
+                for (int i = 0; i < B; ++i) S[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, o = sk;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const int at = (tile * TILE + c) * ROW + i * TILE + 4 * g;
+                sk = mfma16(*reinterpret_cast<const f32x4 *>(block.K + at), S[i], sk);
+                if (!STATES) o = mfma16(*reinterpret_cast<const f32x4 *>(block.Q + at), S[i], o);
+            }
+            f32x4 v = V[0];
+#pragma unroll
+            for (int i = 1; i < TILES; ++i) v = tile == i ? V[i] : v;
+            const f32x4 u = solve(block, decay, tile, g, c, v, sk);
+            if (!STATES) {
+                const f32x4 qs = block.four(block.qscale, tile, g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] *= decay.from[r] * qs[r];
+                o = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + tile * TILE * SIDE + c * SIDE + 4 * g), u, o);
+            }
+            go_on(block, decay, tile, g, c, u, S);
+            if (!STATES) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int slot = tile * TILE + 4 * g + r;
+                    if (live && block.there(d, slot)) give((E *)d.out + ((long)block.time_of(slot) * d.N + n) * d.out_ld + h * d.dv + column, o[r]);
+                }
+            }
+        }
+        block.t0 += TILES * block.span;
+        if (block.t0 >= begin + STEPS) {
+            begin = block.t0;
+            block.span = TILE;
+        }
+        __syncthreads();
+    }
+    if (STATES || d.state_out == nullptr || !live) return;
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = i * TILE + 4 * g + r;
+            if (row < d.dk) d.state_out[state_at + (long)row * d.dv] = S[i][r];
+        }
+}
+
+template <class E, int L>
+void launch_step(const mrl_ctx *ctx, const Delta &d) {
+    const int blocks = (d.dv + 4 * L - 1) / (4 * L), units = d.N * d.H * blocks, rows = (d.dk + 64 / L - 1) / (64 / L);
+    const dim3 grid((units + 3) / 4), block(256);
+    if (rows <= 4) hipLaunchKernelGGL((step_kernel<E, L, 4>), grid, block, 0, ctx->stream, d, units, blocks);
+    else if (rows <= 8) hipLaunchKernelGGL((step_kernel<E, L, 8>), grid, block, 0, ctx->stream, d, units, blocks);
+    else if (rows <= 16) hipLaunchKernelGGL((step_kernel<E, L, 16>), grid, block, 0, ctx->stream, d, units, blocks);
+    else hipLaunchKernelGGL((step_kernel<E, L, 32>), grid, block, 0, ctx->stream, d, units, blocks);
+}
+template <class E, bool STATES, int DK>
+void launch_tiles(const mrl_ctx *ctx, const Delta &d, float *states, int blocks) {
+    const int tiles = column_tiles(d.dv), waves = std::min(MOST_WAVES, tiles), groups = (tiles + waves - 1) / waves;
+    hipLaunchKernelGGL((tiles_kernel<E, DK, STATES>), dim3(d.N * d.H * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK), ctx->stream, d, groups, states, blocks);
+}
+template <class E, bool STATES>
+void launch_tiles(const mrl_ctx *ctx, const Delta &d, float *states = nullptr, int blocks = 0) {
+    switch (padded(d.dk)) {
+        case 16: return launch_tiles<E, STATES, 16>(ctx, d, states, blocks);
+        case 32: return launch_tiles<E, STATES, 32>(ctx, d, states, blocks);
+        case 64: return launch_tiles<E, STATES, 64>(ctx, d, states, blocks);
+        default: return launch_tiles<E, STATES, 128>(ctx, d, states, blocks);
+    }
+}
+template <class E>
+void launch(const mrl_ctx *ctx, const Delta &d) {
+    if (d.T > 1) launch_tiles<E, false>(ctx, d);
+    else if (d.dv <= 32) launch_step<E, 8>(ctx, d);
+    else launch_step<E, 16>(ctx, d);
+}
+
+}  // namespace
+
+// no step at all: the state goes through as it is
+__global__ __launch_bounds__(256) void pass_state_kernel(const float *from, float *to, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) to[i] = from ? from[i] : 0.0f;
+}
+
+int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, float *states, int blocks) {
+    if (dtype == MRL_F32) launch_tiles<float, true>(ctx, d, states, blocks);
+    else launch_tiles<bf16_t, true>(ctx, d, states, blocks);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+
+int check_sizes(const char *who, const mrl_delta *r) {
+    MRL_CHECK_ARG(r->dtype == MRL_F32 || r->dtype == MRL_BF16, "%s: unknown element type %d", who, r->dtype);
+    MRL_CHECK_ARG(r->T >= 0 && r->N >= 0, "%s: negative size", who);
+    MRL_CHECK_ARG(r->T < 1 << 30, "%s: %d steps are 2^30 or more", who, r->T);
+    MRL_CHECK_ARG(r->heads >= 1 && r->key_heads >= 1 && r->heads % r->key_heads == 0, "%s: %d heads on %d key heads", who, r->heads, r->key_heads);
+    MRL_CHECK_ARG(r->key_dim >= 1 && r->key_dim <= MOST_DIM && r->value_dim >= 1 && r->value_dim <= MOST_DIM,
+                  "%s: key_dim %d and value_dim %d: 1 to %d expected", who, r->key_dim, r->value_dim, MOST_DIM);
+    MRL_CHECK_ARG((long)r->N * r->heads < 1L << 22, "%s: %d environments of %d heads are 2^22 states or more", who, r->N, r->heads);
+    MRL_CHECK_ARG(r->heads < 1 << 22, "%s: %d heads are 2^22 or more", who, r->heads);
+    return MRL_OK;
+}
+int check(const char *who, const mrl_ctx *ctx, const mrl_delta *r) {
+    MRL_CHECK_ARG(ctx && r, "%s: NULL ctx or description", who);
+    const int rc = check_sizes(who, r);
+    if (rc != MRL_OK) return rc;
+    if (r->T == 0 || r->N == 0) return MRL_OK;
+    MRL_CHECK_ARG(r->query && r->key && r->value && r->gate && r->rate, "%s: NULL buffer", who);
+    const long k_width = (long)r->key_heads * r->key_dim, v_width = (long)r->heads * r->value_dim;
+    MRL_CHECK_ARG(r->query_ld >= k_width && r->key_ld >= k_width && r->value_ld >= v_width && r->gate_ld >= r->heads && r->rate_ld >= r->heads,
+                  "%s: a row stride is smaller than the row", who);
+    return MRL_OK;
+}
+
+Delta describe(const mrl_delta *r) {
+    Delta d = {};
+    d.T = r->T; d.N = r->N; d.H = r->heads; d.HK = r->key_heads; d.dk = r->key_dim; d.dv = r->value_dim;
+    d.query = r->query; d.key = r->key; d.value = r->value; d.gate = r->gate; d.rate = r->rate;
+    d.query_ld = r->query_ld; d.key_ld = r->key_ld; d.value_ld = r->value_ld; d.gate_ld = r->gate_ld; d.rate_ld = r->rate_ld;
+    d.dones = r->dones; d.prev_dones = r->prev_dones; d.state_in = r->state_in;
+    return d;
+}
+
+}  // namespace delta
+}  // namespace mrl
+
+extern "C" {
+
+int mrl_delta_forward(mrl_ctx *ctx, const mrl_delta *r, void *out, int64_t out_ld, float *state_out, void *workspace,
+                      uint64_t workspace_bytes) {
+    using namespace mrl;
+    using namespace mrl::delta;
+    const char *who = "mrl_delta_forward";
+    const int rc = check(who, ctx, r);
+    if (rc != MRL_OK) return rc;
+    if (r->N == 0) return MRL_OK;
+    const long states = (long)r->N * r->heads * r->key_dim * r->value_dim;
+    MRL_CHECK_ARG(r->T == 0 || out, "%s: NULL buffer", who);
+    MRL_CHECK_ARG(r->T == 0 || out_ld >= (long)r->heads * r->value_dim, "%s: a row stride is smaller than the row", who);
+    const int64_t size = r->dtype == MRL_F32 ? 4 : 2, rows = (int64_t)r->T * r->N;
+    const auto of = [&](const char *name, const void *at, long width, long ld) { return Region(name, at, rows, size * width, size * ld); };
+    const long k_width = (long)r->key_heads * r->key_dim, v_width = (long)r->heads * r->value_dim;
+    const int apart = check_apart(who, {of("out", out, v_width, out_ld), Region("state_out", state_out, 4 * states)},
+                                  {of("query", r->query, k_width, r->query_ld), of("key", r->key, k_width, r->key_ld), of("value", r->value, v_width, r->value_ld),
+                                   of("gate", r->gate, r->heads, r->gate_ld), of("rate", r->rate, r->heads, r->rate_ld), Region("dones", r->dones, 4 * rows),
+                                   Region("prev_dones", r->prev_dones, 4LL * r->N), Region("state_in", r->state_in == state_out ? nullptr : r->state_in, 4 * states)});
+    if (apart != MRL_OK) return apart;
+    OnDevice on(ctx);
+    if (r->T == 0) {
+        if (state_out != nullptr && state_out != r->state_in)
+            hipLaunchKernelGGL(pass_state_kernel, dim3((int)std::min<long>((states + 255) / 256, 4096)), dim3(256), 0, ctx->stream, r->state_in, state_out, states);
+        MRL_CHECK_LAUNCH();
+        return MRL_OK;
+    }
+    Delta d = describe(r);
+    d.out = out; d.out_ld = out_ld; d.state_out = state_out;
+    if (r->dtype == MRL_F32) launch<float>(ctx, d);
+    else launch<bf16_t>(ctx, d);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+
+}  // extern "C"
