@@ -21,6 +21,7 @@ ENV_LUNARLANDER_CONTINUOUS = 5
 ENV_CARRACING = 6
 ENV_HOPPER_PLANAR, ENV_WALKER2D_PLANAR = 7, 8
 F32, BF16 = 0, 1   # element types
+CLIP_TENSORS_WORKSPACE = 16384
 
 
 class Layer(C.Structure):
@@ -33,6 +34,10 @@ class MlpDesc(C.Structure):
 
 class Matrix(C.Structure):
     _fields_ = [("offset", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
+class Tensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32)]
 
 
 class Delta(C.Structure):
@@ -155,6 +160,7 @@ SIGNATURES = {
     "mrl_delta_backward": [P, DELTA, P, I64, P, DELTA_GRADS, P, U64],
     "mrl_orthogonalize_workspace": [I, I, I, C.POINTER(U64)],
     "mrl_orthogonalize": [P, I, I, I, I, P, P, I, D, P, U64],
+    "mrl_clip_tensors": [P, I, C.POINTER(Tensor), D, P, P, U64],
     "mrl_muon_workspace": [I, MP, C.POINTER(U64)],
     "mrl_muon_step": [P, P, P, P, I64, I, MP, I, D, D, I, D, I, D, D, D, D, D, P, U64],
 }

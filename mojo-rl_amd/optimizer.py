@@ -29,6 +29,39 @@ class Adam:
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
+def clip_grad_norm(ctx, out, grads, max_norm, norm=None):
+    """out[i] = grads[i] * min(1, max_norm / (norm + 1e-8)) with the norm of all values of all tensors, which `norm`, one float32 value, receives
+    before clipping (None: not wanted).  grads and out are sequences of contiguous float32 or bfloat16 tensors; out[i] may be grads[i], but
+    not overlap a tensor otherwise.  ppo.clip_grad_norm is the same for one vector."""
+    if len(out) != len(grads):
+        raise _lib.MrlError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
+    entries = []
+    for i, (o, g) in enumerate(zip(out, grads)):
+        kind = _TYPES.get(g.dtype)
+        if kind is None:
+            raise _lib.MrlError("clip_grad_norm: grads[%d]: float32 or bfloat16 expected, got %s" % (i, g.dtype))
+        if o is not g:
+            if o.shape != g.shape or o.dtype is not g.dtype:
+                raise _lib.MrlError("clip_grad_norm: out[%d] %s of %s does not fit %s of %s" % (i, list(o.shape), o.dtype, list(g.shape), g.dtype))
+            if not o.is_contiguous():
+                raise _lib.MrlError("clip_grad_norm: out[%d] must be contiguous" % i)
+        if not g.is_contiguous():
+            raise _lib.MrlError("clip_grad_norm: grads[%d] must be contiguous" % i)
+        if g.device != ctx.device or o.device != ctx.device:
+            _on_device(ctx, "grads[%d]" % i, g)
+            _on_device(ctx, "out[%d]" % i, o)
+        entries.append((g.data_ptr(), o.data_ptr(), g.numel(), kind))
+    if not max_norm >= 0:
+        raise _lib.MrlError("clip_grad_norm: max_norm %s is below 0" % max_norm)
+    if norm is not None:
+        if norm.numel() != 1 or norm.dtype is not torch.float32:
+            raise _lib.MrlError("clip_grad_norm: norm: one float32 value expected, got %s of %s" % (list(norm.shape), norm.dtype))
+        _on_device(ctx, "norm", norm)
+    ws = _scratch(ctx, _lib.CLIP_TENSORS_WORKSPACE)
+    _lib.call("mrl_clip_tensors", ctx.handle, len(entries), (_lib.Tensor * len(entries))(*entries), float(max_norm),
+              None if norm is None else norm.data_ptr(), ws.data_ptr(), _lib.CLIP_TENSORS_WORKSPACE)
+
+
 @functools.lru_cache(maxsize=None)
 def _orthogonalize_bytes(count, rows, cols):
     size = C.c_uint64(0)
