@@ -64,11 +64,11 @@ MRL_DEV void squares(const E *p, int64_t n, int64_t at, double &sum) {
     }
 }
 template <class E>
-MRL_DEV void scaled(const E *p, E *out, int64_t n, int64_t at, float scale) {
+MRL_DEV void scaled(const E *p, E *out, int64_t n, int64_t at, float scale, float unit) {
     const int64_t i = at + threadIdx.x * 8;
-    if (i + 8 <= n) store8(out + i, load8(p + i) * scale);
+    if (i + 8 <= n) store8(out + i, load8(p + i) * scale * unit);
     else
-        for (int64_t j = i; j < n; ++j) give(out + j, value_of(p[j]) * scale);
+        for (int64_t j = i; j < n; ++j) give(out + j, value_of(p[j]) * scale * unit);
 }
 
 MRL_DEV double block_sum(double x, double *shared) {
@@ -101,15 +101,18 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table t, const double *s
     const double norm = sqrt(block_sum(sum, shared));
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) *norm_out = (float)norm;
     const bool clips = norm > max_norm;
-    const float scale = clips ? (float)(max_norm / (norm + 1e-8)) : 1.0f;
+    // a factor among fp32's subnormals, which would have few bits, is taken in two steps, the second a power of two
+    const double factor = clips ? max_norm / (norm + 1e-8) : 1.0;
+    const bool tiny = factor < 0x1p-100;
+    const float scale = (float)(tiny ? factor * 0x1p100 : factor), unit = tiny ? 0x1p-100f : 1.0f;
     const int64_t from = blockIdx.x * t.per, to = min(from + t.per, t.begin[t.count]);
     int k = 0;
     for (int64_t piece = from; piece < to; ++piece) {
         while (piece >= t.begin[k + 1]) ++k;
         if (!clips && t.in[k] == t.out[k]) continue;
         const int64_t at = (piece - t.begin[k]) * PIECE;
-        if (t.bf16[k]) scaled((const bf16_t *)t.in[k], (bf16_t *)t.out[k], t.n[k], at, scale);
-        else scaled((const float *)t.in[k], (float *)t.out[k], t.n[k], at, scale);
+        if (t.bf16[k]) scaled((const bf16_t *)t.in[k], (bf16_t *)t.out[k], t.n[k], at, scale, unit);
+        else scaled((const float *)t.in[k], (float *)t.out[k], t.n[k], at, scale, unit);
     }
 }
 

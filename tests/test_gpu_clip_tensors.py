@@ -39,7 +39,8 @@ def check(mrl, ctx, grads, max_norm, out):
         if scale == 1.0:
             assert torch.equal(got, g)
         else:
-            assert ((got - g * scale).abs() <= OFF[o.dtype] * (g * scale).abs()).all()
+            # (below 2^-126 fp32 goes in steps of 2^-149)
+            assert ((got - g * scale).abs() <= OFF[o.dtype] * (g * scale).abs() + 2.0 ** -149).all()
 
 
 @pytest.mark.parametrize("place", ["in", "out"])
