@@ -505,6 +505,26 @@ int mrl_delta_forward(mrl_ctx *ctx, const mrl_delta *r, void *out, int64_t out_l
 int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, int64_t grad_out_ld, const float *grad_state_out,
                        const mrl_delta_grads *grads, void *workspace, uint64_t workspace_bytes);
 
+/* ------------------------------------------------------------------ gated linear layer
+ * Two linear layers of one input, one the other's gate (no counterpart in the reference):
+ *     out = act(in Wg + bg) * (in Wu + bu),   act: sigmoid, g sigmoid(g), g Phi(g) (Phi the normal distribution's) or tanh.
+ * params are those of a MRL_LINEAR of in_dim -> 2 out_dim, W [in_dim, 2 out_dim] row-major, then the biases: column j of W is Wg's, column
+ * out_dim + j Wu's.  in and out have `rows` rows of `dtype`, `ld` elements apart, and params are of `dtype` too (in bf16 a rounded copy of what the
+ * optimiser keeps).  Sums are fp32, values are rounded when stored.  An infinity in `in` or params makes NaN of what it reaches where dtype is fp32.
+ *
+ * Backward overwrites grads (fp32, laid out like params, whatever the type) and grad_in (may be NULL) from the gradient of out; it works gate and
+ * up out again.  All sums are in a fixed order.  Rows are below 2^26, dims 1 to 65536.
+ *
+ * No element of an output may be one of an input's or of another output's (MRL_E_ARG).  The workspace (device, 16-byte aligned, need not be kept
+ * between calls; NULL where the size is 0) holds at least mrl_gated_linear_workspace's bytes. */
+enum mrl_gate { MRL_GATE_SIGMOID = 0, MRL_GATE_SILU = 1, MRL_GATE_GELU = 2, MRL_GATE_TANH = 3 };
+int mrl_gated_linear_workspace(mrl_ctx *ctx, int dtype, int rows, int in_dim, int out_dim, int backward, uint64_t *bytes);
+int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_dim, int out_dim, const void *in, int64_t in_ld,
+                             const void *params, void *out, int64_t out_ld, void *workspace, uint64_t workspace_bytes);
+int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in_dim, int out_dim, const void *grad_out,
+                              int64_t grad_out_ld, const void *in, int64_t in_ld, const void *params, void *grad_in, int64_t grad_in_ld,
+                              float *grads, void *workspace, uint64_t workspace_bytes);
+
 /* ------------------------------------------------------------------ orthogonalised updates
  * No counterpart in the reference, whose optimisers work element by element.  A matrix's polynomial
  *     X = G / (|G| + eps)  (Frobenius norm);   `steps` times  X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X

@@ -14,6 +14,7 @@ from .envs import (CartPoleEnv, PendulumV2, LunarLanderV2, LunarLanderV2Continuo
                    HalfCheetahPlanarV2, CarRacingV2, HopperPlanar, Walker2dPlanar, VecStepResult)
 from .model import Model, Linear, LinearReLU, LinearTanh, StochasticActor, seq  # noqa: E402
 from .recurrent import GatedRecurrence, GatedDeltaRule  # noqa: E402
+from .gated import GatedLinear  # noqa: E402
 from .optimizer import Adam, Muon, clip_grad_norm, orthogonalize  # noqa: E402
 from .training import Network, Xavier, Kaiming, init_params_small  # noqa: E402
 from . import ppo, checkpoint  # noqa: E402
@@ -21,7 +22,7 @@ from .agents import DeepPPOAgent, DeepPPOContinuousAgent, TrainingMetrics  # noq
 
 __all__ = ["DeviceContext", "CartPoleEnv", "PendulumV2", "LunarLanderV2", "LunarLanderV2Continuous", "BipedalWalkerV2",
            "HalfCheetahPlanarV2", "CarRacingV2", "HopperPlanar", "Walker2dPlanar", "VecStepResult", "MrlError", "Model",
-           "Linear", "LinearReLU", "LinearTanh", "StochasticActor", "seq", "GatedRecurrence", "GatedDeltaRule", "Adam", "Muon", "clip_grad_norm", "orthogonalize", "ppo",
+           "Linear", "LinearReLU", "LinearTanh", "StochasticActor", "seq", "GatedRecurrence", "GatedDeltaRule", "GatedLinear", "Adam", "Muon", "clip_grad_norm", "orthogonalize", "ppo",
            "Network", "Xavier", "Kaiming", "init_params_small", "checkpoint",
            "DeepPPOAgent", "DeepPPOContinuousAgent", "TrainingMetrics",
            "LINEAR", "LINEAR_RELU", "LINEAR_TANH", "STOCHASTIC_ACTOR"]

@@ -158,6 +158,9 @@ SIGNATURES = {
     "mrl_delta_workspace": [P, DELTA, I, C.POINTER(U64)],
     "mrl_delta_forward": [P, DELTA, P, I64, P, P, U64],
     "mrl_delta_backward": [P, DELTA, P, I64, P, DELTA_GRADS, P, U64],
+    "mrl_gated_linear_workspace": [P, I, I, I, I, I, C.POINTER(U64)],
+    "mrl_gated_linear_forward": [P, I, I, I, I, I, P, I64, P, P, I64, P, U64],
+    "mrl_gated_linear_backward": [P, I, I, I, I, I, P, I64, P, I64, P, P, I64, P, P, U64],
     "mrl_orthogonalize_workspace": [I, I, I, C.POINTER(U64)],
     "mrl_orthogonalize": [P, I, I, I, I, P, P, I, D, P, U64],
     "mrl_clip_tensors": [P, I, C.POINTER(Tensor), D, P, P, U64],

@@ -25,6 +25,27 @@ def _on_device(ctx, name, t):
         raise _lib.MrlError("%s: a tensor on %s expected, got one on %s" % (name, ctx.device, t.device))
 
 
+def _rows(ctx, name, t, size, dtype):
+    """(pointer, elements from a row to the next) of a tensor of size (rows, width)."""
+    if t.shape == size and t.dtype is dtype and t.device == ctx.device:
+        row, element = t.stride()
+        if element == 1 and row >= size[1]:
+            return t.data_ptr(), row
+    if t.shape != size:
+        raise _lib.MrlError("%s: a [%d, %d] tensor expected, got %s" % (name, *size, list(t.shape)))
+    if t.dtype != dtype:
+        raise _lib.MrlError("%s: %s expected, got %s" % (name, dtype, t.dtype))
+    _on_device(ctx, name, t)
+    row, element = t.stride()
+    if size[1] > 1 and element != 1 and size[0] > 0:
+        raise _lib.MrlError("%s: the elements of a row must be next to each other, got strides %s" % (name, t.stride()))
+    if size[0] < 2:
+        row = size[1]
+    elif row < size[1]:
+        raise _lib.MrlError("%s: rows overlap, got strides %s" % (name, t.stride()))
+    return t.data_ptr(), row
+
+
 def _scratch(ctx, n):
     """n bytes from torch's allocator on the context's stream: a captured graph keeps its own."""
     if torch.cuda.current_stream(ctx.device) == ctx.stream:

@@ -18,6 +18,7 @@
 #pragma once
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
+#include "gate.hpp"
 
 namespace mrl {
 namespace delta {
@@ -89,19 +90,6 @@ MRL_DEV void store4(bf16_t *p, f32x4 x, int n) {
         if (n > 1) p[1].bits = v[1];
         if (n > 2) p[2].bits = v[2];
     }
-}
-
-// sigmoid(g) and 1 - sigmoid(g), each relative to its own value: e = exp(-g) is 2^y with what rounding y left taken back, the reciprocal
-// takes a Newton step.  The argument is held where e stays finite.  (minimum and maximum keep NaN.)
-MRL_DEV void sigmoid(float g, float &a, float &rest) {
-    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 200.0f);
-    const float y = g * -1.44269502f;
-    float e = __builtin_amdgcn_exp2f(y);
-    e = fmaf(e, fmaf(y, -0.693147182f, -g), e);
-    const float u = 1.0f + e;
-    a = __builtin_amdgcn_rcpf(u);
-    a = fmaf(a, fmaf(-u, a, 1.0f), a);
-    rest = e * a;
 }
 
 MRL_DEV bool is_cut(const Delta &d, int t, int n) {
@@ -246,8 +234,8 @@ struct Block {
             if (there(d, slot)) {
                 const int t = time_of(slot);
                 const long row = (long)t * d.N + n;
-                sigmoid(value_of(((const E *)d.gate)[row * d.gate_ld + h]), a, rest);
-                sigmoid(value_of(((const E *)d.rate)[row * d.rate_ld + h]), b, other);
+                sigmoid_pair(value_of(((const E *)d.gate)[row * d.gate_ld + h]), a, rest);
+                sigmoid_pair(value_of(((const E *)d.rate)[row * d.rate_ld + h]), b, other);
                 odd |= !(a + b < LARGE);
                 if (is_cut(d, t, n)) a = rest = 0.0f;
             }

@@ -28,8 +28,8 @@ __global__ __launch_bounds__(256) void step_kernel(Delta d, int units, int colum
     const E *q_row = (const E *)d.query + n * d.query_ld + hk * d.dk, *k_row = (const E *)d.key + n * d.key_ld + hk * d.dk;
     const f32x4 v = load4((const E *)d.value + n * d.value_ld + (long)h * d.dv + c, mine);
     float a, b, rest;
-    sigmoid(value_of(((const E *)d.gate)[n * d.gate_ld + h]), a, rest);
-    sigmoid(value_of(((const E *)d.rate)[n * d.rate_ld + h]), b, rest);
+    sigmoid_pair(value_of(((const E *)d.gate)[n * d.gate_ld + h]), a, rest);
+    sigmoid_pair(value_of(((const E *)d.rate)[n * d.rate_ld + h]), b, rest);
     float k[R], q[R], kk = 0.0f, qq = 0.0f, qk = 0.0f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {

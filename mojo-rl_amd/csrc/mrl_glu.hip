@@ -1,0 +1,616 @@
+// The gated linear layer: out = act(x Wg + bg) * (x Wu + bu), and its gradient.  x [M, K], [Wg | Wu] the columns of W [K, 2 N].
+//
+//   gate = x Wg + bg, up = x Wu + bu;   dgate = dout up act'(gate), dup = dout act(gate);
+//   dx = dgate Wg^T + dup Wu^T,   dW = x^T [dgate | dup],   db = column sums of [dgate | dup].
+// gate and up are worked out again for the gradient: that is a third of its products, and keeping them would be 8 N bytes per row written and
+// read, more time than the products take.
+//
+// Products run on the bf16 matrix cores with fp32 sums.  bf16 values are operands as they are.  An fp32 value is three bf16 pieces
+// (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup] goes into dx as one piece, like any bf16
+// activation between two products (rounding it costs dx what rounding dx costs), and into dW, which is fp32, as two: 2^-17 of a term off.
+//
+// Operands lie in the workspace as fragments: 16 rows and 32 of the contracted index, a KiB in the order in which the 64 lanes of
+// v_mfma_f32_16x16x32_bf16 hold them (lane 16 g + n: row n, elements 8 g .. 8 g + 7), the pieces of a fragment next to each other, all rows'
+// fragments of 32 of the contracted index one behind the other, zeros past the ends.  Whoever makes an operand writes it so; reading is whole and in
+// order, from memory to LDS past the registers and from there without conflicts.  The 2 N columns of gate and up alternate by 16.
+#include "mlp_split.hpp"
+#include "mrl_host.hpp"
+#include "gate.hpp"
+
+namespace mrl {
+namespace glu {
+namespace {
+
+struct bf16_t { unsigned short bits; };
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4w __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int KIB = 512;   // elements of a fragment's piece
+
+MRL_DEV float value_of(float x) { return x; }
+MRL_DEV float value_of(bf16_t x) { return __uint_as_float((unsigned)x.bits << 16); }
+MRL_DEV void give(float *p, float x) { *p = x; }
+MRL_DEV void give(bf16_t *p, float x) { p->bits = __builtin_bit_cast(unsigned short, (__bf16)x); }
+
+// eight neighbouring values, zeros from `n` on
+MRL_DEV f32x8 load8(const float *p, int n) {
+    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (n >= 8) {
+        const f32x4u a = *reinterpret_cast<const f32x4u *>(p), b = *reinterpret_cast<const f32x4u *>(p + 4);
+        x = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < n) x[i] = p[i];
+    }
+    return x;
+}
+MRL_DEV f32x8 load8(const bf16_t *p, int n) {
+    f32x8 x = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (n >= 8) {
+        const u16x8u v = *reinterpret_cast<const u16x8u *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((unsigned)v[i] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < n) x[i] = value_of(p[i]);
+    }
+    return x;
+}
+
+// the first P pieces of eight values
+template <int P>
+MRL_DEV void put_pieces(const f32x8 x, __bf16 *fragment, int lane) {
+    if constexpr (P == 3) {
+        bf16x8 p[SPLIT];
+        split8(x, p);
+#pragma unroll
+        for (int i = 0; i < P; ++i) *reinterpret_cast<bf16x8 *>(fragment + i * KIB + lane * 8) = p[i];
+    } else {
+        *reinterpret_cast<bf16x8 *>(fragment + lane * 8) = __builtin_convertvector(x, bf16x8);
+    }
+}
+
+// ---------------------------------------------------------------- operands from rows
+// A matrix [rows, columns] of E, `ld` apart, whose columns may be gate and up side by side.
+struct Source {
+    const void *at;
+    long ld;
+    int rows, columns;   // columns: of gate and up each where they alternate
+};
+// Fragments of its rows, contracted along its columns; PAIRED: gate and up alternate by 16 columns.  A wavefront a fragment.
+template <class E, int P, bool PAIRED>
+__global__ __launch_bounds__(256) void along_rows_kernel(Source s, __bf16 *to, int row_fragments, int blocks) {
+    const long fragment = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (fragment >= (long)row_fragments * blocks) return;
+    const int lane = threadIdx.x & 63, block = (int)(fragment / row_fragments), row = (int)(fragment - (long)block * row_fragments) * 16 + (lane & 15), g = lane >> 4;
+    const int column = PAIRED ? block * 16 + (g & 1) * 8 : block * 32 + g * 8;
+    const E *p = (const E *)s.at + row * s.ld + column + (PAIRED && g >= 2 ? s.columns : 0);
+    put_pieces<P>(load8(p, row < s.rows ? s.columns - column : 0), to + fragment * P * KIB, lane);
+}
+// Fragments of its columns, contracted along its rows.  A workgroup 32 rows and 64 columns, turned in LDS.
+template <class E, int P, bool PAIRED>
+__global__ __launch_bounds__(256) void along_columns_kernel(Source s, __bf16 *to, int column_fragments) {
+    __shared__ float tile[64][33];
+    const int across = PAIRED ? 32 : 64, block = blockIdx.y, first = blockIdx.x * across;   // (PAIRED: 32 columns of each)
+    for (int i = threadIdx.x; i < 32 * 64; i += 256) {
+        const int r = i >> 6, c = i & 63, row = block * 32 + r;
+        // fragments in order: PAIRED has gate 0 .. 15, up 0 .. 15, gate 16 .. 31, up 16 .. 31
+        const int column = PAIRED ? first + (c >> 5) * 16 + (c & 15) : first + c;
+        const bool there = row < s.rows && column < s.columns;
+        tile[c][r] = there ? value_of(((const E *)s.at)[row * s.ld + column + (PAIRED && (c & 16) ? s.columns : 0)]) : 0.0f;
+    }
+    __syncthreads();
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, fragment = blockIdx.x * 4 + w;
+    if (fragment >= column_fragments) return;
+    f32x8 x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = tile[w * 16 + (lane & 15)][(lane >> 4) * 8 + i];
+    put_pieces<P>(x, to + ((long)block * column_fragments + fragment) * P * KIB, lane);
+}
+
+// ---------------------------------------------------------------- products
+struct Operand {
+    const __bf16 *at;
+    int fragments;   // of 16 rows
+};
+
+// a wavefront's KiB from memory to LDS
+MRL_DEV void bring(const __bf16 *from, __bf16 *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+// Waits until at most LOADS of the wavefront's loads are under way and none of its LDS reads, then for the workgroup.
+template <int LOADS>
+MRL_DEV void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 7 << 4);   // (vmcnt; lgkmcnt 0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// The tile of a product: A's fragments times B's, PA and PB pieces each, by 8 wavefronts, WR along A and the others along B, FA x FB fragments
+// each.  A stage is 32 of the contracted index; BUFFERS of them are in LDS or on their way.
+template <int PA_, int PB_, int WR_, int FA_, int FB_, int BUFFERS_>
+struct Shape {
+    static constexpr int PA = PA_, PB = PB_, WR = WR_, WC = 8 / WR_, FA = FA_, FB = FB_, BUFFERS = BUFFERS_;
+    static constexpr int ROWS = WR * FA, COLUMNS = WC * FB;   // fragments of the tile
+    static constexpr int STAGE = (ROWS * PA + COLUMNS * PB), LOADS = STAGE / 8;   // KiB, and those that a wavefront brings
+    static constexpr size_t LDS = sizeof(__bf16) * KIB * STAGE * BUFFERS;
+    static_assert(STAGE % 8 == 0 && LDS <= 160 * 1024, "whole loads that fit");
+};
+
+template <class S>
+MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int from, int to, __bf16 *lds, f32x4 (&acc)[S::FA][S::FB]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave / S::WC, column = wave % S::WC;
+    // which KiB of a stage this wavefront brings: A's first, then B's; a tile at the edge reads the last fragments again
+    const __bf16 *src[S::LOADS];
+    long step[S::LOADS];
+#pragma unroll
+    for (int l = 0; l < S::LOADS; ++l) {
+        const int k = wave * S::LOADS + l;
+        const bool of_a = k < S::ROWS * S::PA;
+        const int in = of_a ? k : k - S::ROWS * S::PA, pieces = of_a ? S::PA : S::PB;
+        const Operand &o = of_a ? a : b;
+        const int fragment = min((of_a ? bi * S::ROWS : bj * S::COLUMNS) + in / pieces, o.fragments - 1);
+        step[l] = (long)o.fragments * pieces * KIB;
+        src[l] = o.at + ((long)fragment * pieces + in % pieces) * KIB + from * step[l] + lane * 8;
+    }
+    const auto ask = [&](int stage) {
+        __bf16 *const base = lds + (stage % S::BUFFERS * S::STAGE + wave * S::LOADS) * KIB;
+#pragma unroll
+        for (int l = 0; l < S::LOADS; ++l) {
+            bring(src[l], base + l * KIB);
+            src[l] += step[l];
+        }
+    };
+    const int stages = to - from;
+#pragma unroll
+    for (int s = 0; s < S::BUFFERS - 1; ++s)
+        if (s < stages) ask(s);
+    for (int s = 0; s < stages; ++s) {
+        if (s + S::BUFFERS - 2 < stages) meet<(S::BUFFERS - 2) * S::LOADS>();
+        else meet<0>();
+        if (s + S::BUFFERS - 1 < stages) ask(s + S::BUFFERS - 1);   // into the buffer that everybody has left
+        const __bf16 *const base = lds + s % S::BUFFERS * S::STAGE * KIB + lane * 8;
+        const __bf16 *const pa = base + row * S::FA * S::PA * KIB, *const pb = base + (S::ROWS * S::PA + column * S::FB * S::PB) * KIB;
+        bf16x8 y[S::FB][S::PB];
+#pragma unroll
+        for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+            for (int p = 0; p < S::PB; ++p) y[j][p] = *reinterpret_cast<const bf16x8 *>(pb + (j * S::PB + p) * KIB);
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i) {
+            bf16x8 x[S::PA];
+#pragma unroll
+            for (int p = 0; p < S::PA; ++p) x[p] = *reinterpret_cast<const bf16x8 *>(pa + (i * S::PA + p) * KIB);
+            constexpr int MOST = (S::PA > S::PB ? S::PA : S::PB) - 1;   // pieces' numbers add up to this at most; the smallest products first
+#pragma unroll
+            for (int sum = MOST; sum >= 0; --sum)
+#pragma unroll
+                for (int p = 0; p <= sum; ++p)
+                    if (p < S::PA && sum - p < S::PB) {
+#pragma unroll
+                        for (int j = 0; j < S::FB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[p], y[j][sum - p], acc[i][j], 0, 0, 0);
+                    }
+        }
+    }
+}
+
+// Tiles in order, a share of neighbouring ones to each of the eight XCDs, which workgroups are dealt to in turn.
+MRL_DEV int tile_number(int tiles) {
+    const int xcd = blockIdx.x & 7, whole = tiles >> 3, rest = tiles & 7;
+    return xcd * whole + min(xcd, rest) + (blockIdx.x >> 3);
+}
+
+enum { SIGMOID = MRL_GATE_SIGMOID, SILU = MRL_GATE_SILU, GELU = MRL_GATE_GELU, TANH = MRL_GATE_TANH };
+
+MRL_DEV float activation(int act, float g) {
+    float a, rest;
+    if (act == GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
+    if (act == TANH) return tanhf(g);
+    sigmoid_pair(g, a, rest);
+    return act == SILU ? g * a : a;
+}
+// and its slope
+MRL_DEV void activation(int act, float g, float &value, float &slope) {
+    if (act == GELU) {
+        const float phi = 0.5f * (1.0f + erff(g * 0.70710678f));
+        value = g * phi;
+        slope = fmaf(g * 0.39894228f, expf(-0.5f * g * g), phi);
+    } else if (act == TANH) {
+        value = tanhf(g);
+        slope = fmaf(-value, value, 1.0f);
+    } else {
+        float a, rest;
+        sigmoid_pair(g, a, rest);
+        value = act == SILU ? g * a : a;
+        slope = act == SILU ? a * fmaf(g, rest, 1.0f) : a * rest;
+    }
+}
+
+struct Layer {
+    int M, K, N, act;
+    const void *x, *params, *grad_out;
+    long x_ld, grad_out_ld;
+    void *out, *grad_x;
+    long out_ld, grad_x_ld;
+    float *grads;
+};
+
+// FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
+// (PC pieces, for dW), and the sums of its columns over the wavefront's rows.
+template <class E, class S, bool FORWARD, int PR, int PC>
+__global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b, int row_tiles, int column_tiles, int blocks, __bf16 *rows, __bf16 *columns, float *sums) {
+    extern __shared__ __bf16 lds[];
+    const int tile = tile_number(row_tiles * column_tiles), bi = tile / column_tiles, bj = tile - bi * column_tiles;
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S>(a, b, bi, bj, 0, blocks, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
+    const E *const bias = (const E *)y.params + (long)y.K * 2 * y.N;
+    const int fragments = b.fragments;   // of gate and up
+#pragma unroll
+    for (int j = 0; j < S::FB; j += 2) {
+        const int pair = (bj * S::COLUMNS + wc * S::FB + j) / 2, column = pair * 16 + c;
+        const bool there = column < y.N;
+        if (pair * 2 >= fragments) continue;
+        const float bg = there ? value_of(bias[column]) : 0.0f, bu = there ? value_of(bias[y.N + column]) : 0.0f;
+        float gate_sum = 0.0f, up_sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i) {
+            const int fragment = bi * S::ROWS + wr * S::FA + i, row = fragment * 16 + 4 * g;
+            if (fragment >= a.fragments) continue;
+            if constexpr (FORWARD) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (there && row + r < y.M)
+                        give((E *)y.out + (row + r) * y.out_ld + column, activation(y.act, acc[i][j][r] + bg) * (acc[i][j + 1][r] + bu));
+            } else {
+                f32x4 dg, du;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool inside = there && row + r < y.M;
+                    const float grad = inside ? value_of(((const E *)y.grad_out)[(row + r) * y.grad_out_ld + column]) : 0.0f;
+                    float value, slope;
+                    activation(y.act, acc[i][j][r] + bg, value, slope);
+                    dg[r] = inside ? grad * (acc[i][j + 1][r] + bu) * slope : 0.0f;
+                    du[r] = inside ? grad * value : 0.0f;
+                    gate_sum += dg[r];
+                    up_sum += du[r];
+                }
+                // by columns: a fragment of 16 columns and 32 rows; this lane has rows 4 g .. 4 g + 3 of 16 of them, next to each other
+                const auto put = [&](const f32x4 v, int f) {
+                    bf16x4 p[SPLIT];
+                    split4(v, p);
+                    __bf16 *to = columns + ((long)(fragment >> 1) * fragments + f) * PC * KIB + (16 * ((fragment & 1) * 2 + (g >> 1)) + c) * 8 + (g & 1) * 4;
+#pragma unroll
+                    for (int k = 0; k < PC; ++k) *reinterpret_cast<bf16x4 *>(to + k * KIB) = p[k];
+                    // by rows: a fragment of 16 rows and 32 columns, 16 of the gate and 16 of up
+                    __bf16 *at = rows + ((long)(f >> 1) * a.fragments + fragment) * PR * KIB + (16 * ((f & 1) * 2 + (c >> 3)) + 4 * g) * 8 + (c & 7);
+#pragma unroll
+                    for (int k = 0; k < PR; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) at[k * KIB + r * 8] = p[k][r];
+                };
+                put(dg, 2 * pair);
+                put(du, 2 * pair + 1);
+            }
+        }
+        if constexpr (!FORWARD) {
+            gate_sum += __shfl_xor(gate_sum, 16);
+            up_sum += __shfl_xor(up_sum, 16);
+            gate_sum += __shfl_xor(gate_sum, 32);
+            up_sum += __shfl_xor(up_sum, 32);
+            if (g == 0) {
+                float *to = sums + ((long)(bi * S::WR + wr) * fragments + 2 * pair) * 16 + c;
+                to[0] = gate_sum;
+                to[16] = up_sum;
+            }
+        }
+    }
+}
+
+// dx: rows times the matrix' rows
+template <class E, class S>
+__global__ __launch_bounds__(512) void grad_x_kernel(Layer y, Operand a, Operand b, int row_tiles, int column_tiles, int blocks) {
+    extern __shared__ __bf16 lds[];
+    const int tile = tile_number(row_tiles * column_tiles), bi = tile / column_tiles, bj = tile - bi * column_tiles;
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S>(a, b, bi, bj, 0, blocks, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = (bi * S::ROWS + wr * S::FA + i) * 16 + 4 * g + r, column = (bj * S::COLUMNS + wc * S::FB + j) * 16 + c;
+                if (row < y.M && column < y.K) give((E *)y.grad_x + row * y.grad_x_ld + column, acc[i][j][r]);
+            }
+}
+
+// dW, a share of the rows per workgroup where `parts` is more than 1: [part][K, 2 N]
+template <class S>
+__global__ __launch_bounds__(512) void grad_w_kernel(int K, int N, Operand a, Operand b, int row_tiles, int column_tiles, int blocks, int parts, float *to) {
+    extern __shared__ __bf16 lds[];
+    const int tiles = row_tiles * column_tiles, number = tile_number(tiles * parts), part = number / tiles, tile = number - part * tiles;
+    const int bi = tile / column_tiles, bj = tile - bi * column_tiles;
+    const int per = (blocks + parts - 1) / parts, from = min(blocks, part * per), end = min(blocks, from + per);
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S>(a, b, bi, bj, from, end, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
+    to += (long)part * K * 2 * N;
+#pragma unroll
+    for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int fragment = bj * S::COLUMNS + wc * S::FB + j, row = (bi * S::ROWS + wr * S::FA + i) * 16 + 4 * g + r, column = (fragment >> 1) * 16 + c;
+                if (row < K && column < N) to[(long)row * 2 * N + (fragment & 1) * N + column] = acc[i][j][r];
+            }
+}
+
+// the parts of dW added up, in order, and the biases' gradients from the sums of rows of wavefronts
+__global__ __launch_bounds__(256) void finish_kernel(const float *parts, int count, long values, const float *sums, int rows, int fragments, int N, float *grads) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < values) {
+        if (count > 1) {
+            float sum = parts[i];
+            for (int p = 1; p < count; ++p) sum += parts[p * values + i];
+            grads[i] = sum;
+        }
+    } else if (i < values + 2 * N) {
+        const int column = (int)(i - values), up = column >= N, of = up ? column - N : column;
+        const float *p = sums + ((of >> 4) * 2 + up) * 16 + (of & 15);
+        float sum = 0.0f;
+        for (int r = 0; r < rows; ++r) sum += p[(long)r * fragments * 16];
+        grads[i] = sum;
+    }
+}
+
+// ---------------------------------------------------------------- few rows
+// 16 rows at a time and 16 columns of gate and up by a workgroup, whose wavefronts take shares of K: straight from memory to
+// v_mfma_f32_16x16x4_f32.  Reading the matrix is the work.
+constexpr int FEW_WAVES = 8;
+template <class E>
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(Layer y) {
+    __shared__ f32x4 sums[FEW_WAVES][2][64];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int column = blockIdx.x * 16 + c, row = blockIdx.y * 16 + c;
+    const bool there = column < y.N;
+    const E *const W = (const E *)y.params + (there ? column : 0);
+    f32x4 gate = {0.0f, 0.0f, 0.0f, 0.0f}, up = gate;
+    const int blocks = (y.K + 15) / 16;
+    for (int block = w; block < blocks; block += FEW_WAVES) {
+        const int k = block * 16 + 4 * g;
+        float x[4], wg[4], wu[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool inside = k + r < y.K;
+            const E *const from = W + (long)(inside ? k + r : 0) * 2 * y.N;
+            x[r] = inside && row < y.M ? value_of(((const E *)y.x)[row * y.x_ld + k + r]) : 0.0f;
+            wg[r] = inside ? value_of(from[0]) : 0.0f;
+            wu[r] = inside ? value_of(from[y.N]) : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            gate = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], wg[r], gate, 0, 0, 0);
+            up = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], wu[r], up, 0, 0, 0);
+        }
+    }
+    sums[w][0][lane] = gate;
+    sums[w][1][lane] = up;
+    __syncthreads();
+    if (w != 0 || !there) return;
+    for (int i = 1; i < FEW_WAVES; ++i) {
+        gate += sums[i][0][lane];
+        up += sums[i][1][lane];
+    }
+    const E *const bias = (const E *)y.params + (long)y.K * 2 * y.N;
+    const float bg = value_of(bias[column]), bu = value_of(bias[y.N + column]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int at = blockIdx.y * 16 + 4 * g + r;
+        if (at < y.M) give((E *)y.out + at * y.out_ld + column, activation(y.act, gate[r] + bg) * (up[r] + bu));
+    }
+}
+
+// no row at all: zeros
+__global__ __launch_bounds__(256) void zero_kernel(float *p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.0f;
+}
+
+// ---------------------------------------------------------------- host
+constexpr int FEW = 64;   // rows
+inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
+
+// Where things lie in the workspace, in bytes.
+struct Plan {
+    int M16, K16, N16;   // fragments of the rows, of the matrix' rows and (pairs) of its columns, an even number of the first two
+    int pieces, row_pieces, column_pieces, parts, sum_rows;
+    size_t x_rows, w_columns, x_columns, w_rows, pre_rows, pre_columns, sums, partial, bytes;
+};
+template <class S>
+int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
+
+typedef Shape<1, 1, 2, 4, 4, 4> Bf16Shape;        // 128 x 256
+typedef Shape<1, 2, 2, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
+typedef Shape<3, 3, 2, 4, 2, 3> F32Shape;         // 128 x 128
+
+Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) {
+    Plan p = {};
+    p.M16 = (int)up_to((M + 15) / 16, 2);
+    p.K16 = (int)up_to((K + 15) / 16, 2);
+    p.N16 = (N + 15) / 16;
+    const bool f32 = dtype == MRL_F32;
+    p.pieces = f32 ? 3 : 1;
+    p.row_pieces = f32 ? 3 : 1;
+    p.column_pieces = f32 ? 3 : 2;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t was = at;
+        at += up_to((long)bytes, 256);
+        return was;
+    };
+    const auto fragments = [&](long rows16, long contracted16, int pieces) { return take(sizeof(__bf16) * KIB * (size_t)rows16 * (contracted16 / 2) * pieces); };
+    if (!backward && M <= FEW) return p;
+    p.x_rows = fragments(p.M16, p.K16, p.pieces);
+    p.w_columns = fragments(2L * p.N16, p.K16, p.pieces);
+    if (backward) {
+        p.x_columns = fragments(p.K16, p.M16, p.pieces);
+        p.w_rows = fragments(p.K16, 2L * p.N16, p.pieces);
+        p.pre_rows = fragments(p.M16, 2L * p.N16, p.row_pieces);
+        p.pre_columns = fragments(2L * p.N16, p.M16, p.column_pieces);
+        const int row_tiles = f32 ? (p.M16 + F32Shape::ROWS - 1) / F32Shape::ROWS : (p.M16 + Bf16Shape::ROWS - 1) / Bf16Shape::ROWS;
+        p.sum_rows = row_tiles * (f32 ? F32Shape::WR : Bf16Shape::WR);
+        p.sums = take(sizeof(float) * (size_t)p.sum_rows * 2 * p.N16 * 16);
+        const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16GradShape>(p.K16, 2L * p.N16);
+        const int blocks = p.M16 / 2;
+        p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
+        if (p.parts > 1) p.partial = take(sizeof(float) * (size_t)p.parts * K * 2 * N);
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <class E, int P, bool PAIRED>
+void along_rows(const mrl_ctx *ctx, const Source &s, void *to, int row_fragments, int blocks) {
+    const long all = (long)row_fragments * blocks;
+    hipLaunchKernelGGL((along_rows_kernel<E, P, PAIRED>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, ctx->stream, s, (__bf16 *)to, row_fragments, blocks);
+}
+template <class E, int P, bool PAIRED>
+void along_columns(const mrl_ctx *ctx, const Source &s, void *to, int column_fragments, int blocks) {
+    hipLaunchKernelGGL((along_columns_kernel<E, P, PAIRED>), dim3((column_fragments + 3) / 4, blocks), dim3(256), 0, ctx->stream, s, (__bf16 *)to, column_fragments);
+}
+
+template <class E, class S, class SW, int P, int PR, int PC>
+void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool backward) {
+    const Source x = {y.x, y.x_ld, y.M, y.K}, w = {y.params, 2L * y.N, y.K, y.N};
+    const Operand x_rows = {(const __bf16 *)(ws + p.x_rows), p.M16}, w_columns = {(const __bf16 *)(ws + p.w_columns), 2 * p.N16};
+    along_rows<E, P, false>(ctx, x, ws + p.x_rows, p.M16, p.K16 / 2);
+    along_columns<E, P, true>(ctx, w, ws + p.w_columns, 2 * p.N16, p.K16 / 2);
+    const auto grid = [](long a, long b) { return (a + S::ROWS - 1) / S::ROWS * ((b + S::COLUMNS - 1) / S::COLUMNS); };
+    const int row_tiles = (p.M16 + S::ROWS - 1) / S::ROWS, column_tiles = (2 * p.N16 + S::COLUMNS - 1) / S::COLUMNS;
+    const dim3 pre((unsigned)grid(p.M16, 2L * p.N16));
+    if (!backward) {
+        hipLaunchKernelGGL((pre_kernel<E, S, true, PR, PC>), pre, dim3(512), S::LDS, ctx->stream, y, x_rows, w_columns, row_tiles, column_tiles, p.K16 / 2, nullptr, nullptr, nullptr);
+        return;
+    }
+    along_columns<E, P, false>(ctx, x, ws + p.x_columns, p.K16, p.M16 / 2);
+    along_rows<E, P, true>(ctx, w, ws + p.w_rows, p.K16, p.N16);
+    hipLaunchKernelGGL((pre_kernel<E, S, false, PR, PC>), pre, dim3(512), S::LDS, ctx->stream, y, x_rows, w_columns, row_tiles, column_tiles, p.K16 / 2,
+                       (__bf16 *)(ws + p.pre_rows), (__bf16 *)(ws + p.pre_columns), (float *)(ws + p.sums));
+    const Operand pre_rows = {(const __bf16 *)(ws + p.pre_rows), p.M16}, pre_columns = {(const __bf16 *)(ws + p.pre_columns), 2 * p.N16};
+    const Operand x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
+    if (y.grad_x != nullptr) {
+        const int across = (p.K16 + S::COLUMNS - 1) / S::COLUMNS;
+        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3((unsigned)grid(p.M16, p.K16)), dim3(512), S::LDS, ctx->stream, y, pre_rows, w_rows, row_tiles, across, p.N16);
+    }
+    const int down = (p.K16 + SW::ROWS - 1) / SW::ROWS, across = (2 * p.N16 + SW::COLUMNS - 1) / SW::COLUMNS;
+    const long values = (long)y.K * 2 * y.N;
+    float *const to = p.parts > 1 ? (float *)(ws + p.partial) : y.grads;
+    hipLaunchKernelGGL((grad_w_kernel<SW>), dim3((unsigned)(down * across * p.parts)), dim3(512), SW::LDS, ctx->stream, y.K, y.N, x_columns, pre_columns, down, across, p.M16 / 2, p.parts, to);
+    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)((values + 2 * y.N + 255) / 256)), dim3(256), 0, ctx->stream, to, p.parts, values, (const float *)(ws + p.sums), p.sum_rows,
+                       2 * p.N16, y.N, y.grads);
+}
+
+int check_sizes(const char *who, int dtype, int act, int64_t rows, int in_dim, int out_dim) {
+    MRL_CHECK_ARG(dtype == MRL_F32 || dtype == MRL_BF16, "%s: unknown element type %d", who, dtype);
+    MRL_CHECK_ARG(act >= MRL_GATE_SIGMOID && act <= MRL_GATE_TANH, "%s: unknown activation %d", who, act);
+    MRL_CHECK_ARG(rows >= 0 && rows < 1 << 26, "%s: %lld rows: 0 to 2^26 - 1 expected", who, (long long)rows);
+    MRL_CHECK_ARG(in_dim >= 1 && in_dim <= 1 << 16 && out_dim >= 1 && out_dim <= 1 << 16, "%s: dims %d and %d: 1 to 65536 expected", who, in_dim, out_dim);
+    return MRL_OK;
+}
+int check_workspace(const char *who, size_t need, void *workspace, uint64_t bytes) {
+    MRL_CHECK_ARG(bytes >= need && (need == 0 || workspace != nullptr), "%s: the workspace holds %llu bytes, need %llu", who,
+                  (unsigned long long)(workspace ? bytes : 0), (unsigned long long)need);
+    MRL_CHECK_ARG(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", who);
+    return MRL_OK;
+}
+
+}  // namespace
+}  // namespace glu
+}  // namespace mrl
+
+extern "C" {
+
+int mrl_gated_linear_workspace(mrl_ctx *ctx, int dtype, int rows, int in_dim, int out_dim, int backward, uint64_t *bytes) {
+    using namespace mrl;
+    MRL_CHECK_ARG(ctx && bytes, "mrl_gated_linear_workspace: NULL ctx or result");
+    const int rc = glu::check_sizes("mrl_gated_linear_workspace", dtype, MRL_GATE_SIGMOID, rows, in_dim, out_dim);
+    if (rc != MRL_OK) return rc;
+    *bytes = rows == 0 ? 0 : glu::plan_of(ctx, dtype, rows, in_dim, out_dim, backward != 0).bytes;
+    return MRL_OK;
+}
+
+int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_dim, int out_dim, const void *in, int64_t in_ld, const void *params,
+                             void *out, int64_t out_ld, void *workspace, uint64_t workspace_bytes) {
+    using namespace mrl;
+    using namespace mrl::glu;
+    const char *who = "mrl_gated_linear_forward";
+    MRL_CHECK_ARG(ctx, "%s: ctx is NULL", who);
+    int rc = check_sizes(who, dtype, act, rows, in_dim, out_dim);
+    if (rc != MRL_OK || rows == 0) return rc;
+    MRL_CHECK_ARG(in && params && out, "%s: NULL buffer", who);
+    MRL_CHECK_ARG(in_ld >= in_dim && out_ld >= out_dim, "%s: a row stride is smaller than the row", who);
+    const Plan p = plan_of(ctx, dtype, rows, in_dim, out_dim, false);
+    rc = check_workspace(who, p.bytes, workspace, workspace_bytes);
+    if (rc != MRL_OK) return rc;
+    const int64_t size = dtype == MRL_F32 ? 4 : 2;
+    rc = check_apart(who, {Region("out", out, rows, size * out_dim, size * out_ld), Region("the workspace", p.bytes ? workspace : nullptr, (int64_t)p.bytes)},
+                     {Region("in", in, rows, size * in_dim, size * in_ld), Region("params", params, size * 2 * out_dim * ((int64_t)in_dim + 1))});
+    if (rc != MRL_OK) return rc;
+    OnDevice on(ctx);
+    Layer y = {};
+    y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
+    y.x = in; y.x_ld = in_ld; y.params = params; y.out = out; y.out_ld = out_ld;
+    if (rows <= FEW) {
+        const dim3 grid((out_dim + 15) / 16, (rows + 15) / 16);
+        if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
+        else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
+    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
+    else launch<bf16_t, Bf16Shape, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, false);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+
+int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in_dim, int out_dim, const void *grad_out, int64_t grad_out_ld, const void *in,
+                              int64_t in_ld, const void *params, void *grad_in, int64_t grad_in_ld, float *grads, void *workspace, uint64_t workspace_bytes) {
+    using namespace mrl;
+    using namespace mrl::glu;
+    const char *who = "mrl_gated_linear_backward";
+    MRL_CHECK_ARG(ctx, "%s: ctx is NULL", who);
+    int rc = check_sizes(who, dtype, act, rows, in_dim, out_dim);
+    if (rc != MRL_OK) return rc;
+    MRL_CHECK_ARG(grads, "%s: NULL gradients", who);
+    const int64_t values = 2LL * out_dim * (in_dim + 1), size = dtype == MRL_F32 ? 4 : 2;
+    OnDevice on(ctx);
+    if (rows == 0) {
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::min<int64_t>((values + 255) / 256, 4096)), dim3(256), 0, ctx->stream, grads, (long)values);
+        MRL_CHECK_LAUNCH();
+        return MRL_OK;
+    }
+    MRL_CHECK_ARG(grad_out && in && params, "%s: NULL buffer", who);
+    MRL_CHECK_ARG(in_ld >= in_dim && grad_out_ld >= out_dim && (!grad_in || grad_in_ld >= in_dim), "%s: a row stride is smaller than the row", who);
+    const Plan p = plan_of(ctx, dtype, rows, in_dim, out_dim, true);
+    rc = check_workspace(who, p.bytes, workspace, workspace_bytes);
+    if (rc != MRL_OK) return rc;
+    rc = check_apart(who, {Region("grad_in", grad_in, rows, size * in_dim, size * grad_in_ld), Region("grads", grads, 4 * values), Region("the workspace", workspace, (int64_t)p.bytes)},
+                     {Region("in", in, rows, size * in_dim, size * in_ld), Region("params", params, size * values), Region("grad_out", grad_out, rows, size * out_dim, size * grad_out_ld)});
+    if (rc != MRL_OK) return rc;
+    Layer y = {};
+    y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
+    y.x = in; y.x_ld = in_ld; y.params = params; y.grad_out = grad_out; y.grad_out_ld = grad_out_ld;
+    y.grad_x = grad_in; y.grad_x_ld = grad_in_ld; y.grads = grads;
+    if (dtype == MRL_F32) launch<float, F32Shape, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
+    else launch<bf16_t, Bf16Shape, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,178 @@
+"""GatedLinear against its formulas and their gradients in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+UNIT = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = {"f32": UNIT, "bf16": 2.0 ** -8}
+# Roundings of a sum of n products at its full size: six additions to the sum for every 32 products (one in bf16), those of up to 64 partial sums
+# and of the bias, and 2 units of each product, for the pieces left out.
+ROUNDINGS = lambda n: (6 * n / 32 + 72) * UNIT   # noqa: E731
+ACTIVATIONS = ("sigmoid", "silu", "gelu", "tanh")
+
+
+@pytest.fixture(scope="module")
+def ctx(mrl):
+    return mrl.DeviceContext("cuda:0")
+
+
+def act64(act, g):
+    s = torch.sigmoid(g)
+    return {"sigmoid": s, "silu": g * s, "gelu": 0.5 * g * (1 + torch.erf(g / math.sqrt(2))), "tanh": torch.tanh(g)}[act]
+
+
+class Case:
+    def __init__(self, M, K, N, act, dtype, seed=0, wide=False):
+        gen = torch.Generator().manual_seed(seed + 7 * M + 5 * K + N)
+        self.M, self.K, self.N, self.act, self.dtype, self.tt = M, K, N, act, dtype, TYPES[dtype]
+        x = torch.randn(M, K, generator=gen).to(self.tt)
+        params = torch.cat((torch.randn(K * 2 * N, generator=gen) / math.sqrt(K), torch.randn(2 * N, generator=gen) * 0.2)).to(self.tt)
+        grad = torch.randn(M, N, generator=gen).to(self.tt)
+        if wide:     # rows farther apart than they are long, at odd places
+            room = torch.zeros(M, K + N + 5, dtype=self.tt)
+            room[:, 1:1 + K], room[:, K + 3:K + 3 + N] = x, grad
+            room = room.cuda()
+            self.x, self.grad = room[:, 1:1 + K], room[:, K + 3:K + 3 + N]
+        else:
+            self.x, self.grad = x.cuda(), grad.cuda()
+        self.params = params.cuda()
+
+    def parts64(self):
+        x, p, grad = self.x.cpu().double(), self.params.cpu().double(), self.grad.cpu().double()
+        K, N = self.K, self.N
+        w = p[:K * 2 * N].view(K, 2 * N)
+        pre = x @ w + p[K * 2 * N:]
+        off = ROUNDINGS(K) * (x.abs() @ w.abs() + p[K * 2 * N:].abs())
+        return x, w, grad, pre, off
+
+    def forward64(self):
+        """outputs and what they may be off by: activations' slopes are at most 1.13; their values take some ten roundings"""
+        x, w, grad, pre, off = self.parts64()
+        g, u, og, ou = pre[:, :self.N], pre[:, self.N:], off[:, :self.N], off[:, self.N:]
+        a = act64(self.act, g)
+        return a * u, 1.13 * og * (u.abs() + ou) + (a.abs() + 16 * UNIT * (1 + g.abs())) * ou + 16 * UNIT * (a.abs() + UNIT) * u.abs() + HALF[self.dtype] * (a * u).abs() + 1e-37
+
+    def backward64(self):
+        """(grad_x, what it may be off by), (grads, ...): the slopes' slopes are at most 1; a slope takes some twenty roundings of terms up to
+        1 + |g|.  In bf16 [dgate | dup] is rounded for grad_x, half a step, and taken as two pieces, 2^-17, for the parameters."""
+        x, w, grad, pre, off = self.parts64()
+        N = self.N
+        g = pre[:, :N].clone().requires_grad_()
+        a = act64(self.act, g)
+        slope, = torch.autograd.grad(a.sum(), g)
+        g, a = g.detach(), a.detach()
+        u, og, ou = pre[:, N:], off[:, :N], off[:, N:]
+        d = torch.cat((grad * u * slope, grad * a), 1)
+        few = 24 * UNIT * (1 + g.abs().clamp(max=8))
+        od = torch.cat((grad.abs() * (ou * (slope.abs() + few) + u.abs() * (og + few)), grad.abs() * (1.13 * og + few)), 1)
+        piece, pieces = (2.0 ** -8, 2.0 ** -17) if self.dtype == "bf16" else (0.0, 0.0)
+        gx, ox = d @ w.T, (od + (piece + ROUNDINGS(2 * N)) * d.abs()) @ w.abs().T
+        gw, ow = x.T @ d, x.abs().T @ (od + (pieces + ROUNDINGS(self.M)) * d.abs())
+        gb, ob = d.sum(0), (od + ROUNDINGS(32 * self.M) * d.abs()).sum(0)
+        return (gx, ox + HALF[self.dtype] * gx.abs() + 1e-37), (torch.cat((gw.reshape(-1), gb)), torch.cat((ow.reshape(-1), ob)) + 1e-37)
+
+    def layer(self, mrl):
+        return mrl.GatedLinear(self.K, self.N, self.act)
+
+    def forward(self, mrl, ctx):
+        out = torch.full((self.M, self.N), 7.0, dtype=self.tt, device="cuda")
+        self.layer(mrl).forward_gpu(ctx, out, self.x, self.params)
+        return out
+
+    def backward(self, mrl, ctx, grad_x=True):
+        gx = torch.full((self.M, self.K), 7.0, dtype=self.tt, device="cuda") if grad_x else None
+        grads = torch.full((2 * self.N * (self.K + 1),), 7.0, device="cuda")
+        self.layer(mrl).backward_gpu(ctx, gx, grads, self.grad, self.x, self.params)
+        return gx, grads
+
+
+def near(got, want, off, what):
+    beyond = (got.cpu().double().reshape(want.shape) - want).abs() - off
+    assert beyond.max().item() <= 0, "%s: %g beyond its bound at %d of %s" % (what, beyond.max().item(), beyond.argmax().item(), list(want.shape))
+
+
+# rows below, at and one past a fragment, a tile and what goes straight to registers; odd dims, dims of one, columns past a tile
+SHAPES = [(1, 1, 1), (1, 256, 1024), (16, 64, 48), (17, 33, 31), (64, 100, 20), (65, 32, 16), (66, 7, 5), (127, 96, 130), (128, 64, 128), (129, 65, 129), (300, 256, 7),
+          (257, 40, 300), (1000, 128, 64), (513, 520, 272), (2050, 72, 36)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_forward_and_backward(mrl, ctx, M, K, N, dtype):
+    act = ACTIVATIONS[(M + K + N) % 4]
+    print("gated linear", M, K, N, act, dtype, flush=True)
+    c = Case(M, K, N, act, dtype, wide=M % 2 == 1)
+    out = c.forward(mrl, ctx)
+    ctx.synchronize()
+    near(out, *c.forward64(), "out")
+    gx, grads = c.backward(mrl, ctx)
+    ctx.synchronize()
+    for got, (want, off), what in zip((gx, grads), c.backward64(), ("grad_x", "grads")):
+        near(got, want, off, what)
+    again = c.backward(mrl, ctx)
+    _, alone = c.backward(mrl, ctx, grad_x=False)
+    ctx.synchronize()
+    assert torch.equal(gx, again[0]) and torch.equal(grads, again[1]) and torch.equal(grads, alone)
+
+
+@pytest.mark.parametrize("act", ACTIVATIONS)
+@pytest.mark.parametrize("M", [30, 200])
+def test_activations(mrl, ctx, act, M):
+    c = Case(M, 48, 40, act, "f32", seed=3)
+    c.params[:48 * 80] *= 6      # gates out to where the activations are flat
+    out = c.forward(mrl, ctx)
+    gx, grads = c.backward(mrl, ctx)
+    ctx.synchronize()
+    near(out, *c.forward64(), "out")
+    for got, (want, off), what in zip((gx, grads), c.backward64(), ("grad_x", "grads")):
+        near(got, want, off, what)
+
+
+def test_gradient_against_differences(mrl, ctx):
+    """a step h along a direction changes the weighted outputs by h times the gradient along it, to h^2 and the outputs' roundings"""
+    c = Case(70, 40, 24, "silu", "f32", seed=5)
+    gx, grads = c.backward(mrl, ctx)
+    gen = torch.Generator().manual_seed(1)
+    h = 2.0 ** -6
+    weight = c.grad.double()
+    for name, grad in (("x", gx), ("params", grads)):
+        direction = torch.randn(getattr(c, name).shape, generator=gen).cuda()
+        here = getattr(c, name)
+        sums = []
+        for sign in (1, -1):
+            setattr(c, name, here + sign * h * direction)
+            sums.append((c.forward(mrl, ctx).double() * weight).sum())
+        setattr(c, name, here)
+        want = (grad.double() * direction.double()).sum().item()
+        got = ((sums[0] - sums[1]) / (2 * h)).item()
+        # third derivatives are of the order of the sum of |weight| times cubes of the directions' products, here below 2^8 of the gradient's norm
+        norm = (grad.double().norm() * direction.double().norm()).item()
+        assert abs(got - want) <= 2.0 ** 8 * h * h / 6 * norm / math.sqrt(direction.numel()) + 1e-3 * norm / math.sqrt(direction.numel())
+
+
+def test_empty_and_refused(mrl, ctx):
+    layer = mrl.GatedLinear(8, 4)
+    x, out, params, grads = torch.zeros(0, 8, device="cuda"), torch.zeros(0, 4, device="cuda"), torch.zeros(layer.PARAM_SIZE, device="cuda"), torch.ones(layer.PARAM_SIZE, device="cuda")
+    layer.forward_gpu(ctx, out, x, params)
+    layer.backward_gpu(ctx, None, grads, out, x, params)
+    ctx.synchronize()
+    assert (grads == 0).all()
+    x, out = torch.zeros(100, 8, device="cuda"), torch.zeros(100, 4, device="cuda")
+    with pytest.raises(mrl.MrlError, match="overlap"):
+        layer.forward_gpu(ctx, x[:, :4], x, params)
+    with pytest.raises(mrl.MrlError, match="overlap"):
+        layer.backward_gpu(ctx, x, grads, out, x, params)
+    with pytest.raises(mrl.MrlError, match="overlap"):
+        layer.backward_gpu(ctx, None, params, out, x, params)
+    call, ptr = mrl._lib.call, lambda t: t.data_ptr()   # noqa: E731
+    for args, text in (((0, 0, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "workspace"), ((0, 0, 100, 8, 4, ptr(x), 7, ptr(params), ptr(out), 4, None, 0), "stride"),
+                       ((0, 9, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "activation"), ((7, 0, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "type"),
+                       ((0, 0, 100, 0, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "dims"), ((0, 0, -1, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "rows"),
+                       ((0, 0, 100, 8, 4, None, 8, ptr(params), ptr(out), 4, None, 0), "NULL")):
+        with pytest.raises(mrl.MrlError, match=text):
+            call("mrl_gated_linear_forward", ctx.handle, *args)
