@@ -97,6 +97,14 @@ MRL_DEV bool is_cut(const Delta &d, int t, int n) {
     return row != nullptr && (t > 0 ? row[(long)(t - 1) * d.N + n] : row[n]) > 0.5f;
 }
 
+// What is worked out from these is worked out here and not ahead of the loop around: kept there, the addresses and comparisons of all of a
+// block's phases take more registers than the state.
+MRL_DEV void anew(int &x) { asm volatile("" : "+v"(x)); }
+MRL_DEV void anew(int &x, int &y) {
+    anew(x);
+    anew(y);
+}
+
 MRL_DEV f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // c + A B over 16 values of the contracted index
 MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
@@ -160,23 +168,40 @@ MRL_DEV f32x4 between(const float *a, int g, int n) {
     return out;
 }
 
-// column n of (1 + A)^-1, A [16][SIDE] strictly lower triangular: forward substitution, which is as exact as its terms allow
-// where powers of A would grow (keys that are alike)
-MRL_DEV void invert(const float *A, int n, float (&x)[TILE]) {
-#pragma unroll
-    for (int i = 0; i < TILE; ++i) {
-        float sum = i == n ? 1.0f : 0.0f;
-#pragma unroll
-        for (int p = 0; p < (i + 3) / 4; ++p) {
-            const f32x4 row = *reinterpret_cast<const f32x4 *>(A + i * SIDE + 4 * p);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (4 * p + r < i) sum = fmaf(-row[r], x[4 * p + r], sum);
-        }
-        x[i] = sum;
-    }
+// the sum over the four lane groups, in all of them
+MRL_DEV float sum_groups(float x) {
+    const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(half[0]) + __uint_as_float(half[1]);
+    const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(row[0]) + __uint_as_float(row[1]);
 }
 
+// Rows 4 g + r of column n of (1 + A)^-1, A [16][SIDE] strictly lower triangular: forward substitution, which is as exact as its terms allow
+// where powers of A would grow (keys that are alike).  Four rows at a time: a lane group adds up what its own rows contribute, and all
+// solve the four rows' triangle.
+MRL_DEV f32x4 invert(const float *A, int g, int n) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        f32x4 own[4];
+        float sum[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float *row = A + (4 * p + r) * SIDE;
+            own[r] = *reinterpret_cast<const f32x4 *>(row + 4 * p);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(row + 4 * g);   // (x is 0 for rows not solved yet)
+            if (p > 0) sum[r] = sum_groups(fmaf(v[0], x[0], fmaf(v[1], x[1], fmaf(v[2], x[2], v[3] * x[3]))));
+            sum[r] = (4 * p + r == n ? 1.0f : 0.0f) - (p > 0 ? sum[r] : 0.0f);
+        }
+#pragma unroll
+        for (int r = 1; r < 4; ++r)
+#pragma unroll
+            for (int k = 0; k < r; ++k) sum[r] = fmaf(-own[r][k], sum[k], sum[r]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = g == p ? sum[r] : x[r];
+    }
+    return x;
+}
 
 // What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.
 template <int DK>
@@ -201,20 +226,34 @@ struct Block {
     MRL_DEV f32x4 four(const float *scalars, int tile, int g) const { return *reinterpret_cast<const f32x4 *>(scalars + tile * TILE + 4 * g); }
 
     // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
-    // Whether a value is too large for products with 0, or none.
+    // Whether a value is too large for products with 0, or none.  Loads read a row that is there in place of one that is not, so that
+    // they stand together without a branch among them.
     template <class E, bool QUERIES>
-    MRL_DEV bool load(const Delta &d, int n, int h, int hk) {
+    MRL_DEV bool load(const Delta &d, int n, int h, int hk, int thread) {
         bool odd = false;
-        const int part = (threadIdx.x & 63) % LANES;
-        for (int slot = (int)threadIdx.x / LANES; slot < STEPS; slot += (int)blockDim.x / LANES) {
-            const bool here = there(d, slot);
-            const long row = (long)time_of(slot) * d.N + n;
-            const int count = here ? d.dk - 4 * part : 0;
-            const f32x4 k = load4((const E *)d.key + (here ? row * d.key_ld + hk * d.dk + 4 * part : 0), count);
+        const int part = (thread & 63) % LANES, count = d.dk - 4 * part, first = count > 0 ? 4 * part : 0;
+        const E *const keys = (const E *)d.key + n * d.key_ld + (long)hk * d.dk + first, *const queries = (const E *)d.query + n * d.query_ld + (long)hk * d.dk + first;
+        const long key_step = (long)d.N * d.key_ld, query_step = (long)d.N * d.query_ld;
+        const bool whole = (d.dk & 3) == 0;
+        for (int slot = thread / LANES; slot < STEPS; slot += (int)blockDim.x / LANES) {
+            const bool here = there(d, slot) && count > 0;
+            const long t = min(time_of(slot), d.T - 1);
+            f32x4 k, q = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (whole) {
+                k = load4(keys + t * key_step, 4);
+                if (QUERIES) q = load4(queries + t * query_step, 4);
+            } else {
+                k = load4(keys + t * key_step, count);
+                if (QUERIES) q = load4(queries + t * query_step, count);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                k[i] = here ? k[i] : 0.0f;
+                q[i] = here ? q[i] : 0.0f;
+            }
             *reinterpret_cast<f32x4 *>(K + slot * ROW + 4 * part) = k;
             float kk = fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))), qq = 0.0f;
             if (QUERIES) {
-                const f32x4 q = load4((const E *)d.query + (here ? row * d.query_ld + hk * d.dk + 4 * part : 0), count);
                 *reinterpret_cast<f32x4 *>(Q + slot * ROW + 4 * part) = q;
                 qq = fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3])));
             }
@@ -229,7 +268,7 @@ struct Block {
                 qscale[slot] = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
             }
         }
-        for (int slot = threadIdx.x; slot < STEPS; slot += blockDim.x) {
+        for (int slot = thread; slot < STEPS; slot += blockDim.x) {
             float a = 1.0f, rest = 0.0f, b = 0.0f, other = 0.0f;
             if (there(d, slot)) {
                 const int t = time_of(slot);
@@ -268,26 +307,28 @@ struct Block {
             if (QUERIES) P[i * SIDE + c] = i >= c ? qs[r] * (kc * qk[r]) * decay[r] : 0.0f;
         }
         __builtin_amdgcn_wave_barrier();
-        float x[TILE];
-        invert(T, c, x);
+        const f32x4 x = invert(T, g, c);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int r = 0; r < TILE; ++r)
-            if (g == (r >> 2)) T[r * SIDE + c] = x[r];
+        for (int r = 0; r < 4; ++r) T[(4 * g + r) * SIDE + c] = x[r];
     }
     MRL_DEV bool cut_ahead(int tile) const { return span == 1 && as[tile * TILE] == 0.0f; }   // hides whatever the state holds
 };
 
-// A value tile as a result's registers: row 4 g + r, column c
+// A value tile as a result's registers: row 4 g + r, column c.  `rows` points at the column (at one that is there) of the environment's row of
+// step 0, `step` elements from a step to the next.
 template <class E, int DK>
-MRL_DEV bool load_values(const Delta &d, const Block<DK> &block, const void *rows, long ld, int n, int at, bool live, int g, f32x4 (&V)[Block<DK>::TILES]) {
+MRL_DEV bool load_values(const Delta &d, const Block<DK> &block, const E *rows, long step, bool live, int g, f32x4 (&V)[Block<DK>::TILES]) {
     bool odd = false;
 #pragma unroll
     for (int tile = 0; tile < Block<DK>::TILES; ++tile)
 #pragma unroll
+        for (int r = 0; r < 4; ++r) V[tile][r] = value_of(rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step]);
+#pragma unroll
+    for (int tile = 0; tile < Block<DK>::TILES; ++tile)
+#pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int slot = tile * TILE + 4 * g + r;
-            V[tile][r] = live && block.there(d, slot) ? value_of(((const E *)rows)[((long)block.time_of(slot) * d.N + n) * ld + at]) : 0.0f;
+            V[tile][r] = live && block.there(d, tile * TILE + 4 * g + r) ? V[tile][r] : 0.0f;
             odd |= !(fabsf(V[tile][r]) < LARGE);
         }
     return odd;

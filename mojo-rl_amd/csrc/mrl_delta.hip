@@ -86,11 +86,12 @@ constexpr int MOST_WAVES = 4;
 // all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.  STATES: no outputs, the
 // state ahead of every block instead.
 template <class E, int DK, bool STATES>
-__global__ __launch_bounds__(64 * MOST_WAVES) void tiles_kernel(Delta d, int column_groups, float *states, int blocks) {
+__global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kernel(Delta d, int column_groups, float *states, int blocks) {
     extern __shared__ float lds[];
     constexpr int B = DK / TILE, TILES = Block<DK>::TILES, STEPS = Block<DK>::STEPS, ROW = Block<DK>::ROW;
     Block<DK> block(lds);
-    const int W = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int group = blockIdx.x % column_groups, nh = blockIdx.x / column_groups, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
     const int column_tile = group * W + w, column = column_tile * TILE + c;
     const bool live = column < d.dv;
@@ -105,6 +106,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void tiles_kernel(Delta d, int col
             S[i][r] = d.state_in != nullptr && live && row < d.dk ? d.state_in[state_at + (long)row * d.dv] : 0.0f;
         }
 
+    const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
     block.span = TILE;
     int begin = 0;   // of the block
     for (block.t0 = 0; block.t0 < d.T;) {
@@ -118,18 +120,22 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void tiles_kernel(Delta d, int col
             if (number == blocks - 1) return;
         }
         f32x4 V[TILES];
+        anew(g, c);
+        anew(thread);
         bool odd = is_odd(S);
-        odd |= load_values<E, DK>(d, block, d.value, d.value_ld, n, h * d.dv + column, live, g, V);
-        odd |= block.template load<E, !STATES>(d, n, h, hk);
+        odd |= load_values<E, DK>(d, block, values, (long)d.N * d.value_ld, live, g, V);
+        odd |= block.template load<E, !STATES>(d, n, h, hk, thread);
         if (__syncthreads_or(odd) && block.span == TILE) {
             block.span = 1;
             continue;   // the same block again, one step to a tile
         }
+        anew(g, c);
         for (int tile = w; tile < TILES; tile += W) block.template prepare<!STATES>(tile, g, c);
         __syncthreads();
 #pragma unroll 1
         for (int tile = 0; tile < TILES; ++tile) {
             if (block.t0 + tile * block.span >= d.T) break;
+            anew(g, c);
             Decays decay;
             decay.load(block.as + tile * TILE, g);
             if (block.cut_ahead(tile)) {

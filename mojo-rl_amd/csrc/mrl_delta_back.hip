@@ -47,11 +47,6 @@ MRL_DEV float sum16(float x) {   // over the 16 lanes of a group
     for (int s = 1; s < 16; s *= 2) x += __shfl_xor(x, s);
     return x;
 }
-MRL_DEV float sum_groups(float x) {   // over the four groups
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
 // EK: the type of the gradients of query and key (float where a group's are summed later)
 template <class E, class EK, int DK>
 __global__ __launch_bounds__(64 * MOST_WAVES) void back_kernel(Back p) {
@@ -117,10 +112,12 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void back_kernel(Back p) {
             if (!decltype(keep)::value || tile + 1 < TILES) go_on(block, decay, tile, g, c, u, S);
         }
     };
+    const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
+    const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
     const auto load = [&]() {
-        bool odd = load_values<E, DK>(d, block, d.value, d.value_ld, n, h * d.dv + column, live, g, V);
-        odd |= load_values<E, DK>(d, block, p.grad_out, p.grad_out_ld, n, h * d.dv + column, live, g, dO);
-        odd |= block.template load<E, true>(d, n, h, hk);
+        bool odd = load_values<E, DK>(d, block, values, (long)d.N * d.value_ld, live, g, V);
+        odd |= load_values<E, DK>(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
+        odd |= block.template load<E, true>(d, n, h, hk, threadIdx.x);
         return odd;
     };
 
