@@ -113,9 +113,11 @@ MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
     return c;
 }
 
-constexpr int tiles_of(int DK) { return DK == 128 ? 2 : 4; }   // tiles that a workgroup prepares together: a block
+// Tiles that a workgroup prepares together, a block: as many as leave a CU's LDS room for two workgroups and more.
+constexpr int tiles_forward(int DK) { return DK == 128 ? 2 : 4; }
+constexpr int tiles_backward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int SIDE = TILE + 4;        // floats from a row of a 16 x 16 matrix in LDS to the next
-constexpr size_t rows_floats(int DK) { return 2 * TILE * tiles_of(DK) * (DK + 4) + 2 * tiles_of(DK) * TILE * SIDE + 6 * TILE * tiles_of(DK); }
+constexpr size_t rows_floats(int DK, int tiles) { return 2 * TILE * tiles * (DK + 4) + 3 * tiles * TILE * SIDE + 6 * TILE * tiles; }
 
 // The decays of a tile, from its 16 a in LDS.  Lane 16 g + n holds rows i = 4 g + r of column n.
 struct Decays {
@@ -204,15 +206,16 @@ MRL_DEV f32x4 invert(const float *A, int g, int n) {
 }
 
 // What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.
-template <int DK>
+template <int DK, int TILES_>
 struct Block {
-    static constexpr int TILES = tiles_of(DK), STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
-    float *K, *Q, *Ts, *Ps, *as, *rests, *bs, *rate_rests, *kscale, *qscale;   // rests: 1 - a, 0 at a cut; rate_rests: 1 - b
+    static constexpr int TILES = TILES_, STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
+    float *K, *Q, *As, *Ts, *Ps, *as, *rests, *bs, *rate_rests, *kscale, *qscale;   // rests: 1 - a, 0 at a cut; rate_rests: 1 - b
     int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
     MRL_DEV explicit Block(float *lds) {
         K = lds;
         Q = K + STEPS * ROW;
-        Ts = Q + STEPS * ROW;
+        As = Q + STEPS * ROW;
+        Ts = As + TILES * TILE * SIDE;
         Ps = Ts + TILES * TILE * SIDE;
         as = Ps + TILES * TILE * SIDE;
         rests = as + STEPS;
@@ -299,16 +302,15 @@ struct Block {
         }
         const f32x4 decay = between(as + tile * TILE, g, c), b = four(bs, tile, g), ks = four(kscale, tile, g), qs = four(qscale, tile, g);
         const float kc = kscale[tile * TILE + c];
-        float *T = Ts + tile * TILE * SIDE, *P = Ps + tile * TILE * SIDE;
+        float *A = As + tile * TILE * SIDE, *T = Ts + tile * TILE * SIDE, *P = Ps + tile * TILE * SIDE;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = 4 * g + r;
-            T[i * SIDE + c] = i > c ? b[r] * ks[r] * (kc * kk[r]) * decay[r] : 0.0f;
+            A[i * SIDE + c] = i > c ? b[r] * ks[r] * (kc * kk[r]) * decay[r] : 0.0f;
             if (QUERIES) P[i * SIDE + c] = i >= c ? qs[r] * (kc * qk[r]) * decay[r] : 0.0f;
         }
         __builtin_amdgcn_wave_barrier();
-        const f32x4 x = invert(T, g, c);
-        __builtin_amdgcn_wave_barrier();
+        const f32x4 x = invert(A, g, c);
 #pragma unroll
         for (int r = 0; r < 4; ++r) T[(4 * g + r) * SIDE + c] = x[r];
     }
@@ -317,15 +319,15 @@ struct Block {
 
 // A value tile as a result's registers: row 4 g + r, column c.  `rows` points at the column (at one that is there) of the environment's row of
 // step 0, `step` elements from a step to the next.
-template <class E, int DK>
-MRL_DEV bool load_values(const Delta &d, const Block<DK> &block, const E *rows, long step, bool live, int g, f32x4 (&V)[Block<DK>::TILES]) {
+template <class E, class B, int TILES>
+MRL_DEV bool load_values(const Delta &d, const B &block, const E *rows, long step, bool live, int g, f32x4 (&V)[TILES]) {
     bool odd = false;
 #pragma unroll
-    for (int tile = 0; tile < Block<DK>::TILES; ++tile)
+    for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
         for (int r = 0; r < 4; ++r) V[tile][r] = value_of(rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step]);
 #pragma unroll
-    for (int tile = 0; tile < Block<DK>::TILES; ++tile)
+    for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             V[tile][r] = live && block.there(d, tile * TILE + 4 * g + r) ? V[tile][r] : 0.0f;
@@ -343,37 +345,96 @@ MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
     return odd;
 }
 
-// U[4 g + r][c] of a tile from S0^T k (sk), and S0 <- S1
-template <int DK>
-MRL_DEV f32x4 solve(const Block<DK> &block, const Decays &decay, int tile, int g, int c, const f32x4 v, const f32x4 sk) {
-    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g);
-    f32x4 x;
+// S^T k of a tile's 16 keys (or queries), unscaled: [row of the tile][column of S]
+template <int DK, int TILES>
+MRL_DEV f32x4 ask(const Block<DK, TILES> &block, const float *rows, int tile, int g, int c, const f32x4 (&S)[DK / TILE]) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = b[r] * fmaf(-decay.from[r] * ks[r], sk[r], v[r]);
-    const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
-    return mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    for (int i = 0; i < DK / TILE; ++i) x = mfma16(*reinterpret_cast<const f32x4 *>(rows + (tile * TILE + c) * block.ROW + i * TILE + 4 * g), S[i], x);
+    return x;
 }
-template <int DK>
-MRL_DEV void go_on(const Block<DK> &block, const Decays &decay, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
-    const f32x4 ks = block.four(block.kscale, tile, g);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) u[r] *= decay.to[r] * ks[r];
+// S0 + sum_i k[i] x[i]^T over a tile's keys (or queries), unscaled
+template <int DK, int TILES>
+MRL_DEV void add(const Block<DK, TILES> &block, const float *rows, int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) {
 #pragma unroll
     for (int i = 0; i < DK / TILE; ++i) {
         f32x4 k;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) k[r] = block.K[(tile * TILE + 4 * g + r) * Block<DK>::ROW + i * TILE + c];
-        S[i] = mfma16(k, u, S[i] * decay.whole);
+        for (int r = 0; r < 4; ++r) k[r] = rows[(tile * TILE + 4 * g + r) * block.ROW + i * TILE + c];
+        S[i] = mfma16(k, x, S[i]);
     }
 }
+// U[4 g + r][c] of a tile; read: b F S0^T k, what the keys read of the state
+template <int DK, int TILES>
+MRL_DEV f32x4 solve(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
+    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g);
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        read[r] = b[r] * decay.from[r] * ks[r] * sk[r];
+        x[r] = fmaf(b[r], v[r], -read[r]);
+    }
+    const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
+    return mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+}
+// S0 becomes S1
+template <int DK, int TILES>
+MRL_DEV void go_on(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
+    const f32x4 ks = block.four(block.kscale, tile, g);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) u[r] *= decay.to[r] * ks[r];
+#pragma unroll
+    for (int i = 0; i < DK / TILE; ++i) S[i] *= decay.whole;
+    add(block, block.K, tile, g, c, u, S);
+}
 
-// The backward pass's first launch: S ahead of every block but the first, as the lanes hold it, to
-// states [N * H][blocks][column tiles][DK / 16][64][4]
-int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, float *states, int blocks);
+// ---------------------------------------------------------------- a long rollout of a few environments, in parts
+// Where heads and environments leave CUs without work the steps are cut into parts of `per` blocks.  A part takes the state S ahead of it to
+// M S + B, a product of the steps' contractions and what it makes of a zero state; M and B of all parts come side by side (M as the part's result for
+// the columns of the identity, without values), a second launch goes through them, M S + B, and then every part has its first state.  The
+// same, from the last part to the first and with M^T, for the gradient of the state.  A part with a cut has M = 0, and says so.
+// States are kept as lanes hold them: [environment and head][part][tile of 16 columns][tile of 16 rows][lane][4].
+struct Parts {
+    int count, per;      // count 1: no parts
+    float *ends;         // B of every part, then M: column_tiles(dv) + dk / 16 tiles
+    float *starts;       // S ahead of every part
+    int *cuts;           // whether a part has a cut
+};
 inline int padded(int dk) { return dk <= 16 ? 16 : dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
 inline int column_tiles(int dv) { return (dv + TILE - 1) / TILE; }
-inline int blocks_of(int T, int dk) { return (T + TILE * tiles_of(padded(dk)) - 1) / (TILE * tiles_of(padded(dk))); }
+inline int blocks_of(int T, int tiles) { return (T + TILE * tiles - 1) / (TILE * tiles); }
+constexpr int floats_of(int DK) { return DK * TILE; }   // of a column tile
 
+// How many parts: as many as fill the card twice, where that is four at least.
+inline Parts parts_of(const mrl_ctx *ctx, const mrl_delta *r, int tiles) {
+    Parts p = {};
+    const int blocks = blocks_of(r->T, tiles), tile_columns = column_tiles(r->value_dim);
+    const long groups = (long)r->N * r->heads * ((tile_columns + 3) / 4);
+    const long want = std::min<long>(blocks, 2L * ctx->n_cus / groups);
+    p.count = 1;
+    p.per = blocks;
+    if (want < 4) return p;
+    p.per = (int)((blocks + want - 1) / want);
+    p.count = (blocks + p.per - 1) / p.per;
+    return p;
+}
+inline size_t ends_floats(const mrl_delta *r, const Parts &p) {
+    const int DK = padded(r->key_dim);
+    return p.count > 1 ? (size_t)r->N * r->heads * p.count * (column_tiles(r->value_dim) + DK / TILE) * floats_of(DK) : 0;
+}
+inline size_t starts_floats(const mrl_delta *r, const Parts &p) {
+    return p.count > 1 ? (size_t)r->N * r->heads * p.count * column_tiles(r->value_dim) * floats_of(padded(r->key_dim)) : 0;
+}
+inline size_t cuts_floats(const mrl_delta *r, const Parts &p) { return p.count > 1 ? ((size_t)r->N * r->heads * p.count + 63) / 64 * 64 : 0; }
+
+// M, B and the first states of all parts of blocks of the backward pass
+int launch_starts(const mrl_ctx *ctx, int dtype, const Delta &d, const Parts &p);
+// S ahead of every such block, to states [N * H][blocks][column tiles][DK / 16][64][4]
+int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, const Parts &p, float *states, int blocks);
+// the gradients of the states behind all parts, to p.starts, from those of parts with none behind them in `local`, laid out alike
+int launch_grad_ends(const mrl_ctx *ctx, const Delta &d, const Parts &p, const float *grad_state_out, const float *local);
+
+size_t forward_bytes(const mrl_ctx *ctx, const mrl_delta *r);
 int check_sizes(const char *who, const mrl_delta *r);
 int check(const char *who, const mrl_ctx *ctx, const mrl_delta *r);
 Delta describe(const mrl_delta *r);

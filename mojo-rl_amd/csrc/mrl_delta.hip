@@ -81,56 +81,66 @@ __global__ __launch_bounds__(256) void step_kernel(Delta d, int units, int colum
 
 // ---------------------------------------------------------------- rollouts
 constexpr int MOST_WAVES = 4;
+enum { OUTPUTS, STATES, ENDS };   // of all steps; ahead of every block; M and B of every part
 
-// A workgroup goes through the steps of one head of one environment; each of its wavefronts keeps 16 columns of the state in registers,
-// all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.  STATES: no outputs, the
-// state ahead of every block instead.
-template <class E, int DK, bool STATES>
-__global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kernel(Delta d, int column_groups, float *states, int blocks) {
+// A workgroup goes through a part's steps of one head of one environment; each of its wavefronts keeps 16 columns of the state in registers,
+// all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.
+template <class E, int DK, int TILES, int WHAT>
+__global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kernel(Delta d, Parts parts, int column_groups, float *states, int blocks) {
     extern __shared__ float lds[];
-    constexpr int B = DK / TILE, TILES = Block<DK>::TILES, STEPS = Block<DK>::STEPS, ROW = Block<DK>::ROW;
-    Block<DK> block(lds);
+    constexpr int B = DK / TILE, STEPS = TILE * TILES;
+    Block<DK, TILES> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
-    const int group = blockIdx.x % column_groups, nh = blockIdx.x / column_groups, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % parts.count, nh = at_part / parts.count;
+    const int n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK), tiles = (d.dv + TILE - 1) / TILE;
     const int column_tile = group * W + w, column = column_tile * TILE + c;
     const bool live = column < d.dv;
     const long state_at = (long)nh * d.dk * d.dv + column;
 
     f32x4 S[B];
+    if (WHAT != ENDS && parts.count > 1) {
+        const float *from = parts.starts + (((long)at_part * tiles + min(column_tile, tiles - 1)) * B * 64 + lane) * 4;
 #pragma unroll
-    for (int i = 0; i < B; ++i)
+        for (int i = 0; i < B; ++i) S[i] = *reinterpret_cast<const f32x4 *>(from + i * 256);
+    } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = i * TILE + 4 * g + r;
-            S[i][r] = d.state_in != nullptr && live && row < d.dk ? d.state_in[state_at + (long)row * d.dv] : 0.0f;
-        }
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = i * TILE + 4 * g + r;
+                if (WHAT == ENDS) S[i][r] = column - tiles * TILE == row ? 1.0f : 0.0f;   // the identity's columns come behind the values'
+                else S[i][r] = d.state_in != nullptr && live && row < d.dk ? d.state_in[state_at + (long)row * d.dv] : 0.0f;
+            }
+    }
 
     const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
+    int begin = part * parts.per * STEPS;   // of the block
+    const int end = min(d.T, begin + parts.per * STEPS);
+    bool cut = false;
     block.span = TILE;
-    int begin = 0;   // of the block
-    for (block.t0 = 0; block.t0 < d.T;) {
-        if (STATES && block.t0 == begin) {
+    for (block.t0 = begin; block.t0 < end;) {
+        if (WHAT == STATES && block.t0 == begin) {
             const int number = begin / STEPS;
-            if (number > 0 && column_tile * TILE < d.dv) {
-                float *to = states + ((((long)nh * blocks + number) * ((d.dv + TILE - 1) / TILE) + column_tile) * B * 64 + lane) * 4;
+            if (column_tile < tiles) {
+                float *to = states + ((((long)nh * blocks + number) * tiles + column_tile) * B * 64 + lane) * 4;
 #pragma unroll
                 for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = S[i];
             }
-            if (number == blocks - 1) return;
+            if (begin + STEPS >= end) return;
         }
         f32x4 V[TILES];
         anew(g, c);
         anew(thread);
         bool odd = is_odd(S);
-        odd |= load_values<E, DK>(d, block, values, (long)d.N * d.value_ld, live, g, V);
-        odd |= block.template load<E, !STATES>(d, n, h, hk, thread);
+        odd |= load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
+        odd |= block.template load<E, WHAT == OUTPUTS>(d, n, h, hk, thread);
         if (__syncthreads_or(odd) && block.span == TILE) {
             block.span = 1;
             continue;   // the same block again, one step to a tile
         }
         anew(g, c);
-        for (int tile = w; tile < TILES; tile += W) block.template prepare<!STATES>(tile, g, c);
+        for (int tile = w; tile < TILES; tile += W) block.template prepare<WHAT == OUTPUTS>(tile, g, c);
         __syncthreads();
 #pragma unroll 1
         for (int tile = 0; tile < TILES; ++tile) {
@@ -142,29 +152,31 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, o = sk;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const int at = (tile * TILE + c) * ROW + i * TILE + 4 * g;
-                sk = mfma16(*reinterpret_cast<const f32x4 *>(block.K + at), S[i], sk);
-                if (!STATES) o = mfma16(*reinterpret_cast<const f32x4 *>(block.Q + at), S[i], o);
-            }
-            f32x4 v = V[0];
+            f32x4 v = V[0], read, o;
 #pragma unroll
             for (int i = 1; i < TILES; ++i) v = tile == i ? V[i] : v;
-            const f32x4 u = solve(block, decay, tile, g, c, v, sk);
-            if (!STATES) {
+            const f32x4 sk = ask(block, block.K, tile, g, c, S);
+            if (WHAT == OUTPUTS) o = ask(block, block.Q, tile, g, c, S);
+            const f32x4 u = solve(block, decay, tile, g, c, v, sk, read);
+            if (WHAT == OUTPUTS) {
                 const f32x4 qs = block.four(block.qscale, tile, g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] *= decay.from[r] * qs[r];
                 o = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + tile * TILE * SIDE + c * SIDE + 4 * g), u, o);
             }
             go_on(block, decay, tile, g, c, u, S);
-            if (!STATES) {
+            if (WHAT == OUTPUTS) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int slot = tile * TILE + 4 * g + r;
                     if (live && block.there(d, slot)) give((E *)d.out + ((long)block.time_of(slot) * d.N + n) * d.out_ld + h * d.dv + column, o[r]);
+                }
+            }
+            if (WHAT == ENDS) {
+#pragma unroll
+                for (int i = 0; i < TILE; i += 4) {
+                    const f32x4 a = *reinterpret_cast<const f32x4 *>(block.as + tile * TILE + i);
+                    cut |= a[0] == 0.0f || a[1] == 0.0f || a[2] == 0.0f || a[3] == 0.0f;
                 }
             }
         }
@@ -175,7 +187,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
         }
         __syncthreads();
     }
-    if (STATES || d.state_out == nullptr || !live) return;
+    if (WHAT == ENDS) {
+        if (column_tile >= tiles + B) return;
+        float *to = parts.ends + (((long)at_part * (tiles + B) + column_tile) * B * 64 + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = S[i];
+        if (threadIdx.x == 0 && group == 0) parts.cuts[at_part] = cut;
+    }
+    if (WHAT != OUTPUTS || d.state_out == nullptr || !live || part != parts.count - 1) return;
 #pragma unroll
     for (int i = 0; i < B; ++i)
 #pragma unroll
@@ -183,6 +202,46 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
             const int row = i * TILE + 4 * g + r;
             if (row < d.dk) d.state_out[state_at + (long)row * d.dv] = S[i][r];
         }
+}
+
+// Through the parts: S <- M S + B, from the first to the last, S ahead of each to parts.starts; BACK: S <- M^T S + B from the last to the first, B in
+// `local`, S behind each to parts.starts.  A workgroup 16 columns, a wavefront 16 rows of them; S changes hands through LDS.
+template <int DK, bool BACK>
+__global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, const float *first, const float *local) {
+    __shared__ f32x4 S[2][DK / TILE][64];
+    constexpr int B = DK / TILE;
+    const int tiles = (d.dv + TILE - 1) / TILE, column_tile = blockIdx.x % tiles, nh = blockIdx.x / tiles;
+    const int i = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, column = column_tile * TILE + c;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = i * TILE + 4 * g + r;
+        if (first != nullptr && column < d.dv && row < d.dk) s[r] = first[((long)nh * d.dk + row) * d.dv + column];
+    }
+    for (int step = 0; step < parts.count; ++step) {
+        const int part = BACK ? parts.count - 1 - step : step;
+        const long at = (long)nh * parts.count + part;
+        *reinterpret_cast<f32x4 *>(parts.starts + (((at * tiles + column_tile) * B + i) * 64 + lane) * 4) = s;
+        if (step == parts.count - 1) break;
+        f32x4 (&here)[B][64] = S[step & 1];
+        here[i][lane] = s;
+        const float *const ends = parts.ends + at * (tiles + B) * B * 256, *const M = ends + (long)tiles * B * 256;   // M: [column tile][row tile][lane][4]
+        f32x4 m[B];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            // the operand's row c and contracted 4 g .. 4 g + 3: of M^T four neighbouring rows of a column of M, as they lie; of M a row's columns
+            if (BACK) m[k] = *reinterpret_cast<const f32x4 *>(M + ((i * B + k) * 64 + lane) * 4);
+            else
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[k][r] = M[((k * B + i) * 64 + 16 * (c >> 2) + 4 * g + r) * 4 + (c & 3)];
+        }
+        s = *reinterpret_cast<const f32x4 *>(BACK ? local + (((at * tiles + column_tile) * B + i) * 64 + lane) * 4 : ends + ((column_tile * B + i) * 64 + lane) * 4);
+        __syncthreads();   // (the buffers alternate)
+        if (!parts.cuts[at]) {
+#pragma unroll
+            for (int k = 0; k < B; ++k) s = mfma16(m[k], here[k][lane], s);
+        }
+    }
 }
 
 template <class E, int L>
@@ -194,37 +253,104 @@ void launch_step(const mrl_ctx *ctx, const Delta &d) {
     else if (rows <= 16) hipLaunchKernelGGL((step_kernel<E, L, 16>), grid, block, 0, ctx->stream, d, units, blocks);
     else hipLaunchKernelGGL((step_kernel<E, L, 32>), grid, block, 0, ctx->stream, d, units, blocks);
 }
-template <class E, bool STATES, int DK>
-void launch_tiles(const mrl_ctx *ctx, const Delta &d, float *states, int blocks) {
-    const int tiles = column_tiles(d.dv), waves = std::min(MOST_WAVES, tiles), groups = (tiles + waves - 1) / waves;
-    hipLaunchKernelGGL((tiles_kernel<E, DK, STATES>), dim3(d.N * d.H * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK), ctx->stream, d, groups, states, blocks);
+template <class E, int DK, int TILES, int WHAT>
+void launch_tiles(const mrl_ctx *ctx, const Delta &d, const Parts &p, float *states = nullptr, int blocks = 0) {
+    const int tiles = column_tiles(d.dv) + (WHAT == ENDS ? DK / TILE : 0), waves = std::min(MOST_WAVES, tiles), groups = (tiles + waves - 1) / waves;
+    hipLaunchKernelGGL((tiles_kernel<E, DK, TILES, WHAT>), dim3(d.N * d.H * p.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, TILES), ctx->stream, d, p,
+                       groups, states, blocks);
 }
-template <class E, bool STATES>
-void launch_tiles(const mrl_ctx *ctx, const Delta &d, float *states = nullptr, int blocks = 0) {
-    switch (padded(d.dk)) {
-        case 16: return launch_tiles<E, STATES, 16>(ctx, d, states, blocks);
-        case 32: return launch_tiles<E, STATES, 32>(ctx, d, states, blocks);
-        case 64: return launch_tiles<E, STATES, 64>(ctx, d, states, blocks);
-        default: return launch_tiles<E, STATES, 128>(ctx, d, states, blocks);
-    }
+template <class E, int DK, int TILES>
+void launch_starts(const mrl_ctx *ctx, const Delta &d, const Parts &p) {
+    launch_tiles<E, DK, TILES, ENDS>(ctx, d, p);
+    hipLaunchKernelGGL((parts_kernel<DK, false>), dim3(d.N * d.H * column_tiles(d.dv)), dim3(DK * 4), 0, ctx->stream, d, p, d.state_in, nullptr);
+}
+template <class E, int DK>
+void launch_rollout(const mrl_ctx *ctx, const Delta &d, const Parts &p) {
+    if (p.count > 1) launch_starts<E, DK, tiles_forward(DK)>(ctx, d, p);
+    launch_tiles<E, DK, tiles_forward(DK), OUTPUTS>(ctx, d, p);
 }
 template <class E>
-void launch(const mrl_ctx *ctx, const Delta &d) {
-    if (d.T > 1) launch_tiles<E, false>(ctx, d);
-    else if (d.dv <= 32) launch_step<E, 8>(ctx, d);
-    else launch_step<E, 16>(ctx, d);
+void launch(const mrl_ctx *ctx, const Delta &d, const Parts &p) {
+    if (d.T == 1) return d.dv <= 32 ? launch_step<E, 8>(ctx, d) : launch_step<E, 16>(ctx, d);
+    switch (padded(d.dk)) {
+        case 16: return launch_rollout<E, 16>(ctx, d, p);
+        case 32: return launch_rollout<E, 32>(ctx, d, p);
+        case 64: return launch_rollout<E, 64>(ctx, d, p);
+        default: return launch_rollout<E, 128>(ctx, d, p);
+    }
+}
+
+struct Plan {
+    Parts parts;
+    size_t bytes;
+};
+Plan plan_of(const mrl_ctx *ctx, const mrl_delta *r) {
+    Plan p = {};
+    if (r->T < 2 || r->N == 0) return p;
+    p.parts = parts_of(ctx, r, tiles_forward(padded(r->key_dim)));
+    p.bytes = sizeof(float) * (ends_floats(r, p.parts) + starts_floats(r, p.parts) + cuts_floats(r, p.parts));
+    return p;
 }
 
 }  // namespace
+
+size_t forward_bytes(const mrl_ctx *ctx, const mrl_delta *r) { return plan_of(ctx, r).bytes; }
 
 // no step at all: the state goes through as it is
 __global__ __launch_bounds__(256) void pass_state_kernel(const float *from, float *to, long n) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) to[i] = from ? from[i] : 0.0f;
 }
 
-int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, float *states, int blocks) {
-    if (dtype == MRL_F32) launch_tiles<float, true>(ctx, d, states, blocks);
-    else launch_tiles<bf16_t, true>(ctx, d, states, blocks);
+namespace {
+template <class E, int DK>
+void backward_starts(const mrl_ctx *ctx, const Delta &d, const Parts &p) { launch_starts<E, DK, tiles_backward(DK)>(ctx, d, p); }
+template <class E, int DK>
+void backward_states(const mrl_ctx *ctx, const Delta &d, const Parts &p, float *states, int blocks) {
+    launch_tiles<E, DK, tiles_backward(DK), STATES>(ctx, d, p, states, blocks);
+}
+template <class E>
+void backward_starts(const mrl_ctx *ctx, const Delta &d, const Parts &p) {
+    switch (padded(d.dk)) {
+        case 16: return backward_starts<E, 16>(ctx, d, p);
+        case 32: return backward_starts<E, 32>(ctx, d, p);
+        case 64: return backward_starts<E, 64>(ctx, d, p);
+        default: return backward_starts<E, 128>(ctx, d, p);
+    }
+}
+template <class E>
+void backward_states(const mrl_ctx *ctx, const Delta &d, const Parts &p, float *states, int blocks) {
+    switch (padded(d.dk)) {
+        case 16: return backward_states<E, 16>(ctx, d, p, states, blocks);
+        case 32: return backward_states<E, 32>(ctx, d, p, states, blocks);
+        case 64: return backward_states<E, 64>(ctx, d, p, states, blocks);
+        default: return backward_states<E, 128>(ctx, d, p, states, blocks);
+    }
+}
+template <int DK>
+void grad_ends(const mrl_ctx *ctx, const Delta &d, const Parts &p, const float *grad_state_out, const float *local) {
+    hipLaunchKernelGGL((parts_kernel<DK, true>), dim3(d.N * d.H * column_tiles(d.dv)), dim3(DK * 4), 0, ctx->stream, d, p, grad_state_out, local);
+}
+}  // namespace
+
+int launch_starts(const mrl_ctx *ctx, int dtype, const Delta &d, const Parts &p) {
+    if (dtype == MRL_F32) backward_starts<float>(ctx, d, p);
+    else backward_starts<bf16_t>(ctx, d, p);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+int launch_states(const mrl_ctx *ctx, int dtype, const Delta &d, const Parts &p, float *states, int blocks) {
+    if (dtype == MRL_F32) backward_states<float>(ctx, d, p, states, blocks);
+    else backward_states<bf16_t>(ctx, d, p, states, blocks);
+    MRL_CHECK_LAUNCH();
+    return MRL_OK;
+}
+int launch_grad_ends(const mrl_ctx *ctx, const Delta &d, const Parts &p, const float *grad_state_out, const float *local) {
+    switch (padded(d.dk)) {
+        case 16: grad_ends<16>(ctx, d, p, grad_state_out, local); break;
+        case 32: grad_ends<32>(ctx, d, p, grad_state_out, local); break;
+        case 64: grad_ends<64>(ctx, d, p, grad_state_out, local); break;
+        default: grad_ends<128>(ctx, d, p, grad_state_out, local); break;
+    }
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -280,7 +406,11 @@ int mrl_delta_forward(mrl_ctx *ctx, const mrl_delta *r, void *out, int64_t out_l
     const int64_t size = r->dtype == MRL_F32 ? 4 : 2, rows = (int64_t)r->T * r->N;
     const auto of = [&](const char *name, const void *at, long width, long ld) { return Region(name, at, rows, size * width, size * ld); };
     const long k_width = (long)r->key_heads * r->key_dim, v_width = (long)r->heads * r->value_dim;
-    const int apart = check_apart(who, {of("out", out, v_width, out_ld), Region("state_out", state_out, 4 * states)},
+    const Plan plan = plan_of(ctx, r);
+    MRL_CHECK_ARG(workspace_bytes >= plan.bytes && (plan.bytes == 0 || workspace != nullptr), "%s: the workspace holds %llu bytes, need %llu", who,
+                  (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)plan.bytes);
+    MRL_CHECK_ARG(plan.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", who);
+    const int apart = check_apart(who, {of("out", out, v_width, out_ld), Region("state_out", state_out, 4 * states), Region("the workspace", plan.bytes ? workspace : nullptr, (int64_t)plan.bytes)},
                                   {of("query", r->query, k_width, r->query_ld), of("key", r->key, k_width, r->key_ld), of("value", r->value, v_width, r->value_ld),
                                    of("gate", r->gate, r->heads, r->gate_ld), of("rate", r->rate, r->heads, r->rate_ld), Region("dones", r->dones, 4 * rows),
                                    Region("prev_dones", r->prev_dones, 4LL * r->N), Region("state_in", r->state_in == state_out ? nullptr : r->state_in, 4 * states)});
@@ -294,8 +424,12 @@ int mrl_delta_forward(mrl_ctx *ctx, const mrl_delta *r, void *out, int64_t out_l
     }
     Delta d = describe(r);
     d.out = out; d.out_ld = out_ld; d.state_out = state_out;
-    if (r->dtype == MRL_F32) launch<float>(ctx, d);
-    else launch<bf16_t>(ctx, d);
+    Parts p = plan.parts;
+    p.ends = (float *)workspace;
+    p.starts = p.ends + ends_floats(r, p);
+    p.cuts = (int *)(p.starts + starts_floats(r, p));
+    if (r->dtype == MRL_F32) launch<float>(ctx, d, p);
+    else launch<bf16_t>(ctx, d, p);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }

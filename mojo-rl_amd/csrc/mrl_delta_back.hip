@@ -11,10 +11,14 @@
 // added up as it stands: every term has a[t] in it.  (Sums of row and column dots, of which this is a difference, lose it where a is small.)
 // dgate = (1 - a) times that, 0 at a cut.
 //
-// A first launch leaves the state ahead of every block of tiles in the workspace (mrl_delta.hip).  In the second a workgroup goes through the blocks
+// With what the forward pass leaves, the dots that the lengths and the gates need are sums over the columns:
+//   q[i] dq[i] = dO[i] out[i],   k[i] dk[i] = dX[i] (2 U[i] - b[i] v[i]),   e[i] = dO[i] (F[i] S0^T q[i]) - dX[i] (b[i] F[i] S0^T k[i]),   f[i] = L[i] U[i] (dS1^T k[i]).
+//
+// A first launch leaves the state ahead of every block of tiles in the workspace (mrl_delta.hip).  In the last a workgroup goes through the blocks
 // of one head of one environment from the last to the first: it repeats a block's tiles forwards, keeping each tile's S0 and U in registers,
 // and takes the tiles backwards.  A wavefront holds 16 columns of S0 and dS1; what contracts over the columns (dq, dk, dA, dP) is done by 16
-// rows of the states per wavefront, which they pass through LDS, S0 first and dS1 after it in the same place.
+// rows of the states per wavefront, which they pass through LDS.  A rollout in parts has the gradients of the states behind the parts worked out
+// ahead of that (chain_kernel, and the launch that goes through the parts).
 #include <type_traits>
 #include "delta.hpp"
 
@@ -26,6 +30,7 @@ constexpr int MOST_WAVES = 8;
 
 struct Back {
     Delta d;
+    Parts parts;
     const void *grad_out;
     long grad_out_ld;
     const float *grad_state_out;
@@ -34,51 +39,180 @@ struct Back {
     long query_ld, key_ld, value_ld, gate_ld, rate_ld;
     float *state;
     const float *states;
+    const float *grad_ends;   // of the states behind the parts
+    float *local;             // the same of parts with none behind them
     int blocks;
 };
 
-constexpr size_t back_floats(int DK, int W) {
-    const int columns = TILE * W + 4;
-    return rows_floats(DK) + (size_t)DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 3 * TILE * MOST_WAVES + MOST_WAVES;
+// sums over the 16 lanes of a group, in all of them
+template <int N>
+MRL_DEV float turned(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + N, 0xF, 0xF, false)); }
+MRL_DEV float sum16(float x) {
+    x += turned<8>(x);
+    x += turned<4>(x);
+    x += turned<2>(x);
+    return x + turned<1>(x);
+}
+// what the lanes from this one on have, and those ahead of it
+template <int CONTROL>
+MRL_DEV float moved(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CONTROL, 0xF, 0xF, true)); }
+MRL_DEV float sum_from(float x) {
+    x += moved<0x101>(x);
+    x += moved<0x102>(x);
+    x += moved<0x104>(x);
+    return x + moved<0x108>(x);
+}
+MRL_DEV float sum_ahead(float x) {
+    x = moved<0x111>(x);
+    x += moved<0x111>(x);
+    x += moved<0x112>(x);
+    x += moved<0x114>(x);
+    return x + moved<0x118>(x);
 }
 
-MRL_DEV float sum16(float x) {   // over the 16 lanes of a group
+// What a tile's columns make of dO and dS1: read = L dS1^T k, dX, and dS1 becomes dS0.
+template <int DK, int TILES>
+MRL_DEV void pull(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
+    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
+    read = ask(block, block.K, tile, g, c, dS);
+    f32x4 p_column, t_column;
 #pragma unroll
-    for (int s = 1; s < 16; s *= 2) x += __shfl_xor(x, s);
-    return x;
+    for (int r = 0; r < 4; ++r) {
+        read[r] *= decay.to[r] * ks[r];
+        p_column[r] = block.Ps[(tile * TILE + 4 * g + r) * SIDE + c];
+        t_column[r] = block.Ts[(tile * TILE + 4 * g + r) * SIDE + c];
+    }
+    dX = mfma16(t_column, mfma16(p_column, dO, read), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    f32x4 q_part, k_part;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        q_part[r] = decay.from[r] * qs[r] * dO[r];
+        k_part[r] = -decay.from[r] * ks[r] * b[r] * dX[r];
+    }
+#pragma unroll
+    for (int i = 0; i < DK / TILE; ++i) dS[i] *= decay.whole;
+    add(block, block.Q, tile, g, c, q_part, dS);
+    add(block, block.K, tile, g, c, k_part, dS);
+    if (block.cut_ahead(tile)) {
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i) dS[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 }
+
+template <int B>
+MRL_DEV void first_gradient(const Back &p, int at_part, int nh, int column_tile, int tiles, bool behind, int g, int c, f32x4 (&dS)[B]) {
+    const Delta &d = p.d;
+    const int column = column_tile * TILE + c, lane = threadIdx.x & 63;
+    if (p.parts.count > 1) {
+        const float *from = p.grad_ends + (((long)at_part * tiles + min(column_tile, tiles - 1)) * B * 64 + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < B; ++i) dS[i] = behind ? *reinterpret_cast<const f32x4 *>(from + i * 256) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = i * TILE + 4 * g + r;
+                dS[i][r] = p.grad_state_out != nullptr && column < d.dv && row < d.dk ? p.grad_state_out[((long)nh * d.dk + row) * d.dv + column] : 0.0f;
+            }
+    }
+}
+
+// The gradient of the state ahead of a part with none behind it: the chain of the states' gradients alone.
+template <class E, int DK>
+__global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups) {
+    extern __shared__ float lds[];
+    constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES;
+    const Delta &d = p.d;
+    Block<DK, TILES> block(lds);
+    const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
+    const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % p.parts.count, nh = at_part / p.parts.count;
+    const int n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK), tiles = (d.dv + TILE - 1) / TILE, column_tile = group * W + w, column = column_tile * TILE + c;
+    const bool live = column < d.dv;
+    const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
+    f32x4 dS[B], dO[TILES];
+#pragma unroll
+    for (int i = 0; i < B; ++i) dS[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int number = min(p.blocks, (part + 1) * p.parts.per) - 1; number >= part * p.parts.per; --number) {
+        const int begin = number * STEPS, end = min(begin + STEPS, d.T);
+        block.t0 = begin;
+        block.span = TILE;
+        int rounds = 1;
+        for (int round = 0; round < rounds;) {
+            anew(g, c);
+            anew(thread);
+            bool odd = is_odd(dS);
+            odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
+            odd |= block.template load<E, true>(d, n, h, hk, thread);
+            if (__syncthreads_or(odd) && block.span == TILE) {   // one step to a tile, TILES of them at a time, from the last
+                block.span = 1;
+                rounds = (end - begin + TILES - 1) / TILES;
+                block.t0 = begin + (rounds - 1) * TILES;
+                continue;
+            }
+            anew(g, c);
+            for (int tile = w; tile < TILES; tile += W) block.template prepare<true>(tile, g, c);
+            __syncthreads();
+#pragma unroll
+            for (int tile = TILES - 1; tile >= 0; --tile) {
+                if (block.t0 + tile * block.span >= d.T) continue;
+                anew(g, c);
+                Decays decay;
+                decay.load(block.as + tile * TILE, g);
+                f32x4 read, dX;
+                pull(block, decay, tile, g, c, dO[tile], dS, read, dX);
+            }
+            block.t0 -= TILES;
+            ++round;
+            __syncthreads();
+        }
+    }
+    if (column_tile >= tiles) return;
+    float *to = p.local + (((long)at_part * tiles + column_tile) * B * 64 + lane) * 4;
+#pragma unroll
+    for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = dS[i];
+}
+
+constexpr bool both_states(int DK) { return DK < 128; }   // S0 and dS1 in LDS side by side
+inline int waves_of(int DK, int dv) { return std::max(column_tiles(dv), std::min(4, DK / TILE)); }
+constexpr int DOTS = 5;   // q dq, k dk, e, f, U dX
+size_t back_floats(int DK, int dv) {
+    const int columns = TILE * column_tiles(dv) + 4, W = waves_of(DK, dv);
+    return rows_floats(DK, tiles_backward(DK)) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
+}
+
 // EK: the type of the gradients of query and key (float where a group's are summed later)
 template <class E, class EK, int DK>
-__global__ __launch_bounds__(64 * MOST_WAVES) void back_kernel(Back p) {
+__global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     extern __shared__ float lds[];
-    constexpr int B = DK / TILE, TILES = Block<DK>::TILES, STEPS = Block<DK>::STEPS, ROW = Block<DK>::ROW;
+    constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES, OWN = B <= 4 ? 1 : 2;   // OWN: row tiles of a wavefront
+    constexpr bool BOTH = both_states(DK);
     const Delta &d = p.d;
-    Block<DK> block(lds);
-    const int W = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int columns = TILE * W + 4;
-    float *state = lds + rows_floats(DK), *dOs = state + DK * columns, *dXs = dOs + TILE * columns, *Us = dXs + TILE * columns;
-    float *dAs = Us + TILE * columns, *dPs = dAs + TILE * SIDE, *dots = dPs + TILE * SIDE, *whole = dots + 3 * TILE * MOST_WAVES;
-    const int nh = blockIdx.x, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    Block<DK, TILES> block(lds);
+    const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, tiles = (d.dv + TILE - 1) / TILE;
+    int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
+    const int stride = TILE * tiles + 4;
+    float *const states = lds + rows_floats(DK, TILES), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
+    float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE, *const crossing = dPs + TILE * SIDE;
+    float *const dots = crossing + TILE, *const wholes = dots + 2 * DOTS * TILE * W;   // [2][DOTS][W][16], [2][W]: two tiles' in turn
+    const int at_part = blockIdx.x, part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    const bool owns = w < tiles;   // columns; the other wavefronts have rows only
     const int column = w * TILE + c;
     const bool live = column < d.dv;
     const long state_at = (long)nh * d.dk * d.dv + column;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const int key_at = (p.per_head ? h : hk) * d.dk;
+    const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
+    const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
 
-    f32x4 dS[B];
-#pragma unroll
-    for (int i = 0; i < B; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = i * TILE + 4 * g + r;
-            dS[i][r] = p.grad_state_out != nullptr && live && row < d.dk ? p.grad_state_out[state_at + (long)row * d.dv] : 0.0f;
-        }
-
-    const auto first_state = [&](int number, f32x4 (&S)[B]) {
+    f32x4 dS[B], S[B], V[TILES], dO[TILES], kept[TILES][B], U[TILES], reads[TILES];
+    first_gradient(p, at_part, nh, w, tiles, owns, g, c, dS);
+    const auto first_state = [&](int number) {
         if (number > 0) {
-            const float *from = p.states + ((((long)nh * p.blocks + number) * W + w) * B * 64 + lane) * 4;
+            const float *from = p.states + ((((long)nh * p.blocks + number) * tiles + min(w, tiles - 1)) * B * 64 + lane) * 4;
 #pragma unroll
-            for (int i = 0; i < B; ++i) S[i] = *reinterpret_cast<const f32x4 *>(from + i * 256);
+            for (int i = 0; i < B; ++i) S[i] = owns ? *reinterpret_cast<const f32x4 *>(from + i * 256) : zero;
         } else {
 #pragma unroll
             for (int i = 0; i < B; ++i)
@@ -89,275 +223,243 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void back_kernel(Back p) {
                 }
         }
     };
-    f32x4 S[B], V[TILES], dO[TILES], kept[TILES][B], U[TILES];
     // the tiles that the block holds, forwards; keep: S0 and U of each stay
     const auto forwards = [&](auto keep) {
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile) {
+            anew(g, c);
             Decays decay;
             decay.load(block.as + tile * TILE, g);
             if (block.cut_ahead(tile)) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = zero;
             }
-            f32x4 sk = zero;
-#pragma unroll
-            for (int i = 0; i < B; ++i) sk = mfma16(*reinterpret_cast<const f32x4 *>(block.K + (tile * TILE + c) * ROW + i * TILE + 4 * g), S[i], sk);
-            const f32x4 u = solve(block, decay, tile, g, c, V[tile], sk);
+            f32x4 read;
+            const f32x4 u = solve(block, decay, tile, g, c, V[tile], ask(block, block.K, tile, g, c, S), read);
             if constexpr (decltype(keep)::value) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) kept[tile][i] = S[i];
                 U[tile] = u;
+                reads[tile] = read;
             }
             if (!decltype(keep)::value || tile + 1 < TILES) go_on(block, decay, tile, g, c, u, S);
         }
     };
-    const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
-    const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
     const auto load = [&]() {
-        bool odd = load_values<E, DK>(d, block, values, (long)d.N * d.value_ld, live, g, V);
-        odd |= load_values<E, DK>(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
-        odd |= block.template load<E, true>(d, n, h, hk, threadIdx.x);
+        anew(g, c);
+        anew(thread);
+        bool odd = load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
+        odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
+        odd |= block.template load<E, true>(d, n, h, hk, thread);
         return odd;
     };
+    const auto spread = [&](float *to, const f32x4 (&x)[B]) {   // a wavefront's columns of a state
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[(i * TILE + 4 * g + r) * stride + w * TILE + c] = x[i][r];
+    };
 
-    for (int number = p.blocks - 1; number >= 0; --number) {
+    for (int number = min(p.blocks, (part + 1) * p.parts.per) - 1; number >= part * p.parts.per; --number) {
         const int begin = number * STEPS, end = min(begin + STEPS, d.T);
-        first_state(number, S);
+        first_state(number);
         block.t0 = begin;
         block.span = TILE;
         bool odd = is_odd(S) | is_odd(dS);
         odd |= load();
-        int parts = 1;
+        int rounds = 1;
         if (__syncthreads_or(odd)) {   // one step to a tile, TILES of them at a time
             block.span = 1;
-            parts = (end - begin + TILES - 1) / TILES;
+            rounds = (end - begin + TILES - 1) / TILES;
         }
-        for (int part = parts - 1; part >= 0; --part) {
+        for (int round = rounds - 1; round >= 0; --round) {
             if (block.span == 1) {
-                first_state(number, S);
-                for (int ahead = 0; ahead <= part; ++ahead) {   // up to this part, every time: only where a value is not finite
+                first_state(number);
+                for (int ahead = 0; ahead <= round; ++ahead) {   // up to this round's, every time: only where a value is not finite
                     block.t0 = begin + ahead * TILES;
+                    __syncthreads();
                     load();
                     __syncthreads();
-                    if (ahead == part) break;
+                    if (ahead == round) break;
                     for (int tile = w; tile < TILES; tile += W) block.template prepare<false>(tile, g, c);
                     __syncthreads();
                     forwards(std::false_type{});
-                    __syncthreads();
                 }
             }
+            anew(g, c);
             for (int tile = w; tile < TILES; tile += W) block.template prepare<true>(tile, g, c);
             __syncthreads();
-            forwards(std::true_type{});
+            if (owns) forwards(std::true_type{});
 #pragma unroll
             for (int tile = TILES - 1; tile >= 0; --tile) {
                 if (block.t0 + tile * block.span >= d.T) continue;
-                const float *k_tile = block.K + tile * TILE * ROW, *q_tile = block.Q + tile * TILE * ROW;
-                const float *T = block.Ts + tile * TILE * SIDE, *P = block.Ps + tile * TILE * SIDE;
+                anew(g, c);
+                const float *k_tile = block.K + tile * TILE * block.ROW, *q_tile = block.Q + tile * TILE * block.ROW;
+                const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
+                float *const dot = dots + turn * DOTS * TILE * W;
                 Decays decay;
                 decay.load(block.as + tile * TILE, g);
                 const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
-                const bool cut = block.cut_ahead(tile);
+                f32x4 dS1[BOTH ? 1 : B];
                 // ---- by columns
-                f32x4 dU = zero;
-#pragma unroll
-                for (int i = 0; i < B; ++i) dU = mfma16(*reinterpret_cast<const f32x4 *>(k_tile + c * ROW + i * TILE + 4 * g), dS[i], dU);
-                f32x4 p_column, t_column;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    dU[r] *= decay.to[r] * ks[r];
-                    p_column[r] = P[(4 * g + r) * SIDE + c];
-                    t_column[r] = T[(4 * g + r) * SIDE + c];
-                }
-                dU = mfma16(p_column, dO[tile], dU);
-                const f32x4 dX = mfma16(t_column, dU, zero);
-                float s_ds = 0.0f;
-#pragma unroll
-                for (int i = 0; i < B; ++i)
+                if (owns) {
+                    f32x4 out = ask(block, block.Q, tile, g, c, kept[tile]), e;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        s_ds = fmaf(kept[tile][i][r], dS[i][r], s_ds);
-                        state[(i * TILE + 4 * g + r) * columns + column] = kept[tile][i][r];
+                        out[r] *= decay.from[r] * qs[r];
+                        e[r] = dO[tile][r] * out[r];
                     }
-                s_ds = sum_groups(sum16(s_ds));
-                if (lane == 0) whole[w] = s_ds;
-                f32x4 q_part, k_part;
+                    out = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + (tile * TILE + c) * SIDE + 4 * g), U[tile], out);
+                    float s_ds = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int slot = tile * TILE + 4 * g + r, at = (4 * g + r) * columns + column;
-                    dOs[at] = dO[tile][r];
-                    dXs[at] = dX[r];
-                    Us[at] = U[tile][r];
-                    if (live && block.there(d, slot)) give((E *)p.value + ((long)block.time_of(slot) * d.N + n) * p.value_ld + h * d.dv + column, b[r] * dX[r]);
-                    q_part[r] = decay.from[r] * qs[r] * dO[tile][r];
-                    k_part[r] = -decay.from[r] * ks[r] * b[r] * dX[r];
-                }
-                f32x4 dS0[B];
+                    for (int i = 0; i < B; ++i)
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    f32x4 q, k;
+                        for (int r = 0; r < 4; ++r) s_ds = fmaf(kept[tile][i][r], dS[i][r], s_ds);
+                    s_ds = sum_groups(sum16(s_ds));
+                    if (lane == 0) wholes[turn * W + w] = s_ds;
+                    spread(states, kept[tile]);
+                    if constexpr (BOTH) spread(behind, dS);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < B; ++i) dS1[i] = dS[i];
+                    }
+                    f32x4 read, dX;
+                    pull(block, decay, tile, g, c, dO[tile], dS, read, dX);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        q[r] = q_tile[(4 * g + r) * ROW + i * TILE + c];
-                        k[r] = k_tile[(4 * g + r) * ROW + i * TILE + c];
+                        const int slot = tile * TILE + 4 * g + r, at = (4 * g + r) * stride + column;
+                        dOs[at] = dO[tile][r];
+                        dXs[at] = dX[r];
+                        Us[at] = U[tile][r];
+                        if (live && block.there(d, slot)) give((E *)p.value + ((long)block.time_of(slot) * d.N + n) * p.value_ld + h * d.dv + column, b[r] * dX[r]);
+                        const float sums[DOTS] = {sum16(dO[tile][r] * out[r]), sum16(dX[r] * fmaf(2.0f, U[tile][r], -b[r] * V[tile][r])), sum16(fmaf(-dX[r], reads[tile][r], e[r])),
+                                                  sum16(U[tile][r] * read[r]), sum16(U[tile][r] * dX[r])};
+                        if (c == 0) {
+#pragma unroll
+                            for (int k = 0; k < DOTS; ++k) dot[(k * W + w) * TILE + 4 * g + r] = sums[k];
+                        }
                     }
-                    dS0[i] = mfma16(k, k_part, mfma16(q, q_part, dS[i] * decay.whole));
-                    if (cut) dS0[i] = zero;
                 }
                 __syncthreads();
-                // ---- by rows of S0: the terms of dq and dk with it; by the first wavefront, dA and dP
-                f32x4 dq[B], dk_reads[B], dk_read[B];   // of which this wavefront has every W-th
+                // ---- by rows of the states, their terms of dq and dk; by one wavefront, dA and dP
+                f32x4 dq[OWN], dk[OWN];
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    dq[i] = dk_reads[i] = dk_read[i] = zero;
-                    if (i % W != w) continue;
-                    for (int t = 0; t < W; ++t) {
-                        const f32x4 s = *reinterpret_cast<const f32x4 *>(state + (i * TILE + c) * columns + t * TILE + 4 * g);
-                        dq[i] = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * columns + t * TILE + 4 * g), s, dq[i]);
-                        dk_reads[i] = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * columns + t * TILE + 4 * g), s, dk_reads[i]);
+                for (int o = 0; o < OWN; ++o) {
+                    const int i = w + o * W;
+                    dq[o] = dk[o] = zero;
+                    if (i >= B) continue;
+                    f32x4 of = zero;
+                    for (int t = 0; t < tiles; ++t) {
+                        const f32x4 s = *reinterpret_cast<const f32x4 *>(states + (i * TILE + c) * stride + t * TILE + 4 * g);
+                        dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), s, dq[o]);
+                        dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), s, dk[o]);
+                        if constexpr (BOTH)
+                            of = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
+                                        *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), of);
                     }
-                }
-                f32x4 eq = zero, ek = zero, fk = zero;
-#pragma unroll
-                for (int i = 0; i < B; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        dq[i][r] *= decay.from[r];
-                        dk_reads[i][r] *= -decay.from[r] * b[r];
-                        if (i % W != w) continue;
-                        eq[r] = fmaf(q_tile[(4 * g + r) * ROW + i * TILE + c] * qs[r], dq[i][r], eq[r]);
-                        ek[r] = fmaf(k_tile[(4 * g + r) * ROW + i * TILE + c] * ks[r], dk_reads[i][r], ek[r]);
+                        dq[o][r] *= decay.from[r];
+                        dk[o][r] = fmaf(decay.to[r], of[r], -decay.from[r] * b[r] * dk[o][r]);
                     }
-                f32x4 a_terms = zero, p_terms = zero;   // dA A and dP P
-                if (w == 0) {
+                }
+                if (w == pairs_by) {
                     f32x4 dA = zero, dP = zero;
-                    for (int t = 0; t < W; ++t) {
-                        const f32x4 u = *reinterpret_cast<const f32x4 *>(Us + c * columns + t * TILE + 4 * g);
-                        dA = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * columns + t * TILE + 4 * g), u, dA);
-                        dP = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * columns + t * TILE + 4 * g), u, dP);
+                    for (int t = 0; t < tiles; ++t) {
+                        const f32x4 u = *reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g);
+                        dA = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), u, dA);
+                        dP = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), u, dP);
                     }
                     const f32x4 apart = between(block.as + tile * TILE, g, c);
-                    f32x4 kk = zero, qk = zero;
-#pragma unroll
-                    for (int i = 0; i < B; ++i) {
-                        const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + c * ROW + i * TILE + 4 * g), q = *reinterpret_cast<const f32x4 *>(q_tile + c * ROW + i * TILE + 4 * g);
-                        kk = mfma16(k, k, kk);
-                        qk = mfma16(q, k, qk);
-                    }
-                    const float kc = block.kscale[tile * TILE + c];
+                    f32x4 both;   // dA A + dP P
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int i = 4 * g + r, slot = tile * TILE + i;
-                        if (i == c && block.there(d, slot))
-                            give((E *)p.rate + ((long)block.time_of(slot) * d.N + n) * p.rate_ld + h, block.rate_rests[slot] * dA[r]);
-                        const float a_times = i > c ? -dA[r] * b[r] * apart[r] : 0.0f, p_times = i >= c ? dP[r] * apart[r] : 0.0f;
-                        a_terms[r] = i > c ? a_times * (ks[r] * kc * kk[r]) : 0.0f;
-                        p_terms[r] = i >= c ? p_times * (qs[r] * kc * qk[r]) : 0.0f;
-                        dAs[i * SIDE + c] = a_times;
-                        dPs[i * SIDE + c] = p_times;
+                        const int i = 4 * g + r, at = (tile * TILE + i) * SIDE + c;
+                        const float a_times = i > c ? -dA[r] : 0.0f, p_times = i >= c ? dP[r] : 0.0f;
+                        both[r] = fmaf(a_times, block.As[at], p_times * block.Ps[at]);
+                        dAs[i * SIDE + c] = a_times * b[r] * apart[r];
+                        dPs[i * SIDE + c] = p_times * apart[r];
                     }
-                }
-                __syncthreads();
-                // ---- dS1 in S0's place
-#pragma unroll
-                for (int i = 0; i < B; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) state[(i * TILE + 4 * g + r) * columns + column] = dS[i][r];
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    dS[i] = dS0[i];
-                    if (i % W != w) continue;
-                    for (int t = 0; t < W; ++t)
-                        dk_read[i] = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * columns + t * TILE + 4 * g),
-                                            *reinterpret_cast<const f32x4 *>(state + (i * TILE + c) * columns + t * TILE + 4 * g), dk_read[i]);
-                    f32x4 k, q, a_column, p_column;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        dk_read[i][r] *= decay.to[r];
-                        k[r] = k_tile[(4 * g + r) * ROW + i * TILE + c] * ks[r];
-                        q[r] = q_tile[(4 * g + r) * ROW + i * TILE + c] * qs[r];
-                        fk[r] = fmaf(k[r], dk_read[i][r], fk[r]);
-                        a_column[r] = dAs[(4 * g + r) * SIDE + c];
-                        p_column[r] = dPs[(4 * g + r) * SIDE + c];
-                    }
-                    dq[i] = mfma16(*reinterpret_cast<const f32x4 *>(dPs + c * SIDE + 4 * g), k, dq[i]);
-                    dk_reads[i] = mfma16(*reinterpret_cast<const f32x4 *>(dAs + c * SIDE + 4 * g), k, dk_reads[i]);
-                    dk_read[i] = mfma16(p_column, q, mfma16(a_column, k, dk_read[i]));
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = sum16(eq[r]), y = sum16(ek[r]), z = sum16(fk[r]);
-                    if (c == 0) {
-                        dots[(0 * MOST_WAVES + w) * TILE + 4 * g + r] = x;
-                        dots[(1 * MOST_WAVES + w) * TILE + 4 * g + r] = y;
-                        dots[(2 * MOST_WAVES + w) * TILE + 4 * g + r] = z;
-                    }
-                }
-                float *sums = dAs;   // row i: what the dots of q and k take from the tile's own pairs
-                __syncthreads();
-                if (w == 0) {
-                    f32x4 both = a_terms + p_terms;
-                    float below = both[0] + both[1] + both[2] + both[3];   // rows of this column below the group's own
-                    const float from1 = __shfl(below, 16 + c), from2 = __shfl(below, 32 + c), from3 = __shfl(below, 48 + c), from0 = __shfl(below, c);
-                    const float read = from0 + from1 + from2 + from3;
-                    f32x4 crossing;
-                    float run = (g < 3 ? from3 : 0.0f) + (g < 2 ? from2 : 0.0f) + (g < 1 ? from1 : 0.0f);
-                    f32x4 a_row, p_row;
+                    // sums over the rows from 4 g + r on, and of these over the columns ahead
+                    const float mine = (both[0] + both[1]) + (both[2] + both[3]);
+                    const float of1 = __shfl(mine, 16 + c), of2 = __shfl(mine, 32 + c), of3 = __shfl(mine, 48 + c);
+                    float run = (g < 3 ? of3 : 0.0f) + (g < 2 ? of2 : 0.0f) + (g < 1 ? of1 : 0.0f);
 #pragma unroll
                     for (int r = 3; r >= 0; --r) {
                         run += both[r];
-                        crossing[r] = sum16(c < 4 * g + r ? run : 0.0f);
-                        a_row[r] = sum16(a_terms[r]);
-                        p_row[r] = sum16(p_terms[r]);
+                        const float sum = sum16(c < 4 * g + r ? run : 0.0f);
+                        if (c == 0) crossing[4 * g + r] = sum;
                     }
-                    if (c == 0) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            sums[0 * TILE + 4 * g + r] = p_row[r];
-                            sums[1 * TILE + 4 * g + r] = a_row[r];
-                            sums[3 * TILE + 4 * g + r] = crossing[r];
-                        }
-                    }
-                    if (g == 0) sums[2 * TILE + c] = read;
                 }
                 __syncthreads();
-                f32x4 q_dot = *reinterpret_cast<const f32x4 *>(sums + 4 * g), k_dot = *reinterpret_cast<const f32x4 *>(sums + TILE + 4 * g) + *reinterpret_cast<const f32x4 *>(sums + 2 * TILE + 4 * g);
-                for (int t = 0; t < W; ++t) {
-                    q_dot += *reinterpret_cast<const f32x4 *>(dots + (0 * MOST_WAVES + t) * TILE + 4 * g);
-                    k_dot += *reinterpret_cast<const f32x4 *>(dots + (1 * MOST_WAVES + t) * TILE + 4 * g) + *reinterpret_cast<const f32x4 *>(dots + (2 * MOST_WAVES + t) * TILE + 4 * g);
+                if constexpr (!BOTH) {   // dS1 in S0's place
+                    if (owns) spread(behind, dS1);
+                    __syncthreads();
+#pragma unroll
+                    for (int o = 0; o < OWN; ++o) {
+                        const int i = w + o * W;
+                        if (i >= B) continue;
+                        f32x4 of = zero;
+                        for (int t = 0; t < tiles; ++t)
+                            of = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
+                                        *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), of);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(decay.to[r], of[r], dk[o][r]);
+                    }
+                }
+                // ---- the tile's own pairs, the lengths, gates and rates
+                f32x4 q_dot = zero, k_dot = zero;
+                for (int t = 0; t < tiles; ++t) {
+                    q_dot += *reinterpret_cast<const f32x4 *>(dot + t * TILE + 4 * g);
+                    k_dot += *reinterpret_cast<const f32x4 *>(dot + (W + t) * TILE + 4 * g);
                 }
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
-                    if (i % W != w) continue;
+                for (int o = 0; o < OWN; ++o) {
+                    const int i = w + o * W;
+                    if (i >= B) continue;
+                    f32x4 k, q, a_column, p_column;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int slot = tile * TILE + 4 * g + r, at = i * TILE + c;
+                        k[r] = k_tile[(4 * g + r) * block.ROW + i * TILE + c] * ks[r];
+                        q[r] = q_tile[(4 * g + r) * block.ROW + i * TILE + c] * qs[r];
+                        a_column[r] = dAs[(4 * g + r) * SIDE + c];
+                        p_column[r] = dPs[(4 * g + r) * SIDE + c];
+                    }
+                    dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dPs + c * SIDE + 4 * g), k, dq[o]);
+                    dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dAs + c * SIDE + 4 * g), k, dk[o]);
+                    dk[o] = mfma16(p_column, q, mfma16(a_column, k, dk[o]));
+                    const int at = i * TILE + c;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int slot = tile * TILE + 4 * g + r;
                         if (at >= d.dk || !block.there(d, slot)) continue;
                         const long row = (long)block.time_of(slot) * d.N + n;
-                        const float q = q_tile[(4 * g + r) * ROW + at] * qs[r], k = k_tile[(4 * g + r) * ROW + at] * ks[r];
-                        give((EK *)p.query + row * p.query_ld + key_at + at, qs[r] * fmaf(-(float)d.dk * q, q_dot[r], dq[i][r]));
-                        give((EK *)p.key + row * p.key_ld + key_at + at, ks[r] * fmaf(-k, k_dot[r], dk_reads[i][r] + dk_read[i][r]));
+                        give((EK *)p.query + row * p.query_ld + key_at + at, qs[r] * fmaf(-(float)d.dk * q[r], q_dot[r], dq[o][r]));
+                        give((EK *)p.key + row * p.key_ld + key_at + at, ks[r] * fmaf(-k[r], k_dot[r], dk[o][r]));
                     }
                 }
-                if (w == 0 && lane < TILE && block.there(d, tile * TILE + lane)) {
-                    float sum = sums[3 * TILE + lane], all = 0.0f;
-                    for (int t = 0; t < W; ++t) {
-                        for (int j = 0; j < TILE; ++j)
-                            sum += j < lane ? dots[(2 * MOST_WAVES + t) * TILE + j] : dots[t * TILE + j] + dots[(1 * MOST_WAVES + t) * TILE + j];
-                        all += whole[t];
+                if (w == pairs_by && g == 0) {
+                    float e = 0.0f, f = 0.0f, u_dx = 0.0f, all = 0.0f;
+                    for (int t = 0; t < tiles; ++t) {
+                        e += dot[(2 * W + t) * TILE + c];
+                        f += dot[(3 * W + t) * TILE + c];
+                        u_dx += dot[(4 * W + t) * TILE + c];
+                        all += wholes[turn * W + t];
                     }
-                    sum = fmaf(decay.whole, all, sum);
-                    const int slot = tile * TILE + lane;
-                    give((E *)p.gate + ((long)block.time_of(slot) * d.N + n) * p.gate_ld + h, block.as[slot] == 0.0f ? 0.0f : block.rests[slot] * sum);
+                    const float sum = fmaf(decay.whole, all, crossing[c] + (sum_from(e) + sum_ahead(f)));
+                    const int slot = tile * TILE + c;
+                    if (block.there(d, slot)) {
+                        const long row = (long)block.time_of(slot) * d.N + n;
+                        give((E *)p.gate + row * p.gate_ld + h, block.as[slot] == 0.0f ? 0.0f : block.rests[slot] * sum);
+                        give((E *)p.rate + row * p.rate_ld + h, block.rate_rests[slot] * u_dx);
+                    }
                 }
-                __syncthreads();
+                if constexpr (!BOTH) __syncthreads();
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
-    if (p.state == nullptr || !live) return;
+    if (p.state == nullptr || !live || part != 0) return;
 #pragma unroll
     for (int i = 0; i < B; ++i)
 #pragma unroll
@@ -382,22 +484,42 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(const float *from, int64
 }
 
 struct Plan {
+    Parts parts;
     int blocks;
-    size_t states, partial;   // bytes
+    size_t states, partial, ends, starts, grads, cuts, bytes;   // bytes: of the states ahead of the blocks, the groups' gradients, what the parts take, all
 };
-Plan plan_of(const mrl_delta *r) {
+Plan plan_of(const mrl_ctx *ctx, const mrl_delta *r) {
     Plan p = {};
     if (r->T == 0 || r->N == 0) return p;
-    p.blocks = blocks_of(r->T, r->key_dim);
-    if (p.blocks > 1) p.states = sizeof(float) * (size_t)r->N * r->heads * p.blocks * column_tiles(r->value_dim) * TILE * padded(r->key_dim);
+    const int tiles = tiles_backward(padded(r->key_dim));
+    p.parts = parts_of(ctx, r, tiles);
+    p.blocks = blocks_of(r->T, tiles);
+    if (p.blocks > 1) p.states = sizeof(float) * (size_t)r->N * r->heads * p.blocks * column_tiles(r->value_dim) * floats_of(padded(r->key_dim));
     if (r->heads != r->key_heads) p.partial = (sizeof(float) * (size_t)r->T * r->N * r->heads * r->key_dim + 15) / 16 * 16;
+    p.ends = sizeof(float) * ends_floats(r, p.parts);
+    p.starts = p.grads = sizeof(float) * starts_floats(r, p.parts);
+    p.cuts = sizeof(float) * cuts_floats(r, p.parts);
+    p.bytes = p.states + 2 * p.partial + p.ends + 2 * p.starts + p.grads + p.cuts;
     return p;
 }
 
 template <class E, class EK, int DK>
 void launch(const mrl_ctx *ctx, const Back &p) {
-    const int W = column_tiles(p.d.dv);
-    hipLaunchKernelGGL((back_kernel<E, EK, DK>), dim3(p.d.N * p.d.H), dim3(64 * W), sizeof(float) * back_floats(DK, W), ctx->stream, p);
+    hipLaunchKernelGGL((back_kernel<E, EK, DK>), dim3(p.d.N * p.d.H * p.parts.count), dim3(64 * waves_of(DK, p.d.dv)), sizeof(float) * back_floats(DK, p.d.dv), ctx->stream, p);
+}
+template <class E, int DK>
+void launch_chain(const mrl_ctx *ctx, const Back &p) {
+    const int tiles = column_tiles(p.d.dv), waves = std::min(4, tiles), groups = (tiles + waves - 1) / waves;
+    hipLaunchKernelGGL((chain_kernel<E, DK>), dim3(p.d.N * p.d.H * p.parts.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, tiles_backward(DK)), ctx->stream, p, groups);
+}
+template <class E>
+void launch_chain(const mrl_ctx *ctx, const Back &p) {
+    switch (padded(p.d.dk)) {
+        case 16: return launch_chain<E, 16>(ctx, p);
+        case 32: return launch_chain<E, 32>(ctx, p);
+        case 64: return launch_chain<E, 64>(ctx, p);
+        default: return launch_chain<E, 128>(ctx, p);
+    }
 }
 template <class E, class EK>
 void launch(const mrl_ctx *ctx, const Back &p) {
@@ -436,8 +558,7 @@ int mrl_delta_workspace(mrl_ctx *ctx, const mrl_delta *r, int backward, uint64_t
     MRL_CHECK_ARG(ctx && r && bytes, "mrl_delta_workspace: NULL ctx, description or result");
     const int rc = delta::check_sizes("mrl_delta_workspace", r);
     if (rc != MRL_OK) return rc;
-    const delta::Plan p = backward ? delta::plan_of(r) : delta::Plan{};
-    *bytes = p.states + 2 * p.partial;
+    *bytes = backward ? delta::plan_of(ctx, r).bytes : delta::forward_bytes(ctx, r);
     return MRL_OK;
 }
 
@@ -452,8 +573,8 @@ int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, i
     if (r->N == 0) return MRL_OK;
     const mrl_delta_grads &to = *grads;
     const long states = (long)r->N * r->heads * r->key_dim * r->value_dim, k_width = (long)r->key_heads * r->key_dim, v_width = (long)r->heads * r->value_dim;
-    const Plan plan = plan_of(r);
-    const size_t need = plan.states + 2 * plan.partial;
+    const Plan plan = plan_of(ctx, r);
+    const size_t need = plan.bytes;
     if (r->T > 0) {
         MRL_CHECK_ARG(grad_out && to.query && to.key && to.value && to.gate && to.rate, "%s: NULL buffer", who);
         MRL_CHECK_ARG(grad_out_ld >= v_width && to.query_ld >= k_width && to.key_ld >= k_width && to.value_ld >= v_width && to.gate_ld >= r->heads && to.rate_ld >= r->heads,
@@ -487,12 +608,33 @@ int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, i
     p.query_ld = to.query_ld; p.key_ld = to.key_ld; p.value_ld = to.value_ld; p.gate_ld = to.gate_ld; p.rate_ld = to.rate_ld;
     p.state = to.state;
     p.blocks = plan.blocks;
-    p.states = plan.states ? (const float *)workspace : nullptr;
-    if (plan.blocks > 1) {
-        const int launched = launch_states(ctx, r->dtype, p.d, (float *)workspace, plan.blocks);
+    p.parts = plan.parts;
+    char *at = (char *)workspace;
+    const auto take = [&](size_t bytes) {
+        char *const was = bytes ? at : nullptr;
+        at += bytes;
+        return (float *)was;
+    };
+    float *const ahead = take(plan.states), *const partial = take(2 * plan.partial), *const grad_ends = take(plan.grads);
+    p.parts.ends = take(plan.ends);
+    p.parts.starts = take(plan.starts);
+    p.local = take(plan.grads);
+    p.parts.cuts = (int *)take(plan.cuts);
+    p.states = ahead;
+    p.grad_ends = grad_ends;
+    int launched = MRL_OK;
+    if (plan.parts.count > 1) {
+        launched = launch_starts(ctx, r->dtype, p.d, p.parts);
+        if (launched != MRL_OK) return launched;
+        if (r->dtype == MRL_F32) launch_chain<float>(ctx, p);
+        else launch_chain<bf16_t>(ctx, p);
+        Parts ends = p.parts;
+        ends.starts = grad_ends;
+        launched = launch_grad_ends(ctx, p.d, ends, grad_state_out, p.local);
         if (launched != MRL_OK) return launched;
     }
-    float *const partial = plan.partial ? (float *)((char *)workspace + plan.states) : nullptr;
+    if (plan.blocks > 1) launched = launch_states(ctx, r->dtype, p.d, p.parts, ahead, plan.blocks);
+    if (launched != MRL_OK) return launched;
     if (r->dtype == MRL_F32) launch<float>(ctx, p, partial, plan.partial);
     else launch<bf16_t>(ctx, p, partial, plan.partial);
     MRL_CHECK_LAUNCH();

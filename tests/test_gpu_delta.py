@@ -127,7 +127,9 @@ def near(got, want, heads, off, half, what, size=None):
 SHAPES = [(1, 1, 1, 1, 1, 1), (1, 5, 2, 2, 64, 64), (1, 3, 4, 2, 128, 128), (1, 7, 3, 1, 40, 24), (1, 2, 2, 1, 33, 65), (1, 9, 1, 1, 7, 5),
           (2, 3, 2, 2, 16, 16), (3, 2, 3, 3, 5, 3), (15, 2, 2, 1, 32, 32), (16, 3, 2, 2, 64, 64), (17, 1, 4, 4, 64, 48), (33, 2, 6, 2, 24, 40),
           (64, 2, 2, 2, 64, 64), (65, 3, 2, 1, 128, 128), (32, 1, 1, 1, 128, 16), (33, 2, 2, 2, 100, 17), (130, 2, 3, 1, 40, 24), (129, 1, 2, 2, 17, 128),
-          (200, 3, 2, 2, 64, 64), (300, 1, 2, 1, 128, 100), (97, 40, 1, 1, 16, 80), (70, 5, 3, 3, 1, 1)]
+          (200, 3, 2, 2, 64, 64), (300, 1, 2, 1, 128, 100), (97, 40, 1, 1, 16, 80), (70, 5, 3, 3, 1, 1),
+          # long rollouts of few environments, which go in parts
+          (1000, 1, 1, 1, 8, 8), (700, 2, 3, 1, 24, 40), (600, 1, 2, 2, 64, 64), (500, 2, 1, 1, 128, 72), (1030, 3, 1, 1, 40, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -162,7 +164,7 @@ def test_backward(mrl, ctx, T, N, heads, key_heads, dk, dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("T,N,heads,dk,dv", [(40, 3, 2, 20, 24), (70, 2, 1, 64, 64), (90, 2, 2, 128, 40)])
+@pytest.mark.parametrize("T,N,heads,dk,dv", [(40, 3, 2, 20, 24), (70, 2, 1, 64, 64), (90, 2, 2, 128, 40), (400, 2, 1, 64, 20), (330, 2, 2, 128, 16)])
 def test_what_a_cut_hides(mrl, ctx, T, N, heads, dk, dv, dtype):
     """Infinities and NaN in a first state, in keys, values and gates, in output gradients: nothing behind (backwards: ahead of) a cut
     changes, nor do other environments, and steps ahead of a value that is not finite come out as they do without it."""
