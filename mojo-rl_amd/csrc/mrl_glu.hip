@@ -81,10 +81,11 @@ struct Source {
     long ld;
     int rows, columns;   // columns: of gate and up each where they alternate
 };
-// Fragments of its rows, contracted along its columns; PAIRED: gate and up alternate by 16 columns.  A wavefront a fragment.
+// Fragments of its rows, contracted along its columns; PAIRED: gate and up alternate by 16 columns.  A wavefront a fragment, number `at` of
+// row_fragments * blocks.
 template <class E, int P, bool PAIRED>
-__global__ __launch_bounds__(256) void along_rows_kernel(Source s, __bf16 *to, int row_fragments, int blocks) {
-    const long fragment = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+MRL_DEV void along_rows(const Source &s, __bf16 *to, int row_fragments, int blocks, long at) {
+    const long fragment = at * 4 + (threadIdx.x >> 6);
     if (fragment >= (long)row_fragments * blocks) return;
     const int lane = threadIdx.x & 63, block = (int)(fragment / row_fragments), row = (int)(fragment - (long)block * row_fragments) * 16 + (lane & 15), g = lane >> 4;
     const int column = PAIRED ? block * 16 + (g & 1) * 8 : block * 32 + g * 8;
@@ -93,29 +94,48 @@ __global__ __launch_bounds__(256) void along_rows_kernel(Source s, __bf16 *to, i
 }
 // Fragments of its columns, contracted along its rows.  A workgroup 32 rows and 64 columns, turned in LDS.
 template <class E, int P, bool PAIRED>
-__global__ __launch_bounds__(256) void along_columns_kernel(Source s, __bf16 *to, int column_fragments) {
-    __shared__ float tile[64][33];
-    const int across = PAIRED ? 32 : 64, block = blockIdx.y, first = blockIdx.x * across;   // (PAIRED: 32 columns of each)
-    for (int i = threadIdx.x; i < 32 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63, row = block * 32 + r;
+MRL_DEV void along_columns(const Source &s, __bf16 *to, int column_fragments, long at, float (&tile)[64][33]) {
+    const int groups = (column_fragments + 3) / 4, block = (int)(at / groups), group = (int)(at - (long)block * groups), first = group * (PAIRED ? 32 : 64);   // (PAIRED: 32 of each)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63, row = block * 32 + r;
         // fragments in order: PAIRED has gate 0 .. 15, up 0 .. 15, gate 16 .. 31, up 16 .. 31
         const int column = PAIRED ? first + (c >> 5) * 16 + (c & 15) : first + c;
         const bool there = row < s.rows && column < s.columns;
-        tile[c][r] = there ? value_of(((const E *)s.at)[row * s.ld + column + (PAIRED && (c & 16) ? s.columns : 0)]) : 0.0f;
+        const float x = value_of(((const E *)s.at)[there ? row * s.ld + column + (PAIRED && (c & 16) ? s.columns : 0) : 0]);
+        tile[c][r] = there ? x : 0.0f;
     }
     __syncthreads();
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, fragment = blockIdx.x * 4 + w;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, fragment = group * 4 + w;
     if (fragment >= column_fragments) return;
     f32x8 x;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = tile[w * 16 + (lane & 15)][(lane >> 4) * 8 + i];
     put_pieces<P>(x, to + ((long)block * column_fragments + fragment) * P * KIB, lane);
 }
+// All operands that a call takes from its inputs, one launch: the rows and columns of x, the columns and rows of W, those that are wanted.
+struct Operands {
+    Source x, w;
+    __bf16 *x_rows, *x_columns, *w_columns, *w_rows;
+    int x_row_fragments, x_column_fragments, w_column_fragments, w_row_fragments;
+    unsigned end[4];   // workgroups up to and with each
+};
+template <class E, int P>
+__global__ __launch_bounds__(256) void operands_kernel(Operands o) {
+    __shared__ float tile[64][33];
+    const unsigned b = blockIdx.x;
+    if (b < o.end[0]) along_columns<E, P, true>(o.w, o.w_columns, o.w_column_fragments, b, tile);
+    else if (b < o.end[1]) along_rows<E, P, false>(o.x, o.x_rows, o.x_row_fragments, (o.x_column_fragments + 1) / 2, b - o.end[0]);
+    else if (b < o.end[2]) along_columns<E, P, false>(o.x, o.x_columns, o.x_column_fragments, b - o.end[1], tile);
+    else along_rows<E, P, true>(o.w, o.w_rows, o.w_row_fragments, o.w_column_fragments / 2, b - o.end[2]);
+}
 
 // ---------------------------------------------------------------- products
 struct Operand {
     const __bf16 *at;
     int fragments;   // of 16 rows
+    int rows;        // of a matrix of bf16 that is read as it is, `ld` apart
+    long ld;
 };
 
 // a wavefront's KiB from memory to LDS
@@ -144,7 +164,8 @@ struct Shape {
     static_assert(STAGE % 8 == 0 && LDS <= 160 * 1024, "whole loads that fit");
 };
 
-template <class S>
+// AS_IS: A is a matrix of bf16 whose rows are whole 32 elements and start at 16 bytes: lanes read their eight elements where they are.
+template <class S, bool AS_IS = false>
 MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int from, int to, __bf16 *lds, f32x4 (&acc)[S::FA][S::FB]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave / S::WC, column = wave % S::WC;
     // which KiB of a stage this wavefront brings: A's first, then B's; a tile at the edge reads the last fragments again
@@ -157,8 +178,13 @@ MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int fr
         const int in = of_a ? k : k - S::ROWS * S::PA, pieces = of_a ? S::PA : S::PB;
         const Operand &o = of_a ? a : b;
         const int fragment = min((of_a ? bi * S::ROWS : bj * S::COLUMNS) + in / pieces, o.fragments - 1);
-        step[l] = (long)o.fragments * pieces * KIB;
-        src[l] = o.at + ((long)fragment * pieces + in % pieces) * KIB + from * step[l] + lane * 8;
+        if (AS_IS && of_a) {
+            step[l] = 32;
+            src[l] = a.at + min(fragment * 16 + (lane & 15), a.rows - 1) * a.ld + from * 32 + (lane >> 4) * 8;
+        } else {
+            step[l] = (long)o.fragments * pieces * KIB;
+            src[l] = o.at + ((long)fragment * pieces + in % pieces) * KIB + from * step[l] + lane * 8;
+        }
     }
     const auto ask = [&](int stage) {
         __bf16 *const base = lds + (stage % S::BUFFERS * S::STAGE + wave * S::LOADS) * KIB;
@@ -207,6 +233,21 @@ MRL_DEV int tile_number(int tiles) {
     return xcd * whole + min(xcd, rest) + (blockIdx.x >> 3);
 }
 
+// 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
+// lanes away, then halves one lane away.
+MRL_DEV bf16x4 quad_transpose(bf16x4 v) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 d = __builtin_bit_cast(u32x2, v);
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    const unsigned away = __builtin_amdgcn_mov_dpp(high ? d[0] : d[1], 0x4E, 0xF, 0xF, true);
+    if (high) d[0] = away;
+    else d[1] = away;
+    const unsigned pick = odd ? 0x03020706u : 0x05040100u;   // bytes: 0 .. 3 of the own word, 4 .. 7 of the neighbour's
+#pragma unroll
+    for (int i = 0; i < 2; ++i) d[i] = __builtin_amdgcn_perm(__builtin_amdgcn_mov_dpp(d[i], 0xB1, 0xF, 0xF, true), d[i], pick);
+    return __builtin_bit_cast(bf16x4, d);
+}
+
 enum { SIGMOID = MRL_GATE_SIGMOID, SILU = MRL_GATE_SILU, GELU = MRL_GATE_GELU, TANH = MRL_GATE_TANH };
 
 MRL_DEV float activation(int act, float g) {
@@ -244,12 +285,12 @@ struct Layer {
 
 // FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
 // (PC pieces, for dW), and the sums of its columns over the wavefront's rows.
-template <class E, class S, bool FORWARD, int PR, int PC>
+template <class E, class S, bool FORWARD, bool AS_IS, int PR, int PC>
 __global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b, int row_tiles, int column_tiles, int blocks, __bf16 *rows, __bf16 *columns, float *sums) {
     extern __shared__ __bf16 lds[];
     const int tile = tile_number(row_tiles * column_tiles), bi = tile / column_tiles, bj = tile - bi * column_tiles;
     f32x4 acc[S::FA][S::FB] = {};
-    multiply<S>(a, b, bi, bj, 0, blocks, lds, acc);
+    multiply<S, AS_IS>(a, b, bi, bj, 0, blocks, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
     const E *const bias = (const E *)y.params + (long)y.K * 2 * y.N;
     const int fragments = b.fragments;   // of gate and up
@@ -290,11 +331,9 @@ __global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b,
 #pragma unroll
                     for (int k = 0; k < PC; ++k) *reinterpret_cast<bf16x4 *>(to + k * KIB) = p[k];
                     // by rows: a fragment of 16 rows and 32 columns, 16 of the gate and 16 of up
-                    __bf16 *at = rows + ((long)(f >> 1) * a.fragments + fragment) * PR * KIB + (16 * ((f & 1) * 2 + (c >> 3)) + 4 * g) * 8 + (c & 7);
+                    __bf16 *at = rows + ((long)(f >> 1) * a.fragments + fragment) * PR * KIB + (16 * ((f & 1) * 2 + (c >> 3)) + 4 * g + (c & 3)) * 8 + (c & 4);
 #pragma unroll
-                    for (int k = 0; k < PR; ++k)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) at[k * KIB + r * 8] = p[k][r];
+                    for (int k = 0; k < PR; ++k) *reinterpret_cast<bf16x4 *>(at + k * KIB) = quad_transpose(p[k]);
                 };
                 put(dg, 2 * pair);
                 put(du, 2 * pair + 1);
@@ -355,22 +394,33 @@ __global__ __launch_bounds__(512) void grad_w_kernel(int K, int N, Operand a, Op
             }
 }
 
-// the parts of dW added up, in order, and the biases' gradients from the sums of rows of wavefronts
-__global__ __launch_bounds__(256) void finish_kernel(const float *parts, int count, long values, const float *sums, int rows, int fragments, int N, float *grads) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i < values) {
-        if (count > 1) {
-            float sum = parts[i];
-            for (int p = 1; p < count; ++p) sum += parts[p * values + i];
-            grads[i] = sum;
-        }
-    } else if (i < values + 2 * N) {
-        const int column = (int)(i - values), up = column >= N, of = up ? column - N : column;
-        const float *p = sums + ((of >> 4) * 2 + up) * 16 + (of & 15);
+// The biases' gradients from the sums of rows of wavefronts, by the first workgroups, 64 columns each; the parts of dW added up, in order, by the others.
+__global__ __launch_bounds__(256) void finish_kernel(const float *parts, int count, long values, const float *sums, int rows, int columns, int N, float *grads) {
+    __shared__ float shared[4][64];
+    const int bias_blocks = (columns + 63) / 64;
+    if ((int)blockIdx.x < bias_blocks) {
+        const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, at = blockIdx.x * 64 + lane;
         float sum = 0.0f;
-        for (int r = 0; r < rows; ++r) sum += p[(long)r * fragments * 16];
-        grads[i] = sum;
+        if (at < columns) {
+            float some[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = w; r < rows; r += 16)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r + 4 * i < rows) some[i] += sums[(long)(r + 4 * i) * columns + at];
+            sum = (some[0] + some[1]) + (some[2] + some[3]);
+        }
+        shared[w][lane] = sum;
+        __syncthreads();
+        const int column = (at >> 5) * 16 + (at & 15);
+        if (w == 0 && at < columns && column < N)
+            grads[values + (at & 16 ? N : 0) + column] = (shared[0][lane] + shared[1][lane]) + (shared[2][lane] + shared[3][lane]);
+        return;
     }
+    const long i = (long)(blockIdx.x - bias_blocks) * 256 + threadIdx.x;
+    if (i >= values) return;
+    float sum = parts[i];
+    for (int p = 1; p < count; ++p) sum += parts[p * values + i];
+    grads[i] = sum;
 }
 
 // ---------------------------------------------------------------- few rows
@@ -432,15 +482,19 @@ inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
 // Where things lie in the workspace, in bytes.
 struct Plan {
     int M16, K16, N16;   // fragments of the rows, of the matrix' rows and (pairs) of its columns, an even number of the first two
-    int pieces, row_pieces, column_pieces, parts, sum_rows;
+    int pieces, row_pieces, column_pieces, parts;
     size_t x_rows, w_columns, x_columns, w_rows, pre_rows, pre_columns, sums, partial, bytes;
 };
 template <class S>
 int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
 
-typedef Shape<1, 1, 2, 4, 4, 4> Bf16Shape;        // 128 x 256
+// 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.
+typedef Shape<1, 1, 2, 4, 4, 3> Bf16Shape;
+typedef Shape<1, 1, 4, 1, 2, 4> Bf16Small;
 typedef Shape<1, 2, 2, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
-typedef Shape<3, 3, 2, 4, 2, 3> F32Shape;         // 128 x 128
+typedef Shape<3, 3, 2, 4, 2, 3> F32Shape;
+typedef Shape<3, 3, 4, 1, 2, 3> F32Small;
+constexpr int WR_MOST = 4;
 
 Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) {
     Plan p = {};
@@ -466,9 +520,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.w_rows = fragments(p.K16, 2L * p.N16, p.pieces);
         p.pre_rows = fragments(p.M16, 2L * p.N16, p.row_pieces);
         p.pre_columns = fragments(2L * p.N16, p.M16, p.column_pieces);
-        const int row_tiles = f32 ? (p.M16 + F32Shape::ROWS - 1) / F32Shape::ROWS : (p.M16 + Bf16Shape::ROWS - 1) / Bf16Shape::ROWS;
-        p.sum_rows = row_tiles * (f32 ? F32Shape::WR : Bf16Shape::WR);
-        p.sums = take(sizeof(float) * (size_t)p.sum_rows * 2 * p.N16 * 16);
+        p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
         const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16GradShape>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
@@ -478,45 +530,80 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
     return p;
 }
 
-template <class E, int P, bool PAIRED>
-void along_rows(const mrl_ctx *ctx, const Source &s, void *to, int row_fragments, int blocks) {
-    const long all = (long)row_fragments * blocks;
-    hipLaunchKernelGGL((along_rows_kernel<E, P, PAIRED>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, ctx->stream, s, (__bf16 *)to, row_fragments, blocks);
-}
-template <class E, int P, bool PAIRED>
-void along_columns(const mrl_ctx *ctx, const Source &s, void *to, int column_fragments, int blocks) {
-    hipLaunchKernelGGL((along_columns_kernel<E, P, PAIRED>), dim3((column_fragments + 3) / 4, blocks), dim3(256), 0, ctx->stream, s, (__bf16 *)to, column_fragments);
-}
+template <class E, class S, int P, int PR, int PC>
+struct Launch {
+    static dim3 grid(long a, long b) { return dim3((unsigned)tiles<S>(a, b)); }
+    static int down(long fragments) { return (int)((fragments + S::ROWS - 1) / S::ROWS); }
+    static int across(long fragments) { return (int)((fragments + S::COLUMNS - 1) / S::COLUMNS); }
+    static void forward(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is) {
+        const dim3 tiles = grid(p.M16, 2L * p.N16);
+        if constexpr (P == 1) {
+            if (as_is) {
+                hipLaunchKernelGGL((pre_kernel<E, S, true, true, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, down(p.M16), across(2L * p.N16), p.K16 / 2, nullptr, nullptr, nullptr);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((pre_kernel<E, S, true, false, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, down(p.M16), across(2L * p.N16), p.K16 / 2, nullptr, nullptr, nullptr);
+    }
+    // the number of rows of sums
+    static int gradient(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is, __bf16 *rows, __bf16 *columns, float *sums) {
+        const dim3 tiles = grid(p.M16, 2L * p.N16);
+        const int row_tiles = down(p.M16), column_tiles = across(2L * p.N16);
+        bool done = false;
+        if constexpr (P == 1) {
+            if (as_is) {
+                hipLaunchKernelGGL((pre_kernel<E, S, false, true, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, row_tiles, column_tiles, p.K16 / 2, rows, columns, sums);
+                done = true;
+            }
+        }
+        if (!done) hipLaunchKernelGGL((pre_kernel<E, S, false, false, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, row_tiles, column_tiles, p.K16 / 2, rows, columns, sums);
+        return row_tiles * S::WR;
+    }
+    static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w) {
+        hipLaunchKernelGGL((grad_x_kernel<E, S>), grid(p.M16, p.K16), dim3(512), S::LDS, ctx->stream, y, pre, w, down(p.M16), across(p.K16), p.N16);
+    }
+};
 
-template <class E, class S, class SW, int P, int PR, int PC>
+template <class E, class S, class SMALL, class SW, int P, int PR, int PC>
 void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool backward) {
-    const Source x = {y.x, y.x_ld, y.M, y.K}, w = {y.params, 2L * y.N, y.K, y.N};
-    const Operand x_rows = {(const __bf16 *)(ws + p.x_rows), p.M16}, w_columns = {(const __bf16 *)(ws + p.w_columns), 2 * p.N16};
-    along_rows<E, P, false>(ctx, x, ws + p.x_rows, p.M16, p.K16 / 2);
-    along_columns<E, P, true>(ctx, w, ws + p.w_columns, 2 * p.N16, p.K16 / 2);
-    const auto grid = [](long a, long b) { return (a + S::ROWS - 1) / S::ROWS * ((b + S::COLUMNS - 1) / S::COLUMNS); };
-    const int row_tiles = (p.M16 + S::ROWS - 1) / S::ROWS, column_tiles = (2 * p.N16 + S::COLUMNS - 1) / S::COLUMNS;
-    const dim3 pre((unsigned)grid(p.M16, 2L * p.N16));
+    typedef Launch<E, S, P, PR, PC> Large;
+    typedef Launch<E, SMALL, P, PR, PC> Small;
+    const bool as_is = P == 1 && y.K % 32 == 0 && y.x_ld % 8 == 0 && reinterpret_cast<uintptr_t>(y.x) % 16 == 0;
+    const Operand x_rows = {as_is ? (const __bf16 *)y.x : (const __bf16 *)(ws + p.x_rows), p.M16, y.M, y.x_ld}, w_columns = {(const __bf16 *)(ws + p.w_columns), 2 * p.N16};
+    Operands o = {};
+    o.x = {y.x, y.x_ld, y.M, y.K};
+    o.w = {y.params, 2L * y.N, y.K, y.N};
+    o.x_rows = (__bf16 *)(ws + p.x_rows); o.w_columns = (__bf16 *)(ws + p.w_columns);
+    o.x_columns = (__bf16 *)(ws + p.x_columns); o.w_rows = (__bf16 *)(ws + p.w_rows);
+    o.x_row_fragments = p.M16; o.x_column_fragments = p.K16; o.w_column_fragments = 2 * p.N16; o.w_row_fragments = p.K16;
+    const auto column_blocks = [](long fragments, long blocks) { return (unsigned)((fragments + 3) / 4 * blocks); };
+    const auto row_blocks = [](long fragments, long blocks) { return (unsigned)((fragments * blocks + 3) / 4); };
+    o.end[0] = column_blocks(2L * p.N16, p.K16 / 2);
+    o.end[1] = o.end[0] + (as_is ? 0 : row_blocks(p.M16, p.K16 / 2));
+    o.end[2] = o.end[1] + (backward ? column_blocks(p.K16, p.M16 / 2) : 0);
+    o.end[3] = o.end[2] + (backward && y.grad_x ? row_blocks(p.K16, p.N16) : 0);
+    hipLaunchKernelGGL((operands_kernel<E, P>), dim3(o.end[3]), dim3(256), 0, ctx->stream, o);
+    const auto few = [&](long a, long b) { return tiles<S>(a, b) < ctx->n_cus; };
+    const bool pre_small = few(p.M16, 2L * p.N16);
     if (!backward) {
-        hipLaunchKernelGGL((pre_kernel<E, S, true, PR, PC>), pre, dim3(512), S::LDS, ctx->stream, y, x_rows, w_columns, row_tiles, column_tiles, p.K16 / 2, nullptr, nullptr, nullptr);
+        if (pre_small) Small::forward(ctx, y, p, x_rows, w_columns, as_is);
+        else Large::forward(ctx, y, p, x_rows, w_columns, as_is);
         return;
     }
-    along_columns<E, P, false>(ctx, x, ws + p.x_columns, p.K16, p.M16 / 2);
-    along_rows<E, P, true>(ctx, w, ws + p.w_rows, p.K16, p.N16);
-    hipLaunchKernelGGL((pre_kernel<E, S, false, PR, PC>), pre, dim3(512), S::LDS, ctx->stream, y, x_rows, w_columns, row_tiles, column_tiles, p.K16 / 2,
-                       (__bf16 *)(ws + p.pre_rows), (__bf16 *)(ws + p.pre_columns), (float *)(ws + p.sums));
-    const Operand pre_rows = {(const __bf16 *)(ws + p.pre_rows), p.M16}, pre_columns = {(const __bf16 *)(ws + p.pre_columns), 2 * p.N16};
-    const Operand x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
+    __bf16 *const rows = (__bf16 *)(ws + p.pre_rows), *const columns = (__bf16 *)(ws + p.pre_columns);
+    float *const sums = (float *)(ws + p.sums);
+    const int sum_rows = pre_small ? Small::gradient(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums) : Large::gradient(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums);
+    const Operand pre_rows = {rows, p.M16}, pre_columns = {columns, 2 * p.N16}, x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
     if (y.grad_x != nullptr) {
-        const int across = (p.K16 + S::COLUMNS - 1) / S::COLUMNS;
-        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3((unsigned)grid(p.M16, p.K16)), dim3(512), S::LDS, ctx->stream, y, pre_rows, w_rows, row_tiles, across, p.N16);
+        if (few(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows);
+        else Large::grad_x(ctx, y, p, pre_rows, w_rows);
     }
     const int down = (p.K16 + SW::ROWS - 1) / SW::ROWS, across = (2 * p.N16 + SW::COLUMNS - 1) / SW::COLUMNS;
     const long values = (long)y.K * 2 * y.N;
     float *const to = p.parts > 1 ? (float *)(ws + p.partial) : y.grads;
     hipLaunchKernelGGL((grad_w_kernel<SW>), dim3((unsigned)(down * across * p.parts)), dim3(512), SW::LDS, ctx->stream, y.K, y.N, x_columns, pre_columns, down, across, p.M16 / 2, p.parts, to);
-    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)((values + 2 * y.N + 255) / 256)), dim3(256), 0, ctx->stream, to, p.parts, values, (const float *)(ws + p.sums), p.sum_rows,
-                       2 * p.N16, y.N, y.grads);
+    const long blocks = (2L * p.N16 * 16 + 63) / 64 + (p.parts > 1 ? (values + 255) / 256 : 0);
+    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, to, p.parts, values, sums, sum_rows, 2 * p.N16 * 16, y.N, y.grads);
 }
 
 int check_sizes(const char *who, int dtype, int act, int64_t rows, int in_dim, int out_dim) {
@@ -573,8 +660,8 @@ int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_
         const dim3 grid((out_dim + 15) / 16, (rows + 15) / 16);
         if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
         else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
-    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
-    else launch<bf16_t, Bf16Shape, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, false);
+    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, false);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -607,8 +694,8 @@ int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in
     y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
     y.x = in; y.x_ld = in_ld; y.params = params; y.grad_out = grad_out; y.grad_out_ld = grad_out_ld;
     y.grad_x = grad_in; y.grad_x_ld = grad_in_ld; y.grads = grads;
-    if (dtype == MRL_F32) launch<float, F32Shape, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
-    else launch<bf16_t, Bf16Shape, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
+    if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
