@@ -153,19 +153,45 @@ MRL_DEV void meet() {
     asm volatile("" ::: "memory");
 }
 
-// The tile of a product: A's fragments times B's, PA and PB pieces each, by 8 wavefronts, WR along A and the others along B, FA x FB fragments
-// each.  A stage is 32 of the contracted index; BUFFERS of them are in LDS or on their way.
-template <int PA_, int PB_, int WR_, int FA_, int FB_, int BUFFERS_>
+// The tile of a product: A's fragments times B's, PA and PB pieces each, by WR wavefronts along A and WC along B, FA x FB fragments each.
+// A stage is 32 of the contracted index; BUFFERS of them are in LDS or on their way.
+template <int PA_, int PB_, int WR_, int WC_, int FA_, int FB_, int BUFFERS_>
 struct Shape {
-    static constexpr int PA = PA_, PB = PB_, WR = WR_, WC = 8 / WR_, FA = FA_, FB = FB_, BUFFERS = BUFFERS_;
+    static constexpr int PA = PA_, PB = PB_, WR = WR_, WC = WC_, WAVES = WR * WC, THREADS = 64 * WAVES, FA = FA_, FB = FB_, BUFFERS = BUFFERS_;
     static constexpr int ROWS = WR * FA, COLUMNS = WC * FB;   // fragments of the tile
-    static constexpr int STAGE = (ROWS * PA + COLUMNS * PB), LOADS = STAGE / 8;   // KiB, and those that a wavefront brings
+    static constexpr int STAGE = (ROWS * PA + COLUMNS * PB), LOADS = STAGE / WAVES;   // KiB, and those that a wavefront brings
     static constexpr size_t LDS = sizeof(__bf16) * KIB * STAGE * BUFFERS;
-    static_assert(STAGE % 8 == 0 && LDS <= 160 * 1024, "whole loads that fit");
+    static_assert(STAGE % WAVES == 0 && LDS <= 160 * 1024, "whole loads that fit");
 };
 
-// AS_IS: A is a matrix of bf16 whose rows are whole 32 elements and start at 16 bytes: lanes read their eight elements where they are.
-template <class S, bool AS_IS = false>
+// A product's tiles in order, a share of neighbouring ones to each of the eight XCDs, which workgroups are dealt to in turn.  ACROSS tiles of a row
+// are neighbours, then the same of the next row: the 64 tiles that an XCD works on together share few operands, which its L2 holds (all
+// columns of a row first: 4 MB of W go through the L2 for every row of tiles, and 32768 rows of 512 x 2048 in bf16 take a tenth longer).
+constexpr int ACROSS = 4;
+struct Tiles {
+    int down, across, parts;   // parts: of the contracted index
+    int blocks;                // 32 of it each
+    __host__ __device__ int count() const { return down * across * parts; }
+    MRL_DEV void place(int &bi, int &bj, int &part, int &from, int &to) const {
+        const int xcd = blockIdx.x & 7, share = count() >> 3, rest = count() & 7, number = xcd * share + min(xcd, rest) + (int)(blockIdx.x >> 3);
+        part = number / (down * across);
+        const int tile = number - part * down * across, group = tile / (down * ACROSS), in = tile - group * down * ACROSS, width = min(ACROSS, across - group * ACROSS);
+        bi = in / width;
+        bj = group * ACROSS + in - bi * width;
+        const int per = (blocks + parts - 1) / parts;
+        from = min(blocks, part * per);
+        to = min(blocks, from + per);
+    }
+};
+
+// The sums of a tile.  Operands arrive BUFFERS - 1 stages ahead.  AS_IS: A is a matrix of bf16 whose rows are whole 32 elements and start at
+// 16 bytes: lanes read their eight elements where they are.
+// What bounds it: LDS.  A stage of 128 x 256 in bf16 is 64 KiB read and 24 written, 700 cycles of LDS for 512 of the matrix cores; two
+// workgroups a CU have one finish a tile while the other multiplies.  32768 rows of 512 x 2048 in bf16 take 181 us, of which 16 stages'
+// loop is 100, the activation 19 and writing the outputs 27 at least (this card's library takes 161 us for the product alone); 256 x 256 by
+// eight wavefronts, one workgroup a CU, 228, or 208 with the next tile's operands asked for ahead of a tile's end, which is slower (188) at 128 x 256;
+// four wavefronts of 64 x 128 each 215.
+template <class S, bool AS_IS>
 MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int from, int to, __bf16 *lds, f32x4 (&acc)[S::FA][S::FB]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave / S::WC, column = wave % S::WC;
     // which KiB of a stage this wavefront brings: A's first, then B's; a tile at the edge reads the last fragments again
@@ -227,12 +253,6 @@ MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int fr
     }
 }
 
-// Tiles in order, a share of neighbouring ones to each of the eight XCDs, which workgroups are dealt to in turn.
-MRL_DEV int tile_number(int tiles) {
-    const int xcd = blockIdx.x & 7, whole = tiles >> 3, rest = tiles & 7;
-    return xcd * whole + min(xcd, rest) + (blockIdx.x >> 3);
-}
-
 // 4 x 4 halves of four neighbouring lanes, transposed: element c of lane s becomes element s of lane c.  Pairs change places two
 // lanes away, then halves one lane away.
 MRL_DEV bf16x4 quad_transpose(bf16x4 v) {
@@ -274,6 +294,52 @@ MRL_DEV void activation(int act, float g, float &value, float &slope) {
     }
 }
 
+// 16 x 16 of a matrix [rows, columns] from a result's registers (row 4 g + r, column c) and into them, 0 where it has none.  bf16 goes by
+// four neighbouring columns of a row, which four lanes turn among them.
+MRL_DEV void store_tile(float *p, long ld, const f32x4 v, int row, int column, int rows, int columns, int g, int c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (row + 4 * g + r < rows && column + c < columns) p[(row + 4 * g + r) * ld + column + c] = v[r];
+}
+MRL_DEV void store_tile(bf16_t *p, long ld, const f32x4 v, int row, int column, int rows, int columns, int g, int c) {
+    const u16x4u x = __builtin_bit_cast(u16x4u, quad_transpose(__builtin_convertvector(v, bf16x4)));
+    row += 4 * g + (c & 3);
+    column += c & 12;
+    if (row >= rows) return;
+    bf16_t *const to = p + row * ld + column;
+    if (column + 4 <= columns) *reinterpret_cast<u16x4u *>(to) = x;
+    else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (column + i < columns) to[i].bits = x[i];
+    }
+}
+MRL_DEV f32x4 load_tile(const float *p, long ld, int row, int column, int rows, int columns, int g, int c) {
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const bool there = row + 4 * g + r < rows && column + c < columns;
+        const float x = p[there ? (row + 4 * g + r) * ld + column + c : 0];
+        v[r] = there ? x : 0.0f;
+    }
+    return v;
+}
+MRL_DEV f32x4 load_tile(const bf16_t *p, long ld, int row, int column, int rows, int columns, int g, int c) {
+    row += 4 * g + (c & 3);
+    column += c & 12;
+    u16x4u x = {0, 0, 0, 0};
+    if (row < rows) {
+        const bf16_t *const from = p + row * ld + column;
+        if (column + 4 <= columns) x = *reinterpret_cast<const u16x4u *>(from);
+        else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (column + i < columns) x[i] = from[i].bits;
+        }
+    }
+    return __builtin_convertvector(quad_transpose(__builtin_bit_cast(bf16x4, x)), f32x4);
+}
+
 struct Layer {
     int M, K, N, act;
     const void *x, *params, *grad_out;
@@ -286,14 +352,15 @@ struct Layer {
 // FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
 // (PC pieces, for dW), and the sums of its columns over the wavefront's rows.
 template <class E, class S, bool FORWARD, bool AS_IS, int PR, int PC>
-__global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b, int row_tiles, int column_tiles, int blocks, __bf16 *rows, __bf16 *columns, float *sums) {
+__global__ __launch_bounds__(S::THREADS) void pre_kernel(Layer y, Operand a, Operand b, Tiles all, __bf16 *rows, __bf16 *columns, float *sums) {
     extern __shared__ __bf16 lds[];
-    const int tile = tile_number(row_tiles * column_tiles), bi = tile / column_tiles, bj = tile - bi * column_tiles;
-    f32x4 acc[S::FA][S::FB] = {};
-    multiply<S, AS_IS>(a, b, bi, bj, 0, blocks, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
     const E *const bias = (const E *)y.params + (long)y.K * 2 * y.N;
     const int fragments = b.fragments;   // of gate and up
+    int bi, bj, part, from, to;
+    all.place(bi, bj, part, from, to);
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S, AS_IS>(a, b, bi, bj, from, to, lds, acc);
 #pragma unroll
     for (int j = 0; j < S::FB; j += 2) {
         const int pair = (bj * S::COLUMNS + wc * S::FB + j) / 2, column = pair * 16 + c;
@@ -306,16 +373,17 @@ __global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b,
             const int fragment = bi * S::ROWS + wr * S::FA + i, row = fragment * 16 + 4 * g;
             if (fragment >= a.fragments) continue;
             if constexpr (FORWARD) {
+                f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (there && row + r < y.M)
-                        give((E *)y.out + (row + r) * y.out_ld + column, activation(y.act, acc[i][j][r] + bg) * (acc[i][j + 1][r] + bu));
+                for (int r = 0; r < 4; ++r) v[r] = activation(y.act, acc[i][j][r] + bg) * (acc[i][j + 1][r] + bu);
+                store_tile((E *)y.out, y.out_ld, v, fragment * 16, pair * 16, y.M, y.N, g, c);
             } else {
                 f32x4 dg, du;
+                const f32x4 grads = load_tile((const E *)y.grad_out, y.grad_out_ld, fragment * 16, pair * 16, y.M, y.N, g, c);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const bool inside = there && row + r < y.M;
-                    const float grad = inside ? value_of(((const E *)y.grad_out)[(row + r) * y.grad_out_ld + column]) : 0.0f;
+                    const float grad = grads[r];
                     float value, slope;
                     activation(y.act, acc[i][j][r] + bg, value, slope);
                     dg[r] = inside ? grad * (acc[i][j + 1][r] + bu) * slope : 0.0f;
@@ -355,43 +423,37 @@ __global__ __launch_bounds__(512) void pre_kernel(Layer y, Operand a, Operand b,
 
 // dx: rows times the matrix' rows
 template <class E, class S>
-__global__ __launch_bounds__(512) void grad_x_kernel(Layer y, Operand a, Operand b, int row_tiles, int column_tiles, int blocks) {
+__global__ __launch_bounds__(S::THREADS) void grad_x_kernel(Layer y, Operand a, Operand b, Tiles all) {
     extern __shared__ __bf16 lds[];
-    const int tile = tile_number(row_tiles * column_tiles), bi = tile / column_tiles, bj = tile - bi * column_tiles;
-    f32x4 acc[S::FA][S::FB] = {};
-    multiply<S>(a, b, bi, bj, 0, blocks, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
+    int bi, bj, part, from, to;
+    all.place(bi, bj, part, from, to);
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S, false>(a, b, bi, bj, from, to, lds, acc);
 #pragma unroll
     for (int i = 0; i < S::FA; ++i)
 #pragma unroll
         for (int j = 0; j < S::FB; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = (bi * S::ROWS + wr * S::FA + i) * 16 + 4 * g + r, column = (bj * S::COLUMNS + wc * S::FB + j) * 16 + c;
-                if (row < y.M && column < y.K) give((E *)y.grad_x + row * y.grad_x_ld + column, acc[i][j][r]);
-            }
+            store_tile((E *)y.grad_x, y.grad_x_ld, acc[i][j], (bi * S::ROWS + wr * S::FA + i) * 16, (bj * S::COLUMNS + wc * S::FB + j) * 16, y.M, y.K, g, c);
 }
 
 // dW, a share of the rows per workgroup where `parts` is more than 1: [part][K, 2 N]
 template <class S>
-__global__ __launch_bounds__(512) void grad_w_kernel(int K, int N, Operand a, Operand b, int row_tiles, int column_tiles, int blocks, int parts, float *to) {
+__global__ __launch_bounds__(S::THREADS) void grad_w_kernel(int K, int N, Operand a, Operand b, Tiles all, float *out) {
     extern __shared__ __bf16 lds[];
-    const int tiles = row_tiles * column_tiles, number = tile_number(tiles * parts), part = number / tiles, tile = number - part * tiles;
-    const int bi = tile / column_tiles, bj = tile - bi * column_tiles;
-    const int per = (blocks + parts - 1) / parts, from = min(blocks, part * per), end = min(blocks, from + per);
-    f32x4 acc[S::FA][S::FB] = {};
-    multiply<S>(a, b, bi, bj, from, end, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
-    to += (long)part * K * 2 * N;
+    int bi, bj, part, from, to;
+    all.place(bi, bj, part, from, to);
+    f32x4 acc[S::FA][S::FB] = {};
+    multiply<S, false>(a, b, bi, bj, from, to, lds, acc);
+    float *const here = out + (long)part * K * 2 * N;
 #pragma unroll
     for (int i = 0; i < S::FA; ++i)
 #pragma unroll
-        for (int j = 0; j < S::FB; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int fragment = bj * S::COLUMNS + wc * S::FB + j, row = (bi * S::ROWS + wr * S::FA + i) * 16 + 4 * g + r, column = (fragment >> 1) * 16 + c;
-                if (row < K && column < N) to[(long)row * 2 * N + (fragment & 1) * N + column] = acc[i][j][r];
-            }
+        for (int j = 0; j < S::FB; ++j) {
+            const int fragment = bj * S::COLUMNS + wc * S::FB + j;
+            store_tile(here + (fragment & 1) * N, 2L * N, acc[i][j], (bi * S::ROWS + wr * S::FA + i) * 16, (fragment >> 1) * 16, K, N, g, c);
+        }
 }
 
 // The biases' gradients from the sums of rows of wavefronts, by the first workgroups, 64 columns each; the parts of dW added up, in order, by the others.
@@ -402,12 +464,15 @@ __global__ __launch_bounds__(256) void finish_kernel(const float *parts, int cou
         const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, at = blockIdx.x * 64 + lane;
         float sum = 0.0f;
         if (at < columns) {
-            float some[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int r = w; r < rows; r += 16)
+            float some[16] = {};
+            for (int r = w; r < rows; r += 64)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r + 4 * i < rows) some[i] += sums[(long)(r + 4 * i) * columns + at];
-            sum = (some[0] + some[1]) + (some[2] + some[3]);
+                for (int i = 0; i < 16; ++i) {
+                    const float x = sums[(long)min(r + 4 * i, rows - 1) * columns + at];
+                    some[i] += r + 4 * i < rows ? x : 0.0f;
+                }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += some[i];
         }
         shared[w][lane] = sum;
         __syncthreads();
@@ -416,11 +481,19 @@ __global__ __launch_bounds__(256) void finish_kernel(const float *parts, int cou
             grads[values + (at & 16 ? N : 0) + column] = (shared[0][lane] + shared[1][lane]) + (shared[2][lane] + shared[3][lane]);
         return;
     }
-    const long i = (long)(blockIdx.x - bias_blocks) * 256 + threadIdx.x;
-    if (i >= values) return;
-    float sum = parts[i];
-    for (int p = 1; p < count; ++p) sum += parts[p * values + i];
-    grads[i] = sum;
+    const long i = ((long)(blockIdx.x - bias_blocks) * 256 + threadIdx.x) * 4;
+    if (i + 4 <= values) {
+        f32x4 sum = *reinterpret_cast<const f32x4u *>(parts + i);
+#pragma unroll 4
+        for (int p = 1; p < count; ++p) sum += *reinterpret_cast<const f32x4u *>(parts + p * values + i);
+        *reinterpret_cast<f32x4u *>(grads + i) = sum;
+    } else {
+        for (long j = i; j < values; ++j) {
+            float sum = parts[j];
+            for (int p = 1; p < count; ++p) sum += parts[p * values + j];
+            grads[j] = sum;
+        }
+    }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -489,11 +562,11 @@ template <class S>
 int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
 
 // 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.
-typedef Shape<1, 1, 2, 4, 4, 3> Bf16Shape;
-typedef Shape<1, 1, 4, 1, 2, 4> Bf16Small;
-typedef Shape<1, 2, 2, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
-typedef Shape<3, 3, 2, 4, 2, 3> F32Shape;
-typedef Shape<3, 3, 4, 1, 2, 3> F32Small;
+typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
+typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
+typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
+typedef Shape<3, 3, 2, 4, 4, 2, 3> F32Shape;
+typedef Shape<3, 3, 4, 2, 1, 2, 3> F32Small;
 constexpr int WR_MOST = 4;
 
 Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) {
@@ -530,37 +603,26 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
     return p;
 }
 
+template <class S>
+Tiles tiles_in(long a, long b, int blocks, int parts = 1) { return {(int)((a + S::ROWS - 1) / S::ROWS), (int)((b + S::COLUMNS - 1) / S::COLUMNS), parts, blocks}; }
 template <class E, class S, int P, int PR, int PC>
 struct Launch {
-    static dim3 grid(long a, long b) { return dim3((unsigned)tiles<S>(a, b)); }
-    static int down(long fragments) { return (int)((fragments + S::ROWS - 1) / S::ROWS); }
-    static int across(long fragments) { return (int)((fragments + S::COLUMNS - 1) / S::COLUMNS); }
-    static void forward(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is) {
-        const dim3 tiles = grid(p.M16, 2L * p.N16);
+    template <bool FORWARD>
+    static void pre(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is, __bf16 *rows = nullptr, __bf16 *columns = nullptr,
+                    float *sums = nullptr) {
+        const Tiles t = tiles_in<S>(p.M16, 2L * p.N16, p.K16 / 2);
         if constexpr (P == 1) {
             if (as_is) {
-                hipLaunchKernelGGL((pre_kernel<E, S, true, true, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, down(p.M16), across(2L * p.N16), p.K16 / 2, nullptr, nullptr, nullptr);
+                hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, true, PR, PC>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
                 return;
             }
         }
-        hipLaunchKernelGGL((pre_kernel<E, S, true, false, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, down(p.M16), across(2L * p.N16), p.K16 / 2, nullptr, nullptr, nullptr);
+        hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, PR, PC>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
     }
-    // the number of rows of sums
-    static int gradient(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is, __bf16 *rows, __bf16 *columns, float *sums) {
-        const dim3 tiles = grid(p.M16, 2L * p.N16);
-        const int row_tiles = down(p.M16), column_tiles = across(2L * p.N16);
-        bool done = false;
-        if constexpr (P == 1) {
-            if (as_is) {
-                hipLaunchKernelGGL((pre_kernel<E, S, false, true, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, row_tiles, column_tiles, p.K16 / 2, rows, columns, sums);
-                done = true;
-            }
-        }
-        if (!done) hipLaunchKernelGGL((pre_kernel<E, S, false, false, PR, PC>), tiles, dim3(512), S::LDS, ctx->stream, y, x, w, row_tiles, column_tiles, p.K16 / 2, rows, columns, sums);
-        return row_tiles * S::WR;
-    }
+    static int sum_rows(const Plan &p) { return tiles_in<S>(p.M16, 1, 1).down * S::WR; }
     static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w) {
-        hipLaunchKernelGGL((grad_x_kernel<E, S>), grid(p.M16, p.K16), dim3(512), S::LDS, ctx->stream, y, pre, w, down(p.M16), across(p.K16), p.N16);
+        const Tiles t = tiles_in<S>(p.M16, p.K16, p.N16);
+        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t);
     }
 };
 
@@ -586,23 +648,25 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     const auto few = [&](long a, long b) { return tiles<S>(a, b) < ctx->n_cus; };
     const bool pre_small = few(p.M16, 2L * p.N16);
     if (!backward) {
-        if (pre_small) Small::forward(ctx, y, p, x_rows, w_columns, as_is);
-        else Large::forward(ctx, y, p, x_rows, w_columns, as_is);
+        if (pre_small) Small::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
+        else Large::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
         return;
     }
     __bf16 *const rows = (__bf16 *)(ws + p.pre_rows), *const columns = (__bf16 *)(ws + p.pre_columns);
     float *const sums = (float *)(ws + p.sums);
-    const int sum_rows = pre_small ? Small::gradient(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums) : Large::gradient(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums);
+    if (pre_small) Small::template pre<false>(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums);
+    else Large::template pre<false>(ctx, y, p, x_rows, w_columns, as_is, rows, columns, sums);
+    const int sum_rows = pre_small ? Small::sum_rows(p) : Large::sum_rows(p);
     const Operand pre_rows = {rows, p.M16}, pre_columns = {columns, 2 * p.N16}, x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
     if (y.grad_x != nullptr) {
         if (few(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows);
         else Large::grad_x(ctx, y, p, pre_rows, w_rows);
     }
-    const int down = (p.K16 + SW::ROWS - 1) / SW::ROWS, across = (2 * p.N16 + SW::COLUMNS - 1) / SW::COLUMNS;
+    const Tiles t = tiles_in<SW>(p.K16, 2L * p.N16, p.M16 / 2, p.parts);
     const long values = (long)y.K * 2 * y.N;
     float *const to = p.parts > 1 ? (float *)(ws + p.partial) : y.grads;
-    hipLaunchKernelGGL((grad_w_kernel<SW>), dim3((unsigned)(down * across * p.parts)), dim3(512), SW::LDS, ctx->stream, y.K, y.N, x_columns, pre_columns, down, across, p.M16 / 2, p.parts, to);
-    const long blocks = (2L * p.N16 * 16 + 63) / 64 + (p.parts > 1 ? (values + 255) / 256 : 0);
+    hipLaunchKernelGGL((grad_w_kernel<SW>), dim3(t.count()), dim3(SW::THREADS), SW::LDS, ctx->stream, y.K, y.N, x_columns, pre_columns, t, to);
+    const long blocks = (2L * p.N16 * 16 + 63) / 64 + (p.parts > 1 ? (values + 1023) / 1024 : 0);
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, to, p.parts, values, sums, sum_rows, 2 * p.N16 * 16, y.N, y.grads);
 }
 
