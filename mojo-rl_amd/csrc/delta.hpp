@@ -117,37 +117,25 @@ MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
 constexpr int tiles_forward(int DK) { return DK == 128 ? 2 : 4; }
 constexpr int tiles_backward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int SIDE = TILE + 4;        // floats from a row of a 16 x 16 matrix in LDS to the next
-constexpr size_t rows_floats(int DK, int tiles) { return 2 * TILE * tiles * (DK + 4) + 3 * tiles * TILE * SIDE + 6 * TILE * tiles; }
+constexpr size_t rows_floats(int DK, int tiles) { return 2 * TILE * tiles * (DK + 4) + 3 * tiles * TILE * SIDE + 11 * TILE * tiles + 4; }
 
-// The decays of a tile, from its 16 a in LDS.  Lane 16 g + n holds rows i = 4 g + r of column n.
-struct Decays {
-    float from[4];   // F[i]
-    float to[4];     // L[i]
-    float whole;     // F[15]
-    MRL_DEV void load(const float *a, int g) {
-        float block[4];
-        f32x4 own = {1.0f, 1.0f, 1.0f, 1.0f};
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(a + 4 * p);
-            block[p] = x[0] * x[1] * (x[2] * x[3]);
-            if (p == g) own = x;
-        }
-        float before = 1.0f, behind = 1.0f;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            before = p < g ? before * block[p] : before;
-            behind = p > g ? behind * block[p] : behind;
-        }
-        from[0] = before * own[0];
-#pragma unroll
-        for (int r = 1; r < 4; ++r) from[r] = from[r - 1] * own[r];
-        to[3] = behind;
-#pragma unroll
-        for (int r = 2; r >= 0; --r) to[r] = to[r + 1] * own[r + 1];
-        whole = block[0] * block[1] * (block[2] * block[3]);
+// From one lane to another of a row of 16, `missing` where there is none.
+template <int CONTROL>
+MRL_DEV float moved(float x, float missing) { return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(missing), __float_as_int(x), CONTROL, 0xF, 0xF, false)); }
+// the sum over LANES neighbouring lanes, in all of them
+template <int LANES>
+MRL_DEV float sum_lanes(float x) {
+    x += moved<0xB1>(x, 0.0f);
+    x += moved<0x4E>(x, 0.0f);
+    if (LANES >= 8) x += moved<0x141>(x, 0.0f);
+    if (LANES >= 16) x += moved<0x140>(x, 0.0f);
+    if (LANES >= 32) {
+        const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(row[0]) + __uint_as_float(row[1]);
     }
-};
+    return x;
+}
+
 // G[4 g + r][n], 0 above the diagonal
 MRL_DEV f32x4 between(const float *a, int g, int n) {
     float run = 1.0f;
@@ -209,7 +197,9 @@ MRL_DEV f32x4 invert(const float *A, int g, int n) {
 template <int DK, int TILES_>
 struct Block {
     static constexpr int TILES = TILES_, STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
-    float *K, *Q, *As, *Ts, *Ps, *as, *rests, *bs, *rate_rests, *kscale, *qscale;   // rests: 1 - a, 0 at a cut; rate_rests: 1 - b
+    float *K, *Q, *As, *Ts, *Ps;
+    // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), and F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
+    float *as, *rests, *bs, *rate_rests, *kscale, *qscale, *from, *to, *key_reads, *query_reads, *key_takes, *wholes;
     int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
     MRL_DEV explicit Block(float *lds) {
         K = lds;
@@ -223,9 +213,16 @@ struct Block {
         rate_rests = bs + STEPS;
         kscale = rate_rests + STEPS;
         qscale = kscale + STEPS;
+        from = qscale + STEPS;
+        to = from + STEPS;
+        key_reads = to + STEPS;
+        query_reads = key_reads + STEPS;
+        key_takes = query_reads + STEPS;
+        wholes = key_takes + STEPS;
     }
     MRL_DEV int time_of(int slot) const { return t0 + (slot >> 4) * span + (slot & 15); }
     MRL_DEV bool there(const Delta &d, int slot) const { return (slot & 15) < span && time_of(slot) < d.T; }
+    MRL_DEV bool full(const Delta &d) const { return span == TILE && t0 + STEPS <= d.T; }
     MRL_DEV f32x4 four(const float *scalars, int tile, int g) const { return *reinterpret_cast<const f32x4 *>(scalars + tile * TILE + 4 * g); }
 
     // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
@@ -234,41 +231,51 @@ struct Block {
     template <class E, bool QUERIES>
     MRL_DEV bool load(const Delta &d, int n, int h, int hk, int thread) {
         bool odd = false;
-        const int part = (thread & 63) % LANES, count = d.dk - 4 * part, first = count > 0 ? 4 * part : 0;
+        const int part = (thread & 63) % LANES, count = d.dk - 4 * part, first = count > 0 ? 4 * part : 0, rows = (int)blockDim.x / LANES;
         const E *const keys = (const E *)d.key + n * d.key_ld + (long)hk * d.dk + first, *const queries = (const E *)d.query + n * d.query_ld + (long)hk * d.dk + first;
         const long key_step = (long)d.N * d.key_ld, query_step = (long)d.N * d.query_ld;
-        const bool whole = (d.dk & 3) == 0;
-        for (int slot = thread / LANES; slot < STEPS; slot += (int)blockDim.x / LANES) {
-            const bool here = there(d, slot) && count > 0;
-            const long t = min(time_of(slot), d.T - 1);
-            f32x4 k, q = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (whole) {
-                k = load4(keys + t * key_step, 4);
-                if (QUERIES) q = load4(queries + t * query_step, 4);
-            } else {
-                k = load4(keys + t * key_step, count);
-                if (QUERIES) q = load4(queries + t * query_step, count);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                k[i] = here ? k[i] : 0.0f;
-                q[i] = here ? q[i] : 0.0f;
-            }
+        const bool whole = (d.dk & 3) == 0, all = full(d) && d.dk == DK;
+        const auto take = [&](int slot, f32x4 k, f32x4 q) {
             *reinterpret_cast<f32x4 *>(K + slot * ROW + 4 * part) = k;
-            float kk = fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))), qq = 0.0f;
+            const float kk = sum_lanes<LANES>(fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))));
+            float qq = 0.0f;
             if (QUERIES) {
                 *reinterpret_cast<f32x4 *>(Q + slot * ROW + 4 * part) = q;
-                qq = fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3])));
+                qq = sum_lanes<LANES>(fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3]))));
             }
-#pragma unroll
-            for (int s = 1; s < LANES; s *= 2) {
-                kk += __shfl_xor(kk, s);
-                if (QUERIES) qq += __shfl_xor(qq, s);
-            }
-            odd |= !(kk < LARGE) || !(qq < LARGE);
+            odd |= !(kk + qq < LARGE);
             if (part == 0) {
                 kscale[slot] = 1.0f / sqrtf(kk + EPS);
                 qscale[slot] = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
+            }
+        };
+        if (all) {
+            const int slot = thread / LANES;
+            const E *k = keys + (long)(t0 + slot) * key_step, *q = queries + (long)(t0 + slot) * query_step;
+            for (int ahead = 0; ahead < STEPS; ahead += rows) {
+                if (STEPS % rows != 0 && slot + ahead >= STEPS) break;
+                take(slot + ahead, load4(k, 4), QUERIES ? load4(q, 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                k += rows * key_step;
+                q += rows * query_step;
+            }
+        } else {
+            for (int slot = thread / LANES; slot < STEPS; slot += rows) {
+                const bool here = there(d, slot) && count > 0;
+                const long t = min(time_of(slot), d.T - 1);
+                f32x4 k, q = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (whole) {
+                    k = load4(keys + t * key_step, 4);
+                    if (QUERIES) q = load4(queries + t * query_step, 4);
+                } else {
+                    k = load4(keys + t * key_step, count);
+                    if (QUERIES) q = load4(queries + t * query_step, count);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    k[i] = here ? k[i] : 0.0f;
+                    q[i] = here ? q[i] : 0.0f;
+                }
+                take(slot, k, q);
             }
         }
         for (int slot = thread; slot < STEPS; slot += blockDim.x) {
@@ -289,7 +296,7 @@ struct Block {
         return odd;
     }
 
-    // (1 + A)^-1 and (QUERIES) P of a tile, by one wavefront
+    // (1 + A)^-1, (QUERIES) P and the decays of a tile, by one wavefront
     template <bool QUERIES>
     MRL_DEV void prepare(int tile, int g, int c) {
         const float *k_tile = K + tile * TILE * ROW + c * ROW + 4 * g, *q_tile = Q + tile * TILE * ROW + c * ROW + 4 * g;
@@ -299,6 +306,25 @@ struct Block {
             const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + i * TILE);
             kk = mfma16(k, k, kk);
             if (QUERIES) qk = mfma16(*reinterpret_cast<const f32x4 *>(q_tile + i * TILE), k, qk);
+        }
+        if (g == 0) {
+            const int slot = tile * TILE + c;
+            const float a = as[slot], b = bs[slot], ks = kscale[slot], qs = qscale[slot];
+            float ahead = a, behind = moved<0x101>(a, 1.0f);   // products up to here, and of those behind
+            ahead *= moved<0x111>(ahead, 1.0f);
+            behind *= moved<0x101>(behind, 1.0f);
+            ahead *= moved<0x112>(ahead, 1.0f);
+            behind *= moved<0x102>(behind, 1.0f);
+            ahead *= moved<0x114>(ahead, 1.0f);
+            behind *= moved<0x104>(behind, 1.0f);
+            ahead *= moved<0x118>(ahead, 1.0f);
+            behind *= moved<0x108>(behind, 1.0f);
+            from[slot] = ahead;
+            to[slot] = behind;
+            key_reads[slot] = b * ahead * ks;
+            query_reads[slot] = ahead * qs;
+            key_takes[slot] = behind * ks;
+            if (c == TILE - 1) wholes[tile] = ahead;
         }
         const f32x4 decay = between(as + tile * TILE, g, c), b = four(bs, tile, g), ks = four(kscale, tile, g), qs = four(qscale, tile, g);
         const float kc = kscale[tile * TILE + c];
@@ -321,28 +347,57 @@ struct Block {
 // step 0, `step` elements from a step to the next.
 template <class E, class B, int TILES>
 MRL_DEV bool load_values(const Delta &d, const B &block, const E *rows, long step, bool live, int g, f32x4 (&V)[TILES]) {
-    bool odd = false;
+    float size = 0.0f;
+    if (block.full(d)) {
+        const E *const first = rows + 4 * g * step;
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) V[tile][r] = value_of(first[(long)(block.t0 + tile * TILE + r) * step]);
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) V[tile][r] = live ? V[tile][r] : 0.0f;
+    } else {
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = value_of(rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step]);
+                V[tile][r] = live && block.there(d, tile * TILE + 4 * g + r) ? x : 0.0f;
+            }
+    }
 #pragma unroll
     for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) V[tile][r] = value_of(rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step]);
+        for (int r = 0; r < 4; ++r) size += fabsf(V[tile][r]);
+    return !(size < LARGE);
+}
+// and back: one tile
+template <class E, class B>
+MRL_DEV void store_values(const Delta &d, const B &block, E *rows, long step, bool live, int tile, int g, const f32x4 x) {
+    if (block.full(d)) {
+        E *const first = rows + 4 * g * step;
+        if (live) {
 #pragma unroll
-    for (int tile = 0; tile < TILES; ++tile)
+            for (int r = 0; r < 4; ++r) give(first + (long)(block.t0 + tile * TILE + r) * step, x[r]);
+        }
+    } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            V[tile][r] = live && block.there(d, tile * TILE + 4 * g + r) ? V[tile][r] : 0.0f;
-            odd |= !(fabsf(V[tile][r]) < LARGE);
+            const int slot = tile * TILE + 4 * g + r;
+            if (live && block.there(d, slot)) give(rows + block.time_of(slot) * step, x[r]);
         }
-    return odd;
+    }
 }
 template <int B>
 MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
-    bool odd = false;
+    float size = 0.0f;
 #pragma unroll
     for (int i = 0; i < B; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) odd |= !(fabsf(S[i][r]) < LARGE);
-    return odd;
+        for (int r = 0; r < 4; ++r) size += fabsf(S[i][r]);
+    return !(size < LARGE);
 }
 
 // S^T k of a tile's 16 keys (or queries), unscaled: [row of the tile][column of S]
@@ -366,12 +421,12 @@ MRL_DEV void add(const Block<DK, TILES> &block, const float *rows, int tile, int
 }
 // U[4 g + r][c] of a tile; read: b F S0^T k, what the keys read of the state
 template <int DK, int TILES>
-MRL_DEV f32x4 solve(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
-    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g);
+MRL_DEV f32x4 solve(const Block<DK, TILES> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
+    const f32x4 b = block.four(block.bs, tile, g), reads = block.four(block.key_reads, tile, g);
     f32x4 x;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        read[r] = b[r] * decay.from[r] * ks[r] * sk[r];
+        read[r] = reads[r] * sk[r];
         x[r] = fmaf(b[r], v[r], -read[r]);
     }
     const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
@@ -379,12 +434,11 @@ MRL_DEV f32x4 solve(const Block<DK, TILES> &block, const Decays &decay, int tile
 }
 // S0 becomes S1
 template <int DK, int TILES>
-MRL_DEV void go_on(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
-    const f32x4 ks = block.four(block.kscale, tile, g);
+MRL_DEV void go_on(const Block<DK, TILES> &block, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
+    u *= block.four(block.key_takes, tile, g);
+    const float whole = block.wholes[tile];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) u[r] *= decay.to[r] * ks[r];
-#pragma unroll
-    for (int i = 0; i < DK / TILE; ++i) S[i] *= decay.whole;
+    for (int i = 0; i < DK / TILE; ++i) S[i] *= whole;
     add(block, block.K, tile, g, c, u, S);
 }
 

@@ -115,6 +115,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
     }
 
     const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
+    E *const outs = (E *)d.out + n * d.out_ld + (long)h * d.dv + column;
     int begin = part * parts.per * STEPS;   // of the block
     const int end = min(d.T, begin + parts.per * STEPS);
     bool cut = false;
@@ -146,8 +147,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
         for (int tile = 0; tile < TILES; ++tile) {
             if (block.t0 + tile * block.span >= d.T) break;
             anew(g, c);
-            Decays decay;
-            decay.load(block.as + tile * TILE, g);
             if (block.cut_ahead(tile)) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -157,21 +156,13 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
             for (int i = 1; i < TILES; ++i) v = tile == i ? V[i] : v;
             const f32x4 sk = ask(block, block.K, tile, g, c, S);
             if (WHAT == OUTPUTS) o = ask(block, block.Q, tile, g, c, S);
-            const f32x4 u = solve(block, decay, tile, g, c, v, sk, read);
+            const f32x4 u = solve(block, tile, g, c, v, sk, read);
             if (WHAT == OUTPUTS) {
-                const f32x4 qs = block.four(block.qscale, tile, g);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] *= decay.from[r] * qs[r];
+                o *= block.four(block.query_reads, tile, g);
                 o = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + tile * TILE * SIDE + c * SIDE + 4 * g), u, o);
             }
-            go_on(block, decay, tile, g, c, u, S);
-            if (WHAT == OUTPUTS) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int slot = tile * TILE + 4 * g + r;
-                    if (live && block.there(d, slot)) give((E *)d.out + ((long)block.time_of(slot) * d.N + n) * d.out_ld + h * d.dv + column, o[r]);
-                }
-            }
+            go_on(block, tile, g, c, u, S);
+            if (WHAT == OUTPUTS) store_values(d, block, outs, (long)d.N * d.out_ld, live, tile, g, o);
             if (WHAT == ENDS) {
 #pragma unroll
                 for (int i = 0; i < TILE; i += 4) {

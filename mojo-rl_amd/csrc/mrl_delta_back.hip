@@ -44,55 +44,38 @@ struct Back {
     int blocks;
 };
 
-// sums over the 16 lanes of a group, in all of them
-template <int N>
-MRL_DEV float turned(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + N, 0xF, 0xF, false)); }
-MRL_DEV float sum16(float x) {
-    x += turned<8>(x);
-    x += turned<4>(x);
-    x += turned<2>(x);
-    return x + turned<1>(x);
-}
-// what the lanes from this one on have, and those ahead of it
-template <int CONTROL>
-MRL_DEV float moved(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CONTROL, 0xF, 0xF, true)); }
+MRL_DEV float sum16(float x) { return sum_lanes<16>(x); }
+// of a row's 16 lanes, the sum of those from this one on, and of those ahead of it
 MRL_DEV float sum_from(float x) {
-    x += moved<0x101>(x);
-    x += moved<0x102>(x);
-    x += moved<0x104>(x);
-    return x + moved<0x108>(x);
+    x += moved<0x101>(x, 0.0f);
+    x += moved<0x102>(x, 0.0f);
+    x += moved<0x104>(x, 0.0f);
+    return x + moved<0x108>(x, 0.0f);
 }
 MRL_DEV float sum_ahead(float x) {
-    x = moved<0x111>(x);
-    x += moved<0x111>(x);
-    x += moved<0x112>(x);
-    x += moved<0x114>(x);
-    return x + moved<0x118>(x);
+    x = moved<0x111>(x, 0.0f);
+    x += moved<0x111>(x, 0.0f);
+    x += moved<0x112>(x, 0.0f);
+    x += moved<0x114>(x, 0.0f);
+    return x + moved<0x118>(x, 0.0f);
 }
 
 // What a tile's columns make of dO and dS1: read = L dS1^T k, dX, and dS1 becomes dS0.
 template <int DK, int TILES>
-MRL_DEV void pull(const Block<DK, TILES> &block, const Decays &decay, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
-    const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
-    read = ask(block, block.K, tile, g, c, dS);
+MRL_DEV void pull(const Block<DK, TILES> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
+    read = ask(block, block.K, tile, g, c, dS) * block.four(block.key_takes, tile, g);
     f32x4 p_column, t_column;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        read[r] *= decay.to[r] * ks[r];
         p_column[r] = block.Ps[(tile * TILE + 4 * g + r) * SIDE + c];
         t_column[r] = block.Ts[(tile * TILE + 4 * g + r) * SIDE + c];
     }
     dX = mfma16(t_column, mfma16(p_column, dO, read), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-    f32x4 q_part, k_part;
+    const float whole = block.wholes[tile];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        q_part[r] = decay.from[r] * qs[r] * dO[r];
-        k_part[r] = -decay.from[r] * ks[r] * b[r] * dX[r];
-    }
-#pragma unroll
-    for (int i = 0; i < DK / TILE; ++i) dS[i] *= decay.whole;
-    add(block, block.Q, tile, g, c, q_part, dS);
-    add(block, block.K, tile, g, c, k_part, dS);
+    for (int i = 0; i < DK / TILE; ++i) dS[i] *= whole;
+    add(block, block.Q, tile, g, c, dO * block.four(block.query_reads, tile, g), dS);
+    add(block, block.K, tile, g, c, -dX * block.four(block.key_reads, tile, g), dS);
     if (block.cut_ahead(tile)) {
 #pragma unroll
         for (int i = 0; i < DK / TILE; ++i) dS[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -158,10 +141,8 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
             for (int tile = TILES - 1; tile >= 0; --tile) {
                 if (block.t0 + tile * block.span >= d.T) continue;
                 anew(g, c);
-                Decays decay;
-                decay.load(block.as + tile * TILE, g);
                 f32x4 read, dX;
-                pull(block, decay, tile, g, c, dO[tile], dS, read, dX);
+                pull(block, tile, g, c, dO[tile], dS, read, dX);
             }
             block.t0 -= TILES;
             ++round;
@@ -228,21 +209,19 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile) {
             anew(g, c);
-            Decays decay;
-            decay.load(block.as + tile * TILE, g);
             if (block.cut_ahead(tile)) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = zero;
             }
             f32x4 read;
-            const f32x4 u = solve(block, decay, tile, g, c, V[tile], ask(block, block.K, tile, g, c, S), read);
+            const f32x4 u = solve(block, tile, g, c, V[tile], ask(block, block.K, tile, g, c, S), read);
             if constexpr (decltype(keep)::value) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) kept[tile][i] = S[i];
                 U[tile] = u;
                 reads[tile] = read;
             }
-            if (!decltype(keep)::value || tile + 1 < TILES) go_on(block, decay, tile, g, c, u, S);
+            if (!decltype(keep)::value || tile + 1 < TILES) go_on(block, tile, g, c, u, S);
         }
     };
     const auto load = [&]() {
@@ -297,18 +276,12 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 const float *k_tile = block.K + tile * TILE * block.ROW, *q_tile = block.Q + tile * TILE * block.ROW;
                 const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
                 float *const dot = dots + turn * DOTS * TILE * W;
-                Decays decay;
-                decay.load(block.as + tile * TILE, g);
-                const f32x4 b = block.four(block.bs, tile, g), ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
+                const f32x4 b = block.four(block.bs, tile, g);
                 f32x4 dS1[BOTH ? 1 : B];
                 // ---- by columns
                 if (owns) {
-                    f32x4 out = ask(block, block.Q, tile, g, c, kept[tile]), e;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        out[r] *= decay.from[r] * qs[r];
-                        e[r] = dO[tile][r] * out[r];
-                    }
+                    f32x4 out = ask(block, block.Q, tile, g, c, kept[tile]) * block.four(block.query_reads, tile, g);
+                    const f32x4 e = dO[tile] * out;
                     out = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + (tile * TILE + c) * SIDE + 4 * g), U[tile], out);
                     float s_ds = 0.0f;
 #pragma unroll
@@ -324,14 +297,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         for (int i = 0; i < B; ++i) dS1[i] = dS[i];
                     }
                     f32x4 read, dX;
-                    pull(block, decay, tile, g, c, dO[tile], dS, read, dX);
+                    pull(block, tile, g, c, dO[tile], dS, read, dX);
+                    store_values(d, block, (E *)p.value + n * p.value_ld + (long)h * d.dv + column, (long)d.N * p.value_ld, live, tile, g, b * dX);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int slot = tile * TILE + 4 * g + r, at = (4 * g + r) * stride + column;
+                        const int at = (4 * g + r) * stride + column;
                         dOs[at] = dO[tile][r];
                         dXs[at] = dX[r];
                         Us[at] = U[tile][r];
-                        if (live && block.there(d, slot)) give((E *)p.value + ((long)block.time_of(slot) * d.N + n) * p.value_ld + h * d.dv + column, b[r] * dX[r]);
                         const float sums[DOTS] = {sum16(dO[tile][r] * out[r]), sum16(dX[r] * fmaf(2.0f, U[tile][r], -b[r] * V[tile][r])), sum16(fmaf(-dX[r], reads[tile][r], e[r])),
                                                   sum16(U[tile][r] * read[r]), sum16(U[tile][r] * dX[r])};
                         if (c == 0) {
@@ -342,6 +315,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 }
                 __syncthreads();
                 // ---- by rows of the states, their terms of dq and dk; by one wavefront, dA and dP
+                const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g);
                 f32x4 dq[OWN], dk[OWN];
 #pragma unroll
                 for (int o = 0; o < OWN; ++o) {
@@ -359,8 +333,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        dq[o][r] *= decay.from[r];
-                        dk[o][r] = fmaf(decay.to[r], of[r], -decay.from[r] * b[r] * dk[o][r]);
+                        dq[o][r] *= from[r];
+                        dk[o][r] = fmaf(to[r], of[r], -from[r] * b[r] * dk[o][r]);
                     }
                 }
                 if (w == pairs_by) {
@@ -404,10 +378,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                             of = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
                                         *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), of);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(decay.to[r], of[r], dk[o][r]);
+                        for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(to[r], of[r], dk[o][r]);
                     }
                 }
                 // ---- the tile's own pairs, the lengths, gates and rates
+                const f32x4 ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
                 f32x4 q_dot = zero, k_dot = zero;
                 for (int t = 0; t < tiles; ++t) {
                     q_dot += *reinterpret_cast<const f32x4 *>(dot + t * TILE + 4 * g);
@@ -431,12 +406,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     const int at = i * TILE + c;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int slot = tile * TILE + 4 * g + r;
-                        if (at >= d.dk || !block.there(d, slot)) continue;
-                        const long row = (long)block.time_of(slot) * d.N + n;
-                        give((EK *)p.query + row * p.query_ld + key_at + at, qs[r] * fmaf(-(float)d.dk * q[r], q_dot[r], dq[o][r]));
-                        give((EK *)p.key + row * p.key_ld + key_at + at, ks[r] * fmaf(-k[r], k_dot[r], dk[o][r]));
+                        q[r] = qs[r] * fmaf(-(float)d.dk * q[r], q_dot[r], dq[o][r]);
+                        k[r] = ks[r] * fmaf(-k[r], k_dot[r], dk[o][r]);
                     }
+                    store_values(d, block, (EK *)p.query + n * p.query_ld + key_at + at, (long)d.N * p.query_ld, at < d.dk, tile, g, q);
+                    store_values(d, block, (EK *)p.key + n * p.key_ld + key_at + at, (long)d.N * p.key_ld, at < d.dk, tile, g, k);
                 }
                 if (w == pairs_by && g == 0) {
                     float e = 0.0f, f = 0.0f, u_dx = 0.0f, all = 0.0f;
@@ -446,7 +420,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         u_dx += dot[(4 * W + t) * TILE + c];
                         all += wholes[turn * W + t];
                     }
-                    const float sum = fmaf(decay.whole, all, crossing[c] + (sum_from(e) + sum_ahead(f)));
+                    const float sum = fmaf(block.wholes[tile], all, crossing[c] + (sum_from(e) + sum_ahead(f)));
                     const int slot = tile * TILE + c;
                     if (block.there(d, slot)) {
                         const long row = (long)block.time_of(slot) * d.N + n;
