@@ -114,10 +114,10 @@ MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
 }
 
 // Tiles that a workgroup prepares together, a block: as many as leave a CU's LDS room for two workgroups and more.
-constexpr int tiles_forward(int DK) { return DK == 128 ? 2 : 4; }
+constexpr int tiles_forward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int tiles_backward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int SIDE = TILE + 4;        // floats from a row of a 16 x 16 matrix in LDS to the next
-constexpr size_t rows_floats(int DK, int tiles) { return 2 * TILE * tiles * (DK + 4) + 3 * tiles * TILE * SIDE + 11 * TILE * tiles + 4; }
+constexpr size_t rows_floats(int DK, int tiles, bool keeps) { return 2 * TILE * tiles * (DK + 4) + (keeps ? 3 : 2) * tiles * TILE * SIDE + 13 * TILE * tiles + 4; }
 
 // From one lane to another of a row of 16, `missing` where there is none.
 template <int CONTROL>
@@ -194,24 +194,27 @@ MRL_DEV f32x4 invert(const float *A, int g, int n) {
 }
 
 // What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.
-template <int DK, int TILES_>
+// KEEPS: A beside its inverse.
+template <int DK, int TILES_, bool KEEPS>
 struct Block {
     static constexpr int TILES = TILES_, STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
     float *K, *Q, *As, *Ts, *Ps;
-    // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), and F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
-    float *as, *rests, *bs, *rate_rests, *kscale, *qscale, *from, *to, *key_reads, *query_reads, *key_takes, *wholes;
+    // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), the squares of key and query, F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
+    float *as, *rests, *bs, *rate_rests, *key_lengths, *query_lengths, *kscale, *qscale, *from, *to, *key_reads, *query_reads, *key_takes, *wholes;
     int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
     MRL_DEV explicit Block(float *lds) {
         K = lds;
         Q = K + STEPS * ROW;
         As = Q + STEPS * ROW;
-        Ts = As + TILES * TILE * SIDE;
+        Ts = KEEPS ? As + TILES * TILE * SIDE : As;
         Ps = Ts + TILES * TILE * SIDE;
         as = Ps + TILES * TILE * SIDE;
         rests = as + STEPS;
         bs = rests + STEPS;
         rate_rests = bs + STEPS;
-        kscale = rate_rests + STEPS;
+        key_lengths = rate_rests + STEPS;
+        query_lengths = key_lengths + STEPS;
+        kscale = query_lengths + STEPS;
         qscale = kscale + STEPS;
         from = qscale + STEPS;
         to = from + STEPS;
@@ -244,9 +247,9 @@ struct Block {
                 qq = sum_lanes<LANES>(fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3]))));
             }
             odd |= !(kk + qq < LARGE);
-            if (part == 0) {
-                kscale[slot] = 1.0f / sqrtf(kk + EPS);
-                qscale[slot] = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
+            if (part == 0) {   // (squares for now: prepare() makes lengths of them)
+                kscale[slot] = kk;
+                qscale[slot] = qq;
             }
         };
         if (all) {
@@ -296,20 +299,24 @@ struct Block {
         return odd;
     }
 
-    // (1 + A)^-1, (QUERIES) P and the decays of a tile, by one wavefront
+    // What does not depend on the state, by halves of a tile, a wavefront each: A and (1 + A)^-1; P (QUERIES) and the decays.  Each half makes the
+    // lengths that it needs.
+    static constexpr int HALVES = 2 * TILES;
     template <bool QUERIES>
-    MRL_DEV void prepare(int tile, int g, int c) {
-        const float *k_tile = K + tile * TILE * ROW + c * ROW + 4 * g, *q_tile = Q + tile * TILE * ROW + c * ROW + 4 * g;
-        f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
-#pragma unroll
-        for (int i = 0; i < DK / TILE; ++i) {
-            const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + i * TILE);
-            kk = mfma16(k, k, kk);
-            if (QUERIES) qk = mfma16(*reinterpret_cast<const f32x4 *>(q_tile + i * TILE), k, qk);
-        }
-        if (g == 0) {
+    MRL_DEV void prepare(const Delta &d, int half, int g, int c) {
+        const int tile = half >> 1;
+        const float *k_tile = K + (tile * TILE + c) * ROW + 4 * g, *q_tile = Q + (tile * TILE + c) * ROW + 4 * g;
+        const float kc = 1.0f / sqrtf(kscale[tile * TILE + c] + EPS);
+        const f32x4 decay = between(as + tile * TILE, g, c);
+        f32x4 products = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (half & 1) {
             const int slot = tile * TILE + c;
-            const float a = as[slot], b = bs[slot], ks = kscale[slot], qs = qscale[slot];
+            const float qs = 1.0f / sqrtf((qscale[slot] + EPS) * (float)d.dk), a = as[slot], b = bs[slot];
+            if (QUERIES) {
+#pragma unroll
+                for (int i = 0; i < DK / TILE; ++i)
+                    products = mfma16(*reinterpret_cast<const f32x4 *>(q_tile + i * TILE), *reinterpret_cast<const f32x4 *>(k_tile + i * TILE), products);
+            }
             float ahead = a, behind = moved<0x101>(a, 1.0f);   // products up to here, and of those behind
             ahead *= moved<0x111>(ahead, 1.0f);
             behind *= moved<0x101>(behind, 1.0f);
@@ -319,26 +326,43 @@ struct Block {
             behind *= moved<0x104>(behind, 1.0f);
             ahead *= moved<0x118>(ahead, 1.0f);
             behind *= moved<0x108>(behind, 1.0f);
-            from[slot] = ahead;
-            to[slot] = behind;
-            key_reads[slot] = b * ahead * ks;
-            query_reads[slot] = ahead * qs;
-            key_takes[slot] = behind * ks;
-            if (c == TILE - 1) wholes[tile] = ahead;
-        }
-        const f32x4 decay = between(as + tile * TILE, g, c), b = four(bs, tile, g), ks = four(kscale, tile, g), qs = four(qscale, tile, g);
-        const float kc = kscale[tile * TILE + c];
-        float *A = As + tile * TILE * SIDE, *T = Ts + tile * TILE * SIDE, *P = Ps + tile * TILE * SIDE;
+            if (g == 0) {
+                from[slot] = ahead;
+                to[slot] = behind;
+                key_lengths[slot] = kc;
+                query_lengths[slot] = qs;
+                key_reads[slot] = b * ahead * kc;
+                query_reads[slot] = ahead * qs;
+                key_takes[slot] = behind * kc;
+                if (c == TILE - 1) wholes[tile] = ahead;
+            }
+            if (QUERIES) {
+                const f32x4 squares = four(qscale, tile, g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 4 * g + r;
-            A[i * SIDE + c] = i > c ? b[r] * ks[r] * (kc * kk[r]) * decay[r] : 0.0f;
-            if (QUERIES) P[i * SIDE + c] = i >= c ? qs[r] * (kc * qk[r]) * decay[r] : 0.0f;
-        }
-        __builtin_amdgcn_wave_barrier();
-        const f32x4 x = invert(A, g, c);
+                for (int r = 0; r < 4; ++r) {
+                    const float qi = 1.0f / sqrtf((squares[r] + EPS) * (float)d.dk);
+                    Ps[(tile * TILE + 4 * g + r) * SIDE + c] = 4 * g + r >= c ? qi * (kc * products[r]) * decay[r] : 0.0f;
+                }
+            }
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) T[(4 * g + r) * SIDE + c] = x[r];
+            for (int i = 0; i < DK / TILE; ++i) {
+                const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + i * TILE);
+                products = mfma16(k, k, products);
+            }
+            const f32x4 b = four(bs, tile, g), squares = four(kscale, tile, g);
+            float *A = As + tile * TILE * SIDE;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float ki = 1.0f / sqrtf(squares[r] + EPS);
+                A[(4 * g + r) * SIDE + c] = 4 * g + r > c ? b[r] * ki * (kc * products[r]) * decay[r] : 0.0f;
+            }
+            __builtin_amdgcn_wave_barrier();
+            const f32x4 x = invert(A, g, c);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Ts[(tile * TILE + 4 * g + r) * SIDE + c] = x[r];
+        }
     }
     MRL_DEV bool cut_ahead(int tile) const { return span == 1 && as[tile * TILE] == 0.0f; }   // hides whatever the state holds
 };
@@ -401,16 +425,16 @@ MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
 }
 
 // S^T k of a tile's 16 keys (or queries), unscaled: [row of the tile][column of S]
-template <int DK, int TILES>
-MRL_DEV f32x4 ask(const Block<DK, TILES> &block, const float *rows, int tile, int g, int c, const f32x4 (&S)[DK / TILE]) {
+template <int DK, int TILES, bool KEEPS>
+MRL_DEV f32x4 ask(const Block<DK, TILES, KEEPS> &block, const float *rows, int tile, int g, int c, const f32x4 (&S)[DK / TILE]) {
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < DK / TILE; ++i) x = mfma16(*reinterpret_cast<const f32x4 *>(rows + (tile * TILE + c) * block.ROW + i * TILE + 4 * g), S[i], x);
     return x;
 }
 // S0 + sum_i k[i] x[i]^T over a tile's keys (or queries), unscaled
-template <int DK, int TILES>
-MRL_DEV void add(const Block<DK, TILES> &block, const float *rows, int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) {
+template <int DK, int TILES, bool KEEPS>
+MRL_DEV void add(const Block<DK, TILES, KEEPS> &block, const float *rows, int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) {
 #pragma unroll
     for (int i = 0; i < DK / TILE; ++i) {
         f32x4 k;
@@ -420,8 +444,8 @@ MRL_DEV void add(const Block<DK, TILES> &block, const float *rows, int tile, int
     }
 }
 // U[4 g + r][c] of a tile; read: b F S0^T k, what the keys read of the state
-template <int DK, int TILES>
-MRL_DEV f32x4 solve(const Block<DK, TILES> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
+template <int DK, int TILES, bool KEEPS>
+MRL_DEV f32x4 solve(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
     const f32x4 b = block.four(block.bs, tile, g), reads = block.four(block.key_reads, tile, g);
     f32x4 x;
 #pragma unroll
@@ -433,8 +457,8 @@ MRL_DEV f32x4 solve(const Block<DK, TILES> &block, int tile, int g, int c, const
     return mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 }
 // S0 becomes S1
-template <int DK, int TILES>
-MRL_DEV void go_on(const Block<DK, TILES> &block, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
+template <int DK, int TILES, bool KEEPS>
+MRL_DEV void go_on(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
     u *= block.four(block.key_takes, tile, g);
     const float whole = block.wholes[tile];
 #pragma unroll

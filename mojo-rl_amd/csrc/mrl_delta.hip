@@ -86,10 +86,10 @@ enum { OUTPUTS, STATES, ENDS };   // of all steps; ahead of every block; M and B
 // A workgroup goes through a part's steps of one head of one environment; each of its wavefronts keeps 16 columns of the state in registers,
 // all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.
 template <class E, int DK, int TILES, int WHAT>
-__global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kernel(Delta d, Parts parts, int column_groups, float *states, int blocks) {
+__global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Parts parts, int column_groups, float *states, int blocks) {
     extern __shared__ float lds[];
     constexpr int B = DK / TILE, STEPS = TILE * TILES;
-    Block<DK, TILES> block(lds);
+    Block<DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % parts.count, nh = at_part / parts.count;
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, DK == 128 ? 2 : 3) void tiles_kern
             continue;   // the same block again, one step to a tile
         }
         anew(g, c);
-        for (int tile = w; tile < TILES; tile += W) block.template prepare<WHAT == OUTPUTS>(tile, g, c);
+        for (int half = w; half < block.HALVES; half += W) block.template prepare<WHAT == OUTPUTS>(d, half, g, c);
         __syncthreads();
 #pragma unroll 1
         for (int tile = 0; tile < TILES; ++tile) {
@@ -247,7 +247,7 @@ void launch_step(const mrl_ctx *ctx, const Delta &d) {
 template <class E, int DK, int TILES, int WHAT>
 void launch_tiles(const mrl_ctx *ctx, const Delta &d, const Parts &p, float *states = nullptr, int blocks = 0) {
     const int tiles = column_tiles(d.dv) + (WHAT == ENDS ? DK / TILE : 0), waves = std::min(MOST_WAVES, tiles), groups = (tiles + waves - 1) / waves;
-    hipLaunchKernelGGL((tiles_kernel<E, DK, TILES, WHAT>), dim3(d.N * d.H * p.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, TILES), ctx->stream, d, p,
+    hipLaunchKernelGGL((tiles_kernel<E, DK, TILES, WHAT>), dim3(d.N * d.H * p.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, TILES, false), ctx->stream, d, p,
                        groups, states, blocks);
 }
 template <class E, int DK, int TILES>

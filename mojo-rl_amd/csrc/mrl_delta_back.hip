@@ -61,8 +61,8 @@ MRL_DEV float sum_ahead(float x) {
 }
 
 // What a tile's columns make of dO and dS1: read = L dS1^T k, dX, and dS1 becomes dS0.
-template <int DK, int TILES>
-MRL_DEV void pull(const Block<DK, TILES> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
+template <int DK, int TILES, bool KEEPS>
+MRL_DEV void pull(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
     read = ask(block, block.K, tile, g, c, dS) * block.four(block.key_takes, tile, g);
     f32x4 p_column, t_column;
 #pragma unroll
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
     extern __shared__ float lds[];
     constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES;
     const Delta &d = p.d;
-    Block<DK, TILES> block(lds);
+    Block<DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % p.parts.count, nh = at_part / p.parts.count;
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
                 continue;
             }
             anew(g, c);
-            for (int tile = w; tile < TILES; tile += W) block.template prepare<true>(tile, g, c);
+            for (int half = w; half < block.HALVES; half += W) block.template prepare<true>(d, half, g, c);
             __syncthreads();
 #pragma unroll
             for (int tile = TILES - 1; tile >= 0; --tile) {
@@ -160,7 +160,7 @@ inline int waves_of(int DK, int dv) { return std::max(column_tiles(dv), std::min
 constexpr int DOTS = 5;   // q dq, k dk, e, f, U dX
 size_t back_floats(int DK, int dv) {
     const int columns = TILE * column_tiles(dv) + 4, W = waves_of(DK, dv);
-    return rows_floats(DK, tiles_backward(DK)) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
+    return rows_floats(DK, tiles_backward(DK), true) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
 }
 
 // EK: the type of the gradients of query and key (float where a group's are summed later)
@@ -170,11 +170,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES, OWN = B <= 4 ? 1 : 2;   // OWN: row tiles of a wavefront
     constexpr bool BOTH = both_states(DK);
     const Delta &d = p.d;
-    Block<DK, TILES> block(lds);
+    Block<DK, TILES, true> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, tiles = (d.dv + TILE - 1) / TILE;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int stride = TILE * tiles + 4;
-    float *const states = lds + rows_floats(DK, TILES), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
+    float *const states = lds + rows_floats(DK, TILES, true), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
     float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE, *const crossing = dPs + TILE * SIDE;
     float *const dots = crossing + TILE, *const wholes = dots + 2 * DOTS * TILE * W;   // [2][DOTS][W][16], [2][W]: two tiles' in turn
     const int at_part = blockIdx.x, part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
@@ -260,13 +260,13 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     load();
                     __syncthreads();
                     if (ahead == round) break;
-                    for (int tile = w; tile < TILES; tile += W) block.template prepare<false>(tile, g, c);
+                    for (int half = w; half < block.HALVES; half += W) block.template prepare<false>(d, half, g, c);
                     __syncthreads();
                     forwards(std::false_type{});
                 }
             }
             anew(g, c);
-            for (int tile = w; tile < TILES; tile += W) block.template prepare<true>(tile, g, c);
+            for (int half = w; half < block.HALVES; half += W) block.template prepare<true>(d, half, g, c);
             __syncthreads();
             if (owns) forwards(std::true_type{});
 #pragma unroll
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     }
                 }
                 // ---- the tile's own pairs, the lengths, gates and rates
-                const f32x4 ks = block.four(block.kscale, tile, g), qs = block.four(block.qscale, tile, g);
+                const f32x4 ks = block.four(block.key_lengths, tile, g), qs = block.four(block.query_lengths, tile, g);
                 f32x4 q_dot = zero, k_dot = zero;
                 for (int t = 0; t < tiles; ++t) {
                     q_dot += *reinterpret_cast<const f32x4 *>(dot + t * TILE + 4 * g);
@@ -484,7 +484,7 @@ void launch(const mrl_ctx *ctx, const Back &p) {
 template <class E, int DK>
 void launch_chain(const mrl_ctx *ctx, const Back &p) {
     const int tiles = column_tiles(p.d.dv), waves = std::min(4, tiles), groups = (tiles + waves - 1) / waves;
-    hipLaunchKernelGGL((chain_kernel<E, DK>), dim3(p.d.N * p.d.H * p.parts.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, tiles_backward(DK)), ctx->stream, p, groups);
+    hipLaunchKernelGGL((chain_kernel<E, DK>), dim3(p.d.N * p.d.H * p.parts.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, tiles_backward(DK), false), ctx->stream, p, groups);
 }
 template <class E>
 void launch_chain(const mrl_ctx *ctx, const Back &p) {
