@@ -97,6 +97,13 @@ MRL_DEV bool is_cut(const Delta &d, int t, int n) {
     return row != nullptr && (t > 0 ? row[(long)(t - 1) * d.N + n] : row[n]) > 0.5f;
 }
 
+// This workgroup's number among all, so that neighbours, whose rows share cache lines, are on one of the eight XCDs (workgroups are dealt to them in
+// turn).
+MRL_DEV int group_number() {
+    const int xcd = blockIdx.x & 7, share = gridDim.x >> 3, rest = gridDim.x & 7;
+    return xcd * share + min(xcd, rest) + (int)(blockIdx.x >> 3);
+}
+
 // What is worked out from these is worked out here and not ahead of the loop around: kept there, the addresses and comparisons of all of a
 // block's phases take more registers than the state.
 MRL_DEV void anew(int &x) { asm volatile("" : "+v"(x)); }
@@ -136,26 +143,28 @@ MRL_DEV float sum_lanes(float x) {
     return x;
 }
 
-// G[4 g + r][n], 0 above the diagonal
+// G[4 g + r][n], 0 above the diagonal: in the row of 16 lanes g the products of the a behind n and ahead of 4 g, and from there on those of the group's own.
 MRL_DEV f32x4 between(const float *a, int g, int n) {
-    float run = 1.0f;
-    f32x4 own = {1.0f, 1.0f, 1.0f, 1.0f};
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(a + 4 * p);
-        if (p == g) own = x;
-        if (p < g) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) run = 4 * p + r > n ? run * x[r] : run;
-        }
-    }
+    float mine = n < 4 * g ? a[n] : 1.0f;
+    float run = moved<0x101>(mine, 1.0f);
+    run *= moved<0x101>(run, 1.0f);
+    run *= moved<0x102>(run, 1.0f);
+    run *= moved<0x104>(run, 1.0f);
+    run *= moved<0x108>(run, 1.0f);
+    const f32x4 own = *reinterpret_cast<const f32x4 *>(a + 4 * g);
     f32x4 out;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        run = 4 * g + r > n ? run * own[r] : run;
+        run *= 4 * g + r > n ? own[r] : 1.0f;
         out[r] = 4 * g + r >= n ? run : 0.0f;
     }
     return out;
+}
+
+// 1 / sqrt(x): the hardware's, a step off at most, and one of Newton's steps (0 for an infinity, like the division)
+MRL_DEV float one_over_root(float x) {
+    const float y = __builtin_amdgcn_rsqf(x);
+    return x < 0x1p127f ? fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y) : y;
 }
 
 // the sum over the four lane groups, in all of them
@@ -164,6 +173,17 @@ MRL_DEV float sum_groups(float x) {
     x = __uint_as_float(half[0]) + __uint_as_float(half[1]);
     const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(row[0]) + __uint_as_float(row[1]);
+}
+
+// of two values, at little more than the price of one: their halves trade places first
+MRL_DEV void sum_groups(float &x, float &y) {
+    const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    const float both = __uint_as_float(half[0]) + __uint_as_float(half[1]);   // x's in the lower half of the lanes, y's in the upper
+    const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(both), __float_as_uint(both), false, false);
+    const float sum = __uint_as_float(row[0]) + __uint_as_float(row[1]);
+    const auto back = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    x = __uint_as_float(back[0]);
+    y = __uint_as_float(back[1]);
 }
 
 // Rows 4 g + r of column n of (1 + A)^-1, A [16][SIDE] strictly lower triangular: forward substitution, which is as exact as its terms allow
@@ -180,9 +200,14 @@ MRL_DEV f32x4 invert(const float *A, int g, int n) {
             const float *row = A + (4 * p + r) * SIDE;
             own[r] = *reinterpret_cast<const f32x4 *>(row + 4 * p);
             const f32x4 v = *reinterpret_cast<const f32x4 *>(row + 4 * g);   // (x is 0 for rows not solved yet)
-            if (p > 0) sum[r] = sum_groups(fmaf(v[0], x[0], fmaf(v[1], x[1], fmaf(v[2], x[2], v[3] * x[3]))));
-            sum[r] = (4 * p + r == n ? 1.0f : 0.0f) - (p > 0 ? sum[r] : 0.0f);
+            if (p > 0) sum[r] = fmaf(v[0], x[0], fmaf(v[1], x[1], fmaf(v[2], x[2], v[3] * x[3])));
         }
+        if (p > 0) {
+            sum_groups(sum[0], sum[1]);
+            sum_groups(sum[2], sum[3]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = (4 * p + r == n ? 1.0f : 0.0f) - (p > 0 ? sum[r] : 0.0f);
 #pragma unroll
         for (int r = 1; r < 4; ++r)
 #pragma unroll
@@ -306,12 +331,12 @@ struct Block {
     MRL_DEV void prepare(const Delta &d, int half, int g, int c) {
         const int tile = half >> 1;
         const float *k_tile = K + (tile * TILE + c) * ROW + 4 * g, *q_tile = Q + (tile * TILE + c) * ROW + 4 * g;
-        const float kc = 1.0f / sqrtf(kscale[tile * TILE + c] + EPS);
+        const float kc = one_over_root(kscale[tile * TILE + c] + EPS);
         const f32x4 decay = between(as + tile * TILE, g, c);
         f32x4 products = {0.0f, 0.0f, 0.0f, 0.0f};
         if (half & 1) {
             const int slot = tile * TILE + c;
-            const float qs = 1.0f / sqrtf((qscale[slot] + EPS) * (float)d.dk), a = as[slot], b = bs[slot];
+            const float qs = one_over_root((qscale[slot] + EPS) * (float)d.dk), a = as[slot], b = bs[slot];
             if (QUERIES) {
 #pragma unroll
                 for (int i = 0; i < DK / TILE; ++i)
@@ -340,7 +365,7 @@ struct Block {
                 const f32x4 squares = four(qscale, tile, g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float qi = 1.0f / sqrtf((squares[r] + EPS) * (float)d.dk);
+                    const float qi = one_over_root((squares[r] + EPS) * (float)d.dk);
                     Ps[(tile * TILE + 4 * g + r) * SIDE + c] = 4 * g + r >= c ? qi * (kc * products[r]) * decay[r] : 0.0f;
                 }
             }
@@ -354,7 +379,7 @@ struct Block {
             float *A = As + tile * TILE * SIDE;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float ki = 1.0f / sqrtf(squares[r] + EPS);
+                const float ki = one_over_root(squares[r] + EPS);
                 A[(4 * g + r) * SIDE + c] = 4 * g + r > c ? b[r] * ki * (kc * products[r]) * decay[r] : 0.0f;
             }
             __builtin_amdgcn_wave_barrier();

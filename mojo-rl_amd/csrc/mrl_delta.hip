@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void step_kernel(Delta d, int units, int colum
             sq[j] += __shfl_xor(sq[j], s);
         }
     }
-    const float ks = 1.0f / sqrtf(kk + EPS), qs = 1.0f / sqrtf((qq + EPS) * (float)d.dk);
+    const float ks = one_over_root(kk + EPS), qs = one_over_root((qq + EPS) * (float)d.dk);
     f32x4 u, o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
     Block<DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
-    const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % parts.count, nh = at_part / parts.count;
+    const int number = group_number(), group = number % column_groups, at_part = number / column_groups, part = at_part % parts.count, nh = at_part / parts.count;
     const int n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK), tiles = (d.dv + TILE - 1) / TILE;
     const int column_tile = group * W + w, column = column_tile * TILE + c;
     const bool live = column < d.dv;
@@ -122,9 +122,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
     block.span = TILE;
     for (block.t0 = begin; block.t0 < end;) {
         if (WHAT == STATES && block.t0 == begin) {
-            const int number = begin / STEPS;
             if (column_tile < tiles) {
-                float *to = states + ((((long)nh * blocks + number) * tiles + column_tile) * B * 64 + lane) * 4;
+                float *to = states + ((((long)nh * blocks + begin / STEPS) * tiles + column_tile) * B * 64 + lane) * 4;
 #pragma unroll
                 for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = S[i];
             }

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
     Block<DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
-    const int group = blockIdx.x % column_groups, at_part = blockIdx.x / column_groups, part = at_part % p.parts.count, nh = at_part / p.parts.count;
+    const int at = group_number(), group = at % column_groups, at_part = at / column_groups, part = at_part % p.parts.count, nh = at_part / p.parts.count;
     const int n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK), tiles = (d.dv + TILE - 1) / TILE, column_tile = group * W + w, column = column_tile * TILE + c;
     const bool live = column < d.dv;
     const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     float *const states = lds + rows_floats(DK, TILES, true), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
     float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE, *const crossing = dPs + TILE * SIDE;
     float *const dots = crossing + TILE, *const wholes = dots + 2 * DOTS * TILE * W;   // [2][DOTS][W][16], [2][W]: two tiles' in turn
-    const int at_part = blockIdx.x, part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
+    const int at_part = group_number(), part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
     const bool owns = w < tiles;   // columns; the other wavefronts have rows only
     const int column = w * TILE + c;
     const bool live = column < d.dv;
