@@ -16,6 +16,7 @@
 // its registers is the B operand of a product that contracts its rows, and the A operand of such a product is four neighbouring
 // values of a row.
 #pragma once
+#include <limits.h>
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
 #include "gate.hpp"
@@ -102,6 +103,23 @@ MRL_DEV bool is_cut(const Delta &d, int t, int n) {
 MRL_DEV int group_number() {
     const int xcd = blockIdx.x & 7, share = gridDim.x >> 3, rest = gridDim.x & 7;
     return xcd * share + min(xcd, rest) + (int)(blockIdx.x >> 3);
+}
+
+// The last (or the first) step of [begin, end) that a cut is ahead of, -1 where there is none; by a whole workgroup.  `found`: an int in LDS.
+template <bool LAST>
+MRL_DEV int find_cut(const Delta &d, int begin, int end, int n, int *found) {
+    if (d.dones == nullptr && d.prev_dones == nullptr) return -1;
+    if (threadIdx.x == 0) *found = LAST ? -1 : INT_MAX;
+    __syncthreads();
+    int mine = LAST ? -1 : INT_MAX;
+    for (int t = begin + (int)threadIdx.x; t < end; t += blockDim.x)
+        if (is_cut(d, t, n)) mine = LAST ? max(mine, t) : min(mine, t);
+    if (LAST && mine >= 0) atomicMax(found, mine);
+    if (!LAST && mine < INT_MAX) atomicMin(found, mine);
+    __syncthreads();
+    const int at = *found;
+    __syncthreads();
+    return at == INT_MAX ? -1 : at;
 }
 
 // What is worked out from these is worked out here and not ahead of the loop around: kept there, the addresses and comparisons of all of a
@@ -495,7 +513,8 @@ MRL_DEV void go_on(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c,
 // Where heads and environments leave CUs without work the steps are cut into parts of `per` blocks.  A part takes the state S ahead of it to
 // M S + B, a product of the steps' contractions and what it makes of a zero state; M and B of all parts come side by side (M as the part's result for
 // the columns of the identity, without values), a second launch goes through them, M S + B, and then every part has its first state.  The
-// same, from the last part to the first and with M^T, for the gradient of the state.  A part with a cut has M = 0, and says so.
+// same, from the last part to the first and with M^T, for the gradient of the state.  A part with a cut has M = 0, and says so; its B comes from the
+// steps from the last cut on alone, and the gradient of the state ahead of it from those up to the first cut.
 // States are kept as lanes hold them: [environment and head][part][tile of 16 columns][tile of 16 rows][lane][4].
 struct Parts {
     int count, per;      // count 1: no parts
@@ -508,12 +527,13 @@ inline int column_tiles(int dv) { return (dv + TILE - 1) / TILE; }
 inline int blocks_of(int T, int tiles) { return (T + TILE * tiles - 1) / (TILE * tiles); }
 constexpr int floats_of(int DK) { return DK * TILE; }   // of a column tile
 
-// How many parts: as many as fill the card twice, where that is four at least.
+// How many parts: as many as give every CU PART_GROUPS workgroups, where that is four at least.
+constexpr int PART_GROUPS = 2, MOST_PARTS = 1024;
 inline Parts parts_of(const mrl_ctx *ctx, const mrl_delta *r, int tiles) {
     Parts p = {};
     const int blocks = blocks_of(r->T, tiles), tile_columns = column_tiles(r->value_dim);
     const long groups = (long)r->N * r->heads * ((tile_columns + 3) / 4);
-    const long want = std::min<long>(blocks, 2L * ctx->n_cus / groups);
+    const long want = std::min<long>({(long)blocks, (long)PART_GROUPS * ctx->n_cus / groups, (long)MOST_PARTS});
     p.count = 1;
     p.per = blocks;
     if (want < 4) return p;

@@ -118,7 +118,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
     E *const outs = (E *)d.out + n * d.out_ld + (long)h * d.dv + column;
     int begin = part * parts.per * STEPS;   // of the block
     const int end = min(d.T, begin + parts.per * STEPS);
-    bool cut = false;
+    if (WHAT == ENDS) {
+        const int last = find_cut<true>(d, begin, end, n, (int *)lds);
+        if (threadIdx.x == 0 && group == 0) parts.cuts[at_part] = last >= 0;
+        if (last >= 0) {
+            if (group * W >= tiles) return;   // nobody asks for M
+            begin = last / STEPS * STEPS;
+        }
+    }
     block.span = TILE;
     for (block.t0 = begin; block.t0 < end;) {
         if (WHAT == STATES && block.t0 == begin) {
@@ -162,13 +169,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
             }
             go_on(block, tile, g, c, u, S);
             if (WHAT == OUTPUTS) store_values(d, block, outs, (long)d.N * d.out_ld, live, tile, g, o);
-            if (WHAT == ENDS) {
-#pragma unroll
-                for (int i = 0; i < TILE; i += 4) {
-                    const f32x4 a = *reinterpret_cast<const f32x4 *>(block.as + tile * TILE + i);
-                    cut |= a[0] == 0.0f || a[1] == 0.0f || a[2] == 0.0f || a[3] == 0.0f;
-                }
-            }
         }
         block.t0 += TILES * block.span;
         if (block.t0 >= begin + STEPS) {
@@ -182,7 +182,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
         float *to = parts.ends + (((long)at_part * (tiles + B) + column_tile) * B * 64 + lane) * 4;
 #pragma unroll
         for (int i = 0; i < B; ++i) *reinterpret_cast<f32x4 *>(to + i * 256) = S[i];
-        if (threadIdx.x == 0 && group == 0) parts.cuts[at_part] = cut;
     }
     if (WHAT != OUTPUTS || d.state_out == nullptr || !live || part != parts.count - 1) return;
 #pragma unroll
@@ -199,24 +198,26 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
 template <int DK, bool BACK>
 __global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, const float *first, const float *local) {
     __shared__ f32x4 S[2][DK / TILE][64];
+    __shared__ int cuts[MOST_PARTS];
     constexpr int B = DK / TILE;
     const int tiles = (d.dv + TILE - 1) / TILE, column_tile = blockIdx.x % tiles, nh = blockIdx.x / tiles;
     const int i = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, column = column_tile * TILE + c;
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int part = threadIdx.x; part < parts.count; part += DK * 4) cuts[part] = parts.cuts[(long)nh * parts.count + part];
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f}, next, m[B];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int row = i * TILE + 4 * g + r;
         if (first != nullptr && column < d.dv && row < d.dk) s[r] = first[((long)nh * d.dk + row) * d.dv + column];
     }
-    for (int step = 0; step < parts.count; ++step) {
-        const int part = BACK ? parts.count - 1 - step : step;
+    __syncthreads();
+    const auto part_of = [&](int step) { return BACK ? parts.count - 1 - step : step; };
+    const auto ask = [&](int step) {   // B and M of a step, while the one ahead of it is worked out
+        if (step >= parts.count - 1) return;
+        const int part = part_of(step);
         const long at = (long)nh * parts.count + part;
-        *reinterpret_cast<f32x4 *>(parts.starts + (((at * tiles + column_tile) * B + i) * 64 + lane) * 4) = s;
-        if (step == parts.count - 1) break;
-        f32x4 (&here)[B][64] = S[step & 1];
-        here[i][lane] = s;
         const float *const ends = parts.ends + at * (tiles + B) * B * 256, *const M = ends + (long)tiles * B * 256;   // M: [column tile][row tile][lane][4]
-        f32x4 m[B];
+        next = *reinterpret_cast<const f32x4 *>(BACK ? local + (((at * tiles + column_tile) * B + i) * 64 + lane) * 4 : ends + ((column_tile * B + i) * 64 + lane) * 4);
+        if (cuts[part]) return;
 #pragma unroll
         for (int k = 0; k < B; ++k) {
             // the operand's row c and contracted 4 g .. 4 g + 3: of M^T four neighbouring rows of a column of M, as they lie; of M a row's columns
@@ -225,12 +226,24 @@ __global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, con
 #pragma unroll
                 for (int r = 0; r < 4; ++r) m[k][r] = M[((k * B + i) * 64 + 16 * (c >> 2) + 4 * g + r) * 4 + (c & 3)];
         }
-        s = *reinterpret_cast<const f32x4 *>(BACK ? local + (((at * tiles + column_tile) * B + i) * 64 + lane) * 4 : ends + ((column_tile * B + i) * 64 + lane) * 4);
-        __syncthreads();   // (the buffers alternate)
-        if (!parts.cuts[at]) {
+    };
+    ask(0);
+    for (int step = 0; step < parts.count; ++step) {
+        const int part = part_of(step);
+        *reinterpret_cast<f32x4 *>(parts.starts + ((((long)nh * parts.count + part) * tiles + column_tile) * B + i) * 256 + lane * 4) = s;
+        if (step == parts.count - 1) break;
+        f32x4 after = next, mine[B];
 #pragma unroll
-            for (int k = 0; k < B; ++k) s = mfma16(m[k], here[k][lane], s);
+        for (int k = 0; k < B; ++k) mine[k] = m[k];
+        ask(step + 1);
+        if (!cuts[part]) {
+            f32x4 (&here)[B][64] = S[step & 1];
+            here[i][lane] = s;
+            __syncthreads();   // (the buffers alternate)
+#pragma unroll
+            for (int k = 0; k < B; ++k) after = mfma16(mine[k], here[k][lane], after);
         }
+        s = after;
     }
 }
 

@@ -117,7 +117,9 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
     f32x4 dS[B], dO[TILES];
 #pragma unroll
     for (int i = 0; i < B; ++i) dS[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int number = min(p.blocks, (part + 1) * p.parts.per) - 1; number >= part * p.parts.per; --number) {
+    const int first_block = part * p.parts.per, last_block = min(p.blocks, first_block + p.parts.per) - 1;
+    const int cut = find_cut<false>(d, first_block * STEPS, min(d.T, (last_block + 1) * STEPS), n, (int *)lds);
+    for (int number = cut >= 0 ? cut / STEPS : last_block; number >= first_block; --number) {
         const int begin = number * STEPS, end = min(begin + STEPS, d.T);
         block.t0 = begin;
         block.span = TILE;
