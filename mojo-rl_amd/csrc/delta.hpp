@@ -17,6 +17,7 @@
 // values of a row.
 #pragma once
 #include <limits.h>
+#include <cmath>
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
 #include "gate.hpp"
@@ -527,13 +528,14 @@ inline int column_tiles(int dv) { return (dv + TILE - 1) / TILE; }
 inline int blocks_of(int T, int tiles) { return (T + TILE * tiles - 1) / (TILE * tiles); }
 constexpr int floats_of(int DK) { return DK * TILE; }   // of a column tile
 
-// How many parts: as many as give every CU PART_GROUPS workgroups, where that is four at least.
+// How many parts: as many as give every CU PART_GROUPS workgroups, but no more than sqrt(20 blocks): a part takes some 10 us for each of its
+// blocks, twice, and the way through the parts 1 us for each of them.
 constexpr int PART_GROUPS = 2, MOST_PARTS = 1024;
 inline Parts parts_of(const mrl_ctx *ctx, const mrl_delta *r, int tiles) {
     Parts p = {};
     const int blocks = blocks_of(r->T, tiles), tile_columns = column_tiles(r->value_dim);
     const long groups = (long)r->N * r->heads * ((tile_columns + 3) / 4);
-    const long want = std::min<long>({(long)blocks, (long)PART_GROUPS * ctx->n_cus / groups, (long)MOST_PARTS});
+    const long want = std::min<long>({(long)blocks, (long)PART_GROUPS * ctx->n_cus / groups, (long)std::sqrt(20.0 * blocks), (long)MOST_PARTS});
     p.count = 1;
     p.per = blocks;
     if (want < 4) return p;

@@ -279,7 +279,30 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
                 float *const dot = dots + turn * DOTS * TILE * W;
                 const f32x4 b = block.four(block.bs, tile, g);
-                f32x4 dS1[BOTH ? 1 : B];
+                const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g);
+                f32x4 dq[OWN], dk[OWN];
+                const auto read_by_rows = [&]() {   // L dS1 U of this wavefront's rows
+#pragma unroll
+                    for (int o = 0; o < OWN; ++o) {
+                        const int i = w + o * W;
+                        dk[o] = zero;
+                        if (i >= B) continue;
+                        for (int t = 0; t < tiles; ++t)
+                            dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
+                                           *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), dk[o]);
+                        dk[o] *= to;
+                    }
+                };
+                if (owns) {
+                    spread(behind, dS);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) Us[(4 * g + r) * stride + column] = U[tile][r];
+                }
+                if constexpr (!BOTH) {   // S0 comes in dS1's place
+                    __syncthreads();
+                    read_by_rows();
+                    __syncthreads();
+                }
                 // ---- by columns
                 if (owns) {
                     f32x4 out = ask(block, block.Q, tile, g, c, kept[tile]) * block.four(block.query_reads, tile, g);
@@ -293,11 +316,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     s_ds = sum_groups(sum16(s_ds));
                     if (lane == 0) wholes[turn * W + w] = s_ds;
                     spread(states, kept[tile]);
-                    if constexpr (BOTH) spread(behind, dS);
-                    else {
-#pragma unroll
-                        for (int i = 0; i < B; ++i) dS1[i] = dS[i];
-                    }
                     f32x4 read, dX;
                     pull(block, tile, g, c, dO[tile], dS, read, dX);
                     store_values(d, block, (E *)p.value + n * p.value_ld + (long)h * d.dv + column, (long)d.N * p.value_ld, live, tile, g, b * dX);
@@ -306,7 +324,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         const int at = (4 * g + r) * stride + column;
                         dOs[at] = dO[tile][r];
                         dXs[at] = dX[r];
-                        Us[at] = U[tile][r];
                         const float sums[DOTS] = {sum16(dO[tile][r] * out[r]), sum16(dX[r] * fmaf(2.0f, U[tile][r], -b[r] * V[tile][r])), sum16(fmaf(-dX[r], reads[tile][r], e[r])),
                                                   sum16(U[tile][r] * read[r]), sum16(U[tile][r] * dX[r])};
                         if (c == 0) {
@@ -317,27 +334,21 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 }
                 __syncthreads();
                 // ---- by rows of the states, their terms of dq and dk; by one wavefront, dA and dP
-                const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g);
-                f32x4 dq[OWN], dk[OWN];
+                if constexpr (BOTH) read_by_rows();
 #pragma unroll
                 for (int o = 0; o < OWN; ++o) {
                     const int i = w + o * W;
-                    dq[o] = dk[o] = zero;
+                    dq[o] = zero;
                     if (i >= B) continue;
-                    f32x4 of = zero;
+                    f32x4 reads_by = zero;
                     for (int t = 0; t < tiles; ++t) {
                         const f32x4 s = *reinterpret_cast<const f32x4 *>(states + (i * TILE + c) * stride + t * TILE + 4 * g);
                         dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), s, dq[o]);
-                        dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), s, dk[o]);
-                        if constexpr (BOTH)
-                            of = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
-                                        *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), of);
+                        reads_by = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), s, reads_by);
                     }
+                    dq[o] *= from;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        dq[o][r] *= from[r];
-                        dk[o][r] = fmaf(to[r], of[r], -from[r] * b[r] * dk[o][r]);
-                    }
+                    for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(-from[r] * b[r], reads_by[r], dk[o][r]);
                 }
                 if (w == pairs_by) {
                     f32x4 dA = zero, dP = zero;
@@ -368,21 +379,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     }
                 }
                 __syncthreads();
-                if constexpr (!BOTH) {   // dS1 in S0's place
-                    if (owns) spread(behind, dS1);
-                    __syncthreads();
-#pragma unroll
-                    for (int o = 0; o < OWN; ++o) {
-                        const int i = w + o * W;
-                        if (i >= B) continue;
-                        f32x4 of = zero;
-                        for (int t = 0; t < tiles; ++t)
-                            of = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
-                                        *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), of);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(to[r], of[r], dk[o][r]);
-                    }
-                }
                 // ---- the tile's own pairs, the lengths, gates and rates
                 const f32x4 ks = block.four(block.key_lengths, tile, g), qs = block.four(block.query_lengths, tile, g);
                 f32x4 q_dot = zero, k_dot = zero;
