@@ -27,6 +27,8 @@ namespace delta {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 struct bf16_t { unsigned short bits; };
@@ -84,7 +86,6 @@ MRL_DEV void store4(float *p, f32x4 x, int n) {
     }
 }
 MRL_DEV void store4(bf16_t *p, f32x4 x, int n) {
-    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
     const u16x4u v = __builtin_bit_cast(u16x4u, __builtin_convertvector(x, bf16x4));
     if (n >= 4) *reinterpret_cast<u16x4u *>(p) = v;
     else {
@@ -131,6 +132,19 @@ MRL_DEV void anew(int &x, int &y) {
     anew(y);
 }
 
+// Results of the matrix cores are not read for the ten instructions behind this.  The compiler sees to that within a block and mostly across
+// branches, but in the backward kernels, of many blocks, it has been seen to read a result one instruction behind a branch: products whose next
+// reader may be behind one end with it.  (Only the last needs the wait, whichever it is: one wait behind all of them.)
+MRL_DEV void settle(f32x4 &x) { asm volatile("s_nop 9" : "+v"(x)); }
+template <int N>
+MRL_DEV void settle(f32x4 (&x)[N]) {
+    if constexpr (N == 1) settle(x[0]);
+    else if constexpr (N == 2) asm volatile("s_nop 9" : "+v"(x[0]), "+v"(x[1]));
+    else if constexpr (N == 4) asm volatile("s_nop 9" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+    else asm volatile("s_nop 9" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+    static_assert(N == 1 || N == 2 || N == 4 || N == 8, "the row tiles of a state");
+}
+
 MRL_DEV f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // c + A B over 16 values of the contracted index
 MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
@@ -143,7 +157,6 @@ MRL_DEV f32x4 mfma16(const f32x4 a, const f32x4 b, f32x4 c) {
 constexpr int tiles_forward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int tiles_backward(int DK) { return DK >= 64 ? 2 : 4; }
 constexpr int SIDE = TILE + 4;        // floats from a row of a 16 x 16 matrix in LDS to the next
-constexpr size_t rows_floats(int DK, int tiles, bool keeps) { return 2 * TILE * tiles * (DK + 4) + (keeps ? 3 : 2) * tiles * TILE * SIDE + 13 * TILE * tiles + 4; }
 
 // From one lane to another of a row of 16, `missing` where there is none.
 template <int CONTROL>
@@ -237,19 +250,155 @@ MRL_DEV f32x4 invert(const float *A, int g, int n) {
     return x;
 }
 
-// What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.
-// KEEPS: A beside its inverse.
-template <int DK, int TILES_, bool KEEPS>
+// A state (or its gradient) as an operand: fp32 as it is; next to rows of bf16 in three bf16 pieces (mlp_split.hpp), with which products of
+// fp32 accuracy take a fifth of the matrix cores' time: v_mfma_f32_16x16x32_bf16 does in 16 cycles what eight v_mfma_f32_16x16x4_f32 do in 256.  Of
+// two row tiles, lane group g has rows 4 g .. 4 g + 3 of each.
+template <class E, int DK>
+struct Pieces;
+template <int DK>
+struct Pieces<float, DK> {
+    const f32x4 (&S)[DK / TILE];
+    MRL_DEV explicit Pieces(const f32x4 (&s)[DK / TILE]) : S(s) {}
+};
+template <class V, class F>
+MRL_DEV void split(const F x, V (&p)[3]) {
+    F rest = x;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        p[i] = __builtin_convertvector(rest, V);
+        if (i < 2) rest -= __builtin_convertvector(p[i], F);
+    }
+}
+template <int DK>
+struct Pieces<bf16_t, DK> {
+    bf16x8 p[DK / 32][3];
+    MRL_DEV explicit Pieces(const f32x4 (&S)[DK / TILE]) {
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i) split(__builtin_shufflevector(S[2 * i], S[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7), p[i]);
+    }
+};
+template <>
+struct Pieces<bf16_t, 16> {
+    bf16x4 p[3];
+    MRL_DEV explicit Pieces(const f32x4 (&S)[1]) { split(S[0], p); }
+};
+// (Sixteen of the contracted index go as 32, half of them zeros or other pieces: a result of v_mfma_f32_16x16x16_bf16 that is another product's
+// addend has been seen to come too late here, by a part in 2^18 of the sum.)
+MRL_DEV f32x4 mfma_pieces(const bf16x8 a, const bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+MRL_DEV bf16x8 beside(const bf16x4 a, const bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+MRL_DEV bf16x8 alone(const bf16x4 a) { return beside(a, bf16x4{(__bf16)0.0f, (__bf16)0.0f, (__bf16)0.0f, (__bf16)0.0f}); }
+
+// A block's keys or queries in LDS: rows of fp32; of bf16 rows and columns.
+template <class E, int DK, int STEPS>
+struct Rows;
+template <int DK, int STEPS>
+struct Rows<float, DK, STEPS> {
+    static constexpr int ROW = DK + 4;
+    static constexpr size_t FLOATS = (size_t)STEPS * ROW;
+    float *at;
+    MRL_DEV void put(int slot, int column, const f32x4 x) { *reinterpret_cast<f32x4 *>(at + slot * ROW + column) = x; }
+    // rows 4 g + r of a tile, element c of a column tile
+    MRL_DEV f32x4 column(int tile, int i, int g, int c) const {
+        f32x4 k;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) k[r] = at[(tile * TILE + 4 * g + r) * ROW + i * TILE + c];
+        return k;
+    }
+    // products of a tile's rows with another's: [row of this][row of that]
+    MRL_DEV f32x4 with(const Rows &that, int tile, int g, int c) const {
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i)
+            x = mfma16(*reinterpret_cast<const f32x4 *>(at + (tile * TILE + c) * ROW + i * TILE + 4 * g),
+                       *reinterpret_cast<const f32x4 *>(that.at + (tile * TILE + c) * ROW + i * TILE + 4 * g), x);
+        return x;
+    }
+    // S^T k of a tile's 16 rows k: [row of the tile][column of S]
+    MRL_DEV f32x4 ask(int tile, int g, int c, const Pieces<float, DK> &S) const {
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i) x = mfma16(*reinterpret_cast<const f32x4 *>(at + (tile * TILE + c) * ROW + i * TILE + 4 * g), S.S[i], x);
+        return x;
+    }
+    // S + sum_i k[i] x[i]^T over a tile's rows k
+    MRL_DEV void add(int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) const {
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i) S[i] = mfma16(column(tile, i, g, c), x, S[i]);
+        settle(S);
+    }
+};
+template <int DK, int STEPS>
+struct Rows<bf16_t, DK, STEPS> {
+    static constexpr int ROW = DK + 8, TURNED = STEPS + 4;   // elements from a row to the next, and from a column
+    static constexpr size_t FLOATS = ((size_t)STEPS * ROW + (size_t)DK * TURNED) / 2;
+    float *at;
+    MRL_DEV __bf16 *rows() const { return reinterpret_cast<__bf16 *>(at); }
+    MRL_DEV __bf16 *columns() const { return rows() + STEPS * ROW; }
+    MRL_DEV void put(int slot, int column, const f32x4 x) {
+        const bf16x4 v = __builtin_convertvector(x, bf16x4);
+        *reinterpret_cast<bf16x4 *>(rows() + slot * ROW + column) = v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) columns()[(column + i) * TURNED + slot] = v[i];
+    }
+    MRL_DEV bf16x4 row4(int tile, int i, int g, int c) const { return *reinterpret_cast<const bf16x4 *>(rows() + (tile * TILE + c) * ROW + i * TILE + 4 * g); }
+    MRL_DEV bf16x4 column4(int tile, int i, int g, int c) const { return *reinterpret_cast<const bf16x4 *>(columns() + (i * TILE + c) * TURNED + tile * TILE + 4 * g); }
+    MRL_DEV f32x4 column(int tile, int i, int g, int c) const { return __builtin_convertvector(column4(tile, i, g, c), f32x4); }
+    MRL_DEV f32x4 with(const Rows &that, int tile, int g, int c) const {
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (DK == 16) return mfma_pieces(alone(row4(tile, 0, g, c)), alone(that.row4(tile, 0, g, c)), x);
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i)
+            x = mfma_pieces(beside(row4(tile, 2 * i, g, c), row4(tile, 2 * i + 1, g, c)), beside(that.row4(tile, 2 * i, g, c), that.row4(tile, 2 * i + 1, g, c)), x);
+        return x;
+    }
+    MRL_DEV f32x4 ask(int tile, int g, int c, const Pieces<bf16_t, DK> &S) const {
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, small = x;
+        if constexpr (DK == 16) {
+            const bf16x4 k = row4(tile, 0, g, c);
+            return mfma_pieces(beside(k, k), alone(S.p[0]), x) + mfma_pieces(beside(k, k), beside(S.p[1], S.p[2]), small);
+        } else {
+#pragma unroll
+            for (int i = 0; i < DK / 32; ++i) {
+                const bf16x8 k = beside(row4(tile, 2 * i, g, c), row4(tile, 2 * i + 1, g, c));
+                small = mfma_pieces(k, S.p[i][2], small);
+                x = mfma_pieces(k, S.p[i][0], x);
+                small = mfma_pieces(k, S.p[i][1], small);
+            }
+            return x + small;
+        }
+    }
+    // (two pieces of x side by side are 32 of the contracted index, with each key twice)
+    MRL_DEV void add(int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) const {
+        bf16x4 p[3];
+        split(x, p);
+        const bf16x8 upper = beside(p[0], p[1]), lower = alone(p[2]);
+#pragma unroll
+        for (int i = 0; i < DK / TILE; ++i) {
+            const bf16x4 k = column4(tile, i, g, c);
+            S[i] = mfma_pieces(beside(k, k), upper, mfma_pieces(beside(k, k), lower, S[i]));
+        }
+        settle(S);
+    }
+};
+template <class E>
+constexpr size_t rows_floats(int DK, int tiles, bool keeps) {
+    const size_t steps = (size_t)TILE * tiles, rows = sizeof(E) == 4 ? steps * (DK + 4) : (steps * (DK + 8) + DK * (steps + 4)) / 2;
+    return 2 * rows + (keeps ? 3 : 2) * tiles * TILE * SIDE + 13 * steps + 4;
+}
+
+// What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.  KEEPS: A beside its inverse.
+template <class E, int DK, int TILES_, bool KEEPS>
 struct Block {
-    static constexpr int TILES = TILES_, STEPS = TILE * TILES, ROW = DK + 4, LANES = DK / 4;
-    float *K, *Q, *As, *Ts, *Ps;
+    static constexpr int TILES = TILES_, STEPS = TILE * TILES, LANES = DK / 4;
+    Rows<E, DK, STEPS> keys, queries;
+    float *As, *Ts, *Ps;
     // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), the squares of key and query, F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
     float *as, *rests, *bs, *rate_rests, *key_lengths, *query_lengths, *kscale, *qscale, *from, *to, *key_reads, *query_reads, *key_takes, *wholes;
     int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
     MRL_DEV explicit Block(float *lds) {
-        K = lds;
-        Q = K + STEPS * ROW;
-        As = Q + STEPS * ROW;
+        keys.at = lds;
+        queries.at = lds + keys.FLOATS;
+        As = queries.at + queries.FLOATS;
         Ts = KEEPS ? As + TILES * TILE * SIDE : As;
         Ps = Ts + TILES * TILE * SIDE;
         as = Ps + TILES * TILE * SIDE;
@@ -275,19 +424,19 @@ struct Block {
     // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
     // Whether a value is too large for products with 0, or none.  Loads read a row that is there in place of one that is not, so that
     // they stand together without a branch among them.
-    template <class E, bool QUERIES>
+    template <bool QUERIES>
     MRL_DEV bool load(const Delta &d, int n, int h, int hk, int thread) {
         bool odd = false;
         const int part = (thread & 63) % LANES, count = d.dk - 4 * part, first = count > 0 ? 4 * part : 0, rows = (int)blockDim.x / LANES;
-        const E *const keys = (const E *)d.key + n * d.key_ld + (long)hk * d.dk + first, *const queries = (const E *)d.query + n * d.query_ld + (long)hk * d.dk + first;
+        const E *const key = (const E *)d.key + n * d.key_ld + (long)hk * d.dk + first, *const query = (const E *)d.query + n * d.query_ld + (long)hk * d.dk + first;
         const long key_step = (long)d.N * d.key_ld, query_step = (long)d.N * d.query_ld;
         const bool whole = (d.dk & 3) == 0, all = full(d) && d.dk == DK;
         const auto take = [&](int slot, f32x4 k, f32x4 q) {
-            *reinterpret_cast<f32x4 *>(K + slot * ROW + 4 * part) = k;
+            keys.put(slot, 4 * part, k);
             const float kk = sum_lanes<LANES>(fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))));
             float qq = 0.0f;
             if (QUERIES) {
-                *reinterpret_cast<f32x4 *>(Q + slot * ROW + 4 * part) = q;
+                queries.put(slot, 4 * part, q);
                 qq = sum_lanes<LANES>(fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3]))));
             }
             odd |= !(kk + qq < LARGE);
@@ -298,7 +447,7 @@ struct Block {
         };
         if (all) {
             const int slot = thread / LANES;
-            const E *k = keys + (long)(t0 + slot) * key_step, *q = queries + (long)(t0 + slot) * query_step;
+            const E *k = key + (long)(t0 + slot) * key_step, *q = query + (long)(t0 + slot) * query_step;
             for (int ahead = 0; ahead < STEPS; ahead += rows) {
                 if (STEPS % rows != 0 && slot + ahead >= STEPS) break;
                 take(slot + ahead, load4(k, 4), QUERIES ? load4(q, 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
@@ -311,11 +460,11 @@ struct Block {
                 const long t = min(time_of(slot), d.T - 1);
                 f32x4 k, q = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (whole) {
-                    k = load4(keys + t * key_step, 4);
-                    if (QUERIES) q = load4(queries + t * query_step, 4);
+                    k = load4(key + t * key_step, 4);
+                    if (QUERIES) q = load4(query + t * query_step, 4);
                 } else {
-                    k = load4(keys + t * key_step, count);
-                    if (QUERIES) q = load4(queries + t * query_step, count);
+                    k = load4(key + t * key_step, count);
+                    if (QUERIES) q = load4(query + t * query_step, count);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -349,18 +498,13 @@ struct Block {
     template <bool QUERIES>
     MRL_DEV void prepare(const Delta &d, int half, int g, int c) {
         const int tile = half >> 1;
-        const float *k_tile = K + (tile * TILE + c) * ROW + 4 * g, *q_tile = Q + (tile * TILE + c) * ROW + 4 * g;
         const float kc = one_over_root(kscale[tile * TILE + c] + EPS);
         const f32x4 decay = between(as + tile * TILE, g, c);
-        f32x4 products = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 products;
         if (half & 1) {
             const int slot = tile * TILE + c;
             const float qs = one_over_root((qscale[slot] + EPS) * (float)d.dk), a = as[slot], b = bs[slot];
-            if (QUERIES) {
-#pragma unroll
-                for (int i = 0; i < DK / TILE; ++i)
-                    products = mfma16(*reinterpret_cast<const f32x4 *>(q_tile + i * TILE), *reinterpret_cast<const f32x4 *>(k_tile + i * TILE), products);
-            }
+            if (QUERIES) products = queries.with(keys, tile, g, c);
             float ahead = a, behind = moved<0x101>(a, 1.0f);   // products up to here, and of those behind
             ahead *= moved<0x111>(ahead, 1.0f);
             behind *= moved<0x101>(behind, 1.0f);
@@ -389,11 +533,7 @@ struct Block {
                 }
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < DK / TILE; ++i) {
-                const f32x4 k = *reinterpret_cast<const f32x4 *>(k_tile + i * TILE);
-                products = mfma16(k, k, products);
-            }
+            products = keys.with(keys, tile, g, c);
             const f32x4 b = four(bs, tile, g), squares = four(kscale, tile, g);
             float *A = As + tile * TILE * SIDE;
 #pragma unroll
@@ -468,28 +608,9 @@ MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
     return !(size < LARGE);
 }
 
-// S^T k of a tile's 16 keys (or queries), unscaled: [row of the tile][column of S]
-template <int DK, int TILES, bool KEEPS>
-MRL_DEV f32x4 ask(const Block<DK, TILES, KEEPS> &block, const float *rows, int tile, int g, int c, const f32x4 (&S)[DK / TILE]) {
-    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < DK / TILE; ++i) x = mfma16(*reinterpret_cast<const f32x4 *>(rows + (tile * TILE + c) * block.ROW + i * TILE + 4 * g), S[i], x);
-    return x;
-}
-// S0 + sum_i k[i] x[i]^T over a tile's keys (or queries), unscaled
-template <int DK, int TILES, bool KEEPS>
-MRL_DEV void add(const Block<DK, TILES, KEEPS> &block, const float *rows, int tile, int g, int c, const f32x4 x, f32x4 (&S)[DK / TILE]) {
-#pragma unroll
-    for (int i = 0; i < DK / TILE; ++i) {
-        f32x4 k;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) k[r] = rows[(tile * TILE + 4 * g + r) * block.ROW + i * TILE + c];
-        S[i] = mfma16(k, x, S[i]);
-    }
-}
 // U[4 g + r][c] of a tile; read: b F S0^T k, what the keys read of the state
-template <int DK, int TILES, bool KEEPS>
-MRL_DEV f32x4 solve(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
+template <class E, int DK, int TILES, bool KEEPS>
+MRL_DEV f32x4 solve(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
     const f32x4 b = block.four(block.bs, tile, g), reads = block.four(block.key_reads, tile, g);
     f32x4 x;
 #pragma unroll
@@ -498,16 +619,18 @@ MRL_DEV f32x4 solve(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c
         x[r] = fmaf(b[r], v[r], -read[r]);
     }
     const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
-    return mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    f32x4 u = mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    settle(u);
+    return u;
 }
 // S0 becomes S1
-template <int DK, int TILES, bool KEEPS>
-MRL_DEV void go_on(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
+template <class E, int DK, int TILES, bool KEEPS>
+MRL_DEV void go_on(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, f32x4 u, f32x4 (&S)[DK / TILE]) {
     u *= block.four(block.key_takes, tile, g);
     const float whole = block.wholes[tile];
 #pragma unroll
     for (int i = 0; i < DK / TILE; ++i) S[i] *= whole;
-    add(block, block.K, tile, g, c, u, S);
+    block.keys.add(tile, g, c, u, S);
 }
 
 // ---------------------------------------------------------------- a long rollout of a few environments, in parts

@@ -97,7 +97,7 @@ template <class E, int DK, int TILES, int WHAT>
 __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Parts parts, int column_groups, float *states, int blocks) {
     extern __shared__ float lds[];
     constexpr int B = DK / TILE, STEPS = TILE * TILES;
-    Block<DK, TILES, false> block(lds);
+    Block<E, DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int number = group_number(), group = number % column_groups, at_part = number / column_groups, part = at_part % parts.count, nh = at_part / parts.count;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
         anew(thread);
         bool odd = is_odd(S);
         odd |= load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
-        odd |= block.template load<E, WHAT == OUTPUTS>(d, n, h, hk, thread);
+        odd |= block.template load<WHAT == OUTPUTS>(d, n, h, hk, thread);
         if (__syncthreads_or(odd) && block.span == TILE) {
             block.span = 1;
             continue;   // the same block again, one step to a tile
@@ -168,12 +168,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
             f32x4 v = V[0], read, o;
 #pragma unroll
             for (int i = 1; i < TILES; ++i) v = tile == i ? V[i] : v;
-            const f32x4 sk = ask(block, block.K, tile, g, c, S);
-            if (WHAT == OUTPUTS) o = ask(block, block.Q, tile, g, c, S);
+            const Pieces<E, DK> pieces(S);
+            const f32x4 sk = block.keys.ask(tile, g, c, pieces);
+            if (WHAT == OUTPUTS) o = block.queries.ask(tile, g, c, pieces);
             const f32x4 u = solve(block, tile, g, c, v, sk, read);
             if (WHAT == OUTPUTS) {
                 o *= block.four(block.query_reads, tile, g);
                 o = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + tile * TILE * SIDE + c * SIDE + 4 * g), u, o);
+                settle(o);
             }
             go_on(block, tile, g, c, u, S);
             if (WHAT == OUTPUTS) store_values(d, block, outs, (long)d.N * d.out_ld, live, tile, g, o);
@@ -250,6 +252,7 @@ __global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, con
             __syncthreads();   // (the buffers alternate)
 #pragma unroll
             for (int k = 0; k < B; ++k) after = mfma16(mine[k], here[k][lane], after);
+            settle(after);
         }
         s = after;
     }
@@ -268,7 +271,7 @@ void launch_steps(const mrl_ctx *ctx, const Delta &d) {
 template <class E, int DK, int TILES, int WHAT>
 void launch_tiles(const mrl_ctx *ctx, const Delta &d, const Parts &p, float *states = nullptr, int blocks = 0) {
     const int tiles = column_tiles(d.dv) + (WHAT == ENDS ? DK / TILE : 0), waves = std::min(MOST_WAVES, tiles), groups = (tiles + waves - 1) / waves;
-    hipLaunchKernelGGL((tiles_kernel<E, DK, TILES, WHAT>), dim3(d.N * d.H * p.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, TILES, false), ctx->stream, d, p,
+    hipLaunchKernelGGL((tiles_kernel<E, DK, TILES, WHAT>), dim3(d.N * d.H * p.count * groups), dim3(64 * waves), sizeof(float) * rows_floats<E>(DK, TILES, false), ctx->stream, d, p,
                        groups, states, blocks);
 }
 template <class E, int DK, int TILES>

@@ -61,9 +61,9 @@ MRL_DEV float sum_ahead(float x) {
 }
 
 // What a tile's columns make of dO and dS1: read = L dS1^T k, dX, and dS1 becomes dS0.
-template <int DK, int TILES, bool KEEPS>
-MRL_DEV void pull(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
-    read = ask(block, block.K, tile, g, c, dS) * block.four(block.key_takes, tile, g);
+template <class E, int DK, int TILES, bool KEEPS>
+MRL_DEV void pull(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
+    read = block.keys.ask(tile, g, c, Pieces<E, DK>(dS)) * block.four(block.key_takes, tile, g);
     f32x4 p_column, t_column;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -71,11 +71,12 @@ MRL_DEV void pull(const Block<DK, TILES, KEEPS> &block, int tile, int g, int c, 
         t_column[r] = block.Ts[(tile * TILE + 4 * g + r) * SIDE + c];
     }
     dX = mfma16(t_column, mfma16(p_column, dO, read), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    settle(dX);
     const float whole = block.wholes[tile];
 #pragma unroll
     for (int i = 0; i < DK / TILE; ++i) dS[i] *= whole;
-    add(block, block.Q, tile, g, c, dO * block.four(block.query_reads, tile, g), dS);
-    add(block, block.K, tile, g, c, -dX * block.four(block.key_reads, tile, g), dS);
+    block.queries.add(tile, g, c, dO * block.four(block.query_reads, tile, g), dS);
+    block.keys.add(tile, g, c, -dX * block.four(block.key_reads, tile, g), dS);
     if (block.cut_ahead(tile)) {
 #pragma unroll
         for (int i = 0; i < DK / TILE; ++i) dS[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
     extern __shared__ float lds[];
     constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES;
     const Delta &d = p.d;
-    Block<DK, TILES, false> block(lds);
+    Block<E, DK, TILES, false> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int at = group_number(), group = at % column_groups, at_part = at / column_groups, part = at_part % p.parts.count, nh = at_part / p.parts.count;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
             anew(thread);
             bool odd = is_odd(dS);
             odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
-            odd |= block.template load<E, true>(d, n, h, hk, thread);
+            odd |= block.template load<true>(d, n, h, hk, thread);
             if (__syncthreads_or(odd) && block.span == TILE) {   // one step to a tile, TILES of them at a time, from the last
                 block.span = 1;
                 rounds = (end - begin + TILES - 1) / TILES;
@@ -160,9 +161,10 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
 constexpr bool both_states(int DK) { return DK < 128; }   // S0 and dS1 in LDS side by side
 inline int waves_of(int DK, int dv) { return std::max(column_tiles(dv), std::min(4, DK / TILE)); }
 constexpr int DOTS = 5;   // q dq, k dk, e, f, U dX
+template <class E>
 size_t back_floats(int DK, int dv) {
     const int columns = TILE * column_tiles(dv) + 4, W = waves_of(DK, dv);
-    return rows_floats(DK, tiles_backward(DK), true) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
+    return rows_floats<E>(DK, tiles_backward(DK), true) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
 }
 
 // EK: the type of the gradients of query and key (float where a group's are summed later)
@@ -172,11 +174,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     constexpr int B = DK / TILE, TILES = tiles_backward(DK), STEPS = TILE * TILES, OWN = B <= 4 ? 1 : 2;   // OWN: row tiles of a wavefront
     constexpr bool BOTH = both_states(DK);
     const Delta &d = p.d;
-    Block<DK, TILES, true> block(lds);
+    Block<E, DK, TILES, true> block(lds);
     const int W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, tiles = (d.dv + TILE - 1) / TILE;
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int stride = TILE * tiles + 4;
-    float *const states = lds + rows_floats(DK, TILES, true), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
+    float *const states = lds + rows_floats<E>(DK, TILES, true), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
     float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE, *const crossing = dPs + TILE * SIDE;
     float *const dots = crossing + TILE, *const wholes = dots + 2 * DOTS * TILE * W;   // [2][DOTS][W][16], [2][W]: two tiles' in turn
     const int at_part = group_number(), part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 for (int i = 0; i < B; ++i) S[i] = zero;
             }
             f32x4 read;
-            const f32x4 u = solve(block, tile, g, c, V[tile], ask(block, block.K, tile, g, c, S), read);
+            const f32x4 u = solve(block, tile, g, c, V[tile], block.keys.ask(tile, g, c, Pieces<E, DK>(S)), read);
             if constexpr (decltype(keep)::value) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) kept[tile][i] = S[i];
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
         anew(thread);
         bool odd = load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
         odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
-        odd |= block.template load<E, true>(d, n, h, hk, thread);
+        odd |= block.template load<true>(d, n, h, hk, thread);
         return odd;
     };
     const auto spread = [&](float *to, const f32x4 (&x)[B]) {   // a wavefront's columns of a state
@@ -275,7 +277,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
             for (int tile = TILES - 1; tile >= 0; --tile) {
                 if (block.t0 + tile * block.span >= d.T) continue;
                 anew(g, c);
-                const float *k_tile = block.K + tile * TILE * block.ROW, *q_tile = block.Q + tile * TILE * block.ROW;
                 const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
                 float *const dot = dots + turn * DOTS * TILE * W;
                 const f32x4 b = block.four(block.bs, tile, g);
@@ -290,6 +291,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         for (int t = 0; t < tiles; ++t)
                             dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g),
                                            *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), dk[o]);
+                        settle(dk[o]);
                         dk[o] *= to;
                     }
                 };
@@ -305,9 +307,10 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 }
                 // ---- by columns
                 if (owns) {
-                    f32x4 out = ask(block, block.Q, tile, g, c, kept[tile]) * block.four(block.query_reads, tile, g);
+                    f32x4 out = block.queries.ask(tile, g, c, Pieces<E, DK>(kept[tile])) * block.four(block.query_reads, tile, g);
                     const f32x4 e = dO[tile] * out;
                     out = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + (tile * TILE + c) * SIDE + 4 * g), U[tile], out);
+                    settle(out);
                     float s_ds = 0.0f;
 #pragma unroll
                     for (int i = 0; i < B; ++i)
@@ -346,6 +349,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), s, dq[o]);
                         reads_by = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), s, reads_by);
                     }
+                    settle(dq[o]);
+                    settle(reads_by);
                     dq[o] *= from;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(-from[r] * b[r], reads_by[r], dk[o][r]);
@@ -357,6 +362,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         dA = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), u, dA);
                         dP = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), u, dP);
                     }
+                    settle(dA);
+                    settle(dP);
                     const f32x4 apart = between(block.as + tile * TILE, g, c);
                     f32x4 both;   // dA A + dP P
 #pragma unroll
@@ -390,17 +397,17 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 for (int o = 0; o < OWN; ++o) {
                     const int i = w + o * W;
                     if (i >= B) continue;
-                    f32x4 k, q, a_column, p_column;
+                    f32x4 k = block.keys.column(tile, i, g, c) * ks, q = block.queries.column(tile, i, g, c) * qs, a_column, p_column;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        k[r] = k_tile[(4 * g + r) * block.ROW + i * TILE + c] * ks[r];
-                        q[r] = q_tile[(4 * g + r) * block.ROW + i * TILE + c] * qs[r];
                         a_column[r] = dAs[(4 * g + r) * SIDE + c];
                         p_column[r] = dPs[(4 * g + r) * SIDE + c];
                     }
                     dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dPs + c * SIDE + 4 * g), k, dq[o]);
                     dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dAs + c * SIDE + 4 * g), k, dk[o]);
                     dk[o] = mfma16(p_column, q, mfma16(a_column, k, dk[o]));
+                    settle(dq[o]);
+                    settle(dk[o]);
                     const int at = i * TILE + c;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -477,12 +484,12 @@ Plan plan_of(const mrl_ctx *ctx, const mrl_delta *r) {
 
 template <class E, class EK, int DK>
 void launch(const mrl_ctx *ctx, const Back &p) {
-    hipLaunchKernelGGL((back_kernel<E, EK, DK>), dim3(p.d.N * p.d.H * p.parts.count), dim3(64 * waves_of(DK, p.d.dv)), sizeof(float) * back_floats(DK, p.d.dv), ctx->stream, p);
+    hipLaunchKernelGGL((back_kernel<E, EK, DK>), dim3(p.d.N * p.d.H * p.parts.count), dim3(64 * waves_of(DK, p.d.dv)), sizeof(float) * back_floats<E>(DK, p.d.dv), ctx->stream, p);
 }
 template <class E, int DK>
 void launch_chain(const mrl_ctx *ctx, const Back &p) {
     const int tiles = column_tiles(p.d.dv), waves = std::min(4, tiles), groups = (tiles + waves - 1) / waves;
-    hipLaunchKernelGGL((chain_kernel<E, DK>), dim3(p.d.N * p.d.H * p.parts.count * groups), dim3(64 * waves), sizeof(float) * rows_floats(DK, tiles_backward(DK), false), ctx->stream, p, groups);
+    hipLaunchKernelGGL((chain_kernel<E, DK>), dim3(p.d.N * p.d.H * p.parts.count * groups), dim3(64 * waves), sizeof(float) * rows_floats<E>(DK, tiles_backward(DK), false), ctx->stream, p, groups);
 }
 template <class E>
 void launch_chain(const mrl_ctx *ctx, const Back &p) {
