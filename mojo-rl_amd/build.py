@@ -106,6 +106,90 @@ def check_lane_masks(jobs=8):
         return dict(pool.map(one, SOURCES))
 
 
+# ---- results of the matrix cores read too early
+# A product's registers may be read some instructions behind it; the hardware does not wait for them, the compiler counts.  Behind
+# a taken branch this compiler has been seen to count too few, down to one, and the reader took what had stood there before.
+_STATES = (("16x16x32", 8), ("16x16x16", 8), ("16x16x4_f32", 10), ("32x32", 18))   # what it leaves within a block
+_REGISTERS = re.compile(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b")
+_WRITES_MEMORY = re.compile(r"^(ds_write|(global|buffer|flat|scratch)_(store|atomic))")
+
+
+def _registers(text):
+    found = set()
+    for first, last, alone in _REGISTERS.findall(text):
+        found |= {int(alone)} if alone else set(range(int(first), int(last) + 1))
+    return found
+
+
+def early_reads(lines):
+    """(products, faults) of a unit's assembly, the lines of it."""
+    kernels, code, products, faults = {}, None, 0, []
+    for line in lines:
+        label = re.match(r"^(\.LBB\d+_\d+|_Z\w+):", line)
+        if label and label[1].startswith("_Z"):
+            code = kernels.setdefault(label[1], [])
+        elif label and code is not None:
+            code.append((label[1], None))
+        elif code is not None:
+            op, _, rest = line.split(";")[0].strip().partition(" ")
+            if op and not op.startswith("."):
+                code.append((op, rest.strip()))
+    for kernel, code in kernels.items():
+        at = {op: i for i, (op, rest) in enumerate(code) if rest is None}
+        for i, (op, rest) in enumerate(code):
+            if rest is None or not op.startswith("v_mfma"):
+                continue
+            products += 1
+            states = next((n for shape, n in _STATES if shape in op), 18)
+            todo, seen = [(i + 1, 0, frozenset(_registers(rest.split(",")[0])))], set()
+            while todo:
+                j, waited, live = todo.pop()
+                while j < len(code) and waited < states and live and (j, waited, live) not in seen:
+                    seen.add((j, waited, live))
+                    name, args = code[j]
+                    j += 1
+                    if args is None:
+                        continue
+                    waited += 1
+                    if name == "s_nop":
+                        waited += int(args)
+                    elif name in ("s_endpgm", "s_setpc_b64"):
+                        break
+                    elif name == "s_branch":
+                        j = at[args]
+                    elif name.startswith("s_cbranch"):
+                        todo.append((at[args], waited, live))
+                    elif not name.startswith("s_"):
+                        words = args.split(",")
+                        written = set() if _WRITES_MEMORY.match(name) else _registers(words[0])
+                        read = _registers(",".join(words[1:])) if written else _registers(args)
+                        if name.startswith("v_mfma"):           # (the addend of a like product may follow at once)
+                            read = _registers(",".join(words[1:3]))
+                        elif written & live:                     # overwritten early: no better
+                            read |= written
+                        if read & live:
+                            faults.append((kernel, op + " " + rest, name + " " + args, waited - 1))
+                        live -= written | read
+    return products, faults
+
+
+def check_matrix_results(jobs=8):
+    """Compiles every unit that uses the matrix cores to assembly; {unit: (products, faults)}."""
+    def one(unit):
+        cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(unit, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, unit), "-o", "-"]
+        proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError("hipcc failed: " + " ".join(cmd))
+        return unit, early_reads(proc.stdout.splitlines())
+    units = []
+    for unit in SOURCES:
+        with open(os.path.join(CSRC, unit)) as f:
+            if "mfma" in f.read():
+                units.append(unit)
+    with ThreadPoolExecutor(max_workers=jobs) as pool:
+        return dict(pool.map(one, units))
+
+
 if __name__ == "__main__":
     print(build(verbose=True, incremental="--incremental" in sys.argv))
     sys.exit(0)
