@@ -208,3 +208,199 @@ def test_what_a_cut_hides(mrl, ctx, T, N, heads, dk, dv, dtype):
     first = got_grads[5].cpu().double()
     assert (first[0] == 0).all()
     same(first[1:], grads[5].cpu().double()[1:], 2 * BACKWARD)
+
+
+# ---- calls other than one pass over a rollout with outputs of its own
+def step_rows(c, first, last):
+    return [x[first * c.N:last * c.N] for x in c.rows]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,N,heads,key_heads,dk,dv,lengths", [(21, 5, 2, 1, 24, 40, [1] * 21), (200, 3, 1, 1, 128, 128, [1, 2, 3, 4, 5, 70, 16, 99]), (900, 2, 2, 2, 64, 32, [300, 1, 599])])
+def test_in_pieces_with_the_state_in_place(mrl, ctx, T, N, heads, key_heads, dk, dv, lengths, dtype):
+    """A rollout in pieces, single steps among them, the state updated where it is: what 64 bits give for the whole of it."""
+    c = Case(T, N, heads, key_heads, dk, dv, dtype, packed=True, seed=4)
+    state, prev, at = c.state.clone(), c.prev, 0
+    wide = torch.full((T * N, 2 + heads * dv), 7.0, dtype=c.tt, device="cuda")
+    out = wide[:, 1:-1]
+    for n in lengths:
+        rows, o = step_rows(c, at, at + n), out[at * N:(at + n) * N]
+        if n == 1:
+            c.layer(mrl).step_gpu(ctx, o, *rows, state, prev_dones=prev)
+        else:
+            c.layer(mrl).forward_gpu(ctx, o, *rows, n, state_in=state, state_out=state, dones=c.dones[at:at + n], prev_dones=prev)
+        at += n
+        prev = c.dones[at - 1]
+    assert at == T
+    ctx.synchronize()
+    want, want_last = c.forward64()
+    near(out.contiguous(), want, heads, FORWARD, HALF[dtype], "out")
+    near(state, want_last, heads, FORWARD, UNIT, "state")
+    assert (wide[:, 0] == 7).all() and (wide[:, -1] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,N,heads,dk,dv", [(1, 70, 2, 16, 20), (50, 3, 2, 64, 24), (700, 2, 1, 40, 64), (600, 1, 1, 128, 128)])
+def test_states_and_their_gradients_in_place(mrl, ctx, T, N, heads, dk, dv, dtype):
+    c = Case(T, N, heads, heads, dk, dv, dtype, seed=6)
+    out, last = c.forward(mrl, ctx)
+    grads = c.backward(mrl, ctx)
+    state, grad_state = c.state.clone(), c.grad_last.clone()
+    again, mine = torch.empty_like(out), [torch.empty_like(g) for g in grads[:5]]
+    c.layer(mrl).backward_gpu(ctx, *mine, c.grad_out, *c.rows, T, state_in=state, dones=c.dones, prev_dones=c.prev, grad_state_out=grad_state, grad_state_in=grad_state)
+    c.layer(mrl).forward_gpu(ctx, again, *c.rows, T, state_in=state, state_out=state, dones=c.dones, prev_dones=c.prev)
+    ctx.synchronize()
+    assert torch.equal(again, out) and torch.equal(state, last) and torch.equal(grad_state, grads[5]) and all(torch.equal(a, b) for a, b in zip(mine, grads))
+
+
+@pytest.mark.parametrize("T,N,dk", [(40, 2, 16), (500, 1, 24)])
+def test_gradient_against_differences(mrl, ctx, T, N, dk):
+    """Directional derivatives of the rule in 64 bits, taken as differences."""
+    c = Case(T, N, 2, 1, dk, 12, "f32", seed=8)
+    grads = c.backward(mrl, ctx)
+    ctx.synchronize()
+    inputs = [*c.rows64(), c.state64()]
+    weights, last = c.grad_out.cpu().double(), c.grad_last.cpu().double()
+
+    def loss(at):
+        out, end, _, _ = rule64(at[:5], at[5], c.cut, *c.dims)
+        return ((out.reshape(T * N, -1) * weights).sum() + (end * last).sum()).item()
+    gen = torch.Generator().manual_seed(5)
+    size = weights.abs().sum().item() + last.abs().sum().item()
+    for which, grad in enumerate(grads):
+        grad = grad.cpu().double()
+        v = torch.randn(inputs[which].shape, generator=gen, dtype=torch.float64)
+        eps = 1e-5
+        up, down = list(inputs), list(inputs)
+        up[which], down[which] = inputs[which] + eps * v, inputs[which] - eps * v
+        want = (loss(up) - loss(down)) / (2 * eps)
+        # differences: eps^2 of third derivatives and 2^-52 / eps of the loss's terms; the gradient's own bound for every value
+        assert abs((grad * v).sum().item() - want) <= BACKWARD * grad.abs().max().item() * v.abs().sum().item() + 1e-8 * size, c.NAMES[which:which + 1]
+
+
+def test_gates_and_rates_at_their_ends(mrl, ctx):
+    """Gates and rates that are 0 or 1 to the last bit, infinite ones among them, and rows of zeros for keys and queries."""
+    for dtype in ("f32", "bf16"):
+        c = Case(80, 2, 2, 2, 16, 24, dtype, dones=False, seed=9)
+        q, k, v, gate, rate = c.rows
+        gate[3], gate[20], gate[41], gate[60] = -float("inf"), float("inf"), -200.0, 200.0
+        rate[5], rate[21], rate[43], rate[61] = -float("inf"), float("inf"), -200.0, 200.0
+        k[30], q[31], k[77], q[77] = 0, 0, 0, 0
+        out, last = c.forward(mrl, ctx)
+        grads = c.backward(mrl, ctx)
+        ctx.synchronize()
+        want, want_last = c.forward64()
+        near(out, want, 2, FORWARD, HALF[dtype], "out")
+        near(last, want_last, 2, FORWARD, UNIT, "state_out")
+        wants, terms = c.backward64()
+        for name, x, y in zip((*c.NAMES, "state"), grads, wants):
+            near(x, y, 2, BACKWARD, UNIT if name == "state" else HALF[dtype], "grad_" + name, terms.get(name))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_other_streams_and_captured_graphs(mrl, ctx, dtype):
+    """Two graphs of one context's calls, each with a workspace of its own, replayed on different streams with eager calls between."""
+    cases = [Case(700, 2, 2, 1, 40, 24, dtype, seed=1), Case(65, 20, 1, 1, 128, 64, dtype, seed=2)]
+    wants = [(*c.forward(mrl, ctx), *c.backward(mrl, ctx)) for c in cases]
+    ctx.synchronize()
+    side = torch.cuda.Stream()
+    cctx = mrl.DeviceContext("cuda:0", stream=side)
+    graphs, outs = [], []
+    for c in cases:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append((*c.forward(mrl, cctx), *c.backward(mrl, cctx)))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for o in outs:
+            for t in o:
+                t.fill_(9)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = cases[0].forward(mrl, ctx)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(eager, wants[0]))
+        for o, w in zip(outs, wants):
+            assert all(torch.equal(x, y) for x, y in zip(o, w))
+    del graphs
+    cctx.close()
+
+
+def test_no_steps_and_no_environments(mrl, ctx):
+    lib = mrl._lib.lib()
+    a, b = torch.randn(48, device="cuda"), torch.zeros(48, device="cuda")
+    d = mrl._lib.Delta(0, 0, 3, 1, 1, 4, 4, *(None,) * 5, *(0,) * 5, None, None, a.data_ptr())
+    p, none = ctypes.c_void_p(b.data_ptr()), mrl._lib.DeltaGrads()
+    assert lib.mrl_delta_forward(ctx.handle, ctypes.byref(d), None, 0, p, None, 0) == 0
+    ctx.synchronize()
+    assert torch.equal(a, b)
+    none.state = b.data_ptr()
+    assert lib.mrl_delta_backward(ctx.handle, ctypes.byref(d), None, 0, None, ctypes.byref(none), None, 0) == 0
+    ctx.synchronize()
+    assert not b.any()
+    layer = mrl.GatedDeltaRule(2, 4, 3)
+    empty = [torch.empty(0, w, device="cuda") for w in (6, 8, 8, 6, 2, 2)]
+    layer.forward_gpu(ctx, *empty, 5)
+    layer.backward_gpu(ctx, *empty[1:], *empty, 5)
+    ctx.synchronize()
+
+
+def test_library_refusals(mrl, ctx):
+    lib, x, size = mrl._lib.lib(), torch.zeros(1 << 18, device="cuda"), ctypes.c_uint64(0)
+    at = x.data_ptr()
+    far = at + 4 * (1 << 17)
+
+    def description(**other):
+        d = mrl._lib.Delta(0, 10, 3, 2, 1, 4, 4, at, at, at, at, at, 4, 4, 8, 2, 2, None, None, None)
+        for name, value in other.items():
+            setattr(d, name, value)
+        return d
+    for bad, text in ((dict(dtype=2), b"element type"), (dict(T=-1), b"negative"), (dict(T=1 << 30), b"2^30"), (dict(N=1 << 21), b"2^22"), (dict(heads=3, key_heads=2), b"heads"),
+                      (dict(key_dim=129), b"dim"), (dict(value_dim=0), b"dim"), (dict(key=None), b"NULL"), (dict(query_ld=3), b"stride"), (dict(rate_ld=1), b"stride")):
+        d = description(**bad)
+        assert lib.mrl_delta_forward(ctx.handle, ctypes.byref(d), far, 8, None, None, 0) == -1 and text in lib.mrl_last_error(), (bad, lib.mrl_last_error())
+    assert lib.mrl_delta_forward(ctx.handle, ctypes.byref(description()), None, 8, None, None, 0) == -1 and b"NULL" in lib.mrl_last_error()
+    assert lib.mrl_delta_forward(ctx.handle, ctypes.byref(description()), far, 7, None, None, 0) == -1 and b"stride" in lib.mrl_last_error()
+    grads = mrl._lib.DeltaGrads(far, far + 4096, far + 8192, far + 12288, far + 16384, 4, 4, 8, 2, 2, None)
+    d = description(T=2000, N=1)
+    for backward in (0, 1):
+        assert lib.mrl_delta_workspace(ctx.handle, ctypes.byref(d), backward, ctypes.byref(size)) == 0 and 0 < size.value
+        for ws, n, text in ((None, 0, b"workspace"), (far + 32768 * 4, size.value - 1, b"workspace"), (far + 32768 * 4 + 4, size.value, b"aligned")):
+            if backward:
+                rc = lib.mrl_delta_backward(ctx.handle, ctypes.byref(d), at, 8, None, ctypes.byref(grads), ws, n)
+            else:
+                rc = lib.mrl_delta_forward(ctx.handle, ctypes.byref(d), far, 8, None, ws, n)
+            assert rc == -1 and text in lib.mrl_last_error(), lib.mrl_last_error()
+    ctx.synchronize()
+    assert not x.any()
+
+
+def test_outputs_on_inputs_are_refused(mrl, ctx):
+    """Before anything is launched: the buffers stay as they are."""
+    c = Case(40, 3, 2, 2, 8, 8, "f32", packed=True)
+    wide = c.rows[0]._base if c.rows[0]._base is not None else c.rows[0]
+    before = wide.clone()
+    out = torch.zeros(120, 16, device="cuda")
+    grads = [torch.zeros(120, w, device="cuda") for w in c.widths]
+    flat = torch.zeros(4, 3 * 2 * 64, device="cuda")
+
+    def forward(**other):
+        c.layer(mrl).forward_gpu(ctx, **{**dict(zip(c.NAMES, c.rows)), **dict(output=out, steps=40, state_in=flat[0], state_out=flat[1], dones=c.dones, prev_dones=c.prev), **other})
+
+    def backward(**other):
+        c.layer(mrl).backward_gpu(ctx, **{**dict(zip(c.NAMES, c.rows)), **dict(zip(("grad_" + n for n in c.NAMES), grads)),
+                                          **dict(grad_output=out, steps=40, state_in=flat[0], dones=c.dones, prev_dones=c.prev, grad_state_out=flat[2], grad_state_in=flat[3]), **other})
+    for bad in (dict(output=c.rows[2]), dict(output=wide[:, 8:24]), dict(output=wide[:, 36:52]), dict(state_out=flat.view(-1)[5:5 + 384]), dict(dones=out.view(-1)[:120]),
+                dict(state_out=out.view(-1)[:384]), dict(prev_dones=flat[1][:3])):
+        with pytest.raises(mrl.MrlError, match="overlap"):
+            forward(**bad)
+    for bad in (dict(grad_query=c.rows[0]), dict(grad_query=grads[1]), dict(grad_value=out), dict(grad_gate=grads[4]), dict(grad_state_in=flat[0]),
+                dict(grad_state_out=flat.view(-1)[3 * 384 - 1:4 * 384 - 1]), dict(grad_rate=wide[:, 40:42])):
+        with pytest.raises(mrl.MrlError, match="overlap"):
+            backward(**bad)
+    ctx.synchronize()
+    assert torch.equal(wide, before) and not out.any() and not flat.any() and not any(g.any() for g in grads)

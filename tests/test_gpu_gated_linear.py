@@ -176,3 +176,53 @@ def test_empty_and_refused(mrl, ctx):
                        ((0, 0, 100, 8, 4, None, 8, ptr(params), ptr(out), 4, None, 0), "NULL")):
         with pytest.raises(mrl.MrlError, match=text):
             call("mrl_gated_linear_forward", ctx.handle, *args)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_other_streams_and_captured_graphs(mrl, ctx, dtype):
+    """Two graphs of one context's calls, each with a workspace of its own, replayed on different streams with eager calls between."""
+    cases = [Case(1500, 72, 40, "gelu", dtype, seed=1), Case(20, 33, 65, "silu", dtype, seed=2)]
+    wants = [(c.forward(mrl, ctx), *c.backward(mrl, ctx)) for c in cases]
+    ctx.synchronize()
+    side = torch.cuda.Stream()
+    cctx = mrl.DeviceContext("cuda:0", stream=side)
+    graphs, outs = [], []
+    for c in cases:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append((c.forward(mrl, cctx), *c.backward(mrl, cctx)))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for o in outs:
+            for t in o:
+                t.fill_(9)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = cases[0].forward(mrl, ctx)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, wants[0][0])
+        for o, w in zip(outs, wants):
+            assert all(torch.equal(x, y) for x, y in zip(o, w))
+    del graphs
+    cctx.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M", [40, 300])
+def test_rows_that_are_not_finite(mrl, ctx, M, dtype):
+    """An infinity or NaN in a row of the input reaches that row of the outputs and of grad_input, and no other."""
+    c = Case(M, 70, 50, "silu", dtype, seed=4)
+    out, (gx, _) = c.forward(mrl, ctx), c.backward(mrl, ctx)
+    c.x[17, 3], c.x[M - 1, 69], c.grad[21, 5] = float("nan"), float("inf"), float("inf")
+    bad, (bad_x, bad_grads) = c.forward(mrl, ctx), c.backward(mrl, ctx)
+    ctx.synchronize()
+    rows = torch.ones(M, dtype=torch.bool)
+    rows[[17, M - 1]] = False
+    assert torch.equal(bad[rows], out[rows]) and torch.isnan(bad[17]).all() and not torch.isfinite(bad[M - 1]).all()
+    rows[21] = False
+    assert torch.equal(bad_x[rows], gx[rows]) and not torch.isfinite(bad_x[21]).any() and torch.isnan(bad_x[17]).all()
+    assert torch.isnan(bad_grads.view(-1)[:70 * 100].view(70, 100)[3]).all()
