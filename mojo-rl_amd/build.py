@@ -173,14 +173,32 @@ def early_reads(lines):
     return products, faults
 
 
+def empty_masks(lines):
+    """Kernels with a narrowed lane mask around nothing: what stood there, a copy of a register that the other way around has
+    overwritten, has been seen to be lost."""
+    kernel, last, found = None, "", []
+    for line in lines:
+        label = re.match(r"^(_Z\w+):", line)
+        kernel = label[1] if label else kernel
+        ins = line.split(";")[0].strip()
+        if not ins or ins.startswith("."):
+            continue
+        saved = re.match(r"s_and_saveexec_b64 (s\[\d+:\d+\])", last)
+        if saved and ins == "s_or_b64 exec, exec, " + saved[1]:
+            found.append(kernel)
+        last = ins
+    return found
+
+
 def check_matrix_results(jobs=8):
-    """Compiles every unit that uses the matrix cores to assembly; {unit: (products, faults)}."""
+    """Compiles every unit that uses the matrix cores to assembly; {unit: (products, faults, kernels with empty masks)}."""
     def one(unit):
         cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(unit, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, unit), "-o", "-"]
         proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, text=True)
         if proc.returncode != 0:
             raise RuntimeError("hipcc failed: " + " ".join(cmd))
-        return unit, early_reads(proc.stdout.splitlines())
+        lines = proc.stdout.splitlines()
+        return unit, (*early_reads(lines), empty_masks(lines))
     units = []
     for unit in SOURCES:
         with open(os.path.join(CSRC, unit)) as f:

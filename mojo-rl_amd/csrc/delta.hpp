@@ -53,6 +53,17 @@ MRL_DEV float value_of(bf16_t x) { return __uint_as_float((unsigned)x.bits << 16
 MRL_DEV void give(float *p, float x) { *p = x; }
 MRL_DEV void give(bf16_t *p, float x) { p->bits = __builtin_bit_cast(unsigned short, (__bf16)x); }
 
+// four neighbouring values as they lie
+template <class E> struct Four;
+template <> struct Four<float> { typedef f32x4u type; };
+template <> struct Four<bf16_t> { typedef u16x4u type; };
+MRL_DEV f32x4 values_of(const f32x4u x) { return x; }
+MRL_DEV f32x4 values_of(const u16x4u v) {
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float((unsigned)v[i] << 16);
+    return x;
+}
 // up to four neighbouring values, zeros from `n` on
 MRL_DEV f32x4 load4(const float *p, int n) {
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -67,9 +78,7 @@ MRL_DEV f32x4 load4(const float *p, int n) {
 MRL_DEV f32x4 load4(const bf16_t *p, int n) {
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     if (n >= 4) {
-        const u16x4u v = *reinterpret_cast<const u16x4u *>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float((unsigned)v[i] << 16);
+        x = values_of(*reinterpret_cast<const u16x4u *>(p));
     } else {
         if (n > 0) x[0] = value_of(p[0]);
         if (n > 1) x[1] = value_of(p[1]);
@@ -417,21 +426,39 @@ struct Block {
         wholes = key_takes + STEPS;
     }
     MRL_DEV int time_of(int slot) const { return t0 + (slot >> 4) * span + (slot & 15); }
-    MRL_DEV bool there(const Delta &d, int slot) const { return (slot & 15) < span && time_of(slot) < d.T; }
+    MRL_DEV bool there(const Delta &d, int slot) const { return ((slot & 15) < span) & (time_of(slot) < d.T); }
     MRL_DEV bool full(const Delta &d) const { return span == TILE && t0 + STEPS <= d.T; }
     MRL_DEV f32x4 four(const float *scalars, int tile, int g) const { return *reinterpret_cast<const f32x4 *>(scalars + tile * TILE + 4 * g); }
 
     // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
-    // Whether a value is too large for products with 0, or none.  Loads read a row that is there in place of one that is not, so that
-    // they stand together without a branch among them.
+    // Whether a value is too large for products with 0, or none.  All loads are asked for ahead of the first use of any: one wait for them, not
+    // five.  They read a row that is there in place of one that is not, so that they stand together without a branch among them.
     template <bool QUERIES>
     MRL_DEV bool load(const Delta &d, int n, int h, int hk, int thread) {
+        constexpr int ASKED = STEPS * LANES > 256 ? STEPS * LANES / 256 : 1;   // rows of a thread at a time: all of them where there are four wavefronts
         bool odd = false;
         const int part = (thread & 63) % LANES, count = d.dk - 4 * part, first = count > 0 ? 4 * part : 0, rows = (int)blockDim.x / LANES;
         const E *const key = (const E *)d.key + n * d.key_ld + (long)hk * d.dk + first, *const query = (const E *)d.query + n * d.query_ld + (long)hk * d.dk + first;
         const long key_step = (long)d.N * d.key_ld, query_step = (long)d.N * d.query_ld;
         const bool whole = (d.dk & 3) == 0, all = full(d) && d.dk == DK;
+        E gate = {}, rate = {};   // (a workgroup has as many threads as a block has steps, or more)
+        bool cut = false;
+        if (thread < STEPS) {
+            const int t = min(time_of(thread), d.T - 1);
+            const long row = (long)t * d.N + n;
+            gate = ((const E *)d.gate)[row * d.gate_ld + h];
+            rate = ((const E *)d.rate)[row * d.rate_ld + h];
+            cut = is_cut(d, t, n);
+        }
         const auto take = [&](int slot, f32x4 k, f32x4 q) {
+            if (!all) {
+                const bool here = there(d, slot) & (count > 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    k[j] = here ? k[j] : 0.0f;
+                    q[j] = here ? q[j] : 0.0f;
+                }
+            }
             keys.put(slot, 4 * part, k);
             const float kk = sum_lanes<LANES>(fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))));
             float qq = 0.0f;
@@ -445,49 +472,38 @@ struct Block {
                 qscale[slot] = qq;
             }
         };
-        if (all) {
-            const int slot = thread / LANES;
-            const E *k = key + (long)(t0 + slot) * key_step, *q = query + (long)(t0 + slot) * query_step;
-            for (int ahead = 0; ahead < STEPS; ahead += rows) {
-                if (STEPS % rows != 0 && slot + ahead >= STEPS) break;
-                take(slot + ahead, load4(k, 4), QUERIES ? load4(q, 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                k += rows * key_step;
-                q += rows * query_step;
+        const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (whole) {
+            for (int ahead = thread / LANES; ahead < STEPS; ahead += ASKED * rows) {
+                typename Four<E>::type k[ASKED], q[ASKED];
+#pragma unroll
+                for (int i = 0; i < ASKED; ++i) {
+                    const long t = min(time_of(ahead + i * rows), d.T - 1);
+                    k[i] = *reinterpret_cast<const typename Four<E>::type *>(key + t * key_step);
+                    if (QUERIES) q[i] = *reinterpret_cast<const typename Four<E>::type *>(query + t * query_step);
+                }
+#pragma unroll
+                for (int i = 0; i < ASKED; ++i)
+                    if (ahead + i * rows < STEPS) take(ahead + i * rows, values_of(k[i]), QUERIES ? values_of(q[i]) : none);
             }
         } else {
             for (int slot = thread / LANES; slot < STEPS; slot += rows) {
-                const bool here = there(d, slot) && count > 0;
                 const long t = min(time_of(slot), d.T - 1);
-                f32x4 k, q = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (whole) {
-                    k = load4(key + t * key_step, 4);
-                    if (QUERIES) q = load4(query + t * query_step, 4);
-                } else {
-                    k = load4(key + t * key_step, count);
-                    if (QUERIES) q = load4(query + t * query_step, count);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    k[i] = here ? k[i] : 0.0f;
-                    q[i] = here ? q[i] : 0.0f;
-                }
-                take(slot, k, q);
+                take(slot, load4(key + t * key_step, count), QUERIES ? load4(query + t * query_step, count) : none);
             }
         }
-        for (int slot = thread; slot < STEPS; slot += blockDim.x) {
+        if (thread < STEPS) {
             float a = 1.0f, rest = 0.0f, b = 0.0f, other = 0.0f;
-            if (there(d, slot)) {
-                const int t = time_of(slot);
-                const long row = (long)t * d.N + n;
-                sigmoid_pair(value_of(((const E *)d.gate)[row * d.gate_ld + h]), a, rest);
-                sigmoid_pair(value_of(((const E *)d.rate)[row * d.rate_ld + h]), b, other);
+            if (there(d, thread)) {
+                sigmoid_pair(value_of(gate), a, rest);
+                sigmoid_pair(value_of(rate), b, other);
                 odd |= !(a + b < LARGE);
-                if (is_cut(d, t, n)) a = rest = 0.0f;
+                if (cut) a = rest = 0.0f;
             }
-            as[slot] = a;
-            rests[slot] = rest;
-            bs[slot] = b;
-            rate_rests[slot] = other;
+            as[thread] = a;
+            rests[thread] = rest;
+            bs[thread] = b;
+            rate_rests[thread] = other;
         }
         return odd;
     }
@@ -552,33 +568,33 @@ struct Block {
 };
 
 // A value tile as a result's registers: row 4 g + r, column c.  `rows` points at the column (at one that is there) of the environment's row of
-// step 0, `step` elements from a step to the next.
+// step 0, `step` elements from a step to the next.  First the loads, later what is made of them.
 template <class E, class B, int TILES>
-MRL_DEV bool load_values(const Delta &d, const B &block, const E *rows, long step, bool live, int g, f32x4 (&V)[TILES]) {
-    float size = 0.0f;
+MRL_DEV void ask_values(const Delta &d, const B &block, const E *rows, long step, int g, E (&V)[TILES][4]) {
     if (block.full(d)) {
         const E *const first = rows + 4 * g * step;
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) V[tile][r] = value_of(first[(long)(block.t0 + tile * TILE + r) * step]);
-#pragma unroll
-        for (int tile = 0; tile < TILES; ++tile)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) V[tile][r] = live ? V[tile][r] : 0.0f;
+            for (int r = 0; r < 4; ++r) V[tile][r] = first[(long)(block.t0 + tile * TILE + r) * step];
     } else {
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float x = value_of(rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step]);
-                V[tile][r] = live && block.there(d, tile * TILE + 4 * g + r) ? x : 0.0f;
-            }
+            for (int r = 0; r < 4; ++r) V[tile][r] = rows[min(block.time_of(tile * TILE + 4 * g + r), d.T - 1) * step];
     }
+}
+template <class E, class B, int TILES>
+MRL_DEV bool take_values(const Delta &d, const B &block, const E (&asked)[TILES][4], bool live, int g, f32x4 (&V)[TILES]) {
+    float size = 0.0f;
+    const bool full = block.full(d);
 #pragma unroll
     for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) size += fabsf(V[tile][r]);
+        for (int r = 0; r < 4; ++r) {
+            V[tile][r] = live & (full | block.there(d, tile * TILE + 4 * g + r)) ? value_of(asked[tile][r]) : 0.0f;   // (no branches: the registers may be others' in one of them)
+            size += fabsf(V[tile][r]);
+        }
     return !(size < LARGE);
 }
 // and back: one tile

@@ -147,9 +147,10 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
         f32x4 V[TILES];
         anew(g, c);
         anew(thread);
-        bool odd = is_odd(S);
-        odd |= load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
-        odd |= block.template load<WHAT == OUTPUTS>(d, n, h, hk, thread);
+        E asked[TILES][4];
+        ask_values(d, block, values, (long)d.N * d.value_ld, g, asked);
+        bool odd = block.template load<WHAT == OUTPUTS>(d, n, h, hk, thread);
+        odd |= take_values(d, block, asked, live, g, V) | is_odd(S);
         if (__syncthreads_or(odd) && block.span == TILE) {
             block.span = 1;
             continue;   // the same block again, one step to a tile

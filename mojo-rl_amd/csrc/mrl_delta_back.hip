@@ -128,9 +128,10 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
         for (int round = 0; round < rounds;) {
             anew(g, c);
             anew(thread);
-            bool odd = is_odd(dS);
-            odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
-            odd |= block.template load<true>(d, n, h, hk, thread);
+            E asked[TILES][4];
+            ask_values(d, block, grads, (long)d.N * p.grad_out_ld, g, asked);
+            bool odd = block.template load<true>(d, n, h, hk, thread);
+            odd |= take_values(d, block, asked, live, g, dO) | is_odd(dS);
             if (__syncthreads_or(odd) && block.span == TILE) {   // one step to a tile, TILES of them at a time, from the last
                 block.span = 1;
                 rounds = (end - begin + TILES - 1) / TILES;
@@ -231,10 +232,12 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     const auto load = [&]() {
         anew(g, c);
         anew(thread);
-        bool odd = load_values(d, block, values, (long)d.N * d.value_ld, live, g, V);
-        odd |= load_values(d, block, grads, (long)d.N * p.grad_out_ld, live, g, dO);
-        odd |= block.template load<true>(d, n, h, hk, thread);
-        return odd;
+        E asked_values[TILES][4], asked_grads[TILES][4];
+        ask_values(d, block, values, (long)d.N * d.value_ld, g, asked_values);
+        ask_values(d, block, grads, (long)d.N * p.grad_out_ld, g, asked_grads);
+        bool odd = block.template load<true>(d, n, h, hk, thread);
+        odd |= take_values(d, block, asked_values, live, g, V);
+        return odd | take_values(d, block, asked_grads, live, g, dO);
     };
     const auto spread = [&](float *to, const f32x4 (&x)[B]) {   // a wavefront's columns of a state
 #pragma unroll
@@ -248,8 +251,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
         first_state(number);
         block.t0 = begin;
         block.span = TILE;
-        bool odd = is_odd(S) | is_odd(dS);
-        odd |= load();
+        bool odd = load();
+        odd |= is_odd(S) | is_odd(dS);
         int rounds = 1;
         if (__syncthreads_or(odd)) {   // one step to a tile, TILES of them at a time
             block.span = 1;

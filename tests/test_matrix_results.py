@@ -1,4 +1,4 @@
-"""No kernel reads the result of a matrix product before it is there (see build.early_reads)."""
+"""No kernel reads the result of a matrix product before it is there (see build.early_reads), or has lost what a narrowed lane mask was for."""
 import importlib
 
 import pytest
@@ -38,8 +38,14 @@ def test_a_product_of_a_result_and_a_store_are_reads():
         assert len(build.early_reads(EARLY.replace("v_mul_f32_e32 v6, v1, v5", reader).splitlines())[1]) == 1
 
 
+def test_an_empty_mask_is_found():
+    kept = "_Zkernel:\n\ts_and_saveexec_b64 s[10:11], s[6:7]\n\tv_mov_b32_e32 v17, v0\n\ts_or_b64 exec, exec, s[10:11]\n"
+    assert build.empty_masks(kept.splitlines()) == []
+    assert build.empty_masks(kept.replace("\tv_mov_b32_e32 v17, v0\n", "").splitlines()) == ["_Zkernel"]
+
+
 def test_no_unit_reads_a_result_early():
     found = build.check_matrix_results()
     assert {"mrl_delta.hip", "mrl_delta_back.hip", "mrl_glu.hip", "mrl_muon.hip"} <= set(found)
-    for unit, (products, faults) in found.items():
-        assert products > 0 and faults == [], (unit, faults[:4])
+    for unit, (products, faults, empty) in found.items():
+        assert products > 0 and faults == [] and empty == [], (unit, faults[:4], empty[:4])
