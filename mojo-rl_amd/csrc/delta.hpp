@@ -624,16 +624,13 @@ MRL_DEV bool is_odd(const f32x4 (&S)[B]) {
     return !(size < LARGE);
 }
 
-// U[4 g + r][c] of a tile; read: b F S0^T k, what the keys read of the state
+// U[4 g + r][c] of a tile; sk: S0^T k
 template <class E, int DK, int TILES, bool KEEPS>
-MRL_DEV f32x4 solve(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk, f32x4 &read) {
+MRL_DEV f32x4 solve(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 v, const f32x4 sk) {
     const f32x4 b = block.four(block.bs, tile, g), reads = block.four(block.key_reads, tile, g);
     f32x4 x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        read[r] = reads[r] * sk[r];
-        x[r] = fmaf(b[r], v[r], -read[r]);
-    }
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(b[r], v[r], -reads[r] * sk[r]);
     const f32x4 inverse = *reinterpret_cast<const f32x4 *>(block.Ts + tile * TILE * SIDE + c * SIDE + 4 * g);
     f32x4 u = mfma16(inverse, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
     settle(u);

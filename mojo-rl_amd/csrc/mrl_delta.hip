@@ -166,13 +166,13 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Part
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            f32x4 v = V[0], read, o;
+            f32x4 v = V[0], o;
 #pragma unroll
             for (int i = 1; i < TILES; ++i) v = tile == i ? V[i] : v;
             const Pieces<E, DK> pieces(S);
             const f32x4 sk = block.keys.ask(tile, g, c, pieces);
             if (WHAT == OUTPUTS) o = block.queries.ask(tile, g, c, pieces);
-            const f32x4 u = solve(block, tile, g, c, v, sk, read);
+            const f32x4 u = solve(block, tile, g, c, v, sk);
             if (WHAT == OUTPUTS) {
                 o *= block.four(block.query_reads, tile, g);
                 o = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + tile * TILE * SIDE + c * SIDE + 4 * g), u, o);

@@ -11,8 +11,9 @@
 // added up as it stands: every term has a[t] in it.  (Sums of row and column dots, of which this is a difference, lose it where a is small.)
 // dgate = (1 - a) times that, 0 at a cut.
 //
-// With what the forward pass leaves, the dots that the lengths and the gates need are sums over the columns:
-//   q[i] dq[i] = dO[i] out[i],   k[i] dk[i] = dX[i] (2 U[i] - b[i] v[i]),   e[i] = dO[i] (F[i] S0^T q[i]) - dX[i] (b[i] F[i] S0^T k[i]),   f[i] = L[i] U[i] (dS1^T k[i]).
+// The dots that the lengths need are those of the terms: of a row's pairs they are sums over M's parts,
+//   q[i] dq[i] = q[i] (F[i] S0 dO[i]) + sum_j dP[i][j] P[i][j],   k[i] dk[i] = e's share + f[i] + sum_j dA[i][j] A[i][j] + sum_j (dA[j][i] A[j][i] + dP[j][i] P[j][i]),
+// and drate's is -dA's diagonal.
 //
 // A first launch leaves the state ahead of every block of tiles in the workspace (mrl_delta.hip).  In the last a workgroup goes through the blocks
 // of one head of one environment from the last to the first: it repeats a block's tiles forwards, keeping each tile's S0 and U in registers,
@@ -60,10 +61,10 @@ MRL_DEV float sum_ahead(float x) {
     return x + moved<0x118>(x, 0.0f);
 }
 
-// What a tile's columns make of dO and dS1: read = L dS1^T k, dX, and dS1 becomes dS0.
+// What a tile's columns make of dO and dS1: dX, and dS1 becomes dS0.
 template <class E, int DK, int TILES, bool KEEPS>
-MRL_DEV void pull(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &read, f32x4 &dX) {
-    read = block.keys.ask(tile, g, c, Pieces<E, DK>(dS)) * block.four(block.key_takes, tile, g);
+MRL_DEV void pull(const Block<E, DK, TILES, KEEPS> &block, int tile, int g, int c, const f32x4 dO, f32x4 (&dS)[DK / TILE], f32x4 &dX) {
+    const f32x4 read = block.keys.ask(tile, g, c, Pieces<E, DK>(dS)) * block.four(block.key_takes, tile, g);
     f32x4 p_column, t_column;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -145,8 +146,8 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
             for (int tile = TILES - 1; tile >= 0; --tile) {
                 if (block.t0 + tile * block.span >= d.T) continue;
                 anew(g, c);
-                f32x4 read, dX;
-                pull(block, tile, g, c, dO[tile], dS, read, dX);
+                f32x4 dX;
+                pull(block, tile, g, c, dO[tile], dS, dX);
             }
             block.t0 -= TILES;
             ++round;
@@ -161,11 +162,12 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
 
 constexpr bool both_states(int DK) { return DK < 128; }   // S0 and dS1 in LDS side by side
 inline int waves_of(int DK, int dv) { return std::max(column_tiles(dv), std::min(4, DK / TILE)); }
-constexpr int DOTS = 5;   // q dq, k dk, e, f, U dX
+enum { Q_READS, K_READS, K_TAKES, DOTS };                            // q dq and k dk of the terms with S0, k dk of that with dS1: of a wavefront's rows
+enum { CROSSING, PAIRS_ROW_P, PAIRS_ROW_A, PAIRS_COLUMN, U_DX, OF_PAIRS };   // of the pairs, per step
 template <class E>
 size_t back_floats(int DK, int dv) {
     const int columns = TILE * column_tiles(dv) + 4, W = waves_of(DK, dv);
-    return rows_floats<E>(DK, tiles_backward(DK), true) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + 2 * (DOTS * TILE * W + W) + TILE;
+    return rows_floats<E>(DK, tiles_backward(DK), true) + (size_t)(both_states(DK) ? 2 : 1) * DK * columns + 3 * TILE * columns + 2 * TILE * SIDE + (OF_PAIRS + DOTS * W) * TILE + 2 * W;
 }
 
 // EK: the type of the gradients of query and key (float where a group's are summed later)
@@ -180,8 +182,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     int g = lane >> 4, c = lane & 15, thread = threadIdx.x;
     const int stride = TILE * tiles + 4;
     float *const states = lds + rows_floats<E>(DK, TILES, true), *const behind = BOTH ? states + DK * stride : states, *const dOs = behind + DK * stride;
-    float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE, *const crossing = dPs + TILE * SIDE;
-    float *const dots = crossing + TILE, *const wholes = dots + 2 * DOTS * TILE * W;   // [2][DOTS][W][16], [2][W]: two tiles' in turn
+    float *const dXs = dOs + TILE * stride, *const Us = dXs + TILE * stride, *const dAs = Us + TILE * stride, *const dPs = dAs + TILE * SIDE;
+    float *const of_pairs = dPs + TILE * SIDE, *const dots = of_pairs + OF_PAIRS * TILE, *const wholes = dots + DOTS * TILE * W;   // [OF_PAIRS][16], [DOTS][W][16], [2][W]: two tiles' in turn
     const int at_part = group_number(), part = at_part % p.parts.count, nh = at_part / p.parts.count, n = nh / d.H, h = nh - n * d.H, hk = h / (d.H / d.HK);
     const bool owns = w < tiles;   // columns; the other wavefronts have rows only
     const int column = w * TILE + c;
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
     const E *const values = (const E *)d.value + n * d.value_ld + (long)h * d.dv + min(column, d.dv - 1);
     const E *const grads = (const E *)p.grad_out + n * p.grad_out_ld + (long)h * d.dv + min(column, d.dv - 1);
 
-    f32x4 dS[B], S[B], V[TILES], dO[TILES], kept[TILES][B], U[TILES], reads[TILES];
+    f32x4 dS[B], S[B], V[TILES], dO[TILES], kept[TILES][B], U[TILES];
     first_gradient(p, at_part, nh, w, tiles, owns, g, c, dS);
     const auto first_state = [&](int number) {
         if (number > 0) {
@@ -218,13 +220,11 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) S[i] = zero;
             }
-            f32x4 read;
-            const f32x4 u = solve(block, tile, g, c, V[tile], block.keys.ask(tile, g, c, Pieces<E, DK>(S)), read);
+            const f32x4 u = solve(block, tile, g, c, V[tile], block.keys.ask(tile, g, c, Pieces<E, DK>(S)));
             if constexpr (decltype(keep)::value) {
 #pragma unroll
                 for (int i = 0; i < B; ++i) kept[tile][i] = S[i];
                 U[tile] = u;
-                reads[tile] = read;
             }
             if (!decltype(keep)::value || tile + 1 < TILES) go_on(block, tile, g, c, u, S);
         }
@@ -281,10 +281,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 if (block.t0 + tile * block.span >= d.T) continue;
                 anew(g, c);
                 const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
-                float *const dot = dots + turn * DOTS * TILE * W;
                 const f32x4 b = block.four(block.bs, tile, g);
-                const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g);
-                f32x4 dq[OWN], dk[OWN];
+                const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g), ks = block.four(block.key_lengths, tile, g), qs = block.four(block.query_lengths, tile, g);
+                f32x4 q[OWN], k[OWN], dq[OWN], dk[OWN], sums[DOTS] = {zero, zero, zero};   // (this wavefront's rows)
                 const auto read_by_rows = [&]() {   // L dS1 U of this wavefront's rows
 #pragma unroll
                     for (int o = 0; o < OWN; ++o) {
@@ -296,6 +295,8 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                                            *reinterpret_cast<const f32x4 *>(behind + (i * TILE + c) * stride + t * TILE + 4 * g), dk[o]);
                         settle(dk[o]);
                         dk[o] *= to;
+                        k[o] = block.keys.column(tile, i, g, c) * ks;
+                        sums[K_TAKES] += k[o] * dk[o];
                     }
                 };
                 if (owns) {
@@ -310,10 +311,6 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                 }
                 // ---- by columns
                 if (owns) {
-                    f32x4 out = block.queries.ask(tile, g, c, Pieces<E, DK>(kept[tile])) * block.four(block.query_reads, tile, g);
-                    const f32x4 e = dO[tile] * out;
-                    out = mfma16(*reinterpret_cast<const f32x4 *>(block.Ps + (tile * TILE + c) * SIDE + 4 * g), U[tile], out);
-                    settle(out);
                     float s_ds = 0.0f;
 #pragma unroll
                     for (int i = 0; i < B; ++i)
@@ -322,20 +319,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     s_ds = sum_groups(sum16(s_ds));
                     if (lane == 0) wholes[turn * W + w] = s_ds;
                     spread(states, kept[tile]);
-                    f32x4 read, dX;
-                    pull(block, tile, g, c, dO[tile], dS, read, dX);
+                    f32x4 dX;
+                    pull(block, tile, g, c, dO[tile], dS, dX);
                     store_values(d, block, (E *)p.value + n * p.value_ld + (long)h * d.dv + column, (long)d.N * p.value_ld, live, tile, g, b * dX);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int at = (4 * g + r) * stride + column;
                         dOs[at] = dO[tile][r];
                         dXs[at] = dX[r];
-                        const float sums[DOTS] = {sum16(dO[tile][r] * out[r]), sum16(dX[r] * fmaf(2.0f, U[tile][r], -b[r] * V[tile][r])), sum16(fmaf(-dX[r], reads[tile][r], e[r])),
-                                                  sum16(U[tile][r] * read[r]), sum16(U[tile][r] * dX[r])};
-                        if (c == 0) {
-#pragma unroll
-                            for (int k = 0; k < DOTS; ++k) dot[(k * W + w) * TILE + 4 * g + r] = sums[k];
-                        }
                     }
                 }
                 __syncthreads();
@@ -355,8 +346,20 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     settle(dq[o]);
                     settle(reads_by);
                     dq[o] *= from;
+                    reads_by *= -from * b;
+                    q[o] = block.queries.column(tile, i, g, c) * qs;
+                    sums[Q_READS] += q[o] * dq[o];
+                    sums[K_READS] += k[o] * reads_by;
+                    dk[o] += reads_by;
+                }
+                if (w < B) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) dk[o][r] = fmaf(-from[r] * b[r], reads_by[r], dk[o][r]);
+                    for (int s = 0; s < DOTS; ++s)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float sum = sum16(sums[s][r]);
+                            if (c == 0) dots[(s * W + w) * TILE + 4 * g + r] = sum;
+                        }
                 }
                 if (w == pairs_by) {
                     f32x4 dA = zero, dP = zero;
@@ -369,71 +372,80 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     settle(dP);
                     const f32x4 apart = between(block.as + tile * TILE, g, c);
                     f32x4 both;   // dA A + dP P
+                    float diagonal = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int i = 4 * g + r, at = (tile * TILE + i) * SIDE + c;
                         const float a_times = i > c ? -dA[r] : 0.0f, p_times = i >= c ? dP[r] : 0.0f;
-                        both[r] = fmaf(a_times, block.As[at], p_times * block.Ps[at]);
+                        const float of_a = a_times * block.As[at], of_p = p_times * block.Ps[at], row_a = sum16(of_a), row_p = sum16(of_p);
+                        both[r] = of_a + of_p;
+                        diagonal = i == c ? dA[r] : diagonal;
+                        if (c == 0) {
+                            of_pairs[PAIRS_ROW_A * TILE + i] = row_a;
+                            of_pairs[PAIRS_ROW_P * TILE + i] = row_p;
+                        }
                         dAs[i * SIDE + c] = a_times * b[r] * apart[r];
                         dPs[i * SIDE + c] = p_times * apart[r];
                     }
+                    if (c >> 2 == g) of_pairs[U_DX * TILE + c] = diagonal;
                     // sums over the rows from 4 g + r on, and of these over the columns ahead
                     const float mine = (both[0] + both[1]) + (both[2] + both[3]);
                     const float of1 = __shfl(mine, 16 + c), of2 = __shfl(mine, 32 + c), of3 = __shfl(mine, 48 + c);
+                    if (g == 0) of_pairs[PAIRS_COLUMN * TILE + c] = (mine + of1) + (of2 + of3);
                     float run = (g < 3 ? of3 : 0.0f) + (g < 2 ? of2 : 0.0f) + (g < 1 ? of1 : 0.0f);
 #pragma unroll
                     for (int r = 3; r >= 0; --r) {
                         run += both[r];
                         const float sum = sum16(c < 4 * g + r ? run : 0.0f);
-                        if (c == 0) crossing[4 * g + r] = sum;
+                        if (c == 0) of_pairs[CROSSING * TILE + 4 * g + r] = sum;
                     }
                 }
                 __syncthreads();
                 // ---- the tile's own pairs, the lengths, gates and rates
-                const f32x4 ks = block.four(block.key_lengths, tile, g), qs = block.four(block.query_lengths, tile, g);
-                f32x4 q_dot = zero, k_dot = zero;
-                for (int t = 0; t < tiles; ++t) {
-                    q_dot += *reinterpret_cast<const f32x4 *>(dot + t * TILE + 4 * g);
-                    k_dot += *reinterpret_cast<const f32x4 *>(dot + (W + t) * TILE + 4 * g);
+                const auto pairs = [&](int which) { return *reinterpret_cast<const f32x4 *>(of_pairs + which * TILE + 4 * g); };
+                const int row_waves = min(W, B);
+                f32x4 q_dot = pairs(PAIRS_ROW_P), k_dot = pairs(PAIRS_ROW_A) + pairs(PAIRS_COLUMN);
+                for (int t = 0; t < row_waves; ++t) {
+                    q_dot += *reinterpret_cast<const f32x4 *>(dots + (Q_READS * W + t) * TILE + 4 * g);
+                    k_dot += *reinterpret_cast<const f32x4 *>(dots + (K_READS * W + t) * TILE + 4 * g) + *reinterpret_cast<const f32x4 *>(dots + (K_TAKES * W + t) * TILE + 4 * g);
                 }
 #pragma unroll
                 for (int o = 0; o < OWN; ++o) {
                     const int i = w + o * W;
                     if (i >= B) continue;
-                    f32x4 k = block.keys.column(tile, i, g, c) * ks, q = block.queries.column(tile, i, g, c) * qs, a_column, p_column;
+                    f32x4 a_column, p_column;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         a_column[r] = dAs[(4 * g + r) * SIDE + c];
                         p_column[r] = dPs[(4 * g + r) * SIDE + c];
                     }
-                    dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dPs + c * SIDE + 4 * g), k, dq[o]);
-                    dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dAs + c * SIDE + 4 * g), k, dk[o]);
-                    dk[o] = mfma16(p_column, q, mfma16(a_column, k, dk[o]));
+                    dq[o] = mfma16(*reinterpret_cast<const f32x4 *>(dPs + c * SIDE + 4 * g), k[o], dq[o]);
+                    dk[o] = mfma16(*reinterpret_cast<const f32x4 *>(dAs + c * SIDE + 4 * g), k[o], dk[o]);
+                    dk[o] = mfma16(p_column, q[o], mfma16(a_column, k[o], dk[o]));
                     settle(dq[o]);
                     settle(dk[o]);
                     const int at = i * TILE + c;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        q[r] = qs[r] * fmaf(-(float)d.dk * q[r], q_dot[r], dq[o][r]);
-                        k[r] = ks[r] * fmaf(-k[r], k_dot[r], dk[o][r]);
+                        q[o][r] = qs[r] * fmaf(-(float)d.dk * q[o][r], q_dot[r], dq[o][r]);
+                        k[o][r] = ks[r] * fmaf(-k[o][r], k_dot[r], dk[o][r]);
                     }
-                    store_values(d, block, (EK *)p.query + n * p.query_ld + key_at + at, (long)d.N * p.query_ld, at < d.dk, tile, g, q);
-                    store_values(d, block, (EK *)p.key + n * p.key_ld + key_at + at, (long)d.N * p.key_ld, at < d.dk, tile, g, k);
+                    store_values(d, block, (EK *)p.query + n * p.query_ld + key_at + at, (long)d.N * p.query_ld, at < d.dk, tile, g, q[o]);
+                    store_values(d, block, (EK *)p.key + n * p.key_ld + key_at + at, (long)d.N * p.key_ld, at < d.dk, tile, g, k[o]);
                 }
                 if (w == pairs_by && g == 0) {
-                    float e = 0.0f, f = 0.0f, u_dx = 0.0f, all = 0.0f;
-                    for (int t = 0; t < tiles; ++t) {
-                        e += dot[(2 * W + t) * TILE + c];
-                        f += dot[(3 * W + t) * TILE + c];
-                        u_dx += dot[(4 * W + t) * TILE + c];
-                        all += wholes[turn * W + t];
+                    float e = 0.0f, f = 0.0f, all = 0.0f;
+                    for (int t = 0; t < row_waves; ++t) {
+                        e += dots[(Q_READS * W + t) * TILE + c] + dots[(K_READS * W + t) * TILE + c];
+                        f += dots[(K_TAKES * W + t) * TILE + c];
                     }
-                    const float sum = fmaf(block.wholes[tile], all, crossing[c] + (sum_from(e) + sum_ahead(f)));
+                    for (int t = 0; t < tiles; ++t) all += wholes[turn * W + t];
+                    const float sum = fmaf(block.wholes[tile], all, of_pairs[CROSSING * TILE + c] + (sum_from(e) + sum_ahead(f)));
                     const int slot = tile * TILE + c;
                     if (block.there(d, slot)) {
                         const long row = (long)block.time_of(slot) * d.N + n;
                         give((E *)p.gate + row * p.gate_ld + h, block.as[slot] == 0.0f ? 0.0f : block.rests[slot] * sum);
-                        give((E *)p.rate + row * p.rate_ld + h, block.rate_rests[slot] * u_dx);
+                        give((E *)p.rate + row * p.rate_ld + h, block.rate_rests[slot] * of_pairs[U_DX * TILE + c]);
                     }
                 }
                 if constexpr (!BOTH) __syncthreads();
