@@ -9,7 +9,7 @@ namespace {
 // ---------------------------------------------------------------- a few steps
 // A wavefront holds 4 L columns of a head's state in registers: lane l columns 4 (l % L) on, rows l / L, l / L + 64 / L, ..., at most
 // R of them.  S^T k and S^T q are summed in one pass, out = a S^T q + (q k) u follows from them, and the state is read and written once.
-// Bound by that: a step of 8192 environments of 4 heads of 64 x 64 takes 208 us, 5.3 TB/s, what a copy of 256 MiB gets.
+// Bound by that: a step of 8192 environments of 4 heads of 64 x 64 takes 202 us, 5.5 TB/s, what a copy of 256 MiB gets.
 template <class E, int L, int R>
 __global__ __launch_bounds__(256) void steps_kernel(Delta d, int units, int column_blocks) {
     constexpr int G = 64 / L;
@@ -92,7 +92,9 @@ constexpr int MOST_WAVES = 4;
 enum { OUTPUTS, STATES, ENDS };   // of all steps; ahead of every block; M and B of every part
 
 // A workgroup goes through a part's steps of one head of one environment; each of its wavefronts keeps 16 columns of the state in registers,
-// all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare a tile each.
+// all rows of them.  What does not depend on the state (A, its inverse and P) the wavefronts prepare by halves of a tile.
+// 128 steps of 1024 environments of 4 heads of 64 x 64 in fp32 take 225 us (reading and writing the rows once takes 124): the fp32 matrix cores are busy
+// half of that, 213 us pass with all rows in the L2, and the rest is what a block's phases wait for each other.
 template <class E, int DK, int TILES, int WHAT>
 __global__ __launch_bounds__(64 * MOST_WAVES, 4) void tiles_kernel(Delta d, Parts parts, int column_groups, float *states, int blocks) {
     extern __shared__ float lds[];
@@ -259,6 +261,8 @@ __global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, con
     }
 }
 
+// Up to here the state's own pass is ahead of the tiles: 4 steps of 2048 environments take 72 us (108 by tiles), 2 of 4096 112 (195); 16 of 1024 take 58 by
+// tiles, four times the former's work.
 constexpr int FEW_STEPS = 4;
 template <class E, int L>
 void launch_steps(const mrl_ctx *ctx, const Delta &d) {

@@ -187,7 +187,7 @@ struct Tiles {
 // The sums of a tile.  Operands arrive BUFFERS - 1 stages ahead.  AS_IS: A is a matrix of bf16 whose rows are whole 32 elements and start at
 // 16 bytes: lanes read their eight elements where they are.
 // What bounds it: LDS.  A stage of 128 x 256 in bf16 is 64 KiB read and 24 written, 700 cycles of LDS for 512 of the matrix cores; two
-// workgroups a CU have one finish a tile while the other multiplies.  32768 rows of 512 x 2048 in bf16 take 181 us, of which 16 stages'
+// workgroups a CU have one finish a tile while the other multiplies.  32768 rows of 512 x 2048 in bf16 take 175 us, of which 16 stages'
 // loop is 100, the activation 19 and writing the outputs 27 at least (this card's library takes 161 us for the product alone); 256 x 256 by
 // eight wavefronts, one workgroup a CU, 228, or 208 with the next tile's operands asked for ahead of a tile's end, which is slower (188) at 128 x 256;
 // four wavefronts of 64 x 128 each 215.
@@ -549,7 +549,14 @@ __global__ __launch_bounds__(256) void zero_kernel(float *p, long n) {
 }
 
 // ---------------------------------------------------------------- host
-constexpr int FEW = 64;   // rows
+// Where the matrix cores' fp32 keep up with one launch that reads the matrix, no operands are made.  Its time grows with the products of its
+// workgroups, and it reads a long K with too few loads in flight; the tiles' is 14 us for anything small, two launches.  256 -> 1024: 64 rows 7 us
+// (tiles 14), 128 rows 7.6 (14), 256 rows 11.2 (14) in fp32; 256 -> 4096: 64 rows 11.3 (16.3), 12.5 in bf16 (13.6), 128 rows 19.3 (16.8); 2048 -> 512: 64 rows
+// 19.6 (40.8) in fp32, 26.6 (19.3) in bf16.
+inline bool few(const mrl_ctx *ctx, int dtype, int rows, int K, int N) {
+    const long groups = (long)((rows + 15) / 16) * ((N + 15) / 16);
+    return rows <= 256 && (dtype == MRL_F32 ? groups <= ctx->n_cus || groups * K <= 1 << 18 : K <= 512 && groups * K <= 1 << 18);
+}
 inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
 
 // Where things lie in the workspace, in bytes.
@@ -561,7 +568,8 @@ struct Plan {
 template <class S>
 int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
 
-// 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.
+// 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.  256 -> 683, the gradient: 512 rows in fp32 take 53 us with small
+// tiles and 89 with large ones, 32768 rows 688 and 607; in bf16 33 and 59, 298 and 252.
 typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
 typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
 typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
@@ -585,7 +593,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         return was;
     };
     const auto fragments = [&](long rows16, long contracted16, int pieces) { return take(sizeof(__bf16) * KIB * (size_t)rows16 * (contracted16 / 2) * pieces); };
-    if (!backward && M <= FEW) return p;
+    if (!backward && few(ctx, dtype, M, K, N)) return p;
     p.x_rows = fragments(p.M16, p.K16, p.pieces);
     p.w_columns = fragments(2L * p.N16, p.K16, p.pieces);
     if (backward) {
@@ -596,6 +604,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
         const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16GradShape>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
+        // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 65 us, 120 with whole columns; 32768 rows 607 and 1474
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
         if (p.parts > 1) p.partial = take(sizeof(float) * (size_t)p.parts * K * 2 * N);
     }
@@ -645,8 +654,8 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     o.end[2] = o.end[1] + (backward ? column_blocks(p.K16, p.M16 / 2) : 0);
     o.end[3] = o.end[2] + (backward && y.grad_x ? row_blocks(p.K16, p.N16) : 0);
     hipLaunchKernelGGL((operands_kernel<E, P>), dim3(o.end[3]), dim3(256), 0, ctx->stream, o);
-    const auto few = [&](long a, long b) { return tiles<S>(a, b) < ctx->n_cus; };
-    const bool pre_small = few(p.M16, 2L * p.N16);
+    const auto small = [&](long a, long b) { return tiles<S>(a, b) < ctx->n_cus; };
+    const bool pre_small = small(p.M16, 2L * p.N16);
     if (!backward) {
         if (pre_small) Small::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
         else Large::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
@@ -659,7 +668,7 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     const int sum_rows = pre_small ? Small::sum_rows(p) : Large::sum_rows(p);
     const Operand pre_rows = {rows, p.M16}, pre_columns = {columns, 2 * p.N16}, x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
     if (y.grad_x != nullptr) {
-        if (few(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows);
+        if (small(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows);
         else Large::grad_x(ctx, y, p, pre_rows, w_rows);
     }
     const Tiles t = tiles_in<SW>(p.K16, 2L * p.N16, p.M16 / 2, p.parts);
@@ -720,7 +729,7 @@ int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_
     Layer y = {};
     y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
     y.x = in; y.x_ld = in_ld; y.params = params; y.out = out; y.out_ld = out_ld;
-    if (rows <= FEW) {
+    if (few(ctx, dtype, rows, in_dim, out_dim)) {
         const dim3 grid((out_dim + 15) / 16, (rows + 15) / 16);
         if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
         else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);

@@ -120,6 +120,17 @@ def test_forward_and_backward(mrl, ctx, M, K, N, dtype):
     assert torch.equal(gx, again[0]) and torch.equal(grads, again[1]) and torch.equal(grads, alone)
 
 
+# on both sides of what goes straight to registers: long products, wide outputs, 256 rows and one more
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(1, 2050, 17), (65, 513, 40), (64, 512, 2064), (127, 1100, 640), (128, 520, 272), (129, 530, 700), (256, 40, 64), (257, 40, 64), (16, 3, 4100)])
+def test_few_rows_and_tiles(mrl, ctx, M, K, N, dtype):
+    print("gated linear", M, K, N, dtype, flush=True)
+    c = Case(M, K, N, "silu", dtype, wide=M % 2 == 1)
+    out = c.forward(mrl, ctx)
+    ctx.synchronize()
+    near(out, *c.forward64(), "out")
+
+
 @pytest.mark.parametrize("act", ACTIVATIONS)
 @pytest.mark.parametrize("M", [30, 200])
 def test_activations(mrl, ctx, act, M):
@@ -170,7 +181,7 @@ def test_empty_and_refused(mrl, ctx):
     with pytest.raises(mrl.MrlError, match="overlap"):
         layer.backward_gpu(ctx, None, params, out, x, params)
     call, ptr = mrl._lib.call, lambda t: t.data_ptr()   # noqa: E731
-    for args, text in (((0, 0, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "workspace"), ((0, 0, 100, 8, 4, ptr(x), 7, ptr(params), ptr(out), 4, None, 0), "stride"),
+    for args, text in (((0, 0, 300, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "workspace"), ((0, 0, 100, 8, 4, ptr(x), 7, ptr(params), ptr(out), 4, None, 0), "stride"),
                        ((0, 9, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "activation"), ((7, 0, 100, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "type"),
                        ((0, 0, 100, 0, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "dims"), ((0, 0, -1, 8, 4, ptr(x), 8, ptr(params), ptr(out), 4, None, 0), "rows"),
                        ((0, 0, 100, 8, 4, None, 8, ptr(params), ptr(out), 4, None, 0), "NULL")):
