@@ -134,3 +134,17 @@ def test_library_refuses(mrl, ctx):
             call(good, **kwargs)
     call([(at, at + 64, 8, 0), (at, at + 128, 8, 0)])   # the same input twice is fine
     ctx.synchronize()
+
+
+def test_a_tensor_past_2_to_the_31(mrl, ctx):
+    n = (1 << 31) + 4099
+    big, small = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.full((3,), 2.0, device="cuda")
+    big[-1], big[1 << 31], big[5] = 8.0, 4.0, 2.0
+    norm = torch.empty(1, device="cuda")
+    mrl.clip_grad_norm(ctx, [big, small], [big, small], 2.0, norm=norm)
+    ctx.synchronize()
+    length = (64.0 + 16 + 4 + 12) ** 0.5
+    assert abs(norm.item() - length) <= 1.5 * UNIT * length
+    got = torch.stack([big[-1], big[1 << 31], big[5], *small]).double().cpu()
+    want = torch.tensor([8.0, 4.0, 2.0, 2.0, 2.0, 2.0], dtype=torch.float64) * 2 / length
+    assert ((got - want).abs() <= OFF[torch.bfloat16] * want).all() and torch.count_nonzero(big).item() == 3

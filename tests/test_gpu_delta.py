@@ -404,3 +404,29 @@ def test_outputs_on_inputs_are_refused(mrl, ctx):
             backward(**bad)
     ctx.synchronize()
     assert torch.equal(wide, before) and not out.any() and not flat.any() and not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_far_apart(mrl, ctx, dtype):
+    """Rows whose last element is past 2^31 elements and 2^32 bytes from the first."""
+    ld = 1 << 25
+    c = Case(70, 2, 1, 1, 20, 12, dtype, seed=3)
+    room = torch.empty(140 * ld, dtype=c.tt, device="cuda")
+    wide = room.view(140, ld)
+    widths = [*c.widths, 12]
+    places = [(1 << 24) + 100 * i + 1 for i in range(12)]
+    near_rows, near_out, near_grads = c.rows, torch.empty(140, 12, dtype=c.tt, device="cuda"), [torch.empty(140, w, dtype=c.tt, device="cuda") for w in c.widths]
+    far = [wide[:, at:at + w] for at, w in zip(places, widths + list(c.widths) + [12])]
+    for f, r in zip(far, near_rows):
+        f.copy_(r)
+    far[11].copy_(c.grad_out)
+    layer = c.layer(mrl)
+    for rows, out, grads, grad in ((near_rows, near_out, near_grads, c.grad_out), (far[:5], far[5], far[6:11], far[11])):
+        layer.forward_gpu(ctx, out, *rows, 70, state_in=c.state, dones=c.dones, prev_dones=c.prev)
+        layer.backward_gpu(ctx, *grads, grad, *rows, 70, state_in=c.state, dones=c.dones, prev_dones=c.prev)
+    step = torch.empty(2, 12, dtype=c.tt, device="cuda"), far[5][138:]
+    for rows, out in ((near_rows, step[0]), (far[:5], step[1])):
+        layer.step_gpu(ctx, out, *[r[138:] for r in rows], c.state.clone())
+    ctx.synchronize()
+    assert torch.equal(step[0], step[1]) and all(torch.equal(a, b) for a, b in zip(near_grads, far[6:11]))
+    assert torch.equal(near_out[:138], far[5][:138])

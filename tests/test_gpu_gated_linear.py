@@ -237,3 +237,21 @@ def test_rows_that_are_not_finite(mrl, ctx, M, dtype):
     rows[21] = False
     assert torch.equal(bad_x[rows], gx[rows]) and not torch.isfinite(bad_x[21]).any() and torch.isnan(bad_x[17]).all()
     assert torch.isnan(bad_grads.view(-1)[:70 * 100].view(70, 100)[3]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M", [140, 300])
+def test_rows_far_apart(mrl, ctx, M, dtype):
+    """Rows whose last element is past 2^31 elements and 2^32 bytes from the first."""
+    ld = 1 << 24
+    c = Case(M, 96, 40, "silu", dtype, seed=9)
+    wide = torch.empty(M * ld, dtype=c.tt, device="cuda").view(M, ld)
+    x, grad, out, gx = (wide[:, at:at + w] for at, w in ((1 << 23, 96), ((1 << 23) + 104, 40), ((1 << 23) + 200, 40), (ld - 96, 96)))
+    x.copy_(c.x)
+    grad.copy_(c.grad)
+    want, (want_x, want_grads) = c.forward(mrl, ctx), c.backward(mrl, ctx)
+    grads = torch.empty_like(want_grads)
+    c.layer(mrl).forward_gpu(ctx, out, x, c.params)
+    c.layer(mrl).backward_gpu(ctx, gx, grads, grad, x, c.params)
+    ctx.synchronize()
+    assert torch.equal(out, want) and torch.equal(gx, want_x) and torch.equal(grads, want_grads)
