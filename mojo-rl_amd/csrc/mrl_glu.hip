@@ -7,7 +7,7 @@
 //
 // Products run on the bf16 matrix cores with fp32 sums.  bf16 values are operands as they are.  An fp32 value is three bf16 pieces
 // (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup] goes into dx as one piece, like any bf16
-// activation between two products (rounding it costs dx what rounding dx costs), and into dW, which is fp32, as two: 2^-17 of a term off.
+// activation between two products (rounding it costs dx what rounding dx costs), and into dW, which is fp32, as three, or two (column_pieces).
 //
 // Operands lie in the workspace as fragments: 16 rows and 32 of the contracted index, a KiB in the order in which the 64 lanes of
 // v_mfma_f32_16x16x32_bf16 hold them (lane 16 g + n: row n, elements 8 g .. 8 g + 7), the pieces of a fragment next to each other, all rows'
@@ -572,10 +572,16 @@ int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S
 // tiles and 89 with large ones, 32768 rows 688 and 607; in bf16 33 and 59, 298 and 252.
 typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
 typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
-typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16GradShape;    // 128 x 128, two pieces of [dgate | dup]
+typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16ManyRows;     // dW: 128 x 128, two pieces of [dgate | dup]
+typedef Shape<1, 3, 2, 4, 4, 2, 4> Bf16FewRows;      // and three
 typedef Shape<3, 3, 2, 4, 4, 2, 3> F32Shape;
 typedef Shape<3, 3, 4, 2, 1, 2, 3> F32Small;
 constexpr int WR_MOST = 4;
+
+// The pieces of [dgate | dup] for dW: 22 bits and more.  In bf16, whose other factor is one piece, two (16 bits) from 2^14 rows on: they are 2.5e-6 off
+// in the 2-norm, while fp32 sums of products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7,
+// 2e-7 and 5e-7.  16384 rows of 512 -> 1024 take 217 us with two and 258 with three, 2048 of 256 -> 683 40 and 42.
+inline int column_pieces(int dtype, int M) { return dtype == MRL_F32 || M < 1 << 14 ? 3 : 2; }
 
 Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) {
     Plan p = {};
@@ -585,7 +591,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
     const bool f32 = dtype == MRL_F32;
     p.pieces = f32 ? 3 : 1;
     p.row_pieces = f32 ? 3 : 1;
-    p.column_pieces = f32 ? 3 : 2;
+    p.column_pieces = column_pieces(dtype, M);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         const size_t was = at;
@@ -602,7 +608,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.pre_rows = fragments(p.M16, 2L * p.N16, p.row_pieces);
         p.pre_columns = fragments(2L * p.N16, p.M16, p.column_pieces);
         p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
-        const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16GradShape>(p.K16, 2L * p.N16);
+        const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16ManyRows>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
         // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 65 us, 120 with whole columns; 32768 rows 607 and 1474
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
@@ -734,7 +740,7 @@ int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_
         if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
         else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
     } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, false);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16FewRows, 1, 1, 3>(ctx, y, p, (char *)workspace, false);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -768,7 +774,8 @@ int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in
     y.x = in; y.x_ld = in_ld; y.params = params; y.grad_out = grad_out; y.grad_out_ld = grad_out_ld;
     y.grad_x = grad_in; y.grad_x_ld = grad_in_ld; y.grads = grads;
     if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16GradShape, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
+    else if (p.column_pieces == 3) launch<bf16_t, Bf16Shape, Bf16Small, Bf16FewRows, 1, 1, 3>(ctx, y, p, (char *)workspace, true);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16ManyRows, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }

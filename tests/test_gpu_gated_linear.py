@@ -255,3 +255,18 @@ def test_rows_far_apart(mrl, ctx, M, dtype):
     c.layer(mrl).backward_gpu(ctx, gx, grads, grad, x, c.params)
     ctx.synchronize()
     assert torch.equal(out, want) and torch.equal(gx, want_x) and torch.equal(grads, want_grads)
+
+
+@pytest.mark.parametrize("M", [40, 16383, 16384])
+def test_pieces_of_the_parameters_gradient(mrl, ctx, M):
+    """In bf16: below 2^14 rows the gradient's terms have 22 bits, from there on 16."""
+    c = Case(M, 24, 20, "silu", "bf16", seed=11)
+    _, grads = c.backward(mrl, ctx)
+    ctx.synchronize()
+    _, (want, off) = c.backward64()
+    near(grads, want, off, "grads")
+    # A sum's terms are off independently of each other, each by at most 2^-22 or 2^-16 of itself and by the roundings of the activation's slope, some 24
+    # units; a running sum by half a unit of itself, 6 times for every 32 rows: in the 2-norm over all sums their root squares add.
+    rows = math.sqrt(6 * M / 32)
+    bound = (2.0 ** -22 + 24 * UNIT + rows * UNIT) if M < 1 << 14 else 2.0 ** -16 + 24 * UNIT + rows * UNIT
+    assert (grads.cpu().double() - want).norm() <= bound * want.norm()
