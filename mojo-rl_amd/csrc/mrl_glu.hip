@@ -625,14 +625,15 @@ struct Launch {
     template <bool FORWARD>
     static void pre(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is, __bf16 *rows = nullptr, __bf16 *columns = nullptr,
                     float *sums = nullptr) {
+        constexpr int ROW_PIECES = FORWARD ? 1 : PR, COLUMN_PIECES = FORWARD ? 1 : PC;   // (not written forwards)
         const Tiles t = tiles_in<S>(p.M16, 2L * p.N16, p.K16 / 2);
         if constexpr (P == 1) {
             if (as_is) {
-                hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, true, PR, PC>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
+                hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, true, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
                 return;
             }
         }
-        hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, PR, PC>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
+        hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
     }
     static int sum_rows(const Plan &p) { return tiles_in<S>(p.M16, 1, 1).down * S::WR; }
     static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w) {
