@@ -3,8 +3,8 @@
 // Two launches, each over all tensors in pieces of PIECE values: partial sums of squares, then every workgroup adds up the partial sums
 // (the same order everywhere) and scales its pieces.  Squares and sums are Float64: no value's square overflows or vanishes, and the order of a
 // few thousand partial sums does not show in fp32.  Bound by memory: every value is read twice, the second time out of the last-level
-// cache where the tensors fit, and written once.  107 MB in 20 tensors take 19 us to sum (5.6 TB/s) and 36 to scale (5.9 TB/s), what this card copies
-256 MiB with; 12 small tensors take 4 us twice, and the host 25 to make the two calls.
+// cache where the tensors fit, and written once.  107 MB in 20 tensors take 19 us to sum (5.6 TB/s) and 36 to scale (5.9 TB/s), what this
+// card copies 256 MiB with; 12 small tensors take 4 us twice, and the host 25 to make the two calls.
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
 
@@ -152,6 +152,7 @@ int mrl_clip_tensors(mrl_ctx *ctx, int count, const mrl_tensor *tensors, double 
     const char *who = "mrl_clip_tensors";
     MRL_CHECK_ARG(ctx, "%s: ctx is NULL", who);
     MRL_CHECK_ARG(count >= 0 && (count == 0 || tensors), "%s: %d tensors", who, count);
+    MRL_CHECK_ARG(max_norm >= 0.0, "%s: max_norm %g is below 0", who, max_norm);
     MRL_CHECK_ARG(workspace && workspace_bytes >= MRL_CLIP_TENSORS_WORKSPACE, "%s: the workspace holds %llu bytes, need %d", who,
                   (unsigned long long)(workspace ? workspace_bytes : 0), MRL_CLIP_TENSORS_WORKSPACE);
     MRL_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", who);

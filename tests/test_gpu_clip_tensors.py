@@ -148,3 +148,13 @@ def test_a_tensor_past_2_to_the_31(mrl, ctx):
     got = torch.stack([big[-1], big[1 << 31], big[5], *small]).double().cpu()
     want = torch.tensor([8.0, 4.0, 2.0, 2.0, 2.0, 2.0], dtype=torch.float64) * 2 / length
     assert ((got - want).abs() <= OFF[torch.bfloat16] * want).all() and torch.count_nonzero(big).item() == 3
+
+
+@pytest.mark.parametrize("max_norm", [-1.0, float("nan")])
+def test_library_refuses_a_norm_below_0(mrl, ctx, max_norm):
+    x, ws = torch.ones(8, device="cuda"), torch.empty(mrl._lib.CLIP_TENSORS_WORKSPACE, dtype=torch.uint8, device="cuda")
+    entries = (mrl._lib.Tensor * 1)((x.data_ptr(), x.data_ptr(), 8, 0))
+    with pytest.raises(mrl.MrlError, match="max_norm"):
+        mrl._lib.call("mrl_clip_tensors", ctx.handle, 1, entries, max_norm, None, ws.data_ptr(), mrl._lib.CLIP_TENSORS_WORKSPACE)
+    ctx.synchronize()
+    assert (x == 1).all()
