@@ -421,9 +421,9 @@ __global__ __launch_bounds__(S::THREADS) void pre_kernel(Layer y, Operand a, Ope
     }
 }
 
-// dx: rows times the matrix' rows
+// dx: rows times the matrix' rows; where `all` has parts, their sums to partial [part][M, K]
 template <class E, class S>
-__global__ __launch_bounds__(S::THREADS) void grad_x_kernel(Layer y, Operand a, Operand b, Tiles all) {
+__global__ __launch_bounds__(S::THREADS) void grad_x_kernel(Layer y, Operand a, Operand b, Tiles all, float *partial) {
     extern __shared__ __bf16 lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
     int bi, bj, part, from, to;
@@ -433,8 +433,11 @@ __global__ __launch_bounds__(S::THREADS) void grad_x_kernel(Layer y, Operand a, 
 #pragma unroll
     for (int i = 0; i < S::FA; ++i)
 #pragma unroll
-        for (int j = 0; j < S::FB; ++j)
-            store_tile((E *)y.grad_x, y.grad_x_ld, acc[i][j], (bi * S::ROWS + wr * S::FA + i) * 16, (bj * S::COLUMNS + wc * S::FB + j) * 16, y.M, y.K, g, c);
+        for (int j = 0; j < S::FB; ++j) {
+            const int row = (bi * S::ROWS + wr * S::FA + i) * 16, column = (bj * S::COLUMNS + wc * S::FB + j) * 16;
+            if (partial != nullptr) store_tile(partial + (long)part * y.M * y.K, y.K, acc[i][j], row, column, y.M, y.K, g, c);
+            else store_tile((E *)y.grad_x, y.grad_x_ld, acc[i][j], row, column, y.M, y.K, g, c);
+        }
 }
 
 // dW, a share of the rows per workgroup where `parts` is more than 1: [part][K, 2 N]
@@ -456,10 +459,29 @@ __global__ __launch_bounds__(S::THREADS) void grad_w_kernel(int K, int N, Operan
         }
 }
 
-// The biases' gradients from the sums of rows of wavefronts, by the first workgroups, 64 columns each; the parts of dW added up, in order, by the others.
-__global__ __launch_bounds__(256) void finish_kernel(const float *parts, int count, long values, const float *sums, int rows, int columns, int N, float *grads) {
+// The biases' gradients from the sums of rows of wavefronts, by the first workgroups, 64 columns each; the parts of dW added up, in order, by the next
+// w_blocks, those of dx by the others, 1024 values each.
+struct XParts {
+    const float *at;
+    int count;
+};
+template <class E>
+__global__ __launch_bounds__(256) void finish_kernel(const float *parts, int count, long values, const float *sums, int rows, int columns, int w_blocks, XParts x, Layer y) {
     __shared__ float shared[4][64];
-    const int bias_blocks = (columns + 63) / 64;
+    const int bias_blocks = (columns + 63) / 64, N = y.N;
+    float *const grads = y.grads;
+    if ((int)blockIdx.x >= bias_blocks + w_blocks) {
+        const int all = y.M * y.K;   // (parts come with few tiles)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = ((int)blockIdx.x - bias_blocks - w_blocks) * 1024 + j * 256 + (int)threadIdx.x;
+            if (i >= all) break;
+            float sum = x.at[i];
+            for (int p = 1; p < x.count; ++p) sum += x.at[(long)p * all + i];
+            give((E *)y.grad_x + i / y.K * y.grad_x_ld + i % y.K, sum);
+        }
+        return;
+    }
     if ((int)blockIdx.x < bias_blocks) {
         const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, at = blockIdx.x * 64 + lane;
         float sum = 0.0f;
@@ -562,8 +584,8 @@ inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
 // Where things lie in the workspace, in bytes.
 struct Plan {
     int M16, K16, N16;   // fragments of the rows, of the matrix' rows and (pairs) of its columns, an even number of the first two
-    int pieces, row_pieces, column_pieces, parts;
-    size_t x_rows, w_columns, x_columns, w_rows, pre_rows, pre_columns, sums, partial, bytes;
+    int pieces, row_pieces, column_pieces, parts, x_parts;
+    size_t x_rows, w_columns, x_columns, w_rows, pre_rows, pre_columns, sums, partial, x_partial, bytes;
 };
 template <class S>
 int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
@@ -577,6 +599,7 @@ typedef Shape<1, 3, 2, 4, 4, 2, 4> Bf16FewRows;      // and three
 typedef Shape<3, 3, 2, 4, 4, 2, 3> F32Shape;
 typedef Shape<3, 3, 4, 2, 1, 2, 3> F32Small;
 constexpr int WR_MOST = 4;
+constexpr int X_STAGES = 8;   // of 32 of the contracted index, for a part of dx at least
 
 // The pieces of [dgate | dup] for dW: 22 bits and more.  In bf16, whose other factor is one piece, two (16 bits) from 2^14 rows on: they are 2.5e-6 off
 // in the 2-norm, while fp32 sums of products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7,
@@ -610,9 +633,13 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
         const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16ManyRows>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
-        // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 65 us, 120 with whole columns; 32768 rows 607 and 1474
+        // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 62 us, 116 with whole columns; 32768 rows 607 and 1474
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
         if (p.parts > 1) p.partial = take(sizeof(float) * (size_t)p.parts * K * 2 * N);
+        // so are dx's where there are few rows: 2048 rows of 256 -> 683 in fp32 take 62 us, 69 whole; 512 rows 45 and 55, in bf16 34 and 36
+        const int large = f32 ? tiles<F32Shape>(p.M16, p.K16) : tiles<Bf16Shape>(p.M16, p.K16), small = f32 ? tiles<F32Small>(p.M16, p.K16) : tiles<Bf16Small>(p.M16, p.K16);
+        p.x_parts = large >= ctx->n_cus ? 1 : std::max(1, std::min(p.N16 / X_STAGES, ctx->n_cus / small));
+        if (p.x_parts > 1) p.x_partial = take(sizeof(float) * (size_t)p.x_parts * M * K);
     }
     p.bytes = at;
     return p;
@@ -636,9 +663,9 @@ struct Launch {
         hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
     }
     static int sum_rows(const Plan &p) { return tiles_in<S>(p.M16, 1, 1).down * S::WR; }
-    static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w) {
-        const Tiles t = tiles_in<S>(p.M16, p.K16, p.N16);
-        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t);
+    static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w, float *partial) {
+        const Tiles t = tiles_in<S>(p.M16, p.K16, p.N16, p.x_parts);
+        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t, partial);
     }
 };
 
@@ -675,15 +702,19 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     const int sum_rows = pre_small ? Small::sum_rows(p) : Large::sum_rows(p);
     const Operand pre_rows = {rows, p.M16}, pre_columns = {columns, 2 * p.N16}, x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
     if (y.grad_x != nullptr) {
-        if (small(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows);
-        else Large::grad_x(ctx, y, p, pre_rows, w_rows);
+        float *const partial = p.x_parts > 1 ? (float *)(ws + p.x_partial) : nullptr;
+        if (small(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows, partial);
+        else Large::grad_x(ctx, y, p, pre_rows, w_rows, partial);
     }
     const Tiles t = tiles_in<SW>(p.K16, 2L * p.N16, p.M16 / 2, p.parts);
     const long values = (long)y.K * 2 * y.N;
     float *const to = p.parts > 1 ? (float *)(ws + p.partial) : y.grads;
     hipLaunchKernelGGL((grad_w_kernel<SW>), dim3(t.count()), dim3(SW::THREADS), SW::LDS, ctx->stream, y.K, y.N, x_columns, pre_columns, t, to);
-    const long blocks = (2L * p.N16 * 16 + 63) / 64 + (p.parts > 1 ? (values + 1023) / 1024 : 0);
-    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, to, p.parts, values, sums, sum_rows, 2 * p.N16 * 16, y.N, y.grads);
+    const int bias_blocks = (2 * p.N16 * 16 + 63) / 64;
+    const long w_blocks = p.parts > 1 ? (values + 1023) / 1024 : 0, x_blocks = y.grad_x != nullptr && p.x_parts > 1 ? ((long)y.M * y.K + 1023) / 1024 : 0;
+    const XParts x = {(const float *)(ws + p.x_partial), p.x_parts};
+    hipLaunchKernelGGL(finish_kernel<E>, dim3((unsigned)(bias_blocks + w_blocks + x_blocks)), dim3(256), 0, ctx->stream, to, p.parts, values, sums, sum_rows, 2 * p.N16 * 16,
+                       (int)w_blocks, x, y);
 }
 
 int check_sizes(const char *who, int dtype, int act, int64_t rows, int in_dim, int out_dim) {
