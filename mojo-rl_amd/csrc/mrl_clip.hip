@@ -4,7 +4,7 @@
 // (the same order everywhere) and scales its pieces.  Squares and sums are Float64: no value's square overflows or vanishes, and the order of a
 // few thousand partial sums does not show in fp32.  Bound by memory: every value is read twice, the second time out of the last-level
 // cache where the tensors fit, and written once.  107 MB in 20 tensors take 19 us to sum (5.6 TB/s) and 36 to scale (5.9 TB/s), what this
-// card copies 256 MiB with; 12 small tensors take 4 us twice, and the host 25 to make the two calls.
+// card copies 256 MiB with; 12 small tensors take 4 us twice, and the host 22 to make the two calls.
 #include "mrl_host.hpp"
 #include "mrl_device.hpp"
 

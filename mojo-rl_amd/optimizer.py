@@ -2,6 +2,7 @@
 (deep_rl/optimizer/adam.mojo) and Muon, which updates a network's hidden matrices by their orthogonalised momentum and everything
 else by Adam.  `t` and `lr` live on the host object, as in the reference (the PPO agent anneals `lr` between rollouts); state is
 [PARAM_SIZE, 2] interleaved (m, v)."""
+import array
 import ctypes as C
 import functools
 
@@ -35,22 +36,28 @@ def clip_grad_norm(ctx, out, grads, max_norm, norm=None):
     not overlap a tensor otherwise.  ppo.clip_grad_norm is the same for one vector."""
     if len(out) != len(grads):
         raise _lib.MrlError("clip_grad_norm: %d outputs for %d gradients" % (len(out), len(grads)))
-    entries = []
+    index = ctx.device.index if ctx.device.type == "cuda" else None   # (an int is compared faster than a device)
+    words = []                                                        # a Tensor is four: src, out, n, dtype
     for i, (o, g) in enumerate(zip(out, grads)):
-        kind = _TYPES.get(g.dtype)
+        dtype = g.dtype
+        kind = _TYPES.get(dtype)
         if kind is None:
-            raise _lib.MrlError("clip_grad_norm: grads[%d]: float32 or bfloat16 expected, got %s" % (i, g.dtype))
-        if o is not g:
-            if o.shape != g.shape or o.dtype is not g.dtype:
-                raise _lib.MrlError("clip_grad_norm: out[%d] %s of %s does not fit %s of %s" % (i, list(o.shape), o.dtype, list(g.shape), g.dtype))
-            if not o.is_contiguous():
-                raise _lib.MrlError("clip_grad_norm: out[%d] must be contiguous" % i)
+            raise _lib.MrlError("clip_grad_norm: grads[%d]: float32 or bfloat16 expected, got %s" % (i, dtype))
         if not g.is_contiguous():
             raise _lib.MrlError("clip_grad_norm: grads[%d] must be contiguous" % i)
-        if g.device != ctx.device or o.device != ctx.device:
+        if g.get_device() != index:
             _on_device(ctx, "grads[%d]" % i, g)
+        at = g.data_ptr()
+        if o is g:
+            words += (at, at, g.numel(), kind)
+            continue
+        if o.dtype is not dtype or o.shape != g.shape:
+            raise _lib.MrlError("clip_grad_norm: out[%d] %s of %s does not fit %s of %s" % (i, list(o.shape), o.dtype, list(g.shape), dtype))
+        if not o.is_contiguous():
+            raise _lib.MrlError("clip_grad_norm: out[%d] must be contiguous" % i)
+        if o.get_device() != index:
             _on_device(ctx, "out[%d]" % i, o)
-        entries.append((g.data_ptr(), o.data_ptr(), g.numel(), kind))
+        words += (at, o.data_ptr(), g.numel(), kind)
     if not max_norm >= 0:
         raise _lib.MrlError("clip_grad_norm: max_norm %s is below 0" % max_norm)
     if norm is not None:
@@ -58,8 +65,10 @@ def clip_grad_norm(ctx, out, grads, max_norm, norm=None):
             raise _lib.MrlError("clip_grad_norm: norm: one float32 value expected, got %s of %s" % (list(norm.shape), norm.dtype))
         _on_device(ctx, "norm", norm)
     ws = _scratch(ctx, _lib.CLIP_TENSORS_WORKSPACE)
-    _lib.call("mrl_clip_tensors", ctx.handle, len(entries), (_lib.Tensor * len(entries))(*entries), float(max_norm),
-              None if norm is None else norm.data_ptr(), ws.data_ptr(), _lib.CLIP_TENSORS_WORKSPACE)
+    count = len(grads)
+    tensors = (_lib.Tensor * count).from_buffer(array.array("q", words)) if count else None
+    _lib.call("mrl_clip_tensors", ctx.handle, count, tensors, float(max_norm), None if norm is None else norm.data_ptr(), ws.data_ptr(),
+              _lib.CLIP_TENSORS_WORKSPACE)
 
 
 @functools.lru_cache(maxsize=None)
