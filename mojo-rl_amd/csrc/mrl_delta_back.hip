@@ -20,6 +20,11 @@
 // and takes the tiles backwards.  A wavefront holds 16 columns of S0 and dS1; what contracts over the columns (dq, dk, dA, dP) is done by 16
 // rows of the states per wavefront, which they pass through LDS.  A rollout in parts has the gradients of the states behind the parts worked out
 // ahead of that (chain_kernel, and the launch that goes through the parts).
+//
+// 128 steps of 512 environments of 4 heads of 64 x 64 in fp32 take 501 us, 82 of them the first launch (reading and writing the rows once takes 105, the
+// formulas' products at the rate of a large fp32 one 140).  Bound by what a tile's phases wait for each other: the matrix cores are busy a third of the time,
+// other instructions a quarter; LDS has room for two workgroups of four wavefronts a CU (78 KB; one takes 755 us).  Memory is no part of it: 489
+// with all rows in the L2.  The pairs' sums by two wavefronts instead of one: 501 for 506; the lengths' dots from terms that are there: 507 for 520.
 #include <type_traits>
 #include "delta.hpp"
 
@@ -163,7 +168,8 @@ __global__ __launch_bounds__(256, 2) void chain_kernel(Back p, int column_groups
 constexpr bool both_states(int DK) { return DK < 128; }   // S0 and dS1 in LDS side by side
 inline int waves_of(int DK, int dv) { return std::max(column_tiles(dv), std::min(4, DK / TILE)); }
 enum { Q_READS, K_READS, K_TAKES, DOTS };                            // q dq and k dk of the terms with S0, k dk of that with dS1: of a wavefront's rows
-enum { CROSSING, PAIRS_ROW_P, PAIRS_ROW_A, PAIRS_COLUMN, U_DX, OF_PAIRS };   // of the pairs, per step
+enum { OF_A, OF_P = 3, U_DX = 6, OF_PAIRS };                            // of the pairs, per step: of dA and of dP the next three,
+enum { CROSSING, ROW, COLUMN };                                        // sums over what crosses the step, over its row and over its column
 template <class E>
 size_t back_floats(int DK, int dv) {
     const int columns = TILE * column_tiles(dv) + 4, W = waves_of(DK, dv);
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
             for (int tile = TILES - 1; tile >= 0; --tile) {
                 if (block.t0 + tile * block.span >= d.T) continue;
                 anew(g, c);
-                const int turn = tile & 1, pairs_by = W > B ? W - 1 : tile % W;   // the wavefront that has dA, dP and what hangs on them
+                const int turn = tile & 1, has_a = W > B ? W - 1 : 2 * tile % W, has_p = W > B + 1 ? W - 2 : (2 * tile + 1) % W;   // the wavefronts that have dA and dP
                 const f32x4 b = block.four(block.bs, tile, g);
                 const f32x4 from = block.four(block.from, tile, g), to = block.four(block.to, tile, g), ks = block.four(block.key_lengths, tile, g), qs = block.four(block.query_lengths, tile, g);
                 f32x4 q[OWN], k[OWN], dq[OWN], dk[OWN], sums[DOTS] = {zero, zero, zero};   // (this wavefront's rows)
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     }
                 }
                 __syncthreads();
-                // ---- by rows of the states, their terms of dq and dk; by one wavefront, dA and dP
+                // ---- by rows of the states, their terms of dq and dk; by a wavefront each, dA and dP
                 if constexpr (BOTH) read_by_rows();
 #pragma unroll
                 for (int o = 0; o < OWN; ++o) {
@@ -361,50 +367,46 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                             if (c == 0) dots[(s * W + w) * TILE + 4 * g + r] = sum;
                         }
                 }
-                if (w == pairs_by) {
-                    f32x4 dA = zero, dP = zero;
-                    for (int t = 0; t < tiles; ++t) {
-                        const f32x4 u = *reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g);
-                        dA = mfma16(*reinterpret_cast<const f32x4 *>(dXs + c * stride + t * TILE + 4 * g), u, dA);
-                        dP = mfma16(*reinterpret_cast<const f32x4 *>(dOs + c * stride + t * TILE + 4 * g), u, dP);
-                    }
-                    settle(dA);
-                    settle(dP);
+                const auto pairs = [&](auto of_a) {
+                    constexpr bool A = decltype(of_a)::value;
+                    float *const sums_of = of_pairs + (A ? OF_A : OF_P) * TILE, *const rows = A ? dXs : dOs, *const factors = A ? block.As : block.Ps, *const to = A ? dAs : dPs;
+                    f32x4 d = zero;
+                    for (int t = 0; t < tiles; ++t)
+                        d = mfma16(*reinterpret_cast<const f32x4 *>(rows + c * stride + t * TILE + 4 * g), *reinterpret_cast<const f32x4 *>(Us + c * stride + t * TILE + 4 * g), d);
+                    settle(d);
                     const f32x4 apart = between(block.as + tile * TILE, g, c);
-                    f32x4 both;   // dA A + dP P
+                    f32x4 m;   // dA A or dP P
                     float diagonal = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int i = 4 * g + r, at = (tile * TILE + i) * SIDE + c;
-                        const float a_times = i > c ? -dA[r] : 0.0f, p_times = i >= c ? dP[r] : 0.0f;
-                        const float of_a = a_times * block.As[at], of_p = p_times * block.Ps[at], row_a = sum16(of_a), row_p = sum16(of_p);
-                        both[r] = of_a + of_p;
-                        diagonal = i == c ? dA[r] : diagonal;
-                        if (c == 0) {
-                            of_pairs[PAIRS_ROW_A * TILE + i] = row_a;
-                            of_pairs[PAIRS_ROW_P * TILE + i] = row_p;
-                        }
-                        dAs[i * SIDE + c] = a_times * b[r] * apart[r];
-                        dPs[i * SIDE + c] = p_times * apart[r];
+                        const int i = 4 * g + r;
+                        const float x = A ? (i > c ? -d[r] : 0.0f) : (i >= c ? d[r] : 0.0f);
+                        m[r] = x * factors[(tile * TILE + i) * SIDE + c];
+                        to[i * SIDE + c] = x * apart[r] * (A ? b[r] : 1.0f);
+                        const float row = sum16(m[r]);
+                        if (c == 0) sums_of[ROW * TILE + i] = row;
+                        diagonal = i == c ? d[r] : diagonal;
                     }
-                    if (c >> 2 == g) of_pairs[U_DX * TILE + c] = diagonal;
+                    if (A && c >> 2 == g) of_pairs[U_DX * TILE + c] = diagonal;
                     // sums over the rows from 4 g + r on, and of these over the columns ahead
-                    const float mine = (both[0] + both[1]) + (both[2] + both[3]);
+                    const float mine = (m[0] + m[1]) + (m[2] + m[3]);
                     const float of1 = __shfl(mine, 16 + c), of2 = __shfl(mine, 32 + c), of3 = __shfl(mine, 48 + c);
-                    if (g == 0) of_pairs[PAIRS_COLUMN * TILE + c] = (mine + of1) + (of2 + of3);
+                    if (g == 0) sums_of[COLUMN * TILE + c] = (mine + of1) + (of2 + of3);
                     float run = (g < 3 ? of3 : 0.0f) + (g < 2 ? of2 : 0.0f) + (g < 1 ? of1 : 0.0f);
 #pragma unroll
                     for (int r = 3; r >= 0; --r) {
-                        run += both[r];
+                        run += m[r];
                         const float sum = sum16(c < 4 * g + r ? run : 0.0f);
-                        if (c == 0) of_pairs[CROSSING * TILE + 4 * g + r] = sum;
+                        if (c == 0) sums_of[CROSSING * TILE + 4 * g + r] = sum;
                     }
-                }
+                };
+                if (w == has_a) pairs(std::true_type{});
+                if (w == has_p) pairs(std::false_type{});
                 __syncthreads();
                 // ---- the tile's own pairs, the lengths, gates and rates
-                const auto pairs = [&](int which) { return *reinterpret_cast<const f32x4 *>(of_pairs + which * TILE + 4 * g); };
+                const auto of_pair = [&](int which) { return *reinterpret_cast<const f32x4 *>(of_pairs + which * TILE + 4 * g); };
                 const int row_waves = min(W, B);
-                f32x4 q_dot = pairs(PAIRS_ROW_P), k_dot = pairs(PAIRS_ROW_A) + pairs(PAIRS_COLUMN);
+                f32x4 q_dot = of_pair(OF_P + ROW), k_dot = of_pair(OF_A + ROW) + (of_pair(OF_A + COLUMN) + of_pair(OF_P + COLUMN));
                 for (int t = 0; t < row_waves; ++t) {
                     q_dot += *reinterpret_cast<const f32x4 *>(dots + (Q_READS * W + t) * TILE + 4 * g);
                     k_dot += *reinterpret_cast<const f32x4 *>(dots + (K_READS * W + t) * TILE + 4 * g) + *reinterpret_cast<const f32x4 *>(dots + (K_TAKES * W + t) * TILE + 4 * g);
@@ -433,14 +435,14 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                     store_values(d, block, (EK *)p.query + n * p.query_ld + key_at + at, (long)d.N * p.query_ld, at < d.dk, tile, g, q[o]);
                     store_values(d, block, (EK *)p.key + n * p.key_ld + key_at + at, (long)d.N * p.key_ld, at < d.dk, tile, g, k[o]);
                 }
-                if (w == pairs_by && g == 0) {
+                if (w == has_a && g == 0) {
                     float e = 0.0f, f = 0.0f, all = 0.0f;
                     for (int t = 0; t < row_waves; ++t) {
                         e += dots[(Q_READS * W + t) * TILE + c] + dots[(K_READS * W + t) * TILE + c];
                         f += dots[(K_TAKES * W + t) * TILE + c];
                     }
                     for (int t = 0; t < tiles; ++t) all += wholes[turn * W + t];
-                    const float sum = fmaf(block.wholes[tile], all, of_pairs[CROSSING * TILE + c] + (sum_from(e) + sum_ahead(f)));
+                    const float sum = fmaf(block.wholes[tile], all, (of_pairs[(OF_A + CROSSING) * TILE + c] + of_pairs[(OF_P + CROSSING) * TILE + c]) + (sum_from(e) + sum_ahead(f)));
                     const int slot = tile * TILE + c;
                     if (block.there(d, slot)) {
                         const long row = (long)block.time_of(slot) * d.N + n;
