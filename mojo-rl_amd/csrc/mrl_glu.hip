@@ -574,10 +574,10 @@ __global__ __launch_bounds__(256) void zero_kernel(float *p, long n) {
 // Where the matrix cores' fp32 keep up with one launch that reads the matrix, no operands are made.  Its time grows with the products of its
 // workgroups, and it reads a long K with too few loads in flight; the tiles' is 14 us for anything small, two launches.  256 -> 1024: 64 rows 7 us
 // (tiles 14), 128 rows 7.6 (14), 256 rows 11.2 (14) in fp32; 256 -> 4096: 64 rows 11.3 (16.3), 12.5 in bf16 (13.6), 128 rows 19.3 (16.8); 2048 -> 512: 64 rows
-// 19.6 (40.8) in fp32, 26.6 (19.3) in bf16.
+// 19.6 (40.8) in fp32, 26.6 (19.3) in bf16; 2048 -> 4096: 32 rows 42.5 (59) in fp32, 52 (33.7) in bf16, 64 rows 84 (59).
 inline bool few(const mrl_ctx *ctx, int dtype, int rows, int K, int N) {
     const long groups = (long)((rows + 15) / 16) * ((N + 15) / 16);
-    return rows <= 256 && (dtype == MRL_F32 ? groups <= ctx->n_cus || groups * K <= 1 << 18 : K <= 512 && groups * K <= 1 << 18);
+    return rows <= 256 && (dtype == MRL_F32 ? rows <= 32 || groups <= ctx->n_cus || groups * K <= 1 << 18 : K <= 512 && groups * K <= 1 << 18);
 }
 inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
 

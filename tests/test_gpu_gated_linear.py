@@ -122,7 +122,7 @@ def test_forward_and_backward(mrl, ctx, M, K, N, dtype):
 
 # on both sides of what goes straight to registers: long products, wide outputs, 256 rows and one more
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("M,K,N", [(1, 2050, 17), (65, 513, 40), (64, 512, 2064), (127, 1100, 640), (128, 520, 272), (129, 530, 700), (256, 40, 64), (257, 40, 64), (16, 3, 4100)])
+@pytest.mark.parametrize("M,K,N", [(1, 2050, 17), (65, 513, 40), (64, 512, 2064), (127, 1100, 640), (128, 520, 272), (129, 530, 700), (256, 40, 64), (257, 40, 64), (16, 3, 4100), (32, 1040, 4110), (33, 1040, 4110)])
 def test_few_rows_and_tiles(mrl, ctx, M, K, N, dtype):
     print("gated linear", M, K, N, dtype, flush=True)
     c = Case(M, K, N, "silu", dtype, wide=M % 2 == 1)
