@@ -121,9 +121,9 @@ def _registers(text):
     return found
 
 
-def early_reads(lines):
-    """(products, faults) of a unit's assembly, the lines of it."""
-    kernels, code, products, faults = {}, None, 0, []
+def _kernels(lines):
+    """{kernel: [(instruction, operands) or (label, None)]} of a unit's assembly, the lines of it."""
+    kernels, code = {}, None
     for line in lines:
         label = re.match(r"^(\.LBB\d+_\d+|_Z\w+):", line)
         if label and label[1].startswith("_Z"):
@@ -134,6 +134,12 @@ def early_reads(lines):
             op, _, rest = line.split(";")[0].strip().partition(" ")
             if op and not op.startswith("."):
                 code.append((op, rest.strip()))
+    return kernels
+
+
+def early_reads(lines):
+    """(products, faults) of a unit's assembly, the lines of it."""
+    kernels, products, faults = _kernels(lines), 0, []
     for kernel, code in kernels.items():
         at = {op: i for i, (op, rest) in enumerate(code) if rest is None}
         for i, (op, rest) in enumerate(code):
@@ -190,14 +196,53 @@ def empty_masks(lines):
     return found
 
 
+def stores_around_barriers(lines, name):
+    """{kernel: stores to memory that a loop can come to again without a barrier} of the kernels that have `name` in theirs.  Where a loop
+    hands LDS from one iteration to the next its wavefronts may be one barrier apart, and no more: every way around has one."""
+    found = {}
+    for kernel, code in _kernels(lines).items():
+        if name not in kernel:
+            continue
+        at = {op: i for i, (op, rest) in enumerate(code) if rest is None}
+
+        def behind(i):
+            op, rest = code[i]
+            if rest is None or not op.startswith("s_"):
+                return [i + 1]
+            if op in ("s_barrier", "s_endpgm", "s_setpc_b64"):
+                return []
+            if op == "s_branch":
+                return [at[rest]]
+            return [i + 1, at[rest]] if op.startswith("s_cbranch") else [i + 1]
+        again = []
+        for i, (op, rest) in enumerate(code):
+            if rest is None or not op.startswith(("global_store", "buffer_store", "flat_store")):
+                continue
+            todo, seen = behind(i), set()
+            while todo:
+                j = todo.pop()
+                if j < len(code) and j not in seen:
+                    seen.add(j)
+                    todo += behind(j)
+            if i in seen:
+                again.append(op + " " + rest)
+        found[kernel] = again
+    return found
+
+
+def assembly(unit):
+    """The lines of a unit's assembly."""
+    cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(unit, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, unit), "-o", "-"]
+    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("hipcc failed: " + " ".join(cmd))
+    return proc.stdout.splitlines()
+
+
 def check_matrix_results(jobs=8):
     """Compiles every unit that uses the matrix cores to assembly; {unit: (products, faults, kernels with empty masks)}."""
     def one(unit):
-        cmd = ["hipcc"] + FLAGS + EXTRA_FLAGS.get(unit, []) + ["--cuda-device-only", "-S", os.path.join(CSRC, unit), "-o", "-"]
-        proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, text=True)
-        if proc.returncode != 0:
-            raise RuntimeError("hipcc failed: " + " ".join(cmd))
-        lines = proc.stdout.splitlines()
+        lines = assembly(unit)
         return unit, (*early_reads(lines), empty_masks(lines))
     units = []
     for unit in SOURCES:

@@ -243,24 +243,25 @@ __global__ __launch_bounds__(DK * 4) void parts_kernel(Delta d, Parts parts, con
         }
     };
     ask(0);
-    for (int step = 0; step < parts.count; ++step) {
-        const int part = part_of(step);
-        *reinterpret_cast<f32x4 *>(parts.starts + ((((long)nh * parts.count + part) * tiles + column_tile) * B + i) * 256 + lane * 4) = s;
-        if (step == parts.count - 1) break;
+    const auto put = [&](int step) { *reinterpret_cast<f32x4 *>(parts.starts + ((((long)nh * parts.count + part_of(step)) * tiles + column_tile) * B + i) * 256 + lane * 4) = s; };
+    for (int step = 0; step < parts.count - 1; ++step) {
+        put(step);
         f32x4 after = next, mine[B];
 #pragma unroll
         for (int k = 0; k < B; ++k) mine[k] = m[k];
         ask(step + 1);
-        if (!cuts[part]) {
-            f32x4 (&here)[B][64] = S[step & 1];
-            here[i][lane] = s;
-            __syncthreads();   // (the buffers alternate)
+        const bool goes_on = !cuts[part_of(step)];
+        f32x4 (&here)[B][64] = S[step & 1];
+        if (goes_on) here[i][lane] = s;
+        __syncthreads();   // in every step, also where a cut leaves the buffer as it was: who writes it again is behind the next step's, and all have read it by then
+        if (goes_on) {
 #pragma unroll
             for (int k = 0; k < B; ++k) after = mfma16(mine[k], here[k][lane], after);
             settle(after);
         }
         s = after;
     }
+    put(parts.count - 1);
 }
 
 // Up to here the state's own pass is ahead of the tiles: 4 steps of 2048 environments take 72 us (108 by tiles), 2 of 4096 112 (195); 16 of 1024 take 58 by

@@ -430,3 +430,52 @@ def test_rows_far_apart(mrl, ctx, dtype):
     ctx.synchronize()
     assert torch.equal(step[0], step[1]) and all(torch.equal(a, b) for a, b in zip(near_grads, far[6:11]))
     assert torch.equal(near_out[:138], far[5][:138])
+
+
+# ---- parts with and without cuts
+def parts_of(T, N, heads, dk, dv):
+    """steps of a part of a long rollout, and the number of parts (parts_of in delta.hpp)"""
+    block = 32 if dk > 32 else 64
+    blocks = -(-T // block)
+    groups = N * heads * ((-(-dv // 16) + 7) // 8)
+    want = min(blocks, 2 * torch.cuda.get_device_properties(0).multi_processor_count // groups, int((20.0 * blocks) ** 0.5), 1024)
+    per = -(-blocks // want)
+    return per * block, -(-blocks // per)
+
+
+# by part: whether a cut is ahead of one of its steps (the first, the last, or both)
+PATTERNS = {"every second": ".x" * 16, "and the others": "x." * 16, "two without around one": "..x" * 11, "two with around one": "xx." * 11, "once": ".........x......", "none": "." * 16}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pattern,where", [(p, w) for p in PATTERNS for w in ("first", "last", "both") if p != "none" or w == "first"])
+@pytest.mark.parametrize("T,N,heads,key_heads,dk,dv", [(700, 1, 1, 1, 12, 20), (1020, 2, 2, 1, 24, 40), (630, 1, 2, 2, 60, 33), (610, 2, 1, 1, 128, 24)])
+def test_parts_with_and_without_cuts(mrl, ctx, T, N, heads, key_heads, dk, dv, pattern, where, dtype):
+    """What goes from part to part, where some of them have cuts, against 64 bits: outputs, last states and gradients."""
+    steps, count = parts_of(T, N, heads, dk, dv)
+    assert count >= 8
+    print("delta parts", T, N, heads, key_heads, dk, dv, pattern, where, dtype, steps, count, flush=True)
+    c = Case(T, N, heads, key_heads, dk, dv, dtype, rate=0.0, seed=12)
+    # memories of some tens of steps, as the bounds take them, in every head: what a part leaves reaches the parts behind it
+    c.rows[3].copy_(torch.randn(c.rows[3].shape, generator=torch.Generator().manual_seed(T)) + 4)
+    flags = torch.zeros(T + 1, N)
+    for part in range(count):
+        begin, end = part * steps, min(T, (part + 1) * steps)
+        if PATTERNS[pattern][part % len(PATTERNS[pattern])] == "x":
+            for at in {"first": [begin], "last": [end - 1], "both": [begin, end - 1]}[where]:
+                flags[at] = 1.0
+    c.prev, c.dones, c.cut = flags[0].cuda(), flags[1:].contiguous().cuda(), flags[:-1] > 0.5
+    out, last = c.forward(mrl, ctx)
+    got = c.backward(mrl, ctx)
+    ctx.synchronize()
+    want, want_last = c.forward64()
+    near(out, want, heads, FORWARD, HALF[dtype], "out")
+    near(last, want_last, heads, FORWARD, UNIT, "state_out")
+    wants, terms = c.backward64()
+    for name, x, y in zip((*c.NAMES, "state"), got, wants):
+        near(x, y, key_heads if name in ("query", "key") else heads, BACKWARD, UNIT if name == "state" else HALF[dtype], "grad_" + name, terms.get(name))
+    for _ in range(3):   # nor does it depend on which wavefront is ahead
+        again, again_last = c.forward(mrl, ctx)
+        more = c.backward(mrl, ctx)
+        ctx.synchronize()
+        assert torch.equal(out, again) and torch.equal(last, again_last) and all(torch.equal(x, y) for x, y in zip(got, more))
