@@ -6,8 +6,8 @@
 // read, more time than the products take.
 //
 // Products run on the bf16 matrix cores with fp32 sums.  bf16 values are operands as they are.  An fp32 value is three bf16 pieces
-// (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup] goes into dx as one piece, like any bf16
-// activation between two products (rounding it costs dx what rounding dx costs), and into dW, which is fp32, as three, or two (column_pieces).
+// (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup], which is never rounded to
+// bf16, goes into dx as two (16 bits: 2^-17 of a term, where storing dx costs 2^-9 of it) and into dW, which is fp32, as three, or two (column_pieces).
 //
 // Operands lie in the workspace as fragments: 16 rows and 32 of the contracted index, a KiB in the order in which the 64 lanes of
 // v_mfma_f32_16x16x32_bf16 hold them (lane 16 g + n: row n, elements 8 g .. 8 g + 7), the pieces of a fragment next to each other, all rows'
@@ -592,8 +592,11 @@ int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S
 
 // 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.  256 -> 683, the gradient: 512 rows in fp32 take 53 us with small
 // tiles and 89 with large ones, 32768 rows 688 and 607; in bf16 33 and 59, 298 and 252.
+// Two pieces for dx cost 16384 rows of 512 -> 1024 35 us of 255 (tiles of 128 x 128: 48).
 typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
 typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
+typedef Shape<2, 1, 2, 4, 4, 4, 3> Bf16X;            // dx: 128 x 256, two pieces of [dgate | dup]
+typedef Shape<2, 1, 4, 1, 1, 4, 4> Bf16XSmall;       // and 64 x 64
 typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16ManyRows;     // dW: 128 x 128, two pieces of [dgate | dup]
 typedef Shape<1, 3, 2, 4, 4, 2, 4> Bf16FewRows;      // and three
 typedef Shape<3, 3, 2, 4, 4, 2, 3> F32Shape;
@@ -613,7 +616,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
     p.N16 = (N + 15) / 16;
     const bool f32 = dtype == MRL_F32;
     p.pieces = f32 ? 3 : 1;
-    p.row_pieces = f32 ? 3 : 1;
+    p.row_pieces = f32 ? 3 : 2;
     p.column_pieces = column_pieces(dtype, M);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -637,7 +640,7 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
         if (p.parts > 1) p.partial = take(sizeof(float) * (size_t)p.parts * K * 2 * N);
         // so are dx's where there are few rows: 2048 rows of 256 -> 683 in fp32 take 62 us, 69 whole; 512 rows 45 and 55, in bf16 34 and 36
-        const int large = f32 ? tiles<F32Shape>(p.M16, p.K16) : tiles<Bf16Shape>(p.M16, p.K16), small = f32 ? tiles<F32Small>(p.M16, p.K16) : tiles<Bf16Small>(p.M16, p.K16);
+        const int large = f32 ? tiles<F32Shape>(p.M16, p.K16) : tiles<Bf16X>(p.M16, p.K16), small = f32 ? tiles<F32Small>(p.M16, p.K16) : tiles<Bf16XSmall>(p.M16, p.K16);
         p.x_parts = large >= ctx->n_cus ? 1 : std::max(1, std::min(p.N16 / X_STAGES, ctx->n_cus / small));
         if (p.x_parts > 1) p.x_partial = take(sizeof(float) * (size_t)p.x_parts * M * K);
     }
@@ -663,13 +666,15 @@ struct Launch {
         hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
     }
     static int sum_rows(const Plan &p) { return tiles_in<S>(p.M16, 1, 1).down * S::WR; }
-    static void grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w, float *partial) {
-        const Tiles t = tiles_in<S>(p.M16, p.K16, p.N16, p.x_parts);
-        hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t, partial);
-    }
 };
 
-template <class E, class S, class SMALL, class SW, int P, int PR, int PC>
+template <class E, class S>
+void launch_grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &pre, const Operand &w, float *partial) {
+    const Tiles t = tiles_in<S>(p.M16, p.K16, p.N16, p.x_parts);
+    hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t, partial);
+}
+
+template <class E, class S, class SMALL, class SX, class SXSMALL, class SW, int P, int PR, int PC>
 void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool backward) {
     typedef Launch<E, S, P, PR, PC> Large;
     typedef Launch<E, SMALL, P, PR, PC> Small;
@@ -688,8 +693,7 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     o.end[2] = o.end[1] + (backward ? column_blocks(p.K16, p.M16 / 2) : 0);
     o.end[3] = o.end[2] + (backward && y.grad_x ? row_blocks(p.K16, p.N16) : 0);
     hipLaunchKernelGGL((operands_kernel<E, P>), dim3(o.end[3]), dim3(256), 0, ctx->stream, o);
-    const auto small = [&](long a, long b) { return tiles<S>(a, b) < ctx->n_cus; };
-    const bool pre_small = small(p.M16, 2L * p.N16);
+    const bool pre_small = tiles<S>(p.M16, 2L * p.N16) < ctx->n_cus;
     if (!backward) {
         if (pre_small) Small::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
         else Large::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);
@@ -703,8 +707,8 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     const Operand pre_rows = {rows, p.M16}, pre_columns = {columns, 2 * p.N16}, x_columns = {(const __bf16 *)(ws + p.x_columns), p.K16}, w_rows = {(const __bf16 *)(ws + p.w_rows), p.K16};
     if (y.grad_x != nullptr) {
         float *const partial = p.x_parts > 1 ? (float *)(ws + p.x_partial) : nullptr;
-        if (small(p.M16, p.K16)) Small::grad_x(ctx, y, p, pre_rows, w_rows, partial);
-        else Large::grad_x(ctx, y, p, pre_rows, w_rows, partial);
+        if (tiles<SX>(p.M16, p.K16) < ctx->n_cus) launch_grad_x<E, SXSMALL>(ctx, y, p, pre_rows, w_rows, partial);
+        else launch_grad_x<E, SX>(ctx, y, p, pre_rows, w_rows, partial);
     }
     const Tiles t = tiles_in<SW>(p.K16, 2L * p.N16, p.M16 / 2, p.parts);
     const long values = (long)y.K * 2 * y.N;
@@ -771,8 +775,8 @@ int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_
         const dim3 grid((out_dim + 15) / 16, (rows + 15) / 16);
         if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
         else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
-    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16FewRows, 1, 1, 3>(ctx, y, p, (char *)workspace, false);
+    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16FewRows, 1, 2, 3>(ctx, y, p, (char *)workspace, false);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -805,9 +809,9 @@ int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in
     y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
     y.x = in; y.x_ld = in_ld; y.params = params; y.grad_out = grad_out; y.grad_out_ld = grad_out_ld;
     y.grad_x = grad_in; y.grad_x_ld = grad_in_ld; y.grads = grads;
-    if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
-    else if (p.column_pieces == 3) launch<bf16_t, Bf16Shape, Bf16Small, Bf16FewRows, 1, 1, 3>(ctx, y, p, (char *)workspace, true);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16ManyRows, 1, 1, 2>(ctx, y, p, (char *)workspace, true);
+    if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
+    else if (p.column_pieces == 3) launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16FewRows, 1, 2, 3>(ctx, y, p, (char *)workspace, true);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16ManyRows, 1, 2, 2>(ctx, y, p, (char *)workspace, true);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }

@@ -8,7 +8,8 @@ two inputs to a product; the names follow its `Model` trait (deep_rl/model/model
 Parameters are laid out like those of a Linear(in_dim, 2 * out_dim), [W (in x 2 out, row-major) | b], the gate's columns first, so that
 initialisers and optimisers (Adam, and Muon for a model of that Linear) serve as they are.  Rows are [rows, dim] tensors, float32 or bfloat16,
 elements of a row next to each other and rows at any equal distance; params have the rows' type (in bfloat16 a copy of the parameters that
-the optimiser keeps), gradients of parameters are float32.
+the optimiser keeps), gradients of parameters are float32.  In bfloat16 sums are float32 and rounded where they are stored; the gradients of
+gate and up, which are not stored, go into that of the input with 16 bits.
 """
 import ctypes as C
 

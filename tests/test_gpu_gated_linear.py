@@ -270,3 +270,21 @@ def test_pieces_of_the_parameters_gradient(mrl, ctx, M):
     rows = math.sqrt(6 * M / 32)
     bound = (2.0 ** -22 + 24 * UNIT + rows * UNIT) if M < 1 << 14 else 2.0 ** -16 + 24 * UNIT + rows * UNIT
     assert (grads.cpu().double() - want).norm() <= bound * want.norm()
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 24, 20), (300, 96, 130), (2050, 72, 36), (513, 520, 272), (4200, 1030, 520)])
+def test_grad_input_in_bf16_is_rounded_once(mrl, ctx, M, K, N):
+    """Its terms have 16 bits: beside storing's half step of the value there is 2^-17 of each term, which a sum that cancels shows, and no 2^-8."""
+    c = Case(M, K, N, "silu", "bf16", seed=12)
+    gx, _ = c.backward(mrl, ctx)
+    ctx.synchronize()
+    x, w, grad, pre, off = c.parts64()
+    g, u = pre[:, :N], pre[:, N:]
+    s = torch.sigmoid(g)
+    slope = s * (1 + g * (1 - s))
+    d = torch.cat((grad * u * slope, grad * g * s), 1)
+    few = 24 * UNIT * (1 + g.abs().clamp(max=8))
+    og, ou = off[:, :N], off[:, N:]
+    od = torch.cat((grad.abs() * (ou * (slope.abs() + few) + u.abs() * (og + few)), grad.abs() * (1.13 * og + few)), 1)
+    want = d @ w.T
+    near(gx, want, (od + (2.0 ** -17 + ROUNDINGS(2 * N)) * d.abs()) @ w.abs().T + HALF["bf16"] * want.abs() + 1e-37, "grad_x")
