@@ -7,7 +7,7 @@
 //
 // Products run on the bf16 matrix cores with fp32 sums.  bf16 values are operands as they are.  An fp32 value is three bf16 pieces
 // (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup], which is never rounded to
-// bf16, goes into dx as two (16 bits: 2^-17 of a term, where storing dx costs 2^-9 of it) and into dW, which is fp32, as three, or two (column_pieces).
+// bf16, goes into dx as two (16 bits: 2^-17 of a term, where storing dx costs 2^-9 of it) and into dW, which is fp32, as three.
 //
 // Operands lie in the workspace as fragments: 16 rows and 32 of the contracted index, a KiB in the order in which the 64 lanes of
 // v_mfma_f32_16x16x32_bf16 hold them (lane 16 g + n: row n, elements 8 g .. 8 g + 7), the pieces of a fragment next to each other, all rows'
@@ -349,9 +349,14 @@ struct Layer {
     float *grads;
 };
 
+// Pieces of [dgate | dup].  For dW three, 22 bits and more, as fp32 has them: in bf16 two (16 bits) would be 2.5e-6 off in the 2-norm, where fp32 sums of
+// products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7, 2e-7 and 5e-7.  16384 rows of
+// 512 -> 1024 take 292 us, with two 254; 2048 of 256 -> 683 40 and 38.
+constexpr int COLUMN_PIECES = 3;
+
 // FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
-// (PC pieces, for dW), and the sums of its columns over the wavefront's rows.
-template <class E, class S, bool FORWARD, bool AS_IS, int PR, int PC>
+// (COLUMN_PIECES, for dW), and the sums of its columns over the wavefront's rows.
+template <class E, class S, bool FORWARD, bool AS_IS, int PR>
 __global__ __launch_bounds__(S::THREADS) void pre_kernel(Layer y, Operand a, Operand b, Tiles all, __bf16 *rows, __bf16 *columns, float *sums) {
     extern __shared__ __bf16 lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC, wc = wave % S::WC, g = lane >> 4, c = lane & 15;
@@ -395,9 +400,9 @@ __global__ __launch_bounds__(S::THREADS) void pre_kernel(Layer y, Operand a, Ope
                 const auto put = [&](const f32x4 v, int f) {
                     bf16x4 p[SPLIT];
                     split4(v, p);
-                    __bf16 *to = columns + ((long)(fragment >> 1) * fragments + f) * PC * KIB + (16 * ((fragment & 1) * 2 + (g >> 1)) + c) * 8 + (g & 1) * 4;
+                    __bf16 *to = columns + ((long)(fragment >> 1) * fragments + f) * COLUMN_PIECES * KIB + (16 * ((fragment & 1) * 2 + (g >> 1)) + c) * 8 + (g & 1) * 4;
 #pragma unroll
-                    for (int k = 0; k < PC; ++k) *reinterpret_cast<bf16x4 *>(to + k * KIB) = p[k];
+                    for (int k = 0; k < COLUMN_PIECES; ++k) *reinterpret_cast<bf16x4 *>(to + k * KIB) = p[k];
                     // by rows: a fragment of 16 rows and 32 columns, 16 of the gate and 16 of up
                     __bf16 *at = rows + ((long)(f >> 1) * a.fragments + fragment) * PR * KIB + (16 * ((f & 1) * 2 + (c >> 3)) + 4 * g + (c & 3)) * 8 + (c & 4);
 #pragma unroll
@@ -584,7 +589,7 @@ inline long up_to(long n, long unit) { return (n + unit - 1) / unit * unit; }
 // Where things lie in the workspace, in bytes.
 struct Plan {
     int M16, K16, N16;   // fragments of the rows, of the matrix' rows and (pairs) of its columns, an even number of the first two
-    int pieces, row_pieces, column_pieces, parts, x_parts;
+    int pieces, row_pieces, parts, x_parts;
     size_t x_rows, w_columns, x_columns, w_rows, pre_rows, pre_columns, sums, partial, x_partial, bytes;
 };
 template <class S>
@@ -592,22 +597,16 @@ int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S
 
 // 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.  256 -> 683, the gradient: 512 rows in fp32 take 53 us with small
 // tiles and 89 with large ones, 32768 rows 688 and 607; in bf16 33 and 59, 298 and 252.
-// Two pieces for dx cost 16384 rows of 512 -> 1024 35 us of 255 (tiles of 128 x 128: 48).
+// Two pieces for dx cost 16384 rows of 512 -> 1024 35 us (tiles of 128 x 128: 48).
 typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
 typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
 typedef Shape<2, 1, 2, 4, 4, 4, 3> Bf16X;            // dx: 128 x 256, two pieces of [dgate | dup]
 typedef Shape<2, 1, 4, 1, 1, 4, 4> Bf16XSmall;       // and 64 x 64
-typedef Shape<1, 2, 2, 4, 4, 2, 4> Bf16ManyRows;     // dW: 128 x 128, two pieces of [dgate | dup]
-typedef Shape<1, 3, 2, 4, 4, 2, 4> Bf16FewRows;      // and three
+typedef Shape<1, 3, 2, 4, 4, 2, 4> Bf16W;            // dW: 128 x 128, three pieces of [dgate | dup]
 typedef Shape<3, 3, 2, 4, 4, 2, 3> F32Shape;
 typedef Shape<3, 3, 4, 2, 1, 2, 3> F32Small;
 constexpr int WR_MOST = 4;
 constexpr int X_STAGES = 8;   // of 32 of the contracted index, for a part of dx at least
-
-// The pieces of [dgate | dup] for dW: 22 bits and more.  In bf16, whose other factor is one piece, two (16 bits) from 2^14 rows on: they are 2.5e-6 off
-// in the 2-norm, while fp32 sums of products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7,
-// 2e-7 and 5e-7.  16384 rows of 512 -> 1024 take 217 us with two and 258 with three, 2048 of 256 -> 683 40 and 42.
-inline int column_pieces(int dtype, int M) { return dtype == MRL_F32 || M < 1 << 14 ? 3 : 2; }
 
 Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) {
     Plan p = {};
@@ -617,7 +616,6 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
     const bool f32 = dtype == MRL_F32;
     p.pieces = f32 ? 3 : 1;
     p.row_pieces = f32 ? 3 : 2;
-    p.column_pieces = column_pieces(dtype, M);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         const size_t was = at;
@@ -632,9 +630,9 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.x_columns = fragments(p.K16, p.M16, p.pieces);
         p.w_rows = fragments(p.K16, 2L * p.N16, p.pieces);
         p.pre_rows = fragments(p.M16, 2L * p.N16, p.row_pieces);
-        p.pre_columns = fragments(2L * p.N16, p.M16, p.column_pieces);
+        p.pre_columns = fragments(2L * p.N16, p.M16, COLUMN_PIECES);
         p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
-        const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16ManyRows>(p.K16, 2L * p.N16);
+        const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16W>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
         // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 62 us, 116 with whole columns; 32768 rows 607 and 1474
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
@@ -650,20 +648,20 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
 
 template <class S>
 Tiles tiles_in(long a, long b, int blocks, int parts = 1) { return {(int)((a + S::ROWS - 1) / S::ROWS), (int)((b + S::COLUMNS - 1) / S::COLUMNS), parts, blocks}; }
-template <class E, class S, int P, int PR, int PC>
+template <class E, class S, int P, int PR>
 struct Launch {
     template <bool FORWARD>
     static void pre(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Operand &x, const Operand &w, bool as_is, __bf16 *rows = nullptr, __bf16 *columns = nullptr,
                     float *sums = nullptr) {
-        constexpr int ROW_PIECES = FORWARD ? 1 : PR, COLUMN_PIECES = FORWARD ? 1 : PC;   // (not written forwards)
+        constexpr int ROW_PIECES = FORWARD ? 1 : PR;   // (not written forwards)
         const Tiles t = tiles_in<S>(p.M16, 2L * p.N16, p.K16 / 2);
         if constexpr (P == 1) {
             if (as_is) {
-                hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, true, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
+                hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, true, ROW_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
                 return;
             }
         }
-        hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, ROW_PIECES, COLUMN_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
+        hipLaunchKernelGGL((pre_kernel<E, S, FORWARD, false, ROW_PIECES>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, x, w, t, rows, columns, sums);
     }
     static int sum_rows(const Plan &p) { return tiles_in<S>(p.M16, 1, 1).down * S::WR; }
 };
@@ -674,10 +672,10 @@ void launch_grad_x(const mrl_ctx *ctx, const Layer &y, const Plan &p, const Oper
     hipLaunchKernelGGL((grad_x_kernel<E, S>), dim3(t.count()), dim3(S::THREADS), S::LDS, ctx->stream, y, pre, w, t, partial);
 }
 
-template <class E, class S, class SMALL, class SX, class SXSMALL, class SW, int P, int PR, int PC>
+template <class E, class S, class SMALL, class SX, class SXSMALL, class SW, int P, int PR>
 void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool backward) {
-    typedef Launch<E, S, P, PR, PC> Large;
-    typedef Launch<E, SMALL, P, PR, PC> Small;
+    typedef Launch<E, S, P, PR> Large;
+    typedef Launch<E, SMALL, P, PR> Small;
     const bool as_is = P == 1 && y.K % 32 == 0 && y.x_ld % 8 == 0 && reinterpret_cast<uintptr_t>(y.x) % 16 == 0;
     const Operand x_rows = {as_is ? (const __bf16 *)y.x : (const __bf16 *)(ws + p.x_rows), p.M16, y.M, y.x_ld}, w_columns = {(const __bf16 *)(ws + p.w_columns), 2 * p.N16};
     Operands o = {};
@@ -775,8 +773,8 @@ int mrl_gated_linear_forward(mrl_ctx *ctx, int dtype, int act, int rows, int in_
         const dim3 grid((out_dim + 15) / 16, (rows + 15) / 16);
         if (dtype == MRL_F32) hipLaunchKernelGGL(few_rows_kernel<float>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
         else hipLaunchKernelGGL(few_rows_kernel<bf16_t>, grid, dim3(64 * FEW_WAVES), 0, ctx->stream, y);
-    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, false);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16FewRows, 1, 2, 3>(ctx, y, p, (char *)workspace, false);
+    } else if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3>(ctx, y, p, (char *)workspace, false);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16W, 1, 2>(ctx, y, p, (char *)workspace, false);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }
@@ -809,9 +807,8 @@ int mrl_gated_linear_backward(mrl_ctx *ctx, int dtype, int act, int rows, int in
     y.M = rows; y.K = in_dim; y.N = out_dim; y.act = act;
     y.x = in; y.x_ld = in_ld; y.params = params; y.grad_out = grad_out; y.grad_out_ld = grad_out_ld;
     y.grad_x = grad_in; y.grad_x_ld = grad_in_ld; y.grads = grads;
-    if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3, 3>(ctx, y, p, (char *)workspace, true);
-    else if (p.column_pieces == 3) launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16FewRows, 1, 2, 3>(ctx, y, p, (char *)workspace, true);
-    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16ManyRows, 1, 2, 2>(ctx, y, p, (char *)workspace, true);
+    if (dtype == MRL_F32) launch<float, F32Shape, F32Small, F32Shape, F32Small, F32Shape, 3, 3>(ctx, y, p, (char *)workspace, true);
+    else launch<bf16_t, Bf16Shape, Bf16Small, Bf16X, Bf16XSmall, Bf16W, 1, 2>(ctx, y, p, (char *)workspace, true);
     MRL_CHECK_LAUNCH();
     return MRL_OK;
 }

@@ -288,3 +288,19 @@ def test_grad_input_in_bf16_is_rounded_once(mrl, ctx, M, K, N):
     od = torch.cat((grad.abs() * (ou * (slope.abs() + few) + u.abs() * (og + few)), grad.abs() * (1.13 * og + few)), 1)
     want = d @ w.T
     near(gx, want, (od + (2.0 ** -17 + ROUNDINGS(2 * N)) * d.abs()) @ w.abs().T + HALF["bf16"] * want.abs() + 1e-37, "grad_x")
+
+
+@pytest.mark.parametrize("M", [300, 16383, 16384, 40000])
+def test_the_parameters_gradient_has_the_terms_of_fp32(mrl, ctx, M):
+    """Whatever the number of rows.  All but eight rows of the input are zeros, so that the matrix' gradient has eight terms a sum and hardly any
+    roundings but those of the terms: 2^-22 for the pieces, 24 units for the activation's value and slope, 8 for the sums."""
+    c = Case(M, 24, 20, "silu", "bf16", seed=13)
+    some = torch.randperm(M, generator=torch.Generator().manual_seed(3))[:8]
+    kept = torch.zeros(M, 1, dtype=c.tt)
+    kept[some] = 1
+    c.x.mul_(kept.cuda())
+    _, grads = c.backward(mrl, ctx)
+    ctx.synchronize()
+    _, (want, _) = c.backward64()
+    got, want = grads.cpu().double()[:24 * 40], want[:24 * 40]
+    assert (got - want).norm() <= (2.0 ** -22 + 32 * UNIT) * want.norm()
