@@ -294,6 +294,14 @@ MRL_DEV void activation(int act, float g, float &value, float &slope) {
     }
 }
 
+// sigmoid_pair holds sigmoid(g) from exp(-87) down; what is to have it as a factor (value or slope) goes on to 0 here, so that g sigmoid(g) does for the
+// largest gates.  By four gates and in a branch, which hardly any takes: for every value it costs 32768 rows of 512 -> 2048 in bf16 5 us of 165.
+MRL_DEV void fade(int act, const f32x4 g, f32x4 &x) {
+    if ((act != SIGMOID && act != SILU) || fminf(fminf(g[0], g[1]), fminf(g[2], g[3])) >= -87.0f) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] *= __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g[r] + 87.0f, 0.0f) * 1.44269504f);
+}
+
 // 16 x 16 of a matrix [rows, columns] from a result's registers (row 4 g + r, column c) and into them, 0 where it has none.  bf16 goes by
 // four neighbouring columns of a row, which four lanes turn among them.
 MRL_DEV void store_tile(float *p, long ld, const f32x4 v, int row, int column, int rows, int columns, int g, int c) {
@@ -351,7 +359,7 @@ struct Layer {
 
 // Pieces of [dgate | dup].  For dW three, 22 bits and more, as fp32 has them: in bf16 two (16 bits) would be 2.5e-6 off in the 2-norm, where fp32 sums of
 // products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7, 2e-7 and 5e-7.  16384 rows of
-// 512 -> 1024 take 292 us, with two 254; 2048 of 256 -> 683 40 and 38.
+// 512 -> 1024 take 292 us, with two 254.
 constexpr int COLUMN_PIECES = 3;
 
 // FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
@@ -378,21 +386,32 @@ __global__ __launch_bounds__(S::THREADS) void pre_kernel(Layer y, Operand a, Ope
             const int fragment = bi * S::ROWS + wr * S::FA + i, row = fragment * 16 + 4 * g;
             if (fragment >= a.fragments) continue;
             if constexpr (FORWARD) {
+                const f32x4 gate = acc[i][j] + bg;
                 f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = activation(y.act, acc[i][j][r] + bg) * (acc[i][j + 1][r] + bu);
+                for (int r = 0; r < 4; ++r) v[r] = activation(y.act, gate[r]);
+                fade(y.act, gate, v);
+                v *= acc[i][j + 1] + bu;
                 store_tile((E *)y.out, y.out_ld, v, fragment * 16, pair * 16, y.M, y.N, g, c);
             } else {
-                f32x4 dg, du;
+                f32x4 dg, du, values, slopes;
+                const f32x4 gate = acc[i][j] + bg;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float value, slope;
+                    activation(y.act, gate[r], value, slope);
+                    values[r] = value;
+                    slopes[r] = slope;
+                }
+                fade(y.act, gate, values);
+                fade(y.act, gate, slopes);
                 const f32x4 grads = load_tile((const E *)y.grad_out, y.grad_out_ld, fragment * 16, pair * 16, y.M, y.N, g, c);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const bool inside = there && row + r < y.M;
                     const float grad = grads[r];
-                    float value, slope;
-                    activation(y.act, acc[i][j][r] + bg, value, slope);
-                    dg[r] = inside ? grad * (acc[i][j + 1][r] + bu) * slope : 0.0f;
-                    du[r] = inside ? grad * value : 0.0f;
+                    dg[r] = inside ? grad * (acc[i][j + 1][r] + bu) * slopes[r] : 0.0f;
+                    du[r] = inside ? grad * values[r] : 0.0f;
                     gate_sum += dg[r];
                     up_sum += du[r];
                 }
@@ -562,11 +581,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(Layer y) {
         up += sums[i][1][lane];
     }
     const E *const bias = (const E *)y.params + (long)y.K * 2 * y.N;
-    const float bg = value_of(bias[column]), bu = value_of(bias[y.N + column]);
+    gate += value_of(bias[column]);
+    up += value_of(bias[y.N + column]);
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = activation(y.act, gate[r]);
+    fade(y.act, gate, v);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int at = blockIdx.y * 16 + 4 * g + r;
-        if (at < y.M) give((E *)y.out + at * y.out_ld + column, activation(y.act, gate[r] + bg) * (up[r] + bu));
+        if (at < y.M) give((E *)y.out + at * y.out_ld + column, v[r] * up[r]);
     }
 }
 

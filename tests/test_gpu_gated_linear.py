@@ -304,3 +304,31 @@ def test_the_parameters_gradient_has_the_terms_of_fp32(mrl, ctx, M):
     _, (want, _) = c.backward64()
     got, want = grads.cpu().double()[:24 * 40], want[:24 * 40]
     assert (got - want).norm() <= (2.0 ** -22 + 32 * UNIT) * want.norm()
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M", [3, 300])
+def test_gates_far_below_zero(mrl, ctx, M, dtype, act):
+    """sigmoid(g) and g sigmoid(g) vanish for the largest gates, in value and slope.  16 units of a value, and the steps of 2^-149 in which
+    fp32 goes below 2^-126, up to 110 times.  bf16 goes in steps of 2^-133 there: storing costs half of one, and so do a value's three pieces."""
+    gates = torch.tensor([-3e38, -1e38, -1e30, -1e10, -1000.0, -200.0, -110.0, -100.0, -90.0, -88.0, -87.0, -86.0, -30.0, -1.0, 50.0, 1e4])
+    N = len(gates)
+    params = torch.cat((gates, torch.full((N,), 2.0), torch.zeros(2 * N))).to(TYPES[dtype])
+    x, grad = (torch.ones(M, w, dtype=TYPES[dtype], device="cuda") for w in (1, N))
+    out, gx, grads = torch.full_like(grad, 7.0), torch.full_like(x, 7.0), torch.full((4 * N,), 7.0, device="cuda")
+    layer = mrl.GatedLinear(1, N, act)
+    layer.forward_gpu(ctx, out, x, params.cuda())
+    layer.backward_gpu(ctx, gx, grads, grad, x, params.cuda())
+    ctx.synchronize()
+    g = params[:N].double().requires_grad_()
+    value = act64(act, g)
+    slope, = torch.autograd.grad(value.sum(), g)
+    value = value.detach()
+    off = 16 * UNIT * value.abs() + 110 * 2.0 ** -149
+    assert ((out.cpu().double() - 2 * value).abs() <= 2 * off + HALF[dtype] * 2 * value.abs() + (2.0 ** -134 if dtype == "bf16" else 0.0)).all()
+    got = grads.cpu().double().view(2, 2, N)    # matrix and biases, of gate and up
+    off = 110 * 2.0 ** -149 + 2.0 ** -134
+    steps = (16 + 6 * M) * UNIT                 # a sum over M rows of one value
+    assert ((got[:, 0] - 2 * M * slope).abs() <= 2 * M * (steps * slope.abs() + 16 * UNIT * value.abs() + off)).all()
+    assert ((got[:, 1] - M * value).abs() <= M * (steps * value.abs() + off)).all()
