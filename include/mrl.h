@@ -510,8 +510,8 @@ int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, i
  *     out = act(in Wg + bg) * (in Wu + bu),   act: sigmoid, g sigmoid(g), g Phi(g) (Phi the normal distribution's) or tanh.
  * params are those of a MRL_LINEAR of in_dim -> 2 out_dim, W [in_dim, 2 out_dim] row-major, then the biases: column j of W is Wg's, column
  * out_dim + j Wu's.  in and out have `rows` rows of `dtype`, `ld` elements apart, and params are of `dtype` too (in bf16 a rounded copy of what the
- * optimiser keeps).  Sums are fp32, values are rounded when stored.  An infinity (or
- * a value from 3.39e38 on, bf16's largest) in `in` or params may make NaN of what it reaches where dtype is fp32.
+ * optimiser keeps).  Sums are fp32, values are rounded when stored.  Infinities go
+ * where the formulas send them; where dtype is fp32 sums overflow within 2^-8 of where fp32's do.
  *
  * Backward overwrites grads (fp32, laid out like params, whatever the type) and grad_in (may be NULL) from the gradient of out; it works gate and
  * up out again.  Their gradients are not rounded to bf16 in between: 16 bits of them and more go into grad_in (2^-17 of a term, where storing a sum

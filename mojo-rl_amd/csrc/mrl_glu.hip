@@ -221,6 +221,8 @@ MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int fr
         }
     };
     const int stages = to - from;
+    constexpr bool PIECES = S::PA + S::PB > 2;
+    f32x4 small[PIECES ? S::FA : 1][PIECES ? S::FB : 1] = {};   // all products but those of first pieces, which alone say what an infinity makes (split_sum)
 #pragma unroll
     for (int s = 0; s < S::BUFFERS - 1; ++s)
         if (s < stages) ask(s);
@@ -247,9 +249,20 @@ MRL_DEV void multiply(const Operand &a, const Operand &b, int bi, int bj, int fr
                 for (int p = 0; p <= sum; ++p)
                     if (p < S::PA && sum - p < S::PB) {
 #pragma unroll
-                        for (int j = 0; j < S::FB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[p], y[j][sum - p], acc[i][j], 0, 0, 0);
+                        for (int j = 0; j < S::FB; ++j) {
+                            f32x4 &to = PIECES && sum > 0 ? small[PIECES ? i : 0][PIECES ? j : 0] : acc[i][j];
+                            to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[p], y[j][sum - p], to, 0, 0, 0);
+                        }
                     }
         }
+    }
+    if constexpr (PIECES) {
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = split_sum(acc[i][j][r], small[i][j][r]);
     }
 }
 

@@ -332,3 +332,43 @@ def test_gates_far_below_zero(mrl, ctx, M, dtype, act):
     steps = (16 + 6 * M) * UNIT                 # a sum over M rows of one value
     assert ((got[:, 0] - 2 * M * slope).abs() <= 2 * M * (steps * slope.abs() + 16 * UNIT * value.abs() + off)).all()
     assert ((got[:, 1] - M * value).abs() <= M * (steps * value.abs() + off)).all()
+
+
+def kinds(x):
+    """0 where finite, 1 and -1 infinities, 2 NaN"""
+    return torch.where(torch.isnan(x), 2.0, torch.where(torch.isinf(x), torch.sign(x), torch.zeros_like(x)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("act", ACTIVATIONS)
+@pytest.mark.parametrize("M", [5, 40, 300, 1100])
+def test_infinities_are_what_the_formulas_make_of_them(mrl, ctx, M, act, dtype):
+    """Whatever the number of rows: infinities in the input, in the matrix' gate and up columns, and in the gradient of the output; and an input
+    that is finite and rounds past bf16's largest value."""
+    K, N = 70, 50
+    for where in ("input", "gate", "up", "grad", "largest"):
+        c = Case(M, K, N, act, dtype, seed=21)
+        if where == "input":
+            c.x[2, 3], c.x[4, 69] = float("inf"), -float("inf")
+        elif where == "largest":
+            c.x[2, 3] = torch.finfo(c.tt).max        # 2^128, times weights and gradients with which all stays far from overflowing
+            c.params[3 * 2 * N:4 * 2 * N] = 2.0 ** -120
+            c.grad[2] *= 2.0 ** -20
+        elif where == "grad":
+            c.grad[1, 7], c.grad[3, 49] = float("inf"), -float("inf")
+        else:
+            c.params[5 * 2 * N + (0 if where == "gate" else N) + 11] = float("inf")
+        out = c.forward(mrl, ctx)
+        gx, grads = c.backward(mrl, ctx)
+        ctx.synchronize()
+        x, p, grad = c.x.cpu().double(), c.params.cpu().double(), c.grad.cpu().double()
+        w = p[:K * 2 * N].view(K, 2 * N)
+        pre = x @ w + p[K * 2 * N:]
+        g = pre[:, :N].clone().requires_grad_()
+        a = act64(act, g)
+        slope, = torch.autograd.grad(a.sum(), g)
+        d = torch.cat((grad * pre[:, N:] * slope, grad * a.detach()), 1)
+        want_grads = torch.cat(((x.T @ d).reshape(-1), d.sum(0)))
+        for got, want, what in ((out, a.detach() * pre[:, N:], "out"), (gx, d @ w.T, "grad_x"), (grads, want_grads, "grads")):
+            want = kinds(want.to(got.dtype).double())
+            assert torch.equal(kinds(got.cpu().double()).reshape(want.shape), want), (where, what)
