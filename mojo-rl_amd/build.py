@@ -110,14 +110,14 @@ def check_lane_masks(jobs=8):
 # A product's registers may be read some instructions behind it; the hardware does not wait for them, the compiler counts.  Behind
 # a taken branch this compiler has been seen to count too few, down to one, and the reader took what had stood there before.
 _STATES = (("16x16x32", 8), ("16x16x16", 8), ("16x16x4_f32", 10), ("32x32", 18))   # what it leaves within a block
-_REGISTERS = re.compile(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b")
+_REGISTERS = re.compile(r"\b([va])\[(\d+):(\d+)\]|\b([va])(\d+)\b")
 _WRITES_MEMORY = re.compile(r"^(ds_write|(global|buffer|flat|scratch)_(store|atomic))")
 
 
 def _registers(text):
     found = set()
-    for first, last, alone in _REGISTERS.findall(text):
-        found |= {int(alone)} if alone else set(range(int(first), int(last) + 1))
+    for kind, first, last, other, alone in _REGISTERS.findall(text):
+        found |= {other + alone} if alone else {kind + str(i) for i in range(int(first), int(last) + 1)}
     return found
 
 

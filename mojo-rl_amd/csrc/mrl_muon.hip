@@ -401,7 +401,11 @@ MRL_DEV void small_product(const Group &g, const Mat &m, int bi, int bj, int fro
     auto work = [&](const Operands &o) {
         if (few) {
             multiply_few(o.ph[0], o.pl[0], o.qh[0], o.ql[0], acc[0][0]);
-            if (STAGE == UPDATE) multiply_few(o.ph[0], o.pl[0], o.qh[1], o.ql[1], acc[0][1]);
+            if (STAGE == UPDATE) {
+                multiply_few(o.ph[0], o.pl[0], o.qh[1], o.ql[1], acc[0][1]);
+                // the compiler has been seen to read these 8 instructions later where blocks join, not the 10 that it leaves within one
+                asm volatile("s_nop 9" : "+v"(acc[0][0]), "+v"(acc[0][1]));
+            }
             return;
         }
         multiply<2>(o.pl, o.qh, acc);

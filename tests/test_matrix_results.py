@@ -38,6 +38,13 @@ def test_a_product_of_a_result_and_a_store_are_reads():
         assert len(build.early_reads(EARLY.replace("v_mul_f32_e32 v6, v1, v5", reader).splitlines())[1]) == 1
 
 
+def test_accumulation_registers_are_registers_of_their_own():
+    apart = EARLY.replace("v_mfma_f32_16x16x4_f32 v[0:3], v8, v9, v[0:3]", "v_mfma_f32_16x16x4_f32 a[0:3], v8, v9, a[0:3]")
+    assert build.early_reads(apart.splitlines()) == (1, [])
+    faults = build.early_reads(apart.replace("v_mul_f32_e32 v6, v1, v5", "v_accvgpr_read_b32 v6, a1").splitlines())[1]
+    assert len(faults) == 1 and faults[0][2].startswith("v_accvgpr_read_b32 v6, a1") and faults[0][3] == 1
+
+
 def test_an_empty_mask_is_found():
     kept = "_Zkernel:\n\ts_and_saveexec_b64 s[10:11], s[6:7]\n\tv_mov_b32_e32 v17, v0\n\ts_or_b64 exec, exec, s[10:11]\n"
     assert build.empty_masks(kept.splitlines()) == []
