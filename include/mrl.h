@@ -478,6 +478,7 @@ int mrl_recurrence_backward(mrl_ctx *ctx, int dtype, int T, int N, int D, const 
  * uses the query and key of key head h / (heads / key_heads).  Rows, `ld`, dones, prev_dones and cuts are those of the recurrent layer
  * above: a row of query and key has key_heads * key_dim elements, of value and out heads * value_dim, of gate and rate `heads`;
  * where a step before ended an episode S[t-1] counts as 0, and what a cut hides, infinities and NaN included, reaches nothing behind it.
+ * Keys and queries may have any finite length; sums of values and states overflow within 2^5 of where fp32's do.
  * States are fp32 [N, heads, key_dim, value_dim]; state_in NULL is zeros; state_out = S[T-1], may be NULL, and may be state_in.
  * T = 1 is a step of a collection loop.  Dims are 1 to 128, N * heads is below 2^22, T below 2^30.  Sums and states are fp32, bf16 is rounded
  * when stored.

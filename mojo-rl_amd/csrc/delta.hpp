@@ -36,7 +36,10 @@ struct bf16_t { unsigned short bits; };
 constexpr int TILE = 16;
 constexpr int MOST_DIM = 128;
 constexpr float EPS = 1e-6f;
-constexpr float LARGE = 1e30f;   // beyond this, or NaN: a value that products with 0 must not meet
+// Beyond these, or NaN: blocks go one step to a tile, so that what overflows or is not finite does not meet the 0 of another step.  Below
+// them no product of states, values and their gradients with each other or with keys and queries comes to 2^127: sums of a block's values and states
+// by lane stay below LARGE, squared lengths below LARGE^2.
+constexpr float LARGE = 1e15f, LARGE_SQUARE = 1e30f;
 
 struct Delta {
     int T, N, H, HK, dk, dv;
@@ -207,6 +210,11 @@ MRL_DEV float one_over_root(float x) {
     const float y = __builtin_amdgcn_rsqf(x);
     return x < 0x1p127f ? fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y) : y;
 }
+
+// The power of two to take out of a key or a query whose largest element is `most`, where products of it as it is may overflow: what is left is shorter
+// than 1, and its length, sqrt(EPS) of it included, no less than 2^-5.  (Products of lengths with it undo it: |k| and EPS are in the same units.)
+MRL_DEV int unit_of(float most) { return most > 0.0f ? max(-6, __builtin_amdgcn_frexp_expf(most) + 4) : -6; }
+MRL_DEV float in_units(float x, int unit) { return __builtin_amdgcn_ldexpf(x, -unit); }
 
 // the sum over the four lane groups, in all of them
 MRL_DEV float sum_groups(float x) {
@@ -392,7 +400,7 @@ struct Rows<bf16_t, DK, STEPS> {
 template <class E>
 constexpr size_t rows_floats(int DK, int tiles, bool keeps) {
     const size_t steps = (size_t)TILE * tiles, rows = sizeof(E) == 4 ? steps * (DK + 4) : (steps * (DK + 8) + DK * (steps + 4)) / 2;
-    return 2 * rows + (keeps ? 3 : 2) * tiles * TILE * SIDE + 13 * steps + 4;
+    return 2 * rows + (keeps ? 3 : 2) * tiles * TILE * SIDE + 15 * steps + 4;
 }
 
 // What the wavefronts of a workgroup keep in LDS of a block's rows, from `lds` on.  KEEPS: A beside its inverse.
@@ -401,8 +409,9 @@ struct Block {
     static constexpr int TILES = TILES_, STEPS = TILE * TILES, LANES = DK / 4;
     Rows<E, DK, STEPS> keys, queries;
     float *As, *Ts, *Ps;
-    // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), the squares of key and query, F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
+    // of every step: a, 1 - a (0 at a cut), b, 1 - b, 1 / |k|, 1 / (|q| sqrt(dk)), the squared lengths of key and query, F, L, b F / |k|, F / (|q| sqrt(dk)), L / |k|; of every tile F[15]
     float *as, *rests, *bs, *rate_rests, *key_lengths, *query_lengths, *kscale, *qscale, *from, *to, *key_reads, *query_reads, *key_takes, *wholes;
+    int *key_units, *query_units;   // where span is 1: the powers of two that the key and the query, and all lengths of them here, are without
     int t0, span;   // the first step; steps of a tile: 1 where a value is not finite, so that it goes where the formulas send it and nowhere else
     MRL_DEV explicit Block(float *lds) {
         keys.at = lds;
@@ -423,12 +432,26 @@ struct Block {
         key_reads = to + STEPS;
         query_reads = key_reads + STEPS;
         key_takes = query_reads + STEPS;
-        wholes = key_takes + STEPS;
+        key_units = reinterpret_cast<int *>(key_takes + STEPS);
+        query_units = key_units + STEPS;
+        wholes = key_takes + 3 * STEPS;
     }
     MRL_DEV int time_of(int slot) const { return t0 + (slot >> 4) * span + (slot & 15); }
     MRL_DEV bool there(const Delta &d, int slot) const { return ((slot & 15) < span) & (time_of(slot) < d.T); }
     MRL_DEV bool full(const Delta &d) const { return span == TILE && t0 + STEPS <= d.T; }
     MRL_DEV f32x4 four(const float *scalars, int tile, int g) const { return *reinterpret_cast<const f32x4 *>(scalars + tile * TILE + 4 * g); }
+
+    // a row by LANES lanes of four, and EPS beside its squares, without the row's power of two, which it returns
+    MRL_DEV static int in_row_units(f32x4 &x, float &eps) {
+        float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+        for (int s = 1; s < LANES; s *= 2) most = fmaxf(most, __shfl_xor(most, s));
+        const int unit = unit_of(most);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = in_units(x[j], unit);
+        eps = in_units(EPS, 2 * unit);
+        return unit;
+    }
 
     // Keys, queries (QUERIES), their lengths, gates and rates; rows behind the last step are zeros that change nothing (a = 1, b = 0).
     // Whether a value is too large for products with 0, or none.  All loads are asked for ahead of the first use of any: one wait for them, not
@@ -459,6 +482,14 @@ struct Block {
                     q[j] = here ? q[j] : 0.0f;
                 }
             }
+            float k_eps = EPS, q_eps = EPS;
+            if (span == 1) {
+                const int k_unit = in_row_units(k, k_eps), q_unit = in_row_units(q, q_eps);
+                if (part == 0) {
+                    key_units[slot] = k_unit;
+                    query_units[slot] = q_unit;
+                }
+            }
             keys.put(slot, 4 * part, k);
             const float kk = sum_lanes<LANES>(fmaf(k[0], k[0], fmaf(k[1], k[1], fmaf(k[2], k[2], k[3] * k[3]))));
             float qq = 0.0f;
@@ -466,10 +497,10 @@ struct Block {
                 queries.put(slot, 4 * part, q);
                 qq = sum_lanes<LANES>(fmaf(q[0], q[0], fmaf(q[1], q[1], fmaf(q[2], q[2], q[3] * q[3]))));
             }
-            odd |= !(kk + qq < LARGE);
+            odd |= !(kk + qq < LARGE_SQUARE);
             if (part == 0) {   // (squares for now: prepare() makes lengths of them)
-                kscale[slot] = kk;
-                qscale[slot] = qq;
+                kscale[slot] = kk + k_eps;
+                qscale[slot] = qq + q_eps;
             }
         };
         const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -514,12 +545,12 @@ struct Block {
     template <bool QUERIES>
     MRL_DEV void prepare(const Delta &d, int half, int g, int c) {
         const int tile = half >> 1;
-        const float kc = one_over_root(kscale[tile * TILE + c] + EPS);
+        const float kc = one_over_root(kscale[tile * TILE + c]);
         const f32x4 decay = between(as + tile * TILE, g, c);
         f32x4 products;
         if (half & 1) {
             const int slot = tile * TILE + c;
-            const float qs = one_over_root((qscale[slot] + EPS) * (float)d.dk), a = as[slot], b = bs[slot];
+            const float qs = one_over_root(qscale[slot] * (float)d.dk), a = as[slot], b = bs[slot];
             if (QUERIES) products = queries.with(keys, tile, g, c);
             float ahead = a, behind = moved<0x101>(a, 1.0f);   // products up to here, and of those behind
             ahead *= moved<0x111>(ahead, 1.0f);
@@ -544,7 +575,7 @@ struct Block {
                 const f32x4 squares = four(qscale, tile, g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float qi = one_over_root((squares[r] + EPS) * (float)d.dk);
+                    const float qi = one_over_root(squares[r] * (float)d.dk);
                     Ps[(tile * TILE + 4 * g + r) * SIDE + c] = 4 * g + r >= c ? qi * (kc * products[r]) * decay[r] : 0.0f;
                 }
             }
@@ -554,7 +585,7 @@ struct Block {
             float *A = As + tile * TILE * SIDE;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float ki = one_over_root(squares[r] + EPS);
+                const float ki = one_over_root(squares[r]);
                 A[(4 * g + r) * SIDE + c] = 4 * g + r > c ? b[r] * ki * (kc * products[r]) * decay[r] : 0.0f;
             }
             __builtin_amdgcn_wave_barrier();

@@ -8,7 +8,8 @@ namespace {
 
 // ---------------------------------------------------------------- a few steps
 // A wavefront holds 4 L columns of a head's state in registers: lane l columns 4 (l % L) on, rows l / L, l / L + 64 / L, ..., at most
-// R of them.  S^T k and S^T q are summed in one pass, out = a S^T q + (q k) u follows from them, and the state is read and written once.
+// R of them.  S^T k and S^T q are summed in one pass, out = a S^T q + (q k) u follows from them, and the state is read and written once.  Sums with the
+// key and the query as they come, their lengths afterwards; where one overflows, again with their powers of two taken out first.
 // Bound by that: a step of 8192 environments of 4 heads of 64 x 64 takes 202 us, 5.5 TB/s, what a copy of 256 MiB gets.
 template <class E, int L, int R>
 __global__ __launch_bounds__(256) void steps_kernel(Delta d, int units, int column_blocks) {
@@ -36,37 +37,68 @@ __global__ __launch_bounds__(256) void steps_kernel(Delta d, int units, int colu
         float a, b, rest;
         sigmoid_pair(value_of(((const E *)d.gate)[row * d.gate_ld + h]), a, rest);
         sigmoid_pair(value_of(((const E *)d.rate)[row * d.rate_ld + h]), b, rest);
-        float k[R], q[R], kk = 0.0f, qq = 0.0f, qk = 0.0f;
+        float k[R], q[R], kk, qq, qk, k_eps = EPS, q_eps = EPS;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const bool there = rg + i * G < d.dk;
             k[i] = there ? value_of(k_row[rg + i * G]) : 0.0f;
             q[i] = there ? value_of(q_row[rg + i * G]) : 0.0f;
         }
-        f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 sk, sq;
+        const auto sums = [&]() {
+            kk = qq = qk = 0.0f;
+            sk = sq = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            kk = fmaf(k[i], k[i], kk);
-            qq = fmaf(q[i], q[i], qq);
-            qk = fmaf(q[i], k[i], qk);
+            for (int i = 0; i < R; ++i) {
+                kk = fmaf(k[i], k[i], kk);
+                qq = fmaf(q[i], q[i], qq);
+                qk = fmaf(q[i], k[i], qk);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk[j] = fmaf(k[i], S[i][j], sk[j]);
-                sq[j] = fmaf(q[i], S[i][j], sq[j]);
+                for (int j = 0; j < 4; ++j) {
+                    sk[j] = fmaf(k[i], S[i][j], sk[j]);
+                    sq[j] = fmaf(q[i], S[i][j], sq[j]);
+                }
             }
-        }
 #pragma unroll
-        for (int s = L; s < 64; s *= 2) {
-            kk += __shfl_xor(kk, s);
-            qq += __shfl_xor(qq, s);
-            qk += __shfl_xor(qk, s);
+            for (int s = L; s < 64; s *= 2) {
+                kk += __shfl_xor(kk, s);
+                qq += __shfl_xor(qq, s);
+                qk += __shfl_xor(qk, s);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk[j] += __shfl_xor(sk[j], s);
-                sq[j] += __shfl_xor(sq[j], s);
+                for (int j = 0; j < 4; ++j) {
+                    sk[j] += __shfl_xor(sk[j], s);
+                    sq[j] += __shfl_xor(sq[j], s);
+                }
             }
+        };
+        sums();
+        // 0 where all are finite; where they are not, or no longer, once more without the rows' powers of two
+        float finite = 0.0f * (kk + (qq + q_eps) * (float)d.dk + qk);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) finite = fmaf(0.0f, sk[j], fmaf(0.0f, sq[j], finite));
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(finite != 0.0f) != 0, 0)) {
+            float most_k = 0.0f, most_q = 0.0f;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                most_k = fmaxf(most_k, fabsf(k[i]));
+                most_q = fmaxf(most_q, fabsf(q[i]));
+            }
+#pragma unroll
+            for (int s = L; s < 64; s *= 2) {
+                most_k = fmaxf(most_k, __shfl_xor(most_k, s));
+                most_q = fmaxf(most_q, __shfl_xor(most_q, s));
+            }
+            const int k_unit = unit_of(most_k), q_unit = unit_of(most_q);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                k[i] = in_units(k[i], k_unit);
+                q[i] = in_units(q[i], q_unit);
+            }
+            k_eps = in_units(EPS, 2 * k_unit);
+            q_eps = in_units(EPS, 2 * q_unit);
+            sums();
         }
-        const float ks = one_over_root(kk + EPS), qs = one_over_root((qq + EPS) * (float)d.dk);
+        const float ks = one_over_root(kk + k_eps), qs = one_over_root((qq + q_eps) * (float)d.dk);
         f32x4 u, o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

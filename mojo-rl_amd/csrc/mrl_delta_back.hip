@@ -432,6 +432,13 @@ __global__ __launch_bounds__(64 * MOST_WAVES, 2) void back_kernel(Back p) {
                         q[o][r] = qs[r] * fmaf(-(float)d.dk * q[o][r], q_dot[r], dq[o][r]);
                         k[o][r] = ks[r] * fmaf(-k[o][r], k_dot[r], dk[o][r]);
                     }
+                    if (block.span == 1) {   // lengths are without the rows' powers of two
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            q[o][r] = in_units(q[o][r], block.query_units[tile * TILE + 4 * g + r]);
+                            k[o][r] = in_units(k[o][r], block.key_units[tile * TILE + 4 * g + r]);
+                        }
+                    }
                     store_values(d, block, (EK *)p.query + n * p.query_ld + key_at + at, (long)d.N * p.query_ld, at < d.dk, tile, g, q[o]);
                     store_values(d, block, (EK *)p.key + n * p.key_ld + key_at + at, (long)d.N * p.key_ld, at < d.dk, tile, g, k[o]);
                 }

@@ -479,3 +479,93 @@ def test_parts_with_and_without_cuts(mrl, ctx, T, N, heads, key_heads, dk, dv, p
         more = c.backward(mrl, ctx)
         ctx.synchronize()
         assert torch.equal(out, again) and torch.equal(last, again_last) and all(torch.equal(x, y) for x, y in zip(got, more))
+
+
+# ---- the ends of the range
+def by_episode(c, x):
+    """the parts of [T, N, ...] that cuts separate, by environment"""
+    x = x.reshape(c.T, c.N, *x.shape[1:])
+    for n in range(c.N):
+        starts = [0, *[t for t in range(1, c.T) if c.cut[t, n]], c.T]
+        for first, last in zip(starts, starts[1:]):
+            yield x[first:last, n]
+
+
+def sums_of_terms(c):
+    """What roundings in the gradients of gate and rate are of the size of.  grad_gate = (1 - a) sum_ij S'[i][j] dS'[i][j] is a sum of dk dv terms,
+    grad_rate = (1 - b) sum_j U[j] dX[j] of dv, and either may be far smaller than they are (1280 terms that cancel to a 3000th of their 2-norm
+    in the first step of 600, the only one that meets the first state).  A term is off by its factors' bounds, one term independently of another, so the sum is off
+    by those times the terms' 2-norm.  The terms are the gradients of a gate for every element of the state, and a rate for every column."""
+    heads, key_heads, dk, dv = c.dims
+    T, N = c.T, c.N
+    q, k, v, gate, rate = c.rows64()
+    q, k = (x.reshape(T, N, key_heads, dk) for x in (q, k))
+    q, k = ((x / (x.square().sum(-1, keepdim=True) + EPS).sqrt()).repeat_interleave(heads // key_heads, 2) for x in (q, k))
+    v = v.reshape(T, N, heads, dv)
+    a = torch.sigmoid(gate).reshape(T, N, heads, 1, 1).expand(T, N, heads, dk, dv).clone().requires_grad_()
+    b = torch.sigmoid(rate).reshape(T, N, heads, 1, 1).expand(T, N, heads, 1, dv).clone().requires_grad_()
+    state, loss, weights = c.state64(), 0.0, c.grad_out.cpu().double().reshape(T, N, heads, dv) / dk ** 0.5
+    for t in range(T):
+        state = torch.where(c.cut[t].view(N, 1, 1, 1), torch.zeros_like(state), a[t] * state)
+        state = state + k[t].unsqueeze(3) * (b[t] * (v[t].unsqueeze(2) - k[t].unsqueeze(2) @ state))
+        loss = loss + ((q[t].unsqueeze(2) @ state).squeeze(2) * weights[t]).sum()
+    of_a, of_b = torch.autograd.grad(loss + (state * c.grad_last.cpu().double()).sum(), [a, b])
+    return {name: (p * (1 - p) * g).detach().norm(dim=(3, 4)).reshape(T * N, heads) for name, p, g in (("gate", a, of_a), ("rate", b, of_b))}
+
+
+# (steps: by the state's own pass, within a tile, over tiles, in parts)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,N,heads,key_heads,dk,dv", [(1, 3, 2, 2, 64, 64), (4, 2, 2, 1, 40, 24), (3, 1, 1, 1, 128, 100), (30, 2, 2, 1, 24, 40), (70, 2, 1, 1, 128, 64), (45, 2, 2, 2, 9, 5), (600, 1, 1, 1, 64, 20)])
+@pytest.mark.parametrize("keys,queries,states", [(1e12, 1.0, 1e29), (1.0, 5e17, 1.0), (1e25, 1e25, 1.0), (1e19, 1e-3, 1e30), (1e-12, 1e-12, 1e33), (3e36, 3e36, 1e-20), (1.0, 1.0, 1e35)])
+def test_sizes_of_keys_queries_and_states(mrl, ctx, T, N, heads, key_heads, dk, dv, keys, queries, states, dtype):
+    """A key's and a query's length go out of the results, so that their products with a state are of the state's size; and what large ones make
+    of the steps ahead of a cut does not reach those behind it.  Against 64 bits, episode by episode."""
+    print("delta range", T, N, heads, key_heads, dk, dv, keys, queries, states, dtype, flush=True)
+    c = Case(T, N, heads, key_heads, dk, dv, dtype, rate=0.0, seed=14)
+    if T > 4:   # in the middle of a tile
+        c.dones[T // 2 - 1] = 1.0
+        c.cut = torch.cat((c.prev[None], c.dones[:-1])).cpu() > 0.5
+    c.rows[0].mul_(queries)
+    c.rows[1].mul_(keys)
+    c.state.mul_(states)
+    out, last = c.forward(mrl, ctx)
+    got = c.backward(mrl, ctx)
+    ctx.synchronize()
+    want, want_last = c.forward64()
+    near(last, want_last, heads, FORWARD, UNIT, "state_out")
+    for x, y in zip(by_episode(c, out.cpu().double()), by_episode(c, want)):
+        near(x, y, heads, FORWARD, HALF[dtype], "out")
+    wants, terms = c.backward64()
+    terms.update(sums_of_terms(c))
+    for name, x, y in zip((*c.NAMES, "state"), got, wants):
+        if name == "state":
+            near(x, y, heads, BACKWARD, UNIT, "grad_state")
+            continue
+        size = torch.maximum(terms.get(name, y).detach().abs(), y.detach().abs())
+        for a, b, s in zip(by_episode(c, x.cpu().double()), by_episode(c, y), by_episode(c, size)):
+            near(a, b, key_heads if name in ("query", "key") else heads, BACKWARD, HALF[dtype], "grad_" + name, s)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_cut_within_a_tile_of_large_products(mrl, ctx, dtype):
+    """A state, keys, values and output gradients whose products with each other pass fp32's end, in the steps ahead of a cut: those behind it
+    come out as they do without them."""
+    T, N, heads, dk, dv = 90, 2, 2, 24, 20
+
+    def case():
+        c = Case(T, N, heads, heads, dk, dv, dtype, rate=0.0, seed=15)
+        c.dones[40] = 1.0
+        c.cut = torch.cat((c.prev[None], c.dones[:-1])).cpu() > 0.5
+        return c
+    clean, bad = case(), case()
+    rows = slice(36 * N, 41 * N)
+    bad.state.mul_(1e28)
+    for which, by in ((0, 1e15), (1, 1e14), (2, 1e25)):
+        bad.rows[which][rows] *= by
+    bad.grad_out[rows] *= 1e27
+    results = [(*c.forward(mrl, ctx), *c.backward(mrl, ctx)) for c in (clean, bad)]
+    ctx.synchronize()
+    for x, y in zip(results[1][:1] + results[1][2:7], results[0][:1] + results[0][2:7]):
+        x, y = x.cpu().double()[41 * N:], y.cpu().double()[41 * N:]
+        assert torch.isfinite(x).all() and ((x - y).abs() <= 2 * BACKWARD * y.abs().max() + 2 * HALF[dtype] * y.abs()).all()
+    assert (results[1][1].cpu().double() - results[0][1].cpu().double()).abs().max() <= 2 * FORWARD * results[0][1].abs().max().item()
