@@ -113,17 +113,19 @@ MRL_DEV void along_columns(const Source &s, __bf16 *to, int column_fragments, lo
     for (int i = 0; i < 8; ++i) x[i] = tile[w * 16 + (lane & 15)][(lane >> 4) * 8 + i];
     put_pieces<P>(x, to + ((long)block * column_fragments + fragment) * P * KIB, lane);
 }
-// All operands that a call takes from its inputs, one launch: the rows and columns of x, the columns and rows of W, those that are wanted.
+// All operands that a call takes from its inputs, one launch for up to MOST_WORKGROUPS: the rows and columns of x, the columns and rows of W, those that are wanted.
 struct Operands {
     Source x, w;
     __bf16 *x_rows, *x_columns, *w_columns, *w_rows;
     int x_row_fragments, x_column_fragments, w_column_fragments, w_row_fragments;
     unsigned end[4];   // workgroups up to and with each
+    unsigned first;    // of this launch
 };
+constexpr unsigned MOST_WORKGROUPS = 1u << 23;   // of a launch, whose threads are counted in 32 bits
 template <class E, int P>
 __global__ __launch_bounds__(256) void operands_kernel(Operands o) {
     __shared__ float tile[64][33];
-    const unsigned b = blockIdx.x;
+    const unsigned b = o.first + blockIdx.x;
     if (b < o.end[0]) along_columns<E, P, true>(o.w, o.w_columns, o.w_column_fragments, b, tile);
     else if (b < o.end[1]) along_rows<E, P, false>(o.x, o.x_rows, o.x_row_fragments, (o.x_column_fragments + 1) / 2, b - o.end[0]);
     else if (b < o.end[2]) along_columns<E, P, false>(o.x, o.x_columns, o.x_column_fragments, b - o.end[1], tile);
@@ -727,7 +729,8 @@ void launch(const mrl_ctx *ctx, const Layer &y, const Plan &p, char *ws, bool ba
     o.end[1] = o.end[0] + (as_is ? 0 : row_blocks(p.M16, p.K16 / 2));
     o.end[2] = o.end[1] + (backward ? column_blocks(p.K16, p.M16 / 2) : 0);
     o.end[3] = o.end[2] + (backward && y.grad_x ? row_blocks(p.K16, p.N16) : 0);
-    hipLaunchKernelGGL((operands_kernel<E, P>), dim3(o.end[3]), dim3(256), 0, ctx->stream, o);
+    for (; o.first < o.end[3]; o.first += MOST_WORKGROUPS)
+        hipLaunchKernelGGL((operands_kernel<E, P>), dim3(std::min(MOST_WORKGROUPS, o.end[3] - o.first)), dim3(256), 0, ctx->stream, o);
     const bool pre_small = tiles<S>(p.M16, 2L * p.N16) < ctx->n_cus;
     if (!backward) {
         if (pre_small) Small::template pre<true>(ctx, y, p, x_rows, w_columns, as_is);

@@ -372,3 +372,22 @@ def test_infinities_are_what_the_formulas_make_of_them(mrl, ctx, M, act, dtype):
         for got, want, what in ((out, a.detach() * pre[:, N:], "out"), (gx, d @ w.T, "grad_x"), (grads, want_grads, "grads")):
             want = kinds(want.to(got.dtype).double())
             assert torch.equal(kinds(got.cpu().double()).reshape(want.shape), want), (where, what)
+
+
+def test_more_operands_than_a_launch_has_threads(mrl, ctx):
+    """2^34 values of x, which the gradient lays out twice, in more than 2^32 threads.  Only some rows are not zeros."""
+    M, K, N = (1 << 25) + 5, 513, 3
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GiB of device memory")
+    some = [0, 12345, (1 << 24) + 3, M - 1]
+    c = Case(len(some), K, N, "silu", "bf16", seed=17)
+    x, grad = torch.zeros(M, K, dtype=c.tt, device="cuda"), torch.zeros(M, N, dtype=c.tt, device="cuda")
+    x[some], grad[some] = c.x, c.grad
+    grads = torch.full((2 * N * (K + 1),), 7.0, device="cuda")
+    c.layer(mrl).backward_gpu(ctx, None, grads, grad, x, c.params)
+    ctx.synchronize()
+    _, (want, off) = c.backward64()
+    near(grads, want, off, "grads")
+    del x, grad
+    torch.cuda.empty_cache()
