@@ -563,7 +563,7 @@ int mrl_muon_step(mrl_ctx *ctx, float *params, const float *grads, float *state,
  * mrl_clip_grad_norm for gradients that are not one vector (those of several layers' parameters): norm = sqrt(sum of the squares of all values of
  * all tensors), out = in * max_norm / (norm + 1e-8) where the norm is above max_norm, out = in elsewhere (a NaN norm too; an infinite one
  * gives zeros, and NaN where a value is infinite).  Squares and sums are Float64.  A tensor is n values of `dtype` one behind the
- * other; out may be in, but have no byte of another tensor (MRL_E_ARG).  norm (device, may be NULL) receives the norm before clipping.  The
+ * other; out may be in, but have no byte of another tensor (MRL_E_ARG).  98304 tensors that are not empty at most.  norm (device, may be NULL) receives the norm before clipping.  The
  * workspace (device, 16-byte aligned, need not be kept between calls) holds MRL_CLIP_TENSORS_WORKSPACE bytes. */
 #define MRL_CLIP_TENSORS_WORKSPACE 16384
 typedef struct {

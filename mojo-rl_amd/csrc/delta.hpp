@@ -695,8 +695,9 @@ inline int column_tiles(int dv) { return (dv + TILE - 1) / TILE; }
 inline int blocks_of(int T, int tiles) { return (T + TILE * tiles - 1) / (TILE * tiles); }
 constexpr int floats_of(int DK) { return DK * TILE; }   // of a column tile
 
-// How many parts: as many as give every CU PART_GROUPS workgroups, but no more than sqrt(20 blocks): a part takes some 10 us for each of its
-// blocks, twice, and the way through the parts 1 us for each of them.  8192 steps of 2 environments of 8 heads of 128 x 128 in bf16 take 265 us with two a CU,
+// How many parts: as many as give every CU PART_GROUPS workgroups, but no more than sqrt(20 blocks).  A part takes 13 to 16 us for each of its
+// blocks of 128 x 128, twice, and the way through the parts 0.6 us for each of them, which is least at sqrt(50 blocks), but flat: 10 to 40 make no
+// difference that is not lost between two runs.  8192 steps of 2 environments of 8 heads of 128 x 128 in bf16 take 265 us with two a CU,
 // 274 to 322 with one, 312 with three; the gradient of 1001 steps of 7 environments of 3 heads of 40 x 24 130, 144 and 130.
 constexpr int PART_GROUPS = 2, MOST_PARTS = 1024;
 inline Parts parts_of(const mrl_ctx *ctx, const mrl_delta *r, int tiles) {

@@ -21,10 +21,10 @@
 // rows of the states per wavefront, which they pass through LDS.  A rollout in parts has the gradients of the states behind the parts worked out
 // ahead of that (chain_kernel, and the launch that goes through the parts).
 //
-// 128 steps of 512 environments of 4 heads of 64 x 64 in fp32 take 501 us, 82 of them the first launch (reading and writing the rows once takes 105, the
+// 128 steps of 512 environments of 4 heads of 64 x 64 in fp32 take 503 us, 82 of them the first launch (reading and writing the rows once takes 105, the
 // formulas' products at the rate of a large fp32 one 140).  Bound by what a tile's phases wait for each other: the matrix cores are busy a third of the time,
 // other instructions a quarter; LDS has room for two workgroups of four wavefronts a CU (78 KB; one takes 755 us).  Memory is no part of it: 489
-// with all rows in the L2.  The pairs' sums by two wavefronts instead of one: 501 for 506; the lengths' dots from terms that are there: 507 for 520.
+// with all rows in the L2.  The pairs' sums by two wavefronts instead of one: 5 us; the lengths' dots from terms that are there: 13.
 #include <type_traits>
 #include "delta.hpp"
 

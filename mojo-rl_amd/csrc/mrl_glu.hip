@@ -374,7 +374,7 @@ struct Layer {
 
 // Pieces of [dgate | dup].  For dW three, 22 bits and more, as fp32 has them: in bf16 two (16 bits) would be 2.5e-6 off in the 2-norm, where fp32 sums of
 // products that are not split come to 1.1e-7 for 8 rows, 8e-7 for 2048 and 2e-6 for 32768, three pieces to 1.1e-7, 2e-7 and 5e-7.  16384 rows of
-// 512 -> 1024 take 292 us, with two 254.
+// 512 -> 1024 take 295 us; two took 38 less.
 constexpr int COLUMN_PIECES = 3;
 
 // FORWARD: the layer's outputs.  Otherwise [dgate | dup] as fragments, contracted along the columns (PR pieces, for dx) and along the rows
@@ -634,8 +634,8 @@ struct Plan {
 template <class S>
 int tiles(long a, long b) { return (int)(((a + S::ROWS - 1) / S::ROWS) * ((b + S::COLUMNS - 1) / S::COLUMNS)); }
 
-// 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.  256 -> 683, the gradient: 512 rows in fp32 take 53 us with small
-// tiles and 89 with large ones, 32768 rows 688 and 607; in bf16 33 and 59, 298 and 252.
+// 128 x 256 and 128 x 128 where there are as many tiles as CUs, 64 x 64 elsewhere.  256 -> 683, the gradient: 512 rows in fp32 take 43 us with small
+// tiles and 60 with large ones, 32768 rows 683 and 602; in bf16 35 and 54, 407 and 348.
 // Two pieces for dx cost 16384 rows of 512 -> 1024 35 us (tiles of 128 x 128: 48).
 typedef Shape<1, 1, 2, 4, 4, 4, 3> Bf16Shape;
 typedef Shape<1, 1, 4, 2, 1, 2, 4> Bf16Small;
@@ -673,10 +673,10 @@ Plan plan_of(const mrl_ctx *ctx, int dtype, int M, int K, int N, bool backward) 
         p.sums = take(sizeof(float) * ((size_t)p.M16 + WR_MOST) * 2 * p.N16 * 16);   // (a wavefront has a fragment of rows at least)
         const int all = f32 ? tiles<F32Shape>(p.K16, 2L * p.N16) : tiles<Bf16W>(p.K16, 2L * p.N16);
         const int blocks = p.M16 / 2;
-        // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 62 us, 116 with whole columns; 32768 rows 607 and 1474
+        // dW's tiles are few, its contracted index is long: 2048 rows of 256 -> 683 in fp32 take 56 us, 111 with whole columns; 32768 rows 602 and 1485
         p.parts = (int)std::max<long>(1, std::min<long>((blocks + 7) / 8, (ctx->n_cus + all - 1) / all));
         if (p.parts > 1) p.partial = take(sizeof(float) * (size_t)p.parts * K * 2 * N);
-        // so are dx's where there are few rows: 2048 rows of 256 -> 683 in fp32 take 62 us, 69 whole; 512 rows 45 and 55, in bf16 34 and 36
+        // so are dx's where there are few rows: 2048 rows of 256 -> 683 in fp32 take 56 us, 63 whole; 512 rows 43 and 53, in bf16 35 and 39
         const int large = f32 ? tiles<F32Shape>(p.M16, p.K16) : tiles<Bf16X>(p.M16, p.K16), small = f32 ? tiles<F32Small>(p.M16, p.K16) : tiles<Bf16XSmall>(p.M16, p.K16);
         p.x_parts = large >= ctx->n_cus ? 1 : std::max(1, std::min(p.N16 / X_STAGES, ctx->n_cus / small));
         if (p.x_parts > 1) p.x_partial = take(sizeof(float) * (size_t)p.x_parts * M * K);
