@@ -121,7 +121,8 @@ __global__ __launch_bounds__(256) void steps_kernel(Delta d, int units, int colu
 
 // ---------------------------------------------------------------- rollouts
 // All columns of a head in a workgroup, up to 128, so that its keys are prepared once: 128 steps of 512 environments of 4 heads of 128 x 128 take 255 us in
-// bf16 and 384 in fp32, 285 and 392 with four wavefronts at most (of 64 x 80 163 and 155, the other way around), 8192 steps of 2 environments 265 and 280.
+// bf16 and 384 in fp32, 285 and 392 with four wavefronts at most (of 64 x 80 163 and 155, the other way around), 8192 steps of 2 environments 265 and 280
+// (on one card; others take 260 to 286).
 constexpr int MOST_WAVES = 8;
 enum { OUTPUTS, STATES, ENDS };   // of all steps; ahead of every block; M and B of every part
 
