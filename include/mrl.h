@@ -516,7 +516,7 @@ int mrl_delta_backward(mrl_ctx *ctx, const mrl_delta *r, const void *grad_out, i
  *
  * Backward overwrites grads (fp32, laid out like params, whatever the type) and grad_in (may be NULL) from the gradient of out; it works gate and
  * up out again.  Their gradients are not rounded to bf16 in between: 16 bits of them and more go into grad_in (2^-17 of a term, where storing a sum
- * in bf16 costs 2^-9 of it).  All sums are in a fixed order.  Rows are below 2^26, dims 1 to 65536.
+ * in bf16 costs 2^-8 of it).  All sums are in a fixed order.  Rows are below 2^26, dims 1 to 65536.
  *
  * No element of an output may be one of an input's or of another output's (MRL_E_ARG).  The workspace (device, 16-byte aligned, need not be kept
  * between calls; NULL where the size is 0) holds at least mrl_gated_linear_workspace's bytes. */

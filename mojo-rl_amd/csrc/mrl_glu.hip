@@ -7,7 +7,7 @@
 //
 // Products run on the bf16 matrix cores with fp32 sums.  bf16 values are operands as they are.  An fp32 value is three bf16 pieces
 // (mlp_split.hpp) and a product of two the six largest of nine, 2^-24 of it off.  In bf16 [dgate | dup], which is never rounded to
-// bf16, goes into dx as two (16 bits: 2^-17 of a term, where storing dx costs 2^-9 of it) and into dW, which is fp32, as three.
+// bf16, goes into dx as two (16 bits: 2^-17 of a term, where storing dx costs 2^-8 of it) and into dW, which is fp32, as three.
 //
 // Operands lie in the workspace as fragments: 16 rows and 32 of the contracted index, a KiB in the order in which the 64 lanes of
 // v_mfma_f32_16x16x32_bf16 hold them (lane 16 g + n: row n, elements 8 g .. 8 g + 7), the pieces of a fragment next to each other, all rows'
